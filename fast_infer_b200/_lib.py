@@ -24,6 +24,8 @@ FI_DEVERR_TIMEOUT = 1
 FI_DEVERR_BAD_BLOCK = 2
 FI_DEVERR_CONTEXT_LEN = 4
 FI_STATIC_WEIGHTS = 1
+FI_DTYPE_F16 = 0
+FI_DTYPE_BF16 = 1
 
 _STATUS_NAMES = {
     FI_ERR_INVALID_ARG: "FI_ERR_INVALID_ARG",
@@ -55,6 +57,10 @@ SIGNATURES = {
     "fi_paged_decode_noalloc": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
                                                _i64, _i64, _i64, _i64, _i64, _i64, _i64p, _i64p,
                                                _i64p, _i64p, _i64p, _f32, _i64, _vp, _vp]),
+    "fi_paged_chunk_workspace_size": (_sz, [_i64, _i64, _i64]),
+    "fi_paged_chunk": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
+                                      _i64, _i64, _i64, _i64, _i64, _i64, _i64p, _i64p, _i64p,
+                                      _i64p, _i64p, _f32, _f32, _i64, _i64, _vp, _sz, _vp, _vp]),
     "fi_rope_kv_write": (ctypes.c_int, [_vp, _i64, _i64, _i64, _i64, _i64, _i64p, _vp, _vp, _i64,
                                         _i64, _vp, _i64, _vp, _i64p, _vp, _i64p, _vp, _vp, _vp,
                                         _i64, _i64, _i64, _i64p, _i64p, _i64p, _vp, _vp]),

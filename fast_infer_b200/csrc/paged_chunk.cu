@@ -1,0 +1,767 @@
+// Attention of a chunk of new tokens over the paged KV cache (chunked prefill, verification
+// of drafted tokens, single tokens, and batches that mix them), on sm_100a tensor cores.
+//
+//   o_i = sum_j exp(s_ij - lse_i) v_j,  lse_i = log sum_j exp(s_ij)   (j over visible keys;
+//   the batch, visibility and score are described in chunk_common.cuh; a token that sees
+//   nothing gives o = 0, lse = -inf).
+//
+// Design:
+// * A unit is 2 x (128 / group) consecutive tokens of one sequence for one KV head: two
+//   128-row tiles (rows = token x head of the group) that share every K/V tile.
+// * The work of a launch is one line of (KV head, unit, key tile) steps, cut into equal
+//   contiguous parts, one per CTA. A long prefill, many single tokens over long contexts and
+//   any mixture balance alike, without knowing the lengths on the host: every CTA derives
+//   the line from cu / ctx in shared memory first. A unit cut between CTAs leaves fp32
+//   partial rows in the workspace, joined by chunk_combine_kernel in CTA order (the same bits
+//   on every run).
+// * Roles (384 threads), tensor memory (S0 | S1 | O0 | O1), the lazily rescaled online
+//   softmax and the MMA order are those of the causal prefill kernel (prefill_sm100.cu). K
+//   and V tiles are two pages each, gathered by TMA through the block table.
+// * Slots behind a sequence's last token may hold anything: their scores are replaced by
+//   -inf, and their V rows are zeroed in shared memory before the product (0 * NaN is NaN).
+#include "chunk_common.cuh"
+
+namespace fi {
+
+constexpr int kCkThreads = 384;
+constexpr int kCkRegsSoftmax = 184;  // 2 x 128 x 184 + 128 x 136 = 384 x 168
+constexpr int kCkRegsOther = 136;
+constexpr int kCkStages = 2;
+constexpr int kCkTeardownBar = 15;
+constexpr int kCkMaxBatch = 2048;    // sequences per launch
+constexpr int kCkMaxUnits = 6000;    // token units per launch (per KV head)
+constexpr float kCkRescale = 8.0f;   // log2 units of growth of the max before O is rescaled
+constexpr int kCkEmuPairs = 2;       // of 8 column pairs, exp2 on the FMA pipe
+
+struct CkBarriers {
+  uint64_t q_full[2], q_empty[2];
+  uint64_t k_full[kCkStages], k_empty[kCkStages];
+  uint64_t v_full[kCkStages], v_empty[kCkStages];
+  uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+  uint64_t mma_done;
+  uint32_t tmem_base;
+  uint32_t warp_sums[kCkThreads / 32];
+  uint32_t unit_off[kCkMaxBatch + 1];  // first unit of each sequence
+  uint32_t work[kCkMaxUnits + 1];      // key tiles before each unit
+};
+constexpr int kCkSmemBytes = 1024 + (2 + 2 * kCkStages) * kChunkTileBytes + (int)sizeof(CkBarriers);
+static_assert(kCkSmemBytes <= 227 * 1024, "shared memory");
+
+// The unit whose first part a CTA holds when the rest lies in the next CTAs.
+struct CkJoin {
+  int valid, last_cta, token, hk, rows[2], pad[2];
+};
+
+struct ChunkParams {
+  ChunkBatch b;
+  ScoreForm f;
+  void* o;
+  int64_t os[2];
+  float* lse;  // [total, hq] or null
+  float* ws_o;    // [cta][first, last unit][rows_cap][128]
+  float* ws_lse;  // [cta][first, last unit][rows_cap], log2 domain
+  CkJoin* join;   // [cta]
+  int rows_cap;
+  int* err;
+};
+
+// A CTA's part of a unit: key steps [j0, j1) of its n.
+struct CkUnit {
+  int b, hk;
+  int token, pos;      // first packed row, its position
+  int rows[2];         // live rows of the two tiles
+  int keys, prefix;
+  int np, lo;          // step j is key tile j < np ? j : lo + j - np
+  int j0, j1, n;
+};
+
+__device__ __forceinline__ int ck_tile(const CkUnit& u, int j) {
+  return j < u.np ? j : u.lo + (j - u.np);
+}
+
+// Key tiles that the unit of tokens [t0, t1) of a sequence visits: [0, np) for the prefix and
+// [lo, lo + n - np). A unit that sees nothing visits one (all of it masked).
+__device__ __forceinline__ void ck_tiles(const ChunkBatch& p, const ChunkSeq& s, int t0, int t1,
+                                         int& np, int& lo, int& n) {
+  const int p0 = s.pos0 + t0, p1 = s.pos0 + t1 - 1;
+  const int end = min(s.keys, max(p1 + 1, s.prefix));
+  const int hi = end > 0 ? (end - 1) / kChunkTile : 0;
+  lo = p.window ? min(max(p0 - p.window + 1, 0) / kChunkTile, hi) : 0;
+  np = min((s.prefix + kChunkTile - 1) / kChunkTile, lo);
+  n = np + hi - lo + 1;
+}
+
+// The CTA's next unit: step w of the line, at most up to `end`.
+__device__ __forceinline__ CkUnit ck_unit(const ChunkBatch& p, const CkBarriers* s, uint32_t units,
+                                          int64_t w, int64_t end) {
+  CkUnit u;
+  const uint32_t per_head = s->work[units];
+  u.hk = (int)(w / per_head);
+  const uint32_t r = (uint32_t)(w - (int64_t)u.hk * per_head);
+  const int e = last_le(s->work, (int)units, r);
+  u.b = last_le(s->unit_off, p.batch, (uint32_t)e);
+  const ChunkSeq q = chunk_seq(p, u.b);
+  const int tt = p.tile_tokens;
+  const int t0 = (e - (int)s->unit_off[u.b]) * 2 * tt, t1 = min(t0 + 2 * tt, q.n);
+  ck_tiles(p, q, t0, t1, u.np, u.lo, u.n);
+  u.token = q.start + t0;
+  u.pos = q.pos0 + t0;
+  u.keys = q.keys;
+  u.prefix = q.prefix;
+  u.rows[0] = min(t1 - t0, tt) * p.group;
+  u.rows[1] = max(t1 - t0 - tt, 0) * p.group;
+  u.j0 = (int)(r - s->work[e]);
+  u.j1 = (int)(u.n - u.j0 <= end - w ? u.n : u.j0 + (end - w));
+  return u;
+}
+
+// Scores of one row in log2 units, in place: the cap and the distance bias. `off` = position
+// of column 0's key minus the row's position.
+template <bool kCap, bool kAlibi>
+__device__ __forceinline__ void score_form(uint32_t* sr, const ScoreForm& f, float slope2,
+                                           float off, bool live) {
+  if constexpr (kCap) {
+    const uint64_t cin = f32x2(f.cap_in, f.cap_in), cout = f32x2(f.cap_log2, f.cap_log2);
+    float big = 0.f;
+#pragma unroll
+    for (int c = 0; c < kChunkTile; c += 2)
+      big = fmax3f(big, fabsf(__uint_as_float(sr[c])), fabsf(__uint_as_float(sr[c + 1])));
+    if (__all_sync(0xffffffffu, !live || big * f.cap_in <= 1.f)) {
+#pragma unroll
+      for (int c = 0; c < kChunkTile; c += 2) {
+        const uint64_t u = mul_f32x2(
+            f32x2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), cin);
+        float a, b;
+        f32x2_split(mul_f32x2(tanh_poly_x2(u), cout), a, b);
+        sr[c] = __float_as_uint(a);
+        sr[c + 1] = __float_as_uint(b);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < kChunkTile; c += 2) {
+        const uint64_t u = mul_f32x2(
+            f32x2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), cin);
+        float u0, u1, a, b;
+        f32x2_split(u, u0, u1);
+        f32x2_split(tanh_poly_x2(u), a, b);
+        a = fabsf(u0) <= 1.f ? a : tanh_any(u0);
+        b = fabsf(u1) <= 1.f ? b : tanh_any(u1);
+        sr[c] = __float_as_uint(a * f.cap_log2);
+        sr[c + 1] = __float_as_uint(b * f.cap_log2);
+      }
+    }
+  }
+  if constexpr (kAlibi) {
+#pragma unroll
+    for (int c = 0; c < kChunkTile; ++c) {
+      const float s = __uint_as_float(sr[c]);
+      const float d = fabsf(off + (float)c) * slope2;
+      sr[c] = __float_as_uint(kCap ? s - d : fmaf(s, f.scale_log2, -d));
+    }
+  }
+}
+
+// p = 2^(s * sl2 - mref) of a row, its sum, and p packed in place (see softmax_pass of the
+// prefill kernel: 2 of 8 pairs take exp2 on the FMA pipe).
+template <typename T>
+__device__ __forceinline__ float ck_exp(uint32_t* sr, float sl2, float mref) {
+  const uint64_t sc2 = f32x2(sl2, sl2), nm2 = f32x2(-mref, -mref);
+  uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+  for (int c = 0; c < kChunkTile; c += 2) {
+    const uint64_t xp =
+        fma_f32x2(f32x2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), sc2, nm2);
+    float p0, p1;
+    if (((c >> 1) & 7) < kCkEmuPairs) {
+      exp2_poly_x2(xp, p0, p1);
+    } else {
+      float x0, x1;
+      f32x2_split(xp, x0, x1);
+      p0 = fast_exp2(x0);
+      p1 = fast_exp2(x1);
+    }
+    sum2[(c >> 1) & 3] = add_f32x2(sum2[(c >> 1) & 3], f32x2(p0, p1));
+    sr[c >> 1] = Half16<T>::pack(p0, p1);
+  }
+  float lo, hi;
+  f32x2_split(add_f32x2(add_f32x2(sum2[0], sum2[1]), add_f32x2(sum2[2], sum2[3])), lo, hi);
+  return lo + hi;
+}
+
+// Zero rows [from, 128) of a V tile (both 64-value columns) with one warpgroup.
+__device__ __forceinline__ void zero_v_rows(uint8_t* v, int from, int tid) {
+  const int chunks = (kChunkTile - from) * 8;
+  for (int i = tid; i < 2 * chunks; i += 128) {
+    const int half = i >= chunks, k = half ? i - chunks : i;
+    *reinterpret_cast<uint4*>(v + half * kChunkHalf + from * 128 + k * 16) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+template <typename T, bool kCap, bool kAlibi>
+__global__ void __launch_bounds__(kCkThreads, 1)
+    paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q,
+                       const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v, const ChunkParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_align1024(smem_raw);
+  uint8_t* sQ = smem;
+  uint8_t* sK = smem + 2 * kChunkTileBytes;
+  uint8_t* sV = sK + kCkStages * kChunkTileBytes;
+  CkBarriers* bars = reinterpret_cast<CkBarriers*>(sV + kCkStages * kChunkTileBytes);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = gridDim.x, cta = blockIdx.x;
+
+  if (warp == 0) {
+    tmem_alloc(&bars->tmem_base, 512);
+    tmem_relinquish();
+  }
+  if (threadIdx.x == 32) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&bars->q_full[t], 1);
+      mbar_init(&bars->q_empty[t], 1);
+      mbar_init(&bars->s_full[t], 1);
+      mbar_init(&bars->p_full[t], 4);
+      mbar_init(&bars->o_full[t], 1);
+      mbar_init(&bars->o_empty[t], 4);
+    }
+    for (int s = 0; s < kCkStages; ++s) {
+      mbar_init(&bars->k_full[s], 1);
+      mbar_init(&bars->k_empty[s], 1);
+      mbar_init(&bars->v_full[s], 1);
+      mbar_init(&bars->v_empty[s], 1);
+    }
+    mbar_init(&bars->mma_done, 1);
+    fence_barrier_init();
+  }
+
+  // The line of work: units of each sequence, then key tiles of each unit, both as sums.
+  grid_dep_wait();
+  grid_dep_launch();
+  const ChunkBatch& pb = p.b;
+  if (threadIdx.x == 0) bars->unit_off[0] = bars->work[0] = 0;
+  for (int b = threadIdx.x; b < pb.batch; b += kCkThreads) {
+    const ChunkSeq q = chunk_seq(pb, b);
+    bars->unit_off[b + 1] = (uint32_t)((q.n + 2 * pb.tile_tokens - 1) / (2 * pb.tile_tokens));
+    if (q.bad && cta == 0) set_error(p.err, FI_DEVERR_CONTEXT_LEN);
+  }
+  __syncthreads();
+  block_scan(bars->unit_off, pb.batch, bars->warp_sums);
+  // cu that is not ascending could name more units than the host counted: those are dropped
+  const uint32_t units = min(bars->unit_off[pb.batch], (uint32_t)kCkMaxUnits);
+  if (units != bars->unit_off[pb.batch] && threadIdx.x == 0)
+    set_error(p.err, FI_DEVERR_CONTEXT_LEN);
+  for (int e = threadIdx.x; e < (int)units; e += kCkThreads) {
+    const int b = last_le(bars->unit_off, pb.batch, (uint32_t)e);
+    const ChunkSeq q = chunk_seq(pb, b);
+    const int t0 = (e - (int)bars->unit_off[b]) * 2 * pb.tile_tokens;
+    int np, lo, n;
+    ck_tiles(pb, q, t0, min(t0 + 2 * pb.tile_tokens, q.n), np, lo, n);
+    bars->work[e + 1] = (uint32_t)n;
+  }
+  __syncthreads();
+  block_scan(bars->work, (int)units, bars->warp_sums);
+  const int64_t total = (int64_t)bars->work[units] * pb.hk;
+  const int active = (int)(total < G ? total : G);  // CTAs with work
+  const int64_t w_begin = cta < active ? total * cta / active : 0;
+  const int64_t w_end = cta < active ? total * (cta + 1) / active : 0;
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+
+  if (warp >= 8) {
+    setmaxnreg_dec<kCkRegsOther>();
+    if (warp == 8 && lane == 0) {
+      // ---------------------------------------------------------- TMA producer
+      prefetch_tmap(&tm_q);
+      prefetch_tmap(&tm_k);
+      prefetch_tmap(&tm_v);
+      const uint32_t q_bytes = (uint32_t)(pb.group * pb.tile_tokens * 256);
+      int qc[2] = {0, 0};
+      int g = 0;
+      bool ok = true;
+      for (int64_t w = w_begin; ok && w < w_end;) {
+        const CkUnit u = ck_unit(pb, bars, units, w, w_end);
+        w += u.j1 - u.j0;
+        auto load_q = [&]() {
+          for (int t = 0; t < 2 && ok; ++t) {
+            if (u.rows[t] == 0) continue;
+            if (qc[t] > 0) ok = mbar_wait(&bars->q_empty[t], (qc[t] - 1) & 1, p.err);
+            if (!ok) break;
+            const int token = u.token + t * pb.tile_tokens;
+            uint8_t* dst = sQ + t * kChunkTileBytes;
+            mbar_arrive_expect_tx(&bars->q_full[t], q_bytes);
+            tma_load_4d(dst, &tm_q, &bars->q_full[t], 0, 0, u.hk, token);
+            tma_load_4d(dst + kChunkHalf, &tm_q, &bars->q_full[t], 64, 0, u.hk, token);
+            ++qc[t];
+          }
+        };
+        int ph[2];
+        for (int i = 0; i < 2; ++i) ph[i] = chunk_page(pb, u.b, u.keys, ck_tile(u, u.j0), i);
+        for (int j = u.j0; ok && j < u.j1; ++j, ++g) {
+          const int s = g % kCkStages;
+          const uint32_t par = ((g / kCkStages) - 1) & 1;
+          int next[2] = {0, 0};  // the next tile's pages, read while this one waits
+          if (j + 1 < u.j1)
+            for (int i = 0; i < 2; ++i) next[i] = chunk_page(pb, u.b, u.keys, ck_tile(u, j + 1), i);
+          for (int i = 0; i < 2; ++i)
+            if (ph[i] == pb.num_blocks && ck_tile(u, j) * kChunkTile + i * kChunkPage < u.keys)
+              set_error(p.err, FI_DEVERR_BAD_BLOCK);
+          if (g >= kCkStages && !(ok = mbar_wait(&bars->k_empty[s], par, p.err))) break;
+          uint8_t* dk = sK + s * kChunkTileBytes;
+          mbar_arrive_expect_tx(&bars->k_full[s], kChunkTileBytes);
+          for (int i = 0; i < 2; ++i) {
+            tma_load_4d(dk + i * kChunkHalf / 2, &tm_k, &bars->k_full[s], 0, u.hk, 0, ph[i]);
+            tma_load_4d(dk + kChunkHalf + i * kChunkHalf / 2, &tm_k, &bars->k_full[s], 64, u.hk, 0,
+                        ph[i]);
+          }
+          if (j == u.j0) load_q();
+          if (!ok) break;
+          if (g >= kCkStages && !(ok = mbar_wait(&bars->v_empty[s], par, p.err))) break;
+          uint8_t* dv = sV + s * kChunkTileBytes;
+          mbar_arrive_expect_tx(&bars->v_full[s], kChunkTileBytes);
+          for (int i = 0; i < 2; ++i) {
+            tma_load_4d(dv + i * kChunkHalf / 2, &tm_v, &bars->v_full[s], 0, u.hk, 0, ph[i]);
+            tma_load_4d(dv + kChunkHalf + i * kChunkHalf / 2, &tm_v, &bars->v_full[s], 64, u.hk, 0,
+                        ph[i]);
+          }
+          ph[0] = next[0];
+          ph[1] = next[1];
+        }
+      }
+    } else if (warp == 9 && lane == 0) {
+      // ---------------------------------------------------------- UMMA issuer
+      constexpr uint32_t idesc_qk = umma_idesc<T>(128, 128, 0, 0);
+      constexpr uint32_t idesc_pv = umma_idesc<T>(128, 128, 0, 1);
+      const uint32_t q_addr = smem_u32(sQ), k_addr = smem_u32(sK), v_addr = smem_u32(sV);
+      int qc[2] = {0, 0};  // units seen per tile
+      int sc[2] = {0, 0};  // S tiles issued per tile
+      int g = 0;
+      bool ok = true;
+      auto issue_s = [&](int t, int kstage) {
+        const uint64_t da = umma_desc_sw128(q_addr + t * kChunkTileBytes, 16, 1024);
+        const uint64_t db = umma_desc_sw128(k_addr + kstage * kChunkTileBytes, 16, 1024);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          const uint32_t off = ((kk >> 2) * kChunkHalf + (kk & 3) * 32) >> 4;
+          umma_ss(tmem + t * 128, da + off, db + off, idesc_qk, kk > 0);
+        }
+        umma_commit(&bars->s_full[t]);
+      };
+      auto issue_pv = [&](int t, int vstage, bool first) {
+        const uint64_t db = umma_desc_sw128(v_addr + vstage * kChunkTileBytes, kChunkHalf, 1024);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          umma_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, db + (uint32_t)(kk * 128),
+                  idesc_pv, (!first || kk > 0) ? 1u : 0u);
+      };
+      for (int64_t w = w_begin; ok && w < w_end;) {
+        const CkUnit u = ck_unit(pb, bars, units, w, w_end);
+        w += u.j1 - u.j0;
+        const int n = u.j1 - u.j0;
+        ok = mbar_wait(&bars->k_full[g % kCkStages], (g / kCkStages) & 1, p.err);
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (u.rows[t] == 0) continue;
+          ok = mbar_wait(&bars->q_full[t], qc[t] & 1, p.err);
+          if (!ok) break;
+          tc_fence_after();
+          issue_s(t, g % kCkStages);
+          ++sc[t];
+          if (n == 1) umma_commit(&bars->q_empty[t]);
+        }
+        if (ok) umma_commit(&bars->k_empty[g % kCkStages]);
+        for (int j = 0; ok && j < n; ++j, ++g) {
+          const bool has_next = j + 1 < n;
+          if (has_next) {
+            ok = mbar_wait(&bars->k_full[(g + 1) % kCkStages], ((g + 1) / kCkStages) & 1, p.err);
+            if (!ok) break;
+          }
+          ok = mbar_wait(&bars->v_full[g % kCkStages], (g / kCkStages) & 1, p.err);
+          if (!ok) break;
+          for (int t = 0; t < 2 && ok; ++t) {
+            if (u.rows[t] == 0) continue;
+            ok = mbar_wait(&bars->p_full[t], (sc[t] - 1) & 1, p.err);
+            // the first product of a unit overwrites O: the last unit's epilogue has read it
+            if (ok && j == 0 && qc[t] > 0)
+              ok = mbar_wait(&bars->o_empty[t], (qc[t] - 1) & 1, p.err);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(t, g % kCkStages, j == 0);
+            if (!has_next) {
+              umma_commit(&bars->o_full[t]);
+            } else {
+              issue_s(t, (g + 1) % kCkStages);
+              ++sc[t];
+              if (j + 2 == n) umma_commit(&bars->q_empty[t]);
+            }
+          }
+          if (!ok) break;
+          umma_commit(&bars->v_empty[g % kCkStages]);
+          if (has_next) umma_commit(&bars->k_empty[(g + 1) % kCkStages]);
+        }
+        for (int t = 0; t < 2; ++t)
+          if (u.rows[t] > 0) ++qc[t];
+      }
+      umma_commit(&bars->mma_done);
+      mbar_wait(&bars->mma_done, 0, p.err);
+    }
+    __syncwarp();
+    named_bar_arrive(kCkTeardownBar, kCkThreads);
+    return;
+  }
+
+  // ------------------------------------------- softmax + epilogue, warps 0-7
+  setmaxnreg_inc<kCkRegsSoftmax>();
+  {
+    const int t = warp >> 2;
+    const int quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const uint32_t tS = tmem + lane_off + t * 128;
+    const uint32_t tO = tmem + lane_off + 256 + t * 128;
+    const float sl2 = kCap || kAlibi ? 1.f : p.f.scale_log2;
+    int sc = 0;  // S tiles consumed of this tile
+    int g = 0;   // K/V tiles streamed (all units)
+    int uc = 0;  // units finished
+    bool ok = true;
+    CkJoin join = {};
+    for (int64_t w = w_begin; ok && w < w_end;) {
+      const CkUnit u = ck_unit(pb, bars, units, w, w_end);
+      w += u.j1 - u.j0;
+      const int rows = u.rows[t];
+      if (rows == 0) {
+        g += u.j1 - u.j0;
+        continue;
+      }
+      const bool live = row < rows;             // this row is stored
+      const bool warp_live = quarter * 32 < rows;
+      const int tok = row / pb.group, head = u.hk * pb.group + row % pb.group;
+      const int pos = u.pos + t * pb.tile_tokens + tok;
+      float slope2 = 0.f;
+      if (kAlibi && live) slope2 = p.f.slopes[head] * kLog2e;
+      float m = -INFINITY, l = 0.f;
+      for (int j = u.j0; ok && j < u.j1; ++j, ++sc, ++g) {
+        const int tile = ck_tile(u, j);
+        const int k0 = tile * kChunkTile;
+        bool page_ok[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) page_ok[i] = chunk_page(pb, u.b, u.keys, tile, i) != pb.num_blocks;
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[t], sc & 1, p.err));
+        if (!ok) break;
+        if (t == 0 && k0 + kChunkTile > u.keys) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_full[g % kCkStages],
+                                                 (g / kCkStages) & 1, p.err));
+          if (!ok) break;
+          zero_v_rows(sV + (g % kCkStages) * kChunkTileBytes, max(u.keys - k0, 0), threadIdx.x);
+          fence_proxy_async_smem();
+        }
+        if (warp_live) {
+          tc_fence_after();
+          uint32_t sr[kChunkTile];
+          tmem_ld32(tS + 0, sr + 0);
+          tmem_ld32(tS + 32, sr + 32);
+          tmem_ld32(tS + 64, sr + 64);
+          tmem_ld32(tS + 96, sr + 96);
+          tmem_wait_ld();
+          reg_fence<kChunkTile>(sr);
+          score_form<kCap, kAlibi>(sr, p.f, slope2, (float)(k0 - pos), live);
+          // columns [c_lo, c_hi) and [0, c_pre) are visible
+          const int c_hi = min(pos + 1, u.keys) - k0, c_pre = u.prefix - k0;
+          const int c_lo = pb.window ? pos - pb.window + 1 - k0 : 0;
+          const bool all = !live || ((c_hi >= kChunkTile && c_lo <= 0) || c_pre >= kChunkTile);
+          if (!__all_sync(0xffffffffu, all && page_ok[0] && page_ok[1])) {
+            uint32_t vis[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              vis[i] = (low_bits(c_hi, i) & ~low_bits(c_lo, i)) | low_bits(c_pre, i);
+              if (!page_ok[i >> 1]) vis[i] = 0;
+            }
+#pragma unroll
+            for (int c = 0; c < kChunkTile; ++c)
+              if (!((vis[c >> 5] >> (c & 31)) & 1u)) sr[c] = __float_as_uint(-INFINITY);
+          }
+          float mx8[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float a = __uint_as_float(sr[i]);
+#pragma unroll
+            for (int kk = 1; kk < 15; kk += 2)
+              a = fmax3f(a, __uint_as_float(sr[i + 8 * kk]),
+                         __uint_as_float(sr[i + 8 * (kk + 1)]));
+            mx8[i] = fmaxf(a, __uint_as_float(sr[i + 120]));
+          }
+          const float mx = fmaxf(fmax3f(mx8[0], mx8[1], mx8[2]),
+                                 fmax3f(fmax3f(mx8[3], mx8[4], mx8[5]), mx8[6], mx8[7]));
+          const float m_new = fmaxf(m, mx * sl2);
+          bool rescale = false;
+          float alpha = 1.f;
+          if (j == u.j0) {
+            m = m_new;
+          } else {
+            const bool need = m_new > m + kCkRescale;
+            rescale = __any_sync(0xffffffffu, need);
+            if (need) {
+              alpha = fast_exp2(m - m_new);
+              m = m_new;
+              l *= alpha;
+            }
+          }
+          l += ck_exp<T>(sr, sl2, m == -INFINITY ? 0.f : m);
+          tmem_st32(tS + 0, sr);
+          tmem_st32(tS + 32, sr + 32);
+          if (rescale) {
+            // the previous step's product is complete: S of this step was committed after it
+#pragma unroll
+            for (int cc = 0; cc < 128; cc += 32) {
+              uint32_t ov[32];
+              tmem_ld32(tO + cc, ov);
+              tmem_wait_ld();
+              reg_fence<32>(ov);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+              tmem_st32(tO + cc, ov);
+            }
+          }
+          tmem_wait_st();
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->p_full[t]);
+      }
+      // ----------------------------------------------------------- epilogue
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_full[t], uc & 1, p.err));
+      if (!ok) break;
+      tc_fence_after();
+      const bool begins = u.j0 == 0, ends = u.j1 == u.n;
+      if (begins && !ends) {
+        join.valid = 1;
+        join.last_cta = (int)(((w - u.j1 + u.n) * active - 1) / total);
+        join.token = u.token;
+        join.hk = u.hk;
+        join.rows[0] = u.rows[0];
+        join.rows[1] = u.rows[1];
+      }
+      const bool none = m == -INFINITY;
+      const float inv = none ? 0.f : 1.f / l;
+      const float lse2 = none ? -INFINITY : m + log2f(l);
+      const int64_t out_row = u.token + t * pb.tile_tokens + tok;
+      const int64_t part = (int64_t)(cta * 2 + (begins ? 1 : 0)) * p.rows_cap + t * 128 + row;
+      T* orow = static_cast<T*>(p.o) + out_row * p.os[0] + head * p.os[1];
+      float* prow = p.ws_o + part * 128;
+      if (warp_live) {
+#pragma unroll 1
+        for (int cc = 0; cc < 128; cc += 32) {
+          uint32_t ov[32];
+          tmem_ld32(tO + cc, ov);
+          tmem_wait_ld();
+          reg_fence<32>(ov);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            ov[e] = none ? 0u : __float_as_uint(__uint_as_float(ov[e]) * inv);
+          if (live && begins && ends) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint4 v;
+              v.x = Half16<T>::pack(__uint_as_float(ov[e]), __uint_as_float(ov[e + 1]));
+              v.y = Half16<T>::pack(__uint_as_float(ov[e + 2]), __uint_as_float(ov[e + 3]));
+              v.z = Half16<T>::pack(__uint_as_float(ov[e + 4]), __uint_as_float(ov[e + 5]));
+              v.w = Half16<T>::pack(__uint_as_float(ov[e + 6]), __uint_as_float(ov[e + 7]));
+              *reinterpret_cast<uint4*>(orow + cc + e) = v;
+            }
+          } else if (live) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<uint4*>(prow + cc + e) =
+                  make_uint4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
+          }
+        }
+        if (live) {
+          if (begins && ends) {
+            if (p.lse) p.lse[out_row * pb.hq + head] = lse2 * kLn2;
+          } else {
+            p.ws_lse[part] = lse2;
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->o_empty[t]);
+      ++uc;
+    }
+    if (threadIdx.x == 0) p.join[cta] = join;
+  }
+
+  tc_fence_before();
+  named_bar_sync(kCkTeardownBar, kCkThreads);
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the parts of a unit that several CTAs hold: weights 2^(lse_part - max). A warp per row.
+constexpr int kJoinSlices = 8;
+template <typename T>
+__global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const int cta = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const CkJoin jn = p.join[cta];
+  if (!jn.valid) return;
+  for (int r = blockIdx.y * 8 + warp; r < 256; r += kJoinSlices * 8) {
+    const int t = r >> 7, row = r & 127;
+    if (row >= jn.rows[t]) continue;
+    auto at = [&](int c) { return (int64_t)(c * 2 + (c == cta ? 1 : 0)) * p.rows_cap + r; };
+    float mx = -INFINITY;
+    for (int c = cta + lane; c <= jn.last_cta; c += 32) mx = fmaxf(mx, p.ws_lse[at(c)]);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+    const bool none = mx == -INFINITY;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+    if (!none) {
+      for (int c = cta; c <= jn.last_cta; ++c) {
+        const float wgt = exp2f(p.ws_lse[at(c)] - mx);
+        const float4 v = *reinterpret_cast<const float4*>(p.ws_o + at(c) * 128 + lane * 4);
+        sum += wgt;
+        acc.x = fmaf(wgt, v.x, acc.x);
+        acc.y = fmaf(wgt, v.y, acc.y);
+        acc.z = fmaf(wgt, v.z, acc.z);
+        acc.w = fmaf(wgt, v.w, acc.w);
+      }
+    }
+    const float inv = none ? 0.f : 1.f / sum;
+    const int token = jn.token + t * p.b.tile_tokens + row / p.b.group;
+    const int head = jn.hk * p.b.group + row % p.b.group;
+    uint2 pk;
+    pk.x = Half16<T>::pack(acc.x * inv, acc.y * inv);
+    pk.y = Half16<T>::pack(acc.z * inv, acc.w * inv);
+    T* orow = static_cast<T*>(p.o) + (int64_t)token * p.os[0] + head * p.os[1];
+    *reinterpret_cast<uint2*>(orow + lane * 4) = pk;
+    if (lane == 0 && p.lse)
+      p.lse[(int64_t)token * p.b.hq + head] = none ? -INFINITY : (mx + log2f(sum)) * kLn2;
+  }
+}
+
+template <typename T, bool kCap, bool kAlibi>
+static int launch_chunk(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                        const ChunkParams& p, cudaStream_t st) {
+  static DeviceOnce once;
+  cudaError_t e = once.run([] {
+    // the register split must fit what the block is launched with, or setmaxnreg would wait
+    cudaFuncAttributes a;
+    const cudaError_t e = cudaFuncGetAttributes(&a, paged_chunk_kernel<T, kCap, kAlibi>);
+    if (e != cudaSuccess) return e;
+    if (a.numRegs * kCkThreads < 2 * 128 * kCkRegsSoftmax + 128 * kCkRegsOther)
+      return cudaErrorInvalidConfiguration;
+    return cudaFuncSetAttribute(paged_chunk_kernel<T, kCap, kAlibi>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize, kCkSmemBytes);
+  });
+  if (e != cudaSuccess) return cuda_fail(e, "fi_paged_chunk: kernel set-up");
+  const int grid = sm_count();
+  e = launch_pdl(paged_chunk_kernel<T, kCap, kAlibi>, dim3((unsigned)grid), dim3(kCkThreads),
+                 kCkSmemBytes, st, tq, tk, tv, p);
+  if (e != cudaSuccess) return cuda_fail(e, "fi_paged_chunk: launch");
+  e = launch_pdl(chunk_combine_kernel<T>, dim3((unsigned)grid, kJoinSlices), dim3(256), 0, st, p);
+  if (e != cudaSuccess) return cuda_fail(e, "fi_paged_chunk: combine launch");
+  return FI_OK;
+}
+
+template <typename T>
+static int launch_chunk_form(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                             const ChunkParams& p, bool cap, cudaStream_t st) {
+  if (cap)
+    return p.f.slopes ? launch_chunk<T, true, true>(tq, tk, tv, p, st)
+                      : launch_chunk<T, true, false>(tq, tk, tv, p, st);
+  return p.f.slopes ? launch_chunk<T, false, true>(tq, tk, tv, p, st)
+                    : launch_chunk<T, false, false>(tq, tk, tv, p, st);
+}
+
+// Rows of a unit that can be live: all of them in one tile when the batch is that small.
+static int64_t ck_rows_cap(int64_t total, int64_t group) {
+  const int64_t tile = kChunkTile / group * group;
+  return total * group <= tile ? total * group : 2 * kChunkTile;
+}
+
+static size_t ck_align(size_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace fi
+
+extern "C" size_t fi_paged_chunk_workspace_size(int64_t total_tokens, int64_t num_q_heads,
+                                                int64_t num_kv_heads) {
+  using namespace fi;
+  if (total_tokens <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads ||
+      num_q_heads % num_kv_heads != 0 || num_q_heads / num_kv_heads > 64 ||
+      total_tokens > (1 << 28))
+    return 0;
+  const size_t slots = (size_t)sm_count() * 2 * ck_rows_cap(total_tokens, num_q_heads / num_kv_heads);
+  return ck_align(slots * 128 * 4) + ck_align(slots * 4) + ck_align(sm_count() * sizeof(CkJoin));
+}
+
+extern "C" int fi_paged_chunk(const void* q, const void* k_cache, const void* v_cache, void* o,
+                              float* lse, const int32_t* block_table, const int32_t* cu_seqlens,
+                              const int32_t* context_lens, const int32_t* prefix_lens,
+                              const float* alibi_slopes, int64_t batch, int64_t total_tokens,
+                              int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                              int64_t num_blocks, int64_t block_size, int64_t max_blocks_per_seq,
+                              const int64_t* q_strides, const int64_t* kc_strides,
+                              const int64_t* vc_strides, const int64_t* o_strides,
+                              const int64_t* bt_strides, float sm_scale, float softcap,
+                              int64_t window, int64_t dtype, void* workspace,
+                              size_t workspace_bytes, int32_t* error_flag, void* stream) {
+  using namespace fi;
+  clear_error();
+  const char* what = "fi_paged_chunk";
+  ChunkParams p = {};
+  int r = chunk_batch_args(p.b, what, cu_seqlens, context_lens, prefix_lens, block_table, batch,
+                           total_tokens, num_q_heads, num_kv_heads, head_dim, num_blocks,
+                           block_size, max_blocks_per_seq, bt_strides, window, dtype);
+  if (r != FI_OK) return r;
+  r = chunk_score_args(p.f, what, sm_scale, softcap, alibi_slopes);
+  if (r != FI_OK) return r;
+  if (batch == 0 || total_tokens == 0) return FI_OK;
+  if (!q || !k_cache || !v_cache || !o || !block_table || !cu_seqlens || !context_lens ||
+      !q_strides || !kc_strides || !vc_strides || !o_strides || !bt_strides)
+    return fail(FI_ERR_INVALID_ARG, "fi_paged_chunk: null pointer argument");
+  const int64_t unit_tokens = 2 * p.b.tile_tokens;
+  if (batch > kCkMaxBatch ||
+      (total_tokens + unit_tokens - 1) / unit_tokens + batch > kCkMaxUnits)
+    return fail(FI_ERR_UNSUPPORTED,
+                "fi_paged_chunk: at most %d sequences and %lld tokens with %d query heads per KV "
+                "head; split the batch",
+                kCkMaxBatch, (long long)((kCkMaxUnits - batch) * unit_tokens), p.b.group);
+  if (o_strides[2] != 1 || !aligned16(o) || o_strides[0] % 8 != 0 || o_strides[1] % 8 != 0)
+    return fail(FI_ERR_ALIGNMENT,
+                "fi_paged_chunk o: needs a 16-byte aligned base, unit innermost stride and other "
+                "strides multiple of 8");
+  const size_t need = fi_paged_chunk_workspace_size(total_tokens, num_q_heads, num_kv_heads);
+  if (!workspace || workspace_bytes < need)
+    return fail(FI_ERR_WORKSPACE, "fi_paged_chunk: workspace of %zu bytes, needs %zu",
+                workspace ? workspace_bytes : (size_t)0, need);
+  if (!aligned16(workspace))
+    return fail(FI_ERR_ALIGNMENT, "fi_paged_chunk: workspace not 16-byte aligned");
+  const CUtensorMapDataType type = dtype == FI_DTYPE_F16 ? Half16<__half>::kTmap
+                                                         : Half16<__nv_bfloat16>::kTmap;
+  CUtensorMap tq, tk, tv;
+  if ((r = chunk_q_map(&tq, type, q, p.b, q_strides, "fi_paged_chunk q")) != FI_OK) return r;
+  if ((r = chunk_kv_map(&tk, type, k_cache, p.b, kc_strides, "fi_paged_chunk k_cache")) != FI_OK)
+    return r;
+  if ((r = chunk_kv_map(&tv, type, v_cache, p.b, vc_strides, "fi_paged_chunk v_cache")) != FI_OK)
+    return r;
+  p.o = o;
+  p.os[0] = o_strides[0];
+  p.os[1] = o_strides[1];
+  p.lse = lse;
+  p.rows_cap = (int)ck_rows_cap(total_tokens, p.b.group);
+  const size_t slots = (size_t)sm_count() * 2 * p.rows_cap;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.ws_o = reinterpret_cast<float*>(ws);
+  p.ws_lse = reinterpret_cast<float*>(ws + ck_align(slots * 128 * 4));
+  p.join = reinterpret_cast<CkJoin*>(ws + ck_align(slots * 128 * 4) + ck_align(slots * 4));
+  p.err = error_flag;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == FI_DTYPE_F16 ? launch_chunk_form<__half>(tq, tk, tv, p, softcap > 0.f, st)
+                               : launch_chunk_form<__nv_bfloat16>(tq, tk, tv, p, softcap > 0.f, st);
+}

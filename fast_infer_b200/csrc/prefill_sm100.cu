@@ -34,8 +34,8 @@
 
 #include <math.h>
 
-#include "common.cuh"
 #include "host_common.h"
+#include "umma.cuh"
 
 namespace fi {
 
@@ -72,18 +72,6 @@ __device__ __forceinline__ bool crit_wait(uint64_t* bar, uint32_t parity, int* e
 #else
   return mbar_wait(bar, parity, err);
 #endif
-}
-
-// Shared-memory matrix descriptor, 128-byte swizzle (sm_100 "version 1" format):
-// start address, leading / stride byte offsets (16-byte units), layout type 2.
-__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-  uint64_t d = 0;
-  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
-  d |= (uint64_t)((lbo >> 4) & 0x3FFFu) << 16;
-  d |= (uint64_t)((sbo >> 4) & 0x3FFFu) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
 }
 
 // Instruction descriptor: f16 x f16 -> f32 accumulate, M = 128, N = 128,

@@ -11,6 +11,10 @@ Backward-compatible extensions:
   ``q.shape[1]``), so callers can drop the ``repeat_interleave`` of model.py:110-111.
 * ``paged_attention`` takes optional per-sequence ``context_lens`` (ragged
   batches) and ``pages_per_split`` (split-KV tuning).
+
+Functions without a reference counterpart, for serving long contexts in chunks (fp16 and
+bf16): ``paged_chunk_attention`` (new tokens over the paged cache, with capped scores, a
+distance bias, a window or a prefix).
 """
 
 from __future__ import annotations
@@ -227,3 +231,132 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         _lib.check(st, "paged_attention")
         device_errors(err, "paged_attention")
     return o
+
+
+_DTYPES = {torch.float16: _lib.FI_DTYPE_F16, torch.bfloat16: _lib.FI_DTYPE_BF16}
+
+
+def _int32_on(name: str, t: torch.Tensor, device: torch.device, count: int) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dim() != 1 or t.device != device or t.numel() != count:
+        raise ValueError(f"{name} must be a 1-D int32 tensor of {count} values on {device}")
+    return t.to(torch.int32).contiguous()
+
+
+def _chunk_args(q, caches, block_table, block_size, cu_seqlens, context_lens, sm_scale,
+                alibi_slopes, prefix_lens):
+    """Checks shared by the functions over packed new tokens and a paged cache; returns the
+    tensors as the library takes them."""
+    for name, t in (("q", q), *caches):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor (fast_infer_b200 has no CPU path)")
+        if t.dtype not in _DTYPES or t.dtype != q.dtype:
+            raise TypeError(f"{name} must be float16 or bfloat16 like q, got {t.dtype}")
+        if t.device != q.device:
+            raise ValueError("all tensors must be on the same device")
+    if q.dim() != 3 or q.shape[-1] != HEAD_DIM:
+        raise ValueError(f"q must be [total_tokens, num_q_heads, {HEAD_DIM}]")
+    num_blocks, bs, num_kv_heads, d = caches[0][1].shape if caches[0][1].dim() == 4 else (0,) * 4
+    if d != HEAD_DIM or any(t.shape != caches[0][1].shape for _, t in caches):
+        raise ValueError(f"caches must be [num_blocks, {BLOCK_SIZE}, num_kv_heads, {HEAD_DIM}]")
+    if block_size != bs or bs != BLOCK_SIZE:
+        raise ValueError(f"block_size must be {BLOCK_SIZE} and match the cache")
+    if num_blocks == 0 or num_kv_heads == 0 or q.shape[1] == 0 or q.shape[1] % num_kv_heads != 0:
+        raise ValueError(f"num_q_heads {q.shape[1]} not a multiple of k/v heads {num_kv_heads}")
+    for name, t in caches:
+        if not _tma_ready(t):
+            raise ValueError(f"{name} needs a 16-byte aligned base, unit innermost stride and "
+                             "other strides that are multiples of 8")
+    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.numel() < 1:
+        raise ValueError("cu_seqlens must be a [batch + 1] int32 tensor on q's device")
+    batch = cu_seqlens.numel() - 1
+    cu = _int32_on("cu_seqlens", cu_seqlens, q.device, batch + 1)
+    ctx = _int32_on("context_lens", context_lens, q.device, batch)
+    prefix = None if prefix_lens is None else _int32_on("prefix_lens", prefix_lens, q.device, batch)
+    if (not isinstance(block_table, torch.Tensor) or block_table.dim() != 2
+            or block_table.device != q.device or block_table.shape[0] < batch
+            or block_table.shape[1] == 0):
+        raise ValueError("block_table must be [>= batch, max_blocks_per_seq] on q's device")
+    bt = block_table.to(torch.int32)
+    slopes = None
+    if alibi_slopes is not None:
+        if (not isinstance(alibi_slopes, torch.Tensor) or alibi_slopes.device != q.device
+                or alibi_slopes.shape != (q.shape[1],)):
+            raise ValueError("alibi_slopes must be a [num_q_heads] float32 tensor on q's device")
+        slopes = alibi_slopes.to(torch.float32).contiguous()
+    scale = HEAD_DIM ** -0.5 if sm_scale is None else float(sm_scale)
+    return batch, cu, ctx, prefix, bt, slopes, scale
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def paged_chunk_workspace_bytes(total_tokens: int, num_q_heads: int, num_kv_heads: int) -> int:
+    """Workspace bytes ``paged_chunk_attention`` needs for these sizes (current device)."""
+    return int(_lib.load().fi_paged_chunk_workspace_size(total_tokens, num_q_heads, num_kv_heads))
+
+
+def paged_chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                          block_table: torch.Tensor, block_size: int, cu_seqlens: torch.Tensor,
+                          context_lens: torch.Tensor, sm_scale: float = None, *,
+                          softcap: float = 0.0, alibi_slopes: torch.Tensor = None,
+                          window: int = 0, prefix_lens: torch.Tensor = None,
+                          return_lse: bool = False, out: torch.Tensor = None,
+                          workspace: torch.Tensor = None):
+    """Attention of new tokens over the paged cache that holds them and what came before:
+    chunked prefill, verification of drafted tokens, single tokens, or a batch of all three.
+
+    q: [total_tokens, num_q_heads, 128] fp16 or bf16, packed: sequence b owns rows
+    [cu_seqlens[b], cu_seqlens[b+1]). k_cache, v_cache: [num_blocks, 64, num_kv_heads, 128] of
+    q's type, already holding the new tokens' K and V; block_table: [>= batch, max_blocks].
+    context_lens[b] counts the cached tokens with the new ones, so new token i of sequence b has
+    position ``context_lens[b] - n_b + i``.
+
+    Token p sees key j when j <= p (and j > p - window, if ``window``), or j < prefix_lens[b];
+    never past context_lens[b]. Scores are ``q.k * sm_scale``, capped as ``softcap * tanh(x /
+    softcap)`` if ``softcap``, less ``alibi_slopes[head] * |p - j|`` if given (fp32 [num_q_heads]).
+    A token that sees nothing gives zeros and an lse of -inf.
+
+    Returns o like q (written to ``out`` if given; rows outside every sequence are not written),
+    and with ``return_lse`` also lse: fp32 [total_tokens, num_q_heads], the natural log of the sum
+    of exp(score). ``workspace``: uint8, at least ``paged_chunk_workspace_bytes`` bytes; calls that
+    may run at the same time need one each (the default allocates per call).
+    """
+    batch, cu, ctx, prefix, bt, slopes, scale = _chunk_args(
+        q, (("k_cache", k_cache), ("v_cache", v_cache)), block_table, block_size, cu_seqlens,
+        context_lens, sm_scale, alibi_slopes, prefix_lens)
+    total, num_q_heads, _ = q.shape
+    num_blocks, _, num_kv_heads, _ = k_cache.shape
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+        raise ValueError("out must be shaped and typed like q")
+    lse = torch.empty(total, num_q_heads, dtype=torch.float32, device=q.device) \
+        if return_lse else None
+    if batch > 0 and total > 0:
+        qx = q if _tma_ready(q) else q.clone(memory_format=torch.contiguous_format)
+        ox = out if _tma_ready(out) else out.clone(memory_format=torch.contiguous_format)
+        lib = _lib.load()
+        with with_device(q.device):
+            need = int(lib.fi_paged_chunk_workspace_size(total, num_q_heads, num_kv_heads))
+            if workspace is None:
+                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+            elif workspace.device != q.device or not workspace.is_contiguous():
+                raise ValueError("workspace must be contiguous on q's device")
+            err = error_word(q.device)
+            st = lib.fi_paged_chunk(
+                qx.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), ox.data_ptr(), _ptr(lse),
+                bt.data_ptr(), cu.data_ptr(), ctx.data_ptr(), _ptr(prefix), _ptr(slopes), batch,
+                total, num_q_heads, num_kv_heads, HEAD_DIM, num_blocks, block_size, bt.shape[1],
+                _lib.strides(*qx.stride()), _lib.strides(*k_cache.stride()),
+                _lib.strides(*v_cache.stride()), _lib.strides(*ox.stride()),
+                _lib.strides(*bt.stride()), scale, float(softcap), int(window), _DTYPES[q.dtype],
+                workspace.data_ptr(), workspace.numel() * workspace.element_size(), _ptr(err),
+                stream_of(q.device))
+            _lib.check(st, "paged_chunk_attention")
+            device_errors(err, "paged_chunk_attention")
+        if ox is not out:
+            out.copy_(ox)
+    return (out, lse) if return_lse else out

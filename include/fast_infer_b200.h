@@ -19,7 +19,8 @@
  * Pages with an invalid block-table entry are skipped, never dereferenced.
  *
  * Supported: fp16 Q/K/V/O, head_dim 128, KV page (block) size 64, GQA with
- * num_q_heads % num_kv_heads == 0 and num_q_heads / num_kv_heads <= 8 for decode.
+ * num_q_heads % num_kv_heads == 0 and num_q_heads / num_kv_heads <= 8 for decode. The
+ * entry points with a `dtype` argument also take bf16 (FI_DTYPE_BF16).
  */
 #ifndef FAST_INFER_B200_H
 #define FAST_INFER_B200_H
@@ -52,6 +53,10 @@ extern "C" {
  * it. Results are the same bits either way; without the flag the weights are read
  * only after the dependency wait, so they may be the previous kernel's output. */
 #define FI_STATIC_WEIGHTS 1
+
+/* ---- element types (the `dtype` argument) -------------------------------- */
+#define FI_DTYPE_F16 0
+#define FI_DTYPE_BF16 1
 
 /* Library version (major*10000 + minor*100 + patch). */
 int fi_version(void);
@@ -167,6 +172,47 @@ int fi_paged_decode_noalloc(const void* q, const void* k_cache, const void* v_ca
                             const int64_t* vc_strides, const int64_t* o_strides,
                             const int64_t* bt_strides, float sm_scale, int64_t pages_per_split,
                             int32_t* error_flag, void* stream);
+
+/*
+ * Attention of a chunk of new tokens over the paged cache: chunked prefill, verification of
+ * drafted tokens, single tokens, and batches that mix them (no counterpart in the reference,
+ * which attends over the cache with one token per sequence, kernels/attention.py:191-233).
+ *
+ * q, o         : [total_tokens, num_q_heads, 128] (q_strides / o_strides: 3 entries); sequence
+ *                b owns rows [cu_seqlens[b], cu_seqlens[b+1]) (device int32 [batch + 1],
+ *                non-decreasing). Rows of o outside every sequence are left as they were.
+ * k_cache,
+ * v_cache      : [num_blocks, block_size=64, num_kv_heads, 128] (4 strides each);
+ *                block_table [batch, max_blocks_per_seq] as in fi_paged_decode.
+ * context_lens : [batch] int32, cached tokens of each sequence with the new ones, whose K and
+ *                V are in the cache already. New token i of sequence b has position
+ *                p = context_lens[b] - n_b + i.
+ * Token p sees key j if j < context_lens[b] and (j <= p and (window == 0 or j > p - window),
+ * or j < prefix_lens[b]) (prefix_lens: [batch] int32 or NULL: none; window: 0 = unbounded).
+ * score = f(q.k * sm_scale) - alibi_slopes[h] * |p - j|, f(x) = x, or softcap * tanh(x /
+ * softcap) when softcap > 0 (alibi_slopes: fp32 [num_q_heads] or NULL). sm_scale > 0.
+ * o = softmax over the visible keys . v; lse (fp32 [total_tokens, num_q_heads] or NULL) = the
+ * natural log of the sum of exp(score). A token that sees nothing gets o = 0, lse = -inf.
+ * Slots behind a sequence's last token may hold anything. A page whose block-table entry is
+ * invalid is skipped (FI_DEVERR_BAD_BLOCK); lengths that do not fit total_tokens or the block
+ * table are cut and set FI_DEVERR_CONTEXT_LEN.
+ * dtype: of q, k_cache, v_cache and o. workspace: fi_paged_chunk_workspace_size(...) bytes,
+ * 16-byte aligned. At most 64 query heads per KV head, 2048 sequences, and 6000 units of
+ * 2 * (128 / heads per KV head) tokens. Deterministic: the same bits on every run.
+ */
+size_t fi_paged_chunk_workspace_size(int64_t total_tokens, int64_t num_q_heads,
+                                     int64_t num_kv_heads);
+int fi_paged_chunk(const void* q, const void* k_cache, const void* v_cache, void* o, float* lse,
+                   const int32_t* block_table, const int32_t* cu_seqlens,
+                   const int32_t* context_lens, const int32_t* prefix_lens,
+                   const float* alibi_slopes, int64_t batch, int64_t total_tokens,
+                   int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                   int64_t num_blocks, int64_t block_size, int64_t max_blocks_per_seq,
+                   const int64_t* q_strides, const int64_t* kc_strides,
+                   const int64_t* vc_strides, const int64_t* o_strides,
+                   const int64_t* bt_strides, float sm_scale, float softcap, int64_t window,
+                   int64_t dtype, void* workspace, size_t workspace_bytes, int32_t* error_flag,
+                   void* stream);
 
 /*
  * KV-cache slot write: copy new tokens' K and V rows into their pages.

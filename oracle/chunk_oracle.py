@@ -1,0 +1,62 @@
+"""Oracle of the operators over new tokens and a paged cache (TEST INFRASTRUCTURE ONLY):
+attention of a chunk, the weight each cached token receives, eviction and rotary positions with
+several axes, from their definitions in 64 bits with one loop per sequence and head."""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+
+def gather(cache, table_row, n):
+    """Tokens [n, heads, D] of a sequence in float64; pages with an invalid entry give NaN."""
+    num_blocks = cache.shape[0]
+    out = torch.full((n,) + cache.shape[2:], math.nan, dtype=torch.float64)
+    for j in range(n):
+        page = int(table_row[j // 64])
+        if 0 <= page < num_blocks:
+            out[j] = cache[page, j % 64].double()
+    return out
+
+
+def scores(q, k, pos, valid, *, scale, softcap=0.0, slope=0.0, window=0, prefix=0):
+    """Scores [n, keys] of one head with -inf where a token does not see a key."""
+    s = q.double() @ torch.nan_to_num(k).t() * scale
+    if softcap > 0:
+        s = softcap * torch.tanh(s / softcap)
+    p = pos[:, None]
+    j = torch.arange(k.shape[0])[None]
+    s = s - slope * (p - j).abs().double()
+    see = j <= p
+    if window > 0:
+        see = see & (j > p - window)
+    see = (see | (j < prefix)) & valid[None]
+    return s.masked_fill(~see, -math.inf)
+
+
+def chunk(q, k_cache, v_cache, table, cu, ctx, *, scale=128 ** -0.5, softcap=0.0, slopes=None,
+          window=0, prefix=None):
+    """(o, lse, weight of |v|, largest |q||k| sum) of CPU tensors; the last two bound the error."""
+    total, hq, d = q.shape
+    hk = k_cache.shape[2]
+    o = torch.zeros(total, hq, d, dtype=torch.float64)
+    lse = torch.full((total, hq), -math.inf, dtype=torch.float64)
+    absv = torch.zeros_like(o)
+    for b in range(len(ctx)):
+        lo, hi, n = int(cu[b]), int(cu[b + 1]), int(ctx[b])
+        keys = max(n, 0)
+        k, v = gather(k_cache, table[b], keys), gather(v_cache, table[b], keys)
+        valid = ~torch.isnan(k).all(-1).all(-1)
+        pos = torch.arange(n - (hi - lo), n)
+        for h in range(hq):
+            kh = h // (hq // hk)
+            s = scores(q[lo:hi, h], k[:, kh], pos, valid, scale=scale, softcap=softcap,
+                       slope=float(slopes[h]) if slopes is not None else 0.0, window=window,
+                       prefix=int(prefix[b]) if prefix is not None else 0)
+            w = torch.nan_to_num(torch.softmax(s, -1))
+            x = torch.nan_to_num(v[:, kh])
+            o[lo:hi, h] = w @ x
+            absv[lo:hi, h] = w @ x.abs()
+            lse[lo:hi, h] = torch.logsumexp(s, -1)
+    return o, lse, absv
