@@ -89,6 +89,8 @@ __device__ __forceinline__ uint32_t low_bits(int n, int i) {
 constexpr float kTanh0 = 0.9999999502f, kTanh1 = -0.3333283915f, kTanh2 = 0.1332520408f,
                 kTanh3 = -0.05345702957f, kTanh4 = 0.02028998042f, kTanh5 = -0.006203379104f,
                 kTanh6 = 0.001041022634f;
+constexpr float kExp1 = 0.6931469440f, kExp2 = 0.2402212024f, kExp3 = 0.0555071309f,
+                kExp4 = 0.0096755410f, kExp5 = 0.0013276472f;
 // tanh(u) / u on |u| <= 1 as a polynomial in u^2 (minimax on the relative error, fitted
 // here by a Remez exchange: 5.0e-8), for a pair.
 __device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
@@ -116,23 +118,47 @@ __device__ __forceinline__ float tanh_any(float u) {
   return fmaf(-2.f, r, 1.f);
 }
 
+// 2^x for a pair on the FMA pipe, to 2.2e-7 relative (degree 5, fitted here by a Remez exchange
+// with the constant term set to 1): x = n + f as in exp2_poly_x2. x <= -127, -inf among
+// them, gives exactly 0.
+__device__ __forceinline__ uint64_t exp2_poly5_x2(uint64_t x2) {
+  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23
+  float x0, x1;
+  f32x2_split(x2, x0, x1);
+  const uint64_t x = f32x2(fmaxf(x0, -127.0f), fmaxf(x1, -127.0f));
+  const uint64_t t = add_f32x2(x, f32x2(kMagic, kMagic));
+  const uint64_t n = add_f32x2(t, f32x2(-kMagic, -kMagic));
+  const uint64_t f = fma_f32x2(n, f32x2(-1.0f, -1.0f), x);
+  uint64_t q = fma_f32x2(f32x2(kExp5, kExp5), f, f32x2(kExp4, kExp4));
+  q = fma_f32x2(q, f, f32x2(kExp3, kExp3));
+  q = fma_f32x2(q, f, f32x2(kExp2, kExp2));
+  q = fma_f32x2(q, f, f32x2(kExp1, kExp1));
+  q = fma_f32x2(q, f, f32x2(1.0f, 1.0f));
+  float q0, q1, t0, t1;
+  f32x2_split(q, q0, q1);
+  f32x2_split(t, t0, t1);
+  return f32x2(__uint_as_float(__float_as_uint(q0) + (__float_as_uint(t0) << 23)),
+               __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23)));
+}
+
 // Inclusive sums of a[1..n] in place (a[0] stays); every thread of the block calls it.
 // `warp_sums`: one word per warp. Each thread owns a run of consecutive entries.
-__device__ __forceinline__ void block_scan(uint32_t* a, int n, uint32_t* warp_sums) {
+template <typename U>
+__device__ __forceinline__ void block_scan(U* a, int n, U* warp_sums) {
   const int threads = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int each = (n + threads - 1) / threads;
   const int lo = 1 + min(tid * each, n), hi = 1 + min(tid * each + each, n);
-  uint32_t sum = 0;
+  U sum = 0;
   for (int i = lo; i < hi; ++i) sum += a[i];
-  uint32_t inc = sum;
+  U inc = sum;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const uint32_t v = __shfl_up_sync(0xffffffffu, inc, off);
+    const U v = __shfl_up_sync(0xffffffffu, inc, off);
     if (lane >= off) inc += v;
   }
   if (lane == 31) warp_sums[warp] = inc;
   __syncthreads();
-  uint32_t run = inc - sum;
+  U run = inc - sum;
   for (int w = 0; w < warp; ++w) run += warp_sums[w];
   for (int i = lo; i < hi; ++i) {
     run += a[i];
@@ -142,7 +168,8 @@ __device__ __forceinline__ void block_scan(uint32_t* a, int n, uint32_t* warp_su
 }
 
 // The last i in [0, n) with a[i] <= x (a ascending, a[0] <= x).
-__device__ __forceinline__ int last_le(const uint32_t* a, int n, uint32_t x) {
+template <typename U>
+__device__ __forceinline__ int last_le(const U* a, int n, U x) {
   int lo = 0, hi = n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;

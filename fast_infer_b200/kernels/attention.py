@@ -14,7 +14,7 @@ Backward-compatible extensions:
 
 Functions without a reference counterpart, for serving long contexts in chunks (fp16 and
 bf16): ``paged_chunk_attention`` (new tokens over the paged cache, with capped scores, a
-distance bias, a window or a prefix).
+distance bias, a window or a prefix) and ``attention_mass`` (the weight each cached token received).
 """
 
 from __future__ import annotations
@@ -360,3 +360,65 @@ def paged_chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
         if ox is not out:
             out.copy_(ox)
     return (out, lse) if return_lse else out
+
+
+def attention_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tensor,
+                   block_size: int, cu_seqlens: torch.Tensor, context_lens: torch.Tensor,
+                   lse: torch.Tensor, sm_scale: float = None, *, softcap: float = 0.0,
+                   alibi_slopes: torch.Tensor = None, window: int = 0,
+                   prefix_lens: torch.Tensor = None, mass: torch.Tensor = None,
+                   workspace: torch.Tensor = None) -> torch.Tensor:
+    """Attention weight that each cached token receives from the new tokens, per KV head.
+
+    ``mass[b, hk, j]`` = sum of ``exp(score - lse)`` over sequence b's new tokens and the query
+    heads of hk. Arguments and score form as in ``paged_chunk_attention``, whose ``lse`` this takes;
+    pass the last tokens alone (with ``cu_seqlens`` to match) for the weight of a window of
+    them. ``mass``: fp32 [batch, num_kv_heads, capacity] to add to and return (what cached
+    tokens had before); without it, a new one of the block table's span, 0 where nothing sees.
+    ``workspace``: uint8, at least ``attention_mass_workspace_bytes`` bytes; calls that may run at
+    the same time need one each (the default allocates per call).
+    """
+    batch, cu, ctx, prefix, bt, slopes, scale = _chunk_args(
+        q, (("k_cache", k_cache),), block_table, block_size, cu_seqlens, context_lens, sm_scale,
+        alibi_slopes, prefix_lens)
+    total, num_q_heads, _ = q.shape
+    num_blocks, _, num_kv_heads, _ = k_cache.shape
+    if (not isinstance(lse, torch.Tensor) or lse.shape != (total, num_q_heads)
+            or lse.dtype != torch.float32 or lse.device != q.device):
+        raise ValueError("lse must be [total_tokens, num_q_heads] float32 on q's device")
+    accumulate = mass is not None
+    if mass is None:
+        mass = torch.empty(batch, num_kv_heads, bt.shape[1] * BLOCK_SIZE, dtype=torch.float32,
+                           device=q.device)
+    elif (mass.dim() != 3 or mass.shape[:2] != (batch, num_kv_heads) or not mass.is_contiguous()
+          or mass.dtype != torch.float32 or mass.device != q.device):
+        raise ValueError("mass must be a contiguous [batch, num_kv_heads, capacity] float32 tensor "
+                         "on q's device")
+    if mass.numel() == 0:
+        return mass
+    qx = q if _tma_ready(q) else q.clone(memory_format=torch.contiguous_format)
+    lse = lse.contiguous()
+    lib = _lib.load()
+    with with_device(q.device):
+        if workspace is None:
+            workspace = torch.empty(attention_mass_workspace_bytes(), dtype=torch.uint8,
+                                    device=q.device)
+        elif workspace.device != q.device or not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous on q's device")
+        err = error_word(q.device)
+        st = lib.fi_attention_mass(
+            qx.data_ptr(), k_cache.data_ptr(), lse.data_ptr(), mass.data_ptr(), bt.data_ptr(),
+            cu.data_ptr(), ctx.data_ptr(), _ptr(prefix), _ptr(slopes), batch, total, num_q_heads,
+            num_kv_heads, HEAD_DIM, num_blocks, block_size, bt.shape[1],
+            _lib.strides(*qx.stride()), _lib.strides(*k_cache.stride()),
+            _lib.strides(*bt.stride()), mass.shape[2], int(accumulate), scale, float(softcap),
+            int(window), _DTYPES[q.dtype], workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), _ptr(err), stream_of(q.device))
+        _lib.check(st, "attention_mass")
+        device_errors(err, "attention_mass")
+    return mass
+
+
+def attention_mass_workspace_bytes() -> int:
+    """Workspace bytes ``attention_mass`` needs (current device)."""
+    return int(_lib.load().fi_attention_mass_workspace_size())

@@ -215,6 +215,32 @@ int fi_paged_chunk(const void* q, const void* k_cache, const void* v_cache, void
                    void* stream);
 
 /*
+ * Attention weight that each cached token receives from the new tokens (no counterpart in the
+ * reference; what an eviction from the cache goes by):
+ *   mass[b, hk, j] (+)= sum over query rows i of KV head hk of exp(score_ij - lse_i).
+ * q, k_cache, block_table, cu_seqlens, context_lens, prefix_lens, alibi_slopes, sm_scale, softcap,
+ * window, dtype and the limits: as in fi_paged_chunk (any number of tokens; 2048 sequences);
+ * lse: fp32 [total_tokens, num_q_heads], dense, from that call. mass: fp32 [batch, num_kv_heads,
+ * mass_capacity], dense; accumulate 0 writes all of it (0 where nothing sees, past the
+ * context too), any other value adds to it and leaves the rest as it was. Cached tokens past
+ * mass_capacity are dropped (FI_DEVERR_CONTEXT_LEN). A row with lse = -inf gives no weight, nor
+ * does a page with an invalid block-table entry receive any. workspace:
+ * fi_attention_mass_workspace_size() bytes, 16-byte aligned. Deterministic.
+ */
+size_t fi_attention_mass_workspace_size(void);
+int fi_attention_mass(const void* q, const void* k_cache, const float* lse, float* mass,
+                      const int32_t* block_table, const int32_t* cu_seqlens,
+                      const int32_t* context_lens, const int32_t* prefix_lens,
+                      const float* alibi_slopes, int64_t batch, int64_t total_tokens,
+                      int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                      int64_t num_blocks, int64_t block_size, int64_t max_blocks_per_seq,
+                      const int64_t* q_strides, const int64_t* kc_strides,
+                      const int64_t* bt_strides, int64_t mass_capacity, int64_t accumulate,
+                      float sm_scale, float softcap, int64_t window, int64_t dtype,
+                      void* workspace, size_t workspace_bytes, int32_t* error_flag,
+                      void* stream);
+
+/*
  * KV-cache slot write: copy new tokens' K and V rows into their pages.
  *
  * Replaces: the slot writes of model.py:162-183 (`_store_kv_prefill`), model.py:185-201

@@ -60,3 +60,25 @@ def chunk(q, k_cache, v_cache, table, cu, ctx, *, scale=128 ** -0.5, softcap=0.0
             absv[lo:hi, h] = w @ x.abs()
             lse[lo:hi, h] = torch.logsumexp(s, -1)
     return o, lse, absv
+
+
+def mass(q, k_cache, table, cu, ctx, lse, *, scale=128 ** -0.5, softcap=0.0, slopes=None, window=0,
+         prefix=None):
+    """[batch, hk, table span] of CPU tensors, and the rows that each value sums."""
+    hq, hk = q.shape[1], k_cache.shape[2]
+    out = torch.zeros(len(ctx), hk, table.shape[1] * 64, dtype=torch.float64)
+    for b in range(len(ctx)):
+        lo, hi, n = int(cu[b]), int(cu[b + 1]), int(ctx[b])
+        keys = max(n, 0)
+        k = gather(k_cache, table[b], keys)
+        valid = ~torch.isnan(k).all(-1).all(-1)
+        pos = torch.arange(n - (hi - lo), n)
+        for h in range(hq):
+            kh = h // (hq // hk)
+            s = scores(q[lo:hi, h], k[:, kh], pos, valid, scale=scale, softcap=softcap,
+                       slope=float(slopes[h]) if slopes is not None else 0.0, window=window,
+                       prefix=int(prefix[b]) if prefix is not None else 0)
+            w = torch.exp(s - lse[lo:hi, h].double()[:, None])
+            w[s == -math.inf] = 0.0
+            out[b, kh, :keys] += w.sum(0)
+    return out
