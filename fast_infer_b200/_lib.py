@@ -65,6 +65,13 @@ SIGNATURES = {
     "fi_attention_mass": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
                                          _i64, _i64, _i64, _i64, _i64, _i64, _i64p, _i64p, _i64p,
                                          _i64, _i64, _f32, _f32, _i64, _i64, _vp, _sz, _vp, _vp]),
+    "fi_rope_axes_store": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64,
+                                          _i64, _i64, _i64, _i64, _i64, _i64p, _i64, _i64, _i64,
+                                          _i64, _i64, _i64, _i64p, _i64p, _i64p, _i64p, _i64p,
+                                          _i64, _vp, _vp]),
+    "fi_kv_evict": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
+                                   _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                   _i64, _i64p, _i64p, _i64p, _i64p, _i64p, _i64p, _vp, _vp]),
     "fi_rope_kv_write": (ctypes.c_int, [_vp, _i64, _i64, _i64, _i64, _i64, _i64p, _vp, _vp, _i64,
                                         _i64, _vp, _i64, _vp, _i64p, _vp, _i64p, _vp, _vp, _vp,
                                         _i64, _i64, _i64, _i64p, _i64p, _i64p, _vp, _vp]),

@@ -1,0 +1,386 @@
+// Eviction from the paged KV cache by accumulated attention weight.
+//
+// For every (layer, sequence, KV head) with more than `budget` cached tokens, the first `sinks`,
+// the last `recent` and, of those between, the ones of greatest weight stay, `budget` in all;
+// ties go to the lowest index, and a weight that is negative or NaN counts as 0. What stays
+// keeps its order and moves to slots 0 .. budget-1, of the same pages (in place) or of another
+// pool's.
+//
+// Two launches. evict_select_kernel, a CTA per (layer, sequence, KV head), finds the weight of
+// the last token that stays by its bits: a non-negative float orders like its bits, so three
+// histograms (11, 11 and 10 bits, from the top) leave one value and how many of its equals
+// stay; then each warp lists what it keeps of its run of tokens. evict_copy_kernel moves the
+// rows, 256 bytes each: bound by HBM, so it keeps many independent 16-byte loads in flight.
+#include "common.cuh"
+#include "host_common.h"
+
+namespace fi {
+
+constexpr int kEvPage = 64;
+constexpr int kEvThreads = 512;                  // select
+constexpr int kEvBins = 2048;
+constexpr int kEvStageMax = 48 * 1024;           // tokens whose weights are kept in shared memory
+constexpr int kEvCopyThreads = 256;
+constexpr int kEvSeg = 128;                      // tokens a copy CTA moves, out of place
+constexpr int kEvInThreads = 512;                // copy in place
+constexpr int kEvInSeg = 64;                     // tokens it moves between two barriers
+
+struct EvictArgs {
+  const char* k;
+  const char* v;
+  char* ko;
+  char* vo;
+  const int32_t* bt;
+  const int32_t* bto;
+  const int32_t* lens;
+  const float* mass;
+  int32_t* kept;    // [layers, batch, heads, budget]
+  float* mass_out;  // [layers, batch, heads, budget]
+  int* err;
+  int64_t ks[4], vs[4], kos[4], vos[4];  // bytes: layer, page, slot, head
+  int64_t bts[2], btos[2];
+  int64_t cap;  // tokens of a row of mass
+  int layers, batch, heads, num_blocks, num_blocks_out, max_blocks, max_blocks_out;
+  int budget, recent, sinks, stage;
+};
+
+// Cached tokens of sequence b that the tables can hold.
+__device__ __forceinline__ int evict_len(const EvictArgs& a, int b) {
+  const int n = a.lens[b];
+  return max(0, (int)min((int64_t)n, min((int64_t)a.max_blocks * kEvPage, a.cap)));
+}
+
+__device__ __forceinline__ uint32_t weight_bits(float w) { return w > 0.f ? __float_as_uint(w) : 0u; }
+
+// The bin, from the top, in which the count of larger values reaches `want`: on return `want`
+// is how many of that bin's values stay. hist has kEvBins counts; all threads call it.
+__device__ __forceinline__ int top_bin(const uint32_t* hist, int bins, int& want, uint32_t* sums,
+                                       int* found) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int each = (bins + kEvThreads - 1) / kEvThreads;  // this thread's bins, from the top
+  uint32_t sum = 0;
+  for (int i = 0; i < each; ++i) {
+    const int bin = bins - 1 - (tid * each + i);
+    if (bin >= 0) sum += hist[bin];
+  }
+  uint32_t inc = sum;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const uint32_t x = __shfl_up_sync(0xffffffffu, inc, off);
+    if (lane >= off) inc += x;
+  }
+  if (lane == 31) sums[warp] = inc;
+  __syncthreads();
+  uint32_t above = inc - sum;
+  for (int w = 0; w < warp; ++w) above += sums[w];
+  if (above < (uint32_t)want && above + sum >= (uint32_t)want) {
+    for (int i = 0; i < each; ++i) {
+      const int bin = bins - 1 - (tid * each + i);
+      if (above + hist[bin] >= (uint32_t)want) {
+        found[0] = bin;
+        found[1] = want - (int)above;
+        break;
+      }
+      above += hist[bin];
+    }
+  }
+  __syncthreads();
+  want = found[1];
+  return found[0];
+}
+
+__global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArgs a) {
+  extern __shared__ uint32_t ev_smem[];
+  uint32_t* hist = ev_smem;             // [kEvBins]
+  uint32_t* stage = ev_smem + kEvBins;  // [a.stage]
+  __shared__ uint32_t sums[kEvThreads / 32];
+  __shared__ uint32_t run_over[kEvThreads / 32], run_same[kEvThreads / 32];
+  __shared__ int found[2];
+  grid_dep_wait();
+  grid_dep_launch();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t row = blockIdx.x;
+  const int b = (int)(row / a.heads % a.batch);
+  const float* mass = a.mass + row * a.cap;
+  int32_t* kept = a.kept + row * a.budget;
+  float* mass_out = a.mass_out + row * a.budget;
+  const int n = evict_len(a, b);
+  if (tid == 0 && row % ((int64_t)a.batch * a.heads) == (int64_t)b * a.heads &&
+      row < (int64_t)a.batch * a.heads && n != a.lens[b])
+    set_error(a.err, FI_DEVERR_CONTEXT_LEN);
+  if (n <= a.budget) {
+    for (int i = tid; i < a.budget; i += kEvThreads) {
+      kept[i] = i < n ? i : -1;
+      mass_out[i] = i < n ? mass[i] : 0.f;
+    }
+    return;
+  }
+  const int lo = a.sinks, hi = n - a.recent;  // the tokens that compete
+  const bool staged = n <= a.stage;
+  auto bits = [&](int j) { return staged ? stage[j] : weight_bits(mass[j]); };
+  int want = a.budget - a.sinks - a.recent;
+  uint32_t edge = 0xffffffffu;  // weights above it stay, and `want` of its equals
+  if (want > 0) {
+    uint32_t prefix = 0;
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+      const int bins = pass == 2 ? 1024 : 2048;
+      for (int i = tid; i < bins; i += kEvThreads) hist[i] = 0;
+      __syncthreads();
+      if (pass == 0) {
+        for (int j = tid; j < n; j += kEvThreads) {
+          const uint32_t x = weight_bits(mass[j]);
+          if (staged) stage[j] = x;
+          if (j >= lo && j < hi) atomicAdd(&hist[x >> 21], 1u);
+        }
+      } else {
+        const int top = pass == 1 ? 21 : 10;
+        for (int j = lo + tid; j < hi; j += kEvThreads) {
+          const uint32_t x = bits(j);
+          if (x >> top == prefix) atomicAdd(&hist[(x >> shift) & (bins - 1)], 1u);
+        }
+      }
+      __syncthreads();
+      const int bin = top_bin(hist, bins, want, sums, found);
+      prefix = (prefix << (pass == 2 ? 10 : 11)) | (uint32_t)bin;
+    }
+    edge = prefix;
+  } else if (staged) {
+    for (int j = tid; j < n; j += kEvThreads) stage[j] = weight_bits(mass[j]);
+    __syncthreads();
+  }
+  // Each warp has a run of tokens: count what is over the edge and what equals it, then list.
+  const int each = ((n + kEvThreads - 1) / kEvThreads) * 32;
+  const int j0 = min(warp * each, n), j1 = min(j0 + each, n);
+  uint32_t over = 0, same = 0;
+  for (int j = j0 + lane; j < j1; j += 32) {
+    const bool mid = j >= lo && j < hi;
+    const uint32_t x = mid ? bits(j) : 0u;
+    over += !mid || x > edge;
+    same += mid && x == edge;
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    over += __shfl_xor_sync(0xffffffffu, over, off);
+    same += __shfl_xor_sync(0xffffffffu, same, off);
+  }
+  if (lane == 0) {
+    run_over[warp] = over;
+    run_same[warp] = same;
+  }
+  __syncthreads();
+  uint32_t before_over = 0, before_same = 0;
+  for (int w = 0; w < warp; ++w) {
+    before_over += run_over[w];
+    before_same += run_same[w];
+  }
+  const uint32_t below = (1u << lane) - 1u;
+  for (int base = j0; base < j1; base += 32) {
+    const int j = base + lane;
+    const bool in = j < j1, mid = in && j >= lo && j < hi;
+    const uint32_t x = mid ? bits(j) : 0u;
+    const bool is_over = in && (!mid || x > edge), is_same = mid && x == edge;
+    const uint32_t bo = __ballot_sync(0xffffffffu, is_over), bs = __ballot_sync(0xffffffffu, is_same);
+    const uint32_t same_rank = before_same + __popc(bs & below);
+    if (is_over || (is_same && same_rank < (uint32_t)want)) {
+      const uint32_t at = before_over + __popc(bo & below) + min(same_rank, (uint32_t)want);
+      kept[at] = j;
+      mass_out[at] = mass[j];
+    }
+    before_over += __popc(bo);
+    before_same += __popc(bs);
+  }
+}
+
+// Page and slot of a token, or page -1 if the table's entry is invalid.
+__device__ __forceinline__ int2 evict_slot(const int32_t* bt, const int64_t* bts, int b, int j,
+                                           int max_blocks, int num_blocks) {
+  const int pg = j / kEvPage;
+  int page = -1;
+  if (pg < max_blocks) page = bt[b * bts[0] + (int64_t)pg * bts[1]];
+  if (page >= num_blocks) page = -1;
+  return make_int2(page, j % kEvPage);
+}
+
+__device__ __forceinline__ uint4 ld_stream(const char* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+// Moves one segment of kThreads / 16 * kTokens tokens: a half warp per token and iteration.
+// In place a CTA walks all segments of its (layer, sequence, head) in order. That is safe: a
+// token's new slot is never past its old one, so what a segment writes, later segments do not
+// read; within one, every load comes before any store.
+template <int kThreads, int kSeg, bool kInPlace>
+__global__ void __launch_bounds__(kThreads) evict_copy_kernel(const EvictArgs a, int segs) {
+  constexpr int kPer = kSeg * 16 / kThreads;  // 16-byte pieces of K, and of V, a thread moves
+  __shared__ int2 src[kSeg], dst[kSeg];
+  grid_dep_wait();
+  grid_dep_launch();
+  const int tid = threadIdx.x, piece = tid & 15;
+  // the heads of one stretch of tokens run side by side: their rows are neighbours in memory
+  int64_t r = blockIdx.x;
+  const int h = (int)(r % a.heads);
+  r /= a.heads;
+  const int seg = kInPlace ? 0 : (int)(r % segs);
+  if (!kInPlace) r /= segs;
+  const int b = (int)(r % a.batch), layer = (int)(r / a.batch);
+  const int n = evict_len(a, b);
+  const int count = min(n, a.budget);
+  if (kInPlace && n <= a.budget) return;
+  const int32_t* kept = a.kept + (((int64_t)layer * a.batch + b) * a.heads + h) * a.budget;
+  const char* k = a.k + layer * a.ks[0] + h * a.ks[3] + piece * 16;
+  const char* v = a.v + layer * a.vs[0] + h * a.vs[3] + piece * 16;
+  char* ko = a.ko + layer * a.kos[0] + h * a.kos[3] + piece * 16;
+  char* vo = a.vo + layer * a.vos[0] + h * a.vos[3] + piece * 16;
+  for (int t0 = seg * kSeg; t0 < count; t0 += kSeg) {
+    for (int i = tid; i < min(kSeg, count - t0); i += kThreads) {
+      const int j = kept[t0 + i];
+      src[i] = evict_slot(a.bt, a.bts, b, j, a.max_blocks, a.num_blocks);
+      dst[i] = evict_slot(a.bto, a.btos, b, t0 + i, a.max_blocks_out, a.num_blocks_out);
+      if (src[i].x < 0 || dst[i].x < 0) {
+        set_error(a.err, FI_DEVERR_BAD_BLOCK);
+        src[i].x = -1;
+      } else if (kInPlace && j == t0 + i) {
+        src[i].x = -1;  // it stays where it is
+      }
+    }
+    __syncthreads();
+    uint4 kx[kPer], vx[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int t = (tid >> 4) + i * (kThreads / 16);
+      if (t0 + t < count && src[t].x >= 0) {
+        kx[i] = ld_stream(k + src[t].x * a.ks[1] + src[t].y * a.ks[2]);
+        vx[i] = ld_stream(v + src[t].x * a.vs[1] + src[t].y * a.vs[2]);
+      }
+    }
+    if (kInPlace) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int t = (tid >> 4) + i * (kThreads / 16);
+      if (t0 + t < count && src[t].x >= 0) {
+        *reinterpret_cast<uint4*>(ko + dst[t].x * a.kos[1] + dst[t].y * a.kos[2]) = kx[i];
+        *reinterpret_cast<uint4*>(vo + dst[t].x * a.vos[1] + dst[t].y * a.vos[2]) = vx[i];
+      }
+    }
+    if (!kInPlace) break;
+    __syncthreads();  // src and dst are read before the next segment's are written
+  }
+}
+
+}  // namespace fi
+
+extern "C" int fi_kv_evict(const void* k, const void* v, const int32_t* block_table,
+                           const int32_t* seq_lens, const float* mass, void* k_out, void* v_out,
+                           const int32_t* block_table_out, int32_t* kept, float* mass_out,
+                           int64_t layers, int64_t batch, int64_t num_heads, int64_t head_dim,
+                           int64_t num_blocks, int64_t num_blocks_out, int64_t block_size,
+                           int64_t max_blocks_per_seq, int64_t max_blocks_per_seq_out,
+                           int64_t mass_capacity, int64_t budget, int64_t recent, int64_t sinks,
+                           const int64_t* k_strides, const int64_t* v_strides,
+                           const int64_t* ko_strides, const int64_t* vo_strides,
+                           const int64_t* bt_strides, const int64_t* bto_strides,
+                           int32_t* error_flag, void* stream) {
+  using namespace fi;
+  clear_error();
+  if (layers < 0 || batch < 0 || num_heads <= 0 || num_blocks <= 0 || num_blocks_out <= 0 ||
+      max_blocks_per_seq <= 0 || max_blocks_per_seq_out <= 0 || mass_capacity < 0)
+    return fail(FI_ERR_INVALID_ARG, "fi_kv_evict: bad sizes");
+  if (budget <= 0 || recent < 0 || sinks < 0 || recent > budget || sinks > budget - recent)
+    return fail(FI_ERR_INVALID_ARG,
+                "fi_kv_evict: needs budget >= 1 and recent + sinks <= budget (got %lld, %lld, %lld)",
+                (long long)budget, (long long)recent, (long long)sinks);
+  if (head_dim != 128)
+    return fail(FI_ERR_UNSUPPORTED, "fi_kv_evict: head_dim %lld != 128", (long long)head_dim);
+  if (block_size != kEvPage)
+    return fail(FI_ERR_UNSUPPORTED, "fi_kv_evict: block_size %lld != 64", (long long)block_size);
+  if (budget > max_blocks_per_seq_out * kEvPage)
+    return fail(FI_ERR_INVALID_ARG, "fi_kv_evict: budget %lld does not fit the output block table",
+                (long long)budget);
+  if (layers == 0 || batch == 0) return FI_OK;
+  if (!k || !v || !block_table || !seq_lens || !mass || !k_out || !v_out || !block_table_out ||
+      !kept || !mass_out || !k_strides || !v_strides || !ko_strides || !vo_strides || !bt_strides ||
+      !bto_strides)
+    return fail(FI_ERR_INVALID_ARG, "fi_kv_evict: null pointer argument");
+  const bool in_place = k_out == k;
+  if (in_place != (v_out == v) || in_place != (block_table_out == block_table))
+    return fail(FI_ERR_INVALID_ARG,
+                "fi_kv_evict: in place needs k, v and the block table themselves as outputs, out of "
+                "place none of them");
+  if (num_blocks > (1 << 30) || num_blocks_out > (1 << 30) || max_blocks_per_seq > (1 << 24) ||
+      max_blocks_per_seq_out > (1 << 24))
+    return fail(FI_ERR_UNSUPPORTED, "fi_kv_evict: sizes too large");
+  const int64_t rows = layers * batch * num_heads;
+  const int64_t segs = in_place ? 1 : (budget + kEvSeg - 1) / kEvSeg;
+  if (layers > (1 << 20) || batch > (1 << 20) || num_heads > 65535 || rows > 0x7fffffff ||
+      segs > 0x7fffffff / rows)
+    return fail(FI_ERR_UNSUPPORTED, "fi_kv_evict: sizes too large");
+  EvictArgs a = {};
+  bool ok = aligned16(k) && aligned16(v) && aligned16(k_out) && aligned16(v_out);
+  const int64_t* strides[4] = {k_strides, v_strides, ko_strides, vo_strides};
+  int64_t* bytes[4] = {a.ks, a.vs, a.kos, a.vos};
+  for (int t = 0; t < 4; ++t) {
+    ok = ok && strides[t][4] == 1;
+    for (int i = 0; i < 4; ++i) {
+      ok = ok && strides[t][i] % 8 == 0;
+      bytes[t][i] = strides[t][i] * 2;
+      if (in_place && t >= 2 && strides[t][i] != strides[t - 2][i])
+        return fail(FI_ERR_INVALID_ARG, "fi_kv_evict: in place with other strides");
+    }
+  }
+  if (!ok)
+    return fail(FI_ERR_ALIGNMENT,
+                "fi_kv_evict: caches need 16-byte aligned bases, unit innermost strides and other "
+                "strides that are multiples of 8 elements");
+  a.k = static_cast<const char*>(k);
+  a.v = static_cast<const char*>(v);
+  a.ko = static_cast<char*>(k_out);
+  a.vo = static_cast<char*>(v_out);
+  a.bt = block_table;
+  a.bto = block_table_out;
+  a.lens = seq_lens;
+  a.mass = mass;
+  a.kept = kept;
+  a.mass_out = mass_out;
+  a.err = error_flag;
+  a.bts[0] = bt_strides[0];
+  a.bts[1] = bt_strides[1];
+  a.btos[0] = bto_strides[0];
+  a.btos[1] = bto_strides[1];
+  a.cap = mass_capacity;
+  a.layers = (int)layers;
+  a.batch = (int)batch;
+  a.heads = (int)num_heads;
+  a.num_blocks = (int)num_blocks;
+  a.num_blocks_out = (int)num_blocks_out;
+  a.max_blocks = (int)max_blocks_per_seq;
+  a.max_blocks_out = (int)max_blocks_per_seq_out;
+  a.budget = (int)budget;
+  a.recent = (int)recent;
+  a.sinks = (int)sinks;
+  const int64_t longest = max_blocks_per_seq * kEvPage < mass_capacity
+                              ? max_blocks_per_seq * kEvPage : mass_capacity;
+  a.stage = (int)(longest <= kEvStageMax ? longest : 0);
+  static DeviceOnce once;
+  cudaError_t e = once.run([] {
+    return cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (kEvBins + kEvStageMax) * 4);
+  });
+  if (e != cudaSuccess) return cuda_fail(e, "fi_kv_evict: cudaFuncSetAttribute");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  e = launch_pdl(evict_select_kernel, dim3((unsigned)rows), dim3(kEvThreads),
+                 (size_t)(kEvBins + a.stage) * 4, st, a);
+  if (e != cudaSuccess) return cuda_fail(e, "fi_kv_evict: select launch");
+  if (in_place)
+    e = launch_pdl(evict_copy_kernel<kEvInThreads, kEvInSeg, true>, dim3((unsigned)rows),
+                   dim3(kEvInThreads), 0, st, a, 1);
+  else
+    e = launch_pdl(evict_copy_kernel<kEvCopyThreads, kEvSeg, false>, dim3((unsigned)(rows * segs)),
+                   dim3(kEvCopyThreads), 0, st, a, (int)segs);
+  if (e != cudaSuccess) return cuda_fail(e, "fi_kv_evict: copy launch");
+  return FI_OK;
+}

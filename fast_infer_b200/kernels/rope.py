@@ -1,0 +1,108 @@
+"""Rotary positions with several axes, with the KV-cache slot write, for packed new tokens.
+
+The reference's RoPE (kernels/rope.py:9-44) and its slot writes share one counter, as
+``kv_cache.rope_and_store`` does; here a token's positions (time, height, width of an image or
+video, or one position that an eviction has set apart from the slot) are given, and its slot
+follows from the cache's lengths.
+"""
+
+from __future__ import annotations
+
+from typing import Sequence
+
+import torch
+
+from fast_infer_b200 import _lib
+from fast_infer_b200._runtime import device_errors, error_word, stream_of, with_device
+from fast_infer_b200.kernels.attention import (_DTYPES, BLOCK_SIZE, HEAD_DIM, _int32_on,
+                                               _tma_ready)
+
+
+def rope_axes_store(qkv: torch.Tensor, num_q_heads: int, cos_table: torch.Tensor,
+                    sin_table: torch.Tensor, positions: torch.Tensor, sections: Sequence[int],
+                    k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                    block_size: int, cu_seqlens: torch.Tensor, context_lens: torch.Tensor,
+                    q_out: torch.Tensor = None) -> torch.Tensor:
+    """Rotate q and k of packed new tokens and write k and v to their cache slots, in one launch.
+
+    qkv: [total_tokens, (nq + 2 * nkv) * 128] fp16 or bf16 (q | k | v heads). positions: int32
+    [axes, total_tokens] on the device (1 to 4 axes); sections: how many of the 64 frequencies, in
+    order, use each axis. cos_table, sin_table: fp32 [rows, 128], indexed by position. k_cache,
+    v_cache, block_table, cu_seqlens, context_lens: as in ``paged_chunk_attention``, which takes
+    them next; new token i of sequence b is stored at slot ``context_lens[b] - n_b + i``.
+
+    The rotation is the rotate-half form in fp32, rounded once. Returns the rotated q
+    [total_tokens, nq, 128] (``q_out`` if given; rows outside every sequence are not written).
+    """
+    if not isinstance(qkv, torch.Tensor):
+        raise TypeError("qkv must be a torch.Tensor")
+    if not qkv.is_cuda:
+        raise ValueError("qkv must be a CUDA tensor (fast_infer_b200 has no CPU path)")
+    if qkv.dtype not in _DTYPES:
+        raise TypeError(f"qkv must be float16 or bfloat16, got {qkv.dtype}")
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if not isinstance(t, torch.Tensor) or t.dtype != qkv.dtype or t.device != qkv.device:
+            raise ValueError(f"{name} must have qkv's type and device")
+        if t.dim() != 4 or t.shape != k_cache.shape or t.shape[1] != BLOCK_SIZE \
+                or t.shape[3] != HEAD_DIM or t.numel() == 0:
+            raise ValueError(f"{name} must be [num_blocks, {BLOCK_SIZE}, num_kv_heads, {HEAD_DIM}]")
+        if not _tma_ready(t):
+            raise ValueError(f"{name} needs a 16-byte aligned base, unit innermost stride and "
+                             "other strides that are multiples of 8")
+    if block_size != BLOCK_SIZE:
+        raise ValueError(f"block_size must be {BLOCK_SIZE}")
+    num_blocks, _, nkv, _ = k_cache.shape
+    if num_q_heads < 1 or qkv.dim() != 2 or qkv.shape[1] != (num_q_heads + 2 * nkv) * HEAD_DIM:
+        raise ValueError("qkv must be [total_tokens, (num_q_heads + 2 * num_kv_heads) * head_dim]")
+    total = qkv.shape[0]
+    sections = [int(s) for s in sections]
+    if (not isinstance(positions, torch.Tensor) or positions.device != qkv.device
+            or positions.shape != (len(sections), total)):
+        raise ValueError("positions must be an [axes, total_tokens] int32 tensor on qkv's device, "
+                         "an axis for each section")
+    if not 1 <= len(sections) <= 4 or min(sections) < 0 or sum(sections) != HEAD_DIM // 2:
+        raise ValueError(f"sections must be 1 to 4 counts that add up to {HEAD_DIM // 2}")
+    for name, t in (("cos_table", cos_table), ("sin_table", sin_table)):
+        if (not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != qkv.device
+                or t.dim() != 2 or t.shape[1] != HEAD_DIM or t.stride(1) != 1
+                or t.shape != cos_table.shape or t.stride(0) != cos_table.stride(0)
+                or t.shape[0] == 0):
+            raise ValueError(f"{name} must be a float32 [max_pos, {HEAD_DIM}] table on qkv's device")
+    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.numel() < 1:
+        raise ValueError("cu_seqlens must be a [batch + 1] int32 tensor on qkv's device")
+    batch = cu_seqlens.numel() - 1
+    cu = _int32_on("cu_seqlens", cu_seqlens, qkv.device, batch + 1)
+    ctx = _int32_on("context_lens", context_lens, qkv.device, batch)
+    if (not isinstance(block_table, torch.Tensor) or block_table.dim() != 2
+            or block_table.device != qkv.device or block_table.shape[0] < batch
+            or block_table.shape[1] == 0):
+        raise ValueError("block_table must be [>= batch, max_blocks_per_seq] on qkv's device")
+    if q_out is None:
+        q_out = torch.empty(total, num_q_heads, HEAD_DIM, dtype=qkv.dtype, device=qkv.device)
+    elif (q_out.shape != (total, num_q_heads, HEAD_DIM) or q_out.dtype != qkv.dtype
+          or q_out.device != qkv.device or not _tma_ready(q_out)):
+        raise ValueError("q_out must be [total_tokens, num_q_heads, head_dim] like qkv, 16-byte "
+                         "aligned")
+    if batch == 0 or total == 0:
+        return q_out
+    x = qkv if _tma_ready(qkv) else qkv.clone(memory_format=torch.contiguous_format)
+    pos = positions.to(torch.int32)
+    if pos.stride(1) != 1:
+        pos = pos.contiguous()
+    bt = block_table.to(torch.int32)
+    table_stride = cos_table.stride(0) if cos_table.shape[0] > 1 else HEAD_DIM
+    lib = _lib.load()
+    with with_device(qkv.device):
+        err = error_word(qkv.device)
+        st = lib.fi_rope_axes_store(
+            x.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            cos_table.data_ptr(), sin_table.data_ptr(), pos.data_ptr(), cu.data_ptr(),
+            ctx.data_ptr(), bt.data_ptr(), total, batch, num_q_heads, nkv, HEAD_DIM, len(sections),
+            _lib.strides(*sections), pos.stride(0), cos_table.shape[0], table_stride, num_blocks,
+            block_size, bt.shape[1], _lib.strides(*x.stride()), _lib.strides(*q_out.stride()),
+            _lib.strides(*k_cache.stride()), _lib.strides(*v_cache.stride()),
+            _lib.strides(*bt.stride()), _DTYPES[qkv.dtype],
+            err.data_ptr() if err is not None else None, stream_of(qkv.device))
+        _lib.check(st, "rope_axes_store")
+        device_errors(err, "rope_axes_store")
+    return q_out

@@ -17,7 +17,8 @@ What changes is how it runs:
 
 Extension: ``num_blocks`` may be given explicitly to size the pool independently
 of ``max_seq_len`` (the reference pool holds ceil(max_seq_len/block_size) blocks
-shared by the whole batch).
+shared by the whole batch), and ``dtype`` (fp16, or bf16 for the functions that take it).
+``KVCache.extend`` and ``KVCache.evict`` serve ragged batches in chunks over a bounded cache.
 """
 
 from __future__ import annotations
@@ -34,7 +35,9 @@ class KVCache:
 
     def __init__(self, num_layers: int, num_heads: int, head_dim: int,
                  max_seq_len: int, block_size: int, device: torch.device,
-                 num_blocks: int = None):
+                 num_blocks: int = None, dtype: torch.dtype = torch.float16):
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"dtype must be float16 or bfloat16, got {dtype}")
         self.num_layers = num_layers
         self.num_heads = num_heads
         self.head_dim = head_dim
@@ -44,9 +47,9 @@ class KVCache:
         self.max_blocks_per_seq = (max_seq_len + block_size - 1) // block_size
         self.num_blocks = self.max_blocks_per_seq if num_blocks is None else int(num_blocks)
         self.k = torch.zeros(num_layers, self.num_blocks, block_size, num_heads, head_dim,
-                             dtype=torch.float16, device=self.device)
+                             dtype=dtype, device=self.device)
         self.v = torch.zeros(num_layers, self.num_blocks, block_size, num_heads, head_dim,
-                             dtype=torch.float16, device=self.device)
+                             dtype=dtype, device=self.device)
         self._bt = np.full((1, self.max_blocks_per_seq), -1, np.int32)
         self.block_table = torch.full((1, self.max_blocks_per_seq), -1, dtype=torch.int32,
                                       device=self.device)
@@ -131,6 +134,71 @@ class KVCache:
         n = self.seq_lens.shape[0] if batch is None else batch
         return torch.from_numpy(self.seq_lens[:n].astype(np.int32)).to(self.device)
 
+    # ------------------------------------------------ chunks over a bounded cache
+    def extend(self, n_new) -> tuple:
+        """Make room for n_new[b] more tokens of every sequence (one step, all layers): pages are
+        allocated (the reference's first-free-slot / FIFO rule), ``seq_lens`` grows, and
+        (cu_seqlens, context_lens) come back as device int32 tensors, as ``rope_axes_store``,
+        ``paged_chunk_attention`` and ``attention_mass`` take them. Raises before it changes
+        anything if the pool or a sequence's table is too small."""
+        nn = np.asarray(n_new, np.int64).reshape(-1)
+        if (nn < 0).any():
+            raise ValueError("n_new must not be negative")
+        B = nn.shape[0]
+        self._grow_batch(B)
+        need = -(-(self.seq_lens[:B] + nn) // self.block_size)
+        if (need > self.max_blocks_per_seq).any():
+            raise RuntimeError("Sequence block table full")
+        held = (self._bt[:B] >= 0).sum(1)
+        if int(np.maximum(need - held, 0).sum()) > len(self.free_blocks):
+            raise RuntimeError("KV cache out of memory")
+        for b in range(B):
+            self._ensure_blocks(b, int(need[b]))
+        self.seq_lens[:B] += nn
+        self.sync_block_table()
+        cu = np.concatenate([[0], np.cumsum(nn)]).astype(np.int32)
+        return torch.from_numpy(cu).to(self.device), self.context_lens(B)
+
+    def evict(self, mass: torch.Tensor, budget: int, *, recent: int = 0,
+              sinks: int = 0) -> torch.Tensor:
+        """Keep at most ``budget`` tokens per layer, sequence and KV head, by attention weight
+        (``kernels.eviction.evict_tokens`` in place, for the sequences of ``mass``: fp32 [layers,
+        batch, num_heads, capacity]). Pages past the budget go back to the free list,
+        ``seq_lens`` shrinks, and ``mass`` is compacted like the cache (0 past the kept tokens), so
+        that it goes on accumulating. Returns the old slots that stay, [layers, batch, num_heads,
+        budget] int32, -1 past the last. Keys keep the rotary phase of their position; later tokens
+        need positions of their own (``rope_axes_store``), as slots no longer tell them. Distances
+        and windows of ``paged_chunk_attention`` count slots."""
+        from fast_infer_b200.kernels.eviction import evict_tokens
+        if not isinstance(mass, torch.Tensor) or mass.dim() != 4:
+            raise ValueError("mass must be [layers, batch, num_heads, capacity]")
+        B = mass.shape[1]
+        if B > self._bt.shape[0]:
+            raise ValueError("batch larger than the block table")
+        lens = self.seq_lens[:B]
+        if self.num_tokens > 0 and not lens.any():
+            raise ValueError("evict needs per-sequence lengths (extend or store_kv_ragged)")
+        if B > 0 and int(lens.max()) > mass.shape[3]:
+            raise ValueError(f"mass holds {mass.shape[3]} tokens, a sequence has {int(lens.max())}")
+        self.sync_block_table()
+        kept, mass_out = evict_tokens(self.k, self.v, self.block_table, self.context_lens(B), mass,
+                                      budget, recent=recent, sinks=sinks)
+        n = min(kept.shape[3], mass.shape[3])
+        mass[..., :n].copy_(mass_out[..., :n])
+        mass[..., n:].zero_()
+        for b in range(B):
+            self.seq_lens[b] = min(int(lens[b]), kept.shape[3])
+            keep = -(-int(self.seq_lens[b]) // self.block_size)
+            row = self._bt[b]
+            freed = [int(x) for x in row[keep:] if x >= 0]
+            if freed:
+                row[keep:] = -1
+                self.free_blocks.extend(freed)
+                self._allocated -= len(freed)
+                self._dirty = True
+        self.sync_block_table()
+        return kept
+
     # ------------------------------------------------------------ slot writes
     def write_tokens(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor,
                      start_pos, n_new: torch.Tensor = None):
@@ -145,8 +213,8 @@ class KVCache:
         if B > self.block_table.shape[0]:
             raise ValueError("batch larger than the block table; call _grow_batch first")
         for name, t in (("k", k), ("v", v)):
-            if not t.is_cuda or t.dtype != torch.float16 or t.device != self.device:
-                raise ValueError(f"{name} must be float16 on {self.device}")
+            if not t.is_cuda or t.dtype != self.k.dtype or t.device != self.device:
+                raise ValueError(f"{name} must be {str(self.k.dtype)[6:]} on {self.device}")
         if B == 0 or T == 0:
             return
         kc, vc = self.k[layer_idx], self.v[layer_idx]
@@ -264,6 +332,8 @@ def rope_and_store(cache: KVCache, layer_idx: int, qkv: torch.Tensor, num_q_head
     is given, the rotated k is also written there.
     """
     cache.sync_block_table()
+    if cache.k.dtype != torch.float16:
+        raise ValueError("rope_and_store needs a float16 cache")
     if qkv.dim() != 3 or qkv.dtype != torch.float16 or qkv.device != cache.device:
         raise ValueError("qkv must be [batch, seq, heads*head_dim] float16 on the cache device")
     B, S, W = qkv.shape
@@ -331,6 +401,8 @@ def qkv_rope_store(cache: KVCache, layer_idx: int, x: torch.Tensor, w_rope: torc
     D, nkv = cache.head_dim, cache.num_heads
     x2 = x.reshape(-1, x.shape[-1])
     B, K = x2.shape
+    if cache.k.dtype != torch.float16:
+        raise ValueError("qkv_rope_store needs a float16 cache")
     if x2.dtype != torch.float16 or x2.device != cache.device:
         raise ValueError("x must be float16 on the cache device")
     if w_rope.shape != ((num_q_heads + 2 * nkv) * D, K):

@@ -295,6 +295,63 @@ int fi_rope_kv_write(const void* qkv, int64_t batch, int64_t seq, int64_t num_q_
                      void* stream);
 
 /*
+ * Rotary positions with several axes (time, height, width, ...) and the slot write of packed new
+ * tokens whose position is not their slot (after an eviction; images and video). The reference
+ * ties both to one counter (kernels/rope.py:9-44, model.py:67-75,162-201).
+ *
+ * qkv        : [total_tokens, (nq + 2*nkv) * 128], heads in the order q | k | v (2 strides);
+ *              q_out [total_tokens, nq, 128] (3 strides). Rows outside every sequence of
+ *              cu_seqlens (int32 [batch + 1]) are left as they were.
+ * positions  : int32 [axes, total_tokens], positions_stride elements between axes; sections:
+ *              host int64 [axes], frequencies of each axis in order, 64 together (1 to 4 axes).
+ *              Frequency f of axis a uses row positions[a][t] of cos_table / sin_table (fp32
+ *              [table_rows, table_stride >= 128]) at columns f and f + 64. A token with a
+ *              position outside the table is skipped (FI_DEVERR_CONTEXT_LEN).
+ * Rotate-half form in fp32, rounded once. New token i of sequence b (n_b of them) goes to slot
+ * context_lens[b] - n_b + i (context_lens as in fi_paged_chunk); one without a page sets
+ * FI_DEVERR_BAD_BLOCK, and its k and v are not written. dtype: of qkv, q_out and the caches.
+ */
+int fi_rope_axes_store(const void* qkv, void* q_out, void* k_cache, void* v_cache,
+                       const float* cos_table, const float* sin_table, const int32_t* positions,
+                       const int32_t* cu_seqlens, const int32_t* context_lens,
+                       const int32_t* block_table, int64_t total_tokens, int64_t batch,
+                       int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t axes,
+                       const int64_t* sections, int64_t positions_stride, int64_t table_rows,
+                       int64_t table_stride, int64_t num_blocks, int64_t block_size,
+                       int64_t max_blocks_per_seq, const int64_t* qkv_strides,
+                       const int64_t* q_out_strides, const int64_t* kc_strides,
+                       const int64_t* vc_strides, const int64_t* bt_strides, int64_t dtype,
+                       int32_t* error_flag, void* stream);
+
+/*
+ * Eviction from the paged cache by accumulated attention weight (no counterpart in the
+ * reference). For every (layer, sequence, KV head) with n = seq_lens[b] > budget tokens keep the
+ * first `sinks`, the last `recent` and, of those between, the ones of greatest mass, `budget` in
+ * all (ties: lowest index; negative and NaN count as 0); n <= budget keeps all. What stays keeps
+ * its order and goes to slots 0 .. min(n, budget) - 1.
+ *
+ * k, v      : [layers, num_blocks, block_size=64, num_heads, 128], 16-bit values (5 strides each);
+ *             block_table [batch, max_blocks_per_seq]; seq_lens int32 [batch].
+ * mass      : fp32 [layers, batch, num_heads, mass_capacity], dense.
+ * k_out, v_out, block_table_out: k, v and block_table themselves (in place; pages shared between
+ *             sequences are not allowed), or another pool and table, whose pages the source's do
+ *             not overlap.
+ * kept, mass_out: int32 and fp32 [layers, batch, num_heads, budget], dense: the old slots that
+ *             stay, ascending (-1 past the last), and their mass (0 past the last).
+ * A token whose page is missing in either table is not moved (FI_DEVERR_BAD_BLOCK); lengths past
+ * the table or mass_capacity are cut (FI_DEVERR_CONTEXT_LEN).
+ */
+int fi_kv_evict(const void* k, const void* v, const int32_t* block_table, const int32_t* seq_lens,
+                const float* mass, void* k_out, void* v_out, const int32_t* block_table_out,
+                int32_t* kept, float* mass_out, int64_t layers, int64_t batch, int64_t num_heads,
+                int64_t head_dim, int64_t num_blocks, int64_t num_blocks_out, int64_t block_size,
+                int64_t max_blocks_per_seq, int64_t max_blocks_per_seq_out,
+                int64_t mass_capacity, int64_t budget, int64_t recent, int64_t sinks,
+                const int64_t* k_strides, const int64_t* v_strides, const int64_t* ko_strides,
+                const int64_t* vo_strides, const int64_t* bt_strides, const int64_t* bto_strides,
+                int32_t* error_flag, void* stream);
+
+/*
  * RMSNorm: out[r, :] = x[r, :] * rsqrt(mean(x[r, :]^2) + eps) * weight, fp16 in/out,
  * fp32 arithmetic. x, out: [rows, hidden] with row strides (elements, multiples of 8;
  * unit inner stride); weight: [hidden]. hidden a multiple of 8; 16-byte aligned bases.

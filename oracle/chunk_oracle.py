@@ -82,3 +82,27 @@ def mass(q, k_cache, table, cu, ctx, lse, *, scale=128 ** -0.5, softcap=0.0, slo
             w[s == -math.inf] = 0.0
             out[b, kh, :keys] += w.sum(0)
     return out
+
+
+def evict_keep(weights, budget, recent, sinks):
+    """Old slots that stay of one head's weights (a list of Python floats), ascending."""
+    n = len(weights)
+    if n <= budget:
+        return list(range(n))
+    key = [w if w > 0 else 0.0 for w in weights]  # NaN > 0 is false
+    middle = sorted(range(sinks, n - recent), key=lambda j: (-key[j], j))
+    return sorted(list(range(sinks)) + middle[:budget - sinks - recent] + list(range(n - recent, n)))
+
+
+def rope_axes(x, positions, sections, cos, sin):
+    """Rotate-half RoPE of x [T, H, 128] in float64; frequency f uses its axis's position."""
+    out = torch.empty(x.shape, dtype=torch.float64)
+    f0 = 0
+    for axis, count in enumerate(sections):
+        for f in range(f0, f0 + count):
+            p = positions[axis].long()
+            lo, hi = x[:, :, f].double(), x[:, :, f + 64].double()
+            out[:, :, f] = lo * cos[p, f, None].double() - hi * sin[p, f, None].double()
+            out[:, :, f + 64] = hi * cos[p, f + 64, None].double() + lo * sin[p, f + 64, None].double()
+        f0 += count
+    return out
