@@ -149,6 +149,7 @@ __device__ __forceinline__ void block_scan(U* a, int n, U* warp_sums) {
   const int each = (n + threads - 1) / threads;
   const int lo = 1 + min(tid * each, n), hi = 1 + min(tid * each + each, n);
   U sum = 0;
+#pragma unroll 1
   for (int i = lo; i < hi; ++i) sum += a[i];
   U inc = sum;
 #pragma unroll
@@ -159,7 +160,9 @@ __device__ __forceinline__ void block_scan(U* a, int n, U* warp_sums) {
   if (lane == 31) warp_sums[warp] = inc;
   __syncthreads();
   U run = inc - sum;
+#pragma unroll 1
   for (int w = 0; w < warp; ++w) run += warp_sums[w];
+#pragma unroll 1
   for (int i = lo; i < hi; ++i) {
     run += a[i];
     a[i] = run;
@@ -171,6 +174,7 @@ __device__ __forceinline__ void block_scan(U* a, int n, U* warp_sums) {
 template <typename U>
 __device__ __forceinline__ int last_le(const U* a, int n, U x) {
   int lo = 0, hi = n;
+#pragma unroll 1
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (a[mid] <= x) lo = mid; else hi = mid;

@@ -17,6 +17,12 @@
 // * Roles (384 threads), tensor memory (S0 | S1 | O0 | O1), the lazily rescaled online
 //   softmax and the MMA order are those of the causal prefill kernel (prefill_sm100.cu). K
 //   and V tiles are two pages each, gathered by TMA through the block table.
+// * A unit of at most 32 rows (single tokens, drafted tokens) runs transposed: S^T = K Q^T with
+//   the 128 keys of a tile as tensor-memory lanes and N = its rows, then O^T += V^T P^T with P
+//   through shared memory, so no lane idles and a tile costs a softmax thread its rows, not 128
+//   columns: the unit streams K and V at HBM's rate. The warpgroups take alternate key tiles as
+//   two running softmaxes and merge them at the end. A row's max moves only when some score
+//   passes it by 2^8, found by one vote per tile.
 // * Slots behind a sequence's last token may hold anything: their scores are replaced by
 //   -inf, and their V rows are zeroed in shared memory before the product (0 * NaN is NaN).
 #include "chunk_common.cuh"
@@ -29,9 +35,25 @@ constexpr int kCkRegsOther = 136;
 constexpr int kCkStages = 2;
 constexpr int kCkTeardownBar = 15;
 constexpr int kCkMaxBatch = 2048;    // sequences per launch
-constexpr int kCkMaxUnits = 6000;    // token units per launch (per KV head)
+constexpr int kCkMaxUnits = 4608;    // token units per launch (per KV head)
+constexpr int kCkNarrow = 32;        // rows up to which a unit runs transposed
 constexpr float kCkRescale = 8.0f;   // log2 units of growth of the max before O is rescaled
 constexpr int kCkEmuPairs = 2;       // of 8 column pairs, exp2 on the FMA pipe
+constexpr int kCkSlots = 4;          // units that the scheduler is ahead
+
+// A CTA's part of a unit: key steps [j0, j1) of its n.
+struct alignas(16) CkUnit {
+  int b, hk;
+  int token, pos;      // first packed row, its position
+  int rows[2];         // live rows of the two tiles
+  int keys, prefix;
+  int np, lo;          // step j is key tile j < np ? j : lo + j - np
+  int j0, j1, n;
+  int narrow;          // runs transposed
+  int last_cta;        // the CTA with the unit's last step
+  int valid;           // 0: no unit is left
+};
+static_assert(sizeof(CkUnit) == 64, "read as four 16-byte words");
 
 struct CkBarriers {
   uint64_t q_full[2], q_empty[2];
@@ -39,7 +61,14 @@ struct CkBarriers {
   uint64_t v_full[kCkStages], v_empty[kCkStages];
   uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
   uint64_t mma_done;
+  uint64_t unit_full[kCkSlots], unit_empty[kCkSlots];
+  uint64_t merge;  // both softmax warpgroups, in a transposed unit
   uint32_t tmem_base;
+  // transposed units, per warpgroup: rows' max, partial maxima / sums, scale, slope, position
+  float n_max[2][kCkNarrow], n_red[2][4][kCkNarrow], n_alpha[2][kCkNarrow];
+  float n_slope[2][kCkNarrow], n_pos[2][kCkNarrow];
+  int64_t n_off[kCkNarrow];  // where a row's output goes
+  CkUnit units[kCkSlots];
   uint32_t warp_sums[kCkThreads / 32];
   uint32_t unit_off[kCkMaxBatch + 1];  // first unit of each sequence
   uint32_t work[kCkMaxUnits + 1];      // key tiles before each unit
@@ -52,6 +81,10 @@ struct CkJoin {
   int valid, last_cta, token, hk, rows[2], pad[2];
 };
 
+constexpr int kCkPBytes = kCkNarrow * 256;  // P^T of a transposed unit: 32 rows x 128 keys
+static_assert(kCkNarrow == 32, "a column per lane where rows are summed");
+static_assert(2 * kCkPBytes <= kChunkTileBytes, "P of both warpgroups in one query tile");
+
 struct ChunkParams {
   ChunkBatch b;
   ScoreForm f;
@@ -63,16 +96,6 @@ struct ChunkParams {
   CkJoin* join;   // [cta]
   int rows_cap;
   int* err;
-};
-
-// A CTA's part of a unit: key steps [j0, j1) of its n.
-struct CkUnit {
-  int b, hk;
-  int token, pos;      // first packed row, its position
-  int rows[2];         // live rows of the two tiles
-  int keys, prefix;
-  int np, lo;          // step j is key tile j < np ? j : lo + j - np
-  int j0, j1, n;
 };
 
 __device__ __forceinline__ int ck_tile(const CkUnit& u, int j) {
@@ -91,32 +114,83 @@ __device__ __forceinline__ void ck_tiles(const ChunkBatch& p, const ChunkSeq& s,
   n = np + hi - lo + 1;
 }
 
-// The CTA's next unit: step w of the line, at most up to `end`.
-__device__ __forceinline__ CkUnit ck_unit(const ChunkBatch& p, const CkBarriers* s, uint32_t units,
-                                          int64_t w, int64_t end) {
-  CkUnit u;
+// The scheduler (one thread): walks the CTA's part of the line and hands its units to the other
+// roles through a ring in shared memory.
+__device__ __forceinline__ void ck_schedule(const ChunkBatch& p, CkBarriers* s, uint32_t units,
+                                            int* err) {
+  const int G = gridDim.x, cta = blockIdx.x;
   const uint32_t per_head = s->work[units];
-  u.hk = (int)(w / per_head);
-  const uint32_t r = (uint32_t)(w - (int64_t)u.hk * per_head);
-  const int e = last_le(s->work, (int)units, r);
-  u.b = last_le(s->unit_off, p.batch, (uint32_t)e);
-  const ChunkSeq q = chunk_seq(p, u.b);
+  const int64_t total = (int64_t)per_head * p.hk;
+  const int active = (int)(total < G ? total : G);  // CTAs with work
+  int64_t w = cta < active ? total * cta / active : 0;
+  const int64_t end = cta < active ? total * (cta + 1) / active : 0;
+  int hk = 0, e = 0, b = 0, j0 = 0;
+  if (w < end) {
+    hk = (int)(w / per_head);
+    const uint32_t r = (uint32_t)(w - (int64_t)hk * per_head);
+    e = last_le(s->work, (int)units, r);
+    b = last_le(s->unit_off, p.batch, (uint32_t)e);
+    j0 = (int)(r - s->work[e]);
+  }
+  ChunkSeq q = chunk_seq(p, b);
   const int tt = p.tile_tokens;
-  const int t0 = (e - (int)s->unit_off[u.b]) * 2 * tt, t1 = min(t0 + 2 * tt, q.n);
-  ck_tiles(p, q, t0, t1, u.np, u.lo, u.n);
-  u.token = q.start + t0;
-  u.pos = q.pos0 + t0;
-  u.keys = q.keys;
-  u.prefix = q.prefix;
-  u.rows[0] = min(t1 - t0, tt) * p.group;
-  u.rows[1] = max(t1 - t0 - tt, 0) * p.group;
-  u.j0 = (int)(r - s->work[e]);
-  u.j1 = (int)(u.n - u.j0 <= end - w ? u.n : u.j0 + (end - w));
-  return u;
+#pragma unroll 1
+  for (int i = 0;; ++i) {
+    const int slot = i % kCkSlots;
+    if (i >= kCkSlots && !mbar_wait(&s->unit_empty[slot], ((i / kCkSlots) - 1) & 1, err)) return;
+    CkUnit u;
+    u.valid = w < end;
+    if (u.valid) {
+      const int t0 = (e - (int)s->unit_off[b]) * 2 * tt, t1 = min(t0 + 2 * tt, q.n);
+      ck_tiles(p, q, t0, t1, u.np, u.lo, u.n);
+      u.b = b;
+      u.hk = hk;
+      u.token = q.start + t0;
+      u.pos = q.pos0 + t0;
+      u.keys = q.keys;
+      u.prefix = q.prefix;
+      u.rows[0] = min(t1 - t0, tt) * p.group;
+      u.rows[1] = max(t1 - t0 - tt, 0) * p.group;
+      u.narrow = u.rows[1] == 0 && u.rows[0] <= kCkNarrow;
+      u.j0 = j0;
+      u.j1 = (int)(u.n - j0 <= end - w ? u.n : j0 + (end - w));
+      // the last step of the unit, w - j0 + n - 1, belongs to the last CTA that starts at or before it
+      u.last_cta = u.j1 == u.n ? cta : (int)(((w - j0 + u.n) * active - 1) / total);
+      w += u.j1 - u.j0;
+      j0 = 0;
+      if (++e == (int)units) {
+        e = 0;
+        ++hk;
+      }
+      if (w < end && (e < (int)s->unit_off[b] || e >= (int)s->unit_off[b + 1])) {
+        if (e == 0) b = -1;
+        do ++b; while ((int)s->unit_off[b + 1] <= e);
+        q = chunk_seq(p, b);
+      }
+    }
+    s->units[slot] = u;
+    mbar_arrive(&s->unit_full[slot]);  // released to the waits that read it
+    if (!u.valid) return;
+  }
 }
 
-// Scores of one row in log2 units, in place: the cap and the distance bias. `off` = position
-// of column 0's key minus the row's position.
+// The next unit from the ring (a whole warp, or one thread with kWarp = false).
+template <bool kWarp>
+__device__ __forceinline__ bool ck_next(CkBarriers* s, int& i, CkUnit& u, int* err) {
+  const int slot = i % kCkSlots;
+  bool ok = mbar_wait(&s->unit_full[slot], (i / kCkSlots) & 1, err);
+  if (kWarp) ok = __all_sync(0xffffffffu, ok);
+  if (!ok) return false;
+  u = s->units[slot];
+  if (kWarp) __syncwarp();
+  if (!kWarp || (threadIdx.x & 31) == 0) mbar_arrive(&s->unit_empty[slot]);
+  ++i;
+  return u.valid;
+}
+
+// 32 scores of one row in log2 units, in place: the cap and the distance bias (without either,
+// they stay unscaled). `off` = position of the first column's key minus the row's position; a row
+// that is not `live` has no say in which form of tanh runs.
 template <bool kCap, bool kAlibi>
 __device__ __forceinline__ void score_form(uint32_t* sr, const ScoreForm& f, float slope2,
                                            float off, bool live) {
@@ -124,36 +198,29 @@ __device__ __forceinline__ void score_form(uint32_t* sr, const ScoreForm& f, flo
     const uint64_t cin = f32x2(f.cap_in, f.cap_in), cout = f32x2(f.cap_log2, f.cap_log2);
     float big = 0.f;
 #pragma unroll
-    for (int c = 0; c < kChunkTile; c += 2)
+    for (int c = 0; c < 32; c += 2)
       big = fmax3f(big, fabsf(__uint_as_float(sr[c])), fabsf(__uint_as_float(sr[c + 1])));
-    if (__all_sync(0xffffffffu, !live || big * f.cap_in <= 1.f)) {
+    const bool small = __all_sync(0xffffffffu, !live || big * f.cap_in <= 1.f);
 #pragma unroll
-      for (int c = 0; c < kChunkTile; c += 2) {
-        const uint64_t u = mul_f32x2(
-            f32x2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), cin);
-        float a, b;
-        f32x2_split(mul_f32x2(tanh_poly_x2(u), cout), a, b);
-        sr[c] = __float_as_uint(a);
-        sr[c + 1] = __float_as_uint(b);
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < kChunkTile; c += 2) {
-        const uint64_t u = mul_f32x2(
-            f32x2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), cin);
-        float u0, u1, a, b;
+    for (int c = 0; c < 32; c += 2) {
+      const uint64_t u =
+          mul_f32x2(f32x2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), cin);
+      uint64_t y = tanh_poly_x2(u);
+      if (!small) {
+        float u0, u1, y0, y1;
         f32x2_split(u, u0, u1);
-        f32x2_split(tanh_poly_x2(u), a, b);
-        a = fabsf(u0) <= 1.f ? a : tanh_any(u0);
-        b = fabsf(u1) <= 1.f ? b : tanh_any(u1);
-        sr[c] = __float_as_uint(a * f.cap_log2);
-        sr[c + 1] = __float_as_uint(b * f.cap_log2);
+        f32x2_split(y, y0, y1);
+        y = f32x2(fabsf(u0) <= 1.f ? y0 : tanh_any(u0), fabsf(u1) <= 1.f ? y1 : tanh_any(u1));
       }
+      float a, b;
+      f32x2_split(mul_f32x2(y, cout), a, b);
+      sr[c] = __float_as_uint(a);
+      sr[c + 1] = __float_as_uint(b);
     }
   }
   if constexpr (kAlibi) {
 #pragma unroll
-    for (int c = 0; c < kChunkTile; ++c) {
+    for (int c = 0; c < 32; ++c) {
       const float s = __uint_as_float(sr[c]);
       const float d = fabsf(off + (float)c) * slope2;
       sr[c] = __float_as_uint(kCap ? s - d : fmaf(s, f.scale_log2, -d));
@@ -161,8 +228,8 @@ __device__ __forceinline__ void score_form(uint32_t* sr, const ScoreForm& f, flo
   }
 }
 
-// p = 2^(s * sl2 - mref) of a row, its sum, and p packed in place (see softmax_pass of the
-// prefill kernel: 2 of 8 pairs take exp2 on the FMA pipe).
+// p = 2^(s * sl2 - mref) of a row, its sum, and p packed in place. 2 of 8 pairs take exp2 on the
+// FMA pipe, to 2.2e-7: lse is an output, which a rougher polynomial would show in.
 template <typename T>
 __device__ __forceinline__ float ck_exp(uint32_t* sr, float sl2, float mref) {
   const uint64_t sc2 = f32x2(sl2, sl2), nm2 = f32x2(-mref, -mref);
@@ -173,7 +240,7 @@ __device__ __forceinline__ float ck_exp(uint32_t* sr, float sl2, float mref) {
         fma_f32x2(f32x2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), sc2, nm2);
     float p0, p1;
     if (((c >> 1) & 7) < kCkEmuPairs) {
-      exp2_poly_x2(xp, p0, p1);
+      f32x2_split(exp2_poly5_x2(xp), p0, p1);
     } else {
       float x0, x1;
       f32x2_split(xp, x0, x1);
@@ -191,10 +258,259 @@ __device__ __forceinline__ float ck_exp(uint32_t* sr, float sl2, float mref) {
 // Zero rows [from, 128) of a V tile (both 64-value columns) with one warpgroup.
 __device__ __forceinline__ void zero_v_rows(uint8_t* v, int from, int tid) {
   const int chunks = (kChunkTile - from) * 8;
+#pragma unroll 1
   for (int i = tid; i < 2 * chunks; i += 128) {
     const int half = i >= chunks, k = half ? i - chunks : i;
     *reinterpret_cast<uint4*>(v + half * kChunkHalf + from * 128 + k * 16) = make_uint4(0, 0, 0, 0);
   }
+}
+
+// Ordered like the float it comes from (no NaN), as a signed integer.
+__device__ __forceinline__ int float_order(float x) {
+  const int i = __float_as_int(x);
+  return i ^ ((i >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float order_float(int i) {
+  return __int_as_float(i ^ ((i >> 31) & 0x7fffffff));
+}
+
+// A transposed unit, softmax side: warpgroup t takes key tiles j0 + t, j0 + t + 2, ... A thread is
+// one key of the tile (and, for O^T, one dim). `ok` turns false when a wait runs out; a warp that
+// saw it goes on without waiting, so that every barrier here gets all of its threads.
+template <typename T, bool kCap, bool kAlibi>
+__device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* bars, const CkUnit& u,
+                                            uint8_t* sP, uint8_t* sV, uint32_t tmem, int t,
+                                            int quarter, int lane, int q1, int& sc, int& g,
+                                            int& uc, int& merges, int cta, bool& ok) {
+  const ChunkBatch& pb = p.b;
+  const int rows = u.rows[0], n = u.j1 - u.j0, tid = quarter * 32 + lane;
+  const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+  const uint32_t tS = tmem + lane_off + t * 128, tO = tmem + lane_off + 256;
+  const bool mine = t < n;  // this warpgroup has a key tile
+  const float sl2 = p.f.scale_log2;
+  float l[kCkNarrow];
+#pragma unroll
+  for (int c = 0; c < kCkNarrow; ++c) l[c] = 0.f;
+  float* n_max = bars->n_max[t];
+  if (tid < kCkNarrow) {
+    n_max[tid] = -INFINITY;
+    if (kAlibi) {
+      const bool live = tid < rows;
+      bars->n_slope[t][tid] = live ? p.f.slopes[u.hk * pb.group + tid % pb.group] * kLog2e : 0.f;
+      bars->n_pos[t][tid] = (float)(u.pos + tid / pb.group);
+    }
+  }
+  named_bar_sync(1 + t, 128);
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.err));
+  };
+  auto meet = [&]() {  // both warpgroups
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars->merge);
+    wait(&bars->merge, merges++ & 1);
+  };
+  if (mine) wait(&bars->q_full[1], q1 & 1);
+  // P^T is [rows][128 keys], K-major with the 128-byte swizzle: this thread's column of it
+  uint8_t* pcol = sP + t * kCkPBytes + (tid >> 6) * (kCkPBytes / 2);
+  const uint32_t kbyte = (uint32_t)(tid & 63) * 2;
+#pragma unroll 1
+  for (int j = t; j < n; j += 2, ++sc) {
+    const int tile = ck_tile(u, u.j0 + j), k0 = tile * kChunkTile, key = k0 + tid;
+    const int stage = (g + j) % kCkStages;
+    const bool page_ok = chunk_page(pb, u.b, u.keys, tile, tid >> 6) != pb.num_blocks;
+    wait(&bars->s_full[t], sc & 1);
+    if (k0 + kChunkTile > u.keys) {
+      wait(&bars->v_full[stage], ((g + j) / kCkStages) & 1);
+      zero_v_rows(sV + stage * kChunkTileBytes, max(u.keys - k0, 0), tid);
+    }
+    tc_fence_after();
+    // columns [c_lo, c_hi) see this key
+    int c_lo = 0, c_hi = rows;
+    if (key >= u.prefix) {
+      c_lo = min(max(key - u.pos, 0), kCkNarrow) * pb.group;
+      if (pb.window) c_hi = min(rows, min(max(key + pb.window - u.pos, 0), kCkNarrow) * pb.group);
+    }
+    if (!page_ok || key >= u.keys) c_hi = 0;
+    uint32_t s[kCkNarrow];
+    bool past = false;
+#pragma unroll
+    for (int cc = 0; cc < kCkNarrow; cc += 16) {
+      if (cc < rows) {
+        tmem_ld16(tS + cc, s + cc);
+        tmem_wait_ld();
+        reg_fence<16>(s + cc);
+        const uint32_t vis = (low_bits(c_hi - cc, 0) & ~low_bits(c_lo - cc, 0));
+        bool small = true;
+        if constexpr (kCap) {
+          float big = 0.f;
+#pragma unroll
+          for (int c = cc; c < cc + 16; ++c)
+            big = fmaxf(big, (vis >> (c - cc)) & 1u ? fabsf(__uint_as_float(s[c])) : 0.f);
+          small = __all_sync(0xffffffffu, big * p.f.cap_in <= 1.f);
+        }
+#pragma unroll
+        for (int c = cc; c < cc + 16; c += 2) {
+          float x0 = __uint_as_float(s[c]), x1 = __uint_as_float(s[c + 1]);
+          if constexpr (kCap) {
+            const uint64_t v = mul_f32x2(f32x2(x0, x1), f32x2(p.f.cap_in, p.f.cap_in));
+            uint64_t y = tanh_poly_x2(v);
+            if (!small) {
+              float v0, v1, y0, y1;
+              f32x2_split(v, v0, v1);
+              f32x2_split(y, y0, y1);
+              y = f32x2(fabsf(v0) <= 1.f ? y0 : tanh_any(v0), fabsf(v1) <= 1.f ? y1 : tanh_any(v1));
+            }
+            f32x2_split(mul_f32x2(y, f32x2(p.f.cap_log2, p.f.cap_log2)), x0, x1);
+          } else {
+            x0 *= sl2;
+            x1 *= sl2;
+          }
+          if constexpr (kAlibi) {
+            x0 -= bars->n_slope[t][c] * fabsf(bars->n_pos[t][c] - (float)key);
+            x1 -= bars->n_slope[t][c + 1] * fabsf(bars->n_pos[t][c + 1] - (float)key);
+          }
+          if (!((vis >> (c - cc)) & 1u)) x0 = -INFINITY;
+          if (!((vis >> (c + 1 - cc)) & 1u)) x1 = -INFINITY;
+          past |= x0 > n_max[c] + kCkRescale;
+          past |= x1 > n_max[c + 1] + kCkRescale;
+          s[c] = __float_as_uint(x0);
+          s[c + 1] = __float_as_uint(x1);
+        }
+      }
+    }
+    if (!wg_bar_and(1 + t, !past)) {
+      // some row's max moves: all rows go to their running maximum
+#pragma unroll
+      for (int cc = 0; cc < kCkNarrow; cc += 16)
+        if (cc < rows) {
+#pragma unroll
+          for (int c = cc; c < cc + 16; ++c) {
+            const int mx = __reduce_max_sync(0xffffffffu, float_order(__uint_as_float(s[c])));
+            if (lane == 0) bars->n_red[t][quarter][c] = order_float(mx);
+          }
+        }
+      named_bar_sync(1 + t, 128);
+      if (tid < kCkNarrow) {
+        const float was = n_max[tid];  // a column without a row stays at -inf
+
+        const float now = fmaxf(fmaxf(was, fmaxf(bars->n_red[t][0][tid], bars->n_red[t][1][tid])),
+                                fmaxf(bars->n_red[t][2][tid], bars->n_red[t][3][tid]));
+        bars->n_alpha[t][tid] = was == -INFINITY ? 0.f : fast_exp2(was - now);
+        n_max[tid] = now;
+      }
+      named_bar_sync(1 + t, 128);
+      if (j >= 2) {
+        // the product of this warpgroup's last tile is complete: S here was committed after it
+#pragma unroll
+        for (int cc = 0; cc < kCkNarrow; cc += 16)
+          if (cc < rows) {
+            uint32_t ov[16];
+            tmem_ld16(tO + t * 128 + cc, ov);
+            tmem_wait_ld();
+            reg_fence<16>(ov);
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              const float a = bars->n_alpha[t][cc + c];
+              ov[c] = __float_as_uint(__uint_as_float(ov[c]) * a);
+              l[cc + c] *= a;
+            }
+            tmem_st16(tO + t * 128 + cc, ov);
+          }
+        tmem_wait_st();
+      }
+    }
+#pragma unroll
+    for (int cc = 0; cc < kCkNarrow; cc += 16)
+      if (cc < rows) {
+#pragma unroll
+        for (int c = cc; c < cc + 16; c += 2) {
+          const float m0 = n_max[c], m1 = n_max[c + 1];
+          const float p0 = fast_exp2(__uint_as_float(s[c]) - (m0 == -INFINITY ? 0.f : m0));
+          const float p1 = fast_exp2(__uint_as_float(s[c + 1]) - (m1 == -INFINITY ? 0.f : m1));
+          l[c] += p0;
+          l[c + 1] += p1;
+          const uint32_t pk = Half16<T>::pack(p0, p1);
+          *reinterpret_cast<uint16_t*>(pcol + c * 128 + (kbyte ^ ((c & 7) << 4))) = (uint16_t)pk;
+          *reinterpret_cast<uint16_t*>(pcol + (c + 1) * 128 + (kbyte ^ (((c + 1) & 7) << 4))) =
+              (uint16_t)(pk >> 16);
+        }
+      }
+    fence_proxy_async_smem();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars->p_full[t]);
+  }
+  if (mine) wait(&bars->o_full[t], uc & 1);
+  // sums over the lanes: halves of the columns trade places until lane i has column i
+#pragma unroll
+  for (int half = kCkNarrow / 2; half > 0; half >>= 1) {
+#pragma unroll
+    for (int c = 0; c < half; ++c) {
+      const bool up = lane & half;
+      const float give = up ? l[c] : l[c + half], keep = up ? l[c + half] : l[c];
+      l[c] = keep + __shfl_xor_sync(0xffffffffu, give, half);
+    }
+  }
+  bars->n_red[t][quarter][lane] = l[0];
+  tc_fence_before();
+  meet();
+  tc_fence_after();
+  const bool whole = u.j0 == 0 && u.j1 == u.n;
+  if (t == 0 && tid < rows) {
+    const float m0 = bars->n_max[0][tid], m1 = bars->n_max[1][tid], mx = fmaxf(m0, m1);
+    float l0 = 0.f, l1 = 0.f;
+    for (int i = 0; i < 4; ++i) {
+      l0 += bars->n_red[0][i][tid];
+      l1 += bars->n_red[1][i][tid];
+    }
+    const float w0 = m0 == -INFINITY ? 0.f : exp2f(m0 - mx), w1 = m1 == -INFINITY ? 0.f : exp2f(m1 - mx);
+    const float sum = w0 * l0 + w1 * l1;
+    const bool none = mx == -INFINITY;
+    bars->n_alpha[0][tid] = none ? 0.f : w0 / sum;
+    bars->n_alpha[1][tid] = none ? 0.f : w1 / sum;
+    const float lse2 = none ? -INFINITY : mx + log2f(sum);
+    const int64_t token = u.token + tid / pb.group;
+    const int head = u.hk * pb.group + tid % pb.group;
+    if (whole) {
+      bars->n_off[tid] = token * p.os[0] + head * p.os[1];
+      if (p.lse) p.lse[token * pb.hq + head] = lse2 * kLn2;
+    } else {
+      const int64_t part = (int64_t)(cta * 2 + (u.j0 == 0 ? 1 : 0)) * p.rows_cap + tid;
+      bars->n_off[tid] = part * 128;
+      p.ws_lse[part] = lse2;
+    }
+  }
+  meet();
+#pragma unroll 1
+  for (int cc = t * 16; cc < rows; cc += 32) {
+    uint32_t a0[16], a1[16];
+    tmem_ld16(tO + cc, a0);
+    if (n > 1) tmem_ld16(tO + 128 + cc, a1);
+    tmem_wait_ld();
+    reg_fence<16>(a0);
+    if (n > 1) reg_fence<16>(a1);
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+      const int r = cc + c;
+      if (r < rows) {
+        const float f0 = bars->n_alpha[0][r], f1 = bars->n_alpha[1][r];
+        // a factor of 0 is no tile or nothing seen: the accumulator does not count
+        float v = f0 != 0.f ? f0 * __uint_as_float(a0[c]) : 0.f;
+        if (n > 1 && f1 != 0.f) v = fmaf(f1, __uint_as_float(a1[c]), v);
+        if (whole)
+          static_cast<uint16_t*>(p.o)[bars->n_off[r] + tid] = (uint16_t)Half16<T>::pack(v, 0.f);
+        else
+          p.ws_o[bars->n_off[r] + tid] = v;
+      }
+    }
+  }
+  tc_fence_before();
+  meet();
+  if (mine) {
+    if (lane == 0) mbar_arrive(&bars->o_empty[t]);
+    ++uc;
+  }
+  g += n;
 }
 
 template <typename T, bool kCap, bool kAlibi>
@@ -210,7 +526,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
   CkBarriers* bars = reinterpret_cast<CkBarriers*>(sV + kCkStages * kChunkTileBytes);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int G = gridDim.x, cta = blockIdx.x;
+  const int cta = blockIdx.x;
 
   if (warp == 0) {
     tmem_alloc(&bars->tmem_base, 512);
@@ -232,6 +548,11 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       mbar_init(&bars->v_empty[s], 1);
     }
     mbar_init(&bars->mma_done, 1);
+    mbar_init(&bars->merge, 8);
+    for (int s = 0; s < kCkSlots; ++s) {
+      mbar_init(&bars->unit_full[s], 1);
+      mbar_init(&bars->unit_empty[s], 10);  // TMA, UMMA, the 8 softmax warps
+    }
     fence_barrier_init();
   }
 
@@ -240,6 +561,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
   grid_dep_launch();
   const ChunkBatch& pb = p.b;
   if (threadIdx.x == 0) bars->unit_off[0] = bars->work[0] = 0;
+#pragma unroll 1
   for (int b = threadIdx.x; b < pb.batch; b += kCkThreads) {
     const ChunkSeq q = chunk_seq(pb, b);
     bars->unit_off[b + 1] = (uint32_t)((q.n + 2 * pb.tile_tokens - 1) / (2 * pb.tile_tokens));
@@ -251,6 +573,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
   const uint32_t units = min(bars->unit_off[pb.batch], (uint32_t)kCkMaxUnits);
   if (units != bars->unit_off[pb.batch] && threadIdx.x == 0)
     set_error(p.err, FI_DEVERR_CONTEXT_LEN);
+#pragma unroll 1
   for (int e = threadIdx.x; e < (int)units; e += kCkThreads) {
     const int b = last_le(bars->unit_off, pb.batch, (uint32_t)e);
     const ChunkSeq q = chunk_seq(pb, b);
@@ -261,11 +584,6 @@ __global__ void __launch_bounds__(kCkThreads, 1)
   }
   __syncthreads();
   block_scan(bars->work, (int)units, bars->warp_sums);
-  const int64_t total = (int64_t)bars->work[units] * pb.hk;
-  const int active = (int)(total < G ? total : G);  // CTAs with work
-  const int64_t w_begin = cta < active ? total * cta / active : 0;
-  const int64_t w_end = cta < active ? total * (cta + 1) / active : 0;
-
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -280,16 +598,22 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       prefetch_tmap(&tm_v);
       const uint32_t q_bytes = (uint32_t)(pb.group * pb.tile_tokens * 256);
       int qc[2] = {0, 0};
-      int g = 0;
+      int g = 0, next_unit = 0;
       bool ok = true;
-      for (int64_t w = w_begin; ok && w < w_end;) {
-        const CkUnit u = ck_unit(pb, bars, units, w, w_end);
-        w += u.j1 - u.j0;
+      CkUnit u;
+#pragma unroll 1
+      while (ok && ck_next<false>(bars, next_unit, u, p.err)) {
         auto load_q = [&]() {
-          for (int t = 0; t < 2 && ok; ++t) {
-            if (u.rows[t] == 0) continue;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (!ok || (u.rows[t] == 0 && !u.narrow)) continue;
             if (qc[t] > 0) ok = mbar_wait(&bars->q_empty[t], (qc[t] - 1) & 1, p.err);
-            if (!ok) break;
+            if (!ok) continue;
+            if (t == 1 && u.narrow) {  // the tile's memory holds P of a transposed unit
+              mbar_arrive(&bars->q_full[1]);
+              ++qc[1];
+              continue;
+            }
             const int token = u.token + t * pb.tile_tokens;
             uint8_t* dst = sQ + t * kChunkTileBytes;
             mbar_arrive_expect_tx(&bars->q_full[t], q_bytes);
@@ -300,6 +624,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
         };
         int ph[2];
         for (int i = 0; i < 2; ++i) ph[i] = chunk_page(pb, u.b, u.keys, ck_tile(u, u.j0), i);
+#pragma unroll 1
         for (int j = u.j0; ok && j < u.j1; ++j, ++g) {
           const int s = g % kCkStages;
           const uint32_t par = ((g / kCkStages) - 1) & 1;
@@ -331,12 +656,15 @@ __global__ void __launch_bounds__(kCkThreads, 1)
           ph[1] = next[1];
         }
       }
+    } else if (warp == 10 && lane == 0) {
+      ck_schedule(pb, bars, units, p.err);
     } else if (warp == 9 && lane == 0) {
       // ---------------------------------------------------------- UMMA issuer
       constexpr uint32_t idesc_qk = umma_idesc<T>(128, 128, 0, 0);
       constexpr uint32_t idesc_pv = umma_idesc<T>(128, 128, 0, 1);
       const uint32_t q_addr = smem_u32(sQ), k_addr = smem_u32(sK), v_addr = smem_u32(sV);
-      int qc[2] = {0, 0};  // units seen per tile
+      int qc[2] = {0, 0};  // uses of a query tile
+      int oc[2] = {0, 0};  // uses of an O accumulator
       int sc[2] = {0, 0};  // S tiles issued per tile
       int g = 0;
       bool ok = true;
@@ -357,21 +685,81 @@ __global__ void __launch_bounds__(kCkThreads, 1)
           umma_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, db + (uint32_t)(kk * 128),
                   idesc_pv, (!first || kk > 0) ? 1u : 0u);
       };
-      for (int64_t w = w_begin; ok && w < w_end;) {
-        const CkUnit u = ck_unit(pb, bars, units, w, w_end);
-        w += u.j1 - u.j0;
+      int next_unit = 0;
+      CkUnit u;
+#pragma unroll 1
+      while (ok && ck_next<false>(bars, next_unit, u, p.err)) {
         const int n = u.j1 - u.j0;
+        if (u.narrow) {
+          const uint32_t cols = (uint32_t)(u.rows[0] + 15) / 16 * 16;
+          const uint32_t idesc_s = umma_idesc<T>(128, cols, 0, 0);
+          const uint32_t idesc_o = umma_idesc<T>(128, cols, 1, 0);
+          ok = mbar_wait(&bars->q_full[0], qc[0] & 1, p.err) &&
+               mbar_wait(&bars->q_full[1], qc[1] & 1, p.err);
+          // tile j's warpgroup is t = j & 1; its S count grows by one each, PV waits for the last
+          const int sc0 = sc[0], sc1 = sc[1];
+          auto step_s = [&](int j) {
+            const int st = (g + j) % kCkStages, t = j & 1;
+            if (!(ok = mbar_wait(&bars->k_full[st], ((g + j) / kCkStages) & 1, p.err))) return;
+            tc_fence_after();
+            const uint64_t da = umma_desc_sw128(k_addr + st * kChunkTileBytes, 16, 1024);
+            const uint64_t db = umma_desc_sw128(q_addr, 16, 1024);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) {
+              const uint32_t off = ((kk >> 2) * kChunkHalf + (kk & 3) * 32) >> 4;
+              umma_ss(tmem + t * 128, da + off, db + off, idesc_s, kk > 0);
+            }
+            umma_commit(&bars->s_full[t]);
+            umma_commit(&bars->k_empty[st]);
+            if (j == n - 1) umma_commit(&bars->q_empty[0]);
+          };
+#pragma unroll 1
+          for (int j = -2; ok && j < n; ++j) {
+            if (j < 0) {
+              if (j + 2 < n) step_s(j + 2);
+              continue;
+            }
+            const int st = (g + j) % kCkStages, t = j & 1;
+            ok = mbar_wait(&bars->v_full[st], ((g + j) / kCkStages) & 1, p.err) &&
+                 mbar_wait(&bars->p_full[t], ((t ? sc1 : sc0) + (j >> 1)) & 1, p.err);
+            const int uses = t ? oc[1] : oc[0];
+            if (ok && j < 2 && uses > 0) ok = mbar_wait(&bars->o_empty[t], (uses - 1) & 1, p.err);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t da = umma_desc_sw128(v_addr + st * kChunkTileBytes, kChunkHalf, 1024);
+            const uint64_t db = umma_desc_sw128(q_addr + kChunkTileBytes + t * kCkPBytes, 16, 1024);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)
+              umma_ss(tmem + 256 + t * 128, da + (uint32_t)(kk * 128),
+                      db + (uint32_t)(((kk >> 2) * (kCkPBytes / 2) + (kk & 3) * 32) >> 4), idesc_o,
+                      (j >= 2 || kk > 0) ? 1u : 0u);
+            umma_commit(&bars->v_empty[st]);
+            if (j + 2 >= n) umma_commit(&bars->o_full[t]);
+            else step_s(j + 2);  // its scores overwrite those that P was made of
+          }
+          if (ok) umma_commit(&bars->q_empty[1]);
+          g += n;
+          sc[0] += (n + 1) >> 1;
+          sc[1] += n >> 1;
+          ++qc[0];
+          ++qc[1];
+          ++oc[0];
+          if (n > 1) ++oc[1];
+          continue;
+        }
         ok = mbar_wait(&bars->k_full[g % kCkStages], (g / kCkStages) & 1, p.err);
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (u.rows[t] == 0) continue;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (!ok || u.rows[t] == 0) continue;
           ok = mbar_wait(&bars->q_full[t], qc[t] & 1, p.err);
-          if (!ok) break;
+          if (!ok) continue;
           tc_fence_after();
           issue_s(t, g % kCkStages);
           ++sc[t];
           if (n == 1) umma_commit(&bars->q_empty[t]);
         }
         if (ok) umma_commit(&bars->k_empty[g % kCkStages]);
+#pragma unroll 1
         for (int j = 0; ok && j < n; ++j, ++g) {
           const bool has_next = j + 1 < n;
           if (has_next) {
@@ -380,13 +768,14 @@ __global__ void __launch_bounds__(kCkThreads, 1)
           }
           ok = mbar_wait(&bars->v_full[g % kCkStages], (g / kCkStages) & 1, p.err);
           if (!ok) break;
-          for (int t = 0; t < 2 && ok; ++t) {
-            if (u.rows[t] == 0) continue;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (!ok || u.rows[t] == 0) continue;
             ok = mbar_wait(&bars->p_full[t], (sc[t] - 1) & 1, p.err);
             // the first product of a unit overwrites O: the last unit's epilogue has read it
-            if (ok && j == 0 && qc[t] > 0)
-              ok = mbar_wait(&bars->o_empty[t], (qc[t] - 1) & 1, p.err);
-            if (!ok) break;
+            if (ok && j == 0 && oc[t] > 0)
+              ok = mbar_wait(&bars->o_empty[t], (oc[t] - 1) & 1, p.err);
+            if (!ok) continue;
             tc_fence_after();
             issue_pv(t, g % kCkStages, j == 0);
             if (!has_next) {
@@ -402,7 +791,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
           if (has_next) umma_commit(&bars->k_empty[(g + 1) % kCkStages]);
         }
         for (int t = 0; t < 2; ++t)
-          if (u.rows[t] > 0) ++qc[t];
+          if (u.rows[t] > 0) ++qc[t], ++oc[t];
       }
       umma_commit(&bars->mma_done);
       mbar_wait(&bars->mma_done, 0, p.err);
@@ -425,12 +814,34 @@ __global__ void __launch_bounds__(kCkThreads, 1)
     int sc = 0;  // S tiles consumed of this tile
     int g = 0;   // K/V tiles streamed (all units)
     int uc = 0;  // units finished
+    int q1 = 0;  // uses of query tile 1
+    int merges = 0;
+    // false once a wait ran out; the warp then goes on without waiting (see narrow_unit)
     bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.err));
+    };
     CkJoin join = {};
-    for (int64_t w = w_begin; ok && w < w_end;) {
-      const CkUnit u = ck_unit(pb, bars, units, w, w_end);
-      w += u.j1 - u.j0;
-      const int rows = u.rows[t];
+    int next_unit = 0;
+    CkUnit u;
+#pragma unroll 1
+    while (ck_next<true>(bars, next_unit, u, p.err)) {
+      const int rows = t ? u.rows[1] : u.rows[0];
+      const bool begins = u.j0 == 0, ends = u.j1 == u.n;
+      if (begins && !ends) {
+        join.valid = 1;
+        join.last_cta = u.last_cta;
+        join.token = u.token;
+        join.hk = u.hk;
+        join.rows[0] = u.rows[0];
+        join.rows[1] = u.rows[1];
+      }
+      q1 += u.narrow || u.rows[1] > 0;
+      if (u.narrow) {
+        narrow_unit<T, kCap, kAlibi>(p, bars, u, sQ + kChunkTileBytes, sV, tmem, t, quarter, lane,
+                                     q1 - 1, sc, g, uc, merges, cta, ok);
+        continue;
+      }
       if (rows == 0) {
         g += u.j1 - u.j0;
         continue;
@@ -442,23 +853,46 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       float slope2 = 0.f;
       if (kAlibi && live) slope2 = p.f.slopes[head] * kLog2e;
       float m = -INFINITY, l = 0.f;
-      for (int j = u.j0; ok && j < u.j1; ++j, ++sc, ++g) {
+#pragma unroll 1
+      for (int j = u.j0; j < u.j1; ++j, ++sc, ++g) {
         const int tile = ck_tile(u, j);
         const int k0 = tile * kChunkTile;
-        bool page_ok[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) page_ok[i] = chunk_page(pb, u.b, u.keys, tile, i) != pb.num_blocks;
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[t], sc & 1, p.err));
-        if (!ok) break;
+        const bool page0 = chunk_page(pb, u.b, u.keys, tile, 0) != pb.num_blocks;
+        const bool page1 = chunk_page(pb, u.b, u.keys, tile, 1) != pb.num_blocks;
+        wait(&bars->s_full[t], sc & 1);
         if (t == 0 && k0 + kChunkTile > u.keys) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_full[g % kCkStages],
-                                                 (g / kCkStages) & 1, p.err));
-          if (!ok) break;
+          wait(&bars->v_full[g % kCkStages], (g / kCkStages) & 1);
           zero_v_rows(sV + (g % kCkStages) * kChunkTileBytes, max(u.keys - k0, 0), threadIdx.x);
           fence_proxy_async_smem();
         }
         if (warp_live) {
           tc_fence_after();
+          // columns [c_lo, c_hi) and [0, c_pre) are visible
+          const int c_hi = min(pos + 1, u.keys) - k0, c_pre = u.prefix - k0;
+          const int c_lo = pb.window ? pos - pb.window + 1 - k0 : 0;
+          const bool all = !live || ((c_hi >= kChunkTile && c_lo <= 0) || c_pre >= kChunkTile);
+          const bool mask = !__all_sync(0xffffffffu, all && page0 && page1);
+          if (kCap || kAlibi || mask) {
+            // the score's form and the mask, 32 columns at a time, back into tensor memory
+#pragma unroll 1
+            for (int cc = 0; cc < kChunkTile; cc += 32) {
+              uint32_t sr[32];
+              tmem_ld32(tS + cc, sr);
+              tmem_wait_ld();
+              reg_fence<32>(sr);
+              score_form<kCap, kAlibi>(sr, p.f, slope2, (float)(k0 + cc - pos), live);
+              if (mask) {
+                uint32_t vis = (low_bits(c_hi - cc, 0) & ~low_bits(c_lo - cc, 0)) |
+                               low_bits(c_pre - cc, 0);
+                if (!(cc < 64 ? page0 : page1)) vis = 0;
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                  if (!((vis >> c) & 1u)) sr[c] = __float_as_uint(-INFINITY);
+              }
+              tmem_st32(tS + cc, sr);
+            }
+            tmem_wait_st();
+          }
           uint32_t sr[kChunkTile];
           tmem_ld32(tS + 0, sr + 0);
           tmem_ld32(tS + 32, sr + 32);
@@ -466,22 +900,6 @@ __global__ void __launch_bounds__(kCkThreads, 1)
           tmem_ld32(tS + 96, sr + 96);
           tmem_wait_ld();
           reg_fence<kChunkTile>(sr);
-          score_form<kCap, kAlibi>(sr, p.f, slope2, (float)(k0 - pos), live);
-          // columns [c_lo, c_hi) and [0, c_pre) are visible
-          const int c_hi = min(pos + 1, u.keys) - k0, c_pre = u.prefix - k0;
-          const int c_lo = pb.window ? pos - pb.window + 1 - k0 : 0;
-          const bool all = !live || ((c_hi >= kChunkTile && c_lo <= 0) || c_pre >= kChunkTile);
-          if (!__all_sync(0xffffffffu, all && page_ok[0] && page_ok[1])) {
-            uint32_t vis[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              vis[i] = (low_bits(c_hi, i) & ~low_bits(c_lo, i)) | low_bits(c_pre, i);
-              if (!page_ok[i >> 1]) vis[i] = 0;
-            }
-#pragma unroll
-            for (int c = 0; c < kChunkTile; ++c)
-              if (!((vis[c >> 5] >> (c & 31)) & 1u)) sr[c] = __float_as_uint(-INFINITY);
-          }
           float mx8[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -531,18 +949,8 @@ __global__ void __launch_bounds__(kCkThreads, 1)
         if (lane == 0) mbar_arrive(&bars->p_full[t]);
       }
       // ----------------------------------------------------------- epilogue
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_full[t], uc & 1, p.err));
-      if (!ok) break;
+      wait(&bars->o_full[t], uc & 1);
       tc_fence_after();
-      const bool begins = u.j0 == 0, ends = u.j1 == u.n;
-      if (begins && !ends) {
-        join.valid = 1;
-        join.last_cta = (int)(((w - u.j1 + u.n) * active - 1) / total);
-        join.token = u.token;
-        join.hk = u.hk;
-        join.rows[0] = u.rows[0];
-        join.rows[1] = u.rows[1];
-      }
       const bool none = m == -INFINITY;
       const float inv = none ? 0.f : 1.f / l;
       const float lse2 = none ? -INFINITY : m + log2f(l);
@@ -610,6 +1018,7 @@ __global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p)
   const int cta = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const CkJoin jn = p.join[cta];
   if (!jn.valid) return;
+#pragma unroll 1
   for (int r = blockIdx.y * 8 + warp; r < 256; r += kJoinSlices * 8) {
     const int t = r >> 7, row = r & 127;
     if (row >= jn.rows[t]) continue;

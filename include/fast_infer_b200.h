@@ -197,7 +197,7 @@ int fi_paged_decode_noalloc(const void* q, const void* k_cache, const void* v_ca
  * invalid is skipped (FI_DEVERR_BAD_BLOCK); lengths that do not fit total_tokens or the block
  * table are cut and set FI_DEVERR_CONTEXT_LEN.
  * dtype: of q, k_cache, v_cache and o. workspace: fi_paged_chunk_workspace_size(...) bytes,
- * 16-byte aligned. At most 64 query heads per KV head, 2048 sequences, and 6000 units of
+ * 16-byte aligned. At most 64 query heads per KV head, 2048 sequences, and 4608 units of
  * 2 * (128 / heads per KV head) tokens. Deterministic: the same bits on every run.
  */
 size_t fi_paged_chunk_workspace_size(int64_t total_tokens, int64_t num_q_heads,
