@@ -17,12 +17,15 @@
 // * Roles (384 threads), tensor memory (S0 | S1 | O0 | O1), the lazily rescaled online
 //   softmax and the MMA order are those of the causal prefill kernel (prefill_sm100.cu). K
 //   and V tiles are two pages each, gathered by TMA through the block table.
-// * A unit of at most 32 rows (single tokens, drafted tokens) runs transposed: S^T = K Q^T with
-//   the 128 keys of a tile as tensor-memory lanes and N = its rows, then O^T += V^T P^T with P
-//   through shared memory, so no lane idles and a tile costs a softmax thread its rows, not 128
-//   columns: the unit streams K and V at HBM's rate. The warpgroups take alternate key tiles as
-//   two running softmaxes and merge them at the end. A row's max moves only when some score
-//   passes it by 2^8, found by one vote per tile.
+// * Sequences of at most 32 rows (single tokens, drafted tokens) have a kernel of their own, of
+//   the same roles, in which a unit runs transposed: S^T = K Q^T with the 128 keys of a tile as
+//   tensor-memory lanes and N = its rows, then O^T += V^T P^T with P through shared memory, so
+//   no lane idles and a tile costs a softmax thread its rows, not 128 columns. The warpgroups
+//   take alternate key tiles as two running softmaxes and merge them at the end. A row's max
+//   moves only when some score passes it by 2^8, found by one vote per tile. (One kernel for
+//   both forms was tried: its registers spilled and its code, 150 KB, missed the instruction
+//   caches; long prefills lost 10 %, single tokens 40 %.) A batch that may hold both kinds
+//   launches both kernels, the second beginning on each SM as the first leaves it.
 // * Slots behind a sequence's last token may hold anything: their scores are replaced by
 //   -inf, and their V rows are zeroed in shared memory before the product (0 * NaN is NaN).
 #include "chunk_common.cuh"
@@ -49,11 +52,16 @@ struct alignas(16) CkUnit {
   int keys, prefix;
   int np, lo;          // step j is key tile j < np ? j : lo + j - np
   int j0, j1, n;
-  int narrow;          // runs transposed
+  int pad;
   int last_cta;        // the CTA with the unit's last step
   int valid;           // 0: no unit is left
 };
 static_assert(sizeof(CkUnit) == 64, "read as four 16-byte words");
+
+// The unit whose first part a CTA holds when the rest lies in the next CTAs.
+struct CkJoin {
+  int valid, last_cta, token, hk, rows[2], pad[2];
+};
 
 struct CkBarriers {
   uint64_t q_full[2], q_empty[2];
@@ -66,20 +74,17 @@ struct CkBarriers {
   uint32_t tmem_base;
   // transposed units, per warpgroup: rows' max, partial maxima / sums, scale, slope, position
   float n_max[2][kCkNarrow], n_red[2][4][kCkNarrow], n_alpha[2][kCkNarrow];
+  alignas(16) float n_neg[2][kCkNarrow];  // -max
   float n_slope[2][kCkNarrow], n_pos[2][kCkNarrow];
   int64_t n_off[kCkNarrow];  // where a row's output goes
   CkUnit units[kCkSlots];
+  uint8_t row_token[kChunkTile], row_head[kChunkTile];  // of a tile's rows
   uint32_t warp_sums[kCkThreads / 32];
   uint32_t unit_off[kCkMaxBatch + 1];  // first unit of each sequence
   uint32_t work[kCkMaxUnits + 1];      // key tiles before each unit
 };
 constexpr int kCkSmemBytes = 1024 + (2 + 2 * kCkStages) * kChunkTileBytes + (int)sizeof(CkBarriers);
 static_assert(kCkSmemBytes <= 227 * 1024, "shared memory");
-
-// The unit whose first part a CTA holds when the rest lies in the next CTAs.
-struct CkJoin {
-  int valid, last_cta, token, hk, rows[2], pad[2];
-};
 
 constexpr int kCkPBytes = kCkNarrow * 256;  // P^T of a transposed unit: 32 rows x 128 keys
 static_assert(kCkNarrow == 32, "a column per lane where rows are summed");
@@ -95,6 +100,9 @@ struct ChunkParams {
   float* ws_lse;  // [cta][first, last unit][rows_cap], log2 domain
   CkJoin* join;   // [cta]
   int rows_cap;
+  int unit_tokens;  // tokens of a unit: two tiles, or those of kCkNarrow rows
+  int split_rows;   // sequences of at most so many rows are the narrow kernel's, others the wide's
+  int late_wait;    // the kernel before on the stream is the other one of this call
   int* err;
 };
 
@@ -116,8 +124,8 @@ __device__ __forceinline__ void ck_tiles(const ChunkBatch& p, const ChunkSeq& s,
 
 // The scheduler (one thread): walks the CTA's part of the line and hands its units to the other
 // roles through a ring in shared memory.
-__device__ __forceinline__ void ck_schedule(const ChunkBatch& p, CkBarriers* s, uint32_t units,
-                                            int* err) {
+__device__ __forceinline__ void ck_schedule(const ChunkBatch& p, int unit_tokens, CkBarriers* s,
+                                            uint32_t units, CkJoin* join_out, int* err) {
   const int G = gridDim.x, cta = blockIdx.x;
   const uint32_t per_head = s->work[units];
   const int64_t total = (int64_t)per_head * p.hk;
@@ -134,14 +142,16 @@ __device__ __forceinline__ void ck_schedule(const ChunkBatch& p, CkBarriers* s, 
   }
   ChunkSeq q = chunk_seq(p, b);
   const int tt = p.tile_tokens;
+  CkJoin join = {};
 #pragma unroll 1
   for (int i = 0;; ++i) {
     const int slot = i % kCkSlots;
-    if (i >= kCkSlots && !mbar_wait(&s->unit_empty[slot], ((i / kCkSlots) - 1) & 1, err)) return;
+    if (i >= kCkSlots && !mbar_wait(&s->unit_empty[slot], ((i / kCkSlots) - 1) & 1, err)) break;
     CkUnit u;
     u.valid = w < end;
+    u.pad = 0;
     if (u.valid) {
-      const int t0 = (e - (int)s->unit_off[b]) * 2 * tt, t1 = min(t0 + 2 * tt, q.n);
+      const int t0 = (e - (int)s->unit_off[b]) * unit_tokens, t1 = min(t0 + unit_tokens, q.n);
       ck_tiles(p, q, t0, t1, u.np, u.lo, u.n);
       u.b = b;
       u.hk = hk;
@@ -151,7 +161,6 @@ __device__ __forceinline__ void ck_schedule(const ChunkBatch& p, CkBarriers* s, 
       u.prefix = q.prefix;
       u.rows[0] = min(t1 - t0, tt) * p.group;
       u.rows[1] = max(t1 - t0 - tt, 0) * p.group;
-      u.narrow = u.rows[1] == 0 && u.rows[0] <= kCkNarrow;
       u.j0 = j0;
       u.j1 = (int)(u.n - j0 <= end - w ? u.n : j0 + (end - w));
       // the last step of the unit, w - j0 + n - 1, belongs to the last CTA that starts at or before it
@@ -170,22 +179,33 @@ __device__ __forceinline__ void ck_schedule(const ChunkBatch& p, CkBarriers* s, 
     }
     s->units[slot] = u;
     mbar_arrive(&s->unit_full[slot]);  // released to the waits that read it
-    if (!u.valid) return;
+    if (u.valid && u.j0 == 0 && u.j1 < u.n) {  // begins here and goes on: it is the last one
+      join.valid = 1;
+      join.last_cta = u.last_cta;
+      join.token = u.token;
+      join.hk = u.hk;
+      join.rows[0] = u.rows[0];
+      join.rows[1] = u.rows[1];
+    }
+    if (!u.valid) break;
   }
+  *join_out = join;
 }
 
-// The next unit from the ring (a whole warp, or one thread with kWarp = false).
+// The next unit of the ring, null when none is left; it stays in shared memory, read there by
+// whole warps (or one thread, kWarp = false), until ck_done gives the slot back.
 template <bool kWarp>
-__device__ __forceinline__ bool ck_next(CkBarriers* s, int& i, CkUnit& u, int* err) {
+__device__ __forceinline__ const CkUnit* ck_next(CkBarriers* s, int i, int* err) {
   const int slot = i % kCkSlots;
   bool ok = mbar_wait(&s->unit_full[slot], (i / kCkSlots) & 1, err);
   if (kWarp) ok = __all_sync(0xffffffffu, ok);
-  if (!ok) return false;
-  u = s->units[slot];
+  return ok && s->units[slot].valid ? &s->units[slot] : nullptr;
+}
+template <bool kWarp>
+__device__ __forceinline__ void ck_done(CkBarriers* s, int& i) {
   if (kWarp) __syncwarp();
-  if (!kWarp || (threadIdx.x & 31) == 0) mbar_arrive(&s->unit_empty[slot]);
+  if (!kWarp || (threadIdx.x & 31) == 0) mbar_arrive(&s->unit_empty[i % kCkSlots]);
   ++i;
-  return u.valid;
 }
 
 // 32 scores of one row in log2 units, in place: the cap and the distance bias (without either,
@@ -224,6 +244,42 @@ __device__ __forceinline__ void score_form(uint32_t* sr, const ScoreForm& f, flo
       const float s = __uint_as_float(sr[c]);
       const float d = fabsf(off + (float)c) * slope2;
       sr[c] = __float_as_uint(kCap ? s - d : fmaf(s, f.scale_log2, -d));
+    }
+  }
+}
+
+// 8 scores of one key in log2 units, one per row of a transposed unit.
+template <bool kCap, bool kAlibi>
+__device__ __forceinline__ void score_form8(const uint32_t* raw, float* s, const ScoreForm& f,
+                                             const float* slope2, const float* pos, float key) {
+  bool small = true;
+  if constexpr (kCap) {
+    float big = 0.f;
+#pragma unroll
+    for (int c = 0; c < 8; c += 2)
+      big = fmax3f(big, fabsf(__uint_as_float(raw[c])), fabsf(__uint_as_float(raw[c + 1])));
+    small = __all_sync(0xffffffffu, big * f.cap_in <= 1.f);
+  }
+#pragma unroll
+  for (int c = 0; c < 8; c += 2) {
+    uint64_t x = f32x2(__uint_as_float(raw[c]), __uint_as_float(raw[c + 1]));
+    if constexpr (kCap) {
+      const uint64_t v = mul_f32x2(x, f32x2(f.cap_in, f.cap_in));
+      uint64_t y = tanh_poly_x2(v);
+      if (!small) {
+        float v0, v1, y0, y1;
+        f32x2_split(v, v0, v1);
+        f32x2_split(y, y0, y1);
+        y = f32x2(fabsf(v0) <= 1.f ? y0 : tanh_any(v0), fabsf(v1) <= 1.f ? y1 : tanh_any(v1));
+      }
+      x = mul_f32x2(y, f32x2(f.cap_log2, f.cap_log2));
+    } else {
+      x = mul_f32x2(x, f32x2(f.scale_log2, f.scale_log2));
+    }
+    f32x2_split(x, s[c], s[c + 1]);
+    if constexpr (kAlibi) {
+      s[c] -= slope2[c] * fabsf(pos[c] - key);
+      s[c + 1] -= slope2[c + 1] * fabsf(pos[c + 1] - key);
     }
   }
 }
@@ -280,24 +336,26 @@ __device__ __forceinline__ float order_float(int i) {
 template <typename T, bool kCap, bool kAlibi>
 __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* bars, const CkUnit& u,
                                             uint8_t* sP, uint8_t* sV, uint32_t tmem, int t,
-                                            int quarter, int lane, int q1, int& sc, int& g,
+                                            int quarter, int lane, int& sc, int& g,
                                             int& uc, int& merges, int cta, bool& ok) {
   const ChunkBatch& pb = p.b;
   const int rows = u.rows[0], n = u.j1 - u.j0, tid = quarter * 32 + lane;
   const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
   const uint32_t tS = tmem + lane_off + t * 128, tO = tmem + lane_off + 256;
   const bool mine = t < n;  // this warpgroup has a key tile
-  const float sl2 = p.f.scale_log2;
   float l[kCkNarrow];
 #pragma unroll
   for (int c = 0; c < kCkNarrow; ++c) l[c] = 0.f;
   float* n_max = bars->n_max[t];
+  constexpr float kTop = 256.f;  // 2^kCkRescale
   if (tid < kCkNarrow) {
     n_max[tid] = -INFINITY;
+    bars->n_neg[t][tid] = tid < rows ? INFINITY : -INFINITY;
+    bars->n_alpha[t][tid] = 0.f;
     if (kAlibi) {
       const bool live = tid < rows;
-      bars->n_slope[t][tid] = live ? p.f.slopes[u.hk * pb.group + tid % pb.group] * kLog2e : 0.f;
-      bars->n_pos[t][tid] = (float)(u.pos + tid / pb.group);
+      bars->n_slope[t][tid] = live ? p.f.slopes[u.hk * pb.group + bars->row_head[tid]] * kLog2e : 0.f;
+      bars->n_pos[t][tid] = (float)(u.pos + bars->row_token[tid]);
     }
   }
   named_bar_sync(1 + t, 128);
@@ -309,7 +367,6 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
     if (lane == 0) mbar_arrive(&bars->merge);
     wait(&bars->merge, merges++ & 1);
   };
-  if (mine) wait(&bars->q_full[1], q1 & 1);
   // P^T is [rows][128 keys], K-major with the 128-byte swizzle: this thread's column of it
   uint8_t* pcol = sP + t * kCkPBytes + (tid >> 6) * (kCkPBytes / 2);
   const uint32_t kbyte = (uint32_t)(tid & 63) * 2;
@@ -331,105 +388,98 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
       if (pb.window) c_hi = min(rows, min(max(key + pb.window - u.pos, 0), kCkNarrow) * pb.group);
     }
     if (!page_ok || key >= u.keys) c_hi = 0;
-    uint32_t s[kCkNarrow];
-    bool past = false;
+    const bool mask = !__all_sync(0xffffffffu, c_lo <= 0 && c_hi >= rows);
+    float s[kCkNarrow];  // scores in log2 units, then 2^(score - max)
+    // the first tile sets the rows' max; later ones keep it unless some score passes it by 2^8
+#pragma unroll 1
+    for (bool move = j == t;; move = true) {
 #pragma unroll
-    for (int cc = 0; cc < kCkNarrow; cc += 16) {
-      if (cc < rows) {
-        tmem_ld16(tS + cc, s + cc);
-        tmem_wait_ld();
-        reg_fence<16>(s + cc);
-        const uint32_t vis = (low_bits(c_hi - cc, 0) & ~low_bits(c_lo - cc, 0));
-        bool small = true;
-        if constexpr (kCap) {
-          float big = 0.f;
+      for (int cc = 0; cc < kCkNarrow; cc += 8)
+        if (cc < rows) {
+          uint32_t raw[8];
+          tmem_ld8(tS + cc, raw);
+          tmem_wait_ld();
+          reg_fence<8>(raw);
+          score_form8<kCap, kAlibi>(raw, s + cc, p.f, bars->n_slope[t] + cc, bars->n_pos[t] + cc,
+                                     (float)key);
+          if (mask) {
+            const uint32_t vis = low_bits(c_hi - cc, 0) & ~low_bits(c_lo - cc, 0);
 #pragma unroll
-          for (int c = cc; c < cc + 16; ++c)
-            big = fmaxf(big, (vis >> (c - cc)) & 1u ? fabsf(__uint_as_float(s[c])) : 0.f);
-          small = __all_sync(0xffffffffu, big * p.f.cap_in <= 1.f);
+            for (int c = 0; c < 8; ++c)
+              if (!((vis >> c) & 1u)) s[cc + c] = -INFINITY;
+          }
         }
+      if (move) {
 #pragma unroll
-        for (int c = cc; c < cc + 16; c += 2) {
-          float x0 = __uint_as_float(s[c]), x1 = __uint_as_float(s[c + 1]);
-          if constexpr (kCap) {
-            const uint64_t v = mul_f32x2(f32x2(x0, x1), f32x2(p.f.cap_in, p.f.cap_in));
-            uint64_t y = tanh_poly_x2(v);
-            if (!small) {
-              float v0, v1, y0, y1;
-              f32x2_split(v, v0, v1);
-              f32x2_split(y, y0, y1);
-              y = f32x2(fabsf(v0) <= 1.f ? y0 : tanh_any(v0), fabsf(v1) <= 1.f ? y1 : tanh_any(v1));
+        for (int cc = 0; cc < kCkNarrow; cc += 8)
+          if (cc < rows) {
+#pragma unroll
+            for (int c = cc; c < cc + 8; ++c) {
+              const int mx = __reduce_max_sync(0xffffffffu, float_order(s[c]));
+              if (lane == 0) bars->n_red[t][quarter][c] = order_float(mx);
             }
-            f32x2_split(mul_f32x2(y, f32x2(p.f.cap_log2, p.f.cap_log2)), x0, x1);
-          } else {
-            x0 *= sl2;
-            x1 *= sl2;
           }
-          if constexpr (kAlibi) {
-            x0 -= bars->n_slope[t][c] * fabsf(bars->n_pos[t][c] - (float)key);
-            x1 -= bars->n_slope[t][c + 1] * fabsf(bars->n_pos[t][c + 1] - (float)key);
-          }
-          if (!((vis >> (c - cc)) & 1u)) x0 = -INFINITY;
-          if (!((vis >> (c + 1 - cc)) & 1u)) x1 = -INFINITY;
-          past |= x0 > n_max[c] + kCkRescale;
-          past |= x1 > n_max[c + 1] + kCkRescale;
-          s[c] = __float_as_uint(x0);
-          s[c + 1] = __float_as_uint(x1);
+        named_bar_sync(1 + t, 128);
+        if (tid < rows) {
+          const float was = n_max[tid];
+          const float now = fmaxf(fmaxf(was, fmaxf(bars->n_red[t][0][tid], bars->n_red[t][1][tid])),
+                                  fmaxf(bars->n_red[t][2][tid], bars->n_red[t][3][tid]));
+          bars->n_alpha[t][tid] = was == -INFINITY ? 0.f : fast_exp2(was - now);
+          n_max[tid] = now;
+          bars->n_neg[t][tid] = -now;
+        }
+        named_bar_sync(1 + t, 128);
+        if (j >= 2) {
+          // the product of this warpgroup's last tile is complete: S here was committed after it
+#pragma unroll
+          for (int cc = 0; cc < kCkNarrow; cc += 8)
+            if (cc < rows) {
+              uint32_t ov[8];
+              tmem_ld8(tO + t * 128 + cc, ov);
+              tmem_wait_ld();
+              reg_fence<8>(ov);
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                const float a = bars->n_alpha[t][cc + c];
+                ov[c] = __float_as_uint(__uint_as_float(ov[c]) * a);
+                l[cc + c] *= a;
+              }
+              tmem_st8(tO + t * 128 + cc, ov);
+            }
+          tmem_wait_st();
         }
       }
-    }
-    if (!wg_bar_and(1 + t, !past)) {
-      // some row's max moves: all rows go to their running maximum
+      // A row that has seen nothing has max -inf: a score it sees gives 2^inf, past any bound; one
+      // it does not see gives NaN, which the maximum below passes over and the mask sets to 0. A
+      // column without a row has max +inf: p = 0.
+      float top = 0.f;
 #pragma unroll
-      for (int cc = 0; cc < kCkNarrow; cc += 16)
+      for (int cc = 0; cc < kCkNarrow; cc += 8)
         if (cc < rows) {
 #pragma unroll
-          for (int c = cc; c < cc + 16; ++c) {
-            const int mx = __reduce_max_sync(0xffffffffu, float_order(__uint_as_float(s[c])));
-            if (lane == 0) bars->n_red[t][quarter][c] = order_float(mx);
+          for (int c = cc; c < cc + 8; c += 4) {
+            const float4 nm = *reinterpret_cast<const float4*>(&bars->n_neg[t][c]);
+            s[c] = fast_exp2(s[c] + nm.x);
+            s[c + 1] = fast_exp2(s[c + 1] + nm.y);
+            s[c + 2] = fast_exp2(s[c + 2] + nm.z);
+            s[c + 3] = fast_exp2(s[c + 3] + nm.w);
+            top = fmax3f(fmax3f(top, s[c], s[c + 1]), s[c + 2], s[c + 3]);
+          }
+          if (mask) {
+#pragma unroll
+            for (int c = cc; c < cc + 8; ++c) s[c] = fmaxf(s[c], 0.f);  // NaN -> 0
           }
         }
-      named_bar_sync(1 + t, 128);
-      if (tid < kCkNarrow) {
-        const float was = n_max[tid];  // a column without a row stays at -inf
-
-        const float now = fmaxf(fmaxf(was, fmaxf(bars->n_red[t][0][tid], bars->n_red[t][1][tid])),
-                                fmaxf(bars->n_red[t][2][tid], bars->n_red[t][3][tid]));
-        bars->n_alpha[t][tid] = was == -INFINITY ? 0.f : fast_exp2(was - now);
-        n_max[tid] = now;
-      }
-      named_bar_sync(1 + t, 128);
-      if (j >= 2) {
-        // the product of this warpgroup's last tile is complete: S here was committed after it
-#pragma unroll
-        for (int cc = 0; cc < kCkNarrow; cc += 16)
-          if (cc < rows) {
-            uint32_t ov[16];
-            tmem_ld16(tO + t * 128 + cc, ov);
-            tmem_wait_ld();
-            reg_fence<16>(ov);
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              const float a = bars->n_alpha[t][cc + c];
-              ov[c] = __float_as_uint(__uint_as_float(ov[c]) * a);
-              l[cc + c] *= a;
-            }
-            tmem_st16(tO + t * 128 + cc, ov);
-          }
-        tmem_wait_st();
-      }
+      if (move || wg_bar_and(1 + t, top <= kTop)) break;
     }
 #pragma unroll
-    for (int cc = 0; cc < kCkNarrow; cc += 16)
+    for (int cc = 0; cc < kCkNarrow; cc += 8)
       if (cc < rows) {
 #pragma unroll
-        for (int c = cc; c < cc + 16; c += 2) {
-          const float m0 = n_max[c], m1 = n_max[c + 1];
-          const float p0 = fast_exp2(__uint_as_float(s[c]) - (m0 == -INFINITY ? 0.f : m0));
-          const float p1 = fast_exp2(__uint_as_float(s[c + 1]) - (m1 == -INFINITY ? 0.f : m1));
-          l[c] += p0;
-          l[c + 1] += p1;
-          const uint32_t pk = Half16<T>::pack(p0, p1);
+        for (int c = cc; c < cc + 8; c += 2) {
+          l[c] += s[c];
+          l[c + 1] += s[c + 1];
+          const uint32_t pk = Half16<T>::pack(s[c], s[c + 1]);
           *reinterpret_cast<uint16_t*>(pcol + c * 128 + (kbyte ^ ((c & 7) << 4))) = (uint16_t)pk;
           *reinterpret_cast<uint16_t*>(pcol + (c + 1) * 128 + (kbyte ^ (((c + 1) & 7) << 4))) =
               (uint16_t)(pk >> 16);
@@ -469,8 +519,8 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
     bars->n_alpha[0][tid] = none ? 0.f : w0 / sum;
     bars->n_alpha[1][tid] = none ? 0.f : w1 / sum;
     const float lse2 = none ? -INFINITY : mx + log2f(sum);
-    const int64_t token = u.token + tid / pb.group;
-    const int head = u.hk * pb.group + tid % pb.group;
+    const int64_t token = u.token + bars->row_token[tid];
+    const int head = u.hk * pb.group + bars->row_head[tid];
     if (whole) {
       bars->n_off[tid] = token * p.os[0] + head * p.os[1];
       if (p.lse) p.lse[token * pb.hq + head] = lse2 * kLn2;
@@ -482,15 +532,15 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
   }
   meet();
 #pragma unroll 1
-  for (int cc = t * 16; cc < rows; cc += 32) {
-    uint32_t a0[16], a1[16];
-    tmem_ld16(tO + cc, a0);
-    if (n > 1) tmem_ld16(tO + 128 + cc, a1);
+  for (int cc = t * 8; cc < rows; cc += 16) {
+    uint32_t a0[8], a1[8];
+    tmem_ld8(tO + cc, a0);
+    if (n > 1) tmem_ld8(tO + 128 + cc, a1);
     tmem_wait_ld();
-    reg_fence<16>(a0);
-    if (n > 1) reg_fence<16>(a1);
+    reg_fence<8>(a0);
+    if (n > 1) reg_fence<8>(a1);
 #pragma unroll
-    for (int c = 0; c < 16; ++c) {
+    for (int c = 0; c < 8; ++c) {
       const int r = cc + c;
       if (r < rows) {
         const float f0 = bars->n_alpha[0][r], f1 = bars->n_alpha[1][r];
@@ -513,7 +563,7 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
   g += n;
 }
 
-template <typename T, bool kCap, bool kAlibi>
+template <typename T, bool kCap, bool kAlibi, bool kNarrow>
 __global__ void __launch_bounds__(kCkThreads, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q,
                        const __grid_constant__ CUtensorMap tm_k,
@@ -557,32 +607,50 @@ __global__ void __launch_bounds__(kCkThreads, 1)
   }
 
   // The line of work: units of each sequence, then key tiles of each unit, both as sums.
-  grid_dep_wait();
+  if (!p.late_wait) grid_dep_wait();
   grid_dep_launch();
   const ChunkBatch& pb = p.b;
   if (threadIdx.x == 0) bars->unit_off[0] = bars->work[0] = 0;
+  if (threadIdx.x < kChunkTile) {
+    bars->row_token[threadIdx.x] = (uint8_t)(threadIdx.x / pb.group);
+    bars->row_head[threadIdx.x] = (uint8_t)(threadIdx.x % pb.group);
+  }
+  bool single = true;  // at most one unit in each of this thread's sequences
 #pragma unroll 1
   for (int b = threadIdx.x; b < pb.batch; b += kCkThreads) {
     const ChunkSeq q = chunk_seq(pb, b);
-    bars->unit_off[b + 1] = (uint32_t)((q.n + 2 * pb.tile_tokens - 1) / (2 * pb.tile_tokens));
     if (q.bad && cta == 0) set_error(p.err, FI_DEVERR_CONTEXT_LEN);
+    const bool here = (q.n * pb.group <= p.split_rows) == kNarrow;
+    const int n = here ? (q.n + p.unit_tokens - 1) / p.unit_tokens : 0;
+    bars->unit_off[b + 1] = (uint32_t)n;
+    single &= n == 1;
+    if (n == 1) {
+      int np, lo, tiles;
+      ck_tiles(pb, q, 0, q.n, np, lo, tiles);
+      bars->work[b + 1] = (uint32_t)tiles;
+    }
   }
-  __syncthreads();
-  block_scan(bars->unit_off, pb.batch, bars->warp_sums);
-  // cu that is not ascending could name more units than the host counted: those are dropped
-  const uint32_t units = min(bars->unit_off[pb.batch], (uint32_t)kCkMaxUnits);
-  if (units != bars->unit_off[pb.batch] && threadIdx.x == 0)
-    set_error(p.err, FI_DEVERR_CONTEXT_LEN);
+  uint32_t units;
+  if (__syncthreads_and(single)) {  // unit b is sequence b
+    units = (uint32_t)pb.batch;
+    for (int b = threadIdx.x; b < pb.batch; b += kCkThreads) bars->unit_off[b + 1] = b + 1;
+  } else {
+    block_scan(bars->unit_off, pb.batch, bars->warp_sums);
+    // cu that is not ascending could name more units than the host counted: those are dropped
+    units = min(bars->unit_off[pb.batch], (uint32_t)kCkMaxUnits);
+    if (units != bars->unit_off[pb.batch] && threadIdx.x == 0)
+      set_error(p.err, FI_DEVERR_CONTEXT_LEN);
 #pragma unroll 1
-  for (int e = threadIdx.x; e < (int)units; e += kCkThreads) {
-    const int b = last_le(bars->unit_off, pb.batch, (uint32_t)e);
-    const ChunkSeq q = chunk_seq(pb, b);
-    const int t0 = (e - (int)bars->unit_off[b]) * 2 * pb.tile_tokens;
-    int np, lo, n;
-    ck_tiles(pb, q, t0, min(t0 + 2 * pb.tile_tokens, q.n), np, lo, n);
-    bars->work[e + 1] = (uint32_t)n;
+    for (int e = threadIdx.x; e < (int)units; e += kCkThreads) {
+      const int b = last_le(bars->unit_off, pb.batch, (uint32_t)e);
+      const ChunkSeq q = chunk_seq(pb, b);
+      const int t0 = (e - (int)bars->unit_off[b]) * p.unit_tokens;
+      int np, lo, n;
+      ck_tiles(pb, q, t0, min(t0 + p.unit_tokens, q.n), np, lo, n);
+      bars->work[e + 1] = (uint32_t)n;
+    }
+    __syncthreads();
   }
-  __syncthreads();
   block_scan(bars->work, (int)units, bars->warp_sums);
   tc_fence_before();
   __syncthreads();
@@ -600,20 +668,16 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       int qc[2] = {0, 0};
       int g = 0, next_unit = 0;
       bool ok = true;
-      CkUnit u;
 #pragma unroll 1
-      while (ok && ck_next<false>(bars, next_unit, u, p.err)) {
+      for (const CkUnit* up; ok && (up = ck_next<false>(bars, next_unit, p.err)) != nullptr;
+           ck_done<false>(bars, next_unit)) {
+        const CkUnit& u = *up;
         auto load_q = [&]() {
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (!ok || (u.rows[t] == 0 && !u.narrow)) continue;
+            if (!ok || u.rows[t] == 0) continue;
             if (qc[t] > 0) ok = mbar_wait(&bars->q_empty[t], (qc[t] - 1) & 1, p.err);
             if (!ok) continue;
-            if (t == 1 && u.narrow) {  // the tile's memory holds P of a transposed unit
-              mbar_arrive(&bars->q_full[1]);
-              ++qc[1];
-              continue;
-            }
             const int token = u.token + t * pb.tile_tokens;
             uint8_t* dst = sQ + t * kChunkTileBytes;
             mbar_arrive_expect_tx(&bars->q_full[t], q_bytes);
@@ -657,7 +721,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
         }
       }
     } else if (warp == 10 && lane == 0) {
-      ck_schedule(pb, bars, units, p.err);
+      ck_schedule(pb, p.unit_tokens, bars, units, p.join + cta, p.err);
     } else if (warp == 9 && lane == 0) {
       // ---------------------------------------------------------- UMMA issuer
       constexpr uint32_t idesc_qk = umma_idesc<T>(128, 128, 0, 0);
@@ -686,16 +750,16 @@ __global__ void __launch_bounds__(kCkThreads, 1)
                   idesc_pv, (!first || kk > 0) ? 1u : 0u);
       };
       int next_unit = 0;
-      CkUnit u;
 #pragma unroll 1
-      while (ok && ck_next<false>(bars, next_unit, u, p.err)) {
+      for (const CkUnit* up; ok && (up = ck_next<false>(bars, next_unit, p.err)) != nullptr;
+           ck_done<false>(bars, next_unit)) {
+        const CkUnit& u = *up;
         const int n = u.j1 - u.j0;
-        if (u.narrow) {
+        if constexpr (kNarrow) {
           const uint32_t cols = (uint32_t)(u.rows[0] + 15) / 16 * 16;
           const uint32_t idesc_s = umma_idesc<T>(128, cols, 0, 0);
           const uint32_t idesc_o = umma_idesc<T>(128, cols, 1, 0);
-          ok = mbar_wait(&bars->q_full[0], qc[0] & 1, p.err) &&
-               mbar_wait(&bars->q_full[1], qc[1] & 1, p.err);
+          ok = mbar_wait(&bars->q_full[0], qc[0] & 1, p.err);
           // tile j's warpgroup is t = j & 1; its S count grows by one each, PV waits for the last
           const int sc0 = sc[0], sc1 = sc[1];
           auto step_s = [&](int j) {
@@ -737,16 +801,13 @@ __global__ void __launch_bounds__(kCkThreads, 1)
             if (j + 2 >= n) umma_commit(&bars->o_full[t]);
             else step_s(j + 2);  // its scores overwrite those that P was made of
           }
-          if (ok) umma_commit(&bars->q_empty[1]);
           g += n;
           sc[0] += (n + 1) >> 1;
           sc[1] += n >> 1;
           ++qc[0];
-          ++qc[1];
           ++oc[0];
           if (n > 1) ++oc[1];
-          continue;
-        }
+        } else {
         ok = mbar_wait(&bars->k_full[g % kCkStages], (g / kCkStages) & 1, p.err);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -792,6 +853,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
         }
         for (int t = 0; t < 2; ++t)
           if (u.rows[t] > 0) ++qc[t], ++oc[t];
+        }
       }
       umma_commit(&bars->mma_done);
       mbar_wait(&bars->mma_done, 0, p.err);
@@ -814,41 +876,30 @@ __global__ void __launch_bounds__(kCkThreads, 1)
     int sc = 0;  // S tiles consumed of this tile
     int g = 0;   // K/V tiles streamed (all units)
     int uc = 0;  // units finished
-    int q1 = 0;  // uses of query tile 1
     int merges = 0;
     // false once a wait ran out; the warp then goes on without waiting (see narrow_unit)
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.err));
     };
-    CkJoin join = {};
     int next_unit = 0;
-    CkUnit u;
 #pragma unroll 1
-    while (ck_next<true>(bars, next_unit, u, p.err)) {
+    for (const CkUnit* up; (up = ck_next<true>(bars, next_unit, p.err)) != nullptr;
+         ck_done<true>(bars, next_unit)) {
+      const CkUnit& u = *up;
       const int rows = t ? u.rows[1] : u.rows[0];
       const bool begins = u.j0 == 0, ends = u.j1 == u.n;
-      if (begins && !ends) {
-        join.valid = 1;
-        join.last_cta = u.last_cta;
-        join.token = u.token;
-        join.hk = u.hk;
-        join.rows[0] = u.rows[0];
-        join.rows[1] = u.rows[1];
-      }
-      q1 += u.narrow || u.rows[1] > 0;
-      if (u.narrow) {
-        narrow_unit<T, kCap, kAlibi>(p, bars, u, sQ + kChunkTileBytes, sV, tmem, t, quarter, lane,
-                                     q1 - 1, sc, g, uc, merges, cta, ok);
-        continue;
-      }
+      if constexpr (kNarrow) {
+        narrow_unit<T, kCap, kAlibi>(p, bars, u, sQ + kChunkTileBytes, sV, tmem, t, quarter, lane, sc,
+                                     g, uc, merges, cta, ok);
+      } else {
       if (rows == 0) {
         g += u.j1 - u.j0;
         continue;
       }
       const bool live = row < rows;             // this row is stored
       const bool warp_live = quarter * 32 < rows;
-      const int tok = row / pb.group, head = u.hk * pb.group + row % pb.group;
+      const int tok = bars->row_token[row], head = u.hk * pb.group + bars->row_head[row];
       const int pos = u.pos + t * pb.tile_tokens + tok;
       float slope2 = 0.f;
       if (kAlibi && live) slope2 = p.f.slopes[head] * kLog2e;
@@ -997,10 +1048,11 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->o_empty[t]);
       ++uc;
+      }
     }
-    if (threadIdx.x == 0) p.join[cta] = join;
   }
 
+  if (p.late_wait && threadIdx.x == 0) grid_dep_wait();
   tc_fence_before();
   named_bar_sync(kCkTeardownBar, kCkThreads);
   if (warp == 0) {
@@ -1010,30 +1062,37 @@ __global__ void __launch_bounds__(kCkThreads, 1)
 }
 
 // Joins the parts of a unit that several CTAs hold: weights 2^(lse_part - max). A warp per row.
+// Blocks [0, ctas) join `p`'s units, blocks [ctas, 2 * ctas) those of `p2`.
 constexpr int kJoinSlices = 8;
 template <typename T>
-__global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p) {
+__global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p,
+                                                            const ChunkParams p2, int ctas) {
   grid_dep_wait();
   grid_dep_launch();
-  const int cta = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const CkJoin jn = p.join[cta];
+  const bool second = (int)blockIdx.x >= ctas;
+  const int cta = blockIdx.x - (second ? ctas : 0), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const CkJoin jn = second ? p2.join[cta] : p.join[cta];
   if (!jn.valid) return;
+  const int rows_cap = second ? p2.rows_cap : p.rows_cap;
+  const float* ws_lse = second ? p2.ws_lse : p.ws_lse;
+  const float* ws_o = second ? p2.ws_o : p.ws_o;
 #pragma unroll 1
-  for (int r = blockIdx.y * 8 + warp; r < 256; r += kJoinSlices * 8) {
+  for (int r = blockIdx.y * 8 + warp; r < rows_cap; r += kJoinSlices * 8) {
     const int t = r >> 7, row = r & 127;
-    if (row >= jn.rows[t]) continue;
-    auto at = [&](int c) { return (int64_t)(c * 2 + (c == cta ? 1 : 0)) * p.rows_cap + r; };
+    if (row >= (t ? jn.rows[1] : jn.rows[0])) continue;
+    auto at = [&](int c) { return (int64_t)(c * 2 + (c == cta ? 1 : 0)) * rows_cap + r; };
     float mx = -INFINITY;
-    for (int c = cta + lane; c <= jn.last_cta; c += 32) mx = fmaxf(mx, p.ws_lse[at(c)]);
+    for (int c = cta + lane; c <= jn.last_cta; c += 32) mx = fmaxf(mx, ws_lse[at(c)]);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
     const bool none = mx == -INFINITY;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float sum = 0.f;
     if (!none) {
+#pragma unroll 4
       for (int c = cta; c <= jn.last_cta; ++c) {
-        const float wgt = exp2f(p.ws_lse[at(c)] - mx);
-        const float4 v = *reinterpret_cast<const float4*>(p.ws_o + at(c) * 128 + lane * 4);
+        const float wgt = exp2f(ws_lse[at(c)] - mx);
+        const float4 v = *reinterpret_cast<const float4*>(ws_o + at(c) * 128 + lane * 4);
         sum += wgt;
         acc.x = fmaf(wgt, v.x, acc.x);
         acc.y = fmaf(wgt, v.y, acc.y);
@@ -1054,47 +1113,69 @@ __global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p)
   }
 }
 
-template <typename T, bool kCap, bool kAlibi>
-static int launch_chunk(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                        const ChunkParams& p, cudaStream_t st) {
+template <typename T, bool kCap, bool kAlibi, bool kNarrow>
+static int launch_main(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                       const ChunkParams& p, cudaStream_t st) {
   static DeviceOnce once;
   cudaError_t e = once.run([] {
     // the register split must fit what the block is launched with, or setmaxnreg would wait
     cudaFuncAttributes a;
-    const cudaError_t e = cudaFuncGetAttributes(&a, paged_chunk_kernel<T, kCap, kAlibi>);
+    const cudaError_t e = cudaFuncGetAttributes(&a, paged_chunk_kernel<T, kCap, kAlibi, kNarrow>);
     if (e != cudaSuccess) return e;
     if (a.numRegs * kCkThreads < 2 * 128 * kCkRegsSoftmax + 128 * kCkRegsOther)
       return cudaErrorInvalidConfiguration;
-    return cudaFuncSetAttribute(paged_chunk_kernel<T, kCap, kAlibi>,
+    return cudaFuncSetAttribute(paged_chunk_kernel<T, kCap, kAlibi, kNarrow>,
                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kCkSmemBytes);
   });
   if (e != cudaSuccess) return cuda_fail(e, "fi_paged_chunk: kernel set-up");
-  const int grid = sm_count();
-  e = launch_pdl(paged_chunk_kernel<T, kCap, kAlibi>, dim3((unsigned)grid), dim3(kCkThreads),
-                 kCkSmemBytes, st, tq, tk, tv, p);
-  if (e != cudaSuccess) return cuda_fail(e, "fi_paged_chunk: launch");
-  e = launch_pdl(chunk_combine_kernel<T>, dim3((unsigned)grid, kJoinSlices), dim3(256), 0, st, p);
-  if (e != cudaSuccess) return cuda_fail(e, "fi_paged_chunk: combine launch");
-  return FI_OK;
+  e = launch_pdl(paged_chunk_kernel<T, kCap, kAlibi, kNarrow>, dim3((unsigned)sm_count()),
+                 dim3(kCkThreads), kCkSmemBytes, st, tq, tk, tv, p);
+  return e == cudaSuccess ? FI_OK : cuda_fail(e, "fi_paged_chunk: launch");
 }
 
+template <typename T, bool kNarrow>
+static int launch_form(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                       const ChunkParams& p, cudaStream_t st) {
+  if (p.f.cap_log2 > 0.f)
+    return p.f.slopes ? launch_main<T, true, true, kNarrow>(tq, tk, tv, p, st)
+                      : launch_main<T, true, false, kNarrow>(tq, tk, tv, p, st);
+  return p.f.slopes ? launch_main<T, false, true, kNarrow>(tq, tk, tv, p, st)
+                    : launch_main<T, false, false, kNarrow>(tq, tk, tv, p, st);
+}
+
+// The narrow kernel, the wide one or both (whichever `narrow` and `wide` name), and the join.
 template <typename T>
-static int launch_chunk_form(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                             const ChunkParams& p, bool cap, cudaStream_t st) {
-  if (cap)
-    return p.f.slopes ? launch_chunk<T, true, true>(tq, tk, tv, p, st)
-                      : launch_chunk<T, true, false>(tq, tk, tv, p, st);
-  return p.f.slopes ? launch_chunk<T, false, true>(tq, tk, tv, p, st)
-                    : launch_chunk<T, false, false>(tq, tk, tv, p, st);
-}
-
-// Rows of a unit that can be live: all of them in one tile when the batch is that small.
-static int64_t ck_rows_cap(int64_t total, int64_t group) {
-  const int64_t tile = kChunkTile / group * group;
-  return total * group <= tile ? total * group : 2 * kChunkTile;
+static int launch_chunk(const CUtensorMap& tq_n, const CUtensorMap& tq_w, const CUtensorMap& tk,
+                        const CUtensorMap& tv, const ChunkParams* narrow, const ChunkParams* wide,
+                        cudaStream_t st) {
+  int r = narrow ? launch_form<T, true>(tq_n, tk, tv, *narrow, st) : FI_OK;
+  if (r == FI_OK && wide) r = launch_form<T, false>(tq_w, tk, tv, *wide, st);
+  if (r != FI_OK) return r;
+  const ChunkParams& first = wide ? *wide : *narrow;
+  const int ctas = sm_count();
+  const cudaError_t e =
+      launch_pdl(chunk_combine_kernel<T>, dim3((unsigned)(narrow && wide ? 2 * ctas : ctas), kJoinSlices),
+                 dim3(256), 0, st, first, narrow ? *narrow : first, ctas);
+  return e == cudaSuccess ? FI_OK : cuda_fail(e, "fi_paged_chunk: combine launch");
 }
 
 static size_t ck_align(size_t n) { return (n + 255) / 256 * 256; }
+
+// One kernel's part of the workspace; `p` null: its size alone.
+static size_t ck_workspace(ChunkParams* p, uint8_t* ws, int rows_cap) {
+  const size_t slots = (size_t)sm_count() * 2 * rows_cap;
+  const size_t o = ck_align(slots * 128 * 4), lse = ck_align(slots * 4);
+  if (p) {
+    p->ws_o = reinterpret_cast<float*>(ws);
+    p->ws_lse = reinterpret_cast<float*>(ws + o);
+    p->join = reinterpret_cast<CkJoin*>(ws + o + lse);
+    p->rows_cap = rows_cap;
+  }
+  return o + lse + ck_align(sm_count() * sizeof(CkJoin));
+}
+
+// Whether every sequence can only have so few rows that the narrow kernel serves the batch.
+static bool ck_all_narrow(int64_t total, int64_t group) { return total * group <= kCkNarrow; }
 
 }  // namespace fi
 
@@ -1105,8 +1186,9 @@ extern "C" size_t fi_paged_chunk_workspace_size(int64_t total_tokens, int64_t nu
       num_q_heads % num_kv_heads != 0 || num_q_heads / num_kv_heads > 64 ||
       total_tokens > (1 << 28))
     return 0;
-  const size_t slots = (size_t)sm_count() * 2 * ck_rows_cap(total_tokens, num_q_heads / num_kv_heads);
-  return ck_align(slots * 128 * 4) + ck_align(slots * 4) + ck_align(sm_count() * sizeof(CkJoin));
+  const size_t narrow = ck_workspace(nullptr, nullptr, kCkNarrow);
+  if (ck_all_narrow(total_tokens, num_q_heads / num_kv_heads)) return narrow;
+  return narrow + ck_workspace(nullptr, nullptr, 2 * kChunkTile);
 }
 
 extern "C" int fi_paged_chunk(const void* q, const void* k_cache, const void* v_cache, void* o,
@@ -1134,7 +1216,13 @@ extern "C" int fi_paged_chunk(const void* q, const void* k_cache, const void* v_
   if (!q || !k_cache || !v_cache || !o || !block_table || !cu_seqlens || !context_lens ||
       !q_strides || !kc_strides || !vc_strides || !o_strides || !bt_strides)
     return fail(FI_ERR_INVALID_ARG, "fi_paged_chunk: null pointer argument");
-  const int64_t unit_tokens = 2 * p.b.tile_tokens;
+  // Batches of few tokens per sequence (on average at most kCkNarrow rows) are the narrow
+  // kernel's alone: a sequence with more tokens is several units there, which read its keys once
+  // each (from L2). One sequence with more is the wide kernel's. Other batches may hold both.
+  const int64_t per_unit = p.b.group <= kCkNarrow ? kCkNarrow / p.b.group : 0;
+  const bool use_narrow = per_unit > 0 && (batch > 1 || total_tokens <= per_unit);
+  const bool use_wide = per_unit == 0 || total_tokens > batch * per_unit;
+  const int64_t unit_tokens = use_wide ? 2 * p.b.tile_tokens : per_unit;
   if (batch > kCkMaxBatch ||
       (total_tokens + unit_tokens - 1) / unit_tokens + batch > kCkMaxUnits)
     return fail(FI_ERR_UNSUPPORTED,
@@ -1153,8 +1241,13 @@ extern "C" int fi_paged_chunk(const void* q, const void* k_cache, const void* v_
     return fail(FI_ERR_ALIGNMENT, "fi_paged_chunk: workspace not 16-byte aligned");
   const CUtensorMapDataType type = dtype == FI_DTYPE_F16 ? Half16<__half>::kTmap
                                                          : Half16<__nv_bfloat16>::kTmap;
-  CUtensorMap tq, tk, tv;
-  if ((r = chunk_q_map(&tq, type, q, p.b, q_strides, "fi_paged_chunk q")) != FI_OK) return r;
+  ChunkParams n = p;  // the narrow kernel's
+  n.b.tile_tokens = per_unit > 0 ? (int)per_unit : 1;
+  CUtensorMap tq_n = {}, tq_w = {}, tk, tv;
+  if (use_narrow && (r = chunk_q_map(&tq_n, type, q, n.b, q_strides, "fi_paged_chunk q")) != FI_OK)
+    return r;
+  if (use_wide && (r = chunk_q_map(&tq_w, type, q, p.b, q_strides, "fi_paged_chunk q")) != FI_OK)
+    return r;
   if ((r = chunk_kv_map(&tk, type, k_cache, p.b, kc_strides, "fi_paged_chunk k_cache")) != FI_OK)
     return r;
   if ((r = chunk_kv_map(&tv, type, v_cache, p.b, vc_strides, "fi_paged_chunk v_cache")) != FI_OK)
@@ -1163,14 +1256,23 @@ extern "C" int fi_paged_chunk(const void* q, const void* k_cache, const void* v_
   p.os[0] = o_strides[0];
   p.os[1] = o_strides[1];
   p.lse = lse;
-  p.rows_cap = (int)ck_rows_cap(total_tokens, p.b.group);
-  const size_t slots = (size_t)sm_count() * 2 * p.rows_cap;
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.ws_o = reinterpret_cast<float*>(ws);
-  p.ws_lse = reinterpret_cast<float*>(ws + ck_align(slots * 128 * 4));
-  p.join = reinterpret_cast<CkJoin*>(ws + ck_align(slots * 128 * 4) + ck_align(slots * 4));
   p.err = error_flag;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  {
+    const ChunkBatch nb = n.b;
+    n = p;
+    n.b = nb;
+  }
+  ws += ck_workspace(&n, ws, kCkNarrow);
+  if (use_wide) ck_workspace(&p, ws, 2 * kChunkTile);
+  n.unit_tokens = (int)per_unit;
+  n.split_rows = use_wide ? kCkNarrow : 0x7fffffff;
+  p.unit_tokens = 2 * p.b.tile_tokens;
+  p.split_rows = use_narrow ? kCkNarrow : 0;
+  p.late_wait = use_narrow;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == FI_DTYPE_F16 ? launch_chunk_form<__half>(tq, tk, tv, p, softcap > 0.f, st)
-                               : launch_chunk_form<__nv_bfloat16>(tq, tk, tv, p, softcap > 0.f, st);
+  const ChunkParams* np = use_narrow ? &n : nullptr;
+  const ChunkParams* wp = use_wide ? &p : nullptr;
+  return dtype == FI_DTYPE_F16 ? launch_chunk<__half>(tq_n, tq_w, tk, tv, np, wp, st)
+                               : launch_chunk<__nv_bfloat16>(tq_n, tq_w, tk, tv, np, wp, st);
 }

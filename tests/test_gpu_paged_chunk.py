@@ -81,6 +81,7 @@ SEQS = {
     "long_chunk": [(300, 700)],
     "decode_batch": [(1, c) for c in (1, 63, 64, 65, 400, 129, 250, 7, 191, 320)],
     "mixed": [(1, 300), (130, 131), (7, 500), (1, 1), (90, 90), (2, 66)],
+    "few_tokens_but_one": [(1, 100)] * 9 + [(60, 300), (0, 5)],
     "cached_missing": [(5, 3), (4, 0), (150, 100)],  # fewer cached tokens than new ones
 }
 
