@@ -8,6 +8,7 @@ symbol is absent, the first call raises ``RuntimeError`` naming the build step.
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 from pathlib import Path
 
@@ -130,7 +131,10 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+@functools.lru_cache(maxsize=4096)
 def strides(*vals) -> ctypes.Array:
+    """int64 array of these values. Arrays are shared between calls (the library only reads
+    them): building one costs more than the rest of an argument check."""
     arr = (ctypes.c_int64 * len(vals))(*[int(v) for v in vals])
     return arr
 

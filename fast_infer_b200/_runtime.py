@@ -28,13 +28,24 @@ def device_checks_enabled() -> bool:
     return _checks
 
 
+_here = contextlib.nullcontext()
+
+
 def with_device(device: torch.device):
     if device.type != "cuda":
         raise ValueError("fast_infer_b200 runs on CUDA devices only")
+    if device.index == torch.cuda.current_device():  # nothing to switch, nothing to restore
+        return _here
     return torch.cuda.device(device)
 
 
+# The stream's handle without building a torch.cuda.Stream around it, where torch has that.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_of(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 

@@ -52,7 +52,7 @@ struct alignas(16) CkUnit {
   int keys, prefix;
   int np, lo;          // step j is key tile j < np ? j : lo + j - np
   int j0, j1, n;
-  int pad;
+  int pages_ok;        // no block-table entry of its keys is invalid
   int last_cta;        // the CTA with the unit's last step
   int valid;           // 0: no unit is left
 };
@@ -122,11 +122,12 @@ __device__ __forceinline__ void ck_tiles(const ChunkBatch& p, const ChunkSeq& s,
   n = np + hi - lo + 1;
 }
 
-// The scheduler (one thread): walks the CTA's part of the line and hands its units to the other
-// roles through a ring in shared memory.
+// The scheduler (one warp): walks the CTA's part of the line and hands its units to the other
+// roles through a ring in shared memory. Its lanes look the units' pages over, so that no one
+// else has to unless an entry is invalid.
 __device__ __forceinline__ void ck_schedule(const ChunkBatch& p, int unit_tokens, CkBarriers* s,
                                             uint32_t units, CkJoin* join_out, int* err) {
-  const int G = gridDim.x, cta = blockIdx.x;
+  const int G = gridDim.x, cta = blockIdx.x, lane = threadIdx.x & 31;
   const uint32_t per_head = s->work[units];
   const int64_t total = (int64_t)per_head * p.hk;
   const int active = (int)(total < G ? total : G);  // CTAs with work
@@ -146,10 +147,12 @@ __device__ __forceinline__ void ck_schedule(const ChunkBatch& p, int unit_tokens
 #pragma unroll 1
   for (int i = 0;; ++i) {
     const int slot = i % kCkSlots;
-    if (i >= kCkSlots && !mbar_wait(&s->unit_empty[slot], ((i / kCkSlots) - 1) & 1, err)) break;
+    if (i >= kCkSlots &&
+        !__all_sync(0xffffffffu, mbar_wait(&s->unit_empty[slot], ((i / kCkSlots) - 1) & 1, err)))
+      break;
     CkUnit u;
     u.valid = w < end;
-    u.pad = 0;
+    bool pages_ok = true;
     if (u.valid) {
       const int t0 = (e - (int)s->unit_off[b]) * unit_tokens, t1 = min(t0 + unit_tokens, q.n);
       ck_tiles(p, q, t0, t1, u.np, u.lo, u.n);
@@ -165,6 +168,11 @@ __device__ __forceinline__ void ck_schedule(const ChunkBatch& p, int unit_tokens
       u.j1 = (int)(u.n - j0 <= end - w ? u.n : j0 + (end - w));
       // the last step of the unit, w - j0 + n - 1, belongs to the last CTA that starts at or before it
       u.last_cta = u.j1 == u.n ? cta : (int)(((w - j0 + u.n) * active - 1) / total);
+      for (int j = u.j0 + (lane >> 1); j < u.j1; j += 16) {
+        const int tile = ck_tile(u, j), half = lane & 1;
+        if ((tile * 2 + half) * kChunkPage < u.keys && chunk_page(p, b, u.keys, tile, half) == p.num_blocks)
+          pages_ok = false;
+      }
       w += u.j1 - u.j0;
       j0 = 0;
       if (++e == (int)units) {
@@ -177,8 +185,11 @@ __device__ __forceinline__ void ck_schedule(const ChunkBatch& p, int unit_tokens
         q = chunk_seq(p, b);
       }
     }
-    s->units[slot] = u;
-    mbar_arrive(&s->unit_full[slot]);  // released to the waits that read it
+    u.pages_ok = __all_sync(0xffffffffu, pages_ok);
+    if (lane == 0) {
+      s->units[slot] = u;
+      mbar_arrive(&s->unit_full[slot]);  // released to the waits that read it
+    }
     if (u.valid && u.j0 == 0 && u.j1 < u.n) {  // begins here and goes on: it is the last one
       join.valid = 1;
       join.last_cta = u.last_cta;
@@ -189,7 +200,7 @@ __device__ __forceinline__ void ck_schedule(const ChunkBatch& p, int unit_tokens
     }
     if (!u.valid) break;
   }
-  *join_out = join;
+  if (lane == 0) *join_out = join;
 }
 
 // The next unit of the ring, null when none is left; it stays in shared memory, read there by
@@ -374,7 +385,8 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
   for (int j = t; j < n; j += 2, ++sc) {
     const int tile = ck_tile(u, u.j0 + j), k0 = tile * kChunkTile, key = k0 + tid;
     const int stage = (g + j) % kCkStages;
-    const bool page_ok = chunk_page(pb, u.b, u.keys, tile, tid >> 6) != pb.num_blocks;
+    const bool page_ok =
+        u.pages_ok || chunk_page(pb, u.b, u.keys, tile, tid >> 6) != pb.num_blocks;
     wait(&bars->s_full[t], sc & 1);
     if (k0 + kChunkTile > u.keys) {
       wait(&bars->v_full[stage], ((g + j) / kCkStages) & 1);
@@ -393,14 +405,16 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
     // the first tile sets the rows' max; later ones keep it unless some score passes it by 2^8
 #pragma unroll 1
     for (bool move = j == t;; move = true) {
+      uint32_t raw[kCkNarrow];
+#pragma unroll
+      for (int cc = 0; cc < kCkNarrow; cc += 8)
+        if (cc < rows) tmem_ld8(tS + cc, raw + cc);
+      tmem_wait_ld();
+      reg_fence<kCkNarrow>(raw);
 #pragma unroll
       for (int cc = 0; cc < kCkNarrow; cc += 8)
         if (cc < rows) {
-          uint32_t raw[8];
-          tmem_ld8(tS + cc, raw);
-          tmem_wait_ld();
-          reg_fence<8>(raw);
-          score_form8<kCap, kAlibi>(raw, s + cc, p.f, bars->n_slope[t] + cc, bars->n_pos[t] + cc,
+          score_form8<kCap, kAlibi>(raw + cc, s + cc, p.f, bars->n_slope[t] + cc, bars->n_pos[t] + cc,
                                      (float)key);
           if (mask) {
             const uint32_t vis = low_bits(c_hi - cc, 0) & ~low_bits(c_lo - cc, 0);
@@ -720,7 +734,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
           ph[1] = next[1];
         }
       }
-    } else if (warp == 10 && lane == 0) {
+    } else if (warp == 10) {
       ck_schedule(pb, p.unit_tokens, bars, units, p.join + cta, p.err);
     } else if (warp == 9 && lane == 0) {
       // ---------------------------------------------------------- UMMA issuer
@@ -908,8 +922,9 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       for (int j = u.j0; j < u.j1; ++j, ++sc, ++g) {
         const int tile = ck_tile(u, j);
         const int k0 = tile * kChunkTile;
-        const bool page0 = chunk_page(pb, u.b, u.keys, tile, 0) != pb.num_blocks;
-        const bool page1 = chunk_page(pb, u.b, u.keys, tile, 1) != pb.num_blocks;
+        // (keys past the context are masked by their number)
+        const bool page0 = u.pages_ok || chunk_page(pb, u.b, u.keys, tile, 0) != pb.num_blocks;
+        const bool page1 = u.pages_ok || chunk_page(pb, u.b, u.keys, tile, 1) != pb.num_blocks;
         wait(&bars->s_full[t], sc & 1);
         if (t == 0 && k0 + kChunkTile > u.keys) {
           wait(&bars->v_full[g % kCkStages], (g / kCkStages) & 1);

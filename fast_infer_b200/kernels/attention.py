@@ -19,6 +19,8 @@ distance bias, a window or a prefix) and ``attention_mass`` (the weight each cac
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from fast_infer_b200 import _lib
@@ -40,9 +42,15 @@ def _check_cuda_f16(name: str, t: torch.Tensor) -> None:
 def _tma_ready(t: torch.Tensor) -> bool:
     """True if the tensor can be addressed by a TMA map as is: 16-byte aligned base,
     unit innermost stride, every other stride a multiple of 8 elements."""
-    if t.data_ptr() % 16 != 0 or t.stride(-1) != 1:
+    if t.data_ptr() % 16 != 0:
         return False
-    return all(s % 8 == 0 or n == 1 for s, n in zip(t.stride()[:-1], t.shape[:-1]))
+    st = t.stride()
+    if st[-1] != 1:
+        return False
+    for i in range(len(st) - 1):
+        if st[i] % 8 != 0 and t.shape[i] != 1:
+            return False
+    return True
 
 
 def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -237,51 +245,77 @@ _DTYPES = {torch.float16: _lib.FI_DTYPE_F16, torch.bfloat16: _lib.FI_DTYPE_BF16}
 
 
 def _int32_on(name: str, t: torch.Tensor, device: torch.device, count: int) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or t.dim() != 1 or t.device != device or t.numel() != count:
+    if not isinstance(t, torch.Tensor) or t.device != device or t.shape != (count,):
         raise ValueError(f"{name} must be a 1-D int32 tensor of {count} values on {device}")
-    return t.to(torch.int32).contiguous()
+    if t.dtype != torch.int32:
+        t = t.to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _chunk_args(q, caches, block_table, block_size, cu_seqlens, context_lens, sm_scale,
+def _check_cache(name: str, t: torch.Tensor, like: torch.Tensor, shape) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (fast_infer_b200 has no CPU path)")
+    if t.dtype != like.dtype:
+        raise TypeError(f"{name} must be float16 or bfloat16 like the new tokens, got {t.dtype}")
+    if t.device != like.device:
+        raise ValueError("all tensors must be on the same device")
+    if t.dim() != 4 or t.shape != shape or t.shape[3] != HEAD_DIM or t.numel() == 0:
+        raise ValueError(f"{name} must be [num_blocks, {BLOCK_SIZE}, num_kv_heads, {HEAD_DIM}]")
+    if not _tma_ready(t):
+        raise ValueError(f"{name} needs a 16-byte aligned base, unit innermost stride and "
+                         "other strides that are multiples of 8")
+
+
+def _check_rows(name: str, t: torch.Tensor) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (fast_infer_b200 has no CPU path)")
+    if t.dtype not in _DTYPES:
+        raise TypeError(f"{name} must be float16 or bfloat16, got {t.dtype}")
+
+
+def _batch_args(device, block_table, block_size, k_cache, cu_seqlens, context_lens):
+    """Checks of the packed batch and its block table; (batch, cu, ctx, table) as the library
+    takes them."""
+    if block_size != BLOCK_SIZE or k_cache.shape[1] != BLOCK_SIZE:
+        raise ValueError(f"block_size must be {BLOCK_SIZE} and match the cache")
+    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.numel() < 1:
+        raise ValueError("cu_seqlens must be a [batch + 1] int32 tensor on the tokens' device")
+    batch = cu_seqlens.numel() - 1
+    cu = _int32_on("cu_seqlens", cu_seqlens, device, batch + 1)
+    ctx = _int32_on("context_lens", context_lens, device, batch)
+    if (not isinstance(block_table, torch.Tensor) or block_table.dim() != 2
+            or block_table.device != device or block_table.shape[0] < batch
+            or block_table.shape[1] == 0):
+        raise ValueError("block_table must be [>= batch, max_blocks_per_seq] on the tokens' device")
+    if block_table.dtype != torch.int32:
+        block_table = block_table.to(torch.int32)
+    return batch, cu, ctx, block_table
+
+
+def _chunk_args(q, k_cache, v_cache, block_table, block_size, cu_seqlens, context_lens, sm_scale,
                 alibi_slopes, prefix_lens):
     """Checks shared by the functions over packed new tokens and a paged cache; returns the
     tensors as the library takes them."""
-    for name, t in (("q", q), *caches):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor")
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor (fast_infer_b200 has no CPU path)")
-        if t.dtype not in _DTYPES or t.dtype != q.dtype:
-            raise TypeError(f"{name} must be float16 or bfloat16 like q, got {t.dtype}")
-        if t.device != q.device:
-            raise ValueError("all tensors must be on the same device")
-    if q.dim() != 3 or q.shape[-1] != HEAD_DIM:
+    _check_rows("q", q)
+    if q.dim() != 3 or q.shape[2] != HEAD_DIM:
         raise ValueError(f"q must be [total_tokens, num_q_heads, {HEAD_DIM}]")
-    num_blocks, bs, num_kv_heads, d = caches[0][1].shape if caches[0][1].dim() == 4 else (0,) * 4
-    if d != HEAD_DIM or any(t.shape != caches[0][1].shape for _, t in caches):
-        raise ValueError(f"caches must be [num_blocks, {BLOCK_SIZE}, num_kv_heads, {HEAD_DIM}]")
-    if block_size != bs or bs != BLOCK_SIZE:
-        raise ValueError(f"block_size must be {BLOCK_SIZE} and match the cache")
-    if num_blocks == 0 or num_kv_heads == 0 or q.shape[1] == 0 or q.shape[1] % num_kv_heads != 0:
-        raise ValueError(f"num_q_heads {q.shape[1]} not a multiple of k/v heads {num_kv_heads}")
-    for name, t in caches:
-        if not _tma_ready(t):
-            raise ValueError(f"{name} needs a 16-byte aligned base, unit innermost stride and "
-                             "other strides that are multiples of 8")
-    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.numel() < 1:
-        raise ValueError("cu_seqlens must be a [batch + 1] int32 tensor on q's device")
-    batch = cu_seqlens.numel() - 1
-    cu = _int32_on("cu_seqlens", cu_seqlens, q.device, batch + 1)
-    ctx = _int32_on("context_lens", context_lens, q.device, batch)
-    prefix = None if prefix_lens is None else _int32_on("prefix_lens", prefix_lens, q.device, batch)
-    if (not isinstance(block_table, torch.Tensor) or block_table.dim() != 2
-            or block_table.device != q.device or block_table.shape[0] < batch
-            or block_table.shape[1] == 0):
-        raise ValueError("block_table must be [>= batch, max_blocks_per_seq] on q's device")
-    bt = block_table.to(torch.int32)
+    shape = k_cache.shape if isinstance(k_cache, torch.Tensor) else None
+    _check_cache("k_cache", k_cache, q, shape)
+    if v_cache is not None:
+        _check_cache("v_cache", v_cache, q, shape)
+    if q.shape[1] == 0 or q.shape[1] % shape[2] != 0:
+        raise ValueError(f"num_q_heads {q.shape[1]} not a multiple of k/v heads {shape[2]}")
+    device = q.device
+    batch, cu, ctx, bt = _batch_args(device, block_table, block_size, k_cache, cu_seqlens,
+                                     context_lens)
+    prefix = None if prefix_lens is None else _int32_on("prefix_lens", prefix_lens, device, batch)
     slopes = None
     if alibi_slopes is not None:
-        if (not isinstance(alibi_slopes, torch.Tensor) or alibi_slopes.device != q.device
+        if (not isinstance(alibi_slopes, torch.Tensor) or alibi_slopes.device != device
                 or alibi_slopes.shape != (q.shape[1],)):
             raise ValueError("alibi_slopes must be a [num_q_heads] float32 tensor on q's device")
         slopes = alibi_slopes.to(torch.float32).contiguous()
@@ -291,6 +325,16 @@ def _chunk_args(q, caches, block_table, block_size, cu_seqlens, context_lens, sm
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+@functools.lru_cache(maxsize=4096)
+def _chunk_workspace(device_index: int, total: int, num_q_heads: int, num_kv_heads: int) -> int:
+    return int(_lib.load().fi_paged_chunk_workspace_size(total, num_q_heads, num_kv_heads))
+
+
+@functools.lru_cache(maxsize=64)
+def _mass_workspace(device_index: int) -> int:
+    return int(_lib.load().fi_attention_mass_workspace_size())
 
 
 def paged_chunk_workspace_bytes(total_tokens: int, num_q_heads: int, num_kv_heads: int) -> int:
@@ -325,8 +369,8 @@ def paged_chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     may run at the same time need one each (the default allocates per call).
     """
     batch, cu, ctx, prefix, bt, slopes, scale = _chunk_args(
-        q, (("k_cache", k_cache), ("v_cache", v_cache)), block_table, block_size, cu_seqlens,
-        context_lens, sm_scale, alibi_slopes, prefix_lens)
+        q, k_cache, v_cache, block_table, block_size, cu_seqlens, context_lens, sm_scale,
+        alibi_slopes, prefix_lens)
     total, num_q_heads, _ = q.shape
     num_blocks, _, num_kv_heads, _ = k_cache.shape
     if out is None:
@@ -340,9 +384,10 @@ def paged_chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
         ox = out if _tma_ready(out) else out.clone(memory_format=torch.contiguous_format)
         lib = _lib.load()
         with with_device(q.device):
-            need = int(lib.fi_paged_chunk_workspace_size(total, num_q_heads, num_kv_heads))
             if workspace is None:
-                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+                workspace = torch.empty(
+                    _chunk_workspace(q.device.index, total, num_q_heads, num_kv_heads),
+                    dtype=torch.uint8, device=q.device)
             elif workspace.device != q.device or not workspace.is_contiguous():
                 raise ValueError("workspace must be contiguous on q's device")
             err = error_word(q.device)
@@ -378,8 +423,10 @@ def attention_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Te
     ``workspace``: uint8, at least ``attention_mass_workspace_bytes`` bytes; calls that may run at
     the same time need one each (the default allocates per call).
     """
+    if k_cache is None:
+        raise TypeError("k_cache must be a torch.Tensor")
     batch, cu, ctx, prefix, bt, slopes, scale = _chunk_args(
-        q, (("k_cache", k_cache),), block_table, block_size, cu_seqlens, context_lens, sm_scale,
+        q, k_cache, None, block_table, block_size, cu_seqlens, context_lens, sm_scale,
         alibi_slopes, prefix_lens)
     total, num_q_heads, _ = q.shape
     num_blocks, _, num_kv_heads, _ = k_cache.shape
@@ -401,7 +448,7 @@ def attention_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Te
     lib = _lib.load()
     with with_device(q.device):
         if workspace is None:
-            workspace = torch.empty(attention_mass_workspace_bytes(), dtype=torch.uint8,
+            workspace = torch.empty(_mass_workspace(q.device.index), dtype=torch.uint8,
                                     device=q.device)
         elif workspace.device != q.device or not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous on q's device")

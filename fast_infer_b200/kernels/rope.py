@@ -14,8 +14,8 @@ import torch
 
 from fast_infer_b200 import _lib
 from fast_infer_b200._runtime import device_errors, error_word, stream_of, with_device
-from fast_infer_b200.kernels.attention import (_DTYPES, BLOCK_SIZE, HEAD_DIM, _int32_on,
-                                               _tma_ready)
+from fast_infer_b200.kernels.attention import (_DTYPES, HEAD_DIM, _batch_args, _check_cache,
+                                               _check_rows, _tma_ready)
 
 
 def rope_axes_store(qkv: torch.Tensor, num_q_heads: int, cos_table: torch.Tensor,
@@ -34,23 +34,10 @@ def rope_axes_store(qkv: torch.Tensor, num_q_heads: int, cos_table: torch.Tensor
     The rotation is the rotate-half form in fp32, rounded once. Returns the rotated q
     [total_tokens, nq, 128] (``q_out`` if given; rows outside every sequence are not written).
     """
-    if not isinstance(qkv, torch.Tensor):
-        raise TypeError("qkv must be a torch.Tensor")
-    if not qkv.is_cuda:
-        raise ValueError("qkv must be a CUDA tensor (fast_infer_b200 has no CPU path)")
-    if qkv.dtype not in _DTYPES:
-        raise TypeError(f"qkv must be float16 or bfloat16, got {qkv.dtype}")
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if not isinstance(t, torch.Tensor) or t.dtype != qkv.dtype or t.device != qkv.device:
-            raise ValueError(f"{name} must have qkv's type and device")
-        if t.dim() != 4 or t.shape != k_cache.shape or t.shape[1] != BLOCK_SIZE \
-                or t.shape[3] != HEAD_DIM or t.numel() == 0:
-            raise ValueError(f"{name} must be [num_blocks, {BLOCK_SIZE}, num_kv_heads, {HEAD_DIM}]")
-        if not _tma_ready(t):
-            raise ValueError(f"{name} needs a 16-byte aligned base, unit innermost stride and "
-                             "other strides that are multiples of 8")
-    if block_size != BLOCK_SIZE:
-        raise ValueError(f"block_size must be {BLOCK_SIZE}")
+    _check_rows("qkv", qkv)
+    shape = k_cache.shape if isinstance(k_cache, torch.Tensor) else None
+    _check_cache("k_cache", k_cache, qkv, shape)
+    _check_cache("v_cache", v_cache, qkv, shape)
     num_blocks, _, nkv, _ = k_cache.shape
     if num_q_heads < 1 or qkv.dim() != 2 or qkv.shape[1] != (num_q_heads + 2 * nkv) * HEAD_DIM:
         raise ValueError("qkv must be [total_tokens, (num_q_heads + 2 * num_kv_heads) * head_dim]")
@@ -68,15 +55,8 @@ def rope_axes_store(qkv: torch.Tensor, num_q_heads: int, cos_table: torch.Tensor
                 or t.shape != cos_table.shape or t.stride(0) != cos_table.stride(0)
                 or t.shape[0] == 0):
             raise ValueError(f"{name} must be a float32 [max_pos, {HEAD_DIM}] table on qkv's device")
-    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.numel() < 1:
-        raise ValueError("cu_seqlens must be a [batch + 1] int32 tensor on qkv's device")
-    batch = cu_seqlens.numel() - 1
-    cu = _int32_on("cu_seqlens", cu_seqlens, qkv.device, batch + 1)
-    ctx = _int32_on("context_lens", context_lens, qkv.device, batch)
-    if (not isinstance(block_table, torch.Tensor) or block_table.dim() != 2
-            or block_table.device != qkv.device or block_table.shape[0] < batch
-            or block_table.shape[1] == 0):
-        raise ValueError("block_table must be [>= batch, max_blocks_per_seq] on qkv's device")
+    batch, cu, ctx, bt = _batch_args(qkv.device, block_table, block_size, k_cache, cu_seqlens,
+                                     context_lens)
     if q_out is None:
         q_out = torch.empty(total, num_q_heads, HEAD_DIM, dtype=qkv.dtype, device=qkv.device)
     elif (q_out.shape != (total, num_q_heads, HEAD_DIM) or q_out.dtype != qkv.dtype
@@ -86,10 +66,9 @@ def rope_axes_store(qkv: torch.Tensor, num_q_heads: int, cos_table: torch.Tensor
     if batch == 0 or total == 0:
         return q_out
     x = qkv if _tma_ready(qkv) else qkv.clone(memory_format=torch.contiguous_format)
-    pos = positions.to(torch.int32)
+    pos = positions if positions.dtype == torch.int32 else positions.to(torch.int32)
     if pos.stride(1) != 1:
         pos = pos.contiguous()
-    bt = block_table.to(torch.int32)
     table_stride = cos_table.stride(0) if cos_table.shape[0] > 1 else HEAD_DIM
     lib = _lib.load()
     with with_device(qkv.device):
