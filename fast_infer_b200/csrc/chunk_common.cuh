@@ -141,6 +141,28 @@ __device__ __forceinline__ uint64_t exp2_poly5_x2(uint64_t x2) {
                __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23)));
 }
 
+__device__ __forceinline__ float exp2_poly5(float x) {  // the same for one value
+  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23
+  x = fmaxf(x, -127.0f);
+  const float t = x + kMagic, f = x - (t - kMagic);
+  float q = fmaf(kExp5, f, kExp4);
+  q = fmaf(q, f, kExp3);
+  q = fmaf(q, f, kExp2);
+  q = fmaf(q, f, kExp1);
+  q = fmaf(q, f, 1.0f);
+  return __uint_as_float(__float_as_uint(q) + (__float_as_uint(t) << 23));
+}
+__device__ __forceinline__ float tanh_poly(float u) {  // tanh_poly_x2 for one value
+  const float z = u * u;
+  float q = fmaf(kTanh6, z, kTanh5);
+  q = fmaf(q, z, kTanh4);
+  q = fmaf(q, z, kTanh3);
+  q = fmaf(q, z, kTanh2);
+  q = fmaf(q, z, kTanh1);
+  q = fmaf(q, z, kTanh0);
+  return q * u;
+}
+
 // Inclusive sums of a[1..n] in place (a[0] stays); every thread of the block calls it.
 // `warp_sums`: one word per warp. Each thread owns a run of consecutive entries.
 template <typename U>

@@ -9,29 +9,32 @@
 // Design:
 // * The product is transposed, S^T = K Q^T: keys are the 128 tensor-memory lanes, so a thread
 //   owns one key and sums over the columns (query rows) in registers: no atomics.
-// * A unit is 256 consecutive keys (two tiles) of one sequence and KV head; its steps are the
-//   128-row query tiles that see any of them. The launch's line of (KV head, sequence, unit,
-//   step) is cut into equal parts, one per CTA; a unit cut between CTAs leaves 256 partial
-//   sums each, joined by mass_join_kernel in CTA order (the same bits on every run). One new
-//   token per sequence makes it a stream over K; a whole chunk a stream over Q with K resident.
-// * What bounds a step of 256 keys x 128 rows is its 32768 exponentials (2048 cycles of the SM's
-//   MUFU, against 1024 of the tensor core): 3 of 8 pairs take a polynomial on the FMA pipe.
-// * Roles (640 threads): warps 0-15 = the sums, four warpgroups = two key tiles x two halves of
-//   the columns (four warps per scheduler, or their latencies would show: eight warps took twice
-//   the time), warp 16 = TMA, warp 17 = UMMA issue, warp 18 = the rows' lse (and slopes and
-//   positions) into shared memory, warp 19 = scheduler, then zeros where no new token sees.
-//   Tensor memory: two S buffers per key tile.
+// * A unit is 512 consecutive keys (four tiles) of one sequence and KV head, 256 where sequences
+//   have few new tokens; its steps are the 128-row query tiles that see any of them. The
+//   launch's line of (KV head, sequence, unit, step) is cut into equal parts, one per CTA; a unit
+//   cut between CTAs leaves a partial sum per key each, joined by mass_join_kernel in CTA order
+//   (the same bits on every run). One new token per sequence makes it a stream over K, each
+//   tile reloaded as soon as its product is done; a whole chunk a stream over Q with K resident.
+// * What bounds a chunk's step of 512 keys x 128 rows: its 65536 exponentials (4096 cycles of the
+//   SM's MUFU, against 2048 of the tensor core), of which some run as a polynomial on the FMA
+//   pipe, and the query tile's 32 KB from L2 (units of 256 keys read 6.3 TB/s of them on the
+//   whole GPU and were bound by that).
+// * Roles (640 threads): warps 0-15 = the sums, a warpgroup per key tile (one per warp scheduler
+//   would show its latencies: eight warps took twice the time), warp 16 = TMA, warp 17 = UMMA
+//   issue, warp 18 = the rows' lse (and slopes and positions) into shared memory, warp 19 =
+//   scheduler, then zeros where no new token sees. Tensor memory: S of each key tile.
 #include "chunk_common.cuh"
 
 namespace fi {
 
 constexpr int kMsThreads = 640;
-constexpr int kMsStages = 2;         // K (256 keys) and Q ring slots
-constexpr int kMsKeys = 256;         // keys of a unit
+constexpr int kMsTiles = 4;          // key tiles in shared memory, a warpgroup each
+constexpr int kMsKeys = kMsTiles * kChunkTile;  // most keys of a unit
+constexpr int kMsQ = 2;              // ring slots of query tiles
 constexpr int kMsMaxBatch = 2048;
-constexpr int kMsEmuPairs = 3;       // of 8 column pairs, exp2 on the FMA pipe
+constexpr int kMsEmu = 2;            // of 16 columns, exp2 on the FMA pipe
+constexpr int kMsRows = 4;           // ring slots of the rows' lse
 constexpr int kMsSlots = 4;          // units that the scheduler is ahead
-constexpr int kMsParts = 4;          // unit sums of the second column half in flight
 
 // A CTA's part of a unit: query tiles [q0, q1).
 struct alignas(16) MsUnit {
@@ -48,23 +51,22 @@ struct alignas(16) MsUnit {
 };
 
 struct MsBarriers {
-  uint64_t k_full[kMsStages], k_empty[kMsStages];
-  uint64_t q_full[kMsStages], q_empty[kMsStages];
-  uint64_t s_full[2][2], s_empty[2][2];  // [key tile][buffer]
-  uint64_t part_full[2][kMsParts];       // [key tile]
+  uint64_t k_full[kMsTiles], k_empty[kMsTiles];
+  uint64_t q_full[kMsQ], q_empty[kMsQ];
+  uint64_t l_full[kMsRows], l_empty[kMsRows];
+  uint64_t s_full[kMsTiles], s_empty[kMsTiles];
   uint64_t unit_full[kMsSlots], unit_empty[kMsSlots];
   uint64_t mma_done;
   uint64_t seq[kMsMaxBatch + 1];         // steps before each sequence
   uint64_t warp_sums[kMsThreads / 32];
   uint32_t tmem_base;
   MsUnit units[kMsSlots];
-  alignas(16) float neg_lse[kMsStages][kChunkTile];  // -lse * log2(e), -inf: no such row
-  alignas(16) float slope[kMsStages][kChunkTile];    // distance bias, log2 units
-  alignas(16) float pos[kMsStages][kChunkTile];
-  float part[2][kMsParts][kChunkTile];   // sums of the second column half
+  alignas(16) float neg_lse[kMsRows][kChunkTile];  // -lse * log2(e), -inf: no such row
+  alignas(16) float slope[kMsRows][kChunkTile];    // distance bias, log2 units
+  alignas(16) float pos[kMsRows][kChunkTile];
 };
 constexpr int kMsSmemBytes =
-    1024 + kMsStages * 3 * kChunkTileBytes + (int)sizeof(MsBarriers);
+    1024 + (kMsTiles + kMsQ) * kChunkTileBytes + (int)sizeof(MsBarriers);
 static_assert(kMsSmemBytes <= 227 * 1024, "shared memory");
 
 struct MsJoin {
@@ -80,15 +82,16 @@ struct MassParams {
   float* mass;       // [batch, hk, cap]
   int64_t cap;
   int accumulate;
-  float* ws;     // [cta][first, last unit][256]
+  float* ws;     // [cta][first, last unit][kMsKeys]
   MsJoin* join;  // [cta]
+  int tiles;     // key tiles of a unit: 4, or 2
   int* err;
 };
 
 // Query tiles [a, b) that see any key of unit u.
-__device__ __forceinline__ void ms_steps(const ChunkBatch& p, const ChunkSeq& s, int u, int& a,
-                                         int& b) {
-  const int k0 = u * kMsKeys, k1 = min(k0 + kMsKeys, s.keys) - 1;
+__device__ __forceinline__ void ms_steps(const ChunkBatch& p, const ChunkSeq& s, int keys, int u,
+                                         int& a, int& b) {
+  const int k0 = u * keys, k1 = min(k0 + keys, s.keys) - 1;
   int lo = 0, hi = s.n;
   if (k0 >= s.prefix) {
     lo = max(k0 - s.pos0, 0);
@@ -97,14 +100,28 @@ __device__ __forceinline__ void ms_steps(const ChunkBatch& p, const ChunkSeq& s,
   a = lo / p.tile_tokens;
   b = lo < hi ? (hi - 1) / p.tile_tokens + 1 : a;
 }
-__device__ __forceinline__ int ms_units(const ChunkSeq& s) {
-  return (s.keys + kMsKeys - 1) / kMsKeys;
+__device__ __forceinline__ int ms_units(const ChunkSeq& s, int keys) {
+  return (s.keys + keys - 1) / keys;
 }
+
+// Place in a ring of mbarriers: a slot and the parity of its current phase. The side that fills
+// waits for parity ^ 1, which a fresh barrier has passed.
+struct MsRing {
+  int i = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next(int n) {
+    if (++i == n) {
+      i = 0;
+      parity ^= 1;
+    }
+  }
+};
 
 // The scheduler (one warp): walks the CTA's part of the line and hands its units to the other
 // roles through a ring in shared memory.
-__device__ __forceinline__ void ms_schedule(const ChunkBatch& p, MsBarriers* m, int64_t cap,
-                                            MsJoin* join_out, int* err) {
+__device__ __forceinline__ void ms_schedule(const ChunkBatch& p, MsBarriers* m, int ktiles,
+                                            int64_t cap, MsJoin* join_out, int* err) {
+  const int ukeys = ktiles * kChunkTile;
   const int G = gridDim.x, cta = blockIdx.x, lane = threadIdx.x & 31;
   const int64_t per_head = (int64_t)m->seq[p.batch];
   const int64_t total = per_head * p.hk;
@@ -123,7 +140,7 @@ __device__ __forceinline__ void ms_schedule(const ChunkBatch& p, MsBarriers* m, 
 #pragma unroll 1
     for (int base = 0;; base += 32) {  // the unit that holds step r of the sequence
       int a = 0, e = 0;
-      if (base + lane < ms_units(s)) ms_steps(p, s, base + lane, a, e);
+      if (base + lane < ms_units(s, ukeys)) ms_steps(p, s, ukeys, base + lane, a, e);
       uint64_t inc = (uint64_t)(e - a);
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
@@ -155,7 +172,7 @@ __device__ __forceinline__ void ms_schedule(const ChunkBatch& p, MsBarriers* m, 
     if (v.valid) {
       int a, e;
       while (true) {  // the line holds only units with steps
-        ms_steps(p, s, u, a, e);
+        ms_steps(p, s, ukeys, u, a, e);
         if (e > a) break;
         ++u;
       }
@@ -174,15 +191,15 @@ __device__ __forceinline__ void ms_schedule(const ChunkBatch& p, MsBarriers* m, 
       v.fresh = fresh;
       v.begins = skip == 0;
       v.whole = v.begins && v.q1 == e;
-      if (lane < 4 && (u * 4 + lane) * kChunkPage < s.keys)
-        pages_ok = chunk_page(p, b, s.keys, u * 2 + (lane >> 1), lane & 1) != p.num_blocks;
+      if (lane < 2 * ktiles && (u * 2 * ktiles + lane) * kChunkPage < s.keys)
+        pages_ok = chunk_page(p, b, s.keys, u * ktiles + (lane >> 1), lane & 1) != p.num_blocks;
       if (v.begins && !v.whole) {  // it goes on in the next CTA: the last one here
         const int64_t keys = min((int64_t)s.keys, cap);
         join.valid = 1;
         join.last_cta = (int)(((w + n) * active - 1) / total);
-        join.keys = (int)min(keys - u * (int64_t)kMsKeys, (int64_t)kMsKeys);
-        join.span = (int)min(cap - u * (int64_t)kMsKeys, (int64_t)kMsKeys);
-        join.at = ((int64_t)b * p.hk + hk) * cap + u * (int64_t)kMsKeys;
+        join.keys = (int)min(keys - u * (int64_t)ukeys, (int64_t)ukeys);
+        join.span = (int)min(cap - u * (int64_t)ukeys, (int64_t)ukeys);
+        join.at = ((int64_t)b * p.hk + hk) * cap + u * (int64_t)ukeys;
       }
       w += v.q1 - v.q0;
       skip = 0;
@@ -233,9 +250,10 @@ __global__ void __launch_bounds__(kMsThreads, 1)
                       const __grid_constant__ CUtensorMap tm_k, const MassParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_align1024(smem_raw);
-  uint8_t* sK = smem;                                      // [stage][2 tiles]
-  uint8_t* sQ = smem + kMsStages * 2 * kChunkTileBytes;    // [stage]
-  MsBarriers* bars = reinterpret_cast<MsBarriers*>(sQ + kMsStages * kChunkTileBytes);
+  uint8_t* sK = smem;                                // [tile]
+  uint8_t* sQ = smem + kMsTiles * kChunkTileBytes;   // [slot]
+  MsBarriers* bars = reinterpret_cast<MsBarriers*>(sQ + kMsQ * kChunkTileBytes);
+  const int ktiles = p.tiles, ukeys = ktiles * kChunkTile;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = blockIdx.x;
   const ChunkBatch& pb = p.b;
@@ -246,18 +264,19 @@ __global__ void __launch_bounds__(kMsThreads, 1)
     tmem_relinquish();
   }
   if (threadIdx.x == 32) {
-    for (int s = 0; s < kMsStages; ++s) {
+    for (int s = 0; s < kMsTiles; ++s) {
       mbar_init(&bars->k_full[s], 1);
       mbar_init(&bars->k_empty[s], 1);
-      mbar_init(&bars->q_full[s], 2);    // TMA, warp 18
-      mbar_init(&bars->q_empty[s], 17);  // UMMA, the 16 summing warps
+      mbar_init(&bars->s_full[s], 1);
+      mbar_init(&bars->s_empty[s], 4);
     }
-    for (int t = 0; t < 2; ++t) {
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&bars->s_full[t][i], 1);
-        mbar_init(&bars->s_empty[t][i], 8);
-      }
-      for (int i = 0; i < kMsParts; ++i) mbar_init(&bars->part_full[t][i], 4);
+    for (int s = 0; s < kMsQ; ++s) {
+      mbar_init(&bars->q_full[s], 1);
+      mbar_init(&bars->q_empty[s], 1);
+    }
+    for (int s = 0; s < kMsRows; ++s) {
+      mbar_init(&bars->l_full[s], 1);
+      mbar_init(&bars->l_empty[s], 16);
     }
     for (int i = 0; i < kMsSlots; ++i) {
       mbar_init(&bars->unit_full[i], 1);
@@ -268,7 +287,7 @@ __global__ void __launch_bounds__(kMsThreads, 1)
   }
   // Query rows that TMA never writes: zeros, so that their columns hold finite scores.
 #pragma unroll 1
-  for (int i = threadIdx.x; i < kMsStages * 2 * (kChunkTile - tile_rows) * 8; i += kMsThreads) {
+  for (int i = threadIdx.x; i < kMsQ * 2 * (kChunkTile - tile_rows) * 8; i += kMsThreads) {
     const int part = i / ((kChunkTile - tile_rows) * 8), k = i % ((kChunkTile - tile_rows) * 8);
     *reinterpret_cast<uint4*>(sQ + part * kChunkHalf + tile_rows * 128 + k * 16) =
         make_uint4(0, 0, 0, 0);
@@ -286,9 +305,9 @@ __global__ void __launch_bounds__(kMsThreads, 1)
     uint64_t steps = 0;
     if (s.n > 0) {
 #pragma unroll 1
-      for (int u = lane; u < ms_units(s); u += 32) {
+      for (int u = lane; u < ms_units(s, ukeys); u += 32) {
         int a, e;
-        ms_steps(pb, s, u, a, e);
+        ms_steps(pb, s, ukeys, u, a, e);
         steps += e - a;
       }
     }
@@ -308,86 +327,99 @@ __global__ void __launch_bounds__(kMsThreads, 1)
       // ---------------------------------------------------------- TMA producer
       prefetch_tmap(&tm_q);
       prefetch_tmap(&tm_k);
-      int kc = 0, qc = 0, next_unit = 0;
+      int tile = 0, next_unit = 0;  // key tiles loaded: tile i goes to slot i % kMsTiles
+      uint32_t k_parity = 1;        // of the slots' current round
+      MsRing qr;
       bool ok = true;
 #pragma unroll 1
       for (const MsUnit* up; ok && (up = ms_next<false>(bars, next_unit, p.err)) != nullptr;
            ms_done<false>(bars, next_unit)) {
         const MsUnit& u = *up;
-        int ph[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          ph[i] = chunk_page(pb, u.b, u.keys, u.u * 2 + (i >> 1), i & 1);
-          if (ph[i] == pb.num_blocks && (u.u * 4 + i) * kChunkPage < u.keys)
-            set_error(p.err, FI_DEVERR_BAD_BLOCK);
-        }
-        const int ks = kc % kMsStages;
-        if (kc >= kMsStages && !(ok = mbar_wait(&bars->k_empty[ks], ((kc / kMsStages) - 1) & 1, p.err)))
-          break;
-        ++kc;
-        mbar_arrive_expect_tx(&bars->k_full[ks], 2 * kChunkTileBytes);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint8_t* dst = sK + (ks * 2 + (i >> 1)) * kChunkTileBytes + (i & 1) * (kChunkHalf / 2);
-          tma_load_4d(dst, &tm_k, &bars->k_full[ks], 0, u.hk, 0, ph[i]);
-          tma_load_4d(dst + kChunkHalf, &tm_k, &bars->k_full[ks], 64, u.hk, 0, ph[i]);
-        }
-        if (!ms_loads(u)) continue;
-#pragma unroll 1
-        for (int q = u.q0; q < u.q1; ++q) {
-          const int qs = qc % kMsStages;
-          if (qc >= kMsStages && !(ok = mbar_wait(&bars->q_empty[qs], ((qc / kMsStages) - 1) & 1, p.err)))
-            break;
-          ++qc;
+        const bool loads = ms_loads(u);
+        auto load_q = [&](int q) {
+          const int qs = qr.i;
+          if (!(ok = mbar_wait(&bars->q_empty[qs], qr.parity ^ 1, p.err))) return;
+          qr.next(kMsQ);
           const int token = u.start + q * pb.tile_tokens;
           uint8_t* dst = sQ + qs * kChunkTileBytes;
           mbar_arrive_expect_tx(&bars->q_full[qs], (uint32_t)(tile_rows * 256));
           tma_load_4d(dst, &tm_q, &bars->q_full[qs], 0, 0, u.hk, token);
           tma_load_4d(dst + kChunkHalf, &tm_q, &bars->q_full[qs], 64, 0, u.hk, token);
+        };
+#pragma unroll 1
+        for (int t = 0; ok && t < ktiles; ++t) {
+          int ph[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            ph[i] = chunk_page(pb, u.b, u.keys, u.u * ktiles + t, i);
+            if (ph[i] == pb.num_blocks && ((u.u * ktiles + t) * 2 + i) * kChunkPage < u.keys)
+              set_error(p.err, FI_DEVERR_BAD_BLOCK);
+          }
+          const int slot = tile % kMsTiles;
+          if (!(ok = mbar_wait(&bars->k_empty[slot], k_parity, p.err))) break;
+          if (++tile % kMsTiles == 0) k_parity ^= 1;
+          mbar_arrive_expect_tx(&bars->k_full[slot], kChunkTileBytes);
+          uint8_t* dst = sK + slot * kChunkTileBytes;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            tma_load_4d(dst + i * (kChunkHalf / 2), &tm_k, &bars->k_full[slot], 0, u.hk, 0, ph[i]);
+            tma_load_4d(dst + kChunkHalf + i * (kChunkHalf / 2), &tm_k, &bars->k_full[slot], 64,
+                        u.hk, 0, ph[i]);
+          }
+          // the first query tile goes out behind the first key tile: the slots of the others may
+          // have to wait for the unit before
+          if (t == 0 && loads) load_q(u.q0);
         }
+        if (!loads) continue;
+#pragma unroll 1
+        for (int q = u.q0 + 1; ok && q < u.q1; ++q) load_q(q);
       }
     }
   } else if (warp == 17) {
     if (lane == 0) {
       // ---------------------------------------------------------- UMMA issuer
       const uint32_t k_addr = smem_u32(sK), q_addr = smem_u32(sQ);
-      int kc = 0, qc = 0, sc = 0, next_unit = 0;
+      int tile = 0, next_unit = 0, qs = 0;
+      uint32_t k_parity = 0;
+      uint32_t s_parity = (1u << kMsTiles) - 1;  // of each slot's s_empty
+      MsRing qr;
       bool ok = true;
 #pragma unroll 1
       for (const MsUnit* up; ok && (up = ms_next<false>(bars, next_unit, p.err)) != nullptr;
            ms_done<false>(bars, next_unit)) {
         const MsUnit& u = *up;
-        const int ks = kc % kMsStages;
-        if (!(ok = mbar_wait(&bars->k_full[ks], (kc / kMsStages) & 1, p.err))) break;
-        ++kc;
+        const int slot0 = tile % kMsTiles;
 #pragma unroll 1
-        for (int q = u.q0; q < u.q1; ++q, ++sc) {
+        for (int q = u.q0; ok && q < u.q1; ++q) {
           if (ms_loads(u)) {
-            if (!(ok = mbar_wait(&bars->q_full[qc % kMsStages], (qc / kMsStages) & 1, p.err))) break;
-            ++qc;
+            qs = qr.i;
+            if (!(ok = mbar_wait(&bars->q_full[qs], qr.parity, p.err))) break;
+            qr.next(kMsQ);
           }
-          const int qs = (qc - 1) % kMsStages, buf = sc & 1;
           const int rows = min(u.n - q * pb.tile_tokens, pb.tile_tokens) * pb.group;
           const uint32_t idesc = umma_idesc<T>(128, (uint32_t)(rows + 15) / 16 * 16, 0, 0);
           const uint64_t db = umma_desc_sw128(q_addr + qs * kChunkTileBytes, 16, 1024);
 #pragma unroll 1
-          for (int t = 0; t < 2 && ok; ++t) {
-            if (sc >= 2) ok = mbar_wait(&bars->s_empty[t][buf], ((sc >> 1) - 1) & 1, p.err);
+          for (int t = 0; ok && t < ktiles; ++t) {
+            const int slot = slot0 + t;
+            if (q == u.q0) ok = mbar_wait(&bars->k_full[slot], k_parity, p.err);
+            ok = ok && mbar_wait(&bars->s_empty[slot], (s_parity >> slot) & 1, p.err);
             if (!ok) break;
+            s_parity ^= 1u << slot;
             tc_fence_after();
-            const uint64_t da = umma_desc_sw128(k_addr + (ks * 2 + t) * kChunkTileBytes, 16, 1024);
+            const uint64_t da = umma_desc_sw128(k_addr + slot * kChunkTileBytes, 16, 1024);
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk) {
               const uint32_t off = ((kk >> 2) * kChunkHalf + (kk & 3) * 32) >> 4;
-              umma_ss(tmem + (t * 2 + buf) * 128, da + off, db + off, idesc, kk > 0);
+              umma_ss(tmem + slot * 128, da + off, db + off, idesc, kk > 0);
             }
-            umma_commit(&bars->s_full[t][buf]);
+            umma_commit(&bars->s_full[slot]);
+            if (q == u.q1 - 1) umma_commit(&bars->k_empty[slot]);
           }
-          if (!ok) break;
-          if (ms_frees(u)) umma_commit(&bars->q_empty[qs]);
+          if (ok && ms_frees(u)) umma_commit(&bars->q_empty[qs]);
         }
-        if (!ok) break;
-        umma_commit(&bars->k_empty[ks]);
+        tile += ktiles;
+        if (tile % kMsTiles == 0) k_parity ^= 1;
       }
       umma_commit(&bars->mma_done);
       mbar_wait(&bars->mma_done, 0, p.err);
@@ -396,49 +428,60 @@ __global__ void __launch_bounds__(kMsThreads, 1)
     // -------------------------------------------------- the rows' lse, a column each
     int qc = 0, next_unit = 0;
     bool ok = true;
+    int tok[4], head[4];  // of this lane's columns, -1: no row of a tile
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = lane + 32 * i;
+      tok[i] = c < tile_rows ? c / pb.group : -1;
+      head[i] = c % pb.group;
+    }
 #pragma unroll 1
     for (const MsUnit* up; ok && (up = ms_next<true>(bars, next_unit, p.err)) != nullptr;
          ms_done<true>(bars, next_unit)) {
       const MsUnit& u = *up;
       if (!ms_loads(u)) continue;
-#pragma unroll 1
-      for (int q = u.q0; ok && q < u.q1; ++q) {
-        const int qs = qc % kMsStages;
-        float nl[4], sl[4], ps[4];
+      const float* lse = p.lse + (int64_t)u.start * pb.hq + u.hk * pb.group;
+      // a tile's values are read while the one before waits for its slot
+      auto load = [&](int q, float* v) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int c = lane + 32 * i, tok = q * pb.tile_tokens + c / pb.group;
-          const int head = u.hk * pb.group + c % pb.group;
-          nl[i] = -INFINITY;
-          sl[i] = ps[i] = 0.f;
-          if (c < tile_rows && tok < u.n) {
-            const float v = p.lse[(int64_t)(u.start + tok) * pb.hq + head];
-            if (v != -INFINITY) nl[i] = -v * kLog2e;
-            if (kAlibi) {
-              sl[i] = p.f.slopes[head] * kLog2e;
-              ps[i] = (float)(u.pos0 + tok);
-            }
-          }
+          const int k = q * pb.tile_tokens + tok[i];
+          v[i] = -INFINITY;
+          if (tok[i] >= 0 && q < u.q1 && k < u.n) v[i] = lse[(int64_t)k * pb.hq + head[i]];
         }
-        if (qc >= kMsStages)
+      };
+      float now[4], next[4], sl[4];
+      load(u.q0, now);
+      if (kAlibi) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          sl[i] = tok[i] >= 0 ? p.f.slopes[u.hk * pb.group + head[i]] * kLog2e : 0.f;
+      }
+#pragma unroll 1
+      for (int q = u.q0; q < u.q1; ++q) {
+        load(q + 1, next);
+        const int ls = qc % kMsRows;
+        if (qc >= kMsRows)
           ok = __all_sync(0xffffffffu,
-                          mbar_wait(&bars->q_empty[qs], ((qc / kMsStages) - 1) & 1, p.err));
+                          mbar_wait(&bars->l_empty[ls], ((qc / kMsRows) - 1) & 1, p.err));
         if (!ok) break;
         ++qc;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          bars->neg_lse[qs][lane + 32 * i] = nl[i];
+          const int c = lane + 32 * i;
+          bars->neg_lse[ls][c] = now[i] == -INFINITY ? -INFINITY : -now[i] * kLog2e;
           if (kAlibi) {
-            bars->slope[qs][lane + 32 * i] = sl[i];
-            bars->pos[qs][lane + 32 * i] = ps[i];
+            bars->slope[ls][c] = sl[i];
+            bars->pos[ls][c] = (float)(u.pos0 + q * pb.tile_tokens + tok[i]);
           }
+          now[i] = next[i];
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->q_full[qs]);
+        if (lane == 0) mbar_arrive(&bars->l_full[ls]);
       }
     }
   } else if (warp == 19) {
-    ms_schedule(pb, bars, p.cap, p.join + cta, p.err);
+    ms_schedule(pb, bars, ktiles, p.cap, p.join + cta, p.err);
     // zeros where no new token sees (unless the call adds to mass)
     if (!p.accumulate) {
 #pragma unroll 1
@@ -446,21 +489,21 @@ __global__ void __launch_bounds__(kMsThreads, 1)
         const ChunkSeq s = chunk_seq(pb, (int)(r / pb.hk));
         float* row = p.mass + r * p.cap;
 #pragma unroll 1
-        for (int64_t k0 = 0; k0 < p.cap; k0 += kMsKeys) {
+        for (int64_t k0 = 0; k0 < p.cap; k0 += ukeys) {
           int a = 0, e = 0;
-          if (s.n > 0 && k0 < s.keys) ms_steps(pb, s, (int)(k0 / kMsKeys), a, e);
+          if (s.n > 0 && k0 < s.keys) ms_steps(pb, s, ukeys, (int)(k0 / ukeys), a, e);
           if (e > a) continue;
-          for (int64_t j = k0 + lane; j < k0 + kMsKeys && j < p.cap; j += 32) row[j] = 0.f;
+          for (int64_t j = k0 + lane; j < k0 + ukeys && j < p.cap; j += 32) row[j] = 0.f;
         }
       }
     }
   } else {
     // ------------------------------------------------------------- sums, warps 0-15
-    const int t = warp >> 3, second = (warp >> 2) & 1, quarter = warp & 3;
+    const int slot = warp >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;
-    const uint32_t tS = tmem + ((uint32_t)(quarter * 32) << 16) + t * 256;
-    const uint64_t sc2 = f32x2(p.f.scale_log2, p.f.scale_log2);
-    int sc = 0, qc = 0, next_unit = 0;
+    const uint32_t tS = tmem + ((uint32_t)(quarter * 32) << 16) + slot * 128;
+    int qc = 0, next_unit = 0;
+    uint32_t s_parity = 0;
     // false once a wait ran out; the warp then goes on without waiting, its sums no longer count
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -470,129 +513,119 @@ __global__ void __launch_bounds__(kMsThreads, 1)
     for (const MsUnit* up; (up = ms_next<true>(bars, next_unit, p.err)) != nullptr;
          ms_done<true>(bars, next_unit)) {
       const MsUnit& u = *up;
-      const int key = u.u * kMsKeys + t * kChunkTile + row;
-      const bool page_ok = u.pages_ok || chunk_page(pb, u.b, u.keys, u.u * 2 + t, row >> 6) !=
-                                             pb.num_blocks;
+      // units of two tiles take the slots in turn
+      const int t = slot - (ktiles == 2 && (next_unit & 1) ? 2 : 0);
+      const bool mine = t >= 0 && t < ktiles;
+      const int tile0 = u.u * ukeys + t * kChunkTile, key = tile0 + row;
+      const bool page_ok = u.pages_ok || !mine ||
+                           chunk_page(pb, u.b, u.keys, u.u * ktiles + t, row >> 6) != pb.num_blocks;
+      // tokens [open, shut) see every key of this tile
+      int open = 0, shut = u.n;
+      if (tile0 + kChunkTile > u.prefix) {
+        open = tile0 + kChunkTile - 1 - u.pos0;
+        if (pb.window) shut = min(u.n, tile0 + pb.window - u.pos0);
+      }
+      if (!u.pages_ok) shut = 0;
+      const bool loads = ms_loads(u), frees = ms_frees(u);
       float acc = 0.f;
 #pragma unroll 1
-      for (int q = u.q0; q < u.q1; ++q, ++sc) {
-        const bool loads = ms_loads(u);
+      for (int q = u.q0; q < u.q1; ++q) {
         if (loads) ++qc;
-        const int qs = (qc - 1) % kMsStages, buf = sc & 1;
-        // columns [c_lo, c_hi) see this key
-        const int tok0 = q * pb.tile_tokens;
-        const int rows = min(u.n - tok0, pb.tile_tokens) * pb.group;
-        int c_lo = 0, c_hi = rows;
-        if (key >= u.prefix) {
-          c_lo = min(max(key - u.pos0 - tok0, 0), kChunkTile) * pb.group;
-          if (pb.window)
-            c_hi = min(rows, min(max(key + pb.window - u.pos0 - tok0, 0), kChunkTile) * pb.group);
+        const int ls = (qc - 1) % kMsRows;
+        if (loads) wait(&bars->l_full[ls], ((qc - 1) / kMsRows) & 1);
+        if (!mine) {  // another warpgroup's keys; the rows' slot is given back by all
+          __syncwarp();
+          if (lane == 0 && frees) mbar_arrive(&bars->l_empty[ls]);
+          continue;
         }
-        if (!page_ok) c_hi = 0;
-        // this warpgroup's columns: one half, in 16s
-        const int cols = (rows + 15) / 16 * 16, mid = (cols / 2 + 15) / 16 * 16;
-        const int c0 = second ? mid : 0, c1 = second ? cols : mid;
-        if (loads) wait(&bars->q_full[qs], ((qc - 1) / kMsStages) & 1);
-        wait(&bars->s_full[t][buf], (sc >> 1) & 1);
+        const int tok0 = q * pb.tile_tokens;
+        const bool mask = tok0 < open || tok0 + pb.tile_tokens > shut;
+        int cols = tile_rows, c_lo = 0, c_hi = kChunkTile;
+        if (mask) {  // columns [c_lo, c_hi) see this key
+          cols = c_hi = min(u.n - tok0, pb.tile_tokens) * pb.group;
+          if (key >= u.prefix) {
+            c_lo = min(max(key - u.pos0 - tok0, 0), kChunkTile) * pb.group;
+            if (pb.window)
+              c_hi = min(cols, min(max(key + pb.window - u.pos0 - tok0, 0), kChunkTile) * pb.group);
+          }
+          if (!page_ok) c_hi = 0;
+        }
+        wait(&bars->s_full[slot], s_parity);
+        s_parity ^= 1;
         tc_fence_after();
-        uint64_t sum2[2] = {0ull, 0ull};
+        // (scalar arithmetic: packed pairs save issue slots on paper, but cost 1.5 moves a value)
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-        for (int cc = c0; cc < c1; cc += 16) {
+        for (int cc = 0; cc < cols; cc += 16) {
           uint32_t raw[16];
-          tmem_ld16(tS + buf * 128 + cc, raw);
-          const float4* nl4 = reinterpret_cast<const float4*>(&bars->neg_lse[qs][cc]);
-          uint64_t x[8];
+          tmem_ld16(tS + cc, raw);
+          float x[16];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const float4 v = nl4[c];
-            x[2 * c] = f32x2(v.x, v.y);
-            x[2 * c + 1] = f32x2(v.z, v.w);
+          for (int c = 0; c < 16; c += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(&bars->neg_lse[ls][cc + c]);
+            x[c] = v.x;
+            x[c + 1] = v.y;
+            x[c + 2] = v.z;
+            x[c + 3] = v.w;
           }
           if constexpr (kAlibi) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const float4 sl = reinterpret_cast<const float4*>(&bars->slope[qs][cc])[c];
-              const float4 ps = reinterpret_cast<const float4*>(&bars->pos[qs][cc])[c];
+            for (int c = 0; c < 16; c += 4) {
+              const float4 sl = *reinterpret_cast<const float4*>(&bars->slope[ls][cc + c]);
+              const float4 ps = *reinterpret_cast<const float4*>(&bars->pos[ls][cc + c]);
               const float k = (float)key;
-              x[2 * c] = add_f32x2(x[2 * c], f32x2(-sl.x * fabsf(k - ps.x), -sl.y * fabsf(k - ps.y)));
-              x[2 * c + 1] =
-                  add_f32x2(x[2 * c + 1], f32x2(-sl.z * fabsf(k - ps.z), -sl.w * fabsf(k - ps.w)));
+              x[c] = fmaf(-sl.x, fabsf(k - ps.x), x[c]);
+              x[c + 1] = fmaf(-sl.y, fabsf(k - ps.y), x[c + 1]);
+              x[c + 2] = fmaf(-sl.z, fabsf(k - ps.z), x[c + 2]);
+              x[c + 3] = fmaf(-sl.w, fabsf(k - ps.w), x[c + 3]);
             }
           }
           tmem_wait_ld();
           reg_fence<16>(raw);
           if constexpr (kCap) {
-            const uint64_t cin = f32x2(p.f.cap_in, p.f.cap_in);
-            const uint64_t cout = f32x2(p.f.cap_log2, p.f.cap_log2);
             float big = 0.f;
 #pragma unroll
             for (int c = 0; c < 16; c += 2)
               big = fmax3f(big, fabsf(__uint_as_float(raw[c])), fabsf(__uint_as_float(raw[c + 1])));
-            const bool small = __all_sync(0xffffffffu, big * p.f.cap_in <= 1.f);
+            if (__all_sync(0xffffffffu, big * p.f.cap_in <= 1.f)) {
+              // (in pairs: the polynomial is long enough to pay for the packing)
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              const uint64_t v = mul_f32x2(
-                  f32x2(__uint_as_float(raw[2 * c]), __uint_as_float(raw[2 * c + 1])), cin);
-              uint64_t y = tanh_poly_x2(v);
-              if (!small) {
-                float v0, v1, y0, y1;
-                f32x2_split(v, v0, v1);
-                f32x2_split(y, y0, y1);
-                y = f32x2(fabsf(v0) <= 1.f ? y0 : tanh_any(v0), fabsf(v1) <= 1.f ? y1 : tanh_any(v1));
+              for (int c = 0; c < 16; c += 2) {
+                const uint64_t v = mul_f32x2(
+                    f32x2(__uint_as_float(raw[c]), __uint_as_float(raw[c + 1])), f32x2(p.f.cap_in, p.f.cap_in));
+                f32x2_split(fma_f32x2(tanh_poly_x2(v), f32x2(p.f.cap_log2, p.f.cap_log2),
+                                      f32x2(x[c], x[c + 1])), x[c], x[c + 1]);
               }
-              x[c] = fma_f32x2(y, cout, x[c]);
+            } else {
+#pragma unroll
+              for (int c = 0; c < 16; ++c) {
+                const float v = __uint_as_float(raw[c]) * p.f.cap_in;
+                x[c] = fmaf(fabsf(v) <= 1.f ? tanh_poly(v) : tanh_any(v), p.f.cap_log2, x[c]);
+              }
             }
           } else {
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-              x[c] = fma_f32x2(f32x2(__uint_as_float(raw[2 * c]), __uint_as_float(raw[2 * c + 1])),
-                               sc2, x[c]);
+            for (int c = 0; c < 16; ++c) x[c] = fmaf(__uint_as_float(raw[c]), p.f.scale_log2, x[c]);
           }
-          if (!__all_sync(0xffffffffu, c_lo <= cc && c_hi >= min(cc + 16, tile_rows))) {
+          if (mask) {
             const uint32_t vis = low_bits(c_hi - cc, 0) & ~low_bits(c_lo - cc, 0);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              float a, b;
-              f32x2_split(x[c], a, b);
-              x[c] = f32x2((vis >> (2 * c)) & 1u ? a : -INFINITY,
-                           (vis >> (2 * c + 1)) & 1u ? b : -INFINITY);
-            }
+            for (int c = 0; c < 16; ++c)
+              if (!((vis >> c) & 1u)) x[c] = -INFINITY;
           }
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            uint64_t e;
-            if (c < kMsEmuPairs) {
-              e = exp2_poly5_x2(x[c]);
-            } else {
-              float a, b;
-              f32x2_split(x[c], a, b);
-              e = f32x2(fast_exp2(a), fast_exp2(b));
-            }
-            sum2[c & 1] = add_f32x2(sum2[c & 1], e);
-          }
+          for (int c = 0; c < 16; ++c)
+            sum[c & 3] += c < kMsEmu ? exp2_poly5(x[c]) : fast_exp2(x[c]);
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&bars->s_empty[t][buf]);
-          if (ms_frees(u)) mbar_arrive(&bars->q_empty[qs]);
+          mbar_arrive(&bars->s_empty[slot]);
+          if (frees) mbar_arrive(&bars->l_empty[ls]);
         }
-        float s0, s1;
-        f32x2_split(add_f32x2(sum2[0], sum2[1]), s0, s1);
-        acc += s0 + s1;
+        acc += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       }
-      // The second half's sum goes to the first half's warp through shared memory. A slot is
-      // free again kMsParts units later: the S buffers keep the halves within two steps, and so
-      // within two units, of each other.
-      const int slot = next_unit % kMsParts;
-      if (second) {
-        bars->part[t][slot][row] = acc;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->part_full[t][slot]);
-        continue;
-      }
-      wait(&bars->part_full[t][slot], (next_unit / kMsParts) & 1);
-      acc += bars->part[t][slot][row];
+      if (!mine) continue;
       if (u.whole) {
         const int64_t keys = min((int64_t)u.keys, p.cap);
         float* dst = p.mass + ((int64_t)u.b * pb.hk + u.hk) * p.cap + key;
@@ -724,6 +757,8 @@ extern "C" int fi_attention_mass(const void* q, const void* k_cache, const float
   p.accumulate = accumulate != 0;
   p.ws = static_cast<float*>(workspace);
   p.join = reinterpret_cast<MsJoin*>(p.ws + (size_t)sm_count() * 2 * kMsKeys);
+  // Sequences of few tokens have one step a unit: smaller units even the CTAs' parts out.
+  p.tiles = total_tokens > batch * p.b.tile_tokens ? 4 : 2;
   p.err = error_flag;
   return dtype == FI_DTYPE_F16 ? launch_mass_form<__half>(tq, tk, p, softcap > 0.f, st)
                                : launch_mass_form<__nv_bfloat16>(tq, tk, p, softcap > 0.f, st);
