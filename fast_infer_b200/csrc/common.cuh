@@ -266,6 +266,20 @@ __device__ __forceinline__ bool wg_bar_and(int id, bool pred) {
   return r != 0;
 }
 
+// The same for the first `threads` threads that name the barrier.
+__device__ __forceinline__ bool bar_and(int id, int threads, bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, %2, %3, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)pred), "r"(id), "r"(threads)
+      : "memory");
+  return r != 0;
+}
+
 // Thread-block cluster barrier (every thread of every CTA of the cluster arrives),
 // with release / acquire ordering of shared-memory accesses across the cluster.
 __device__ __forceinline__ void cluster_sync_all() {

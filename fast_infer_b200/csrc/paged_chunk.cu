@@ -41,7 +41,7 @@ constexpr int kCkMaxBatch = 2048;    // sequences per launch
 constexpr int kCkMaxUnits = 4608;    // token units per launch (per KV head)
 constexpr int kCkNarrow = 32;        // rows up to which a unit runs transposed
 constexpr float kCkRescale = 8.0f;   // log2 units of growth of the max before O is rescaled
-constexpr int kCkEmuPairs = 2;       // of 8 column pairs, exp2 on the FMA pipe
+constexpr int kCkEmuPairs = 1;       // of 8 column pairs, exp2 on the FMA pipe
 constexpr int kCkSlots = 4;          // units that the scheduler is ahead
 
 // A CTA's part of a unit: key steps [j0, j1) of its n.
@@ -295,8 +295,8 @@ __device__ __forceinline__ void score_form8(const uint32_t* raw, float* s, const
   }
 }
 
-// p = 2^(s * sl2 - mref) of a row, its sum, and p packed in place. 2 of 8 pairs take exp2 on the
-// FMA pipe, to 2.2e-7: lse is an output, which a rougher polynomial would show in.
+// p = 2^(s * sl2 - mref) of a row, its sum, and p packed in place. 1 of 8 pairs takes exp2 on the
+// FMA pipe (0: 4772 us for a chunk of 4096 tokens over 61003, 1: 3587, 2: 3746, 3: 3802), to 2.2e-7: lse is an output, which a rougher polynomial would show in.
 template <typename T>
 __device__ __forceinline__ float ck_exp(uint32_t* sr, float sl2, float mref) {
   const uint64_t sc2 = f32x2(sl2, sl2), nm2 = f32x2(-mref, -mref);
@@ -672,7 +672,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
   const uint32_t tmem = bars->tmem_base;
 
   if (warp >= 8) {
-    setmaxnreg_dec<kCkRegsOther>();
+    if constexpr (!kNarrow) setmaxnreg_dec<kCkRegsOther>();
     if (warp == 8 && lane == 0) {
       // ---------------------------------------------------------- TMA producer
       prefetch_tmap(&tm_q);
@@ -878,7 +878,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
   }
 
   // ------------------------------------------- softmax + epilogue, warps 0-7
-  setmaxnreg_inc<kCkRegsSoftmax>();
+  if constexpr (!kNarrow) setmaxnreg_inc<kCkRegsSoftmax>();
   {
     const int t = warp >> 2;
     const int quarter = warp & 3;
@@ -1137,7 +1137,7 @@ static int launch_main(const CUtensorMap& tq, const CUtensorMap& tk, const CUten
     cudaFuncAttributes a;
     const cudaError_t e = cudaFuncGetAttributes(&a, paged_chunk_kernel<T, kCap, kAlibi, kNarrow>);
     if (e != cudaSuccess) return e;
-    if (a.numRegs * kCkThreads < 2 * 128 * kCkRegsSoftmax + 128 * kCkRegsOther)
+    if (!kNarrow && a.numRegs * kCkThreads < 2 * 128 * kCkRegsSoftmax + 128 * kCkRegsOther)
       return cudaErrorInvalidConfiguration;
     return cudaFuncSetAttribute(paged_chunk_kernel<T, kCap, kAlibi, kNarrow>,
                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kCkSmemBytes);
