@@ -7,19 +7,26 @@
 // pool's.
 //
 // Two launches. evict_select_kernel, a CTA per (layer, sequence, KV head), finds the weight of
-// the last token that stays by its bits: a non-negative float orders like its bits, so three
-// histograms (11, 11 and 10 bits, from the top) leave one value and how many of its equals
-// stay; then each warp lists what it keeps of its run of tokens. evict_copy_kernel moves the
-// rows, 256 bytes each: bound by HBM, so it keeps many independent 16-byte loads in flight.
+// the last token that stays, the edge, by its bits: a non-negative float orders like its bits.
+// One histogram of 2048 bins over the 16 octaves below the greatest weight leaves a bin of few
+// weights, among which the edge is found by rank. Where that bin holds many (weights far below
+// the greatest, or equal), three histograms of the plain bits (11, 11 and 10, from the top) do
+// it instead (taken first, 88 us for 28 layers x 8 heads of 32768 tokens against 62; counting bit
+// by bit in registers, 109). Then each warp lists what it keeps of its run of tokens. evict_copy_kernel moves
+// the rows, 256 bytes each: bound by HBM (600 us for 3.76 GB read and written), so it keeps many
+// independent 16-byte loads in flight.
 #include "common.cuh"
 #include "host_common.h"
 
 namespace fi {
 
 constexpr int kEvPage = 64;
-constexpr int kEvThreads = 512;                  // select
+// threads of a selection: 28 x 16 x 8 rows of 900 to 4096 tokens take 90 us with 512 (256: 94, 128: 215),
+// 28 x 8 rows of 32768 take 62 us with 1024 (512: 83)
+constexpr int kEvShort = 512, kEvLong = 1024;
 constexpr int kEvBins = 2048;
-constexpr int kEvStageMax = 48 * 1024;           // tokens whose weights are kept in shared memory
+constexpr int kEvStageMax = 12 * 1024;           // tokens whose weights are kept in shared memory
+constexpr int kEvList = 1024;                    // weights of the edge's bin that are ranked
 constexpr int kEvCopyThreads = 256;
 constexpr int kEvSeg = 128;                      // tokens a copy CTA moves, out of place
 constexpr int kEvInThreads = 512;                // copy in place
@@ -54,10 +61,11 @@ __device__ __forceinline__ uint32_t weight_bits(float w) { return w > 0.f ? __fl
 
 // The bin, from the top, in which the count of larger values reaches `want`: on return `want`
 // is how many of that bin's values stay. hist has kEvBins counts; all threads call it.
+template <int kThreads>
 __device__ __forceinline__ int top_bin(const uint32_t* hist, int bins, int& want, uint32_t* sums,
                                        int* found) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int each = (bins + kEvThreads - 1) / kEvThreads;  // this thread's bins, from the top
+  const int each = (bins + kThreads - 1) / kThreads;  // this thread's bins, from the top
   uint32_t sum = 0;
   for (int i = 0; i < each; ++i) {
     const int bin = bins - 1 - (tid * each + i);
@@ -89,13 +97,15 @@ __device__ __forceinline__ int top_bin(const uint32_t* hist, int bins, int& want
   return found[0];
 }
 
-__global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArgs a) {
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads) evict_select_kernel(const EvictArgs a) {
   extern __shared__ uint32_t ev_smem[];
   uint32_t* hist = ev_smem;             // [kEvBins]
   uint32_t* stage = ev_smem + kEvBins;  // [a.stage]
-  __shared__ uint32_t sums[kEvThreads / 32];
-  __shared__ uint32_t run_over[kEvThreads / 32], run_same[kEvThreads / 32];
+  __shared__ uint32_t sums[kThreads / 32];
+  __shared__ uint32_t run_over[kThreads / 32], run_same[kThreads / 32];
   __shared__ int found[2];
+  __shared__ uint32_t listed, list[kEvList];
   grid_dep_wait();
   grid_dep_launch();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -109,7 +119,7 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
       row < (int64_t)a.batch * a.heads && n != a.lens[b])
     set_error(a.err, FI_DEVERR_CONTEXT_LEN);
   if (n <= a.budget) {
-    for (int i = tid; i < a.budget; i += kEvThreads) {
+    for (int i = tid; i < a.budget; i += kThreads) {
       kept[i] = i < n ? i : -1;
       mass_out[i] = i < n ? mass[i] : 0.f;
     }
@@ -117,79 +127,143 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
   }
   const int lo = a.sinks, hi = n - a.recent;  // the tokens that compete
   const bool staged = n <= a.stage;
-  auto bits = [&](int j) { return staged ? stage[j] : weight_bits(mass[j]); };
+  // f(token, weight's bits) for tokens [from, to): eight reads on their way at a time
+  auto sweep = [&](int from, int to, bool first, auto&& f) {
+#pragma unroll 1
+    for (int j0 = from + tid; j0 < to; j0 += 8 * kThreads) {
+      uint32_t x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int j = j0 + k * kThreads;
+        x[k] = 0;
+        if (j < to) x[k] = staged && !first ? stage[j] : __float_as_uint(mass[j]);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (j0 + k * kThreads < to) f(j0 + k * kThreads, x[k]);
+    }
+  };
   int want = a.budget - a.sinks - a.recent;
   uint32_t edge = 0xffffffffu;  // weights above it stay, and `want` of its equals
-  if (want > 0) {
-    uint32_t prefix = 0;
+  uint32_t top = 0;             // the greatest weight that competes
+  sweep(0, n, true, [&](int j, uint32_t raw) {
+    if (staged) stage[j] = raw;
+    if (j >= lo && j < hi) top = max(top, weight_bits(__uint_as_float(raw)));
+  });
 #pragma unroll
-    for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-      const int bins = pass == 2 ? 1024 : 2048;
-      for (int i = tid; i < bins; i += kEvThreads) hist[i] = 0;
-      __syncthreads();
-      if (pass == 0) {
-        for (int j = tid; j < n; j += kEvThreads) {
-          const uint32_t x = weight_bits(mass[j]);
-          if (staged) stage[j] = x;
-          if (j >= lo && j < hi) atomicAdd(&hist[x >> 21], 1u);
+  for (int off = 16; off > 0; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+  if (lane == 0) sums[warp] = top;
+  for (int i = tid; i < kEvBins; i += kThreads) hist[i] = 0;
+  if (tid == 0) listed = 0;
+  __syncthreads();
+  if (want > 0) {
+    for (int w = 0; w < kThreads / 32; ++w) top = max(top, sums[w]);
+    // bin: 7 bits below the exponent over 16 octaves; all that is smaller shares bin 0, whose
+    // count no one needs
+    const int base = (int)(top >> 16) - (kEvBins - 1);
+    auto bin_of = [&](uint32_t x) { return max((int)(x >> 16) - base, 0); };
+    sweep(lo, hi, false, [&](int, uint32_t raw) {
+      const int k = bin_of(weight_bits(__uint_as_float(raw)));
+      if (k > 0) atomicAdd(&hist[k], 1u);
+    });
+    __syncthreads();
+    if (tid == 0) hist[0] = 0x3fffffffu;  // whatever is left
+    __syncthreads();
+    int in_bin = want;
+    const int bin = top_bin<kThreads>(hist, kEvBins, in_bin, sums, found);
+    sweep(lo, hi, false, [&](int, uint32_t raw) {
+      const uint32_t x = weight_bits(__uint_as_float(raw));
+      if (bin_of(x) == bin) {
+        const uint32_t at = atomicAdd(&listed, 1u);
+        if (at < kEvList) list[at] = x;
+      }
+    });
+    __syncthreads();
+    if (listed <= kEvList) {
+      for (int i = tid; i < (int)listed; i += kThreads) {
+        const uint32_t x = list[i];
+        int over = 0, same = 0;
+        for (int k = 0; k < (int)listed; ++k) {
+          over += list[k] > x;
+          same += list[k] == x;
         }
-      } else {
-        const int top = pass == 1 ? 21 : 10;
-        for (int j = lo + tid; j < hi; j += kEvThreads) {
-          const uint32_t x = bits(j);
-          if (x >> top == prefix) atomicAdd(&hist[(x >> shift) & (bins - 1)], 1u);
+        if (over < in_bin && in_bin <= over + same) {  // all that are equal write the same
+          found[0] = (int)x;
+          found[1] = in_bin - over;
         }
       }
       __syncthreads();
-      const int bin = top_bin(hist, bins, want, sums, found);
-      prefix = (prefix << (pass == 2 ? 10 : 11)) | (uint32_t)bin;
+      edge = (uint32_t)found[0];
+      want = found[1];
+    } else {
+      uint32_t prefix = 0;
+#pragma unroll 1
+      for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const int bins = pass == 2 ? 1024 : 2048;
+        const int high = pass == 0 ? 31 : pass == 1 ? 21 : 10;  // (bit 31 is never set)
+        __syncthreads();
+        for (int i = tid; i < bins; i += kThreads) hist[i] = 0;
+        __syncthreads();
+        sweep(lo, hi, false, [&](int, uint32_t raw) {
+          const uint32_t x = weight_bits(__uint_as_float(raw));
+          if (x >> high == prefix) atomicAdd(&hist[(x >> shift) & (bins - 1)], 1u);
+        });
+        __syncthreads();
+        prefix = (prefix << (pass == 2 ? 10 : 11)) | (uint32_t)top_bin<kThreads>(hist, bins, want, sums, found);
+      }
+      edge = prefix;
     }
-    edge = prefix;
-  } else if (staged) {
-    for (int j = tid; j < n; j += kEvThreads) stage[j] = weight_bits(mass[j]);
-    __syncthreads();
   }
-  // Each warp has a run of tokens: count what is over the edge and what equals it, then list.
-  const int each = ((n + kEvThreads - 1) / kEvThreads) * 32;
+  // Each warp has a run of tokens: it counts what is over the edge and what equals it, then lists
+  // what stays; 8 x 32 tokens at a time.
+  const int each = ((n + kThreads - 1) / kThreads) * 32;
   const int j0 = min(warp * each, n), j1 = min(j0 + each, n);
-  uint32_t over = 0, same = 0;
-  for (int j = j0 + lane; j < j1; j += 32) {
-    const bool mid = j >= lo && j < hi;
-    const uint32_t x = mid ? bits(j) : 0u;
-    over += !mid || x > edge;
-    same += mid && x == edge;
-  }
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    over += __shfl_xor_sync(0xffffffffu, over, off);
-    same += __shfl_xor_sync(0xffffffffu, same, off);
-  }
-  if (lane == 0) {
-    run_over[warp] = over;
-    run_same[warp] = same;
-  }
-  __syncthreads();
   uint32_t before_over = 0, before_same = 0;
-  for (int w = 0; w < warp; ++w) {
-    before_over += run_over[w];
-    before_same += run_same[w];
-  }
   const uint32_t below = (1u << lane) - 1u;
-  for (int base = j0; base < j1; base += 32) {
-    const int j = base + lane;
-    const bool in = j < j1, mid = in && j >= lo && j < hi;
-    const uint32_t x = mid ? bits(j) : 0u;
-    const bool is_over = in && (!mid || x > edge), is_same = mid && x == edge;
-    const uint32_t bo = __ballot_sync(0xffffffffu, is_over), bs = __ballot_sync(0xffffffffu, is_same);
-    const uint32_t same_rank = before_same + __popc(bs & below);
-    if (is_over || (is_same && same_rank < (uint32_t)want)) {
-      const uint32_t at = before_over + __popc(bo & below) + min(same_rank, (uint32_t)want);
-      kept[at] = j;
-      mass_out[at] = mass[j];
+#pragma unroll 1
+  for (int list_now = 0; list_now < 2; ++list_now) {
+    uint32_t n_over = 0, n_same = 0;
+#pragma unroll 1
+    for (int base = j0; base < j1; base += 256) {
+      uint32_t raw[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int j = base + k * 32 + lane;
+        raw[k] = 0;
+        if (j < j1) raw[k] = staged ? stage[j] : __float_as_uint(mass[j]);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (base + k * 32 >= j1) break;
+        const int j = base + k * 32 + lane;
+        const bool in = j < j1, mid = in && j >= lo && j < hi;
+        const uint32_t x = weight_bits(__uint_as_float(raw[k]));
+        const bool is_over = in && (!mid || x > edge), is_same = mid && x == edge;
+        const uint32_t bo = __ballot_sync(0xffffffffu, is_over), bs = __ballot_sync(0xffffffffu, is_same);
+        if (list_now) {
+          const uint32_t same_rank = before_same + n_same + __popc(bs & below);
+          if (is_over || (is_same && same_rank < (uint32_t)want)) {
+            const uint32_t at =
+                before_over + n_over + __popc(bo & below) + min(same_rank, (uint32_t)want);
+            kept[at] = j;
+            mass_out[at] = __uint_as_float(raw[k]);
+          }
+        }
+        n_over += __popc(bo);
+        n_same += __popc(bs);
+      }
     }
-    before_over += __popc(bo);
-    before_same += __popc(bs);
+    if (list_now) break;
+    if (lane == 0) {
+      run_over[warp] = n_over;
+      run_same[warp] = n_same;
+    }
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) {
+      before_over += run_over[w];
+      before_same += run_same[w];
+    }
   }
 }
 
@@ -367,13 +441,16 @@ extern "C" int fi_kv_evict(const void* k, const void* v, const int32_t* block_ta
   a.stage = (int)(longest <= kEvStageMax ? longest : 0);
   static DeviceOnce once;
   cudaError_t e = once.run([] {
-    return cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    return cudaFuncSetAttribute(evict_select_kernel<kEvLong>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 (kEvBins + kEvStageMax) * 4);
   });
   if (e != cudaSuccess) return cuda_fail(e, "fi_kv_evict: cudaFuncSetAttribute");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  e = launch_pdl(evict_select_kernel, dim3((unsigned)rows), dim3(kEvThreads),
-                 (size_t)(kEvBins + a.stage) * 4, st, a);
+  const size_t smem = (size_t)(kEvBins + a.stage) * 4;
+  if (longest <= 16 * kEvShort)
+    e = launch_pdl(evict_select_kernel<kEvShort>, dim3((unsigned)rows), dim3(kEvShort), smem, st, a);
+  else
+    e = launch_pdl(evict_select_kernel<kEvLong>, dim3((unsigned)rows), dim3(kEvLong), smem, st, a);
   if (e != cudaSuccess) return cuda_fail(e, "fi_kv_evict: select launch");
   if (in_place)
     e = launch_pdl(evict_copy_kernel<kEvInThreads, kEvInSeg, true>, dim3((unsigned)rows),

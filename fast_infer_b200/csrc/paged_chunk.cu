@@ -155,7 +155,9 @@ __device__ __forceinline__ void ck_schedule(const ChunkBatch& p, int unit_tokens
     bool pages_ok = true;
     if (u.valid) {
       const int t0 = (e - (int)s->unit_off[b]) * unit_tokens, t1 = min(t0 + unit_tokens, q.n);
-      ck_tiles(p, q, t0, t1, u.np, u.lo, u.n);
+      int tiles;
+      ck_tiles(p, q, t0, t1, u.np, u.lo, tiles);
+      u.n = (int)(s->work[e + 1] - s->work[e]);  // the line's own count: the walk always ends
       u.b = b;
       u.hk = hk;
       u.token = q.start + t0;
@@ -332,15 +334,6 @@ __device__ __forceinline__ void zero_v_rows(uint8_t* v, int from, int tid) {
   }
 }
 
-// Ordered like the float it comes from (no NaN), as a signed integer.
-__device__ __forceinline__ int float_order(float x) {
-  const int i = __float_as_int(x);
-  return i ^ ((i >> 31) & 0x7fffffff);
-}
-__device__ __forceinline__ float order_float(int i) {
-  return __int_as_float(i ^ ((i >> 31) & 0x7fffffff));
-}
-
 // A transposed unit, softmax side: warpgroup t takes key tiles j0 + t, j0 + t + 2, ... A thread is
 // one key of the tile (and, for O^T, one dim). `ok` turns false when a wait runs out; a warp that
 // saw it goes on without waiting, so that every barrier here gets all of its threads.
@@ -369,6 +362,7 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
       bars->n_pos[t][tid] = (float)(u.pos + bars->row_token[tid]);
     }
   }
+  __syncwarp();
   named_bar_sync(1 + t, 128);
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.err));
@@ -427,12 +421,24 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
 #pragma unroll
         for (int cc = 0; cc < kCkNarrow; cc += 8)
           if (cc < rows) {
+            // over the lanes: columns trade places until four lanes have one
+            float mx[8];
 #pragma unroll
-            for (int c = cc; c < cc + 8; ++c) {
-              const int mx = __reduce_max_sync(0xffffffffu, float_order(s[c]));
-              if (lane == 0) bars->n_red[t][quarter][c] = order_float(mx);
+            for (int c = 0; c < 8; ++c) mx[c] = s[cc + c];
+#pragma unroll
+            for (int half = 4; half > 0; half >>= 1) {
+              const bool up = lane & (half * 4);
+#pragma unroll
+              for (int c = 0; c < half; ++c) {
+                const float give = up ? mx[c] : mx[c + half], keep = up ? mx[c + half] : mx[c];
+                mx[c] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, half * 4));
+              }
             }
+            mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], 2));
+            mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], 1));
+            if ((lane & 3) == 0) bars->n_red[t][quarter][cc + (lane >> 2)] = mx[0];
           }
+        __syncwarp();
         named_bar_sync(1 + t, 128);
         if (tid < rows) {
           const float was = n_max[tid];
@@ -442,6 +448,7 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
           n_max[tid] = now;
           bars->n_neg[t][tid] = -now;
         }
+        __syncwarp();
         named_bar_sync(1 + t, 128);
         if (j >= 2) {
           // the product of this warpgroup's last tile is complete: S here was committed after it
@@ -1068,6 +1075,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
   }
 
   if (p.late_wait && threadIdx.x == 0) grid_dep_wait();
+  __syncwarp();
   tc_fence_before();
   named_bar_sync(kCkTeardownBar, kCkThreads);
   if (warp == 0) {
@@ -1078,7 +1086,6 @@ __global__ void __launch_bounds__(kCkThreads, 1)
 
 // Joins the parts of a unit that several CTAs hold: weights 2^(lse_part - max). A warp per row.
 // Blocks [0, ctas) join `p`'s units, blocks [ctas, 2 * ctas) those of `p2`.
-constexpr int kJoinSlices = 8;
 template <typename T>
 __global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p,
                                                             const ChunkParams p2, int ctas) {
@@ -1092,7 +1099,7 @@ __global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p,
   const float* ws_lse = second ? p2.ws_lse : p.ws_lse;
   const float* ws_o = second ? p2.ws_o : p.ws_o;
 #pragma unroll 1
-  for (int r = blockIdx.y * 8 + warp; r < rows_cap; r += kJoinSlices * 8) {
+  for (int r = blockIdx.y * 8 + warp; r < rows_cap; r += gridDim.y * 8) {
     const int t = r >> 7, row = r & 127;
     if (row >= (t ? jn.rows[1] : jn.rows[0])) continue;
     auto at = [&](int c) { return (int64_t)(c * 2 + (c == cta ? 1 : 0)) * rows_cap + r; };
@@ -1169,7 +1176,7 @@ static int launch_chunk(const CUtensorMap& tq_n, const CUtensorMap& tq_w, const 
   const ChunkParams& first = wide ? *wide : *narrow;
   const int ctas = sm_count();
   const cudaError_t e =
-      launch_pdl(chunk_combine_kernel<T>, dim3((unsigned)(narrow && wide ? 2 * ctas : ctas), kJoinSlices),
+      launch_pdl(chunk_combine_kernel<T>, dim3((unsigned)(narrow && wide ? 2 * ctas : ctas), (unsigned)(first.rows_cap / 8)),
                  dim3(256), 0, st, first, narrow ? *narrow : first, ctas);
   return e == cudaSuccess ? FI_OK : cuda_fail(e, "fi_paged_chunk: combine launch");
 }

@@ -138,7 +138,7 @@ __device__ __forceinline__ void ms_schedule(const ChunkBatch& p, MsBarriers* m, 
     s = chunk_seq(p, b);
     uint64_t r = r0 - m->seq[b];
 #pragma unroll 1
-    for (int base = 0;; base += 32) {  // the unit that holds step r of the sequence
+    for (int base = 0; base < ms_units(s, ukeys); base += 32) {  // the unit of step r
       int a = 0, e = 0;
       if (base + lane < ms_units(s, ukeys)) ms_steps(p, s, ukeys, base + lane, a, e);
       uint64_t inc = (uint64_t)(e - a);
@@ -170,13 +170,13 @@ __device__ __forceinline__ void ms_schedule(const ChunkBatch& p, MsBarriers* m, 
     bool pages_ok = true;
     v.valid = w < end;
     if (v.valid) {
-      int a, e;
-      while (true) {  // the line holds only units with steps
+      int a = 0, e = 0;
+      for (; u < ms_units(s, ukeys); ++u) {  // the line holds only units with steps
         ms_steps(p, s, ukeys, u, a, e);
         if (e > a) break;
-        ++u;
       }
-      const int n = e - a;
+      const int n = max(e - a, 1);  // (1: lengths changed meanwhile; the walk ends all the same)
+      e = a + n;
       v.q0 = a + skip;
       v.q1 = (int)(e - v.q0 <= end - w ? e : v.q0 + (end - w));
       v.b = b;

@@ -50,6 +50,13 @@ struct Unpack<__nv_bfloat16> {
 
 constexpr int kRaThreads = 256;
 
+__device__ __forceinline__ int axis_of(uint64_t axis_end, int f) {
+  int axis = 0;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) axis += f >= (int)((axis_end >> (16 * i)) & 0xffff);
+  return axis;
+}
+
 // `split` warps share a token (small batches have too few tokens to fill the GPU).
 template <typename T>
 __global__ void __launch_bounds__(kRaThreads) rope_axes_kernel(const RopeAxesArgs a, int split) {
@@ -61,6 +68,10 @@ __global__ void __launch_bounds__(kRaThreads) rope_axes_kernel(const RopeAxesArg
   const int c = lane & 7, sub = lane >> 3;  // 8-value piece, head within the group of four
   const int end = min(max(a.cu[a.batch], 0), a.total);
   const int heads = a.nq + 2 * a.nkv;
+  const int axis8 = axis_of(a.axis_end, c * 8);
+  const bool vector_tables =
+      __all_sync(0xffffffffu, axis8 == axis_of(a.axis_end, c * 8 + 7)) && a.table_stride % 4 == 0 &&
+      ((reinterpret_cast<uintptr_t>(a.cos_tab) | reinterpret_cast<uintptr_t>(a.sin_tab)) & 15) == 0;
   if (a.err && blockIdx.x == 0)
     for (int b = threadIdx.x; b < a.batch; b += kRaThreads)
       if (a.cu[b] < 0 || a.cu[b + 1] < a.cu[b] || a.cu[b + 1] > a.total)
@@ -68,11 +79,23 @@ __global__ void __launch_bounds__(kRaThreads) rope_axes_kernel(const RopeAxesArg
   for (int64_t w = (int64_t)blockIdx.x * (kRaThreads / 32) + (threadIdx.x >> 5); w < work;
        w += warps) {
     const int t = (int)(w / split), part = (int)(w % split);
+    // the first heads are on their way while the token's place is looked up
+    const T* x = static_cast<const T*>(a.qkv) + (int64_t)t * a.xs + c * 8;
+    const int h0 = part * 4 + sub, step = split * 4;
+    uint4 lo_next = make_uint4(0, 0, 0, 0), hi_next = lo_next;
+    if (h0 < heads) {
+      lo_next = *reinterpret_cast<const uint4*>(x + h0 * 128);
+      hi_next = *reinterpret_cast<const uint4*>(x + h0 * 128 + 64);
+    }
     if (t < a.cu[0] || t >= end) continue;  // rows outside every sequence stay as they were
-    int lo = 0, hi = a.batch;               // the last b with cu[b] <= t
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.cu[mid] <= t) lo = mid; else hi = mid;
+    // the last b with cu[b] <= t: the lanes probe 32 places at a time
+    int lo = 0, n = a.batch;
+    while (n > 1) {
+      const int gap = (n + 31) / 32, probe = lane * gap;
+      const uint32_t le = __ballot_sync(0xffffffffu, probe < n && a.cu[lo + (probe < n ? probe : 0)] <= t);
+      const int i = max(31 - __clz((int)le), 0);  // (cu not ascending: any of them)
+      n = min(gap, n - i * gap);
+      lo += i * gap;
     }
     if (t >= a.cu[lo + 1]) continue;  // cu is not ascending: the token has no sequence
     const int64_t slot = (int64_t)a.ctx[lo] - (a.cu[lo + 1] - t);
@@ -82,36 +105,46 @@ __global__ void __launch_bounds__(kRaThreads) rope_axes_kernel(const RopeAxesArg
       page = a.bt[lo * a.bts[0] + (slot / kChunkPage) * a.bts[1]];
     const bool store = page >= 0 && page < a.num_blocks;
     if (!store && lane == 0) set_error(a.err, FI_DEVERR_BAD_BLOCK);
-    // this lane's 8 frequencies and their cos / sin in both halves
+    // this lane's 8 frequencies and their cos / sin in both halves: as vectors where one axis has
+    // all 8 and the tables allow
     float cl[8], sl[8], ch[8], sh[8];
     bool in_table = true;
+    if (vector_tables) {
+      const int64_t p = a.pos[axis8 * a.pos_stride + t];
+      in_table = p >= 0 && p < a.table_rows;
+      const int64_t off = (in_table ? p : 0) * a.table_stride + c * 8;
+      const float* ct = a.cos_tab + off;
+      const float* st = a.sin_tab + off;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int f = c * 8 + e;
-      int axis = 0;
-#pragma unroll
-      for (int i = 0; i < 3; ++i) axis += f >= (int)((a.axis_end >> (16 * i)) & 0xffff);
-      const int64_t p = a.pos[axis * a.pos_stride + t];
-      if (p < 0 || p >= a.table_rows) {
-        in_table = false;
-        cl[e] = sl[e] = ch[e] = sh[e] = 0.f;
-        continue;
+      for (int e = 0; e < 8; e += 4) {
+        *reinterpret_cast<float4*>(cl + e) = *reinterpret_cast<const float4*>(ct + e);
+        *reinterpret_cast<float4*>(sl + e) = *reinterpret_cast<const float4*>(st + e);
+        *reinterpret_cast<float4*>(ch + e) = *reinterpret_cast<const float4*>(ct + 64 + e);
+        *reinterpret_cast<float4*>(sh + e) = *reinterpret_cast<const float4*>(st + 64 + e);
       }
-      const float* ct = a.cos_tab + p * a.table_stride;
-      const float* st = a.sin_tab + p * a.table_stride;
-      cl[e] = ct[f];
-      sl[e] = st[f];
-      ch[e] = ct[f + 64];
-      sh[e] = st[f + 64];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int64_t p = a.pos[axis_of(a.axis_end, c * 8 + e) * a.pos_stride + t];
+        const bool in = p >= 0 && p < a.table_rows;
+        in_table &= in;
+        const int64_t off = (in ? p : 0) * a.table_stride + c * 8 + e;
+        cl[e] = a.cos_tab[off];
+        sl[e] = a.sin_tab[off];
+        ch[e] = a.cos_tab[off + 64];
+        sh[e] = a.sin_tab[off + 64];
+      }
     }
     if (!__all_sync(0xffffffffu, in_table)) {
       if (lane == 0) set_error(a.err, FI_DEVERR_CONTEXT_LEN);
       continue;
     }
-    const T* x = static_cast<const T*>(a.qkv) + (int64_t)t * a.xs;
-    for (int h = part * 4 + sub; h < heads; h += split * 4) {
-      const uint4 lo_raw = *reinterpret_cast<const uint4*>(x + h * 128 + c * 8);
-      const uint4 hi_raw = *reinterpret_cast<const uint4*>(x + h * 128 + 64 + c * 8);
+    for (int h = h0; h < heads; h += step) {
+      const uint4 lo_raw = lo_next, hi_raw = hi_next;
+      if (h + step < heads) {
+        lo_next = *reinterpret_cast<const uint4*>(x + (h + step) * 128);
+        hi_next = *reinterpret_cast<const uint4*>(x + (h + step) * 128 + 64);
+      }
       uint4 lo_out = lo_raw, hi_out = hi_raw;
       if (h < a.nq + a.nkv) {
         const uint32_t* pl = reinterpret_cast<const uint32_t*>(&lo_raw);

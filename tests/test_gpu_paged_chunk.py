@@ -167,13 +167,22 @@ def test_lengths_beyond_the_table_are_cut_and_reported(cuda_device):
     check(out, lse, ref, torch.float16)
 
 
-def test_rows_outside_every_sequence_stay(cuda_device, device_checks):
+@pytest.mark.parametrize("seqs", [[(5, 70), (9, 9)], [(2, 70), (1, 9)], [(45, 300)]])
+def test_rows_outside_every_sequence_stay(cuda_device, device_checks, seqs):
+    """A padded batch: rows behind the last sequence hold NaN and infinities, their outputs stay; so
+    do rows before the first."""
     from fast_infer_b200.kernels.attention import paged_chunk_attention
-    q, k, v, table, cu, ctx = (t.to(cuda_device) for t in make([(5, 70), (9, 9)], 6, 2, torch.float16))
-    q = torch.cat([q, q[:7]])
-    out = torch.full_like(q, 7.0)
-    got = paged_chunk_attention(q, k, v, table, PAGE, cu, ctx, out=out)
-    assert got.data_ptr() == out.data_ptr() and (out[14:] == 7.0).all() and not (out[:14] == 7.0).all()
+    q, k, v, table, cu, ctx = make(seqs, 6, 2, torch.float16)
+    n = q.shape[0]
+    pad = torch.full((4, 6, D), math.nan, dtype=q.dtype)
+    pad[2:] = math.inf
+    big = torch.cat([pad, q, pad]).to(cuda_device)
+    out = torch.full_like(big, 7.0)
+    got, lse = paged_chunk_attention(big, k.to(cuda_device), v.to(cuda_device), table.to(cuda_device), PAGE,
+                                     (cu + 4).to(cuda_device), ctx.to(cuda_device), out=out, return_lse=True)
+    assert got.data_ptr() == out.data_ptr()
+    assert (out[:4] == 7.0).all() and (out[4 + n:] == 7.0).all()
+    check(out[4:4 + n], lse[4:4 + n], oracle((q, k, v, table, cu, ctx)), torch.float16)
 
 
 def test_strides(cuda_device, device_checks):
