@@ -39,18 +39,20 @@ def _check_cuda_f16(name: str, t: torch.Tensor) -> None:
         raise TypeError(f"{name} must be float16, got {t.dtype}")
 
 
+@functools.lru_cache(maxsize=4096)
+def _tma_strides(shape, strides) -> bool:
+    if strides[-1] != 1:
+        return False
+    for i in range(len(strides) - 1):
+        if strides[i] % 8 != 0 and shape[i] != 1:
+            return False
+    return True
+
+
 def _tma_ready(t: torch.Tensor) -> bool:
     """True if the tensor can be addressed by a TMA map as is: 16-byte aligned base,
     unit innermost stride, every other stride a multiple of 8 elements."""
-    if t.data_ptr() % 16 != 0:
-        return False
-    st = t.stride()
-    if st[-1] != 1:
-        return False
-    for i in range(len(st) - 1):
-        if st[i] % 8 != 0 and t.shape[i] != 1:
-            return False
-    return True
+    return t.data_ptr() % 16 == 0 and _tma_strides(t.shape, t.stride())
 
 
 def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -245,11 +247,17 @@ _DTYPES = {torch.float16: _lib.FI_DTYPE_F16, torch.bfloat16: _lib.FI_DTYPE_BF16}
 
 
 def _int32_on(name: str, t: torch.Tensor, device: torch.device, count: int) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or t.device != device or t.shape != (count,):
+    if (not isinstance(t, torch.Tensor) or t.device != device or t.dim() != 1
+            or t.numel() != count):
         raise ValueError(f"{name} must be a 1-D int32 tensor of {count} values on {device}")
     if t.dtype != torch.int32:
         t = t.to(torch.int32)
     return t if t.is_contiguous() else t.contiguous()
+
+
+@functools.lru_cache(maxsize=4096)
+def _cache_shape(shape) -> bool:
+    return len(shape) == 4 and shape[3] == HEAD_DIM and 0 not in shape
 
 
 def _check_cache(name: str, t: torch.Tensor, like: torch.Tensor, shape) -> None:
@@ -261,7 +269,7 @@ def _check_cache(name: str, t: torch.Tensor, like: torch.Tensor, shape) -> None:
         raise TypeError(f"{name} must be float16 or bfloat16 like the new tokens, got {t.dtype}")
     if t.device != like.device:
         raise ValueError("all tensors must be on the same device")
-    if t.dim() != 4 or t.shape != shape or t.shape[3] != HEAD_DIM or t.numel() == 0:
+    if t.shape != shape or not _cache_shape(shape):
         raise ValueError(f"{name} must be [num_blocks, {BLOCK_SIZE}, num_kv_heads, {HEAD_DIM}]")
     if not _tma_ready(t):
         raise ValueError(f"{name} needs a 16-byte aligned base, unit innermost stride and "
@@ -287,9 +295,8 @@ def _batch_args(device, block_table, block_size, k_cache, cu_seqlens, context_le
     batch = cu_seqlens.numel() - 1
     cu = _int32_on("cu_seqlens", cu_seqlens, device, batch + 1)
     ctx = _int32_on("context_lens", context_lens, device, batch)
-    if (not isinstance(block_table, torch.Tensor) or block_table.dim() != 2
-            or block_table.device != device or block_table.shape[0] < batch
-            or block_table.shape[1] == 0):
+    shape = block_table.shape if isinstance(block_table, torch.Tensor) else ()
+    if len(shape) != 2 or block_table.device != device or shape[0] < batch or shape[1] == 0:
         raise ValueError("block_table must be [>= batch, max_blocks_per_seq] on the tokens' device")
     if block_table.dtype != torch.int32:
         block_table = block_table.to(torch.int32)

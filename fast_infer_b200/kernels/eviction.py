@@ -22,7 +22,8 @@ def _check_pools(what: str, k: torch.Tensor, v: torch.Tensor) -> None:
             raise ValueError(f"{what}{name} must be a CUDA tensor (fast_infer_b200 has no CPU path)")
         if t.dtype not in (torch.float16, torch.bfloat16):
             raise TypeError(f"{what}{name} must be float16 or bfloat16, got {t.dtype}")
-        if t.dim() != 5 or t.shape[2] != BLOCK_SIZE or t.shape[4] != HEAD_DIM:
+        shape = t.shape
+        if len(shape) != 5 or shape[2] != BLOCK_SIZE or shape[4] != HEAD_DIM:
             raise ValueError(f"{what}{name} must be [layers, num_blocks, {BLOCK_SIZE}, num_heads, "
                              f"{HEAD_DIM}]")
     if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
@@ -30,8 +31,9 @@ def _check_pools(what: str, k: torch.Tensor, v: torch.Tensor) -> None:
 
 
 def _check_table(name: str, t: torch.Tensor, batch: int, device: torch.device) -> None:
-    if (not isinstance(t, torch.Tensor) or t.dim() != 2 or t.shape[0] < batch or t.shape[1] == 0
-            or t.dtype != torch.int32 or t.device != device):
+    shape = t.shape if isinstance(t, torch.Tensor) else ()
+    if (len(shape) != 2 or shape[0] < batch or shape[1] == 0 or t.dtype != torch.int32
+            or t.device != device):
         raise ValueError(f"{name} must be a [>= batch, max_blocks] int32 tensor on the cache's device")
 
 
@@ -54,13 +56,14 @@ def evict_tokens(k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor,
     """
     _check_pools("", k, v)
     layers, num_blocks, _, heads, _ = k.shape
-    if not isinstance(seq_lens, torch.Tensor) or seq_lens.dim() != 1 or seq_lens.device != k.device:
+    device = k.device
+    if not isinstance(seq_lens, torch.Tensor) or seq_lens.dim() != 1 or seq_lens.device != device:
         raise ValueError("seq_lens must be a [batch] int32 tensor on the cache's device")
     batch = seq_lens.numel()
-    _check_table("block_table", block_table, batch, k.device)
+    _check_table("block_table", block_table, batch, device)
     if (not isinstance(mass, torch.Tensor) or mass.dim() != 4
             or mass.shape[:3] != (layers, batch, heads) or mass.dtype != torch.float32
-            or mass.device != k.device):
+            or mass.device != device):
         raise ValueError("mass must be a [layers, batch, num_heads, capacity] float32 tensor on the "
                          "cache's device")
     budget, recent, sinks = int(budget), int(recent), int(sinks)
@@ -72,22 +75,23 @@ def evict_tokens(k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor,
     else:
         k_out, v_out, table_out = out
         _check_pools("out ", k_out, v_out)
-        if (k_out.shape[0] != layers or k_out.shape[3] != heads or k_out.dtype != k.dtype
-                or k_out.device != k.device):
+        out_shape = k_out.shape
+        if (out_shape[0] != layers or out_shape[3] != heads or k_out.dtype != k.dtype
+                or k_out.device != device):
             raise ValueError("out pools need the same layers, heads, type and device as k and v")
-        _check_table("out block_table", table_out, batch, k.device)
+        _check_table("out block_table", table_out, batch, device)
     if budget > table_out.shape[1] * BLOCK_SIZE:
         raise ValueError(f"budget {budget} does not fit the block table")
     shape = (layers, batch, heads, budget)
-    kept = torch.empty(shape, dtype=torch.int32, device=k.device)
-    mass_out = torch.empty(shape, dtype=torch.float32, device=k.device)
+    kept = torch.empty(shape, dtype=torch.int32, device=device)
+    mass_out = torch.empty(shape, dtype=torch.float32, device=device)
     if kept.numel() == 0:
         return kept, mass_out
-    lens = seq_lens.to(torch.int32).contiguous()
-    mass = mass.contiguous()
+    lens = seq_lens if seq_lens.dtype == torch.int32 else seq_lens.to(torch.int32)
+    lens, mass = lens.contiguous(), mass.contiguous()
     lib = _lib.load()
-    with with_device(k.device):
-        err = error_word(k.device)
+    with with_device(device):
+        err = error_word(device)
         st = lib.fi_kv_evict(
             k.data_ptr(), v.data_ptr(), block_table.data_ptr(), lens.data_ptr(), mass.data_ptr(),
             k_out.data_ptr(), v_out.data_ptr(), table_out.data_ptr(), kept.data_ptr(),
@@ -96,7 +100,7 @@ def evict_tokens(k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor,
             sinks, _lib.strides(*k.stride()), _lib.strides(*v.stride()),
             _lib.strides(*k_out.stride()), _lib.strides(*v_out.stride()),
             _lib.strides(*block_table.stride()), _lib.strides(*table_out.stride()),
-            err.data_ptr() if err is not None else None, stream_of(k.device))
+            err.data_ptr() if err is not None else None, stream_of(device))
         _lib.check(st, "evict_tokens")
         device_errors(err, "evict_tokens")
     return kept, mass_out
