@@ -54,6 +54,8 @@ int chunk_score_args(ScoreForm& f, const char* what, float sm_scale, float softc
   f.cap_in = softcap > 0.f ? (float)((double)sm_scale / (double)softcap) : 0.f;
   f.cap_log2 = (float)((double)softcap * log2e);
   f.slopes = slopes;
+  if (!isfinite(f.cap_in) || !isfinite(f.scale_log2) || !isfinite(f.cap_log2))
+    return fail(FI_ERR_INVALID_ARG, "%s: sm_scale or softcap outside what fp32 scores hold", what);
   return FI_OK;
 }
 

@@ -72,7 +72,7 @@ struct CkBarriers {
   uint64_t unit_full[kCkSlots], unit_empty[kCkSlots];
   uint64_t merge;  // both softmax warpgroups, in a transposed unit
   uint32_t tmem_base;
-  // transposed units, per warpgroup: rows' max, partial maxima / sums, scale, slope, position
+  // transposed units, per warpgroup: rows' max, partial maxima / sums, scale, slope, token
   float n_max[2][kCkNarrow], n_red[2][4][kCkNarrow], n_alpha[2][kCkNarrow];
   alignas(16) float n_neg[2][kCkNarrow];  // -max
   float n_slope[2][kCkNarrow], n_pos[2][kCkNarrow];
@@ -261,7 +261,8 @@ __device__ __forceinline__ void score_form(uint32_t* sr, const ScoreForm& f, flo
   }
 }
 
-// 8 scores of one key in log2 units, one per row of a transposed unit.
+// 8 scores of one key in log2 units, one per row of a transposed unit. `pos` and `key` count from
+// the unit's first token, so that distances are exact at any position.
 template <bool kCap, bool kAlibi>
 __device__ __forceinline__ void score_form8(const uint32_t* raw, float* s, const ScoreForm& f,
                                              const float* slope2, const float* pos, float key) {
@@ -359,7 +360,7 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
     if (kAlibi) {
       const bool live = tid < rows;
       bars->n_slope[t][tid] = live ? p.f.slopes[u.hk * pb.group + bars->row_head[tid]] * kLog2e : 0.f;
-      bars->n_pos[t][tid] = (float)(u.pos + bars->row_token[tid]);
+      bars->n_pos[t][tid] = (float)bars->row_token[tid];
     }
   }
   __syncwarp();
@@ -395,6 +396,7 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
     }
     if (!page_ok || key >= u.keys) c_hi = 0;
     const bool mask = !__all_sync(0xffffffffu, c_lo <= 0 && c_hi >= rows);
+    const uint32_t vis = low_bits(c_hi, 0) & ~low_bits(c_lo, 0);
     float s[kCkNarrow];  // scores in log2 units, then 2^(score - max)
     // the first tile sets the rows' max; later ones keep it unless some score passes it by 2^8
 #pragma unroll 1
@@ -409,12 +411,11 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
       for (int cc = 0; cc < kCkNarrow; cc += 8)
         if (cc < rows) {
           score_form8<kCap, kAlibi>(raw + cc, s + cc, p.f, bars->n_slope[t] + cc, bars->n_pos[t] + cc,
-                                     (float)key);
+                                     (float)(key - u.pos));
           if (mask) {
-            const uint32_t vis = low_bits(c_hi - cc, 0) & ~low_bits(c_lo - cc, 0);
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-              if (!((vis >> c) & 1u)) s[cc + c] = -INFINITY;
+            for (int c = cc; c < cc + 8; ++c)
+              if (!((vis >> c) & 1u)) s[c] = -INFINITY;
           }
         }
       if (move) {
@@ -471,8 +472,9 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
         }
       }
       // A row that has seen nothing has max -inf: a score it sees gives 2^inf, past any bound; one
-      // it does not see gives NaN, which the maximum below passes over and the mask sets to 0. A
-      // column without a row has max +inf: p = 0.
+      // it does not see gives NaN, which the maximum below passes over and the mask sets to 0 (a
+      // score that is NaN stays: the row's result shows it). A column without a row has max +inf:
+      // p = 0.
       float top = 0.f;
 #pragma unroll
       for (int cc = 0; cc < kCkNarrow; cc += 8)
@@ -488,7 +490,8 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
           }
           if (mask) {
 #pragma unroll
-            for (int c = cc; c < cc + 8; ++c) s[c] = fmaxf(s[c], 0.f);  // NaN -> 0
+            for (int c = cc; c < cc + 8; ++c)
+              if (!((vis >> c) & 1u)) s[c] = 0.f;
           }
         }
       if (move || wg_bar_and(1 + t, top <= kTop)) break;

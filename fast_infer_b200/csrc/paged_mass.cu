@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(kMsThreads, 1)
           bars->neg_lse[ls][c] = now[i] == -INFINITY ? -INFINITY : -now[i] * kLog2e;
           if (kAlibi) {
             bars->slope[ls][c] = sl[i];
-            bars->pos[ls][c] = (float)(u.pos0 + q * pb.tile_tokens + tok[i]);
+            bars->pos[ls][c] = (float)(q * pb.tile_tokens + tok[i]);  // from the first new token
           }
           now[i] = next[i];
         }
@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(kMsThreads, 1)
             for (int c = 0; c < 16; c += 4) {
               const float4 sl = *reinterpret_cast<const float4*>(&bars->slope[ls][cc + c]);
               const float4 ps = *reinterpret_cast<const float4*>(&bars->pos[ls][cc + c]);
-              const float k = (float)key;
+              const float k = (float)(key - u.pos0);
               x[c] = fmaf(-sl.x, fabsf(k - ps.x), x[c]);
               x[c + 1] = fmaf(-sl.y, fabsf(k - ps.y), x[c + 1]);
               x[c + 2] = fmaf(-sl.z, fabsf(k - ps.z), x[c + 2]);

@@ -368,7 +368,8 @@ def paged_chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     Token p sees key j when j <= p (and j > p - window, if ``window``), or j < prefix_lens[b];
     never past context_lens[b]. Scores are ``q.k * sm_scale``, capped as ``softcap * tanh(x /
     softcap)`` if ``softcap``, less ``alibi_slopes[head] * |p - j|`` if given (fp32 [num_q_heads]).
-    A token that sees nothing gives zeros and an lse of -inf.
+    A token that sees nothing gives zeros and an lse of -inf. Slots past context_lens[b] may hold
+    anything; V before them has to be finite, seen or not (hidden keys count with weight 0).
 
     Returns o like q (written to ``out`` if given; rows outside every sequence are not written),
     and with ``return_lse`` also lse: fp32 [total_tokens, num_q_heads], the natural log of the sum

@@ -193,7 +193,8 @@ int fi_paged_decode_noalloc(const void* q, const void* k_cache, const void* v_ca
  * softcap) when softcap > 0 (alibi_slopes: fp32 [num_q_heads] or NULL). sm_scale > 0.
  * o = softmax over the visible keys . v; lse (fp32 [total_tokens, num_q_heads] or NULL) = the
  * natural log of the sum of exp(score). A token that sees nothing gets o = 0, lse = -inf.
- * Slots behind a sequence's last token may hold anything. A page whose block-table entry is
+ * Slots behind a sequence's last token may hold anything; V of a cached token has to be finite even
+ * where a token does not see it (it counts with weight 0). A page whose block-table entry is
  * invalid is skipped (FI_DEVERR_BAD_BLOCK); lengths that do not fit total_tokens or the block
  * table are cut and set FI_DEVERR_CONTEXT_LEN.
  * dtype: of q, k_cache, v_cache and o. workspace: fi_paged_chunk_workspace_size(...) bytes,

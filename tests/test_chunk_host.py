@@ -41,8 +41,9 @@ def test_chunk_and_mass_refusals(call):
                 dict(scale=INF), dict(ptr=None)):
         assert call(lib, **bad) == BAD, bad
     soft = "softcap" if call is _mass else "cap"
-    for x in (-1.0, NAN, INF):
+    for x in (-1.0, NAN, INF, 1e-45, 3e38):  # (the last two: scale / cap or cap * log2(e) past fp32)
         assert call(lib, **{soft: x}) == BAD
+    assert call(lib, scale=3e38) == BAD
     for unsup in (dict(d=64), dict(bs=16), dict(hq=130, hk=2), dict(batch=2049), dict(total=(1 << 28) + 1),
                   dict(mb=(1 << 20) + 1)):
         assert call(lib, **unsup) == UNSUPPORTED, unsup

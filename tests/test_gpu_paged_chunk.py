@@ -269,3 +269,49 @@ def test_many_sequences(cuda_device, device_checks):
     check(*run(batch, cuda_device), oracle(batch), torch.float16)
     with pytest.raises(RuntimeError, match="split the batch"):
         run(make(seqs + [(1, 1)], 2, 1, torch.float16), cuda_device)
+
+
+@pytest.mark.parametrize("hq,hk,new,ctx", [(4, 1, 8, 8), (4, 1, 7, 300), (6, 2, 150, 400), (8, 8, 20, 20)])
+def test_nan_keys_show_where_they_are_seen(cuda_device, device_checks, hq, hk, new, ctx):
+    """A NaN key makes NaN of the rows that see it and leaves those before it as they were."""
+    batch = make([(new, ctx)], hq, hk, torch.float16)
+    bad = new // 2  # a new token
+    slot = ctx - new + bad
+    batch[1][batch[3][0, slot // PAGE], slot % PAGE] = math.nan
+    out, lse = run(batch, cuda_device)
+    ref = oracle(batch)  # (takes a NaN key for one that no row sees)
+    check(out[:bad], lse[:bad], tuple(x[:bad] for x in ref), torch.float16)
+    assert torch.isnan(out[bad:]).all() and torch.isnan(lse[bad:]).all()
+
+
+@pytest.mark.parametrize("hq,hk,new", [(2, 1, 3), (2, 1, 90)])
+def test_distances_at_far_positions(cuda_device, device_checks, hq, hk, new):
+    """Past 2^24 positions are not fp32 numbers, but distances within the window are: scores are off
+    by the rounding of slope * distance (2^-24 * 2^8 in log2 units) beside what `check` counts."""
+    from fast_infer_b200.kernels.attention import attention_mass
+    g = torch.Generator().manual_seed(5)
+    ctx, window = (1 << 24) + 5003, 200
+    k, v = (torch.randn(5, PAGE, hk, D, generator=g).half() for _ in range(2))
+    table = torch.randint(0, 5, (1, ctx // PAGE + 1), generator=g).int()
+    q = torch.randn(new, hq, D, generator=g).half()
+    slopes = torch.tensor([0.5, 0.25])
+    # the same keys as a short sequence: pages from the one that holds the first visible key
+    first = (ctx - new - window) // PAGE
+    short = (q, k, v, table[:, first:], torch.tensor([0, new]).int(),
+             torch.tensor([ctx - first * PAGE]).int())
+    ref = oracle(short, alibi_slopes=slopes, window=window)
+    far = tuple(t.to(cuda_device) for t in
+                (q, k, v, table, torch.tensor([0, new]).int(), torch.tensor([ctx]).int()))
+    form = dict(alibi_slopes=slopes, window=window)
+    out, lse = run(far, cuda_device, **form)
+    check(out, lse, ref, torch.float16)
+    near = run(short, cuda_device, **form)
+    got = attention_mass(far[0], far[1], far[3], PAGE, far[4], far[5], near[1],
+                         alibi_slopes=slopes.to(cuda_device), window=window)
+    s = tuple(t.to(cuda_device) for t in short)
+    want = attention_mass(s[0], s[1], s[3], PAGE, s[4], s[5], near[1],
+                          alibi_slopes=slopes.to(cuda_device), window=window)
+    n = want.shape[2]
+    # (each within 2^-15 relative of the definition: see the tests of attention_mass)
+    assert ((got[:, :, first * PAGE:first * PAGE + n] - want).abs() <= want * 2.0 ** -14).all()
+    assert not got[:, :, :first * PAGE].any()
