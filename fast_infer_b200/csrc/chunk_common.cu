@@ -54,6 +54,16 @@ int chunk_score_args(ScoreForm& f, const char* what, float sm_scale, float softc
   f.cap_in = softcap > 0.f ? (float)((double)sm_scale / (double)softcap) : 0.f;
   f.cap_log2 = (float)((double)softcap * log2e);
   f.slopes = slopes;
+  // tanh(u) / u in u^2 on |u| <= 1/3, minimax (2.4e-8 before the coefficients' rounding); where their
+  // powers of cap_in could leave fp32's range, no score takes this form
+  const double c[4] = {0.9999999763, -0.3333264747, 0.1330220246, -0.04939617807};
+  f.tiny_max = -1.f;
+  if (f.cap_in > 1e-5f && f.cap_in < 1e4f) {
+    const double in = (double)sm_scale / (double)softcap;
+    double to = (double)sm_scale * log2e;
+    for (int i = 0; i < 4; ++i, to *= in * in) f.tiny[i] = (float)(c[i] * to);
+    f.tiny_max = (float)(1.0 / 3.0 / in);
+  }
   if (!isfinite(f.cap_in) || !isfinite(f.scale_log2) || !isfinite(f.cap_log2))
     return fail(FI_ERR_INVALID_ARG, "%s: sm_scale or softcap outside what fp32 scores hold", what);
   return FI_OK;

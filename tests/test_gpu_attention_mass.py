@@ -159,3 +159,10 @@ def test_many_sequences(cuda_device, device_checks):
     batch = make(seqs, 2, 1, torch.float16)
     lse = oracle(batch)[1].float()
     check(run(batch, cuda_device, lse), oracle_mass(batch, lse))
+
+
+@pytest.mark.parametrize("softcap", [1e-3, 1e6])
+def test_caps_far_from_the_scores(cuda_device, device_checks, softcap):
+    batch = make([(20, 200), (1, 77), (100, 130)], 4, 2, torch.float16)
+    lse = oracle(batch, softcap=softcap)[1].float()
+    check(run(batch, cuda_device, lse, softcap=softcap), oracle_mass(batch, lse, softcap=softcap))

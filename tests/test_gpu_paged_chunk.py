@@ -315,3 +315,10 @@ def test_distances_at_far_positions(cuda_device, device_checks, hq, hk, new):
     # (each within 2^-15 relative of the definition: see the tests of attention_mass)
     assert ((got[:, :, first * PAGE:first * PAGE + n] - want).abs() <= want * 2.0 ** -14).all()
     assert not got[:, :, :first * PAGE].any()
+
+
+@pytest.mark.parametrize("softcap", [1e-3, 1e6])
+def test_caps_far_from_the_scores(cuda_device, device_checks, softcap):
+    """All scores at the cap's ends, and a cap that changes none."""
+    batch = make([(20, 200), (1, 77), (100, 130)], 4, 2, torch.float16)
+    check(*run(batch, cuda_device, softcap=softcap), oracle(batch, softcap=softcap), torch.float16)
