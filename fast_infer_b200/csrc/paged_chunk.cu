@@ -96,12 +96,15 @@ struct ChunkParams {
   void* o;
   int64_t os[2];
   float* lse;  // [total, hq] or null
-  float* ws_o;    // [cta][first, last unit][rows_cap][128]
+  // [cta][first, last unit], then rows_cap rows of 128: as they are (narrow), or 32 rows' 4 values
+  // side by side (wide, whose threads have a row each)
+  float* ws_o;
   float* ws_lse;  // [cta][first, last unit][rows_cap], log2 domain
   CkJoin* join;   // [cta]
   int rows_cap;
   int unit_tokens;  // tokens of a unit: two tiles, or those of kCkNarrow rows
   int split_rows;   // sequences of at most so many rows are the narrow kernel's, others the wide's
+  int o_wide;       // rows of o are 32-byte aligned
   int late_wait;    // the kernel before on the stream is the other one of this call
   int* err;
 };
@@ -1047,7 +1050,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       const int64_t out_row = u.token + t * pb.tile_tokens + tok;
       const int64_t part = (int64_t)(cta * 2 + (begins ? 1 : 0)) * p.rows_cap + t * 128 + row;
       T* orow = static_cast<T*>(p.o) + out_row * p.os[0] + head * p.os[1];
-      float* prow = p.ws_o + part * 128;
+      float* prow = p.ws_o + (part & ~31) * 128 + (part & 31) * 4;
       if (warp_live) {
 #pragma unroll 1
         for (int cc = 0; cc < 128; cc += 32) {
@@ -1060,18 +1063,22 @@ __global__ void __launch_bounds__(kCkThreads, 1)
             ov[e] = none ? 0u : __float_as_uint(__uint_as_float(ov[e]) * inv);
           if (live && begins && ends) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              uint4 v;
-              v.x = Half16<T>::pack(__uint_as_float(ov[e]), __uint_as_float(ov[e + 1]));
-              v.y = Half16<T>::pack(__uint_as_float(ov[e + 2]), __uint_as_float(ov[e + 3]));
-              v.z = Half16<T>::pack(__uint_as_float(ov[e + 4]), __uint_as_float(ov[e + 5]));
-              v.w = Half16<T>::pack(__uint_as_float(ov[e + 6]), __uint_as_float(ov[e + 7]));
-              *reinterpret_cast<uint4*>(orow + cc + e) = v;
+            for (int e = 0; e < 32; e += 16) {
+              uint32_t pk[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                pk[i] = Half16<T>::pack(__uint_as_float(ov[e + 2 * i]), __uint_as_float(ov[e + 2 * i + 1]));
+              if (p.o_wide) {
+                st_global_v8(orow + cc + e, pk);
+              } else {
+                *reinterpret_cast<uint4*>(orow + cc + e) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                *reinterpret_cast<uint4*>(orow + cc + e + 8) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
+              }
             }
           } else if (live) {
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<uint4*>(prow + cc + e) =
+              *reinterpret_cast<uint4*>(prow + (cc + e) * 32) =
                   make_uint4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
           }
         }
@@ -1101,55 +1108,59 @@ __global__ void __launch_bounds__(kCkThreads, 1)
   }
 }
 
-// Joins the parts of a unit that several CTAs hold: weights 2^(lse_part - max). A warp per row.
-// Blocks [0, ctas) join `p`'s units, blocks [ctas, 2 * ctas) those of `p2`.
+// Joins the parts of a unit that several CTAs hold: weights 2^(lse_part - max), the max running.
+// A block joins 8 rows of one CTA's unit: `p`'s first, then `p2`'s. A thread has 4 values of a row: a
+// warp those of one row, or of 8 rows where 32 rows lie side by side.
 template <typename T>
-__global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p,
-                                                            const ChunkParams p2, int ctas) {
+__global__ void __launch_bounds__(256, 8) chunk_combine_kernel(const ChunkParams p,
+                                                               const ChunkParams p2) {
   grid_dep_wait();
   grid_dep_launch();
-  const bool second = (int)blockIdx.x >= ctas;
-  const int cta = blockIdx.x - (second ? ctas : 0), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool second = (int)blockIdx.y >= p.rows_cap / 8;
+  const int cta = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r0 = ((int)blockIdx.y - (second ? p.rows_cap / 8 : 0)) * 8;
   const CkJoin jn = second ? p2.join[cta] : p.join[cta];
   if (!jn.valid) return;
   const int rows_cap = second ? p2.rows_cap : p.rows_cap;
+  const bool by_row = rows_cap == kCkNarrow;
   const float* ws_lse = second ? p2.ws_lse : p.ws_lse;
   const float* ws_o = second ? p2.ws_o : p.ws_o;
-#pragma unroll 1
-  for (int r = blockIdx.y * 8 + warp; r < rows_cap; r += gridDim.y * 8) {
-    const int t = r >> 7, row = r & 127;
-    if (row >= (t ? jn.rows[1] : jn.rows[0])) continue;
-    auto at = [&](int c) { return (int64_t)(c * 2 + (c == cta ? 1 : 0)) * rows_cap + r; };
-    float mx = -INFINITY;
-    for (int c = cta + lane; c <= jn.last_cta; c += 32) mx = fmaxf(mx, ws_lse[at(c)]);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-    const bool none = mx == -INFINITY;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-    if (!none) {
-#pragma unroll 4
-      for (int c = cta; c <= jn.last_cta; ++c) {
-        const float wgt = exp2f(ws_lse[at(c)] - mx);
-        const float4 v = *reinterpret_cast<const float4*>(ws_o + at(c) * 128 + lane * 4);
-        sum += wgt;
-        acc.x = fmaf(wgt, v.x, acc.x);
-        acc.y = fmaf(wgt, v.y, acc.y);
-        acc.z = fmaf(wgt, v.z, acc.z);
-        acc.w = fmaf(wgt, v.w, acc.w);
-      }
+  const int r = r0 + (by_row ? warp : lane & 7), t = r >> 7, row = r & 127;
+  const int col = (by_row ? lane : warp * 4 + (lane >> 3)) * 4;
+  if (row >= (t ? jn.rows[1] : jn.rows[0])) return;
+  const int off = by_row ? r * 128 + col : (r & ~31) * 128 + col * 32 + (r & 31) * 4;
+  float mx = -INFINITY, sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+  for (int c = cta; c <= jn.last_cta; ++c) {
+    const int at = (c * 2 + (c == cta ? 1 : 0)) * rows_cap;
+    const float l = ws_lse[at + r];
+    const float4 v = *reinterpret_cast<const float4*>(ws_o + at * 128 + off);
+    if (l > mx) {
+      const float a = exp2f(mx - l);
+      mx = l;
+      sum *= a;
+      acc.x *= a;
+      acc.y *= a;
+      acc.z *= a;
+      acc.w *= a;
     }
-    const float inv = none ? 0.f : 1.f / sum;
-    const int token = jn.token + t * p.b.tile_tokens + row / p.b.group;
-    const int head = jn.hk * p.b.group + row % p.b.group;
-    uint2 pk;
-    pk.x = Half16<T>::pack(acc.x * inv, acc.y * inv);
-    pk.y = Half16<T>::pack(acc.z * inv, acc.w * inv);
-    T* orow = static_cast<T*>(p.o) + (int64_t)token * p.os[0] + head * p.os[1];
-    *reinterpret_cast<uint2*>(orow + lane * 4) = pk;
-    if (lane == 0 && p.lse)
-      p.lse[(int64_t)token * p.b.hq + head] = none ? -INFINITY : (mx + log2f(sum)) * kLn2;
+    const float wgt = l == -INFINITY ? 0.f : exp2f(l - mx);
+    sum += wgt;
+    acc.x = fmaf(wgt, v.x, acc.x);
+    acc.y = fmaf(wgt, v.y, acc.y);
+    acc.z = fmaf(wgt, v.z, acc.z);
+    acc.w = fmaf(wgt, v.w, acc.w);
   }
+  const bool none = sum == 0.f;
+  const float inv = none ? 0.f : 1.f / sum;
+  const int64_t token = jn.token + t * p.b.tile_tokens + row / p.b.group;
+  const int head = jn.hk * p.b.group + row % p.b.group;
+  uint2 pk;
+  pk.x = Half16<T>::pack(acc.x * inv, acc.y * inv);
+  pk.y = Half16<T>::pack(acc.z * inv, acc.w * inv);
+  *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + token * p.os[0] + head * p.os[1] + col) = pk;
+  if (col == 0 && p.lse) p.lse[token * p.b.hq + head] = none ? -INFINITY : (mx + log2f(sum)) * kLn2;
 }
 
 template <typename T, bool kCap, bool kAlibi, bool kNarrow>
@@ -1191,10 +1202,9 @@ static int launch_chunk(const CUtensorMap& tq_n, const CUtensorMap& tq_w, const 
   if (r == FI_OK && wide) r = launch_form<T, false>(tq_w, tk, tv, *wide, st);
   if (r != FI_OK) return r;
   const ChunkParams& first = wide ? *wide : *narrow;
-  const int ctas = sm_count();
-  const cudaError_t e =
-      launch_pdl(chunk_combine_kernel<T>, dim3((unsigned)(narrow && wide ? 2 * ctas : ctas), (unsigned)(first.rows_cap / 8)),
-                 dim3(256), 0, st, first, narrow ? *narrow : first, ctas);
+  const int parts = (first.rows_cap + (narrow && wide ? narrow->rows_cap : 0)) / 8;
+  const cudaError_t e = launch_pdl(chunk_combine_kernel<T>, dim3((unsigned)sm_count(), (unsigned)parts),
+                                   dim3(256), 0, st, first, narrow ? *narrow : first);
   return e == cudaSuccess ? FI_OK : cuda_fail(e, "fi_paged_chunk: combine launch");
 }
 
@@ -1294,6 +1304,7 @@ extern "C" int fi_paged_chunk(const void* q, const void* k_cache, const void* v_
   p.o = o;
   p.os[0] = o_strides[0];
   p.os[1] = o_strides[1];
+  p.o_wide = reinterpret_cast<uintptr_t>(o) % 32 == 0 && o_strides[0] % 16 == 0 && o_strides[1] % 16 == 0;
   p.lse = lse;
   p.err = error_flag;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
