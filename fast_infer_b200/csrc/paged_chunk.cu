@@ -42,6 +42,11 @@ constexpr int kCkMaxUnits = 4608;    // token units per launch (per KV head)
 constexpr int kCkNarrow = 32;        // rows up to which a unit runs transposed
 constexpr float kCkRescale = 8.0f;   // log2 units of growth of the max before O is rescaled
 constexpr int kCkEmuPairs = 1;       // of 8 column pairs, exp2 on the FMA pipe
+// Steps that a unit's start and end are worth: with 0 and 0 / 1 and 2 / 3 and 2 / 4 and 3, 64 single
+// tokens over 1000 with 2048 new over 2000 take 177 / 170 / 168 / 171 us, and 64 over 4000 with 512 new
+// (units of the narrow kernel, all in a few CTAs' parts) 294 / 252 / 200 / 201.
+constexpr int kCkPadNarrow = 3, kCkPadWide = 2;
+constexpr int kCkManyNew = 500;      // new tokens past one each that the wide kernel is launched for
 constexpr int kCkSlots = 4;          // units that the scheduler is ahead
 
 // A CTA's part of a unit: key steps [j0, j1) of its n.
@@ -81,7 +86,7 @@ struct CkBarriers {
   uint8_t row_token[kChunkTile], row_head[kChunkTile];  // of a tile's rows
   uint32_t warp_sums[kCkThreads / 32];
   uint32_t unit_off[kCkMaxBatch + 1];  // first unit of each sequence
-  uint32_t work[kCkMaxUnits + 1];      // key tiles before each unit
+  uint32_t work[kCkMaxUnits + 1];      // steps before each unit
 };
 constexpr int kCkSmemBytes = 1024 + (2 + 2 * kCkStages) * kChunkTileBytes + (int)sizeof(CkBarriers);
 static_assert(kCkSmemBytes <= 227 * 1024, "shared memory");
@@ -127,22 +132,23 @@ __device__ __forceinline__ void ck_tiles(const ChunkBatch& p, const ChunkSeq& s,
 
 // The scheduler (one warp): walks the CTA's part of the line and hands its units to the other
 // roles through a ring in shared memory. Its lanes look the units' pages over, so that no one
-// else has to unless an entry is invalid.
-__device__ __forceinline__ void ck_schedule(const ChunkBatch& p, int unit_tokens, CkBarriers* s,
-                                            uint32_t units, CkJoin* join_out, int* err) {
+// else has to unless an entry is invalid. On the line a unit is `pad` steps longer than its key tiles,
+// which stand for what it costs to begin and end one; its step j is at pad + j.
+__device__ __forceinline__ void ck_schedule(const ChunkBatch& p, int unit_tokens, int pad,
+                                            CkBarriers* s, uint32_t units, CkJoin* join_out, int* err) {
   const int G = gridDim.x, cta = blockIdx.x, lane = threadIdx.x & 31;
   const uint32_t per_head = s->work[units];
   const int64_t total = (int64_t)per_head * p.hk;
   const int active = (int)(total < G ? total : G);  // CTAs with work
   int64_t w = cta < active ? total * cta / active : 0;
   const int64_t end = cta < active ? total * (cta + 1) / active : 0;
-  int hk = 0, e = 0, b = 0, j0 = 0;
+  int hk = 0, e = 0, b = 0, at = 0;  // `at`: where in the unit this CTA begins
   if (w < end) {
     hk = (int)(w / per_head);
     const uint32_t r = (uint32_t)(w - (int64_t)hk * per_head);
     e = last_le(s->work, (int)units, r);
     b = last_le(s->unit_off, p.batch, (uint32_t)e);
-    j0 = (int)(r - s->work[e]);
+    at = (int)(r - s->work[e]);
   }
   ChunkSeq q = chunk_seq(p, b);
   const int tt = p.tile_tokens;
@@ -154,13 +160,15 @@ __device__ __forceinline__ void ck_schedule(const ChunkBatch& p, int unit_tokens
         !__all_sync(0xffffffffu, mbar_wait(&s->unit_empty[slot], ((i / kCkSlots) - 1) & 1, err)))
       break;
     CkUnit u;
-    u.valid = w < end;
+    const int len = w < end ? (int)(s->work[e + 1] - s->work[e]) : 0;
+    const int stop = len - at <= end - w ? len : at + (int)(end - w);
+    u.valid = stop > pad;  // (not so: no unit, or one whose steps are all in the next CTA)
     bool pages_ok = true;
     if (u.valid) {
       const int t0 = (e - (int)s->unit_off[b]) * unit_tokens, t1 = min(t0 + unit_tokens, q.n);
       int tiles;
       ck_tiles(p, q, t0, t1, u.np, u.lo, tiles);
-      u.n = (int)(s->work[e + 1] - s->work[e]);  // the line's own count: the walk always ends
+      u.n = len - pad;  // the line's own count: the walk always ends
       u.b = b;
       u.hk = hk;
       u.token = q.start + t0;
@@ -169,17 +177,17 @@ __device__ __forceinline__ void ck_schedule(const ChunkBatch& p, int unit_tokens
       u.prefix = q.prefix;
       u.rows[0] = min(t1 - t0, tt) * p.group;
       u.rows[1] = max(t1 - t0 - tt, 0) * p.group;
-      u.j0 = j0;
-      u.j1 = (int)(u.n - j0 <= end - w ? u.n : j0 + (end - w));
-      // the last step of the unit, w - j0 + n - 1, belongs to the last CTA that starts at or before it
-      u.last_cta = u.j1 == u.n ? cta : (int)(((w - j0 + u.n) * active - 1) / total);
+      u.j0 = max(at - pad, 0);
+      u.j1 = stop - pad;
+      // the last step of the unit, w - at + len - 1, belongs to the last CTA that starts at or before it
+      u.last_cta = stop == len ? cta : (int)(((w - at + len) * active - 1) / total);
       for (int j = u.j0 + (lane >> 1); j < u.j1; j += 16) {
         const int tile = ck_tile(u, j), half = lane & 1;
         if ((tile * 2 + half) * kChunkPage < u.keys && chunk_page(p, b, u.keys, tile, half) == p.num_blocks)
           pages_ok = false;
       }
-      w += u.j1 - u.j0;
-      j0 = 0;
+      w += stop - at;
+      at = 0;
       if (++e == (int)units) {
         e = 0;
         ++hk;
@@ -656,6 +664,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
     bars->row_token[threadIdx.x] = (uint8_t)(threadIdx.x / pb.group);
     bars->row_head[threadIdx.x] = (uint8_t)(threadIdx.x % pb.group);
   }
+  constexpr int kPad = kNarrow ? kCkPadNarrow : kCkPadWide;
   bool single = true;  // at most one unit in each of this thread's sequences
 #pragma unroll 1
   for (int b = threadIdx.x; b < pb.batch; b += kCkThreads) {
@@ -668,7 +677,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
     if (n == 1) {
       int np, lo, tiles;
       ck_tiles(pb, q, 0, q.n, np, lo, tiles);
-      bars->work[b + 1] = (uint32_t)tiles;
+      bars->work[b + 1] = (uint32_t)(tiles + kPad);
     }
   }
   uint32_t units;
@@ -688,7 +697,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       const int t0 = (e - (int)bars->unit_off[b]) * p.unit_tokens;
       int np, lo, n;
       ck_tiles(pb, q, t0, min(t0 + p.unit_tokens, q.n), np, lo, n);
-      bars->work[e + 1] = (uint32_t)n;
+      bars->work[e + 1] = (uint32_t)(n + kPad);
     }
     __syncthreads();
   }
@@ -762,7 +771,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
         }
       }
     } else if (warp == 10) {
-      ck_schedule(pb, p.unit_tokens, bars, units, p.join + cta, p.err);
+      ck_schedule(pb, p.unit_tokens, kPad, bars, units, p.join + cta, p.err);
     } else if (warp == 9 && lane == 0) {
       // ---------------------------------------------------------- UMMA issuer
       constexpr uint32_t idesc_qk = umma_idesc<T>(128, 128, 0, 0);
@@ -1267,10 +1276,14 @@ extern "C" int fi_paged_chunk(const void* q, const void* k_cache, const void* v_
     return fail(FI_ERR_INVALID_ARG, "fi_paged_chunk: null pointer argument");
   // Batches of few tokens per sequence (on average at most kCkNarrow rows) are the narrow
   // kernel's alone: a sequence with more tokens is several units there, which read its keys once
-  // each (from L2). One sequence with more is the wide kernel's. Other batches may hold both.
+  // each (from L2), unless there are many new tokens: 512 of one sequence over 2000 beside 64
+  // single ones over 4000 take 238 us there and 219 in both kernels, but the wide one costs 11 us
+  // when it has nothing to do. One sequence with more is the wide kernel's. Other batches may hold
+  // both.
   const int64_t per_unit = p.b.group <= kCkNarrow ? kCkNarrow / p.b.group : 0;
   const bool use_narrow = per_unit > 0 && (batch > 1 || total_tokens <= per_unit);
-  const bool use_wide = per_unit == 0 || total_tokens > batch * per_unit;
+  const bool use_wide =
+      per_unit == 0 || total_tokens > batch * per_unit || total_tokens - batch >= kCkManyNew;
   const int64_t unit_tokens = use_wide ? 2 * p.b.tile_tokens : per_unit;
   if (batch > kCkMaxBatch ||
       (total_tokens + unit_tokens - 1) / unit_tokens + batch > kCkMaxUnits)

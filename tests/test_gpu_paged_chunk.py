@@ -82,6 +82,8 @@ SEQS = {
     "decode_batch": [(1, c) for c in (1, 63, 64, 65, 400, 129, 250, 7, 191, 320)],
     "mixed": [(1, 300), (130, 131), (7, 500), (1, 1), (90, 90), (2, 66)],
     "few_tokens_but_one": [(1, 100)] * 9 + [(60, 300), (0, 5)],
+    "many_tokens_in_one": [(1, 70)] * 70 + [(600, 650), (0, 9), (15, 40)],
+    "many_tokens_in_few_rows_each": [(9, 30 + i) for i in range(80)],
     "cached_missing": [(5, 3), (4, 0), (150, 100)],  # fewer cached tokens than new ones
 }
 
