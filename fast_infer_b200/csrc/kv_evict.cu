@@ -6,15 +6,15 @@
 // keeps its order and moves to slots 0 .. budget-1, of the same pages (in place) or of another
 // pool's.
 //
-// Two launches. evict_select_kernel, a CTA per (layer, sequence, KV head), finds the weight of
-// the last token that stays, the edge, by its bits: a non-negative float orders like its bits.
-// One histogram of 2048 bins over the 16 octaves below the greatest weight leaves a bin of few
-// weights, among which the edge is found by rank. Where that bin holds many (weights far below
-// the greatest, or equal), three histograms of the plain bits (11, 11 and 10, from the top) do
-// it instead (taken first, 88 us for 28 layers x 8 heads of 32768 tokens against 62; counting bit
-// by bit in registers, 109). Then each warp lists what it keeps of its run of tokens. evict_copy_kernel moves
-// the rows, 256 bytes each: bound by HBM (600 us for 3.76 GB read and written), so it keeps many
-// independent 16-byte loads in flight.
+// evict_row_kernel, a CTA per (layer, sequence, KV head), finds the weight of the last token that
+// stays, the edge, by its bits: a non-negative float orders like its bits. One histogram of 2048
+// bins over the 16 octaves below the greatest weight leaves a bin of few weights, among which the
+// edge is found by rank. Where that bin holds many (weights far below the greatest, or equal),
+// three histograms of the plain bits (11, 11 and 10, from the top) do it instead (taken first, 88
+// us for 28 layers x 8 heads of 32768 tokens against 62; counting bit by bit in registers, 109).
+// Then each warp lists what it keeps of its run of tokens. The move of the rows, 256 bytes each, is
+// bound by HBM (600 us for 3.76 GB read and written), so it keeps many independent 16-byte loads in
+// flight; it follows in the same kernel or in evict_copy_kernel.
 #include "common.cuh"
 #include "host_common.h"
 
@@ -30,6 +30,7 @@ constexpr int kEvList = 1024;                    // weights of the edge's bin th
 constexpr int kEvCopyThreads = 256;
 constexpr int kEvSeg = 128;                      // tokens a copy CTA moves, out of place
 constexpr int kEvInThreads = 512;                // copy in place
+constexpr int kEvRowSeg = 128;                   // tokens a CTA that selected them moves at a time
 constexpr int kEvInSeg = 64;                     // tokens it moves between two barriers
 
 struct EvictArgs {
@@ -97,8 +98,9 @@ __device__ __forceinline__ int top_bin(const uint32_t* hist, int bins, int& want
   return found[0];
 }
 
+// Lists in kept and mass_out what stays of one row; all threads of the CTA call it.
 template <int kThreads>
-__global__ void __launch_bounds__(kThreads) evict_select_kernel(const EvictArgs a) {
+__device__ __forceinline__ void evict_select(const EvictArgs& a, int64_t row) {
   extern __shared__ uint32_t ev_smem[];
   uint32_t* hist = ev_smem;             // [kEvBins]
   uint32_t* stage = ev_smem + kEvBins;  // [a.stage]
@@ -106,10 +108,7 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const EvictArgs 
   __shared__ uint32_t run_over[kThreads / 32], run_same[kThreads / 32];
   __shared__ int found[2];
   __shared__ uint32_t listed, list[kEvList];
-  grid_dep_wait();
-  grid_dep_launch();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t row = blockIdx.x;
   const int b = (int)(row / a.heads % a.batch);
   const float* mass = a.mass + row * a.cap;
   int32_t* kept = a.kept + row * a.budget;
@@ -284,33 +283,25 @@ __device__ __forceinline__ uint4 ld_stream(const char* p) {
   return v;
 }
 
-// Moves one segment of kThreads / 16 * kTokens tokens: a half warp per token and iteration.
-// In place a CTA walks all segments of its (layer, sequence, head) in order. That is safe: a
-// token's new slot is never past its old one, so what a segment writes, later segments do not
-// read; within one, every load comes before any store.
+// Moves the kept tokens [t0, t1) of a row, kSeg at a time, a half warp per token and iteration. In
+// place that is safe when one CTA walks all of the row: a token's new slot is never past its old
+// one, so what a segment writes, later segments do not read; within one, every load comes before any
+// store.
 template <int kThreads, int kSeg, bool kInPlace>
-__global__ void __launch_bounds__(kThreads) evict_copy_kernel(const EvictArgs a, int segs) {
+__device__ __forceinline__ void evict_move(const EvictArgs& a, int layer, int b, int h, int t0, int t1) {
   constexpr int kPer = kSeg * 16 / kThreads;  // 16-byte pieces of K, and of V, a thread moves
   __shared__ int2 src[kSeg], dst[kSeg];
-  grid_dep_wait();
-  grid_dep_launch();
   const int tid = threadIdx.x, piece = tid & 15;
-  // the heads of one stretch of tokens run side by side: their rows are neighbours in memory
-  int64_t r = blockIdx.x;
-  const int h = (int)(r % a.heads);
-  r /= a.heads;
-  const int seg = kInPlace ? 0 : (int)(r % segs);
-  if (!kInPlace) r /= segs;
-  const int b = (int)(r % a.batch), layer = (int)(r / a.batch);
   const int n = evict_len(a, b);
-  const int count = min(n, a.budget);
+  const int count = min(min(n, a.budget), t1);
   if (kInPlace && n <= a.budget) return;
   const int32_t* kept = a.kept + (((int64_t)layer * a.batch + b) * a.heads + h) * a.budget;
   const char* k = a.k + layer * a.ks[0] + h * a.ks[3] + piece * 16;
   const char* v = a.v + layer * a.vs[0] + h * a.vs[3] + piece * 16;
   char* ko = a.ko + layer * a.kos[0] + h * a.kos[3] + piece * 16;
   char* vo = a.vo + layer * a.vos[0] + h * a.vos[3] + piece * 16;
-  for (int t0 = seg * kSeg; t0 < count; t0 += kSeg) {
+#pragma unroll 1
+  for (; t0 < count; t0 += kSeg) {
     for (int i = tid; i < min(kSeg, count - t0); i += kThreads) {
       const int j = kept[t0 + i];
       src[i] = evict_slot(a.bt, a.bts, b, j, a.max_blocks, a.num_blocks);
@@ -341,9 +332,38 @@ __global__ void __launch_bounds__(kThreads) evict_copy_kernel(const EvictArgs a,
         *reinterpret_cast<uint4*>(vo + dst[t].x * a.vos[1] + dst[t].y * a.vos[2]) = vx[i];
       }
     }
-    if (!kInPlace) break;
     __syncthreads();  // src and dst are read before the next segment's are written
   }
+}
+
+// A CTA per row: selection, then (kMove) the row's move to another pool.
+template <int kThreads, bool kMove>
+__global__ void __launch_bounds__(kThreads) evict_row_kernel(const EvictArgs a) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const int64_t row = blockIdx.x;
+  evict_select<kThreads>(a, row);
+  if (kMove) {
+    __syncthreads();
+    const int64_t seq = row / a.heads;
+    evict_move<kThreads, kEvRowSeg, false>(a, (int)(seq / a.batch), (int)(seq % a.batch),
+                                           (int)(row % a.heads), 0, a.budget);
+  }
+}
+
+// The move of rows that evict_row_kernel has listed: a CTA per row in place, else per kSeg tokens.
+template <int kThreads, int kSeg, bool kInPlace>
+__global__ void __launch_bounds__(kThreads) evict_copy_kernel(const EvictArgs a, int segs) {
+  grid_dep_wait();
+  grid_dep_launch();
+  // the heads of one stretch of tokens run side by side: their rows are neighbours in memory
+  int64_t r = blockIdx.x;
+  const int h = (int)(r % a.heads);
+  r /= a.heads;
+  const int seg = kInPlace ? 0 : (int)(r % segs);
+  if (!kInPlace) r /= segs;
+  evict_move<kThreads, kSeg, kInPlace>(a, (int)(r / a.batch), (int)(r % a.batch), h, seg * kSeg,
+                                       kInPlace ? a.budget : min((seg + 1) * kSeg, a.budget));
 }
 
 }  // namespace fi
@@ -441,20 +461,26 @@ extern "C" int fi_kv_evict(const void* k, const void* v, const int32_t* block_ta
   a.stage = (int)(longest <= kEvStageMax ? longest : 0);
   static DeviceOnce once;
   cudaError_t e = once.run([] {
-    return cudaFuncSetAttribute(evict_select_kernel<kEvLong>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (kEvBins + kEvStageMax) * 4);
+    return cudaFuncSetAttribute(evict_row_kernel<kEvLong, false>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize, (kEvBins + kEvStageMax) * 4);
   });
   if (e != cudaSuccess) return cuda_fail(e, "fi_kv_evict: cudaFuncSetAttribute");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const size_t smem = (size_t)(kEvBins + a.stage) * 4;
-  if (longest <= 16 * kEvShort)
-    e = launch_pdl(evict_select_kernel<kEvShort>, dim3((unsigned)rows), dim3(kEvShort), smem, st, a);
-  else
-    e = launch_pdl(evict_select_kernel<kEvLong>, dim3((unsigned)rows), dim3(kEvLong), smem, st, a);
+  const dim3 grid((unsigned)rows);
+  const bool is_short = longest <= 16 * kEvShort;
+  // Many short rows: one kernel, whose selections run beside other rows' moves (28 x 16 x 8 rows of
+  // 900 to 4096 tokens to 1024: 628 us, 689 in two; 28 x 3 x 8 of 8192 to 2048: 281, 271 in two;
+  // in place, where a row's move has to wait for its own reads, 138 against 128 for 28 x 4 x 8).
+  if (is_short && !in_place && rows >= 5 * sm_count()) {
+    e = launch_pdl(evict_row_kernel<kEvShort, true>, grid, dim3(kEvShort), smem, st, a);
+    return e == cudaSuccess ? FI_OK : cuda_fail(e, "fi_kv_evict: launch");
+  }
+  e = is_short ? launch_pdl(evict_row_kernel<kEvShort, false>, grid, dim3(kEvShort), smem, st, a)
+               : launch_pdl(evict_row_kernel<kEvLong, false>, grid, dim3(kEvLong), smem, st, a);
   if (e != cudaSuccess) return cuda_fail(e, "fi_kv_evict: select launch");
   if (in_place)
-    e = launch_pdl(evict_copy_kernel<kEvInThreads, kEvInSeg, true>, dim3((unsigned)rows),
-                   dim3(kEvInThreads), 0, st, a, 1);
+    e = launch_pdl(evict_copy_kernel<kEvInThreads, kEvInSeg, true>, grid, dim3(kEvInThreads), 0, st, a, 1);
   else
     e = launch_pdl(evict_copy_kernel<kEvCopyThreads, kEvSeg, false>, dim3((unsigned)(rows * segs)),
                    dim3(kEvCopyThreads), 0, st, a, (int)segs);

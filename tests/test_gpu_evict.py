@@ -201,3 +201,31 @@ def test_cache_evict_bookkeeping(cuda_device, device_checks):
         cache.extend([1000, 0])
     _, ctx = cache.extend([60, 0])
     assert ctx.tolist() == [160, 70] and len(cache.free_blocks) == 4
+
+
+@pytest.mark.parametrize("budget,recent,sinks", [(70, 8, 2), (200, 0, 4), (1, 0, 0)])
+def test_many_rows(cuda_device, device_checks, budget, recent, sinks):
+    """Rows enough for selection and move to share a kernel, lengths from none to past the budget."""
+    lens = [150, 0, 70, 71, 64, 300, 1, 129, 200, 33] * 4
+    run_both(make(lens, 2, 10, seed=7), cuda_device, budget, recent, sinks)
+
+
+def test_many_rows_with_a_missing_page(cuda_device):
+    """A token whose page is missing in either table is reported and not moved; the rest is."""
+    from fast_infer_b200._runtime import device_checks as checks
+    from fast_infer_b200.kernels.eviction import evict_tokens
+    k, v, table, lens, mass = make([130] * 40, 2, 10, seed=8)
+    table[3, 1] = -1
+    out = torch.zeros(2, 40, PAGE, 10, D, dtype=k.dtype)
+    table_out = torch.arange(40).int().view(40, 1)
+    table_out[5, 0] = 99
+    kd, vd, td, ld, md, ko, vo, to = (t.to(cuda_device) for t in
+                                      (k, v, table, lens, mass, out, out, table_out))
+    with checks(True), pytest.raises(RuntimeError, match="block_table entry"):
+        evict_tokens(kd, vd, td, ld, md, 60, out=(ko, vo, to))
+    for b in (0, 3, 5, 39):
+        for h in (0, 9):
+            for r, j in enumerate(evict_keep(mass[1, b, h, :130].tolist(), 60, 0, 0)):
+                gone = b == 5 or (b == 3 and PAGE <= j < 2 * PAGE)
+                want = torch.zeros(D).half() if gone else k[1, table[b, j // PAGE], j % PAGE, h]
+                assert torch.equal(ko[1, b, r, h].cpu(), want)
