@@ -290,7 +290,7 @@ __device__ __forceinline__ uint4 ld_stream(const char* p) {
 template <int kThreads, int kSeg, bool kInPlace>
 __device__ __forceinline__ void evict_move(const EvictArgs& a, int layer, int b, int h, int t0, int t1) {
   constexpr int kPer = kSeg * 16 / kThreads;  // 16-byte pieces of K, and of V, a thread moves
-  __shared__ int2 src[kSeg], dst[kSeg];
+  __shared__ int2 src_ring[3][kSeg], dst_ring[3][kSeg];
   const int tid = threadIdx.x, piece = tid & 15;
   const int n = evict_len(a, b);
   const int count = min(min(n, a.budget), t1);
@@ -300,20 +300,26 @@ __device__ __forceinline__ void evict_move(const EvictArgs& a, int layer, int b,
   const char* v = a.v + layer * a.vs[0] + h * a.vs[3] + piece * 16;
   char* ko = a.ko + layer * a.kos[0] + h * a.kos[3] + piece * 16;
   char* vo = a.vo + layer * a.vos[0] + h * a.vos[3] + piece * 16;
-#pragma unroll 1
-  for (; t0 < count; t0 += kSeg) {
-    for (int i = tid; i < min(kSeg, count - t0); i += kThreads) {
-      const int j = kept[t0 + i];
-      src[i] = evict_slot(a.bt, a.bts, b, j, a.max_blocks, a.num_blocks);
-      dst[i] = evict_slot(a.bto, a.btos, b, t0 + i, a.max_blocks_out, a.num_blocks_out);
-      if (src[i].x < 0 || dst[i].x < 0) {
+  auto look_up = [&](int from, int2* src, int2* dst) {
+    for (int i = tid; i < min(kSeg, count - from); i += kThreads) {
+      const int j = kept[from + i];
+      int2 at = evict_slot(a.bt, a.bts, b, j, a.max_blocks, a.num_blocks);
+      dst[i] = evict_slot(a.bto, a.btos, b, from + i, a.max_blocks_out, a.num_blocks_out);
+      if (at.x < 0 || dst[i].x < 0) {
         set_error(a.err, FI_DEVERR_BAD_BLOCK);
-        src[i].x = -1;
-      } else if (kInPlace && j == t0 + i) {
-        src[i].x = -1;  // it stays where it is
+        at.x = -1;
+      } else if (kInPlace && j == from + i) {
+        at.x = -1;  // it stays where it is
       }
+      src[i] = at;
     }
-    __syncthreads();
+  };
+  look_up(t0, src_ring[0], dst_ring[0]);
+  __syncthreads();
+#pragma unroll 1
+  for (int slot = 0; t0 < count; t0 += kSeg) {
+    const int2 *src = src_ring[slot], *dst = dst_ring[slot];
+    slot = slot == 2 ? 0 : slot + 1;
     uint4 kx[kPer], vx[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -323,7 +329,8 @@ __device__ __forceinline__ void evict_move(const EvictArgs& a, int layer, int b,
         vx[i] = ld_stream(v + src[t].x * a.vs[1] + src[t].y * a.vs[2]);
       }
     }
-    if (kInPlace) __syncthreads();
+    look_up(t0 + kSeg, src_ring[slot], dst_ring[slot]);  // (last read two barriers ago)
+    __syncthreads();  // the loads of all threads are done, the next segment's places known
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int t = (tid >> 4) + i * (kThreads / 16);
@@ -332,7 +339,6 @@ __device__ __forceinline__ void evict_move(const EvictArgs& a, int layer, int b,
         *reinterpret_cast<uint4*>(vo + dst[t].x * a.vos[1] + dst[t].y * a.vos[2]) = vx[i];
       }
     }
-    __syncthreads();  // src and dst are read before the next segment's are written
   }
 }
 
