@@ -342,8 +342,8 @@ __device__ __forceinline__ void evict_move(const EvictArgs& a, int layer, int b,
   }
 }
 
-// A CTA per row: selection, then (kMove) the row's move to another pool.
-template <int kThreads, bool kMove>
+// A CTA per row: selection, then (kMove) the row's move.
+template <int kThreads, bool kMove, bool kInPlace>
 __global__ void __launch_bounds__(kThreads) evict_row_kernel(const EvictArgs a) {
   grid_dep_wait();
   grid_dep_launch();
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(kThreads) evict_row_kernel(const EvictArgs a) 
   if (kMove) {
     __syncthreads();
     const int64_t seq = row / a.heads;
-    evict_move<kThreads, kEvRowSeg, false>(a, (int)(seq / a.batch), (int)(seq % a.batch),
+    evict_move<kThreads, kInPlace ? kEvInSeg : kEvRowSeg, kInPlace>(a, (int)(seq / a.batch), (int)(seq % a.batch),
                                            (int)(row % a.heads), 0, a.budget);
   }
 }
@@ -467,8 +467,16 @@ extern "C" int fi_kv_evict(const void* k, const void* v, const int32_t* block_ta
   a.stage = (int)(longest <= kEvStageMax ? longest : 0);
   static DeviceOnce once;
   cudaError_t e = once.run([] {
-    return cudaFuncSetAttribute(evict_row_kernel<kEvLong, false>,
-                                cudaFuncAttributeMaxDynamicSharedMemorySize, (kEvBins + kEvStageMax) * 4);
+    const void* kernels[] = {(const void*)evict_row_kernel<kEvLong, false, false>,
+                             (const void*)evict_row_kernel<kEvShort, false, false>,
+                             (const void*)evict_row_kernel<kEvShort, true, false>,
+                             (const void*)evict_row_kernel<kEvShort, true, true>};
+    for (const void* f : kernels) {
+      const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (kEvBins + kEvStageMax) * 4);
+      if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
   });
   if (e != cudaSuccess) return cuda_fail(e, "fi_kv_evict: cudaFuncSetAttribute");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -476,14 +484,15 @@ extern "C" int fi_kv_evict(const void* k, const void* v, const int32_t* block_ta
   const dim3 grid((unsigned)rows);
   const bool is_short = longest <= 16 * kEvShort;
   // Many short rows: one kernel, whose selections run beside other rows' moves (28 x 16 x 8 rows of
-  // 900 to 4096 tokens to 1024: 628 us, 689 in two; 28 x 3 x 8 of 8192 to 2048: 281, 271 in two;
-  // in place, where a row's move has to wait for its own reads, 138 against 128 for 28 x 4 x 8).
-  if (is_short && !in_place && rows >= 5 * sm_count()) {
-    e = launch_pdl(evict_row_kernel<kEvShort, true>, grid, dim3(kEvShort), smem, st, a);
+  // 2048 tokens to 1024: 633 us, 690 in two, in place 645 and 695; 1 x 100 x 8: 155 and 164, in
+  // place 161 and 168). Fewer rows leave SMs without one to move (28 x 3 x 8 of 8192 to 2048: 281 and 271).
+  if (is_short && rows >= 5 * sm_count()) {
+    e = in_place ? launch_pdl(evict_row_kernel<kEvShort, true, true>, grid, dim3(kEvShort), smem, st, a)
+                 : launch_pdl(evict_row_kernel<kEvShort, true, false>, grid, dim3(kEvShort), smem, st, a);
     return e == cudaSuccess ? FI_OK : cuda_fail(e, "fi_kv_evict: launch");
   }
-  e = is_short ? launch_pdl(evict_row_kernel<kEvShort, false>, grid, dim3(kEvShort), smem, st, a)
-               : launch_pdl(evict_row_kernel<kEvLong, false>, grid, dim3(kEvLong), smem, st, a);
+  e = is_short ? launch_pdl(evict_row_kernel<kEvShort, false, false>, grid, dim3(kEvShort), smem, st, a)
+               : launch_pdl(evict_row_kernel<kEvLong, false, false>, grid, dim3(kEvLong), smem, st, a);
   if (e != cudaSuccess) return cuda_fail(e, "fi_kv_evict: select launch");
   if (in_place)
     e = launch_pdl(evict_copy_kernel<kEvInThreads, kEvInSeg, true>, grid, dim3(kEvInThreads), 0, st, a, 1);

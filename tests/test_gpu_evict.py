@@ -210,6 +210,13 @@ def test_many_rows(cuda_device, device_checks, budget, recent, sinks):
     run_both(make(lens, 2, 10, seed=7), cuda_device, budget, recent, sinks)
 
 
+def test_many_rows_with_room_for_more(cuda_device, device_checks):
+    """Tables and masses that reach further than any sequence (the most shared memory of a short row)."""
+    k, v, table, lens, mass = make([70, 200, 3, 130] * 10, 2, 10, seed=7, cap=8192)
+    table = torch.nn.functional.pad(table, (0, 128 - table.shape[1]), value=-1)
+    run_both((k, v, table, lens, mass), cuda_device, 65, 8, 2)
+
+
 def test_many_rows_with_a_missing_page(cuda_device):
     """A token whose page is missing in either table is reported and not moved; the rest is."""
     from fast_infer_b200._runtime import device_checks as checks
