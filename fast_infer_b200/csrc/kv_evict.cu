@@ -21,8 +21,8 @@
 namespace fi {
 
 constexpr int kEvPage = 64;
-// threads of a selection: 28 x 16 x 8 rows of 900 to 4096 tokens take 90 us with 512 (256: 94, 128: 215),
-// 28 x 8 rows of 32768 take 62 us with 1024 (512: 83)
+// threads of a selection: 28 x 16 x 8 rows of 900 to 4096 tokens take 90 us with 512 (256: 94, 128:
+// 215), 28 x 8 rows of 32768 take 62 us with 1024 (512: 83)
 constexpr int kEvShort = 512, kEvLong = 1024;
 constexpr int kEvBins = 2048;
 constexpr int kEvStageMax = 12 * 1024;           // tokens whose weights are kept in shared memory
@@ -279,14 +279,15 @@ __device__ __forceinline__ int2 evict_slot(const int32_t* bt, const int64_t* bts
 __device__ __forceinline__ uint4 ld_stream(const char* p) {
   uint4 v;
   asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
   return v;
 }
 
 // Moves the kept tokens [t0, t1) of a row, kSeg at a time, a half warp per token and iteration. In
 // place that is safe when one CTA walks all of the row: a token's new slot is never past its old
-// one, so what a segment writes, later segments do not read; within one, every load comes before any
-// store.
+// one, so what a segment writes, later segments do not read; within one, every load comes before
+// any store. The places of the next segment are looked up while this one's values are on their way
+// (in place, 28 x 16 x 8 rows: 779 -> 695 us; segments of 128 tokens 768).
 template <int kThreads, int kSeg, bool kInPlace>
 __device__ __forceinline__ void evict_move(const EvictArgs& a, int layer, int b, int h, int t0, int t1) {
   constexpr int kPer = kSeg * 16 / kThreads;  // 16-byte pieces of K, and of V, a thread moves
@@ -352,8 +353,8 @@ __global__ void __launch_bounds__(kThreads) evict_row_kernel(const EvictArgs a) 
   if (kMove) {
     __syncthreads();
     const int64_t seq = row / a.heads;
-    evict_move<kThreads, kInPlace ? kEvInSeg : kEvRowSeg, kInPlace>(a, (int)(seq / a.batch), (int)(seq % a.batch),
-                                           (int)(row % a.heads), 0, a.budget);
+    evict_move<kThreads, kInPlace ? kEvInSeg : kEvRowSeg, kInPlace>(
+        a, (int)(seq / a.batch), (int)(seq % a.batch), (int)(row % a.heads), 0, a.budget);
   }
 }
 
@@ -485,7 +486,8 @@ extern "C" int fi_kv_evict(const void* k, const void* v, const int32_t* block_ta
   const bool is_short = longest <= 16 * kEvShort;
   // Many short rows: one kernel, whose selections run beside other rows' moves (28 x 16 x 8 rows of
   // 2048 tokens to 1024: 633 us, 690 in two, in place 645 and 695; 1 x 100 x 8: 155 and 164, in
-  // place 161 and 168). Fewer rows leave SMs without one to move (28 x 3 x 8 of 8192 to 2048: 281 and 271).
+  // place 161 and 168). Fewer rows leave SMs without one to move (28 x 3 x 8 of 8192 to 2048: 281
+  // and 271).
   if (is_short && rows >= 5 * sm_count()) {
     e = in_place ? launch_pdl(evict_row_kernel<kEvShort, true, true>, grid, dim3(kEvShort), smem, st, a)
                  : launch_pdl(evict_row_kernel<kEvShort, true, false>, grid, dim3(kEvShort), smem, st, a);

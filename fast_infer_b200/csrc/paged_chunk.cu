@@ -25,7 +25,13 @@
 //   moves only when some score passes it by 2^8, found by one vote per tile. (One kernel for
 //   both forms was tried: its registers spilled and its code, 150 KB, missed the instruction
 //   caches; long prefills lost 10 %, single tokens 40 %.) A batch that may hold both kinds
-//   launches both kernels, the second beginning on each SM as the first leaves it.
+//   launches both kernels, the second beginning on each SM as the first leaves it. (Sharing the
+//   SMs out between them by cost was no faster: a step of 24 rows costs as much as a wide one.)
+// * What bounds it: a wide step of 256 rows x 128 keys takes 3850 cycles, of which its products need
+//   2040 of the tensor core and its exponentials 1800 of the special function units; issue slots and
+//   the chain through tensor memory are the rest. 4096 tokens over 61003: 3.43 to 3.56 ms, 890 to 925 TFLOP/s at the power cap's
+//   1.45 GHz; 4225 over 2000: 223 us, 959 TFLOP/s. Single tokens are bound by HBM: 64 over 4000
+//   each, 179 us, 5.9 TB/s; one over 512 by its two launches, 12.4 us.
 // * Slots behind a sequence's last token may hold anything: their scores are replaced by
 //   -inf, and their V rows are zeroed in shared memory before the product (0 * NaN is NaN).
 #include "chunk_common.cuh"
@@ -43,10 +49,10 @@ constexpr int kCkNarrow = 32;        // rows up to which a unit runs transposed
 constexpr float kCkRescale = 8.0f;   // log2 units of growth of the max before O is rescaled
 constexpr int kCkEmuPairs = 1;       // of 8 column pairs, exp2 on the FMA pipe
 // Steps that a unit's start and end are worth: with 0 and 0 / 1 and 2 / 3 and 2 / 4 and 3, 64 single
-// tokens over 1000 with 2048 new over 2000 take 177 / 170 / 168 / 171 us, and 64 over 4000 with 512 new
-// (units of the narrow kernel, all in a few CTAs' parts) 294 / 252 / 200 / 201.
+// tokens over 1000 beside 2048 new over 2000 take 177 / 170 / 168 / 171 us, and 64 over 4000 beside
+// 512 new (units of the narrow kernel, all in a few CTAs' parts) 294 / 252 / 200 / 201.
 constexpr int kCkPadNarrow = 3, kCkPadWide = 2;
-constexpr int kCkManyNew = 500;      // new tokens past one each that the wide kernel is launched for
+constexpr int kCkManyNew = 500;      // new tokens past one each for which both kernels run
 constexpr int kCkSlots = 4;          // units that the scheduler is ahead
 
 // A CTA's part of a unit: key steps [j0, j1) of its n.
@@ -132,10 +138,11 @@ __device__ __forceinline__ void ck_tiles(const ChunkBatch& p, const ChunkSeq& s,
 
 // The scheduler (one warp): walks the CTA's part of the line and hands its units to the other
 // roles through a ring in shared memory. Its lanes look the units' pages over, so that no one
-// else has to unless an entry is invalid. On the line a unit is `pad` steps longer than its key tiles,
-// which stand for what it costs to begin and end one; its step j is at pad + j.
+// else has to unless an entry is invalid. On the line a unit is `pad` steps longer than its key
+// tiles, which stand for what it costs to begin and end one; its step j is at pad + j.
 __device__ __forceinline__ void ck_schedule(const ChunkBatch& p, int unit_tokens, int pad,
-                                            CkBarriers* s, uint32_t units, CkJoin* join_out, int* err) {
+                                            CkBarriers* s, uint32_t units, CkJoin* join_out,
+                                            int* err) {
   const int G = gridDim.x, cta = blockIdx.x, lane = threadIdx.x & 31;
   const uint32_t per_head = s->work[units];
   const int64_t total = (int64_t)per_head * p.hk;
@@ -179,11 +186,12 @@ __device__ __forceinline__ void ck_schedule(const ChunkBatch& p, int unit_tokens
       u.rows[1] = max(t1 - t0 - tt, 0) * p.group;
       u.j0 = max(at - pad, 0);
       u.j1 = stop - pad;
-      // the last step of the unit, w - at + len - 1, belongs to the last CTA that starts at or before it
+      // the unit's last step, w - at + len - 1, is the last CTA's that starts at or before it
       u.last_cta = stop == len ? cta : (int)(((w - at + len) * active - 1) / total);
       for (int j = u.j0 + (lane >> 1); j < u.j1; j += 16) {
         const int tile = ck_tile(u, j), half = lane & 1;
-        if ((tile * 2 + half) * kChunkPage < u.keys && chunk_page(p, b, u.keys, tile, half) == p.num_blocks)
+        if ((tile * 2 + half) * kChunkPage < u.keys &&
+            chunk_page(p, b, u.keys, tile, half) == p.num_blocks)
           pages_ok = false;
       }
       w += stop - at;
@@ -233,10 +241,10 @@ __device__ __forceinline__ void ck_done(CkBarriers* s, int& i) {
 }
 
 // 32 scores of one row in log2 units, in place: the cap and the distance bias (without either,
-// they stay unscaled). The short form of small capped scores: 376 us for 4225 tokens of 24 sequences
-// and a cap of 50, 532 without it (scores past it pay 5 % for the test). With one key per
-// thread (score_form8) it costs more in code than it saves: 48 against 45 us. `off` = position of the first column's key minus the row's position; a row
-// that is not `live` has no say in which form of tanh runs.
+// they stay unscaled). `off` = position of the first column's key minus the row's position; a row
+// that is not `live` has no say in which form of tanh runs. The short form for small scores: 374 us
+// for 4225 tokens of 24 sequences and a cap of 50, 532 without it (scores past it pay 5 % for the
+// test). Where a thread has one key (score_form8) its code costs more than it saves: 48 against 45 us.
 template <bool kCap, bool kAlibi>
 __device__ __forceinline__ void score_form(uint32_t* sr, const ScoreForm& f, float slope2,
                                            float off, bool live) {
@@ -324,7 +332,8 @@ __device__ __forceinline__ void score_form8(const uint32_t* raw, float* s, const
 }
 
 // p = 2^(s * sl2 - mref) of a row, its sum, and p packed in place. 1 of 8 pairs takes exp2 on the
-// FMA pipe (0: 4772 us for a chunk of 4096 tokens over 61003, 1: 3587, 2: 3746, 3: 3802), to 2.2e-7: lse is an output, which a rougher polynomial would show in.
+// FMA pipe (0: 4772 us for a chunk of 4096 tokens over 61003, 1: 3587, 2: 3746, 3: 3802), to 2.2e-7:
+// lse is an output, which a rougher polynomial would show in.
 template <typename T>
 __device__ __forceinline__ float ck_exp(uint32_t* sr, float sl2, float mref) {
   const uint64_t sc2 = f32x2(sl2, sl2), nm2 = f32x2(-mref, -mref);
@@ -1118,8 +1127,8 @@ __global__ void __launch_bounds__(kCkThreads, 1)
 }
 
 // Joins the parts of a unit that several CTAs hold: weights 2^(lse_part - max), the max running.
-// A block joins 8 rows of one CTA's unit: `p`'s first, then `p2`'s. A thread has 4 values of a row: a
-// warp those of one row, or of 8 rows where 32 rows lie side by side.
+// A block joins 8 rows of one CTA's unit: `p`'s first, then `p2`'s. A thread has 4 values of a
+// row: a warp those of one row, or of 8 rows where 32 rows lie side by side.
 template <typename T>
 __global__ void __launch_bounds__(256, 8) chunk_combine_kernel(const ChunkParams p,
                                                                const ChunkParams p2) {
@@ -1212,8 +1221,9 @@ static int launch_chunk(const CUtensorMap& tq_n, const CUtensorMap& tq_w, const 
   if (r != FI_OK) return r;
   const ChunkParams& first = wide ? *wide : *narrow;
   const int parts = (first.rows_cap + (narrow && wide ? narrow->rows_cap : 0)) / 8;
-  const cudaError_t e = launch_pdl(chunk_combine_kernel<T>, dim3((unsigned)sm_count(), (unsigned)parts),
-                                   dim3(256), 0, st, first, narrow ? *narrow : first);
+  const cudaError_t e =
+      launch_pdl(chunk_combine_kernel<T>, dim3((unsigned)sm_count(), (unsigned)parts), dim3(256), 0,
+                 st, first, narrow ? *narrow : first);
   return e == cudaSuccess ? FI_OK : cuda_fail(e, "fi_paged_chunk: combine launch");
 }
 
@@ -1317,7 +1327,8 @@ extern "C" int fi_paged_chunk(const void* q, const void* k_cache, const void* v_
   p.o = o;
   p.os[0] = o_strides[0];
   p.os[1] = o_strides[1];
-  p.o_wide = reinterpret_cast<uintptr_t>(o) % 32 == 0 && o_strides[0] % 16 == 0 && o_strides[1] % 16 == 0;
+  p.o_wide = reinterpret_cast<uintptr_t>(o) % 32 == 0 && o_strides[0] % 16 == 0 &&
+             o_strides[1] % 16 == 0;
   p.lse = lse;
   p.err = error_flag;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
