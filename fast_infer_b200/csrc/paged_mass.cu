@@ -19,7 +19,7 @@
 //   SM's MUFU, against 2048 of the tensor core), of which some run as a polynomial on the FMA
 //   pipe, and the query tile's 32 KB from L2 (units of 256 keys read 6.3 TB/s of them on the
 //   whole GPU and were bound by that). 2048 tokens over 30011: 473 us, 825 TFLOP/s; single tokens of
-//   16 sequences over 1000 to 4095: 23 us, 3.1 TB/s (9 us of it start and drain).
+//   16 sequences over 1000 to 4095: 22 us, 3.3 TB/s (8 us of it start and drain).
 // * Roles (640 threads): warps 0-15 = the sums, a warpgroup per key tile (one per warp scheduler
 //   would show its latencies: eight warps took twice the time), warp 16 = TMA, warp 17 = UMMA
 //   issue, warp 18 = the rows' lse (and slopes and positions) into shared memory, warp 19 =
@@ -687,6 +687,9 @@ static int launch_mass(const CUtensorMap& tq, const CUtensorMap& tk, const MassP
   e = launch_pdl(paged_mass_kernel<T, kCap, kAlibi>, dim3((unsigned)grid), dim3(kMsThreads),
                  kMsSmemBytes, st, tq, tk, p);
   if (e != cudaSuccess) return cuda_fail(e, "fi_attention_mass: launch");
+  // No sequence has more than one query tile: every unit is one step, in one CTA (16 single tokens
+  // over 1000 to 4095: 22 us, 23 with the join).
+  if (p.b.total <= p.b.tile_tokens) return FI_OK;
   e = launch_pdl(mass_join_kernel, dim3((unsigned)grid), dim3(kMsKeys), 0, st, p);
   if (e != cudaSuccess) return cuda_fail(e, "fi_attention_mass: join launch");
   return FI_OK;
