@@ -30,7 +30,7 @@
 // * What bounds it: a wide step of 256 rows x 128 keys takes 3850 cycles, of which its products need
 //   2040 of the tensor core and its exponentials 1800 of the special function units; issue slots and
 //   the chain through tensor memory are the rest. 4096 tokens over 61003: 3.43 to 3.56 ms, 890 to 925 TFLOP/s at the power cap's
-//   1.45 GHz; 4225 over 2000: 223 us, 959 TFLOP/s. Single tokens are bound by HBM: 64 over 4000
+//   1.45 GHz; 4225 over 2000: 214 us, 999 TFLOP/s. Single tokens are bound by HBM: 64 over 4000
 //   each, 179 us, 5.9 TB/s; one over 512 by its two launches, 12.4 us.
 // * Slots behind a sequence's last token may hold anything: their scores are replaced by
 //   -inf, and their V rows are zeroed in shared memory before the product (0 * NaN is NaN).
@@ -1127,57 +1127,62 @@ __global__ void __launch_bounds__(kCkThreads, 1)
 }
 
 // Joins the parts of a unit that several CTAs hold: weights 2^(lse_part - max), the max running.
-// A block joins 8 rows of one CTA's unit: `p`'s first, then `p2`'s. A thread has 4 values of a
-// row: a warp those of one row, or of 8 rows where 32 rows lie side by side.
+// A block joins kCkJoinRows rows of one CTA's unit: `p`'s first, then `p2`'s. A thread has 8 values
+// of a row: a warp those of two rows, or of 16 rows where 32 rows lie side by side. Bound by issue
+// slots, not by memory (512 new tokens over 2000: 34.4 us in all; 4 values a thread 35.8).
+constexpr int kCkJoinRows = 16;
 template <typename T>
-__global__ void __launch_bounds__(256, 8) chunk_combine_kernel(const ChunkParams p,
+__global__ void __launch_bounds__(256, 5) chunk_combine_kernel(const ChunkParams p,
                                                                const ChunkParams p2) {
   grid_dep_wait();
   grid_dep_launch();
-  const bool second = (int)blockIdx.y >= p.rows_cap / 8;
+  const bool second = (int)blockIdx.y >= p.rows_cap / kCkJoinRows;
   const int cta = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r0 = ((int)blockIdx.y - (second ? p.rows_cap / 8 : 0)) * 8;
+  const int r0 = ((int)blockIdx.y - (second ? p.rows_cap / kCkJoinRows : 0)) * kCkJoinRows;
   const CkJoin jn = second ? p2.join[cta] : p.join[cta];
   if (!jn.valid) return;
   const int rows_cap = second ? p2.rows_cap : p.rows_cap;
   const bool by_row = rows_cap == kCkNarrow;
   const float* ws_lse = second ? p2.ws_lse : p.ws_lse;
   const float* ws_o = second ? p2.ws_o : p.ws_o;
-  const int r = r0 + (by_row ? warp : lane & 7), t = r >> 7, row = r & 127;
-  const int col = (by_row ? lane : warp * 4 + (lane >> 3)) * 4;
+  const int r = r0 + (by_row ? warp * 2 + (lane >> 4) : lane & 15), t = r >> 7, row = r & 127;
+  const int col = (by_row ? lane & 15 : warp * 2 + (lane >> 4)) * 8;
   if (row >= (t ? jn.rows[1] : jn.rows[0])) return;
   const int off = by_row ? r * 128 + col : (r & ~31) * 128 + col * 32 + (r & 31) * 4;
-  float mx = -INFINITY, sum = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
+  const int far = by_row ? 4 : 128;  // from the first 4 values to the others
+  float mx = -INFINITY, sum = 0.f, acc[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+#pragma unroll 4
   for (int c = cta; c <= jn.last_cta; ++c) {
     const int at = (c * 2 + (c == cta ? 1 : 0)) * rows_cap;
     const float l = ws_lse[at + r];
-    const float4 v = *reinterpret_cast<const float4*>(ws_o + at * 128 + off);
+    const float* src = ws_o + at * 128 + off;
+    const float4 v = *reinterpret_cast<const float4*>(src);
+    const float4 w = *reinterpret_cast<const float4*>(src + far);
+    const float x[8] = {v.x, v.y, v.z, v.w, w.x, w.y, w.z, w.w};
     if (l > mx) {
-      const float a = exp2f(mx - l);
+      const float a = fast_exp2(mx - l);
       mx = l;
       sum *= a;
-      acc.x *= a;
-      acc.y *= a;
-      acc.z *= a;
-      acc.w *= a;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] *= a;
     }
-    const float wgt = l == -INFINITY ? 0.f : exp2f(l - mx);
+    const float wgt = l == -INFINITY ? 0.f : fast_exp2(l - mx);
     sum += wgt;
-    acc.x = fmaf(wgt, v.x, acc.x);
-    acc.y = fmaf(wgt, v.y, acc.y);
-    acc.z = fmaf(wgt, v.z, acc.z);
-    acc.w = fmaf(wgt, v.w, acc.w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = fmaf(wgt, x[i], acc[i]);
   }
   const bool none = sum == 0.f;
   const float inv = none ? 0.f : 1.f / sum;
   const int64_t token = jn.token + t * p.b.tile_tokens + row / p.b.group;
   const int head = jn.hk * p.b.group + row % p.b.group;
-  uint2 pk;
-  pk.x = Half16<T>::pack(acc.x * inv, acc.y * inv);
-  pk.y = Half16<T>::pack(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + token * p.os[0] + head * p.os[1] + col) = pk;
+  uint4 pk;
+  pk.x = Half16<T>::pack(acc[0] * inv, acc[1] * inv);
+  pk.y = Half16<T>::pack(acc[2] * inv, acc[3] * inv);
+  pk.z = Half16<T>::pack(acc[4] * inv, acc[5] * inv);
+  pk.w = Half16<T>::pack(acc[6] * inv, acc[7] * inv);
+  *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + token * p.os[0] + head * p.os[1] + col) = pk;
   if (col == 0 && p.lse) p.lse[token * p.b.hq + head] = none ? -INFINITY : (mx + log2f(sum)) * kLn2;
 }
 
@@ -1220,7 +1225,7 @@ static int launch_chunk(const CUtensorMap& tq_n, const CUtensorMap& tq_w, const 
   if (r == FI_OK && wide) r = launch_form<T, false>(tq_w, tk, tv, *wide, st);
   if (r != FI_OK) return r;
   const ChunkParams& first = wide ? *wide : *narrow;
-  const int parts = (first.rows_cap + (narrow && wide ? narrow->rows_cap : 0)) / 8;
+  const int parts = (first.rows_cap + (narrow && wide ? narrow->rows_cap : 0)) / kCkJoinRows;
   const cudaError_t e =
       launch_pdl(chunk_combine_kernel<T>, dim3((unsigned)sm_count(), (unsigned)parts), dim3(256), 0,
                  st, first, narrow ? *narrow : first);
