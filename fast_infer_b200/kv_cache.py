@@ -144,6 +144,8 @@ class KVCache:
         nn = np.asarray(n_new, np.int64).reshape(-1)
         if (nn < 0).any():
             raise ValueError("n_new must not be negative")
+        if self.num_tokens > 0 and not self.seq_lens.any():
+            raise ValueError("extend needs per-sequence lengths (its own, or store_kv_ragged's)")
         B = nn.shape[0]
         self._grow_batch(B)
         need = -(-(self.seq_lens[:B] + nn) // self.block_size)

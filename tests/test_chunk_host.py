@@ -179,6 +179,9 @@ def test_evict_needs_lengths_and_room():
     cache.num_tokens = 10  # the reference's batch-wide counter alone says nothing per sequence
     with pytest.raises(ValueError, match="per-sequence"):
         cache.evict(torch.zeros(1, 1, 2, 256), 8)
+    with pytest.raises(ValueError, match="per-sequence"):  # it would write over those 10 tokens
+        cache.extend([100])
+    cache.reset()
     cache.extend([100])
     with pytest.raises(ValueError, match="holds 64"):
         cache.evict(torch.zeros(1, 1, 2, 64), 8)
