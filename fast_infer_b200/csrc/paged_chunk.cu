@@ -34,6 +34,8 @@
 //   each, 179 us, 5.9 TB/s; one over 512 by its two launches, 12.4 us.
 // * Slots behind a sequence's last token may hold anything: their scores are replaced by
 //   -inf, and their V rows are zeroed in shared memory before the product (0 * NaN is NaN).
+#include <float.h>
+
 #include "chunk_common.cuh"
 
 namespace fi {
@@ -85,7 +87,7 @@ struct CkBarriers {
   uint32_t tmem_base;
   // transposed units, per warpgroup: rows' max, partial maxima / sums, scale, slope, token
   float n_max[2][kCkNarrow], n_red[2][4][kCkNarrow], n_alpha[2][kCkNarrow];
-  alignas(16) float n_neg[2][kCkNarrow];  // -max
+  alignas(16) float n_neg[2][kCkNarrow];  // -max; FLT_MAX: no score yet, -inf: no such row
   float n_slope[2][kCkNarrow], n_pos[2][kCkNarrow];
   int64_t n_off[kCkNarrow];  // where a row's output goes
   CkUnit units[kCkSlots];
@@ -389,7 +391,7 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
   constexpr float kTop = 256.f;  // 2^kCkRescale
   if (tid < kCkNarrow) {
     n_max[tid] = -INFINITY;
-    bars->n_neg[t][tid] = tid < rows ? INFINITY : -INFINITY;
+    bars->n_neg[t][tid] = tid < rows ? FLT_MAX : -INFINITY;
     bars->n_alpha[t][tid] = 0.f;
     if (kAlibi) {
       const bool live = tid < rows;
@@ -481,7 +483,7 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
                                   fmaxf(bars->n_red[t][2][tid], bars->n_red[t][3][tid]));
           bars->n_alpha[t][tid] = was == -INFINITY ? 0.f : fast_exp2(was - now);
           n_max[tid] = now;
-          bars->n_neg[t][tid] = -now;
+          bars->n_neg[t][tid] = now == -INFINITY ? FLT_MAX : -now;
         }
         __syncwarp();
         named_bar_sync(1 + t, 128);
@@ -505,10 +507,9 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
           tmem_wait_st();
         }
       }
-      // A row that has seen nothing has max -inf: a score it sees gives 2^inf, past any bound; one
-      // it does not see gives NaN, which the maximum below passes over and the mask sets to 0 (a
-      // score that is NaN stays: the row's result shows it). A column without a row has max +inf:
-      // p = 0.
+      // A row whose max is still -inf (it has seen nothing, or keys that score -inf alone) adds
+      // FLT_MAX: a finite score gives 2^FLT_MAX, past any bound, and one of -inf the weight 0. A
+      // score that is NaN stays: the row's result shows it. A column without a row adds -inf: p = 0.
       float top = 0.f;
 #pragma unroll
       for (int cc = 0; cc < kCkNarrow; cc += 8)

@@ -1,0 +1,98 @@
+"""Infinite keys that are seen: a score of -inf has weight 0, one of +inf makes NaN of the rows that see it and of no
+other, in both forms of the attention kernel."""
+
+import math
+
+import pytest
+import torch
+
+from tests.test_gpu_paged_chunk import PAGE, check, make, run
+
+pytestmark = pytest.mark.gpu
+
+
+def slot(batch, b, j):
+    """(page, row) of token j of sequence b."""
+    return int(batch[3][b, j // PAGE]), j % PAGE
+
+
+def positive(batch):
+    """The batch with a first dim of q, changed in place, that makes q.k = -inf in every row where k[0] = -inf."""
+    batch[0][..., 0] = batch[0][..., 0].abs() + 0.5
+    return batch
+
+
+def hide(batch, b, keys):
+    for j in keys:
+        batch[1][slot(batch, b, j)][..., 0] = -math.inf
+
+
+def reference(batch):
+    """The definition in 64 bits, with infinities as they are: (o, lse, weight of |v|)."""
+    q, k, v, table, cu, ctx = batch
+    total, hq, d = q.shape
+    hk = k.shape[2]
+    o, absv = (torch.zeros(total, hq, d, dtype=torch.float64) for _ in range(2))
+    lse = torch.full((total, hq), -math.inf, dtype=torch.float64)
+    for b, n in enumerate(ctx.tolist()):
+        lo, hi = int(cu[b]), int(cu[b + 1])
+        j = torch.arange(n)
+        pages = table[b, j // PAGE].long()
+        kb, vb = k[pages, j % PAGE].double(), v[pages, j % PAGE].double()
+        see = j <= torch.arange(n - (hi - lo), n)[:, None]
+        for h in range(hq):
+            kh = h // (hq // hk)
+            # (elementwise: a matrix product may not say what 0 * inf is)
+            s = (q[lo:hi, None, h].double() * kb[None, :, kh]).sum(-1) * d ** -0.5
+            s = s.masked_fill(~see, -math.inf)
+            top = s.amax(-1, keepdim=True)
+            e = torch.exp(s - torch.where(top == -math.inf, 0.0, top))
+            l = e.sum(-1, keepdim=True)
+            w = e / torch.where(l == 0, 1.0, l)
+            o[lo:hi, h], absv[lo:hi, h] = w @ vb[:, kh], w @ vb[:, kh].abs()
+            lse[lo:hi, h] = (torch.where(top == -math.inf, 0.0, top) + torch.log(l))[:, 0]
+    return o, lse, absv
+
+
+def agree(got, ref, dtype=torch.float16):
+    """NaN exactly where the definition has NaN; elsewhere the attention tests' tolerance."""
+    out, lse = got
+    nan = torch.isnan(ref[1])
+    assert torch.equal(torch.isnan(lse.cpu()), nan)
+    assert torch.equal(torch.isnan(out.cpu()).all(-1), nan) and torch.equal(torch.isnan(out.cpu()).any(-1), nan)
+    if not nan.all():
+        rows = ~nan.any(-1)
+        check(out.cpu()[rows], lse.cpu()[rows], tuple(x[rows] for x in ref), dtype)
+
+
+# Which keys of the last sequence score -inf: the newest alone in its tile, a whole first tile, all but the newest, all,
+# a few anywhere, the second warpgroup's first tile.
+HIDDEN = {"newest_alone": (129, [128]), "first_tile": (300, range(128)), "all_but_newest": (260, range(259)),
+          "all": (140, range(140)), "some": (400, [0, 1, 16, 130, 399]), "second_tile": (384, range(128, 256))}
+
+
+@pytest.mark.parametrize("hq,hk,new", [(2, 1, 1), (6, 2, 5), (6, 2, 90), (8, 8, 33)])
+@pytest.mark.parametrize("name", list(HIDDEN))
+def test_keys_that_score_minus_infinity_have_weight_zero(cuda_device, device_checks, name, hq, hk, new):
+    ctx, keys = HIDDEN[name]
+    batch = positive(make([(new, 200), (new, ctx)], hq, hk, torch.float16))
+    hide(batch, 1, keys)
+    agree(run(batch, cuda_device), reference(batch))
+
+
+@pytest.mark.parametrize("new", [1, 5])
+@pytest.mark.parametrize("name", list(HIDDEN))
+def test_keys_that_score_minus_infinity_in_a_whole_unit(cuda_device, device_checks, name, new):
+    """So many sequences that a CTA has all key tiles of a unit: its two warpgroups merge their rows."""
+    ctx, keys = HIDDEN[name]
+    batch = positive(make([(new, ctx)] * 300, 2, 1, torch.float16))
+    for b in range(0, 300, 3):
+        hide(batch, b, keys)
+    agree(run(batch, cuda_device), reference(batch))
+
+
+def test_key_that_scores_plus_infinity_shows(cuda_device, device_checks):
+    for hq, hk, new, ctx, j in ((2, 1, 1, 129, 128), (2, 1, 1, 300, 3), (6, 2, 90, 300, 250), (6, 2, 90, 300, 256)):
+        batch = positive(make([(new, ctx)], hq, hk, torch.float16))
+        batch[1][slot(batch, 0, j)][..., 0] = math.inf
+        agree(run(batch, cuda_device), reference(batch))
