@@ -131,7 +131,7 @@ __device__ __forceinline__ float tanh_any(float u) {
 
 // 2^x for a pair on the FMA pipe, to 2.2e-7 relative (degree 5, fitted here by a Remez exchange
 // with the constant term set to 1): x = n + f as in exp2_poly_x2. x <= -127, -inf among
-// them, gives exactly 0.
+// them, gives exactly 0; so does NaN, for callers that know of it otherwise.
 __device__ __forceinline__ uint64_t exp2_poly5_x2(uint64_t x2) {
   constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23
   float x0, x1;

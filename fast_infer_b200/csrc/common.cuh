@@ -339,6 +339,18 @@ __device__ __forceinline__ float fmax3f(float a, float b, float c) {
   return r;
 }
 
+// Maxima that are NaN where an operand is (fmaxf passes NaN over).
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // Packed fp32x2 helpers (sm_100 FFMA2 / FADD2): two lanes of work per instruction.
 __device__ __forceinline__ uint64_t f32x2(float lo, float hi) {
   uint64_t r;

@@ -468,19 +468,20 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
 #pragma unroll
               for (int c = 0; c < half; ++c) {
                 const float give = up ? mx[c] : mx[c + half], keep = up ? mx[c + half] : mx[c];
-                mx[c] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, half * 4));
+                mx[c] = fmax_nan(keep, __shfl_xor_sync(0xffffffffu, give, half * 4));
               }
             }
-            mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], 2));
-            mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], 1));
+            mx[0] = fmax_nan(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], 2));
+            mx[0] = fmax_nan(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], 1));
             if ((lane & 3) == 0) bars->n_red[t][quarter][cc + (lane >> 2)] = mx[0];
           }
         __syncwarp();
         named_bar_sync(1 + t, 128);
         if (tid < rows) {
           const float was = n_max[tid];
-          const float now = fmaxf(fmaxf(was, fmaxf(bars->n_red[t][0][tid], bars->n_red[t][1][tid])),
-                                  fmaxf(bars->n_red[t][2][tid], bars->n_red[t][3][tid]));
+          const float now = fmax3_nan(
+              was, fmax_nan(bars->n_red[t][0][tid], bars->n_red[t][1][tid]),
+              fmax_nan(bars->n_red[t][2][tid], bars->n_red[t][3][tid]));
           bars->n_alpha[t][tid] = was == -INFINITY ? 0.f : fast_exp2(was - now);
           n_max[tid] = now;
           bars->n_neg[t][tid] = now == -INFINITY ? FLT_MAX : -now;
@@ -509,7 +510,8 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
       }
       // A row whose max is still -inf (it has seen nothing, or keys that score -inf alone) adds
       // FLT_MAX: a finite score gives 2^FLT_MAX, past any bound, and one of -inf the weight 0. A
-      // score that is NaN stays: the row's result shows it. A column without a row adds -inf: p = 0.
+      // score that is NaN makes NaN of its weight and, where the max moves, of the max: -inf is left
+      // to rows that no score of theirs counts in. A column without a row adds -inf: p = 0.
       float top = 0.f;
 #pragma unroll
       for (int cc = 0; cc < kCkNarrow; cc += 8)
@@ -566,7 +568,7 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
   tc_fence_after();
   const bool whole = u.j0 == 0 && u.j1 == u.n;
   if (t == 0 && tid < rows) {
-    const float m0 = bars->n_max[0][tid], m1 = bars->n_max[1][tid], mx = fmaxf(m0, m1);
+    const float m0 = bars->n_max[0][tid], m1 = bars->n_max[1][tid], mx = fmax_nan(m0, m1);
     float l0 = 0.f, l1 = 0.f;
     for (int i = 0; i < 4; ++i) {
       l0 += bars->n_red[0][i][tid];
@@ -1018,19 +1020,20 @@ __global__ void __launch_bounds__(kCkThreads, 1)
             float a = __uint_as_float(sr[i]);
 #pragma unroll
             for (int kk = 1; kk < 15; kk += 2)
-              a = fmax3f(a, __uint_as_float(sr[i + 8 * kk]),
-                         __uint_as_float(sr[i + 8 * (kk + 1)]));
-            mx8[i] = fmaxf(a, __uint_as_float(sr[i + 120]));
+              a = fmax3_nan(a, __uint_as_float(sr[i + 8 * kk]),
+                            __uint_as_float(sr[i + 8 * (kk + 1)]));
+            mx8[i] = fmax_nan(a, __uint_as_float(sr[i + 120]));
           }
-          const float mx = fmaxf(fmax3f(mx8[0], mx8[1], mx8[2]),
-                                 fmax3f(fmax3f(mx8[3], mx8[4], mx8[5]), mx8[6], mx8[7]));
-          const float m_new = fmaxf(m, mx * sl2);
+          // NaN where any score is: the whole row is NaN then, whichever columns hold it
+          const float mx = fmax_nan(fmax3_nan(mx8[0], mx8[1], mx8[2]),
+                                    fmax3_nan(fmax3_nan(mx8[3], mx8[4], mx8[5]), mx8[6], mx8[7]));
+          const float m_new = fmax_nan(m, mx * sl2);
           bool rescale = false;
           float alpha = 1.f;
           if (j == u.j0) {
             m = m_new;
           } else {
-            const bool need = m_new > m + kCkRescale;
+            const bool need = !(m_new <= m + kCkRescale) && m == m;  // (once to NaN; it stays)
             rescale = __any_sync(0xffffffffu, need);
             if (need) {
               alpha = fast_exp2(m - m_new);

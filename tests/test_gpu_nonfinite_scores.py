@@ -1,5 +1,5 @@
-"""Infinite keys that are seen: a score of -inf has weight 0, one of +inf makes NaN of the rows that see it and of no
-other, in both forms of the attention kernel."""
+"""Infinite and NaN keys and queries that are seen: a score of -inf has weight 0, a NaN or +inf one makes NaN of
+the rows that see it and of no other, in both forms of the attention kernel."""
 
 import math
 
@@ -96,3 +96,28 @@ def test_key_that_scores_plus_infinity_shows(cuda_device, device_checks):
         batch = positive(make([(new, ctx)], hq, hk, torch.float16))
         batch[1][slot(batch, 0, j)][..., 0] = math.inf
         agree(run(batch, cuda_device), reference(batch))
+
+
+@pytest.mark.parametrize("hq,hk,new,ctx", [(2, 1, 1, 700), (6, 2, 4, 300), (6, 2, 90, 300), (6, 2, 300, 900)])
+def test_nan_query_shows_in_its_rows_alone(cuda_device, device_checks, hq, hk, new, ctx):
+    batch = make([(new, ctx), (new, 70)], hq, hk, torch.float16, garbage=0.0)
+    batch[0][new - 1, 1, 5] = math.nan
+    agree(run(batch, cuda_device), reference(batch))
+
+
+@pytest.mark.parametrize("hq,hk,new,ctx,j", [
+    (2, 1, 1, 1, 0), (6, 2, 3, 3, 0), (6, 2, 90, 90, 0),  # the only key that the first token sees
+    (2, 1, 1, 129, 128), (2, 1, 2, 130, 128), (6, 2, 60, 257, 256),  # alone in the last tile of a cut unit
+    (2, 1, 1, 385, 384), (2, 1, 1, 385, 130), (2, 1, 1, 385, 0)])
+def test_nan_key_shows_in_every_row_that_sees_it(cuda_device, device_checks, hq, hk, new, ctx, j):
+    batch = make([(new, ctx)], hq, hk, torch.float16, garbage=0.0)
+    batch[1][slot(batch, 0, j)] = math.nan
+    agree(run(batch, cuda_device), reference(batch))
+
+
+@pytest.mark.parametrize("j", list(range(144, 160)))
+def test_nan_key_shows_at_every_column(cuda_device, device_checks, j):
+    """Wide units, whose columns take two forms of exp2 in turn."""
+    batch = make([(90, 300)], 6, 2, torch.float16, garbage=0.0)
+    batch[1][slot(batch, 0, j)][1, 7] = math.nan  # one KV head of two
+    agree(run(batch, cuda_device), reference(batch))
