@@ -152,16 +152,18 @@ __device__ __forceinline__ uint64_t exp2_poly5_x2(uint64_t x2) {
                __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23)));
 }
 
-__device__ __forceinline__ float exp2_poly5(float x) {  // the same for one value
-  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23
-  x = fmaxf(x, -127.0f);
+// sum + 2^x with the same polynomial for one value: the power of two is a factor, so that NaN stays
+// NaN (in the bits of a sum of exponents it would not). x <= -127 adds exactly 0.
+__device__ __forceinline__ float add_exp2_poly5(float sum, float x) {
+  constexpr float kMagic = 12582912.0f + 127.0f;  // 1.5 * 2^23, and the exponent's bias
+  x = fmax_nan(x, -127.0f);
   const float t = x + kMagic, f = x - (t - kMagic);
   float q = fmaf(kExp5, f, kExp4);
   q = fmaf(q, f, kExp3);
   q = fmaf(q, f, kExp2);
   q = fmaf(q, f, kExp1);
   q = fmaf(q, f, 1.0f);
-  return __uint_as_float(__float_as_uint(q) + (__float_as_uint(t) << 23));
+  return fmaf(q, __uint_as_float(__float_as_uint(t) << 23), sum);
 }
 __device__ __forceinline__ float tanh_poly(float u) {  // tanh_poly_x2 for one value
   const float z = u * u;

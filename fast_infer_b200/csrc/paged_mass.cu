@@ -622,7 +622,7 @@ __global__ void __launch_bounds__(kMsThreads, 1)
           }
 #pragma unroll
           for (int c = 0; c < 16; ++c)
-            sum[c & 3] += c < kMsEmu ? exp2_poly5(x[c]) : fast_exp2(x[c]);
+            sum[c & 3] = c < kMsEmu ? add_exp2_poly5(sum[c & 3], x[c]) : sum[c & 3] + fast_exp2(x[c]);
         }
         tc_fence_before();
         __syncwarp();

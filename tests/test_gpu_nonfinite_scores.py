@@ -1,12 +1,15 @@
-"""Infinite and NaN keys and queries that are seen: a score of -inf has weight 0, a NaN or +inf one makes NaN of
-the rows that see it and of no other, in both forms of the attention kernel."""
+"""Infinite and NaN keys, queries and lse that are seen: a score of -inf has weight 0, a NaN or +inf one makes NaN of
+the rows that see it and of no other, in both forms of the attention kernel and in the weights received."""
 
 import math
 
 import pytest
 import torch
 
-from tests.test_gpu_paged_chunk import PAGE, check, make, run
+from tests.test_gpu_attention_mass import check as check_mass
+from tests.test_gpu_attention_mass import oracle_mass
+from tests.test_gpu_attention_mass import run as run_mass
+from tests.test_gpu_paged_chunk import PAGE, check, make, oracle, run
 
 pytestmark = pytest.mark.gpu
 
@@ -121,3 +124,41 @@ def test_nan_key_shows_at_every_column(cuda_device, device_checks, j):
     batch = make([(90, 300)], 6, 2, torch.float16, garbage=0.0)
     batch[1][slot(batch, 0, j)][1, 7] = math.nan  # one KV head of two
     agree(run(batch, cuda_device), reference(batch))
+
+
+def mass_with_nan(batch, lse, dev, nan_keys=(), nan_rows=()):
+    """Weights of a batch whose one sequence has a NaN key or NaN rows: NaN there and right elsewhere."""
+    q, k, v, table, cu, ctx = batch
+    got = run_mass(batch, dev, lse).cpu()
+    hq, hk = q.shape[1], k.shape[2]
+    new, n = q.shape[0], int(ctx[0])
+    nan = torch.zeros(got.shape, dtype=torch.bool)
+    for j in nan_keys:
+        nan[0, :, j] = True
+    for i, h in nan_rows:
+        nan[0, h // (hq // hk), :n - new + i + 1] = True
+    assert torch.equal(torch.isnan(got), nan)
+    clean = (torch.nan_to_num(q), torch.nan_to_num(k), v, table, cu, ctx)
+    ref = oracle_mass(clean, torch.nan_to_num(lse))
+    check_mass(torch.where(nan, 0.0, got), torch.where(nan, 0.0, ref))
+
+
+@pytest.mark.parametrize("hq,hk,new", [(1, 1, 1), (2, 1, 1), (2, 2, 2), (6, 2, 5), (6, 2, 90), (8, 1, 40)])
+def test_nan_in_mass_shows(cuda_device, device_checks, hq, hk, new):
+    """A NaN key makes NaN of its own weight, a NaN query row or lse of the keys that the row sees."""
+    ctx = 300
+    base = make([(new, ctx)], hq, hk, torch.float16, garbage=0.0)
+    lse = oracle(base)[1].float()
+    for j in (0, ctx - new, 131):
+        if j > ctx - new:
+            continue
+        batch = tuple(t.clone() for t in base)
+        batch[1][slot(batch, 0, j)] = math.nan
+        mass_with_nan(batch, lse, cuda_device, nan_keys=[j])
+    for i, h in ((0, 0), (new - 1, hq - 1), (new // 2, hq // 2)):
+        bad = lse.clone()
+        bad[i, h] = math.nan
+        mass_with_nan(base, bad, cuda_device, nan_rows=[(i, h)])
+        batch = tuple(t.clone() for t in base)
+        batch[0][i, h, 77] = math.nan
+        mass_with_nan(batch, lse, cuda_device, nan_rows=[(i, h)])
