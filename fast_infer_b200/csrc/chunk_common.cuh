@@ -153,10 +153,11 @@ __device__ __forceinline__ uint64_t exp2_poly5_x2(uint64_t x2) {
 }
 
 // sum + 2^x with the same polynomial for one value: the power of two is a factor, so that NaN stays
-// NaN (in the bits of a sum of exponents it would not). x <= -127 adds exactly 0.
+// NaN (in the bits of a sum of exponents it would not). x <= -127 adds exactly 0, x >= 127.5
+// infinity.
 __device__ __forceinline__ float add_exp2_poly5(float sum, float x) {
   constexpr float kMagic = 12582912.0f + 127.0f;  // 1.5 * 2^23, and the exponent's bias
-  x = fmax_nan(x, -127.0f);
+  x = fmin_nan(fmax_nan(x, -127.0f), 128.0f);
   const float t = x + kMagic, f = x - (t - kMagic);
   float q = fmaf(kExp5, f, kExp4);
   q = fmaf(q, f, kExp3);

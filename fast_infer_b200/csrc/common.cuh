@@ -339,10 +339,15 @@ __device__ __forceinline__ float fmax3f(float a, float b, float c) {
   return r;
 }
 
-// Maxima that are NaN where an operand is (fmaxf passes NaN over).
+// Extremes that are NaN where an operand is (fmaxf and fminf pass NaN over).
 __device__ __forceinline__ float fmax_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float fmin_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 __device__ __forceinline__ float fmax3_nan(float a, float b, float c) {

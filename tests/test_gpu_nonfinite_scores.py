@@ -162,3 +162,17 @@ def test_nan_in_mass_shows(cuda_device, device_checks, hq, hk, new):
         batch = tuple(t.clone() for t in base)
         batch[0][i, h, 77] = math.nan
         mass_with_nan(batch, lse, cuda_device, nan_rows=[(i, h)])
+
+
+@pytest.mark.parametrize("hq", [1, 2, 16, 17])
+def test_mass_past_fp32_is_infinite(cuda_device, device_checks, hq):
+    """An lse far below the scores (of a call with a narrower mask, say): weights past fp32 are +inf, not wrapped; those
+    below it hold."""
+    batch = make([(1, 200)], hq, 1, torch.float16, garbage=0.0)
+    lse = oracle(batch)[1].float()
+    got = run_mass(batch, cuda_device, lse - 60.0).cpu()
+    check_mass(got, oracle_mass(batch, lse - 60.0), 8.0)  # arguments of up to 2^7 in log2 units
+    for down in (200.0, 1000.0, 1e30, math.inf):
+        row = (lse - down) if down < math.inf else torch.full_like(lse, -3e38)
+        got = run_mass(batch, cuda_device, row).cpu()
+        assert (got[0, 0, :200] == math.inf).all() and not got[0, 0, 200:].any()
