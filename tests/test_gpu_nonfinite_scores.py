@@ -164,6 +164,18 @@ def test_nan_in_mass_shows(cuda_device, device_checks, hq, hk, new):
         mass_with_nan(batch, lse, cuda_device, nan_rows=[(i, h)])
 
 
+@pytest.mark.parametrize("hq,hk,new", [(1, 1, 1), (6, 2, 5), (6, 2, 90), (7, 1, 90), (8, 8, 200)])
+def test_mass_of_keys_that_score_minus_infinity_is_zero(cuda_device, device_checks, hq, hk, new):
+    """Groups whose tiles do not fill 128 rows among them: the columns left over hold products with 0."""
+    batch = positive(make([(new, 700)], hq, hk, torch.float16, garbage=0.0))
+    lse = oracle(batch)[1].float()
+    ref = oracle_mass(batch, lse)
+    keys = [0, 3, 100, 255, 400]
+    hide(batch, 0, keys)
+    ref[0, :, keys] = 0.0
+    check_mass(run_mass(batch, cuda_device, lse), ref)
+
+
 @pytest.mark.parametrize("hq", [1, 2, 16, 17])
 def test_mass_past_fp32_is_infinite(cuda_device, device_checks, hq):
     """An lse far below the scores (of a call with a narrower mask, say): weights past fp32 are +inf, not wrapped; those
