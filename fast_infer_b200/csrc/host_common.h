@@ -58,6 +58,10 @@ class DeviceOnce {
   std::atomic<bool> done_[kMaxCachedDevices] = {};
 };
 
+// Whether a dimension's stride (16-bit elements) keeps 16-byte accesses aligned; one of size 1 is never
+// stepped over.
+inline bool stride_ok(int64_t size, int64_t stride) { return size == 1 || stride % 8 == 0; }
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Programmatic dependent launch is on unless the environment sets FI_PDL=0.

@@ -424,10 +424,11 @@ extern "C" int fi_kv_evict(const void* k, const void* v, const int32_t* block_ta
   bool ok = aligned16(k) && aligned16(v) && aligned16(k_out) && aligned16(v_out);
   const int64_t* strides[4] = {k_strides, v_strides, ko_strides, vo_strides};
   int64_t* bytes[4] = {a.ks, a.vs, a.kos, a.vos};
+  const int64_t sizes[4] = {layers, num_blocks, block_size, num_heads};
   for (int t = 0; t < 4; ++t) {
     ok = ok && strides[t][4] == 1;
     for (int i = 0; i < 4; ++i) {
-      ok = ok && strides[t][i] % 8 == 0;
+      ok = ok && stride_ok(t >= 2 && i == 1 ? num_blocks_out : sizes[i], strides[t][i]);
       bytes[t][i] = strides[t][i] * 2;
       if (in_place && t >= 2 && strides[t][i] != strides[t - 2][i])
         return fail(FI_ERR_INVALID_ARG, "fi_kv_evict: in place with other strides");

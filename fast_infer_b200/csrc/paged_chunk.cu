@@ -1310,7 +1310,8 @@ extern "C" int fi_paged_chunk(const void* q, const void* k_cache, const void* v_
                 "fi_paged_chunk: at most %d sequences and %lld tokens with %d query heads per KV "
                 "head; split the batch",
                 kCkMaxBatch, (long long)((kCkMaxUnits - batch) * unit_tokens), p.b.group);
-  if (o_strides[2] != 1 || !aligned16(o) || o_strides[0] % 8 != 0 || o_strides[1] % 8 != 0)
+  if (o_strides[2] != 1 || !aligned16(o) || !stride_ok(total_tokens, o_strides[0]) ||
+      !stride_ok(num_q_heads, o_strides[1]))
     return fail(FI_ERR_ALIGNMENT,
                 "fi_paged_chunk o: needs a 16-byte aligned base, unit innermost stride and other "
                 "strides multiple of 8");
@@ -1336,8 +1337,9 @@ extern "C" int fi_paged_chunk(const void* q, const void* k_cache, const void* v_
   p.o = o;
   p.os[0] = o_strides[0];
   p.os[1] = o_strides[1];
-  p.o_wide = reinterpret_cast<uintptr_t>(o) % 32 == 0 && o_strides[0] % 16 == 0 &&
-             o_strides[1] % 16 == 0;
+  p.o_wide = reinterpret_cast<uintptr_t>(o) % 32 == 0 &&
+             (total_tokens == 1 || o_strides[0] % 16 == 0) &&
+             (num_q_heads == 1 || o_strides[1] % 16 == 0);
   p.lse = lse;
   p.err = error_flag;
   uint8_t* ws = static_cast<uint8_t*>(workspace);

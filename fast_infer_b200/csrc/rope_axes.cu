@@ -231,9 +231,11 @@ extern "C" int fi_rope_axes_store(const void* qkv, void* q_out, void* k_cache, v
       num_kv_heads > 65535 || num_blocks > (1 << 30) || max_blocks_per_seq > (1 << 24))
     return fail(FI_ERR_UNSUPPORTED, "fi_rope_axes_store: sizes too large");
   bool ok = qkv_strides[1] == 1 && q_out_strides[2] == 1 && kc_strides[3] == 1 &&
-            vc_strides[3] == 1 && qkv_strides[0] % 8 == 0 && q_out_strides[0] % 8 == 0 &&
-            q_out_strides[1] % 8 == 0;
-  for (int i = 0; i < 3; ++i) ok = ok && kc_strides[i] % 8 == 0 && vc_strides[i] % 8 == 0;
+            vc_strides[3] == 1 && stride_ok(total_tokens, qkv_strides[0]) &&
+            stride_ok(total_tokens, q_out_strides[0]) && stride_ok(num_q_heads, q_out_strides[1]);
+  const int64_t cache_sizes[3] = {num_blocks, block_size, num_kv_heads};
+  for (int i = 0; i < 3; ++i)
+    ok = ok && stride_ok(cache_sizes[i], kc_strides[i]) && stride_ok(cache_sizes[i], vc_strides[i]);
   ok = ok && aligned16(qkv) && aligned16(q_out) && aligned16(k_cache) && aligned16(v_cache);
   if (!ok)
     return fail(FI_ERR_ALIGNMENT,
