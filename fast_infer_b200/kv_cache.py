@@ -147,13 +147,16 @@ class KVCache:
         if self.num_tokens > 0 and not self.seq_lens.any():
             raise ValueError("extend needs per-sequence lengths (its own, or store_kv_ragged's)")
         B = nn.shape[0]
-        self._grow_batch(B)
-        need = -(-(self.seq_lens[:B] + nn) // self.block_size)
+        old = min(B, self._bt.shape[0])
+        lens, held = nn.copy(), np.zeros(B, np.int64)  # (sequences past the table hold nothing yet)
+        lens[:old] += self.seq_lens[:old]
+        held[:old] = (self._bt[:old] >= 0).sum(1)
+        need = -(-lens // self.block_size)
         if (need > self.max_blocks_per_seq).any():
             raise RuntimeError("Sequence block table full")
-        held = (self._bt[:B] >= 0).sum(1)
         if int(np.maximum(need - held, 0).sum()) > len(self.free_blocks):
             raise RuntimeError("KV cache out of memory")
+        self._grow_batch(B)
         for b in range(B):
             self._ensure_blocks(b, int(need[b]))
         self.seq_lens[:B] += nn
