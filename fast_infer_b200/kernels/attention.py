@@ -427,7 +427,9 @@ def attention_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Te
     heads of hk. Arguments and score form as in ``paged_chunk_attention``, whose ``lse`` this takes;
     pass the last tokens alone (with ``cu_seqlens`` to match) for the weight of a window of
     them. ``mass``: fp32 [batch, num_kv_heads, capacity] to add to and return (what cached
-    tokens had before); without it, a new one of the block table's span, 0 where nothing sees.
+    tokens had before); without it, a new one of the block table's span, 0 where nothing sees. The
+    weights of cached tokens past a ``mass`` that is shorter than a sequence are dropped, which only
+    device checks (``FAST_INFER_B200_CHECK=1``) report, with a RuntimeError.
     ``workspace``: uint8, at least ``attention_mass_workspace_bytes`` bytes; calls that may run at
     the same time need one each (the default allocates per call).
     """

@@ -51,6 +51,10 @@ def evict_tokens(k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor,
     sequences. ``out`` = (k_out, v_out, block_table_out) writes them to those pools' pages instead
     and leaves the source as it was (the pages read and written must not overlap).
 
+    ``capacity`` and the block table have to reach as far as every sequence: a longer one counts as if
+    it ended there (``recent`` with it), and its newest tokens are lost. Lengths are on the device, so
+    only device checks (``FAST_INFER_B200_CHECK=1``) report that, with a RuntimeError.
+
     Returns (kept, mass_out), both [layers, batch, num_heads, budget]: the old slots that stay,
     ascending (int32, -1 past the last), and their mass (0 past the last).
     """
