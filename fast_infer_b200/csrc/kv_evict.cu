@@ -488,7 +488,7 @@ extern "C" int fi_kv_evict(const void* k, const void* v, const int32_t* block_ta
   // Many short rows: one kernel, whose selections run beside other rows' moves (28 x 16 x 8 rows of
   // 2048 tokens to 1024: 633 us, 690 in two, in place 645 and 695; 1 x 100 x 8: 155 and 164, in
   // place 161 and 168). Fewer rows leave SMs without one to move (28 x 3 x 8 of 8192 to 2048: 281
-  // and 271).
+  // and 271; a few short rows, whose move is less than a launch, were not measured).
   if (is_short && rows >= 5 * sm_count()) {
     e = in_place ? launch_pdl(evict_row_kernel<kEvShort, true, true>, grid, dim3(kEvShort), smem, st, a)
                  : launch_pdl(evict_row_kernel<kEvShort, true, false>, grid, dim3(kEvShort), smem, st, a);

@@ -27,11 +27,13 @@
 //   caches; long prefills lost 10 %, single tokens 40 %.) A batch that may hold both kinds
 //   launches both kernels, the second beginning on each SM as the first leaves it. (Sharing the
 //   SMs out between them by cost was no faster: a step of 24 rows costs as much as a wide one.)
-// * What bounds it: a wide step of 256 rows x 128 keys takes 3850 cycles, of which its products need
-//   2040 of the tensor core and its exponentials 1800 of the special function units; issue slots and
-//   the chain through tensor memory are the rest. 4096 tokens over 61003: 3.43 to 3.56 ms, 890 to 925 TFLOP/s at the power cap's
-//   1.45 GHz; 4225 over 2000: 214 us, 999 TFLOP/s. Single tokens are bound by HBM: 64 over 4000
-//   each, 179 us, 5.9 TB/s; one over 512 by its two launches, 12.4 us.
+// * What bounds it: a wide step of 256 rows x 128 keys takes 3850 cycles, of which (by count, not by
+//   counters) its products need 2040 of the tensor core and its exponentials 1800 of the special
+//   function units; issue slots and the chain through tensor memory are the rest. 4096 tokens over
+//   61003: 3.18 ms, 999 TFLOP/s, in a burst of 15 ms; repeated for seconds 3.71 ms, 856 TFLOP/s, at
+//   the 1.39 GHz that the power cap leaves. 4225 over 2000: 215 us, 992 TFLOP/s (for seconds 250, at
+//   1.69 GHz). Single tokens are bound by HBM: 64 over 4000 each, 178 us, 5.9 TB/s; one over 512 by
+//   its two launches, 12.3 us.
 // * Slots behind a sequence's last token may hold anything: their scores are replaced by
 //   -inf, and their V rows are zeroed in shared memory before the product (0 * NaN is NaN).
 #include <float.h>
@@ -336,6 +338,10 @@ __device__ __forceinline__ void score_form8(const uint32_t* raw, float* s, const
 // p = 2^(s * sl2 - mref) of a row, its sum, and p packed in place. 1 of 8 pairs takes exp2 on the
 // FMA pipe (0: 4772 us for a chunk of 4096 tokens over 61003, 1: 3587, 2: 3746, 3: 3802), to 2.2e-7:
 // lse is an output, which a rougher polynomial would show in.
+// The sum takes p in 32 bits; the product with V takes it in V's type, as kind::f16 asks of both
+// operands: half a step (2^-12 .. 2^-11, bf16 2^-9 .. 2^-8) of each p, which adds to the output's own
+// rounding: 3.0e-4 in place of 2.1e-4 (root mean square, relative; bf16 2.3e-3 and 1.7e-3). P as the
+// sum of two such values would take the product twice.
 template <typename T>
 __device__ __forceinline__ float ck_exp(uint32_t* sr, float sl2, float mref) {
   const uint64_t sc2 = f32x2(sl2, sl2), nm2 = f32x2(-mref, -mref);
@@ -538,7 +544,7 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
       if (cc < rows) {
 #pragma unroll
         for (int c = cc; c < cc + 8; c += 2) {
-          l[c] += s[c];
+          l[c] += s[c];  // in 32 bits; P is rounded to V's type for the product (see ck_exp)
           l[c + 1] += s[c + 1];
           const uint32_t pk = Half16<T>::pack(s[c], s[c + 1]);
           *reinterpret_cast<uint16_t*>(pcol + c * 128 + (kbyte ^ ((c & 7) << 4))) = (uint16_t)pk;

@@ -18,8 +18,9 @@
 // * What bounds a chunk's step of 512 keys x 128 rows: its 65536 exponentials (4096 cycles of the
 //   SM's MUFU, against 2048 of the tensor core), of which some run as a polynomial on the FMA
 //   pipe, and the query tile's 32 KB from L2 (units of 256 keys read 6.3 TB/s of them on the
-//   whole GPU and were bound by that). 2048 tokens over 30011: 473 us, 825 TFLOP/s; single tokens of
-//   16 sequences over 1000 to 4095: 22 us, 3.3 TB/s (8 us of it start and drain).
+//   whole GPU and were bound by that). 2048 tokens over 30011: 482 us, 811 TFLOP/s, in a burst of
+//   10 ms; repeated for seconds 516 us at the 1.84 GHz that the power cap leaves. Single tokens of 16
+//   sequences over 1000 to 4095: 22 us, 3.3 TB/s (8 us of it start and drain).
 // * Roles (640 threads): warps 0-15 = the sums, a warpgroup per key tile (one per warp scheduler
 //   would show its latencies: eight warps took twice the time), warp 16 = TMA, warp 17 = UMMA
 //   issue, warp 18 = the rows' lse (and slopes and positions) into shared memory, warp 19 =

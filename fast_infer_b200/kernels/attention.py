@@ -369,7 +369,10 @@ def paged_chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     never past context_lens[b]. Scores are ``q.k * sm_scale``, capped as ``softcap * tanh(x /
     softcap)`` if ``softcap``, less ``alibi_slopes[head] * |p - j|`` if given (fp32 [num_q_heads]).
     A token that sees nothing gives zeros and an lse of -inf. Slots past context_lens[b] may hold
-    anything; V before them has to be finite, seen or not (hidden keys count with weight 0).
+    anything; V before them has to be finite, seen or not (hidden keys count with weight 0). A key
+    whose score is -inf has weight 0; a NaN or +inf score makes NaN of the rows that see it. Pages with
+    an invalid block-table entry are skipped and lengths that do not fit are cut, which only device
+    checks (``FAST_INFER_B200_CHECK=1``) report, with a RuntimeError.
 
     Returns o like q (written to ``out`` if given; rows outside every sequence are not written),
     and with ``return_lse`` also lse: fp32 [total_tokens, num_q_heads], the natural log of the sum

@@ -32,7 +32,9 @@ def rope_axes_store(qkv: torch.Tensor, num_q_heads: int, cos_table: torch.Tensor
     them next; new token i of sequence b is stored at slot ``context_lens[b] - n_b + i``.
 
     The rotation is the rotate-half form in fp32, rounded once. Returns the rotated q
-    [total_tokens, nq, 128] (``q_out`` if given; rows outside every sequence are not written).
+    [total_tokens, nq, 128] (``q_out`` if given; rows outside every sequence are not written). A token
+    with a position outside the tables is skipped, and one whose slot has no page is not stored, which
+    only device checks (``FAST_INFER_B200_CHECK=1``) report, with a RuntimeError.
     """
     _check_rows("qkv", qkv)
     shape = k_cache.shape if isinstance(k_cache, torch.Tensor) else None

@@ -192,7 +192,8 @@ int fi_paged_decode_noalloc(const void* q, const void* k_cache, const void* v_ca
  * score = f(q.k * sm_scale) - alibi_slopes[h] * |p - j|, f(x) = x, or softcap * tanh(x /
  * softcap) when softcap > 0 (alibi_slopes: fp32 [num_q_heads] or NULL). sm_scale > 0.
  * o = softmax over the visible keys . v; lse (fp32 [total_tokens, num_q_heads] or NULL) = the
- * natural log of the sum of exp(score). A token that sees nothing gets o = 0, lse = -inf.
+ * natural log of the sum of exp(score). A token that sees nothing gets o = 0, lse = -inf. A score of
+ * -inf counts as weight 0; a NaN or +inf one makes NaN of the row.
  * Slots behind a sequence's last token may hold anything; V of a cached token has to be finite even
  * where a token does not see it (it counts with weight 0). A page whose block-table entry is
  * invalid is skipped (FI_DEVERR_BAD_BLOCK); lengths that do not fit total_tokens or the block
@@ -225,7 +226,8 @@ int fi_paged_chunk(const void* q, const void* k_cache, const void* v_cache, void
  * mass_capacity], dense; accumulate 0 writes all of it (0 where nothing sees, past the
  * context too), any other value adds to it and leaves the rest as it was. Cached tokens past
  * mass_capacity are dropped (FI_DEVERR_CONTEXT_LEN). A row with lse = -inf gives no weight, nor
- * does a page with an invalid block-table entry receive any. workspace:
+ * does a page with an invalid block-table entry receive any; a NaN score makes NaN of its
+ * key's weight, a NaN lse of all that its row sees, and a weight past fp32 is infinite. workspace:
  * fi_attention_mass_workspace_size() bytes, 16-byte aligned. Deterministic.
  */
 size_t fi_attention_mass_workspace_size(void);
