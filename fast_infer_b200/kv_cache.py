@@ -140,7 +140,8 @@ class KVCache:
         allocated (the reference's first-free-slot / FIFO rule), ``seq_lens`` grows, and
         (cu_seqlens, context_lens) come back as device int32 tensors, as ``rope_axes_store``,
         ``paged_chunk_attention`` and ``attention_mass`` take them. Raises before it changes
-        anything if the pool or a sequence's table is too small."""
+        anything if the pool or a sequence's table is too small. Only tokens of its own and of
+        ``store_kv_ragged`` count: ``store`` and ``write_tokens`` alone keep no lengths."""
         nn = np.asarray(n_new, np.int64).reshape(-1)
         if (nn < 0).any():
             raise ValueError("n_new must not be negative")
@@ -181,7 +182,7 @@ class KVCache:
         if B > self._bt.shape[0]:
             raise ValueError("batch larger than the block table")
         lens = self.seq_lens[:B]
-        if self.num_tokens > 0 and not lens.any():
+        if not lens.any() and (self.num_tokens > 0 or (self._bt[:B] >= 0).any()):
             raise ValueError("evict needs per-sequence lengths (extend or store_kv_ragged)")
         if B > 0 and int(lens.max()) > mass.shape[3]:
             raise ValueError(f"mass holds {mass.shape[3]} tokens, a sequence has {int(lens.max())}")

@@ -21,3 +21,12 @@ def test_extend_that_raises_does_not_grow_the_batch(n_new, match):
     cu, ctx = cache.extend([1, 0, 100])  # and one that fits grows it
     assert cu.tolist() == [0, 1, 1, 101] and ctx.tolist() == [71, 64, 100]
     assert cache.block_table.tolist() == [[0, 1, -1, -1], [2, -1, -1, -1], [3, 4, -1, -1]]
+
+
+def test_evict_refuses_pages_whose_tokens_it_does_not_know():
+    """Tokens written by store / write_tokens into pages of alloc_block have no length: all their pages would go."""
+    cache = KVCache(1, 2, 128, 256, 64, torch.device("cpu"), num_blocks=5)
+    cache.alloc_block(0)
+    with pytest.raises(ValueError, match="per-sequence"):
+        cache.evict(torch.zeros(1, 1, 2, 256), 8)
+    assert cache.free_blocks == [1, 2, 3, 4] and cache._bt[0, 0] == 0
