@@ -27,6 +27,9 @@ FI_DEVERR_CONTEXT_LEN = 4
 FI_STATIC_WEIGHTS = 1
 FI_DTYPE_F16 = 0
 FI_DTYPE_BF16 = 1
+FI_DTYPE_I8 = 2
+FI_DTYPE_E4M3 = 3
+FI_DTYPE_F32 = 4
 
 _STATUS_NAMES = {
     FI_ERR_INVALID_ARG: "FI_ERR_INVALID_ARG",
@@ -70,6 +73,13 @@ SIGNATURES = {
                                           _i64, _i64, _i64, _i64, _i64, _i64p, _i64, _i64, _i64,
                                           _i64, _i64, _i64, _i64p, _i64p, _i64p, _i64p, _i64p,
                                           _i64, _vp, _vp]),
+    "fi_rope_axes_store8": (ctypes.c_int, [_vp] * 12 + [_i64] * 6 + [_i64p] + [_i64] * 6 +
+                            [_i64p] * 7 + [_i64, _i64, _vp, _vp]),
+    "fi_read_kv8": (ctypes.c_int, [_vp] * 9 + [_i64] * 7 + [_i64p] * 7 + [_i64, _i64, _vp, _vp]),
+    "fi_draft_tree": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "fi_accept_drafts": (ctypes.c_int, [_vp] * 7 + [_i64, _i64, _vp, _vp]),
+    "fi_keep_accepted": (ctypes.c_int, [_vp] * 9 + [_i64] * 8 + [_i64p] * 5 + [_i64, _vp, _vp]),
+    "fi_sample_tokens": (ctypes.c_int, [_vp] * 6 + [_f32, _i64, _f32, _f32, _vp] + [_i64] * 4 + [_vp]),
     "fi_kv_evict": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
                                    _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                    _i64, _i64p, _i64p, _i64p, _i64p, _i64p, _i64p, _vp, _vp]),

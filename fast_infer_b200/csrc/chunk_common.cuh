@@ -218,6 +218,21 @@ __device__ __forceinline__ int last_le(const U* a, int n, U x) {
   return lo;
 }
 
+// The sequence of packed row t, cu[0] <= t < cu[batch]: the last b with cu[b] <= t, found by a warp, whose lanes
+// probe 32 places at a time; -1 where cu is not ascending and t has none.
+__device__ __forceinline__ int token_sequence(const int32_t* cu, int batch, int t, int lane) {
+  int lo = 0, n = batch;
+  while (n > 1) {
+    const int gap = (n + 31) / 32, probe = lane * gap;
+    const uint32_t le =
+        __ballot_sync(0xffffffffu, probe < n && cu[lo + (probe < n ? probe : 0)] <= t);
+    const int i = max(31 - __clz((int)le), 0);  // (cu not ascending: any of them)
+    n = min(gap, n - i * gap);
+    lo += i * gap;
+  }
+  return t >= cu[lo + 1] ? -1 : lo;
+}
+
 // Host: fill the parts that both entry points check alike. Returns FI_OK or an error.
 int chunk_batch_args(ChunkBatch& p, const char* what, const int32_t* cu, const int32_t* ctx,
                      const int32_t* prefix, const int32_t* bt, int64_t batch, int64_t total,

@@ -1,0 +1,76 @@
+// 8-bit codes of cached rows: a row of 128 values x (one token, one head) is held as codes and one fp32
+// scale, x ~ code * scale with scale = max|x| / Q and code = Q * x / max|x| rounded to the nearest
+// code, ties to even; Q = 127 (int8) or 448 (e4m3, its largest value).
+//
+// Q * x is exact for x of 16 bits (11 bits times 7), and a quotient of such numbers that is not a tie
+// lies further from one than half a step of fp32, so one IEEE division gives the codes of exact
+// arithmetic. Both codes are exact in fp16 and bf16.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "umma.cuh"
+
+namespace fi {
+
+struct CodeI8 {
+  static constexpr float kTop = 127.f;
+  // codes of 4 values of at most 127
+  __device__ static __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+    const uint32_t x = (uint32_t)__float2int_rn(a) & 0xff, y = (uint32_t)__float2int_rn(b) & 0xff;
+    const uint32_t z = (uint32_t)__float2int_rn(c) & 0xff, w = (uint32_t)__float2int_rn(d);
+    return x | (y << 8) | (z << 16) | (w << 24);
+  }
+  // Two bytes of `v` (already offset by `bias`) as fp16: 0x64uu is 1024 + uu.
+  static constexpr uint32_t kBias = 0x80808080u;  // code + 128 is the byte xor 0x80
+  template <uint32_t kSel>
+  __device__ static __forceinline__ uint32_t half2_of(uint32_t biased) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, 0x64646464, %2;" : "=r"(r) : "r"(biased), "n"(kSel));
+    const __half2 m = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
+    const __half2 h = __hsub2(*reinterpret_cast<__half2*>(&r), m);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  // fp16 pairs of codes (0, 1) and (2, 3)
+  __device__ static __forceinline__ void decode4(uint32_t v, uint32_t& lo, uint32_t& hi) {
+    const uint32_t b = v ^ kBias;
+    lo = half2_of<0x4140>(b);
+    hi = half2_of<0x4342>(b);
+  }
+};
+
+struct CodeE4M3 {
+  static constexpr float kTop = 448.f;
+  __device__ static __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+  }
+  __device__ static __forceinline__ void decode4(uint32_t v, uint32_t& lo, uint32_t& hi) {
+    asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\n"
+        "cvt.rn.f16x2.e4m3x2 %1, b;\n}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(v));
+  }
+};
+
+// Codes of `v[0..N)`, a lane's part of a row whose greatest magnitude is `top`, and the row's scale. NaN or an
+// infinity in the row (top then is one) gives the scale NaN and codes 0, so that every reader sees it.
+template <typename C, int N>
+__device__ __forceinline__ float encode_row(const float* v, float top, uint32_t* codes) {
+  const bool finite = top < INFINITY;
+  // Q * x within fp32: a power of two off both (what that makes subnormal has the code 0 all the same)
+  const float shrink = top > 1e30f ? 0x1p-20f : 1.f;
+  const float den = top * shrink, num = C::kTop * shrink;
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    float z[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      z[j] = finite && top > 0.f ? __fdiv_rn(v[i + j] * num, den) : 0.f;
+    codes[i / 4] = C::encode4(z[0], z[1], z[2], z[3]);
+  }
+  return finite ? __fdiv_rn(top, C::kTop) : __int_as_float(0x7fffffff);
+}
+
+}  // namespace fi

@@ -1,0 +1,704 @@
+// Sampling of one token per row of logits, with temperature, top-k, top-p and min-p, from a given
+// uniform number.
+//
+// With x the row, M its maximum and w_i = exp((x_i - M) / T), tokens are ordered by x descending, ties by
+// index. Top-k keeps the first k, top-p those of them whose mass before them is below p times
+// theirs all, min-p those with w >= min_p. All three keep a head of the order, so together they are one
+// cut: a value c and how many of the tokens that equal c stay (the lowest indexes). The token is the
+// first index whose running sum of kept w passes u times the whole.
+//
+// * Sums decide between neighbours whose masses lie 1e-6 apart or less, so weights are computed to 2^-45
+//   (in fp64: 2^(n/32) from a table times a polynomial) and added as integers: any order gives the
+//   same sum, on every run and for every split of the row. A token is the one that 64-bit arithmetic
+//   finds, but for a boundary within 1e-11 of u.
+// * A cluster of up to 8 CTAs holds a row in shared memory, read once. The cut is found by
+//   histograms over 512 bins, first of M - x, then of the bits of x within the bin that holds it, until
+//   the bin is one value; bins add integers by shared-memory atomics (three 15- or 16-bit limbs, so
+//   that no sum of a CTA's values overflows 32 bits) and are joined through distributed
+//   shared memory.
+// * The last pass adds kept weights in index order, 256 tokens a warp at a time; the 256 that hold
+//   the target are looked at again by one warp.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <float.h>
+
+#include "common.cuh"
+#include "host_common.h"
+
+namespace cg = cooperative_groups;
+
+namespace fi {
+
+constexpr int kSaThreads = 512;
+constexpr int kSaWarps = kSaThreads / 32;
+constexpr int kSaBins = kSaThreads;     // a bin per thread where bins are joined
+constexpr int kSaStep = 256;            // tokens of a warp's step
+constexpr int kSaSteps = 8;             // steps of a warp at most: 32768 tokens a CTA, as the limbs allow
+constexpr int kSaMaxCluster = 8;
+constexpr int64_t kSaMaxVocab = (int64_t)kSaMaxCluster * kSaWarps * kSaSteps * kSaStep;
+
+struct SampleArgs {
+  const void* x;
+  int64_t stride;
+  const float* u;
+  const float* temperature;  // these four: null, or one value per row
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature1, top_p1, min_p1;
+  int top_k1;
+  int32_t* out;
+  int vocab, chunk;  // chunk: tokens of a warp
+};
+
+template <typename T>
+__device__ __forceinline__ float logit(T x);
+template <>
+__device__ __forceinline__ float logit(float x) { return x; }
+template <>
+__device__ __forceinline__ float logit(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float logit(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// Low bits of a key that say nothing, by type.
+template <typename T>
+struct KeyGrain { static constexpr int kBits = 0; };
+template <>
+struct KeyGrain<__half> { static constexpr int kBits = 13; };
+template <>
+struct KeyGrain<__nv_bfloat16> { static constexpr int kBits = 16; };
+
+// Eight consecutive logits from shared memory, -0 as 0.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float* x) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p);
+    *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(p + 4);
+  } else {
+    const uint4 raw = *reinterpret_cast<const uint4*>(p);
+    const T* t = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = logit(t[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] += 0.f;
+}
+
+// Unsigned keys in the order of the floats.
+__device__ __forceinline__ uint32_t key_of(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float of_key(uint32_t k) {
+  return __uint_as_float(k ^ ((uint32_t)((int32_t)~k >> 31) | 0x80000000u));
+}
+
+// What a pass knows of its row.
+struct Row {
+  float top;      // M
+  float floor_x;  // no weight below it: under half a unit, or x = -inf
+  double m, c32;  // M, 32 * log2(e) / T
+};
+
+// exp((x - M) / T) in units of 2^-45, for x >= floor_x: 2^(n / 32) times e^r, |r| <= ln 2 / 64, by the
+// series to r^6 (its rest is 4e-18).
+__device__ __forceinline__ uint64_t weight(const Row& row, const double* tab, float x) {
+  constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52
+  constexpr double kC1 = 0.021660849392498291, kC2 = 2.3459619820224679e-4,
+                   kC3 = 1.6938509724371820e-6, kC4 = 9.1725627018246433e-9,
+                   kC5 = 3.9737099845494162e-11, kC6 = 1.4345655584131936e-13;
+  const double y = ((double)x - row.m) * row.c32;
+  const double t = y + kMagic;
+  const int n = __double2loint(t);
+  const double r = y - (t - kMagic);
+  double q = fma(kC6, r, kC5);
+  q = fma(q, r, kC4);
+  q = fma(q, r, kC3);
+  q = fma(q, r, kC2);
+  q = fma(q, r, kC1);
+  q = fma(q, r, 1.0);
+  const double s = q * tab[n & 31];
+  const double w = __hiloint2double(__double2hiint(s) + ((n >> 5) << 20), __double2loint(s));
+  // 128's last bit is 2^-45
+  return (uint64_t)__double_as_longlong(w + 128.0) - (uint64_t)__double_as_longlong(128.0);
+}
+
+struct SaPart {  // what a CTA tells the others about its slice
+  float top, low;  // greatest logit; least of its threads' greatest ones
+  float least;     // least logit above -inf
+  int threads;     // threads with a logit above -inf
+  int bad;         // NaN or +inf
+  int index;       // greedy: first index of the greatest
+  int ties;
+  uint64_t mass;
+};
+struct SaShared {
+  double tab[32];
+  uint64_t step_mass[kSaWarps * kSaSteps];
+  uint64_t scan[kSaWarps];
+  uint32_t hist[2][kSaBins][3];
+  SaPart part;
+  float w_top[kSaWarps], w_low[kSaWarps], w_least[kSaWarps];
+  int w_ties[kSaWarps];
+  // the bin that a search chose
+  uint64_t above, held, total;
+  uint32_t edge[2];
+  int bin;
+  uint32_t min_key;
+};
+
+// Sum over the block's threads before this one, and of all, of a 64-bit value.
+__device__ __forceinline__ uint64_t block_exclusive(uint64_t v, uint64_t* warp_sums, uint64_t& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint64_t inc = v;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const uint64_t o = __shfl_up_sync(0xffffffffu, inc, off);
+    if (lane >= off) inc += o;
+  }
+  if (lane == 31) warp_sums[warp] = inc;
+  __syncthreads();
+  uint64_t before = 0;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kSaWarps; ++w) {
+    const uint64_t s = warp_sums[w];
+    if (w < warp) before += s;
+    all += s;
+  }
+  __syncthreads();
+  return before + inc - v;
+}
+
+__device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+
+// A cut: tokens whose key is above `key` stay, and of those that have it the first `ties` by index.
+struct Cut {
+  uint32_t key;
+  int64_t ties;
+  bool all_ties;
+};
+
+// The bin of a value in a search's first level.
+__device__ __forceinline__ int linear_bin(float top, float scale, float x) {
+  return min((int)((top - x) * scale), kSaBins - 1);
+}
+
+// The cut at which the count of tokens reaches `want` (kMass = false), or the mass that `share` of all from
+// lo_key on, less `drop`, asks for. `above` of the result's group: what lies before it.
+template <typename T, bool kMass>
+__device__ __forceinline__ Cut search(cg::cluster_group& cluster, SaShared* s, const T* x, int steps,
+                                      int chunk_base, const Row& row, uint32_t lo_key, int64_t want,
+                                      double share, uint64_t drop, int& level) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int ctas = (int)cluster.num_blocks();
+  uint32_t hi_key = key_of(row.top);
+  const float range = row.top - of_key(lo_key);
+  const float scale = range > 0.f && range < FLT_MAX ? (float)(kSaBins - 1) / range : 0.f;
+  uint64_t above = 0, held = 0;
+  double target = 0.0;
+  bool first = true;
+  int shift = 0;
+#pragma unroll 1
+  while (true) {
+    uint32_t(*hist)[3] = s->hist[level & 1];
+#pragma unroll 1
+    for (int st = 0; st < steps; ++st) {
+      float v[8];
+      load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t k = key_of(v[i]);
+        if (k < lo_key || k > hi_key || v[i] == -INFINITY) continue;
+        const int b = first ? linear_bin(row.top, scale, v[i])
+                            : (int)((hi_key >> shift) - (k >> shift));
+        if constexpr (kMass) {
+          if (v[i] < row.floor_x) continue;
+          const uint64_t w = weight(row, s->tab, v[i]);
+          const uint32_t l0 = (uint32_t)w & 0x7fff, l1 = (uint32_t)(w >> 15) & 0x7fff,
+                         l2 = (uint32_t)(w >> 30);
+          if (l0) atomicAdd(&hist[b][0], l0);
+          if (l1) atomicAdd(&hist[b][1], l1);
+          if (l2) atomicAdd(&hist[b][2], l2);
+        } else {
+          atomicAdd(&hist[b][0], 1u);
+        }
+      }
+    }
+    cluster.sync();
+    ++level;
+    // every CTA has read the other buffer before it came here
+    for (int i = tid; i < kSaBins * 3; i += kSaThreads) (&s->hist[level & 1][0][0])[i] = 0;
+    uint64_t mine = 0;
+    for (int r = 0; r < ctas; ++r) {
+      const uint32_t* h = cluster.map_shared_rank(&hist[tid][0], r);
+      mine += kMass ? (uint64_t)h[0] + ((uint64_t)h[1] << 15) + ((uint64_t)h[2] << 30) : h[0];
+    }
+    uint64_t all;
+    const uint64_t before = above + block_exclusive(mine, s->scan, all);
+    if (kMass && first) target = fmax(share * (double)(all - drop), 1.0);
+    const bool pick = kMass ? (double)before < target && (double)(before + mine) >= target
+                            : before < (uint64_t)want && before + mine >= (uint64_t)want;
+    if (tid == 0) s->bin = -1;
+    __syncthreads();
+    if (pick && mine > 0) {
+      s->bin = tid;
+      s->above = before;
+      s->held = mine;
+    }
+    __syncthreads();
+    const int bin = s->bin;
+    if (bin < 0) {  // fewer tokens than wanted: all stay
+      return {0u, 0, true};
+    }
+    above = s->above;
+    held = s->held;
+    if (first) {
+      // the bin's keys, by a 32-way search of each edge: bins fall as keys rise
+      if (warp < 2) {
+        uint32_t lo = lo_key, hi = hi_key;  // edge 0: least key in the bin; edge 1: greatest
+#pragma unroll 1
+        while (hi > lo) {
+          const uint32_t gap = (hi - lo) / 32 + 1;
+          const uint32_t probe = lo + min((uint32_t)lane * gap, hi - lo);
+          const int b = linear_bin(row.top, scale, of_key(probe));
+          const uint32_t in = __ballot_sync(0xffffffffu, warp == 0 ? b > bin : b >= bin);
+          // probes of an edge's near side form a head of the lanes
+          const int n = in == 0xffffffffu ? 32 : __ffs((int)~in) - 1;
+          if (warp == 0) {  // the least key with b <= bin lies in (probe n-1, probe n]
+            const uint32_t new_hi = n < 32 ? lo + min((uint32_t)n * gap, hi - lo) : hi;
+            lo = n > 0 ? min(lo + min((uint32_t)(n - 1) * gap, hi - lo) + 1, new_hi) : lo;
+            hi = new_hi;
+          } else {  // the greatest key with b >= bin lies in [probe n-1, probe n)
+            const uint32_t new_lo = n > 0 ? lo + min((uint32_t)(n - 1) * gap, hi - lo) : lo;
+            hi = n < 32 ? max(lo + min((uint32_t)n * gap, hi - lo), new_lo + 1) - 1 : hi;
+            lo = new_lo;
+          }
+        }
+        if (lane == 0) s->edge[warp] = lo;
+      }
+      __syncthreads();
+      lo_key = s->edge[0];
+      hi_key = s->edge[1];
+      first = false;
+    } else {
+      const uint32_t top_bits = (hi_key >> shift) - (uint32_t)bin;
+      const uint32_t lo = top_bits << shift, hi = lo + ((1u << shift) - 1);
+      lo_key = max(lo_key, lo);
+      hi_key = min(hi_key, hi);
+    }
+    constexpr int grain = KeyGrain<T>::kBits;
+    if ((lo_key >> grain) == (hi_key >> grain)) break;
+    shift = grain;
+    while ((hi_key >> shift) - (lo_key >> shift) >= kSaBins) ++shift;
+  }
+  // the group's one value: a positive number's key ends in zeros, a negative one's in ones
+  constexpr uint32_t low = (1u << KeyGrain<T>::kBits) - 1;
+  const uint32_t key = hi_key & 0x80000000u ? hi_key & ~low : hi_key | low;
+  Cut cut = {key, 0, false};
+  if constexpr (kMass) {
+    const double w = (double)weight(row, s->tab, of_key(key));
+    const int64_t group = (int64_t)(held / (uint64_t)w);
+    int64_t r = (int64_t)ceil((target - (double)above) / w);
+    r = max((int64_t)1, min(r, group));
+    while (r > 1 && (double)(above + (uint64_t)(r - 1) * (uint64_t)w) >= target) --r;
+    while (r < group && (double)(above + (uint64_t)r * (uint64_t)w) < target) ++r;
+    cut.ties = r;
+    cut.all_ties = r >= group;
+  } else {
+    cut.ties = want - (int64_t)above;
+    cut.all_ties = cut.ties >= (int64_t)held;
+  }
+  if (tid == 0) s->held = held;
+  __syncthreads();
+  return cut;
+}
+
+__device__ __forceinline__ Cut tighter(const Cut& a, const Cut& b) {
+  if (a.key != b.key) return a.key > b.key ? a : b;
+  if (a.all_ties || b.all_ties) return a.all_ties ? b : a;
+  return a.ties < b.ties ? a : b;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kSaThreads) sample_kernel(const SampleArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  SaShared* s = reinterpret_cast<SaShared*>(smem);
+  T* x = reinterpret_cast<T*>(smem + (sizeof(SaShared) + 15) / 16 * 16);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int row_id = blockIdx.x / ctas;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int slice = a.chunk * kSaWarps, base = rank * slice;
+  const int here = max(0, min(slice, a.vocab - base));  // tokens of this CTA
+  const int steps = a.chunk / kSaStep, chunk_base = warp * a.chunk;
+  for (int i = tid; i < 2 * kSaBins * 3; i += kSaThreads) (&s->hist[0][0][0])[i] = 0;
+  if (tid < 32) s->tab[tid] = exp2(tid / 32.0);
+  grid_dep_wait();
+  grid_dep_launch();
+  // The slice into shared memory: 16 bytes at a time from the first aligned token on (rows of an odd
+  // vocabulary begin anywhere), -inf past its end.
+  {
+    const T* g = static_cast<const T*>(a.x) + row_id * a.stride + base;
+    constexpr int kVec = 16 / (int)sizeof(T);
+    const int off = (int)((reinterpret_cast<uintptr_t>(g) & 15) / sizeof(T));
+    const int head = min(here, off == 0 ? 0 : kVec - off), vecs = (here - head) / kVec;
+    const uint4* gv = reinterpret_cast<const uint4*>(g + head);
+    constexpr int kBatch = 8;
+    for (int i0 = tid; i0 < vecs; i0 += kSaThreads * kBatch) {
+      uint4 v[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (i0 + j * kSaThreads < vecs) v[j] = __ldg(gv + i0 + j * kSaThreads);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = i0 + j * kSaThreads;
+        if (i >= vecs) break;
+        if (head == 0) {
+          *reinterpret_cast<uint4*>(x + i * kVec) = v[j];
+        } else {
+          const T* t = reinterpret_cast<const T*>(&v[j]);
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) x[head + i * kVec + e] = t[e];
+        }
+      }
+    }
+    for (int i = tid; i < head; i += kSaThreads) x[i] = g[i];
+    for (int i = head + vecs * kVec + tid; i < here; i += kSaThreads) x[i] = g[i];
+    for (int i = here + tid; i < slice; i += kSaThreads) x[i] = (T)(-INFINITY);
+  }
+  __syncthreads();
+
+  // the row's greatest and least logits, and whether one is NaN or +inf
+  float top = -INFINITY, least = INFINITY;
+  bool bad = false;
+#pragma unroll 1
+  for (int st = 0; st < steps; ++st) {
+    float v[8];
+    load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      bad |= !(v[i] < INFINITY);
+      top = fmaxf(top, v[i]);
+      least = fminf(least, v[i] == -INFINITY ? INFINITY : v[i]);
+    }
+  }
+  float low = top == -INFINITY ? INFINITY : top;  // least of the threads' greatest
+  const int threads = __syncthreads_count(top > -INFINITY);
+  const int any_bad = __syncthreads_or(bad);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, off));
+    least = fminf(least, __shfl_xor_sync(0xffffffffu, least, off));
+  }
+  if (lane == 0) {
+    s->w_top[warp] = top;
+    s->w_low[warp] = low;
+    s->w_least[warp] = least;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < kSaWarps; ++w) {
+      top = fmaxf(top, s->w_top[w]);
+      low = fminf(low, s->w_low[w]);
+      least = fminf(least, s->w_least[w]);
+    }
+    s->part.top = top;
+    s->part.low = low;
+    s->part.least = least;
+    s->part.threads = threads;
+    s->part.bad = any_bad;
+  }
+  cluster.sync();
+  int with = 0, broken = 0;
+  top = -INFINITY;
+  low = least = INFINITY;
+  for (int r = 0; r < ctas; ++r) {
+    const SaPart* p = cluster.map_shared_rank(&s->part, r);
+    top = fmaxf(top, p->top);
+    low = fminf(low, p->low);
+    least = fminf(least, p->least);
+    with += p->threads;
+    broken |= p->bad;
+  }
+
+  const float temp = a.temperature ? a.temperature[row_id] : a.temperature1;
+  const int64_t k = a.top_k ? a.top_k[row_id] : a.top_k1;
+  const float top_p = a.top_p ? a.top_p[row_id] : a.top_p1;
+  const float min_p = a.min_p ? a.min_p[row_id] : a.min_p1;
+  const float u = a.u[row_id];
+  int level = 0;
+  if (broken || top == -INFINITY) {
+    if (rank == 0 && tid == 0) a.out[row_id] = -1;
+  } else if (!(temp > 0.f)) {
+    // the first of the greatest
+    int at = INT_MAX;
+#pragma unroll 1
+    for (int st = 0; st < steps && at == INT_MAX; ++st) {
+      float v[8];
+      load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
+#pragma unroll
+      for (int i = 7; i >= 0; --i)
+        if (v[i] == top) at = base + chunk_base + st * kSaStep + lane * 8 + i;
+      at = __reduce_min_sync(0xffffffffu, at);
+    }
+    if (lane == 0) s->w_ties[warp] = at;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 0; w < kSaWarps; ++w) at = min(at, s->w_ties[w]);
+      s->part.index = at;
+    }
+    cluster.sync();
+    if (rank == 0 && tid == 0) {
+      for (int r = 0; r < ctas; ++r) at = min(at, cluster.map_shared_rank(&s->part, r)->index);
+      a.out[row_id] = at;
+    }
+  } else {
+    Row row;
+    row.top = top;
+    row.m = (double)top;
+    row.c32 = 46.166241308446829 / (double)temp;  // 32 * log2(e)
+    // 2^-46 and less rounds to no unit
+    row.floor_x = fmaxf((float)((double)top - 32.3 * (double)temp), -FLT_MAX);
+    // what min-p keeps, x - M >= T * log(min_p) (exp(x - M) would round to 1 near M): the least float
+    // that passes, found beside its estimate
+    Cut cut = {0u, 0, true};
+    if (min_p > 0.f) {
+      if (warp == 0) {
+        const double least_d = (double)temp * log((double)min_p);
+        const uint32_t mid = key_of((float)fmax((double)top + least_d, -(double)FLT_MAX));
+        const uint32_t probe = min(mid - 16 + lane, key_of(top));
+        const bool in = (double)of_key(probe) - row.m >= least_d || probe == key_of(top);
+        const uint32_t hit = __ballot_sync(0xffffffffu, in);
+        const uint32_t found = __shfl_sync(0xffffffffu, probe, max(__ffs((int)hit) - 1, 0));
+        if (lane == 0) s->min_key = hit ? found : key_of(top);
+      }
+      __syncthreads();
+      cut.key = s->min_key;
+    }
+    uint64_t drop = 0;
+    if (k > 0 && k < a.vocab) {
+      // as many threads as `with` have a logit of at least `low`
+      const float from = k <= with ? low : least;
+      const Cut c = search<T, false>(cluster, s, x, steps, chunk_base, row, key_of(from), k, 0.0, 0,
+                                     level);
+      if (c.key != 0 && !c.all_ties) {
+        const float value = of_key(c.key);
+        if (value >= row.floor_x)
+          drop = (s->held - (uint64_t)c.ties) * weight(row, s->tab, value);
+      }
+      __syncthreads();
+      const Cut before = cut;
+      cut = c;
+      if (top_p < 1.f) {
+        const Cut p = search<T, true>(cluster, s, x, steps, chunk_base, row,
+                                      max(c.key, key_of(row.floor_x)), 0, (double)top_p, drop, level);
+        cut = tighter(cut, p);
+      }
+      cut = tighter(before, cut);
+    } else if (top_p < 1.f) {
+      const Cut p = search<T, true>(cluster, s, x, steps, chunk_base, row,
+                                    max(key_of(least), key_of(row.floor_x)), 0, (double)top_p, 0, level);
+      cut = tighter(cut, p);
+    }
+
+    // ties before this warp's tokens, where only some of them stay
+    int64_t rank_of_tie = 0;
+    if (!cut.all_ties) {
+      int n = 0;
+#pragma unroll 1
+      for (int st = 0; st < steps; ++st) {
+        float v[8];
+        load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n += key_of(v[i]) == cut.key;
+      }
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (lane == 0) s->w_ties[warp] = n;
+      __syncthreads();
+      if (tid == 0) {
+        int t = 0;
+        for (int w = 0; w < kSaWarps; ++w) t += s->w_ties[w];
+        s->part.ties = t;
+      }
+      cluster.sync();
+      for (int r = 0; r < rank; ++r) rank_of_tie += cluster.map_shared_rank(&s->part, r)->ties;
+      for (int w = 0; w < warp; ++w) rank_of_tie += s->w_ties[w];
+    }
+    // kept weights of 8 tokens; `tie` counts the ties before this lane's
+    auto kept = [&](const float* v, int64_t tie, uint64_t* w) {
+      uint64_t sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t key = key_of(v[i]);
+        bool in = v[i] >= row.floor_x && key >= cut.key;
+        if (!cut.all_ties && key == cut.key) in = in && tie++ < cut.ties;
+        w[i] = in ? weight(row, s->tab, v[i]) : 0;
+        sum += w[i];
+      }
+      return sum;
+    };
+    // ties in the lanes before this one, and in the warp
+    auto ties_before = [&](const float* v, int& all) {
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) n += key_of(v[i]) == cut.key;
+      int inc = n;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, inc, off);
+        if (lane >= off) inc += o;
+      }
+      all = __shfl_sync(0xffffffffu, inc, 31);
+      return inc - n;
+    };
+    const int64_t first_tie = rank_of_tie;
+#pragma unroll 1
+    for (int st = 0; st < steps; ++st) {
+      float v[8];
+      uint64_t w[8];
+      load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
+      int all = 0;
+      const int64_t tie = rank_of_tie + (cut.all_ties ? 0 : ties_before(v, all));
+      const uint64_t sum = warp_sum(kept(v, tie, w));
+      rank_of_tie += all;
+      if (lane == 0) s->step_mass[warp * steps + st] = sum;
+    }
+    __syncthreads();
+    const int cells = kSaWarps * steps;
+    uint64_t all;
+    const uint64_t cell = tid < cells ? s->step_mass[tid] : 0;
+    const uint64_t before = block_exclusive(cell, s->scan, all);
+    if (tid == 0) s->part.mass = all;
+    cluster.sync();
+    uint64_t mass = 0, ahead = 0;
+    int last = 0;  // the last CTA with a kept token
+    for (int r = 0; r < ctas; ++r) {
+      const uint64_t m = cluster.map_shared_rank(&s->part, r)->mass;
+      if (r < rank) ahead += m;
+      if (m > 0) last = r;
+      mass += m;
+    }
+    // the first cell whose running sum passes the target; the last kept one where none does (u = 1, NaN)
+    const double target = (double)u * (double)mass;
+    const bool none = !((double)mass > target);
+    if (tid == 0) s->bin = -1;
+    __syncthreads();
+    if (cell > 0) {
+      const bool hit = (double)(ahead + before + cell) > target && !((double)(ahead + before) > target);
+      const bool first_cell = ahead + before == 0 && (double)0 > target;  // (u below 0)
+      if (none ? rank == last && before + cell == all : hit || first_cell) {
+        s->bin = tid;
+        s->above = ahead + before;
+      }
+    }
+    __syncthreads();
+    if (s->bin >= 0 && warp == s->bin / steps) {
+      const int st = s->bin % steps;
+      float v[8];
+      uint64_t w[8];
+      int64_t tie = first_tie;
+      if (!cut.all_ties) {
+        int in_warp = 0;
+        for (int i = 0; i <= st; ++i) {
+          load8<T>(x + chunk_base + i * kSaStep + lane * 8, v);
+          const int lanes = ties_before(v, in_warp);
+          tie += i < st ? in_warp : lanes;
+        }
+      }
+      load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
+      const uint64_t sum = kept(v, tie, w);
+      uint64_t inc = sum;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const uint64_t o = __shfl_up_sync(0xffffffffu, inc, off);
+        if (lane >= off) inc += o;
+      }
+      uint64_t run = s->above + inc - sum;
+      int at = none ? -1 : INT_MAX;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        run += w[i];
+        const int id = base + chunk_base + st * kSaStep + lane * 8 + i;
+        if (w[i] > 0) {
+          if (none) at = max(at, id);
+          else if ((double)run > target) at = min(at, id);
+        }
+      }
+      at = none ? __reduce_max_sync(0xffffffffu, at) : __reduce_min_sync(0xffffffffu, at);
+      if (lane == 0) a.out[row_id] = at;
+    }
+  }
+  cluster.sync();  // (no CTA leaves while another may read its shared memory)
+}
+
+template <typename T>
+static int launch_sample(const SampleArgs& a, int64_t rows, int ctas, cudaStream_t st) {
+  const size_t smem =
+      (sizeof(SaShared) + 15) / 16 * 16 + (size_t)a.chunk * kSaWarps * sizeof(T);
+  static DeviceOnce once;
+  cudaError_t e = once.run([] {
+    return cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)((sizeof(SaShared) + 15) / 16 * 16) +
+                                    kSaWarps * kSaSteps * kSaStep * (int)sizeof(T));
+  });
+  if (e != cudaSuccess) return cuda_fail(e, "fi_sample_tokens: kernel set-up");
+  e = launch_pdl_cluster(sample_kernel<T>, dim3((unsigned)(rows * ctas)), dim3(kSaThreads), smem, st,
+                         (unsigned)ctas, a);
+  return e == cudaSuccess ? FI_OK : cuda_fail(e, "fi_sample_tokens launch");
+}
+
+}  // namespace fi
+
+extern "C" int fi_sample_tokens(const void* logits, const float* u, const float* temperature,
+                                const int32_t* top_k, const float* top_p, const float* min_p,
+                                float temperature_scalar, int64_t top_k_scalar, float top_p_scalar,
+                                float min_p_scalar, int32_t* out, int64_t rows, int64_t vocab,
+                                int64_t row_stride, int64_t dtype, void* stream) {
+  using namespace fi;
+  clear_error();
+  if (rows < 0 || vocab <= 0) return fail(FI_ERR_INVALID_ARG, "fi_sample_tokens: bad sizes");
+  if (dtype != FI_DTYPE_F16 && dtype != FI_DTYPE_BF16 && dtype != FI_DTYPE_F32)
+    return fail(FI_ERR_INVALID_ARG, "fi_sample_tokens: unknown dtype %lld", (long long)dtype);
+  if (vocab > kSaMaxVocab || rows > (1 << 24))
+    return fail(FI_ERR_UNSUPPORTED, "fi_sample_tokens: at most %lld tokens a row and %d rows",
+                (long long)kSaMaxVocab, 1 << 24);
+  if (rows == 0) return FI_OK;
+  if (!logits || !u || !out)
+    return fail(FI_ERR_INVALID_ARG, "fi_sample_tokens: null pointer argument");
+  const int size = dtype == FI_DTYPE_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(logits) % size != 0)
+    return fail(FI_ERR_ALIGNMENT, "fi_sample_tokens: logits not aligned to their type");
+  // as few CTAs a row as its tokens allow, more where there are too few rows for two CTAs an SM
+  int ctas = 1;
+  while (ctas < kSaMaxCluster && ((int64_t)ctas * kSaWarps * kSaSteps * kSaStep < vocab ||
+                                  (rows * ctas < 2 * sm_count() &&
+                                   (int64_t)ctas * kSaWarps * kSaStep < vocab)))
+    ctas *= 2;
+  const int64_t per_warp = (vocab + ctas * kSaWarps - 1) / (ctas * kSaWarps);
+  SampleArgs a = {};
+  a.x = logits;
+  a.stride = row_stride;
+  a.u = u;
+  a.temperature = temperature;
+  a.top_k = top_k;
+  a.top_p = top_p;
+  a.min_p = min_p;
+  a.temperature1 = temperature_scalar;
+  a.top_k1 = top_k_scalar > vocab ? (int)vocab : (int)(top_k_scalar < 0 ? 0 : top_k_scalar);
+  a.top_p1 = top_p_scalar;
+  a.min_p1 = min_p_scalar;
+  a.out = out;
+  a.vocab = (int)vocab;
+  a.chunk = (int)((per_warp + kSaStep - 1) / kSaStep * kSaStep);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == FI_DTYPE_F32) return launch_sample<float>(a, rows, ctas, st);
+  return dtype == FI_DTYPE_F16 ? launch_sample<__half>(a, rows, ctas, st)
+                               : launch_sample<__nv_bfloat16>(a, rows, ctas, st);
+}

@@ -244,6 +244,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
 
 _DTYPES = {torch.float16: _lib.FI_DTYPE_F16, torch.bfloat16: _lib.FI_DTYPE_BF16}
+# Codes of an 8-bit cache, and every type of a page pool.
+CODE_DTYPES = {torch.int8: _lib.FI_DTYPE_I8, torch.float8_e4m3fn: _lib.FI_DTYPE_E4M3}
+POOL_DTYPES = {**_DTYPES, **CODE_DTYPES}
 
 
 def _int32_on(name: str, t: torch.Tensor, device: torch.device, count: int) -> torch.Tensor:
@@ -274,6 +277,52 @@ def _check_cache(name: str, t: torch.Tensor, like: torch.Tensor, shape) -> None:
     if not _tma_ready(t):
         raise ValueError(f"{name} needs a 16-byte aligned base, unit innermost stride and "
                          "other strides that are multiples of 8")
+
+
+@functools.lru_cache(maxsize=4096)
+def _code_strides(shape, strides) -> bool:
+    return strides[-1] == 1 and all(st % 16 == 0 or n == 1 for n, st in zip(shape[:-1], strides))
+
+
+def _check_codes(name: str, t: torch.Tensor, like: torch.Tensor, shape, dtype) -> None:
+    """Like ``_check_cache`` for a pool of 8-bit codes."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype != dtype:
+        raise TypeError(f"k_cache and v_cache must have the same type, got {dtype} and {t.dtype}")
+    if t.device != like.device:
+        raise ValueError("all tensors must be on the same device")
+    if t.shape != shape or not _cache_shape(shape):
+        raise ValueError(f"{name} must be [num_blocks, {BLOCK_SIZE}, num_kv_heads, {HEAD_DIM}]")
+    if t.data_ptr() % 16 != 0 or not _code_strides(t.shape, t.stride()):
+        raise ValueError(f"{name} needs a 16-byte aligned base, unit innermost stride and "
+                         "other strides that are multiples of 16")
+
+
+def _check_scales(pool: torch.Tensor, k_scale, v_scale, shape) -> None:
+    """The scales that go with a pool: fp32 of this shape for codes, none for 16-bit values."""
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if pool.dtype not in CODE_DTYPES:
+            if t is not None:
+                raise ValueError(f"{name} goes with an int8 or float8_e4m3fn cache only")
+        elif (not isinstance(t, torch.Tensor) or t.dtype != torch.float32
+              or t.device != pool.device or t.shape != shape):
+            raise ValueError(f"{name} must be a float32 tensor {list(shape)} on the cache's device "
+                             "([..., num_blocks, num_kv_heads, 64])")
+
+
+def _check_pages(k_cache, v_cache, k_scale, v_scale, like) -> tuple:
+    """Checks of one layer's pages, 16-bit like the rows `like` or codes with scales; their shape."""
+    shape = k_cache.shape if isinstance(k_cache, torch.Tensor) else None
+    if isinstance(k_cache, torch.Tensor) and k_cache.dtype in CODE_DTYPES:
+        for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+            _check_codes(name, t, like, shape, k_cache.dtype)
+    else:
+        _check_cache("k_cache", k_cache, like, shape)
+        _check_cache("v_cache", v_cache, like, shape)
+    if k_scale is not None or v_scale is not None or k_cache.dtype in CODE_DTYPES:
+        _check_scales(k_cache, k_scale, v_scale, (shape[0], shape[2], BLOCK_SIZE))
+    return shape
 
 
 def _check_rows(name: str, t: torch.Tensor) -> None:

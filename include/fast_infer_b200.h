@@ -57,6 +57,12 @@ extern "C" {
 /* ---- element types (the `dtype` argument) -------------------------------- */
 #define FI_DTYPE_F16 0
 #define FI_DTYPE_BF16 1
+/* Codes of an 8-bit cache: a row of 128 (one token, one head) stands for code * scale, with the scale
+ * max|x| / 127 (int8) or max|x| / 448 (e4m3) in fp32; scale pools are [num_blocks, num_kv_heads,
+ * 64]. A row that held NaN or an infinity has the scale NaN. */
+#define FI_DTYPE_I8 2
+#define FI_DTYPE_E4M3 3
+#define FI_DTYPE_F32 4 /* logits */
 
 /* Library version (major*10000 + minor*100 + patch). */
 int fi_version(void);
@@ -353,6 +359,103 @@ int fi_kv_evict(const void* k, const void* v, const int32_t* block_table, const 
                 const int64_t* k_strides, const int64_t* v_strides, const int64_t* ko_strides,
                 const int64_t* vo_strides, const int64_t* bt_strides, const int64_t* bto_strides,
                 int32_t* error_flag, void* stream);
+
+/*
+ * fi_rope_axes_store into a cache of 8-bit codes: k (rotated, from its fp32 values) and v are
+ * quantised row by row as they are written. k_cache, v_cache: [num_blocks, 64, num_kv_heads, 128]
+ * codes of cache_dtype (FI_DTYPE_I8, FI_DTYPE_E4M3; strides in elements, multiples of 16);
+ * k_scale, v_scale: fp32 [num_blocks, num_kv_heads, 64] (3 strides each). code = 127 * x / max|x|
+ * (448 for e4m3), rounded to the nearest code, ties to even. All else as in fi_rope_axes_store;
+ * dtype: of qkv and q_out.
+ */
+int fi_rope_axes_store8(const void* qkv, void* q_out, void* k_cache, void* v_cache, float* k_scale,
+                        float* v_scale, const float* cos_table, const float* sin_table,
+                        const int32_t* positions, const int32_t* cu_seqlens,
+                        const int32_t* context_lens, const int32_t* block_table,
+                        int64_t total_tokens, int64_t batch, int64_t num_q_heads,
+                        int64_t num_kv_heads, int64_t head_dim, int64_t axes,
+                        const int64_t* sections, int64_t positions_stride, int64_t table_rows,
+                        int64_t table_stride, int64_t num_blocks, int64_t block_size,
+                        int64_t max_blocks_per_seq, const int64_t* qkv_strides,
+                        const int64_t* q_out_strides, const int64_t* kc_strides,
+                        const int64_t* vc_strides, const int64_t* ks_strides,
+                        const int64_t* vs_strides, const int64_t* bt_strides, int64_t dtype,
+                        int64_t cache_dtype, int32_t* error_flag, void* stream);
+
+/*
+ * Read cached tokens back from a cache of 8-bit codes: row t of sequence b (n_b of them, packed by
+ * cu_seqlens) is its cached token context_lens[b] - n_b + t. k_out, v_out: [total_tokens,
+ * num_kv_heads, 128] of `dtype` (3 strides each), code * scale in fp32, rounded once; rows outside
+ * every sequence are left as they were, a row whose slot has no page is zero (FI_DEVERR_BAD_BLOCK).
+ */
+int fi_read_kv8(const void* k_cache, const void* v_cache, const float* k_scale,
+                const float* v_scale, void* k_out, void* v_out, const int32_t* cu_seqlens,
+                const int32_t* context_lens, const int32_t* block_table, int64_t total_tokens,
+                int64_t batch, int64_t num_kv_heads, int64_t head_dim, int64_t num_blocks,
+                int64_t block_size, int64_t max_blocks_per_seq, const int64_t* kc_strides,
+                const int64_t* vc_strides, const int64_t* ks_strides, const int64_t* vs_strides,
+                const int64_t* ko_strides, const int64_t* vo_strides, const int64_t* bt_strides,
+                int64_t dtype, int64_t cache_dtype, int32_t* error_flag, void* stream);
+
+/*
+ * Shape of draft trees. New token i of sequence b (packed by cu_seqlens) is node i of its tree;
+ * parents[i] (int32 [total_tokens], numbers within the sequence) is below i, any other value makes
+ * node i a root. mask: int32 [total_tokens, mask_words]; bit j % 32 of word j / 32 of row i is set
+ * where node j is i or an ancestor fewer than `window` steps up (0: any). depths: int32
+ * [total_tokens], steps to the root. Bits past the mask are dropped (FI_DEVERR_CONTEXT_LEN);
+ * rows outside every sequence are left as they were.
+ */
+int fi_draft_tree(const int32_t* parents, const int32_t* cu_seqlens, int32_t* mask,
+                  int32_t* depths, int64_t total_tokens, int64_t batch, int64_t mask_words,
+                  int64_t window, int32_t* error_flag, void* stream);
+
+/*
+ * Acceptance of drafted tokens: from node 0 of each sequence (always accepted) to the first child
+ * whose token is the one sampled after the node, until there is none. tokens, sampled, parents:
+ * int32 [total_tokens]; path: int32 [total_tokens], entry cu[b] + d the number of the d-th
+ * accepted node, -1 past the last; counts, next_tokens: int32 [batch], how many nodes are accepted
+ * and what was sampled after the last (0 and -1 for a sequence without new tokens).
+ */
+int fi_accept_drafts(const int32_t* tokens, const int32_t* sampled, const int32_t* parents,
+                     const int32_t* cu_seqlens, int32_t* path, int32_t* counts,
+                     int32_t* next_tokens, int64_t total_tokens, int64_t batch,
+                     int32_t* error_flag, void* stream);
+
+/*
+ * Move of the accepted tokens' K and V, all layers, in place: slot past_b + path[d] goes to slot
+ * past_b + d, for 0 < d < counts[b] and past_b = context_lens[b] - n_b (context_lens as in the
+ * attention call before it). k, v: [layers, num_blocks, 64, num_heads, 128] of `dtype` (5 strides
+ * each); with an 8-bit type k_scale, v_scale: fp32 [layers, num_blocks, num_heads, 64] (4 strides
+ * each), which move along. path and counts: from fi_accept_drafts (ascending nodes). A token whose
+ * page is missing is not moved (FI_DEVERR_BAD_BLOCK). Pages must not be shared between sequences.
+ */
+int fi_keep_accepted(void* k, void* v, float* k_scale, float* v_scale,
+                     const int32_t* block_table, const int32_t* cu_seqlens,
+                     const int32_t* context_lens, const int32_t* path, const int32_t* counts,
+                     int64_t layers, int64_t batch, int64_t total_tokens, int64_t num_heads,
+                     int64_t head_dim, int64_t num_blocks, int64_t block_size,
+                     int64_t max_blocks_per_seq, const int64_t* k_strides,
+                     const int64_t* v_strides, const int64_t* ks_strides,
+                     const int64_t* vs_strides, const int64_t* bt_strides, int64_t dtype,
+                     int32_t* error_flag, void* stream);
+
+/*
+ * One token per row of logits, from a given uniform number (the reference takes the greatest logit on
+ * the host). logits: [rows, vocab] of `dtype` (F16, BF16, F32), row_stride elements apart, unit
+ * inner stride; out, u: int32 and fp32 [rows], u in [0, 1). temperature, top_k, top_p, min_p:
+ * per row, or NULL for the scalar. With w_i = exp((x_i - max x) / temperature) and tokens ordered
+ * by x descending, ties by index: top_k keeps the first top_k (0: all); top_p < 1 those of them
+ * before which the mass is below top_p times the mass of them all (the first always stays);
+ * min_p > 0 those with w >= min_p (in [0, 1]). out = the first index whose running sum of kept w is
+ * above u times the sum of all kept w. temperature 0 (or below, or NaN): the first of the greatest
+ * logits. -inf hides a token; a row with NaN or +inf, or without a logit above -inf, gives -1.
+ * At most 262144 tokens a row. Deterministic: the same token on every run.
+ */
+int fi_sample_tokens(const void* logits, const float* u, const float* temperature,
+                     const int32_t* top_k, const float* top_p, const float* min_p,
+                     float temperature_scalar, int64_t top_k_scalar, float top_p_scalar,
+                     float min_p_scalar, int32_t* out, int64_t rows, int64_t vocab,
+                     int64_t row_stride, int64_t dtype, void* stream);
 
 /*
  * RMSNorm: out[r, :] = x[r, :] * rsqrt(mean(x[r, :]^2) + eps) * weight, fp16 in/out,
