@@ -94,4 +94,17 @@ int chunk_kv_map(CUtensorMap* m, CUtensorMapDataType type, const void* kv, const
   return encode_tiled(m, type, 4, kv, dims, sb, box, CU_TENSOR_MAP_SWIZZLE_128B, what);
 }
 
+int chunk_code_map(CUtensorMap* m, const void* codes, const ChunkBatch& p, const int64_t* st,
+                   const char* what) {
+  if (st[3] != 1) return fail(FI_ERR_ALIGNMENT, "%s: innermost stride must be 1", what);
+  const uint64_t dims[4] = {(uint64_t)kChunkTile, (uint64_t)p.hk, (uint64_t)kChunkPage,
+                            (uint64_t)p.num_blocks};
+  uint64_t sb[3] = {(uint64_t)st[2], (uint64_t)st[1], (uint64_t)st[0]};
+  if (p.hk == 1) sb[0] = (uint64_t)kChunkTile;
+  if (p.num_blocks == 1) sb[2] = (uint64_t)kChunkTile;
+  const uint32_t box[4] = {(uint32_t)kChunkTile, 1, (uint32_t)kChunkPage, 1};
+  return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, codes, dims, sb, box,
+                      CU_TENSOR_MAP_SWIZZLE_NONE, what);
+}
+
 }  // namespace fi

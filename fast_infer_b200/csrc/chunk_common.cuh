@@ -36,6 +36,11 @@ struct ChunkBatch {
   int hq, hk, group;
   int num_blocks, max_blocks;
   int tile_tokens;  // tokens of one 128-row tile: 128 / group
+  // Draft trees (null: none): bit i of a token's `words` words says whether it sees new token i of its
+  // sequence; depths are its positions from the first new slot on (null: not needed).
+  const int32_t* tree;
+  const int32_t* depths;
+  int words;
 };
 
 struct ScoreForm {
@@ -80,6 +85,15 @@ __device__ __forceinline__ int chunk_page(const ChunkBatch& p, int b, int keys, 
   if (pg * kChunkPage >= keys) return p.num_blocks;
   const int ph = p.bt[b * p.bts[0] + (int64_t)pg * p.bts[1]];
   return ph < 0 || ph >= p.num_blocks ? p.num_blocks : ph;
+}
+
+// Bits [at, at + 32) of a token's tree mask (bit 0 is the sequence's first new token).
+__device__ __forceinline__ uint32_t tree_bits(const ChunkBatch& p, int token, int at) {
+  const int32_t* row = p.tree + (int64_t)token * p.words;
+  const int w = at >> 5;
+  const uint32_t lo = w >= 0 && w < p.words ? (uint32_t)row[w] : 0u;
+  const uint32_t hi = (at & 31) && w + 1 >= 0 && w + 1 < p.words ? (uint32_t)row[w + 1] : 0u;
+  return __funnelshift_r(lo, hi, at & 31);
 }
 
 // The low n bits of word i of a 128-bit mask.
@@ -249,5 +263,8 @@ int chunk_q_map(CUtensorMap* m, CUtensorMapDataType type, const void* q, const C
 // of the 64 slots of a page.
 int chunk_kv_map(CUtensorMap* m, CUtensorMapDataType type, const void* kv, const ChunkBatch& p,
                  const int64_t* st, const char* what);
+// The same over a pool of 8-bit codes: a box is the 128 codes of the 64 slots of a page, unswizzled.
+int chunk_code_map(CUtensorMap* m, const void* codes, const ChunkBatch& p, const int64_t* st,
+                   const char* what);
 
 }  // namespace fi

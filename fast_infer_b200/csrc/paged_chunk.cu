@@ -38,13 +38,22 @@
 //   -inf, and their V rows are zeroed in shared memory before the product (0 * NaN is NaN).
 #include <float.h>
 
+#include <type_traits>
+
 #include "chunk_common.cuh"
+#include "quant8.cuh"
 
 namespace fi {
 
 constexpr int kCkThreads = 384;
 constexpr int kCkRegsSoftmax = 184;  // 2 x 128 x 184 + 128 x 136 = 384 x 168
 constexpr int kCkRegsOther = 136;
+constexpr int kCkThreadsCodes = 512;  // with 8-bit codes: four more warps that turn codes into tiles
+constexpr int kCkRegsOtherCodes = 72;  // 2 x 128 x 184 + 2 x 128 x 72 = 512 x 128
+constexpr int kCkConvertBar = 14;
+// Scales of a key tile are read after its product is done, that is after its stage may be filled again: the
+// place of tile j is written for tile j + 4 once S of tile j + 2 is complete, which waits for P of tile j + 1.
+constexpr int kCkScaleSlots = 4;
 constexpr int kCkStages = 2;
 constexpr int kCkTeardownBar = 15;
 constexpr int kCkMaxBatch = 2048;    // sequences per launch
@@ -64,7 +73,7 @@ struct alignas(16) CkUnit {
   int b, hk;
   int token, pos;      // first packed row, its position
   int rows[2];         // live rows of the two tiles
-  int keys, prefix;
+  int keys, prefix;    // with a tree, `prefix` is the sequence's first new slot instead
   int np, lo;          // step j is key tile j < np ? j : lo + j - np
   int j0, j1, n;
   int pages_ok;        // no block-table entry of its keys is invalid
@@ -85,6 +94,8 @@ struct CkBarriers {
   uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
   uint64_t mma_done;
   uint64_t unit_full[kCkSlots], unit_empty[kCkSlots];
+  uint64_t kc_full[kCkStages], vc_full[kCkStages];  // codes have arrived
+  alignas(16) float k_scale[kCkScaleSlots][kChunkTile];
   uint64_t merge;  // both softmax warpgroups, in a transposed unit
   uint32_t tmem_base;
   // transposed units, per warpgroup: rows' max, partial maxima / sums, scale, slope, token
@@ -94,7 +105,7 @@ struct CkBarriers {
   int64_t n_off[kCkNarrow];  // where a row's output goes
   CkUnit units[kCkSlots];
   uint8_t row_token[kChunkTile], row_head[kChunkTile];  // of a tile's rows
-  uint32_t warp_sums[kCkThreads / 32];
+  uint32_t warp_sums[kCkThreadsCodes / 32];
   uint32_t unit_off[kCkMaxBatch + 1];  // first unit of each sequence
   uint32_t work[kCkMaxUnits + 1];      // steps before each unit
 };
@@ -121,6 +132,8 @@ struct ChunkParams {
   int split_rows;   // sequences of at most so many rows are the narrow kernel's, others the wide's
   int o_wide;       // rows of o are 32-byte aligned
   int late_wait;    // the kernel before on the stream is the other one of this call
+  const float* scale[2];  // of k and v, with 8-bit codes
+  int64_t ss[2][3];       // page, head, slot
   int* err;
 };
 
@@ -132,8 +145,9 @@ __device__ __forceinline__ int ck_tile(const CkUnit& u, int j) {
 // [lo, lo + n - np). A unit that sees nothing visits one (all of it masked).
 __device__ __forceinline__ void ck_tiles(const ChunkBatch& p, const ChunkSeq& s, int t0, int t1,
                                          int& np, int& lo, int& n) {
-  const int p0 = s.pos0 + t0, p1 = s.pos0 + t1 - 1;
-  const int end = min(s.keys, max(p1 + 1, s.prefix));
+  // (a tree's token may see any new token, and stands at the first new slot or behind it)
+  const int p0 = s.pos0 + (p.tree ? 0 : t0), p1 = s.pos0 + t1 - 1;
+  const int end = p.tree ? s.keys : min(s.keys, max(p1 + 1, s.prefix));
   const int hi = end > 0 ? (end - 1) / kChunkTile : 0;
   lo = p.window ? min(max(p0 - p.window + 1, 0) / kChunkTile, hi) : 0;
   np = min((s.prefix + kChunkTile - 1) / kChunkTile, lo);
@@ -185,7 +199,7 @@ __device__ __forceinline__ void ck_schedule(const ChunkBatch& p, int unit_tokens
       u.token = q.start + t0;
       u.pos = q.pos0 + t0;
       u.keys = q.keys;
-      u.prefix = q.prefix;
+      u.prefix = p.tree ? q.pos0 : q.prefix;
       u.rows[0] = min(t1 - t0, tt) * p.group;
       u.rows[1] = max(t1 - t0 - tt, 0) * p.group;
       u.j0 = max(at - pad, 0);
@@ -380,7 +394,7 @@ __device__ __forceinline__ void zero_v_rows(uint8_t* v, int from, int tid) {
 // A transposed unit, softmax side: warpgroup t takes key tiles j0 + t, j0 + t + 2, ... A thread is
 // one key of the tile (and, for O^T, one dim). `ok` turns false when a wait runs out; a warp that
 // saw it goes on without waiting, so that every barrier here gets all of its threads.
-template <typename T, bool kCap, bool kAlibi>
+template <typename T, bool kCap, bool kAlibi, bool kTree>
 __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* bars, const CkUnit& u,
                                             uint8_t* sP, uint8_t* sV, uint32_t tmem, int t,
                                             int quarter, int lane, int& sc, int& g,
@@ -432,13 +446,27 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
     tc_fence_after();
     // columns [c_lo, c_hi) see this key
     int c_lo = 0, c_hi = rows;
-    if (key >= u.prefix) {
+    uint32_t tree_vis = 0xffffffffu;
+    if constexpr (kTree) {
+      // a new token's key: the bits of the unit's tokens; one before them: by the tokens' depths
+      if (key >= u.prefix || pb.window) {
+        tree_vis = 0;
+#pragma unroll 4
+        for (int i = 0; i * pb.group < rows; ++i) {
+          const bool see = key >= u.prefix
+                               ? (tree_bits(pb, u.token + i, key - u.prefix) & 1u) != 0
+                               : key > u.prefix + pb.depths[u.token + i] - pb.window;
+          if (see) tree_vis |= low_bits((i + 1) * pb.group, 0) & ~low_bits(i * pb.group, 0);
+        }
+      }
+    } else if (key >= u.prefix) {
       c_lo = min(max(key - u.pos, 0), kCkNarrow) * pb.group;
       if (pb.window) c_hi = min(rows, min(max(key + pb.window - u.pos, 0), kCkNarrow) * pb.group);
     }
     if (!page_ok || key >= u.keys) c_hi = 0;
-    const bool mask = !__all_sync(0xffffffffu, c_lo <= 0 && c_hi >= rows);
-    const uint32_t vis = low_bits(c_hi, 0) & ~low_bits(c_lo, 0);
+    const uint32_t vis = low_bits(c_hi, 0) & ~low_bits(c_lo, 0) & tree_vis;
+    const bool mask = !__all_sync(
+        0xffffffffu, kTree ? (vis & low_bits(rows, 0)) == low_bits(rows, 0) : c_lo <= 0 && c_hi >= rows);
     float s[kCkNarrow];  // scores in log2 units, then 2^(score - max)
     // the first tile sets the rows' max; later ones keep it unless some score passes it by 2^8
 #pragma unroll 1
@@ -630,8 +658,121 @@ __device__ __forceinline__ void narrow_unit(const ChunkParams& p, CkBarriers* ba
   g += n;
 }
 
-template <typename T, bool kCap, bool kAlibi, bool kNarrow>
-__global__ void __launch_bounds__(kCkThreads, 1)
+// Scores of one row times the scales of their keys.
+template <int N>
+__device__ __forceinline__ void scale_columns(uint32_t* sr, const float* scale) {
+#pragma unroll
+  for (int c = 0; c < N; c += 4) {
+    const float4 f = *reinterpret_cast<const float4*>(scale + c);
+    sr[c] = __float_as_uint(__uint_as_float(sr[c]) * f.x);
+    sr[c + 1] = __float_as_uint(__uint_as_float(sr[c + 1]) * f.y);
+    sr[c + 2] = __float_as_uint(__uint_as_float(sr[c + 2]) * f.z);
+    sr[c + 3] = __float_as_uint(__uint_as_float(sr[c + 3]) * f.w);
+  }
+}
+
+// 16 codes as 16-bit values of type T: as they are (exact), or times a scale in fp32, rounded once.
+template <typename T, typename Code, bool kScaled>
+__device__ __forceinline__ void spread16(const uint4& raw, float scale, uint32_t* out) {
+  const uint32_t r[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t h[2];
+    Code::decode4(r[i], h[0], h[1]);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if constexpr (!kScaled && std::is_same_v<T, __half>) {
+        out[2 * i + j] = h[j];
+      } else {
+        float2 f = __half22float2(*reinterpret_cast<__half2*>(&h[j]));
+        if (kScaled) f.x *= scale, f.y *= scale;
+        out[2 * i + j] = Half16<T>::pack(f.x, f.y);
+      }
+    }
+  }
+}
+
+// Four warps between TMA and the tensor core: the codes of a tile (128 keys x 128 bytes) lie in the first
+// half of its 16-bit place; all of them are read into registers, and then written as the swizzled tile of
+// two 64-value columns. K keeps its codes, which are exact, and its scales go to the softmax warps: scores
+// are scaled in fp32, as lse is an output. V is scaled here and rounded to T, half a step (fp16 2^-12 to
+// 2^-11) beside the one of P. Rows of keys past the context, or without a page, are zero.
+template <typename T, typename Code>
+__device__ __forceinline__ void code_tiles(const ChunkParams& p, CkBarriers* bars, uint8_t* sK,
+                                           uint8_t* sV) {
+  const ChunkBatch& pb = p.b;
+  const int tid = threadIdx.x & 127, lane = tid & 31;
+  const int piece = tid & 7, row0 = tid >> 3;  // rows row0, row0 + 16, ...
+  // two 16-byte chunks of a row's column, in an order that keeps the 8 lanes of a row off each
+  // other's banks (the two columns' chunks share them)
+  const int column = piece >> 2, chunk = (piece & 3) * 2;
+  int g = 0, next_unit = 0;
+  bool ok = true;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.err));
+  };
+#pragma unroll 1
+  for (const CkUnit* up; (up = ck_next<true>(bars, next_unit, p.err)) != nullptr;
+       ck_done<true>(bars, next_unit)) {
+    const CkUnit& u = *up;
+#pragma unroll 1
+    for (int j = u.j0; j < u.j1; ++j, ++g) {
+      const int s = g % kCkStages, tile = ck_tile(u, j);
+      const uint32_t par = (g / kCkStages) & 1;
+      int page[2];
+      for (int i = 0; i < 2; ++i) page[i] = chunk_page(pb, u.b, u.keys, tile, i);
+#pragma unroll 1
+      for (int kv = 0; kv < 2; ++kv) {
+        float scale[8];
+        bool held[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = row0 + 16 * i, pg = page[i >> 2];
+          held[i] = pg != pb.num_blocks && tile * kChunkTile + r < u.keys;
+          scale[i] = held[i] ? p.scale[kv][pg * p.ss[kv][0] + u.hk * p.ss[kv][1] +
+                                           (r & (kChunkPage - 1)) * p.ss[kv][2]]
+                             : 0.f;
+        }
+        uint8_t* dst = (kv ? sV : sK) + s * kChunkTileBytes;
+        wait(kv ? &bars->vc_full[s] : &bars->kc_full[s], par);
+        uint4 raw[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          raw[i] = *reinterpret_cast<const uint4*>(dst + (row0 + 16 * i) * 128 + piece * 16);
+          if (!held[i]) raw[i] = make_uint4(0, 0, 0, 0);
+        }
+        __syncwarp();
+        named_bar_sync(kCkConvertBar, 128);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = row0 + 16 * i;
+          uint32_t v[8];
+          if (kv) spread16<T, Code, true>(raw[i], scale[i], v);
+          else spread16<T, Code, false>(raw[i], 1.f, v);
+          uint8_t* col = dst + column * kChunkHalf + r * 128;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int which = h ^ column;
+            const uint4 w = which ? make_uint4(v[4], v[5], v[6], v[7])
+                                  : make_uint4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<uint4*>(col + (((chunk + which) ^ (r & 7)) << 4)) = w;
+          }
+          if (kv == 0 && piece == 0) bars->k_scale[g % kCkScaleSlots][r] = scale[i];
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(kv ? &bars->v_full[s] : &bars->k_full[s]);
+      }
+    }
+  }
+}
+
+template <typename Code>
+constexpr int kCkThreadsOf = std::is_void_v<Code> ? kCkThreads : kCkThreadsCodes;
+
+// Code: the type of 8-bit pages (void: 16-bit pages of type T).
+template <typename T, bool kCap, bool kAlibi, bool kNarrow, bool kTree, typename Code>
+__global__ void __launch_bounds__(kCkThreadsOf<Code>, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q,
                        const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const ChunkParams p) {
@@ -642,6 +783,8 @@ __global__ void __launch_bounds__(kCkThreads, 1)
   uint8_t* sV = sK + kCkStages * kChunkTileBytes;
   CkBarriers* bars = reinterpret_cast<CkBarriers*>(sV + kCkStages * kChunkTileBytes);
 
+  constexpr bool kCode = !std::is_void_v<Code>;
+  constexpr int kThreads = kCkThreadsOf<Code>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = blockIdx.x;
 
@@ -659,16 +802,18 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       mbar_init(&bars->o_empty[t], 4);
     }
     for (int s = 0; s < kCkStages; ++s) {
-      mbar_init(&bars->k_full[s], 1);
+      mbar_init(&bars->k_full[s], kCode ? 4 : 1);
       mbar_init(&bars->k_empty[s], 1);
-      mbar_init(&bars->v_full[s], 1);
+      mbar_init(&bars->v_full[s], kCode ? 4 : 1);
       mbar_init(&bars->v_empty[s], 1);
+      mbar_init(&bars->kc_full[s], 1);
+      mbar_init(&bars->vc_full[s], 1);
     }
     mbar_init(&bars->mma_done, 1);
     mbar_init(&bars->merge, 8);
     for (int s = 0; s < kCkSlots; ++s) {
       mbar_init(&bars->unit_full[s], 1);
-      mbar_init(&bars->unit_empty[s], 10);  // TMA, UMMA, the 8 softmax warps
+      mbar_init(&bars->unit_empty[s], kCode ? 14 : 10);  // TMA, UMMA, the 8 softmax (and 4 code) warps
     }
     fence_barrier_init();
   }
@@ -685,7 +830,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
   constexpr int kPad = kNarrow ? kCkPadNarrow : kCkPadWide;
   bool single = true;  // at most one unit in each of this thread's sequences
 #pragma unroll 1
-  for (int b = threadIdx.x; b < pb.batch; b += kCkThreads) {
+  for (int b = threadIdx.x; b < pb.batch; b += kThreads) {
     const ChunkSeq q = chunk_seq(pb, b);
     if (q.bad && cta == 0) set_error(p.err, FI_DEVERR_CONTEXT_LEN);
     const bool here = (q.n * pb.group <= p.split_rows) == kNarrow;
@@ -701,7 +846,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
   uint32_t units;
   if (__syncthreads_and(single)) {  // unit b is sequence b
     units = (uint32_t)pb.batch;
-    for (int b = threadIdx.x; b < pb.batch; b += kCkThreads) bars->unit_off[b + 1] = b + 1;
+    for (int b = threadIdx.x; b < pb.batch; b += kThreads) bars->unit_off[b + 1] = b + 1;
   } else {
     block_scan(bars->unit_off, pb.batch, bars->warp_sums);
     // cu that is not ascending could name more units than the host counted: those are dropped
@@ -709,7 +854,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
     if (units != bars->unit_off[pb.batch] && threadIdx.x == 0)
       set_error(p.err, FI_DEVERR_CONTEXT_LEN);
 #pragma unroll 1
-    for (int e = threadIdx.x; e < (int)units; e += kCkThreads) {
+    for (int e = threadIdx.x; e < (int)units; e += kThreads) {
       const int b = last_le(bars->unit_off, pb.batch, (uint32_t)e);
       const ChunkSeq q = chunk_seq(pb, b);
       const int t0 = (e - (int)bars->unit_off[b]) * p.unit_tokens;
@@ -726,7 +871,8 @@ __global__ void __launch_bounds__(kCkThreads, 1)
   const uint32_t tmem = bars->tmem_base;
 
   if (warp >= 8) {
-    if constexpr (!kNarrow) setmaxnreg_dec<kCkRegsOther>();
+    if constexpr (kCode) setmaxnreg_dec<kCkRegsOtherCodes>();
+    else if constexpr (!kNarrow) setmaxnreg_dec<kCkRegsOther>();
     if (warp == 8 && lane == 0) {
       // ---------------------------------------------------------- TMA producer
       prefetch_tmap(&tm_q);
@@ -768,21 +914,33 @@ __global__ void __launch_bounds__(kCkThreads, 1)
               set_error(p.err, FI_DEVERR_BAD_BLOCK);
           if (g >= kCkStages && !(ok = mbar_wait(&bars->k_empty[s], par, p.err))) break;
           uint8_t* dk = sK + s * kChunkTileBytes;
+          if constexpr (kCode) {  // codes into the tile's first half; the code warps spread them out
+            mbar_arrive_expect_tx(&bars->kc_full[s], kChunkHalf);
+            for (int i = 0; i < 2; ++i)
+              tma_load_4d(dk + i * kChunkHalf / 2, &tm_k, &bars->kc_full[s], 0, u.hk, 0, ph[i]);
+          } else {
           mbar_arrive_expect_tx(&bars->k_full[s], kChunkTileBytes);
           for (int i = 0; i < 2; ++i) {
             tma_load_4d(dk + i * kChunkHalf / 2, &tm_k, &bars->k_full[s], 0, u.hk, 0, ph[i]);
             tma_load_4d(dk + kChunkHalf + i * kChunkHalf / 2, &tm_k, &bars->k_full[s], 64, u.hk, 0,
                         ph[i]);
           }
+          }
           if (j == u.j0) load_q();
           if (!ok) break;
           if (g >= kCkStages && !(ok = mbar_wait(&bars->v_empty[s], par, p.err))) break;
           uint8_t* dv = sV + s * kChunkTileBytes;
+          if constexpr (kCode) {
+            mbar_arrive_expect_tx(&bars->vc_full[s], kChunkHalf);
+            for (int i = 0; i < 2; ++i)
+              tma_load_4d(dv + i * kChunkHalf / 2, &tm_v, &bars->vc_full[s], 0, u.hk, 0, ph[i]);
+          } else {
           mbar_arrive_expect_tx(&bars->v_full[s], kChunkTileBytes);
           for (int i = 0; i < 2; ++i) {
             tma_load_4d(dv + i * kChunkHalf / 2, &tm_v, &bars->v_full[s], 0, u.hk, 0, ph[i]);
             tma_load_4d(dv + kChunkHalf + i * kChunkHalf / 2, &tm_v, &bars->v_full[s], 64, u.hk, 0,
                         ph[i]);
+          }
           }
           ph[0] = next[0];
           ph[1] = next[1];
@@ -926,8 +1084,11 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       umma_commit(&bars->mma_done);
       mbar_wait(&bars->mma_done, 0, p.err);
     }
+    if constexpr (kCode) {
+      if (warp >= 12) code_tiles<T, Code>(p, bars, sK, sV);
+    }
     __syncwarp();
-    named_bar_arrive(kCkTeardownBar, kCkThreads);
+    named_bar_arrive(kCkTeardownBar, kThreads);
     return;
   }
 
@@ -958,7 +1119,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       const int rows = t ? u.rows[1] : u.rows[0];
       const bool begins = u.j0 == 0, ends = u.j1 == u.n;
       if constexpr (kNarrow) {
-        narrow_unit<T, kCap, kAlibi>(p, bars, u, sQ + kChunkTileBytes, sV, tmem, t, quarter, lane, sc,
+        narrow_unit<T, kCap, kAlibi, kTree>(p, bars, u, sQ + kChunkTileBytes, sV, tmem, t, quarter, lane, sc,
                                      g, uc, merges, cta, ok);
       } else {
       if (rows == 0) {
@@ -980,7 +1141,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
         const bool page0 = u.pages_ok || chunk_page(pb, u.b, u.keys, tile, 0) != pb.num_blocks;
         const bool page1 = u.pages_ok || chunk_page(pb, u.b, u.keys, tile, 1) != pb.num_blocks;
         wait(&bars->s_full[t], sc & 1);
-        if (t == 0 && k0 + kChunkTile > u.keys) {
+        if (!kCode && t == 0 && k0 + kChunkTile > u.keys) {
           wait(&bars->v_full[g % kCkStages], (g / kCkStages) & 1);
           zero_v_rows(sV + (g % kCkStages) * kChunkTileBytes, max(u.keys - k0, 0), threadIdx.x);
           fence_proxy_async_smem();
@@ -988,8 +1149,16 @@ __global__ void __launch_bounds__(kCkThreads, 1)
         if (warp_live) {
           tc_fence_after();
           // columns [c_lo, c_hi) and [0, c_pre) are visible
-          const int c_hi = min(pos + 1, u.keys) - k0, c_pre = u.prefix - k0;
-          const int c_lo = pb.window ? pos - pb.window + 1 - k0 : 0;
+          int c_hi = min(pos + 1, u.keys) - k0, c_pre = u.prefix - k0;
+          int c_lo = pb.window ? pos - pb.window + 1 - k0 : 0;
+          int c_tree = kChunkTile;  // columns from here on go by the tree's bits
+          if (kTree && pb.tree) {
+            c_tree = u.prefix - k0;
+            c_hi = min(c_tree, u.keys - k0);
+            c_pre = 0;
+            if (pb.window && live)
+              c_lo = u.prefix + pb.depths[u.token + t * pb.tile_tokens + tok] - pb.window + 1 - k0;
+          }
           const bool all = !live || ((c_hi >= kChunkTile && c_lo <= 0) || c_pre >= kChunkTile);
           const bool mask = !__all_sync(0xffffffffu, all && page0 && page1);
           if (kCap || kAlibi || mask) {
@@ -1000,10 +1169,14 @@ __global__ void __launch_bounds__(kCkThreads, 1)
               tmem_ld32(tS + cc, sr);
               tmem_wait_ld();
               reg_fence<32>(sr);
+              if constexpr (kCode) scale_columns<32>(sr, bars->k_scale[g % kCkScaleSlots] + cc);
               score_form<kCap, kAlibi>(sr, p.f, slope2, (float)(k0 + cc - pos), live);
               if (mask) {
                 uint32_t vis = (low_bits(c_hi - cc, 0) & ~low_bits(c_lo - cc, 0)) |
                                low_bits(c_pre - cc, 0);
+                if (kTree && pb.tree && live && cc + 32 > c_tree)
+                  vis |= tree_bits(pb, u.token + t * pb.tile_tokens + tok, cc - c_tree) &
+                         low_bits(u.keys - k0 - cc, 0);
                 if (!(cc < 64 ? page0 : page1)) vis = 0;
 #pragma unroll
                 for (int c = 0; c < 32; ++c)
@@ -1020,6 +1193,9 @@ __global__ void __launch_bounds__(kCkThreads, 1)
           tmem_ld32(tS + 96, sr + 96);
           tmem_wait_ld();
           reg_fence<kChunkTile>(sr);
+          if constexpr (kCode) {
+            if (!(kCap || mask)) scale_columns<kChunkTile>(sr, bars->k_scale[g % kCkScaleSlots]);
+          }
           float mx8[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -1129,7 +1305,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
   if (p.late_wait && threadIdx.x == 0) grid_dep_wait();
   __syncwarp();
   tc_fence_before();
-  named_bar_sync(kCkTeardownBar, kCkThreads);
+  named_bar_sync(kCkTeardownBar, kThreads);
   if (warp == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -1196,43 +1372,66 @@ __global__ void __launch_bounds__(256, 5) chunk_combine_kernel(const ChunkParams
   if (col == 0 && p.lse) p.lse[token * p.b.hq + head] = none ? -INFINITY : (mx + log2f(sum)) * kLn2;
 }
 
-template <typename T, bool kCap, bool kAlibi, bool kNarrow>
+template <typename T, bool kCap, bool kAlibi, bool kNarrow, bool kTree, typename Code>
 static int launch_main(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                        const ChunkParams& p, cudaStream_t st) {
+  constexpr auto kernel = paged_chunk_kernel<T, kCap, kAlibi, kNarrow, kTree, Code>;
   static DeviceOnce once;
   cudaError_t e = once.run([] {
     // the register split must fit what the block is launched with, or setmaxnreg would wait
     cudaFuncAttributes a;
-    const cudaError_t e = cudaFuncGetAttributes(&a, paged_chunk_kernel<T, kCap, kAlibi, kNarrow>);
+    const cudaError_t e = cudaFuncGetAttributes(&a, kernel);
     if (e != cudaSuccess) return e;
-    if (!kNarrow && a.numRegs * kCkThreads < 2 * 128 * kCkRegsSoftmax + 128 * kCkRegsOther)
+    constexpr bool kCode = !std::is_void_v<Code>;
+    const int split = 2 * 128 * kCkRegsSoftmax +
+                      (kCode ? 2 * 128 * kCkRegsOtherCodes : 128 * kCkRegsOther);
+    if ((kCode || !kNarrow) && a.numRegs * kCkThreadsOf<Code> < split)
       return cudaErrorInvalidConfiguration;
-    return cudaFuncSetAttribute(paged_chunk_kernel<T, kCap, kAlibi, kNarrow>,
-                                cudaFuncAttributeMaxDynamicSharedMemorySize, kCkSmemBytes);
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCkSmemBytes);
   });
   if (e != cudaSuccess) return cuda_fail(e, "fi_paged_chunk: kernel set-up");
-  e = launch_pdl(paged_chunk_kernel<T, kCap, kAlibi, kNarrow>, dim3((unsigned)sm_count()),
-                 dim3(kCkThreads), kCkSmemBytes, st, tq, tk, tv, p);
+  e = launch_pdl(kernel, dim3((unsigned)sm_count()), dim3(kCkThreadsOf<Code>), kCkSmemBytes, st, tq,
+                 tk, tv, p);
   return e == cudaSuccess ? FI_OK : cuda_fail(e, "fi_paged_chunk: launch");
 }
 
 template <typename T, bool kNarrow>
 static int launch_form(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                        const ChunkParams& p, cudaStream_t st) {
-  if (p.f.cap_log2 > 0.f)
-    return p.f.slopes ? launch_main<T, true, true, kNarrow>(tq, tk, tv, p, st)
-                      : launch_main<T, true, false, kNarrow>(tq, tk, tv, p, st);
-  return p.f.slopes ? launch_main<T, false, true, kNarrow>(tq, tk, tv, p, st)
-                    : launch_main<T, false, false, kNarrow>(tq, tk, tv, p, st);
+  const bool cap = p.f.cap_log2 > 0.f;
+  if (p.b.tree)  // (without a distance bias)
+    return cap ? launch_main<T, true, false, kNarrow, true, void>(tq, tk, tv, p, st)
+               : launch_main<T, false, false, kNarrow, true, void>(tq, tk, tv, p, st);
+  if (cap)
+    return p.f.slopes ? launch_main<T, true, true, kNarrow, false, void>(tq, tk, tv, p, st)
+                      : launch_main<T, true, false, kNarrow, false, void>(tq, tk, tv, p, st);
+  return p.f.slopes ? launch_main<T, false, true, kNarrow, false, void>(tq, tk, tv, p, st)
+                    : launch_main<T, false, false, kNarrow, false, void>(tq, tk, tv, p, st);
 }
 
-// The narrow kernel, the wide one or both (whichever `narrow` and `wide` name), and the join.
+// The wide kernel over 8-bit pages.
+template <typename T, typename Code>
+static int launch_codes(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                        const ChunkParams& p, cudaStream_t st) {
+  return p.f.cap_log2 > 0.f ? launch_main<T, true, false, false, true, Code>(tq, tk, tv, p, st)
+                            : launch_main<T, false, false, false, true, Code>(tq, tk, tv, p, st);
+}
+
+// The narrow kernel, the wide one or both (whichever `narrow` and `wide` name), and the join. `codes`: the
+// type of the pages, or that of q.
 template <typename T>
 static int launch_chunk(const CUtensorMap& tq_n, const CUtensorMap& tq_w, const CUtensorMap& tk,
                         const CUtensorMap& tv, const ChunkParams* narrow, const ChunkParams* wide,
-                        cudaStream_t st) {
-  int r = narrow ? launch_form<T, true>(tq_n, tk, tv, *narrow, st) : FI_OK;
-  if (r == FI_OK && wide) r = launch_form<T, false>(tq_w, tk, tv, *wide, st);
+                        int64_t codes, cudaStream_t st) {
+  int r = FI_OK;
+  if (codes == FI_DTYPE_I8) {
+    r = launch_codes<T, CodeI8>(tq_w, tk, tv, *wide, st);
+  } else if (codes == FI_DTYPE_E4M3) {
+    r = launch_codes<T, CodeE4M3>(tq_w, tk, tv, *wide, st);
+  } else {
+    if (narrow) r = launch_form<T, true>(tq_n, tk, tv, *narrow, st);
+    if (r == FI_OK && wide) r = launch_form<T, false>(tq_w, tk, tv, *wide, st);
+  }
   if (r != FI_OK) return r;
   const ChunkParams& first = wide ? *wide : *narrow;
   const int parts = (first.rows_cap + (narrow && wide ? narrow->rows_cap : 0)) / kCkJoinRows;
@@ -1274,38 +1473,52 @@ extern "C" size_t fi_paged_chunk_workspace_size(int64_t total_tokens, int64_t nu
   return narrow + ck_workspace(nullptr, nullptr, 2 * kChunkTile);
 }
 
-extern "C" int fi_paged_chunk(const void* q, const void* k_cache, const void* v_cache, void* o,
-                              float* lse, const int32_t* block_table, const int32_t* cu_seqlens,
-                              const int32_t* context_lens, const int32_t* prefix_lens,
-                              const float* alibi_slopes, int64_t batch, int64_t total_tokens,
-                              int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
-                              int64_t num_blocks, int64_t block_size, int64_t max_blocks_per_seq,
-                              const int64_t* q_strides, const int64_t* kc_strides,
-                              const int64_t* vc_strides, const int64_t* o_strides,
-                              const int64_t* bt_strides, float sm_scale, float softcap,
-                              int64_t window, int64_t dtype, void* workspace,
-                              size_t workspace_bytes, int32_t* error_flag, void* stream) {
-  using namespace fi;
+namespace fi {
+
+// What fi_paged_tree has beside fi_paged_chunk's arguments.
+struct ChunkExtra {
+  const int32_t* tree;
+  const int32_t* depths;
+  int64_t words;
+  const float* scale[2];
+  const int64_t* ss[2];
+  int64_t cache_dtype;
+};
+
+static int paged_chunk(const char* what, const void* q, const void* k_cache, const void* v_cache,
+                       void* o, float* lse, const int32_t* block_table, const int32_t* cu_seqlens,
+                       const int32_t* context_lens, const int32_t* prefix_lens,
+                       const float* alibi_slopes, int64_t batch, int64_t total_tokens,
+                       int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                       int64_t num_blocks, int64_t block_size, int64_t max_blocks_per_seq,
+                       const int64_t* q_strides, const int64_t* kc_strides,
+                       const int64_t* vc_strides, const int64_t* o_strides,
+                       const int64_t* bt_strides, float sm_scale, float softcap, int64_t window,
+                       int64_t dtype, const ChunkExtra& extra, void* workspace,
+                       size_t workspace_bytes, int32_t* error_flag, void* stream) {
   clear_error();
-  const char* what = "fi_paged_chunk";
   ChunkParams p = {};
   int r = chunk_batch_args(p.b, what, cu_seqlens, context_lens, prefix_lens, block_table, batch,
                            total_tokens, num_q_heads, num_kv_heads, head_dim, num_blocks,
                            block_size, max_blocks_per_seq, bt_strides, window, dtype);
   if (r != FI_OK) return r;
+  p.b.tree = extra.tree;
+  p.b.depths = extra.depths;
+  p.b.words = (int)extra.words;
   r = chunk_score_args(p.f, what, sm_scale, softcap, alibi_slopes);
   if (r != FI_OK) return r;
   if (batch == 0 || total_tokens == 0) return FI_OK;
   if (!q || !k_cache || !v_cache || !o || !block_table || !cu_seqlens || !context_lens ||
       !q_strides || !kc_strides || !vc_strides || !o_strides || !bt_strides)
-    return fail(FI_ERR_INVALID_ARG, "fi_paged_chunk: null pointer argument");
+    return fail(FI_ERR_INVALID_ARG, "%s: null pointer argument", what);
   // Batches of few tokens per sequence (on average at most kCkNarrow rows) are the narrow
   // kernel's alone: a sequence with more tokens is several units there, which read its keys once
   // each (from L2), unless there are many new tokens: 512 of one sequence over 2000 beside 64
   // single ones over 4000 take 238 us there and 219 in both kernels, but the wide one costs 11 us
   // when it has nothing to do. One sequence with more is the wide kernel's. Other batches may hold
   // both.
-  const int64_t per_unit = p.b.group <= kCkNarrow ? kCkNarrow / p.b.group : 0;
+  const bool codes = extra.cache_dtype != dtype;
+  const int64_t per_unit = !codes && p.b.group <= kCkNarrow ? kCkNarrow / p.b.group : 0;
   const bool use_narrow = per_unit > 0 && (batch > 1 || total_tokens <= per_unit);
   const bool use_wide =
       per_unit == 0 || total_tokens > batch * per_unit || total_tokens - batch >= kCkManyNew;
@@ -1313,33 +1526,41 @@ extern "C" int fi_paged_chunk(const void* q, const void* k_cache, const void* v_
   if (batch > kCkMaxBatch ||
       (total_tokens + unit_tokens - 1) / unit_tokens + batch > kCkMaxUnits)
     return fail(FI_ERR_UNSUPPORTED,
-                "fi_paged_chunk: at most %d sequences and %lld tokens with %d query heads per KV "
+                "%s: at most %d sequences and %lld tokens with %d query heads per KV "
                 "head; split the batch",
-                kCkMaxBatch, (long long)((kCkMaxUnits - batch) * unit_tokens), p.b.group);
+                what, kCkMaxBatch, (long long)((kCkMaxUnits - batch) * unit_tokens), p.b.group);
   if (o_strides[2] != 1 || !aligned16(o) || !stride_ok(total_tokens, o_strides[0]) ||
       !stride_ok(num_q_heads, o_strides[1]))
     return fail(FI_ERR_ALIGNMENT,
-                "fi_paged_chunk o: needs a 16-byte aligned base, unit innermost stride and other "
-                "strides multiple of 8");
+                "%s o: needs a 16-byte aligned base, unit innermost stride and other "
+                "strides multiple of 8",
+                what);
   const size_t need = fi_paged_chunk_workspace_size(total_tokens, num_q_heads, num_kv_heads);
   if (!workspace || workspace_bytes < need)
-    return fail(FI_ERR_WORKSPACE, "fi_paged_chunk: workspace of %zu bytes, needs %zu",
+    return fail(FI_ERR_WORKSPACE, "%s: workspace of %zu bytes, needs %zu", what,
                 workspace ? workspace_bytes : (size_t)0, need);
   if (!aligned16(workspace))
-    return fail(FI_ERR_ALIGNMENT, "fi_paged_chunk: workspace not 16-byte aligned");
+    return fail(FI_ERR_ALIGNMENT, "%s: workspace not 16-byte aligned", what);
   const CUtensorMapDataType type = dtype == FI_DTYPE_F16 ? Half16<__half>::kTmap
                                                          : Half16<__nv_bfloat16>::kTmap;
   ChunkParams n = p;  // the narrow kernel's
   n.b.tile_tokens = per_unit > 0 ? (int)per_unit : 1;
   CUtensorMap tq_n = {}, tq_w = {}, tk, tv;
-  if (use_narrow && (r = chunk_q_map(&tq_n, type, q, n.b, q_strides, "fi_paged_chunk q")) != FI_OK)
+  if (use_narrow && (r = chunk_q_map(&tq_n, type, q, n.b, q_strides, what)) != FI_OK)
     return r;
-  if (use_wide && (r = chunk_q_map(&tq_w, type, q, p.b, q_strides, "fi_paged_chunk q")) != FI_OK)
+  if (use_wide && (r = chunk_q_map(&tq_w, type, q, p.b, q_strides, what)) != FI_OK)
     return r;
-  if ((r = chunk_kv_map(&tk, type, k_cache, p.b, kc_strides, "fi_paged_chunk k_cache")) != FI_OK)
-    return r;
-  if ((r = chunk_kv_map(&tv, type, v_cache, p.b, vc_strides, "fi_paged_chunk v_cache")) != FI_OK)
-    return r;
+  if (codes) {
+    if ((r = chunk_code_map(&tk, k_cache, p.b, kc_strides, what)) != FI_OK) return r;
+    if ((r = chunk_code_map(&tv, v_cache, p.b, vc_strides, what)) != FI_OK) return r;
+    for (int kv = 0; kv < 2; ++kv) {
+      p.scale[kv] = extra.scale[kv];
+      for (int i = 0; i < 3; ++i) p.ss[kv][i] = extra.ss[kv][i];
+    }
+  } else {
+    if ((r = chunk_kv_map(&tk, type, k_cache, p.b, kc_strides, what)) != FI_OK) return r;
+    if ((r = chunk_kv_map(&tv, type, v_cache, p.b, vc_strides, what)) != FI_OK) return r;
+  }
   p.o = o;
   p.os[0] = o_strides[0];
   p.os[1] = o_strides[1];
@@ -1364,6 +1585,79 @@ extern "C" int fi_paged_chunk(const void* q, const void* k_cache, const void* v_
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const ChunkParams* np = use_narrow ? &n : nullptr;
   const ChunkParams* wp = use_wide ? &p : nullptr;
-  return dtype == FI_DTYPE_F16 ? launch_chunk<__half>(tq_n, tq_w, tk, tv, np, wp, st)
-                               : launch_chunk<__nv_bfloat16>(tq_n, tq_w, tk, tv, np, wp, st);
+  return dtype == FI_DTYPE_F16
+             ? launch_chunk<__half>(tq_n, tq_w, tk, tv, np, wp, extra.cache_dtype, st)
+             : launch_chunk<__nv_bfloat16>(tq_n, tq_w, tk, tv, np, wp, extra.cache_dtype, st);
+}
+
+}  // namespace fi
+
+extern "C" int fi_paged_chunk(const void* q, const void* k_cache, const void* v_cache, void* o,
+                              float* lse, const int32_t* block_table, const int32_t* cu_seqlens,
+                              const int32_t* context_lens, const int32_t* prefix_lens,
+                              const float* alibi_slopes, int64_t batch, int64_t total_tokens,
+                              int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                              int64_t num_blocks, int64_t block_size, int64_t max_blocks_per_seq,
+                              const int64_t* q_strides, const int64_t* kc_strides,
+                              const int64_t* vc_strides, const int64_t* o_strides,
+                              const int64_t* bt_strides, float sm_scale, float softcap,
+                              int64_t window, int64_t dtype, void* workspace,
+                              size_t workspace_bytes, int32_t* error_flag, void* stream) {
+  fi::ChunkExtra extra = {};
+  extra.cache_dtype = dtype;
+  return fi::paged_chunk("fi_paged_chunk", q, k_cache, v_cache, o, lse, block_table, cu_seqlens,
+                         context_lens, prefix_lens, alibi_slopes, batch, total_tokens, num_q_heads,
+                         num_kv_heads, head_dim, num_blocks, block_size, max_blocks_per_seq,
+                         q_strides, kc_strides, vc_strides, o_strides, bt_strides, sm_scale,
+                         softcap, window, dtype, extra, workspace, workspace_bytes, error_flag,
+                         stream);
+}
+
+extern "C" size_t fi_paged_tree_workspace_size(int64_t total_tokens, int64_t num_q_heads,
+                                               int64_t num_kv_heads) {
+  return fi_paged_chunk_workspace_size(total_tokens, num_q_heads, num_kv_heads);
+}
+
+extern "C" int fi_paged_tree(const void* q, const void* k_cache, const void* v_cache,
+                             const float* k_scale, const float* v_scale, void* o, float* lse,
+                             const int32_t* block_table, const int32_t* cu_seqlens,
+                             const int32_t* context_lens, const int32_t* tree_mask,
+                             const int32_t* depths, int64_t mask_words, int64_t batch,
+                             int64_t total_tokens, int64_t num_q_heads, int64_t num_kv_heads,
+                             int64_t head_dim, int64_t num_blocks, int64_t block_size,
+                             int64_t max_blocks_per_seq, const int64_t* q_strides,
+                             const int64_t* kc_strides, const int64_t* vc_strides,
+                             const int64_t* ks_strides, const int64_t* vs_strides,
+                             const int64_t* o_strides, const int64_t* bt_strides, float sm_scale,
+                             float softcap, int64_t window, int64_t dtype, int64_t cache_dtype,
+                             void* workspace, size_t workspace_bytes, int32_t* error_flag,
+                             void* stream) {
+  using namespace fi;
+  clear_error();
+  const bool codes = cache_dtype == FI_DTYPE_I8 || cache_dtype == FI_DTYPE_E4M3;
+  if (!codes && cache_dtype != dtype)
+    return fail(FI_ERR_INVALID_ARG, "fi_paged_tree: unknown cache_dtype %lld",
+                (long long)cache_dtype);
+  if (tree_mask && (mask_words <= 0 || mask_words > (1 << 16)))
+    return fail(FI_ERR_INVALID_ARG, "fi_paged_tree: mask_words must be 1 to 65536");
+  if (tree_mask && window > 0 && !depths)
+    return fail(FI_ERR_INVALID_ARG, "fi_paged_tree: a window over a tree needs depths");
+  if (codes && batch > 0 && total_tokens > 0 && (!k_scale || !v_scale || !ks_strides || !vs_strides))
+    return fail(FI_ERR_INVALID_ARG, "fi_paged_tree: 8-bit pages need their scales");
+  ChunkExtra extra = {};
+  extra.tree = tree_mask;
+  extra.depths = depths;
+  extra.words = mask_words;
+  extra.cache_dtype = cache_dtype;
+  if (codes) {
+    extra.scale[0] = k_scale;
+    extra.scale[1] = v_scale;
+    extra.ss[0] = ks_strides;
+    extra.ss[1] = vs_strides;
+  }
+  return paged_chunk("fi_paged_tree", q, k_cache, v_cache, o, lse, block_table, cu_seqlens,
+                     context_lens, nullptr, nullptr, batch, total_tokens, num_q_heads,
+                     num_kv_heads, head_dim, num_blocks, block_size, max_blocks_per_seq, q_strides,
+                     kc_strides, vc_strides, o_strides, bt_strides, sm_scale, softcap, window,
+                     dtype, extra, workspace, workspace_bytes, error_flag, stream);
 }

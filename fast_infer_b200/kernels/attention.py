@@ -14,7 +14,8 @@ Backward-compatible extensions:
 
 Functions without a reference counterpart, for serving long contexts in chunks (fp16 and
 bf16): ``paged_chunk_attention`` (new tokens over the paged cache, with capped scores, a
-distance bias, a window or a prefix) and ``attention_mass`` (the weight each cached token received).
+distance bias, a window or a prefix), ``attention_mass`` (the weight each cached token received) and
+``paged_tree_attention`` (trees of drafted tokens, and caches of 8-bit codes).
 """
 
 from __future__ import annotations
@@ -353,16 +354,19 @@ def _batch_args(device, block_table, block_size, k_cache, cu_seqlens, context_le
 
 
 def _chunk_args(q, k_cache, v_cache, block_table, block_size, cu_seqlens, context_lens, sm_scale,
-                alibi_slopes, prefix_lens):
-    """Checks shared by the functions over packed new tokens and a paged cache; returns the
-    tensors as the library takes them."""
+                alibi_slopes, prefix_lens, scales=None):
+    """Checks shared by the functions over packed new tokens and a paged cache (of 8-bit codes, if the
+    function takes `scales`); returns the tensors as the library takes them."""
     _check_rows("q", q)
     if q.dim() != 3 or q.shape[2] != HEAD_DIM:
         raise ValueError(f"q must be [total_tokens, num_q_heads, {HEAD_DIM}]")
     shape = k_cache.shape if isinstance(k_cache, torch.Tensor) else None
-    _check_cache("k_cache", k_cache, q, shape)
-    if v_cache is not None:
-        _check_cache("v_cache", v_cache, q, shape)
+    if scales is not None:
+        _check_pages(k_cache, v_cache, *scales, q)
+    else:
+        _check_cache("k_cache", k_cache, q, shape)
+        if v_cache is not None:
+            _check_cache("v_cache", v_cache, q, shape)
     if q.shape[1] == 0 or q.shape[1] % shape[2] != 0:
         raise ValueError(f"num_q_heads {q.shape[1]} not a multiple of k/v heads {shape[2]}")
     device = q.device
@@ -462,6 +466,102 @@ def paged_chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
                 stream_of(q.device))
             _lib.check(st, "paged_chunk_attention")
             device_errors(err, "paged_chunk_attention")
+        if ox is not out:
+            out.copy_(ox)
+    return (out, lse) if return_lse else out
+
+
+@functools.lru_cache(maxsize=4096)
+def _tree_workspace(device_index: int, total: int, num_q_heads: int, num_kv_heads: int) -> int:
+    return int(_lib.load().fi_paged_tree_workspace_size(total, num_q_heads, num_kv_heads))
+
+
+def paged_tree_workspace_bytes(total_tokens: int, num_q_heads: int, num_kv_heads: int) -> int:
+    """Workspace bytes ``paged_tree_attention`` needs for these sizes (current device)."""
+    return int(_lib.load().fi_paged_tree_workspace_size(total_tokens, num_q_heads, num_kv_heads))
+
+
+def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         block_table: torch.Tensor, block_size: int, cu_seqlens: torch.Tensor,
+                         context_lens: torch.Tensor, sm_scale: float = None, *,
+                         tree_mask: torch.Tensor = None, depths: torch.Tensor = None,
+                         k_scale: torch.Tensor = None, v_scale: torch.Tensor = None,
+                         softcap: float = 0.0, window: int = 0, return_lse: bool = False,
+                         out: torch.Tensor = None, workspace: torch.Tensor = None):
+    """Attention of trees of drafted tokens over the paged cache that holds them and what came
+    before, 16-bit or of 8-bit codes; without a tree, of single tokens, chains and prompts' chunks.
+
+    q, block_table, cu_seqlens, context_lens, sm_scale, softcap, out, workspace: as in
+    ``paged_chunk_attention`` (new token i of sequence b lies in slot ``context_lens[b] - n_b + i``).
+    k_cache, v_cache: [num_blocks, 64, num_kv_heads, 128] of q's type; or codes, int8 or
+    float8_e4m3fn, with k_scale, v_scale (fp32 [num_blocks, num_kv_heads, 64]), as
+    ``rope_axes_store`` writes them: a row stands for code * scale.
+
+    tree_mask: int32 [total_tokens, words] (``kernels.drafting.draft_tree``): new token i sees new
+    token j of its sequence where bit j % 32 of word j // 32 is set, and every token cached before
+    them. With ``window``, a token of position ``context_lens[b] - n_b + depths[i]`` (depths: int32
+    [total_tokens], from ``draft_tree`` too) sees of those before the new ones only what is less than
+    ``window`` behind it; among the new ones the mask alone decides (give ``draft_tree`` the window).
+    Without tree_mask the new tokens are a chain: ``paged_chunk_attention``, which this equals for
+    16-bit caches.
+
+    A token that sees nothing gives zeros and an lse of -inf. Slots past context_lens[b] may hold
+    anything; V (and its scale) before them has to be finite, seen or not. A key whose score is -inf
+    has weight 0; a NaN or +inf score makes NaN of the rows that see it. Pages with an invalid
+    block-table entry are skipped and lengths that do not fit are cut, which only device checks
+    (``FAST_INFER_B200_CHECK=1``) report, with a RuntimeError.
+
+    Returns o like q (rows outside every sequence are not written), and with ``return_lse`` also lse:
+    fp32 [total_tokens, num_q_heads]. ``workspace``: uint8, at least ``paged_tree_workspace_bytes``.
+    """
+    batch, cu, ctx, _, bt, _, scale = _chunk_args(
+        q, k_cache, v_cache, block_table, block_size, cu_seqlens, context_lens, sm_scale, None, None,
+        (k_scale, v_scale))
+    total, num_q_heads, _ = q.shape
+    num_blocks, _, num_kv_heads, _ = k_cache.shape
+    device = q.device
+    words = 0
+    if tree_mask is not None:
+        if (not isinstance(tree_mask, torch.Tensor) or tree_mask.dim() != 2
+                or tree_mask.dtype != torch.int32 or tree_mask.device != device
+                or tree_mask.shape[0] != total or tree_mask.shape[1] == 0):
+            raise ValueError("tree_mask must be an int32 tensor [total_tokens, words] on q's device")
+        if window and depths is None:
+            raise ValueError("a window over a tree needs depths")
+        tree_mask, words = tree_mask.contiguous(), tree_mask.shape[1]
+    if depths is not None:
+        depths = _int32_on("depths", depths, device, total)
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != device:
+        raise ValueError("out must be shaped and typed like q")
+    lse = torch.empty(total, num_q_heads, dtype=torch.float32, device=device) \
+        if return_lse else None
+    if batch > 0 and total > 0:
+        qx = q if _tma_ready(q) else q.clone(memory_format=torch.contiguous_format)
+        ox = out if _tma_ready(out) else out.clone(memory_format=torch.contiguous_format)
+        lib = _lib.load()
+        with with_device(device):
+            if workspace is None:
+                workspace = torch.empty(
+                    _tree_workspace(device.index, total, num_q_heads, num_kv_heads),
+                    dtype=torch.uint8, device=device)
+            elif workspace.device != device or not workspace.is_contiguous():
+                raise ValueError("workspace must be contiguous on q's device")
+            err = error_word(device)
+            st = lib.fi_paged_tree(
+                qx.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale),
+                ox.data_ptr(), _ptr(lse), bt.data_ptr(), cu.data_ptr(), ctx.data_ptr(),
+                _ptr(tree_mask), _ptr(depths), words, batch, total, num_q_heads, num_kv_heads,
+                HEAD_DIM, num_blocks, block_size, bt.shape[1], _lib.strides(*qx.stride()),
+                _lib.strides(*k_cache.stride()), _lib.strides(*v_cache.stride()),
+                None if k_scale is None else _lib.strides(*k_scale.stride()),
+                None if v_scale is None else _lib.strides(*v_scale.stride()),
+                _lib.strides(*ox.stride()), _lib.strides(*bt.stride()), scale, float(softcap),
+                int(window), _DTYPES[q.dtype], POOL_DTYPES[k_cache.dtype], workspace.data_ptr(),
+                workspace.numel() * workspace.element_size(), _ptr(err), stream_of(device))
+            _lib.check(st, "paged_tree_attention")
+            device_errors(err, "paged_tree_attention")
         if ox is not out:
             out.copy_(ox)
     return (out, lse) if return_lse else out

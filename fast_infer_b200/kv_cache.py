@@ -17,8 +17,10 @@ What changes is how it runs:
 
 Extension: ``num_blocks`` may be given explicitly to size the pool independently
 of ``max_seq_len`` (the reference pool holds ceil(max_seq_len/block_size) blocks
-shared by the whole batch), and ``dtype`` (fp16, or bf16 for the functions that take it).
-``KVCache.extend`` and ``KVCache.evict`` serve ragged batches in chunks over a bounded cache.
+shared by the whole batch), and ``dtype`` (fp16, or bf16 for the functions that take it, or int8
+or float8_e4m3fn codes with the scales ``k_scale`` and ``v_scale`` beside them).
+``KVCache.extend`` and ``KVCache.evict`` serve ragged batches in chunks over a bounded cache,
+``KVCache.accept`` drafted tokens.
 """
 
 from __future__ import annotations
@@ -36,8 +38,9 @@ class KVCache:
     def __init__(self, num_layers: int, num_heads: int, head_dim: int,
                  max_seq_len: int, block_size: int, device: torch.device,
                  num_blocks: int = None, dtype: torch.dtype = torch.float16):
-        if dtype not in (torch.float16, torch.bfloat16):
-            raise TypeError(f"dtype must be float16 or bfloat16, got {dtype}")
+        coded = dtype in (torch.int8, torch.float8_e4m3fn)
+        if not coded and dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"dtype must be float16, bfloat16, int8 or float8_e4m3fn, got {dtype}")
         self.num_layers = num_layers
         self.num_heads = num_heads
         self.head_dim = head_dim
@@ -50,6 +53,12 @@ class KVCache:
                              dtype=dtype, device=self.device)
         self.v = torch.zeros(num_layers, self.num_blocks, block_size, num_heads, head_dim,
                              dtype=dtype, device=self.device)
+        # Scale of every cached row of 8-bit codes (``kernels.rope.rope_axes_store`` writes them).
+        self.k_scale = self.v_scale = None
+        if coded:
+            self.k_scale = torch.zeros(num_layers, self.num_blocks, num_heads, block_size,
+                                       dtype=torch.float32, device=self.device)
+            self.v_scale = torch.zeros_like(self.k_scale)
         self._bt = np.full((1, self.max_blocks_per_seq), -1, np.int32)
         self.block_table = torch.full((1, self.max_blocks_per_seq), -1, dtype=torch.int32,
                                       device=self.device)
@@ -194,14 +203,43 @@ class KVCache:
         mass[..., n:].zero_()
         for b in range(B):
             self.seq_lens[b] = min(int(lens[b]), kept.shape[3])
-            keep = -(-int(self.seq_lens[b]) // self.block_size)
-            row = self._bt[b]
-            freed = [int(x) for x in row[keep:] if x >= 0]
-            if freed:
-                row[keep:] = -1
-                self.free_blocks.extend(freed)
-                self._allocated -= len(freed)
-                self._dirty = True
+            self._free_past(b)
+        self.sync_block_table()
+        return kept
+
+    def _free_past(self, b: int):
+        """Pages of sequence b past its ``seq_lens`` go back to the free list."""
+        keep = -(-int(self.seq_lens[b]) // self.block_size)
+        row = self._bt[b]
+        freed = [int(x) for x in row[keep:] if x >= 0]
+        if freed:
+            row[keep:] = -1
+            self.free_blocks.extend(freed)
+            self._allocated -= len(freed)
+            self._dirty = True
+
+    def accept(self, cu_seqlens: torch.Tensor, context_lens: torch.Tensor, path: torch.Tensor,
+               counts: torch.Tensor) -> np.ndarray:
+        """Keep only the accepted ones of the new tokens that ``extend`` made room for: their K and V
+        move to consecutive slots in all layers (``kernels.drafting.keep_accepted``), ``seq_lens``
+        shrinks to them, and pages past it go back to the free list. cu_seqlens, context_lens: as
+        ``extend`` returned them; path, counts: from ``kernels.drafting.accept_drafts``. Returns the
+        counts on the host (the call waits for them)."""
+        from fast_infer_b200.kernels.drafting import keep_accepted
+        self.sync_block_table()
+        B = context_lens.numel()
+        if B > self._bt.shape[0]:
+            raise ValueError("batch larger than the block table")
+        keep_accepted(self.k, self.v, self.block_table, self.block_size, cu_seqlens, context_lens,
+                      path, counts, k_scale=self.k_scale, v_scale=self.v_scale)
+        host = torch.cat([cu_seqlens.to(torch.int32), context_lens.to(torch.int32),
+                          counts.to(torch.int32)]).cpu().numpy().astype(np.int64)
+        new, ctx, kept = np.diff(host[:B + 1]), host[B + 1:2 * B + 1], host[2 * B + 1:]
+        if (ctx != self.seq_lens[:B]).any() or (kept < 0).any() or (kept > new).any():
+            raise ValueError("accept needs the lengths of the last extend and counts of its tokens")
+        self.seq_lens[:B] = ctx - new + kept
+        for b in range(B):
+            self._free_past(b)
         self.sync_block_table()
         return kept
 
@@ -211,6 +249,8 @@ class KVCache:
         """Write k, v [B, T, H, D] at logical positions start_pos[b] + t of each
         sequence (start_pos: int or [B] int32 device tensor) — one kernel launch."""
         self.sync_block_table()
+        if self.k_scale is not None:
+            raise ValueError("a cache of 8-bit codes is written by rope_axes_store")
         if k.shape != v.shape or k.dim() != 4:
             raise ValueError("k, v must both be [batch, tokens, heads, head_dim]")
         B, T, H, D = k.shape

@@ -223,6 +223,34 @@ int fi_paged_chunk(const void* q, const void* k_cache, const void* v_cache, void
                    void* stream);
 
 /*
+ * fi_paged_chunk for trees of drafted tokens, and over pages of 8-bit codes.
+ *
+ * tree_mask: int32 [total_tokens, mask_words], dense: new token i of a sequence sees its new token j
+ * where bit j % 32 of word j / 32 of its row is set (fi_draft_tree), and, beside them, every token
+ * cached before the new ones: position pos_i = context_lens[b] - n_b + depths[i], it sees cached
+ * token j when window == 0 or j > pos_i - window (depths: int32 [total_tokens], needed with a
+ * window only; the mask alone decides among the new tokens). NULL: the new tokens are a chain, as
+ * in fi_paged_chunk. A token that sees nothing gets o = 0, lse = -inf.
+ * cache_dtype: dtype, or FI_DTYPE_I8 / FI_DTYPE_E4M3 with k_scale, v_scale (fp32 [num_blocks,
+ * num_kv_heads, 64], 3 strides each): K and V are code * scale; strides of the pages in elements,
+ * multiples of 16. Scales of cached tokens have to be finite, seen or not, for V (weight 0 * NaN).
+ * All else, limits and workspace too (fi_paged_tree_workspace_size), as in fi_paged_chunk.
+ */
+size_t fi_paged_tree_workspace_size(int64_t total_tokens, int64_t num_q_heads,
+                                    int64_t num_kv_heads);
+int fi_paged_tree(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                  const float* v_scale, void* o, float* lse, const int32_t* block_table,
+                  const int32_t* cu_seqlens, const int32_t* context_lens, const int32_t* tree_mask,
+                  const int32_t* depths, int64_t mask_words, int64_t batch, int64_t total_tokens,
+                  int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t num_blocks,
+                  int64_t block_size, int64_t max_blocks_per_seq, const int64_t* q_strides,
+                  const int64_t* kc_strides, const int64_t* vc_strides, const int64_t* ks_strides,
+                  const int64_t* vs_strides, const int64_t* o_strides, const int64_t* bt_strides,
+                  float sm_scale, float softcap, int64_t window, int64_t dtype,
+                  int64_t cache_dtype, void* workspace, size_t workspace_bytes,
+                  int32_t* error_flag, void* stream);
+
+/*
  * Attention weight that each cached token receives from the new tokens (no counterpart in the
  * reference; what an eviction from the cache goes by):
  *   mass[b, hk, j] (+)= sum over query rows i of KV head hk of exp(score_ij - lse_i).
