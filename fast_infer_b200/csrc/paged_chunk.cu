@@ -1459,21 +1459,18 @@ static size_t ck_workspace(ChunkParams* p, uint8_t* ws, int rows_cap) {
 // Whether every sequence can only have so few rows that the narrow kernel serves the batch.
 static bool ck_all_narrow(int64_t total, int64_t group) { return total * group <= kCkNarrow; }
 
-}  // namespace fi
-
-extern "C" size_t fi_paged_chunk_workspace_size(int64_t total_tokens, int64_t num_q_heads,
-                                                int64_t num_kv_heads) {
-  using namespace fi;
+// Workspace of a call: a part for each kernel that it may launch.
+static size_t ck_workspace_size(int64_t total_tokens, int64_t num_q_heads, int64_t num_kv_heads,
+                                bool codes) {
   if (total_tokens <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads ||
       num_q_heads % num_kv_heads != 0 || num_q_heads / num_kv_heads > 64 ||
       total_tokens > (1 << 28))
     return 0;
   const size_t narrow = ck_workspace(nullptr, nullptr, kCkNarrow);
+  if (codes) return ck_workspace(nullptr, nullptr, 2 * kChunkTile);
   if (ck_all_narrow(total_tokens, num_q_heads / num_kv_heads)) return narrow;
   return narrow + ck_workspace(nullptr, nullptr, 2 * kChunkTile);
 }
-
-namespace fi {
 
 // What fi_paged_tree has beside fi_paged_chunk's arguments.
 struct ChunkExtra {
@@ -1535,7 +1532,7 @@ static int paged_chunk(const char* what, const void* q, const void* k_cache, con
                 "%s o: needs a 16-byte aligned base, unit innermost stride and other "
                 "strides multiple of 8",
                 what);
-  const size_t need = fi_paged_chunk_workspace_size(total_tokens, num_q_heads, num_kv_heads);
+  const size_t need = ck_workspace_size(total_tokens, num_q_heads, num_kv_heads, codes);
   if (!workspace || workspace_bytes < need)
     return fail(FI_ERR_WORKSPACE, "%s: workspace of %zu bytes, needs %zu", what,
                 workspace ? workspace_bytes : (size_t)0, need);
@@ -1575,7 +1572,7 @@ static int paged_chunk(const char* what, const void* q, const void* k_cache, con
     n = p;
     n.b = nb;
   }
-  ws += ck_workspace(&n, ws, kCkNarrow);
+  if (!codes) ws += ck_workspace(&n, ws, kCkNarrow);
   if (use_wide) ck_workspace(&p, ws, 2 * kChunkTile);
   n.unit_tokens = (int)per_unit;
   n.split_rows = use_wide ? kCkNarrow : 0x7fffffff;
@@ -1591,6 +1588,11 @@ static int paged_chunk(const char* what, const void* q, const void* k_cache, con
 }
 
 }  // namespace fi
+
+extern "C" size_t fi_paged_chunk_workspace_size(int64_t total_tokens, int64_t num_q_heads,
+                                                int64_t num_kv_heads) {
+  return fi::ck_workspace_size(total_tokens, num_q_heads, num_kv_heads, false);
+}
 
 extern "C" int fi_paged_chunk(const void* q, const void* k_cache, const void* v_cache, void* o,
                               float* lse, const int32_t* block_table, const int32_t* cu_seqlens,
@@ -1614,8 +1616,9 @@ extern "C" int fi_paged_chunk(const void* q, const void* k_cache, const void* v_
 }
 
 extern "C" size_t fi_paged_tree_workspace_size(int64_t total_tokens, int64_t num_q_heads,
-                                               int64_t num_kv_heads) {
-  return fi_paged_chunk_workspace_size(total_tokens, num_q_heads, num_kv_heads);
+                                               int64_t num_kv_heads, int64_t cache_dtype) {
+  return fi::ck_workspace_size(total_tokens, num_q_heads, num_kv_heads,
+                               cache_dtype == FI_DTYPE_I8 || cache_dtype == FI_DTYPE_E4M3);
 }
 
 extern "C" int fi_paged_tree(const void* q, const void* k_cache, const void* v_cache,
