@@ -124,6 +124,86 @@ __device__ __forceinline__ uint64_t weight(const Row& row, const double* tab, fl
   return (uint64_t)__double_as_longlong(w + 128.0) - (uint64_t)__double_as_longlong(128.0);
 }
 
+// 16-bit logits: keys of the raw bits, in the order of the values, both zeros alike.
+template <typename T>
+struct Bits16 {
+  static constexpr int kRegion = 0;
+};
+template <>
+struct Bits16<__nv_bfloat16> {
+  static constexpr int kRegion = 2048;  // 16 octaves
+  static constexpr uint32_t kLowest = 0x8000 - 0x7f7f;
+  __device__ static __forceinline__ float value(uint32_t k) {
+    return __uint_as_float((k >= 0x8000 ? k - 0x8000 : (0x8000 - k) | 0x8000) << 16);
+  }
+  __device__ static __forceinline__ uint32_t bits_below(float x) {
+    return __bfloat16_as_ushort(__float2bfloat16_rd(x));
+  }
+  __device__ static __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a),
+                                         *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+};
+template <>
+struct Bits16<__half> {
+  static constexpr int kRegion = 8192;  // 8 octaves
+  static constexpr uint32_t kLowest = 0x8000 - 0x7bff;
+  __device__ static __forceinline__ float value(uint32_t k) {
+    return __half2float(
+        __ushort_as_half((unsigned short)(k >= 0x8000 ? k - 0x8000 : (0x8000 - k) | 0x8000)));
+  }
+  __device__ static __forceinline__ uint32_t bits_below(float x) {
+    return __half_as_ushort(__float2half_rd(x));
+  }
+  __device__ static __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    const __half2 m = __hmax2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+};
+__device__ __forceinline__ uint32_t keys16(uint32_t pair) {
+  uint32_t neg;  // 0xffff in the halves below 0
+  asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(neg) : "r"(pair));
+  return (pair ^ (neg | 0x80008000u)) + (neg & 0x00010001u);
+}
+
+// Bins of one 16-bit value each, descending: `n1` from the row's greatest down, `n2` further ones of negative values,
+// whose first lies `off2` below the greatest. What lies between the two (values near 0, of many octaves) is one lump.
+struct Values {
+  uint32_t top, lowest;  // keys: M, and of the least value with a weight
+  uint32_t n1, off2, n2;
+};
+template <typename T>
+__device__ __forceinline__ Values value_bins(const Row& row) {
+  constexpr uint32_t R = Bits16<T>::kRegion;
+  Values v;
+  v.top = keys16(Bits16<T>::bits_below(row.top)) & 0xffff;
+  v.lowest = max(keys16(Bits16<T>::bits_below(row.floor_x)) & 0xffff, Bits16<T>::kLowest);
+  const bool positive = v.top >= 0x8000;
+  const uint32_t limit = positive ? max(0x8000u, v.lowest) : v.lowest;
+  v.n1 = min(v.top - limit + 1, R);
+  v.n2 = v.off2 = 0;
+  if (positive && v.lowest < 0x8000) {
+    const uint32_t top2 = min(v.lowest + R - 1, 0x7fffu);
+    v.n2 = top2 - v.lowest + 1;
+    v.off2 = v.top - top2;
+  }
+  return v;
+}
+// Bin of the value d keys below the greatest; -1: none.
+template <typename T>
+__device__ __forceinline__ int value_bin(const Values& v, uint32_t d) {
+  constexpr int R = Bits16<T>::kRegion;
+  return d < v.n1 ? (int)d : d - v.off2 < v.n2 ? (int)(d - v.off2) + R : -1;
+}
+// Key of a bin; 0 past its region's end.
+template <typename T>
+__device__ __forceinline__ uint32_t bin_key(const Values& v, uint32_t bin) {
+  constexpr uint32_t R = Bits16<T>::kRegion;
+  if (bin < R) return bin < v.n1 ? v.top - bin : 0;
+  return bin - R < v.n2 ? v.top - v.off2 - (bin - R) : 0;
+}
+
 struct SaPart {  // what a CTA tells the others about its slice
   float top, low;  // greatest logit; least of its threads' greatest ones
   float least;     // least logit above -inf
@@ -131,22 +211,28 @@ struct SaPart {  // what a CTA tells the others about its slice
   int bad;         // NaN or +inf
   int index;       // greedy: first index of the greatest
   int ties;
-  uint64_t mass;
+  int lump_count;
+  uint64_t mass, lump_mass;
 };
 struct SaShared {
   double tab[32];
   uint64_t step_mass[kSaWarps * kSaSteps];
   uint64_t scan[kSaWarps];
-  uint32_t hist[2][kSaBins][3];
   SaPart part;
   float w_top[kSaWarps], w_low[kSaWarps], w_least[kSaWarps];
   int w_ties[kSaWarps];
   // the bin that a search chose
-  uint64_t above, held, total;
+  uint64_t above, held;
+  int64_t tie_base;
   uint32_t edge[2];
   int bin;
   uint32_t min_key;
+  uint64_t lump_mass[kSaWarps];
 };
+// Histograms: two of generic bins by turns, or one of 16-bit values, a count of 16 bits each.
+template <typename T>
+constexpr int kSaHistBytes = Bits16<T>::kRegion * 4 > 2 * kSaBins * 12 ? Bits16<T>::kRegion * 4
+                                                                       : 2 * kSaBins * 12;
 
 // Sum over the block's threads before this one, and of all, of a 64-bit value.
 __device__ __forceinline__ uint64_t block_exclusive(uint64_t v, uint64_t* warp_sums, uint64_t& all) {
@@ -184,6 +270,16 @@ struct Cut {
   bool all_ties;
 };
 
+// How many of a group of equal weights w stay when the mass before them is `above`: those before which the
+// mass is below the target.
+__device__ __forceinline__ int64_t kept_ties(double target, uint64_t above, uint64_t w, int64_t group) {
+  int64_t r = (int64_t)ceil((target - (double)above) / (double)w);
+  r = max((int64_t)1, min(r, group));
+  while (r > 1 && (double)(above + (uint64_t)(r - 1) * w) >= target) --r;
+  while (r < group && (double)(above + (uint64_t)r * w) < target) ++r;
+  return r;
+}
+
 // The bin of a value in a search's first level.
 __device__ __forceinline__ int linear_bin(float top, float scale, float x) {
   return min((int)((top - x) * scale), kSaBins - 1);
@@ -192,7 +288,8 @@ __device__ __forceinline__ int linear_bin(float top, float scale, float x) {
 // The cut at which the count of tokens reaches `want` (kMass = false), or the mass that `share` of all from
 // lo_key on, less `drop`, asks for. `above` of the result's group: what lies before it.
 template <typename T, bool kMass>
-__device__ __forceinline__ Cut search(cg::cluster_group& cluster, SaShared* s, const T* x, int steps,
+__device__ __noinline__ Cut search(cg::cluster_group& cluster, SaShared* s,
+                                   uint32_t (*hists)[kSaBins][3], const T* x, int steps,
                                       int chunk_base, const Row& row, uint32_t lo_key, int64_t want,
                                       double share, uint64_t drop, int& level) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -206,7 +303,7 @@ __device__ __forceinline__ Cut search(cg::cluster_group& cluster, SaShared* s, c
   int shift = 0;
 #pragma unroll 1
   while (true) {
-    uint32_t(*hist)[3] = s->hist[level & 1];
+    uint32_t(*hist)[3] = hists[level & 1];
 #pragma unroll 1
     for (int st = 0; st < steps; ++st) {
       float v[8];
@@ -233,7 +330,7 @@ __device__ __forceinline__ Cut search(cg::cluster_group& cluster, SaShared* s, c
     cluster.sync();
     ++level;
     // every CTA has read the other buffer before it came here
-    for (int i = tid; i < kSaBins * 3; i += kSaThreads) (&s->hist[level & 1][0][0])[i] = 0;
+    for (int i = tid; i < kSaBins * 3; i += kSaThreads) (&hists[level & 1][0][0])[i] = 0;
     uint64_t mine = 0;
     for (int r = 0; r < ctas; ++r) {
       const uint32_t* h = cluster.map_shared_rank(&hist[tid][0], r);
@@ -302,14 +399,10 @@ __device__ __forceinline__ Cut search(cg::cluster_group& cluster, SaShared* s, c
   const uint32_t key = hi_key & 0x80000000u ? hi_key & ~low : hi_key | low;
   Cut cut = {key, 0, false};
   if constexpr (kMass) {
-    const double w = (double)weight(row, s->tab, of_key(key));
-    const int64_t group = (int64_t)(held / (uint64_t)w);
-    int64_t r = (int64_t)ceil((target - (double)above) / w);
-    r = max((int64_t)1, min(r, group));
-    while (r > 1 && (double)(above + (uint64_t)(r - 1) * (uint64_t)w) >= target) --r;
-    while (r < group && (double)(above + (uint64_t)r * (uint64_t)w) < target) ++r;
-    cut.ties = r;
-    cut.all_ties = r >= group;
+    const uint64_t w = weight(row, s->tab, of_key(key));
+    const int64_t group = (int64_t)(held / w);
+    cut.ties = kept_ties(target, above, w, group);
+    cut.all_ties = cut.ties >= group;
   } else {
     cut.ties = want - (int64_t)above;
     cut.all_ties = cut.ties >= (int64_t)held;
@@ -325,11 +418,79 @@ __device__ __forceinline__ Cut tighter(const Cut& a, const Cut& b) {
   return a.ties < b.ties ? a : b;
 }
 
+// The first value at which the running count passes `want` - 1, or the running mass reaches `target`: a thread has
+// `kBinsEach` bins, whose sums `count` and `mass` begin after `before_count` and `before_mass`. Its warp then takes a
+// lane per bin. False: it lies in the lump (or nowhere).
+struct ValueCut {
+  uint32_t key16;
+  uint32_t group;       // tokens that have the value
+  uint64_t count, mass; // before it
+};
+template <typename T, bool kMass>
+__device__ __forceinline__ bool value_cross(cg::cluster_group& cluster, SaShared* s,
+                                            const uint32_t* counts, const Row& row, const Values& v,
+                                            uint64_t count, uint64_t mass, uint64_t before_count,
+                                            uint64_t before_mass, uint64_t want, double target,
+                                            ValueCut& cut) {
+  constexpr int kEach = 2 * Bits16<T>::kRegion / kSaThreads;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const bool here = kMass ? (double)before_mass < target && (double)(before_mass + mass) >= target
+                          : before_count < want && before_count + count >= want;
+  __syncthreads();
+  if (tid == 0) s->bin = -1;
+  __syncthreads();
+  if (here && count > 0) {
+    s->bin = tid;
+    s->above = before_mass;
+    s->held = before_count;
+  }
+  __syncthreads();
+  const int owner = s->bin;
+  if (owner < 0) return false;
+  if (warp == owner >> 5) {
+    const int bin = owner * kEach + lane;
+    uint32_t n = 0;
+    uint64_t w = 0;
+    const uint32_t key = lane < kEach ? bin_key<T>(v, bin) : 0;
+    if (key != 0) {
+      for (int r = 0; r < (int)cluster.num_blocks(); ++r)
+        n += (cluster.map_shared_rank(counts, r)[bin >> 1] >> (16 * (bin & 1))) & 0xffff;
+      const float value = Bits16<T>::value(key);
+      if (n > 0 && value >= row.floor_x) w = weight(row, s->tab, value);
+    }
+    uint64_t c = n, m = n * w;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const uint64_t oc = __shfl_up_sync(0xffffffffu, c, off), om = __shfl_up_sync(0xffffffffu, m, off);
+      if (lane >= off) c += oc, m += om;
+    }
+    c += s->held;
+    m += s->above;
+    const uint32_t past = __ballot_sync(
+        0xffffffffu, n > 0 && (kMass ? (double)m >= target : c >= want));
+    __syncwarp();
+    if (past && lane == __ffs((int)past) - 1) {
+      s->edge[0] = key;
+      s->edge[1] = n;
+      s->held = c - n;
+      s->above = m - n * w;
+    }
+  }
+  __syncthreads();
+  cut.key16 = s->edge[0];
+  cut.group = s->edge[1];
+  cut.count = s->held;
+  cut.mass = s->above;
+  return true;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kSaThreads) sample_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   SaShared* s = reinterpret_cast<SaShared*>(smem);
-  T* x = reinterpret_cast<T*>(smem + (sizeof(SaShared) + 15) / 16 * 16);
+  uint32_t* counts = reinterpret_cast<uint32_t*>(smem + (sizeof(SaShared) + 15) / 16 * 16);
+  auto hists = reinterpret_cast<uint32_t(*)[kSaBins][3]>(counts);
+  T* x = reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(counts) + kSaHistBytes<T>);
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int row_id = blockIdx.x / ctas;
@@ -337,7 +498,7 @@ __global__ void __launch_bounds__(kSaThreads) sample_kernel(const SampleArgs a) 
   const int slice = a.chunk * kSaWarps, base = rank * slice;
   const int here = max(0, min(slice, a.vocab - base));  // tokens of this CTA
   const int steps = a.chunk / kSaStep, chunk_base = warp * a.chunk;
-  for (int i = tid; i < 2 * kSaBins * 3; i += kSaThreads) (&s->hist[0][0][0])[i] = 0;
+  for (int i = tid; i < kSaHistBytes<T> / 4; i += kSaThreads) counts[i] = 0;
   if (tid < 32) s->tab[tid] = exp2(tid / 32.0);
   grid_dep_wait();
   grid_dep_launch();
@@ -377,6 +538,24 @@ __global__ void __launch_bounds__(kSaThreads) sample_kernel(const SampleArgs a) 
   // the row's greatest and least logits, and whether one is NaN or +inf
   float top = -INFINITY, least = INFINITY;
   bool bad = false;
+  if constexpr (sizeof(T) == 2) {
+    uint4 m;
+    m.x = m.y = m.z = m.w = (Bits16<T>::bits_below(-INFINITY)) * 0x10001u;
+#pragma unroll 2
+    for (int st = 0; st < steps; ++st) {
+      const uint4 v =
+          *reinterpret_cast<const uint4*>(x + chunk_base + st * kSaStep + lane * 8);
+      m.x = Bits16<T>::max2(m.x, v.x);
+      m.y = Bits16<T>::max2(m.y, v.y);
+      m.z = Bits16<T>::max2(m.z, v.z);
+      m.w = Bits16<T>::max2(m.w, v.w);
+    }
+    const uint32_t both = Bits16<T>::max2(Bits16<T>::max2(m.x, m.y), Bits16<T>::max2(m.z, m.w));
+    const T* t = reinterpret_cast<const T*>(&both);
+    top = fmax_nan(logit(t[0]), logit(t[1])) + 0.f;
+    bad = !(top < INFINITY);
+    least = -FLT_MAX;  // (a bound is all that the search asks for)
+  } else {
 #pragma unroll 1
   for (int st = 0; st < steps; ++st) {
     float v[8];
@@ -387,6 +566,7 @@ __global__ void __launch_bounds__(kSaThreads) sample_kernel(const SampleArgs a) 
       top = fmaxf(top, v[i]);
       least = fminf(least, v[i] == -INFINITY ? INFINITY : v[i]);
     }
+  }
   }
   float low = top == -INFINITY ? INFINITY : top;  // least of the threads' greatest
   const int threads = __syncthreads_count(top > -INFINITY);
@@ -482,35 +662,176 @@ __global__ void __launch_bounds__(kSaThreads) sample_kernel(const SampleArgs a) 
       __syncthreads();
       cut.key = s->min_key;
     }
-    uint64_t drop = 0;
-    if (k > 0 && k < a.vocab) {
-      // as many threads as `with` have a logit of at least `low`
-      const float from = k <= with ? low : least;
-      const Cut c = search<T, false>(cluster, s, x, steps, chunk_base, row, key_of(from), k, 0.0, 0,
-                                     level);
-      if (c.key != 0 && !c.all_ties) {
-        const float value = of_key(c.key);
-        if (value >= row.floor_x)
-          drop = (s->held - (uint64_t)c.ties) * weight(row, s->tab, value);
+    int64_t rank_of_tie = 0;  // ties before this CTA's (later: this warp's) tokens
+    uint64_t own = 0;         // kept mass of this CTA's tokens, where the values' counts tell it
+    bool counted = false;
+    if constexpr (sizeof(T) == 2) {
+      constexpr int kEach = 2 * Bits16<T>::kRegion / kSaThreads;
+      const Values bins = value_bins<T>(row);
+      int lump_n = 0;
+      uint64_t lump_m = 0;
+#pragma unroll 1
+      for (int st = 0; st < steps; ++st) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(x + chunk_base + st * kSaStep + lane * 8);
+        const uint32_t pair[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          // (no key is above the greatest: the halves do not borrow)
+          const uint32_t below = bins.top * 0x10001u - keys16(pair[i >> 1]);
+          const uint32_t d = i & 1 ? below >> 16 : below & 0xffff;
+          const int bin = value_bin<T>(bins, d);
+          if (bin >= 0) {
+            atomicAdd(&counts[bin >> 1], 1u << (16 * (bin & 1)));
+          } else if (d <= bins.top - bins.lowest) {
+            const float v = Bits16<T>::value(bins.top - d);
+            ++lump_n;
+            if (v >= row.floor_x) lump_m += weight(row, s->tab, v);
+          }
+        }
+      }
+      const uint64_t own_lump_m = warp_sum(lump_m);
+      lump_n = __reduce_add_sync(0xffffffffu, lump_n);
+      if (lane == 0) {
+        s->w_ties[warp] = lump_n;
+        s->lump_mass[warp] = own_lump_m;
       }
       __syncthreads();
-      const Cut before = cut;
-      cut = c;
-      if (top_p < 1.f) {
-        const Cut p = search<T, true>(cluster, s, x, steps, chunk_base, row,
-                                      max(c.key, key_of(row.floor_x)), 0, (double)top_p, drop, level);
+      if (tid == 0) {
+        int n = 0;
+        uint64_t m = 0;
+        for (int w = 0; w < kSaWarps; ++w) n += s->w_ties[w], m += s->lump_mass[w];
+        s->part.lump_count = n;
+        s->part.lump_mass = m;
+      }
+      cluster.sync();
+      uint64_t lump_count = 0, lump_mass = 0;
+      for (int r = 0; r < ctas; ++r) {
+        lump_count += cluster.map_shared_rank(&s->part, r)->lump_count;
+        lump_mass += cluster.map_shared_rank(&s->part, r)->lump_mass;
+      }
+      // the sums of this thread's bins, of all CTAs and of this one
+      uint64_t count = 0, mass = 0, own_mass = 0;
+#pragma unroll 2
+      for (int i = 0; i < kEach; i += 2) {
+        const int word = (tid * kEach + i) >> 1;
+        uint32_t n[2] = {0, 0};
+        for (int r = 0; r < ctas; ++r) {
+          const uint32_t h = cluster.map_shared_rank(counts, r)[word];
+          n[0] += h & 0xffff;
+          n[1] += h >> 16;
+        }
+        const uint32_t mine = counts[word];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (n[j] == 0) continue;
+          const float v = Bits16<T>::value(bin_key<T>(bins, tid * kEach + i + j));
+          const uint64_t w = v >= row.floor_x ? weight(row, s->tab, v) : 0;
+          count += n[j];
+          mass += n[j] * w;
+          own_mass += (j ? mine >> 16 : mine & 0xffff) * w;
+        }
+      }
+      uint64_t all_count, all_mass;
+      uint64_t before_count = block_exclusive(count, s->scan, all_count);
+      uint64_t before_mass = block_exclusive(mass, s->scan, all_mass);
+      if (tid >= kSaThreads / 2) before_count += lump_count, before_mass += lump_mass;
+      all_count += lump_count;
+      all_mass += lump_mass;
+      counted = true;
+      Cut c = {0u, 0, true};
+      ValueCut vc;
+      if (k > 0 && (uint64_t)k < all_count) {
+        counted = value_cross<T, false>(cluster, s, counts, row, bins, count, mass, before_count,
+                                        before_mass, (uint64_t)k, 0.0, vc);
+        if (counted) {
+          const float v = Bits16<T>::value(vc.key16);
+          c = {key_of(v), k - (int64_t)vc.count, k - (int64_t)vc.count >= (int64_t)vc.group};
+          all_mass = vc.mass + (v >= row.floor_x ? c.ties * weight(row, s->tab, v) : 0);
+        }
+      }
+      if (counted && top_p < 1.f) {
+        const double target = fmax((double)top_p * (double)all_mass, 1.0);
+        counted = value_cross<T, true>(cluster, s, counts, row, bins, count, mass, before_count,
+                                       before_mass, 0, target, vc);
+        if (counted) {
+          const float v = Bits16<T>::value(vc.key16);
+          const int64_t r = kept_ties(target, vc.mass, weight(row, s->tab, v), vc.group);
+          c = tighter(c, {key_of(v), r, r >= (int64_t)vc.group});
+        }
+      }
+      if (counted) {
+        c = tighter(cut, c);
+        // a cut (of min-p) within the lump is left to the search
+        const uint32_t lump_hi = bins.top - bins.n1;  // its greatest key
+        const uint32_t lump_lo = bins.n2 ? bins.top - bins.off2 + 1 : bins.lowest;
+        const bool lump_in = lump_count > 0 && c.key <= key_of(Bits16<T>::value(lump_lo));
+        if (lump_count > 0 && !lump_in && c.key <= key_of(Bits16<T>::value(lump_hi))) counted = false;
+        if (counted) {
+          // this CTA's kept mass: bins above the cut, and its share of the ties
+          uint64_t m = 0;
+          const uint32_t last = bin_key<T>(bins, tid * kEach + kEach - 1);
+          if (last != 0 && key_of(Bits16<T>::value(last)) > c.key) {
+            m = own_mass;
+          } else if (count > 0) {
+#pragma unroll 1
+            for (int i = 0; i < kEach; ++i) {
+              const int bin = tid * kEach + i;
+              const uint32_t key16 = bin_key<T>(bins, bin);
+              const float v = Bits16<T>::value(key16);
+              if (key16 == 0 || key_of(v) < c.key) break;
+              int64_t n = (counts[bin >> 1] >> (16 * (bin & 1))) & 0xffff;
+              if (key_of(v) == c.key && !c.all_ties) {
+                int64_t ahead = 0;
+                for (int r = 0; r < rank; ++r)
+                  ahead += (cluster.map_shared_rank(counts, r)[bin >> 1] >> (16 * (bin & 1))) & 0xffff;
+                s->tie_base = ahead;
+                n = max((int64_t)0, min(n, c.ties - ahead));
+              }
+              if (n > 0 && v >= row.floor_x) m += n * weight(row, s->tab, v);
+            }
+          }
+          if (tid == 0 && lump_in) m += s->part.lump_mass;
+          block_exclusive(m, s->scan, own);
+          if (!c.all_ties) rank_of_tie = s->tie_base;
+          cut = c;
+        }
+      }
+      if (!counted) {  // the histograms' place is taken by the search's
+        cluster.sync();
+        for (int i = tid; i < kSaHistBytes<T> / 4; i += kSaThreads) counts[i] = 0;
+        __syncthreads();
+      }
+    }
+    if (!counted) {
+      uint64_t drop = 0;
+      if (k > 0 && k < a.vocab) {
+        // as many threads as `with` have a logit of at least `low`
+        const float from = k <= with ? low : least;
+        const Cut c = search<T, false>(cluster, s, hists, x, steps, chunk_base, row, key_of(from), k, 0.0, 0,
+                                       level);
+        if (c.key != 0 && !c.all_ties) {
+          const float value = of_key(c.key);
+          if (value >= row.floor_x)
+            drop = (s->held - (uint64_t)c.ties) * weight(row, s->tab, value);
+        }
+        __syncthreads();
+        const Cut before = cut;
+        cut = c;
+        if (top_p < 1.f) {
+          const Cut p = search<T, true>(cluster, s, hists, x, steps, chunk_base, row,
+                                        max(c.key, key_of(row.floor_x)), 0, (double)top_p, drop, level);
+          cut = tighter(cut, p);
+        }
+        cut = tighter(before, cut);
+      } else if (top_p < 1.f) {
+        const Cut p = search<T, true>(cluster, s, hists, x, steps, chunk_base, row,
+                                      max(key_of(least), key_of(row.floor_x)), 0, (double)top_p, 0, level);
         cut = tighter(cut, p);
       }
-      cut = tighter(before, cut);
-    } else if (top_p < 1.f) {
-      const Cut p = search<T, true>(cluster, s, x, steps, chunk_base, row,
-                                    max(key_of(least), key_of(row.floor_x)), 0, (double)top_p, 0, level);
-      cut = tighter(cut, p);
     }
 
     // ties before this warp's tokens, where only some of them stay
-    int64_t rank_of_tie = 0;
-    if (!cut.all_ties) {
+    auto count_ties = [&]() {
       int n = 0;
 #pragma unroll 1
       for (int st = 0; st < steps; ++st) {
@@ -522,6 +843,10 @@ __global__ void __launch_bounds__(kSaThreads) sample_kernel(const SampleArgs a) 
       n = __reduce_add_sync(0xffffffffu, n);
       if (lane == 0) s->w_ties[warp] = n;
       __syncthreads();
+      for (int w = 0; w < warp; ++w) rank_of_tie += s->w_ties[w];
+    };
+    if (!cut.all_ties && !counted) {
+      count_ties();
       if (tid == 0) {
         int t = 0;
         for (int w = 0; w < kSaWarps; ++w) t += s->w_ties[w];
@@ -529,7 +854,6 @@ __global__ void __launch_bounds__(kSaThreads) sample_kernel(const SampleArgs a) 
       }
       cluster.sync();
       for (int r = 0; r < rank; ++r) rank_of_tie += cluster.map_shared_rank(&s->part, r)->ties;
-      for (int w = 0; w < warp; ++w) rank_of_tie += s->w_ties[w];
     }
     // kept weights of 8 tokens; `tie` counts the ties before this lane's
     auto kept = [&](const float* v, int64_t tie, uint64_t* w) {
@@ -558,24 +882,31 @@ __global__ void __launch_bounds__(kSaThreads) sample_kernel(const SampleArgs a) 
       all = __shfl_sync(0xffffffffu, inc, 31);
       return inc - n;
     };
-    const int64_t first_tie = rank_of_tie;
-#pragma unroll 1
-    for (int st = 0; st < steps; ++st) {
-      float v[8];
-      uint64_t w[8];
-      load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
-      int all = 0;
-      const int64_t tie = rank_of_tie + (cut.all_ties ? 0 : ties_before(v, all));
-      const uint64_t sum = warp_sum(kept(v, tie, w));
-      rank_of_tie += all;
-      if (lane == 0) s->step_mass[warp * steps + st] = sum;
-    }
-    __syncthreads();
     const int cells = kSaWarps * steps;
-    uint64_t all;
-    const uint64_t cell = tid < cells ? s->step_mass[tid] : 0;
-    const uint64_t before = block_exclusive(cell, s->scan, all);
-    if (tid == 0) s->part.mass = all;
+    int64_t first_tie = 0;
+    uint64_t cell = 0, before = 0, all = 0;  // a thread's cell: 256 tokens of the CTA
+    auto add_cells = [&]() {
+      first_tie = rank_of_tie;
+#pragma unroll 1
+      for (int st = 0; st < steps; ++st) {
+        float v[8];
+        uint64_t w[8];
+        load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
+        int in_step = 0;
+        const int64_t tie = rank_of_tie + (cut.all_ties ? 0 : ties_before(v, in_step));
+        const uint64_t sum = warp_sum(kept(v, tie, w));
+        rank_of_tie += in_step;
+        if (lane == 0) s->step_mass[warp * steps + st] = sum;
+      }
+      __syncthreads();
+      cell = tid < cells ? s->step_mass[tid] : 0;
+      before = block_exclusive(cell, s->scan, all);
+    };
+    if (!counted) {
+      add_cells();
+      own = all;
+    }
+    if (tid == 0) s->part.mass = own;
     cluster.sync();
     uint64_t mass = 0, ahead = 0;
     int last = 0;  // the last CTA with a kept token
@@ -588,6 +919,13 @@ __global__ void __launch_bounds__(kSaThreads) sample_kernel(const SampleArgs a) 
     // the first cell whose running sum passes the target; the last kept one where none does (u = 1, NaN)
     const double target = (double)u * (double)mass;
     const bool none = !((double)mass > target);
+    if (counted && own > 0 &&
+        (none ? rank == last
+              : (double)(ahead + own) > target && (ahead == 0 || !((double)ahead > target)))) {
+      // this CTA alone looks for the token
+      if (!cut.all_ties) count_ties();
+      add_cells();
+    }
     if (tid == 0) s->bin = -1;
     __syncthreads();
     if (cell > 0) {
@@ -641,11 +979,11 @@ __global__ void __launch_bounds__(kSaThreads) sample_kernel(const SampleArgs a) 
 template <typename T>
 static int launch_sample(const SampleArgs& a, int64_t rows, int ctas, cudaStream_t st) {
   const size_t smem =
-      (sizeof(SaShared) + 15) / 16 * 16 + (size_t)a.chunk * kSaWarps * sizeof(T);
+      (sizeof(SaShared) + 15) / 16 * 16 + kSaHistBytes<T> + (size_t)a.chunk * kSaWarps * sizeof(T);
   static DeviceOnce once;
   cudaError_t e = once.run([] {
     return cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)((sizeof(SaShared) + 15) / 16 * 16) +
+                                (int)((sizeof(SaShared) + 15) / 16 * 16) + kSaHistBytes<T> +
                                     kSaWarps * kSaSteps * kSaStep * (int)sizeof(T));
   });
   if (e != cudaSuccess) return cuda_fail(e, "fi_sample_tokens: kernel set-up");
