@@ -217,44 +217,62 @@ struct SaPart {  // what a CTA tells the others about its slice
 struct SaShared {
   double tab[32];
   uint64_t step_mass[kSaWarps * kSaSteps];
-  uint64_t scan[kSaWarps];
+  uint64_t scan[2 * kSaWarps];
   SaPart part;
   float w_top[kSaWarps], w_low[kSaWarps], w_least[kSaWarps];
   int w_ties[kSaWarps];
   // the bin that a search chose
   uint64_t above, held;
-  int64_t tie_base;
+  int64_t tie_base[2];
+  int tie_end;
   uint32_t edge[2];
   int bin;
   uint32_t min_key;
   uint64_t lump_mass[kSaWarps];
 };
-// Histograms: two of generic bins by turns, or one of 16-bit values, a count of 16 bits each.
+// Histograms: two of generic bins by turns, or one of 16-bit values. Where their weights fit in twice the bytes (bf16)
+// they take the same place afterwards.
 template <typename T>
-constexpr int kSaHistBytes = Bits16<T>::kRegion * 4 > 2 * kSaBins * 12 ? Bits16<T>::kRegion * 4
-                                                                       : 2 * kSaBins * 12;
+constexpr int kSaValueBins = 2 * Bits16<T>::kRegion;
+template <typename T>
+constexpr bool kSaTable = kSaValueBins<T> > 0 && kSaValueBins<T> * 8 <= 32768;
+template <typename T>
+constexpr int kSaHistBytes = kSaTable<T>                ? kSaValueBins<T> * 8
+                             : kSaValueBins<T> > 0 ? kSaValueBins<T> * 4
+                                                   : 2 * kSaBins * 12;
 
-// Sum over the block's threads before this one, and of all, of a 64-bit value.
-__device__ __forceinline__ uint64_t block_exclusive(uint64_t v, uint64_t* warp_sums, uint64_t& all) {
+// Sums over the block's threads before this one, and of all, of N 64-bit values. `warp_sums`: N x kSaWarps.
+template <int N>
+__device__ __forceinline__ void block_exclusive(const uint64_t* v, uint64_t* warp_sums, uint64_t* before,
+                                                uint64_t* all) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint64_t inc = v;
+  uint64_t inc[N];
 #pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const uint64_t o = __shfl_up_sync(0xffffffffu, inc, off);
-    if (lane >= off) inc += o;
-  }
-  if (lane == 31) warp_sums[warp] = inc;
-  __syncthreads();
-  uint64_t before = 0;
-  all = 0;
+  for (int i = 0; i < N; ++i) inc[i] = v[i];
 #pragma unroll
-  for (int w = 0; w < kSaWarps; ++w) {
-    const uint64_t s = warp_sums[w];
-    if (w < warp) before += s;
-    all += s;
+  for (int off = 1; off < 32; off <<= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint64_t o = __shfl_up_sync(0xffffffffu, inc[i], off);
+      if (lane >= off) inc[i] += o;
+    }
+  if (lane == 31)
+#pragma unroll
+    for (int i = 0; i < N; ++i) warp_sums[i * kSaWarps + warp] = inc[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    uint64_t w = lane < kSaWarps ? warp_sums[i * kSaWarps + lane] : 0;
+#pragma unroll
+    for (int off = 1; off < kSaWarps; off <<= 1) {
+      const uint64_t o = __shfl_up_sync(0xffffffffu, w, off);
+      if (lane >= off) w += o;
+    }
+    all[i] = __shfl_sync(0xffffffffu, w, kSaWarps - 1);
+    const uint64_t warps = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
+    before[i] = (warp ? warps : 0) + inc[i] - v[i];
   }
   __syncthreads();
-  return before + inc - v;
 }
 
 __device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
@@ -336,8 +354,9 @@ __device__ __noinline__ Cut search(cg::cluster_group& cluster, SaShared* s,
       const uint32_t* h = cluster.map_shared_rank(&hist[tid][0], r);
       mine += kMass ? (uint64_t)h[0] + ((uint64_t)h[1] << 15) + ((uint64_t)h[2] << 30) : h[0];
     }
-    uint64_t all;
-    const uint64_t before = above + block_exclusive(mine, s->scan, all);
+    uint64_t all, before;
+    block_exclusive<1>(&mine, s->scan, &before, &all);
+    before += above;
     if (kMass && first) target = fmax(share * (double)(all - drop), 1.0);
     const bool pick = kMass ? (double)before < target && (double)(before + mine) >= target
                             : before < (uint64_t)want && before + mine >= (uint64_t)want;
@@ -419,8 +438,7 @@ __device__ __forceinline__ Cut tighter(const Cut& a, const Cut& b) {
 }
 
 // The first value at which the running count passes `want` - 1, or the running mass reaches `target`: a thread has
-// `kBinsEach` bins, whose sums `count` and `mass` begin after `before_count` and `before_mass`. Its warp then takes a
-// lane per bin. False: it lies in the lump (or nowhere).
+// kEach bins, whose count and mass are `sums`, with `before` before them. Its warp then takes a lane per bin. False: it lies in the lump (or nowhere).
 struct ValueCut {
   uint32_t key16;
   uint32_t group;       // tokens that have the value
@@ -429,20 +447,19 @@ struct ValueCut {
 template <typename T, bool kMass>
 __device__ __forceinline__ bool value_cross(cg::cluster_group& cluster, SaShared* s,
                                             const uint32_t* counts, const Row& row, const Values& v,
-                                            uint64_t count, uint64_t mass, uint64_t before_count,
-                                            uint64_t before_mass, uint64_t want, double target,
-                                            ValueCut& cut) {
-  constexpr int kEach = 2 * Bits16<T>::kRegion / kSaThreads;
+                                            const uint64_t* sums, const uint64_t* before,
+                                            uint64_t want, double target, ValueCut& cut) {
+  constexpr int kEach = kSaValueBins<T> / kSaThreads;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const bool here = kMass ? (double)before_mass < target && (double)(before_mass + mass) >= target
-                          : before_count < want && before_count + count >= want;
+  const bool here = kMass ? (double)before[1] < target && (double)(before[1] + sums[1]) >= target
+                          : before[0] < want && before[0] + sums[0] >= want;
   __syncthreads();
   if (tid == 0) s->bin = -1;
   __syncthreads();
-  if (here && count > 0) {
+  if (here && sums[0] > 0) {
     s->bin = tid;
-    s->above = before_mass;
-    s->held = before_count;
+    s->above = before[1];
+    s->held = before[0];
   }
   __syncthreads();
   const int owner = s->bin;
@@ -454,7 +471,7 @@ __device__ __forceinline__ bool value_cross(cg::cluster_group& cluster, SaShared
     const uint32_t key = lane < kEach ? bin_key<T>(v, bin) : 0;
     if (key != 0) {
       for (int r = 0; r < (int)cluster.num_blocks(); ++r)
-        n += (cluster.map_shared_rank(counts, r)[bin >> 1] >> (16 * (bin & 1))) & 0xffff;
+        n += cluster.map_shared_rank(counts, r)[bin];
       const float value = Bits16<T>::value(key);
       if (n > 0 && value >= row.floor_x) w = weight(row, s->tab, value);
     }
@@ -485,7 +502,7 @@ __device__ __forceinline__ bool value_cross(cg::cluster_group& cluster, SaShared
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kSaThreads) sample_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   SaShared* s = reinterpret_cast<SaShared*>(smem);
   uint32_t* counts = reinterpret_cast<uint32_t*>(smem + (sizeof(SaShared) + 15) / 16 * 16);
@@ -503,7 +520,9 @@ __global__ void __launch_bounds__(kSaThreads) sample_kernel(const SampleArgs a) 
   grid_dep_wait();
   grid_dep_launch();
   // The slice into shared memory: 16 bytes at a time from the first aligned token on (rows of an odd
-  // vocabulary begin anywhere), -inf past its end.
+  // vocabulary begin anywhere), -inf past its end. 16-bit values show their greatest on the way.
+  float top = -INFINITY, least = INFINITY;
+  bool bad = false;
   {
     const T* g = static_cast<const T*>(a.x) + row_id * a.stride + base;
     constexpr int kVec = 16 / (int)sizeof(T);
@@ -511,6 +530,8 @@ __global__ void __launch_bounds__(kSaThreads) sample_kernel(const SampleArgs a) 
     const int head = min(here, off == 0 ? 0 : kVec - off), vecs = (here - head) / kVec;
     const uint4* gv = reinterpret_cast<const uint4*>(g + head);
     constexpr int kBatch = 8;
+    uint4 m = make_uint4(0, 0, 0, 0);
+    if constexpr (sizeof(T) == 2) m.x = m.y = m.z = m.w = Bits16<T>::bits_below(-INFINITY) * 0x10001u;
     for (int i0 = tid; i0 < vecs; i0 += kSaThreads * kBatch) {
       uint4 v[kBatch];
 #pragma unroll
@@ -527,48 +548,48 @@ __global__ void __launch_bounds__(kSaThreads) sample_kernel(const SampleArgs a) 
 #pragma unroll
           for (int e = 0; e < kVec; ++e) x[head + i * kVec + e] = t[e];
         }
+        if constexpr (sizeof(T) == 2) {
+          m.x = Bits16<T>::max2(m.x, v[j].x);
+          m.y = Bits16<T>::max2(m.y, v[j].y);
+          m.z = Bits16<T>::max2(m.z, v[j].z);
+          m.w = Bits16<T>::max2(m.w, v[j].w);
+        }
       }
     }
-    for (int i = tid; i < head; i += kSaThreads) x[i] = g[i];
-    for (int i = head + vecs * kVec + tid; i < here; i += kSaThreads) x[i] = g[i];
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t both = Bits16<T>::max2(Bits16<T>::max2(m.x, m.y), Bits16<T>::max2(m.z, m.w));
+      const T* t = reinterpret_cast<const T*>(&both);
+      top = fmax_nan(logit(t[0]), logit(t[1]));
+    }
+    auto single = [&](int i) {
+      x[i] = g[i];
+      if constexpr (sizeof(T) == 2) top = fmax_nan(top, logit(g[i]));
+    };
+    for (int i = tid; i < head; i += kSaThreads) single(i);
+    for (int i = head + vecs * kVec + tid; i < here; i += kSaThreads) single(i);
     for (int i = here + tid; i < slice; i += kSaThreads) x[i] = (T)(-INFINITY);
   }
   __syncthreads();
 
   // the row's greatest and least logits, and whether one is NaN or +inf
-  float top = -INFINITY, least = INFINITY;
-  bool bad = false;
   if constexpr (sizeof(T) == 2) {
-    uint4 m;
-    m.x = m.y = m.z = m.w = (Bits16<T>::bits_below(-INFINITY)) * 0x10001u;
-#pragma unroll 2
-    for (int st = 0; st < steps; ++st) {
-      const uint4 v =
-          *reinterpret_cast<const uint4*>(x + chunk_base + st * kSaStep + lane * 8);
-      m.x = Bits16<T>::max2(m.x, v.x);
-      m.y = Bits16<T>::max2(m.y, v.y);
-      m.z = Bits16<T>::max2(m.z, v.z);
-      m.w = Bits16<T>::max2(m.w, v.w);
-    }
-    const uint32_t both = Bits16<T>::max2(Bits16<T>::max2(m.x, m.y), Bits16<T>::max2(m.z, m.w));
-    const T* t = reinterpret_cast<const T*>(&both);
-    top = fmax_nan(logit(t[0]), logit(t[1])) + 0.f;
+    top += 0.f;
     bad = !(top < INFINITY);
     least = -FLT_MAX;  // (a bound is all that the search asks for)
   } else {
 #pragma unroll 1
-  for (int st = 0; st < steps; ++st) {
-    float v[8];
-    load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
+    for (int st = 0; st < steps; ++st) {
+      float v[8];
+      load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      bad |= !(v[i] < INFINITY);
-      top = fmaxf(top, v[i]);
-      least = fminf(least, v[i] == -INFINITY ? INFINITY : v[i]);
+      for (int i = 0; i < 8; ++i) {
+        bad |= !(v[i] < INFINITY);
+        top = fmaxf(top, v[i]);
+        least = fminf(least, v[i] == -INFINITY ? INFINITY : v[i]);
+      }
     }
   }
-  }
-  float low = top == -INFINITY ? INFINITY : top;  // least of the threads' greatest
+  float low = top > -INFINITY ? top : INFINITY;  // least of the threads' greatest
   const int threads = __syncthreads_count(top > -INFINITY);
   const int any_bad = __syncthreads_or(bad);
 #pragma unroll
@@ -613,10 +634,12 @@ __global__ void __launch_bounds__(kSaThreads) sample_kernel(const SampleArgs a) 
   const float top_p = a.top_p ? a.top_p[row_id] : a.top_p1;
   const float min_p = a.min_p ? a.min_p[row_id] : a.min_p1;
   const float u = a.u[row_id];
-  int level = 0;
   if (broken || top == -INFINITY) {
     if (rank == 0 && tid == 0) a.out[row_id] = -1;
-  } else if (!(temp > 0.f)) {
+    cluster.sync();  // (no CTA leaves while another may read its shared memory)
+    return;
+  }
+  if (!(temp > 0.f)) {
     // the first of the greatest
     int at = INT_MAX;
 #pragma unroll 1
@@ -639,237 +662,244 @@ __global__ void __launch_bounds__(kSaThreads) sample_kernel(const SampleArgs a) 
       for (int r = 0; r < ctas; ++r) at = min(at, cluster.map_shared_rank(&s->part, r)->index);
       a.out[row_id] = at;
     }
-  } else {
-    Row row;
-    row.top = top;
-    row.m = (double)top;
-    row.c32 = 46.166241308446829 / (double)temp;  // 32 * log2(e)
-    // 2^-46 and less rounds to no unit
-    row.floor_x = fmaxf((float)((double)top - 32.3 * (double)temp), -FLT_MAX);
-    // what min-p keeps, x - M >= T * log(min_p) (exp(x - M) would round to 1 near M): the least float
-    // that passes, found beside its estimate
-    Cut cut = {0u, 0, true};
-    if (min_p > 0.f) {
-      if (warp == 0) {
-        const double least_d = (double)temp * log((double)min_p);
-        const uint32_t mid = key_of((float)fmax((double)top + least_d, -(double)FLT_MAX));
-        const uint32_t probe = min(mid - 16 + lane, key_of(top));
-        const bool in = (double)of_key(probe) - row.m >= least_d || probe == key_of(top);
-        const uint32_t hit = __ballot_sync(0xffffffffu, in);
-        const uint32_t found = __shfl_sync(0xffffffffu, probe, max(__ffs((int)hit) - 1, 0));
-        if (lane == 0) s->min_key = hit ? found : key_of(top);
-      }
-      __syncthreads();
-      cut.key = s->min_key;
+    cluster.sync();
+    return;
+  }
+
+  Row row;
+  row.top = top;
+  row.m = (double)top;
+  row.c32 = 46.166241308446829 / (double)temp;  // 32 * log2(e)
+  // 2^-46 and less rounds to no unit
+  row.floor_x = fmaxf((float)((double)top - 32.3 * (double)temp), -FLT_MAX);
+  // what min-p keeps, x - M >= T * log(min_p) (exp(x - M) would round to 1 near M): the least float
+  // that passes, found beside its estimate
+  Cut cut = {0u, 0, true};
+  if (min_p > 0.f) {
+    if (warp == 0) {
+      const double least_d = (double)temp * log((double)min_p);
+      const uint32_t mid = key_of((float)fmax((double)top + least_d, -(double)FLT_MAX));
+      const uint32_t probe = min(mid - 16 + lane, key_of(top));
+      const bool in = (double)of_key(probe) - row.m >= least_d || probe == key_of(top);
+      const uint32_t hit = __ballot_sync(0xffffffffu, in);
+      const uint32_t found = __shfl_sync(0xffffffffu, probe, max(__ffs((int)hit) - 1, 0));
+      if (lane == 0) s->min_key = hit ? found : key_of(top);
     }
-    int64_t rank_of_tie = 0;  // ties before this CTA's (later: this warp's) tokens
-    uint64_t own = 0;         // kept mass of this CTA's tokens, where the values' counts tell it
-    bool counted = false;
-    if constexpr (sizeof(T) == 2) {
-      constexpr int kEach = 2 * Bits16<T>::kRegion / kSaThreads;
-      const Values bins = value_bins<T>(row);
-      int lump_n = 0;
-      uint64_t lump_m = 0;
+    __syncthreads();
+    cut.key = s->min_key;
+  }
+
+  int64_t ties_before = 0, own_ties = 0;  // tokens that equal the cut: before this CTA, and in it
+  uint64_t own = 0;                       // kept mass of this CTA's tokens
+  bool counted = false;                   // whether the values' counts tell these
+  [[maybe_unused]] Values bins = {};
+  if constexpr (sizeof(T) == 2) {
+    constexpr int kEach = kSaValueBins<T> / kSaThreads;
+    bins = value_bins<T>(row);
+    int lump_n = 0;
+    uint64_t lump_m = 0;
 #pragma unroll 1
-      for (int st = 0; st < steps; ++st) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(x + chunk_base + st * kSaStep + lane * 8);
-        const uint32_t pair[4] = {raw.x, raw.y, raw.z, raw.w};
+    for (int st = 0; st < steps; ++st) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(x + chunk_base + st * kSaStep + lane * 8);
+      const uint32_t pair[4] = {raw.x, raw.y, raw.z, raw.w};
+      uint32_t lumps = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          // (no key is above the greatest: the halves do not borrow)
-          const uint32_t below = bins.top * 0x10001u - keys16(pair[i >> 1]);
+      for (int i = 0; i < 8; ++i) {
+        // (no key is above the greatest: the halves do not borrow)
+        const uint32_t below = bins.top * 0x10001u - keys16(pair[i >> 1]);
+        const uint32_t d = i & 1 ? below >> 16 : below & 0xffff;
+        const int bin = value_bin<T>(bins, d);
+        if (bin >= 0) atomicAdd(&counts[bin], 1u);
+        else lumps |= 1u << i;
+      }
+      if (lumps) {
+#pragma unroll 1
+        for (; lumps; lumps &= lumps - 1) {
+          const int i = __ffs((int)lumps) - 1;
+          const uint32_t word = i < 4 ? (i < 2 ? raw.x : raw.y) : (i < 6 ? raw.z : raw.w);
+          const uint32_t below = bins.top * 0x10001u - keys16(word);
           const uint32_t d = i & 1 ? below >> 16 : below & 0xffff;
-          const int bin = value_bin<T>(bins, d);
-          if (bin >= 0) {
-            atomicAdd(&counts[bin >> 1], 1u << (16 * (bin & 1)));
-          } else if (d <= bins.top - bins.lowest) {
+          if (d <= bins.top - bins.lowest) {
             const float v = Bits16<T>::value(bins.top - d);
             ++lump_n;
             if (v >= row.floor_x) lump_m += weight(row, s->tab, v);
           }
         }
       }
-      const uint64_t own_lump_m = warp_sum(lump_m);
-      lump_n = __reduce_add_sync(0xffffffffu, lump_n);
-      if (lane == 0) {
-        s->w_ties[warp] = lump_n;
-        s->lump_mass[warp] = own_lump_m;
-      }
-      __syncthreads();
-      if (tid == 0) {
-        int n = 0;
-        uint64_t m = 0;
-        for (int w = 0; w < kSaWarps; ++w) n += s->w_ties[w], m += s->lump_mass[w];
-        s->part.lump_count = n;
-        s->part.lump_mass = m;
-      }
-      cluster.sync();
-      uint64_t lump_count = 0, lump_mass = 0;
-      for (int r = 0; r < ctas; ++r) {
-        lump_count += cluster.map_shared_rank(&s->part, r)->lump_count;
-        lump_mass += cluster.map_shared_rank(&s->part, r)->lump_mass;
-      }
-      // the sums of this thread's bins, of all CTAs and of this one
-      uint64_t count = 0, mass = 0, own_mass = 0;
-#pragma unroll 2
-      for (int i = 0; i < kEach; i += 2) {
-        const int word = (tid * kEach + i) >> 1;
-        uint32_t n[2] = {0, 0};
-        for (int r = 0; r < ctas; ++r) {
-          const uint32_t h = cluster.map_shared_rank(counts, r)[word];
-          n[0] += h & 0xffff;
-          n[1] += h >> 16;
-        }
-        const uint32_t mine = counts[word];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          if (n[j] == 0) continue;
-          const float v = Bits16<T>::value(bin_key<T>(bins, tid * kEach + i + j));
-          const uint64_t w = v >= row.floor_x ? weight(row, s->tab, v) : 0;
-          count += n[j];
-          mass += n[j] * w;
-          own_mass += (j ? mine >> 16 : mine & 0xffff) * w;
-        }
-      }
-      uint64_t all_count, all_mass;
-      uint64_t before_count = block_exclusive(count, s->scan, all_count);
-      uint64_t before_mass = block_exclusive(mass, s->scan, all_mass);
-      if (tid >= kSaThreads / 2) before_count += lump_count, before_mass += lump_mass;
-      all_count += lump_count;
-      all_mass += lump_mass;
-      counted = true;
-      Cut c = {0u, 0, true};
-      ValueCut vc;
-      if (k > 0 && (uint64_t)k < all_count) {
-        counted = value_cross<T, false>(cluster, s, counts, row, bins, count, mass, before_count,
-                                        before_mass, (uint64_t)k, 0.0, vc);
-        if (counted) {
-          const float v = Bits16<T>::value(vc.key16);
-          c = {key_of(v), k - (int64_t)vc.count, k - (int64_t)vc.count >= (int64_t)vc.group};
-          all_mass = vc.mass + (v >= row.floor_x ? c.ties * weight(row, s->tab, v) : 0);
-        }
-      }
-      if (counted && top_p < 1.f) {
-        const double target = fmax((double)top_p * (double)all_mass, 1.0);
-        counted = value_cross<T, true>(cluster, s, counts, row, bins, count, mass, before_count,
-                                       before_mass, 0, target, vc);
-        if (counted) {
-          const float v = Bits16<T>::value(vc.key16);
-          const int64_t r = kept_ties(target, vc.mass, weight(row, s->tab, v), vc.group);
-          c = tighter(c, {key_of(v), r, r >= (int64_t)vc.group});
-        }
-      }
-      if (counted) {
-        c = tighter(cut, c);
-        // a cut (of min-p) within the lump is left to the search
-        const uint32_t lump_hi = bins.top - bins.n1;  // its greatest key
-        const uint32_t lump_lo = bins.n2 ? bins.top - bins.off2 + 1 : bins.lowest;
-        const bool lump_in = lump_count > 0 && c.key <= key_of(Bits16<T>::value(lump_lo));
-        if (lump_count > 0 && !lump_in && c.key <= key_of(Bits16<T>::value(lump_hi))) counted = false;
-        if (counted) {
-          // this CTA's kept mass: bins above the cut, and its share of the ties
-          uint64_t m = 0;
-          const uint32_t last = bin_key<T>(bins, tid * kEach + kEach - 1);
-          if (last != 0 && key_of(Bits16<T>::value(last)) > c.key) {
-            m = own_mass;
-          } else if (count > 0) {
+    }
+    const uint64_t warp_lump_m = warp_sum(lump_m);
+    lump_n = __reduce_add_sync(0xffffffffu, lump_n);
+    if (lane == 0) {
+      s->w_ties[warp] = lump_n;
+      s->lump_mass[warp] = warp_lump_m;
+    }
+    __syncthreads();
+    if (tid == 0) {
+      int n = 0;
+      uint64_t m = 0;
+      for (int w = 0; w < kSaWarps; ++w) n += s->w_ties[w], m += s->lump_mass[w];
+      s->part.lump_count = n;
+      s->part.lump_mass = m;
+    }
+    cluster.sync();
+    uint64_t lump_count = 0, lump_mass = 0;
+    for (int r = 0; r < ctas; ++r) {
+      lump_count += cluster.map_shared_rank(&s->part, r)->lump_count;
+      lump_mass += cluster.map_shared_rank(&s->part, r)->lump_mass;
+    }
+    // the sums of this thread's bins, of all CTAs and of this one
+    uint64_t sums[2] = {0, 0}, before[2], all[2], own_mass = 0;
 #pragma unroll 1
-            for (int i = 0; i < kEach; ++i) {
-              const int bin = tid * kEach + i;
-              const uint32_t key16 = bin_key<T>(bins, bin);
-              const float v = Bits16<T>::value(key16);
-              if (key16 == 0 || key_of(v) < c.key) break;
-              int64_t n = (counts[bin >> 1] >> (16 * (bin & 1))) & 0xffff;
-              if (key_of(v) == c.key && !c.all_ties) {
-                int64_t ahead = 0;
-                for (int r = 0; r < rank; ++r)
-                  ahead += (cluster.map_shared_rank(counts, r)[bin >> 1] >> (16 * (bin & 1))) & 0xffff;
-                s->tie_base = ahead;
-                n = max((int64_t)0, min(n, c.ties - ahead));
-              }
-              if (n > 0 && v >= row.floor_x) m += n * weight(row, s->tab, v);
-            }
-          }
-          if (tid == 0 && lump_in) m += s->part.lump_mass;
-          block_exclusive(m, s->scan, own);
-          if (!c.all_ties) rank_of_tie = s->tie_base;
-          cut = c;
-        }
+    for (int i = 0; i < kEach; i += 4) {
+      const int bin = tid * kEach + i;
+      uint32_t n[4] = {0, 0, 0, 0};
+      for (int r = 0; r < ctas; ++r) {
+        const uint4 h = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(counts, r) + bin);
+        n[0] += h.x;
+        n[1] += h.y;
+        n[2] += h.z;
+        n[3] += h.w;
       }
-      if (!counted) {  // the histograms' place is taken by the search's
-        cluster.sync();
-        for (int i = tid; i < kSaHistBytes<T> / 4; i += kSaThreads) counts[i] = 0;
-        __syncthreads();
+      const uint4 mine = *reinterpret_cast<const uint4*>(counts + bin);
+      const uint32_t mine4[4] = {mine.x, mine.y, mine.z, mine.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (n[j] == 0) continue;
+        const float v = Bits16<T>::value(bin_key<T>(bins, bin + j));
+        const uint64_t w = v >= row.floor_x ? weight(row, s->tab, v) : 0;
+        sums[0] += n[j];
+        sums[1] += n[j] * w;
+        own_mass += mine4[j] * w;
       }
     }
-    if (!counted) {
-      uint64_t drop = 0;
-      if (k > 0 && k < a.vocab) {
-        // as many threads as `with` have a logit of at least `low`
-        const float from = k <= with ? low : least;
-        const Cut c = search<T, false>(cluster, s, hists, x, steps, chunk_base, row, key_of(from), k, 0.0, 0,
-                                       level);
-        if (c.key != 0 && !c.all_ties) {
-          const float value = of_key(c.key);
-          if (value >= row.floor_x)
-            drop = (s->held - (uint64_t)c.ties) * weight(row, s->tab, value);
+    block_exclusive<2>(sums, s->scan, before, all);
+    if (tid >= kSaThreads / 2) before[0] += lump_count, before[1] += lump_mass;
+    all[0] += lump_count;
+    all[1] += lump_mass;
+    counted = true;
+    Cut c = {0u, 0, true};
+    ValueCut vc;
+    if (k > 0 && (uint64_t)k < all[0]) {
+      counted = value_cross<T, false>(cluster, s, counts, row, bins, sums, before, (uint64_t)k, 0.0, vc);
+      if (counted) {
+        const float v = Bits16<T>::value(vc.key16);
+        c = {key_of(v), k - (int64_t)vc.count, k - (int64_t)vc.count >= (int64_t)vc.group};
+        all[1] = vc.mass + (v >= row.floor_x ? c.ties * weight(row, s->tab, v) : 0);
+      }
+    }
+    if (counted && top_p < 1.f) {
+      const double target = fmax((double)top_p * (double)all[1], 1.0);
+      counted = value_cross<T, true>(cluster, s, counts, row, bins, sums, before, 0, target, vc);
+      if (counted) {
+        const float v = Bits16<T>::value(vc.key16);
+        const int64_t r = kept_ties(target, vc.mass, weight(row, s->tab, v), vc.group);
+        c = tighter(c, {key_of(v), r, r >= (int64_t)vc.group});
+      }
+    }
+    if (counted) {
+      c = tighter(cut, c);
+      // a cut (of min-p) within the lump is left to the search
+      const uint32_t lump_hi = bins.top - bins.n1;  // its greatest key
+      const uint32_t lump_lo = bins.n2 ? bins.top - bins.off2 + 1 : bins.lowest;
+      const bool lump_in = lump_count > 0 && c.key <= key_of(Bits16<T>::value(lump_lo));
+      if (lump_count > 0 && !lump_in && c.key <= key_of(Bits16<T>::value(lump_hi))) counted = false;
+      if (counted) {
+        // this CTA's kept mass: bins above the cut, and its share of the ties
+        uint64_t m = 0;
+        const uint32_t last = bin_key<T>(bins, tid * kEach + kEach - 1);
+        if (last != 0 && key_of(Bits16<T>::value(last)) > c.key) {
+          m = own_mass;
+        } else if (sums[0] > 0) {
+#pragma unroll 1
+          for (int i = 0; i < kEach; ++i) {
+            const int bin = tid * kEach + i;
+            const uint32_t key16 = bin_key<T>(bins, bin);
+            const float v = Bits16<T>::value(key16);
+            if (key16 == 0 || key_of(v) < c.key) break;
+            int64_t n = counts[bin];
+            if (key_of(v) == c.key && !c.all_ties) {
+              int64_t ahead = 0;
+              for (int r = 0; r < rank; ++r) ahead += cluster.map_shared_rank(counts, r)[bin];
+              s->tie_base[0] = ahead;
+              s->tie_base[1] = n;
+              n = max((int64_t)0, min(n, c.ties - ahead));
+            }
+            if (n > 0 && v >= row.floor_x) m += n * weight(row, s->tab, v);
+          }
         }
-        __syncthreads();
-        const Cut before = cut;
+        if (tid == 0 && lump_in) m += s->part.lump_mass;
+        uint64_t unused;
+        block_exclusive<1>(&m, s->scan, &unused, &own);
+        if (!c.all_ties) {
+          ties_before = s->tie_base[0];
+          own_ties = s->tie_base[1];
+        }
         cut = c;
-        if (top_p < 1.f) {
-          const Cut p = search<T, true>(cluster, s, hists, x, steps, chunk_base, row,
-                                        max(c.key, key_of(row.floor_x)), 0, (double)top_p, drop, level);
-          cut = tighter(cut, p);
-        }
-        cut = tighter(before, cut);
-      } else if (top_p < 1.f) {
+      }
+    }
+    if (!counted) {  // the histograms' place is taken by the search's
+      cluster.sync();
+      for (int i = tid; i < kSaHistBytes<T> / 4; i += kSaThreads) counts[i] = 0;
+      __syncthreads();
+    }
+  }
+  if (!counted) {
+    int level = 0;
+    uint64_t drop = 0;
+    if (k > 0 && k < a.vocab) {
+      // as many threads as `with` have a logit of at least `low`
+      const float from = k <= with ? low : least;
+      const Cut c = search<T, false>(cluster, s, hists, x, steps, chunk_base, row, key_of(from), k, 0.0,
+                                     0, level);
+      if (c.key != 0 && !c.all_ties) {
+        const float value = of_key(c.key);
+        if (value >= row.floor_x) drop = (s->held - (uint64_t)c.ties) * weight(row, s->tab, value);
+      }
+      __syncthreads();
+      const Cut before = cut;
+      cut = c;
+      if (top_p < 1.f) {
         const Cut p = search<T, true>(cluster, s, hists, x, steps, chunk_base, row,
-                                      max(key_of(least), key_of(row.floor_x)), 0, (double)top_p, 0, level);
+                                      max(c.key, key_of(row.floor_x)), 0, (double)top_p, drop, level);
         cut = tighter(cut, p);
       }
+      cut = tighter(before, cut);
+    } else if (top_p < 1.f) {
+      const Cut p = search<T, true>(cluster, s, hists, x, steps, chunk_base, row,
+                                    max(key_of(least), key_of(row.floor_x)), 0, (double)top_p, 0, level);
+      cut = tighter(cut, p);
     }
+  }
 
-    // ties before this warp's tokens, where only some of them stay
-    auto count_ties = [&]() {
-      int n = 0;
+  // Which ties stay: those whose index in this CTA is below tie_end. Where that lies within the CTA, its
+  // 256-token steps' ties are counted first.
+  const int cells = kSaWarps * steps;
+  auto tie_counts = [&]() {  // of this thread's cell
 #pragma unroll 1
-      for (int st = 0; st < steps; ++st) {
-        float v[8];
-        load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
+    for (int st = 0; st < steps; ++st) {
+      float v[8];
+      load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
+      int n = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) n += key_of(v[i]) == cut.key;
-      }
+      for (int i = 0; i < 8; ++i) n += key_of(v[i]) == cut.key;
       n = __reduce_add_sync(0xffffffffu, n);
-      if (lane == 0) s->w_ties[warp] = n;
-      __syncthreads();
-      for (int w = 0; w < warp; ++w) rank_of_tie += s->w_ties[w];
-    };
-    if (!cut.all_ties && !counted) {
-      count_ties();
-      if (tid == 0) {
-        int t = 0;
-        for (int w = 0; w < kSaWarps; ++w) t += s->w_ties[w];
-        s->part.ties = t;
-      }
-      cluster.sync();
-      for (int r = 0; r < rank; ++r) rank_of_tie += cluster.map_shared_rank(&s->part, r)->ties;
+      if (lane == 0) s->step_mass[warp * steps + st] = (uint64_t)n;
     }
-    // kept weights of 8 tokens; `tie` counts the ties before this lane's
-    auto kept = [&](const float* v, int64_t tie, uint64_t* w) {
-      uint64_t sum = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t key = key_of(v[i]);
-        bool in = v[i] >= row.floor_x && key >= cut.key;
-        if (!cut.all_ties && key == cut.key) in = in && tie++ < cut.ties;
-        w[i] = in ? weight(row, s->tab, v[i]) : 0;
-        sum += w[i];
-      }
-      return sum;
-    };
-    // ties in the lanes before this one, and in the warp
-    auto ties_before = [&](const float* v, int& all) {
+    __syncthreads();
+    return tid < cells ? s->step_mass[tid] : 0;
+  };
+  auto find_tie_end = [&](int64_t keep, uint64_t in_cell) {  // place of tie number `keep`, 0 <= keep < own_ties
+    uint64_t before, all;
+    block_exclusive<1>(&in_cell, s->scan, &before, &all);
+    if (in_cell > 0 && (int64_t)before <= keep && keep < (int64_t)(before + in_cell)) {
+      s->bin = tid;
+      s->above = before;
+    }
+    __syncthreads();
+    const int cell = s->bin;
+    if (warp == cell / steps) {
+      float v[8];
+      load8<T>(x + cell * kSaStep + lane * 8, v);
       int n = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) n += key_of(v[i]) == cut.key;
@@ -879,101 +909,137 @@ __global__ void __launch_bounds__(kSaThreads) sample_kernel(const SampleArgs a) 
         const int o = __shfl_up_sync(0xffffffffu, inc, off);
         if (lane >= off) inc += o;
       }
-      all = __shfl_sync(0xffffffffu, inc, 31);
-      return inc - n;
-    };
-    const int cells = kSaWarps * steps;
-    int64_t first_tie = 0;
-    uint64_t cell = 0, before = 0, all = 0;  // a thread's cell: 256 tokens of the CTA
-    auto add_cells = [&]() {
-      first_tie = rank_of_tie;
+      int64_t at = (int64_t)s->above + inc - n;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (key_of(v[i]) == cut.key && at++ == keep) s->tie_end = cell * kSaStep + lane * 8 + i;
+    }
+    __syncthreads();
+    return s->tie_end;
+  };
+  int tie_end = INT_MAX;
+  if (!cut.all_ties && !counted) {
+    const uint64_t in_cell = tie_counts();
+    uint64_t before, all;
+    block_exclusive<1>(&in_cell, s->scan, &before, &all);
+    own_ties = (int64_t)all;
+    if (tid == 0) s->part.ties = (int)all;
+    cluster.sync();
+    for (int r = 0; r < rank; ++r) ties_before += cluster.map_shared_rank(&s->part, r)->ties;
+    const int64_t keep = cut.ties - ties_before;
+    if (keep < own_ties) tie_end = keep > 0 ? find_tie_end(keep, in_cell) : 0;
+  }
+  // kept weights of the 8 tokens at `at`
+  auto kept = [&](int at, uint64_t* w) {
+    uint64_t sum = 0;
+    float v[8];
+    load8<T>(x + at, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t key = key_of(v[i]);
+      const bool in = v[i] >= row.floor_x && (key > cut.key || (key == cut.key && at + i < tie_end));
+      w[i] = 0;
+      if (in) {
+        bool looked_up = false;
+        if constexpr (kSaTable<T>) {
+          if (counted) {
+            const uint32_t raw = reinterpret_cast<const uint16_t*>(x)[at + i];
+            const int bin = value_bin<T>(bins, bins.top - (keys16(raw) & 0xffff));
+            if (bin >= 0) {
+              w[i] = reinterpret_cast<const uint64_t*>(counts)[bin];
+              looked_up = true;
+            }
+          }
+        }
+        if (!looked_up) w[i] = weight(row, s->tab, v[i]);
+      }
+      sum += w[i];
+    }
+    return sum;
+  };
+  uint64_t cell = 0, before = 0, all = 0;  // a thread's cell: 256 tokens of the CTA
+  auto add_cells = [&]() {
 #pragma unroll 1
-      for (int st = 0; st < steps; ++st) {
-        float v[8];
-        uint64_t w[8];
-        load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
-        int in_step = 0;
-        const int64_t tie = rank_of_tie + (cut.all_ties ? 0 : ties_before(v, in_step));
-        const uint64_t sum = warp_sum(kept(v, tie, w));
-        rank_of_tie += in_step;
-        if (lane == 0) s->step_mass[warp * steps + st] = sum;
+    for (int st = 0; st < steps; ++st) {
+      uint64_t w[8];
+      const uint64_t sum = warp_sum(kept(chunk_base + st * kSaStep + lane * 8, w));
+      if (lane == 0) s->step_mass[warp * steps + st] = sum;
+    }
+    __syncthreads();
+    cell = tid < cells ? s->step_mass[tid] : 0;
+    block_exclusive<1>(&cell, s->scan, &before, &all);
+  };
+  if (!counted) {
+    add_cells();
+    own = all;
+  }
+  if (tid == 0) {
+    s->part.mass = own;
+    s->bin = -1;
+  }
+  cluster.sync();
+  uint64_t mass = 0, ahead = 0;
+  int last = 0;  // the last CTA with a kept token
+  for (int r = 0; r < ctas; ++r) {
+    const uint64_t m = cluster.map_shared_rank(&s->part, r)->mass;
+    if (r < rank) ahead += m;
+    if (m > 0) last = r;
+    mass += m;
+  }
+  cluster.sync();  // (all have read; from here on each CTA is on its own)
+  // the first CTA, cell and token whose running sum passes the target; the last kept one where none
+  // does (u = 1, NaN)
+  const double target = (double)u * (double)mass;
+  const bool none = !((double)mass > target);
+  auto passes = [&](uint64_t sum_before, uint64_t part) {
+    return (double)(sum_before + part) > target && (sum_before == 0 || !((double)sum_before > target));
+  };
+  if (own == 0 || !(none ? rank == last : passes(ahead, own))) return;
+  if (counted) {
+    if (!cut.all_ties) {
+      const int64_t keep = cut.ties - ties_before;
+      if (keep < own_ties) tie_end = keep > 0 ? find_tie_end(keep, tie_counts()) : 0;
+      if (tid == 0) s->bin = -1;
+    }
+    if constexpr (kSaTable<T>) {  // the values' weights, over their counts
+      __syncthreads();
+      for (int bin = tid; bin < kSaValueBins<T>; bin += kSaThreads) {
+        const uint32_t key16 = bin_key<T>(bins, bin);
+        const float v = Bits16<T>::value(key16);
+        if (key16 != 0 && v >= row.floor_x && key_of(v) >= cut.key)
+          reinterpret_cast<uint64_t*>(counts)[bin] = weight(row, s->tab, v);
       }
       __syncthreads();
-      cell = tid < cells ? s->step_mass[tid] : 0;
-      before = block_exclusive(cell, s->scan, all);
-    };
-    if (!counted) {
-      add_cells();
-      own = all;
     }
-    if (tid == 0) s->part.mass = own;
-    cluster.sync();
-    uint64_t mass = 0, ahead = 0;
-    int last = 0;  // the last CTA with a kept token
-    for (int r = 0; r < ctas; ++r) {
-      const uint64_t m = cluster.map_shared_rank(&s->part, r)->mass;
-      if (r < rank) ahead += m;
-      if (m > 0) last = r;
-      mass += m;
-    }
-    // the first cell whose running sum passes the target; the last kept one where none does (u = 1, NaN)
-    const double target = (double)u * (double)mass;
-    const bool none = !((double)mass > target);
-    if (counted && own > 0 &&
-        (none ? rank == last
-              : (double)(ahead + own) > target && (ahead == 0 || !((double)ahead > target)))) {
-      // this CTA alone looks for the token
-      if (!cut.all_ties) count_ties();
-      add_cells();
-    }
-    if (tid == 0) s->bin = -1;
-    __syncthreads();
-    if (cell > 0) {
-      const bool hit = (double)(ahead + before + cell) > target && !((double)(ahead + before) > target);
-      const bool first_cell = ahead + before == 0 && (double)0 > target;  // (u below 0)
-      if (none ? rank == last && before + cell == all : hit || first_cell) {
-        s->bin = tid;
-        s->above = ahead + before;
-      }
-    }
-    __syncthreads();
-    if (s->bin >= 0 && warp == s->bin / steps) {
-      const int st = s->bin % steps;
-      float v[8];
-      uint64_t w[8];
-      int64_t tie = first_tie;
-      if (!cut.all_ties) {
-        int in_warp = 0;
-        for (int i = 0; i <= st; ++i) {
-          load8<T>(x + chunk_base + i * kSaStep + lane * 8, v);
-          const int lanes = ties_before(v, in_warp);
-          tie += i < st ? in_warp : lanes;
-        }
-      }
-      load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
-      const uint64_t sum = kept(v, tie, w);
-      uint64_t inc = sum;
+    add_cells();
+  }
+  if (cell > 0 && (none ? before + cell == all : passes(ahead + before, cell))) {
+    s->bin = tid;
+    s->above = ahead + before;
+  }
+  __syncthreads();
+  if (s->bin < 0 || warp != s->bin / steps) return;
+  const int at0 = s->bin * kSaStep + lane * 8;
+  uint64_t w[8];
+  const uint64_t sum = kept(at0, w);
+  uint64_t inc = sum;
 #pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const uint64_t o = __shfl_up_sync(0xffffffffu, inc, off);
-        if (lane >= off) inc += o;
-      }
-      uint64_t run = s->above + inc - sum;
-      int at = none ? -1 : INT_MAX;
+  for (int off = 1; off < 32; off <<= 1) {
+    const uint64_t o = __shfl_up_sync(0xffffffffu, inc, off);
+    if (lane >= off) inc += o;
+  }
+  uint64_t run = s->above + inc - sum;
+  int at = none ? -1 : INT_MAX;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        run += w[i];
-        const int id = base + chunk_base + st * kSaStep + lane * 8 + i;
-        if (w[i] > 0) {
-          if (none) at = max(at, id);
-          else if ((double)run > target) at = min(at, id);
-        }
-      }
-      at = none ? __reduce_max_sync(0xffffffffu, at) : __reduce_min_sync(0xffffffffu, at);
-      if (lane == 0) a.out[row_id] = at;
+  for (int i = 0; i < 8; ++i) {
+    run += w[i];
+    if (w[i] > 0) {
+      if (none) at = max(at, base + at0 + i);
+      else if ((double)run > target) at = min(at, base + at0 + i);
     }
   }
-  cluster.sync();  // (no CTA leaves while another may read its shared memory)
+  at = none ? __reduce_max_sync(0xffffffffu, at) : __reduce_min_sync(0xffffffffu, at);
+  if (lane == 0) a.out[row_id] = at;
 }
 
 template <typename T>
@@ -1013,9 +1079,11 @@ extern "C" int fi_sample_tokens(const void* logits, const float* u, const float*
   const int size = dtype == FI_DTYPE_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(logits) % size != 0)
     return fail(FI_ERR_ALIGNMENT, "fi_sample_tokens: logits not aligned to their type");
-  // as few CTAs a row as its tokens allow, more where there are too few rows for two CTAs an SM
+  // as few CTAs a row as its tokens allow (bf16: 32768 each, else 16384: two CTAs an SM), more where there are too
+  // few rows for two CTAs an SM
   int ctas = 1;
-  while (ctas < kSaMaxCluster && ((int64_t)ctas * kSaWarps * kSaSteps * kSaStep < vocab ||
+  const int64_t most = (int64_t)kSaWarps * kSaSteps * kSaStep / (dtype == FI_DTYPE_BF16 ? 1 : 2);
+  while (ctas < kSaMaxCluster && (ctas * most < vocab ||
                                   (rows * ctas < 2 * sm_count() &&
                                    (int64_t)ctas * kSaWarps * kSaStep < vocab)))
     ctas *= 2;
