@@ -65,7 +65,7 @@ SIGNATURES = {
     "fi_paged_chunk": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
                                       _i64, _i64, _i64, _i64, _i64, _i64, _i64p, _i64p, _i64p,
                                       _i64p, _i64p, _f32, _f32, _i64, _i64, _vp, _sz, _vp, _vp]),
-    "fi_paged_tree_workspace_size": (_sz, [_i64, _i64, _i64, _i64]),
+    "fi_paged_tree_workspace_size": (_sz, [_i64, _i64, _i64]),
     "fi_paged_tree": (ctypes.c_int, [_vp] * 12 + [_i64] * 9 + [_i64p] * 7 + [_f32, _f32, _i64, _i64, _i64,
                                                                             _vp, _sz, _vp, _vp]),
     "fi_attention_mass_workspace_size": (_sz, []),

@@ -40,7 +40,7 @@
 
 #include <type_traits>
 
-#include "chunk_common.cuh"
+#include "paged_chunk.cuh"
 #include "quant8.cuh"
 
 namespace fi {
@@ -56,9 +56,6 @@ constexpr int kCkConvertBar = 14;
 constexpr int kCkScaleSlots = 4;
 constexpr int kCkStages = 2;
 constexpr int kCkTeardownBar = 15;
-constexpr int kCkMaxBatch = 2048;    // sequences per launch
-constexpr int kCkMaxUnits = 4608;    // token units per launch (per KV head)
-constexpr int kCkNarrow = 32;        // rows up to which a unit runs transposed
 constexpr float kCkRescale = 8.0f;   // log2 units of growth of the max before O is rescaled
 constexpr int kCkEmuPairs = 1;       // of 8 column pairs, exp2 on the FMA pipe
 // Steps that a unit's start and end are worth: with 0 and 0 / 1 and 2 / 3 and 2 / 4 and 3, 64 single
@@ -81,11 +78,6 @@ struct alignas(16) CkUnit {
   int valid;           // 0: no unit is left
 };
 static_assert(sizeof(CkUnit) == 64, "read as four 16-byte words");
-
-// The unit whose first part a CTA holds when the rest lies in the next CTAs.
-struct CkJoin {
-  int valid, last_cta, token, hk, rows[2], pad[2];
-};
 
 struct CkBarriers {
   uint64_t q_full[2], q_empty[2];
@@ -116,42 +108,8 @@ constexpr int kCkPBytes = kCkNarrow * 256;  // P^T of a transposed unit: 32 rows
 static_assert(kCkNarrow == 32, "a column per lane where rows are summed");
 static_assert(2 * kCkPBytes <= kChunkTileBytes, "P of both warpgroups in one query tile");
 
-struct ChunkParams {
-  ChunkBatch b;
-  ScoreForm f;
-  void* o;
-  int64_t os[2];
-  float* lse;  // [total, hq] or null
-  // [cta][first, last unit], then rows_cap rows of 128: as they are (narrow), or 32 rows' 4 values
-  // side by side (wide, whose threads have a row each)
-  float* ws_o;
-  float* ws_lse;  // [cta][first, last unit][rows_cap], log2 domain
-  CkJoin* join;   // [cta]
-  int rows_cap;
-  int unit_tokens;  // tokens of a unit: two tiles, or those of kCkNarrow rows
-  int split_rows;   // sequences of at most so many rows are the narrow kernel's, others the wide's
-  int o_wide;       // rows of o are 32-byte aligned
-  int late_wait;    // the kernel before on the stream is the other one of this call
-  const float* scale[2];  // of k and v, with 8-bit codes
-  int64_t ss[2][3];       // page, head, slot
-  int* err;
-};
-
 __device__ __forceinline__ int ck_tile(const CkUnit& u, int j) {
   return j < u.np ? j : u.lo + (j - u.np);
-}
-
-// Key tiles that the unit of tokens [t0, t1) of a sequence visits: [0, np) for the prefix and
-// [lo, lo + n - np). A unit that sees nothing visits one (all of it masked).
-__device__ __forceinline__ void ck_tiles(const ChunkBatch& p, const ChunkSeq& s, int t0, int t1,
-                                         int& np, int& lo, int& n) {
-  // (a tree's token may see any new token, and stands at the first new slot or behind it)
-  const int p0 = s.pos0 + (p.tree ? 0 : t0), p1 = s.pos0 + t1 - 1;
-  const int end = p.tree ? s.keys : min(s.keys, max(p1 + 1, s.prefix));
-  const int hi = end > 0 ? (end - 1) / kChunkTile : 0;
-  lo = p.window ? min(max(p0 - p.window + 1, 0) / kChunkTile, hi) : 0;
-  np = min((s.prefix + kChunkTile - 1) / kChunkTile, lo);
-  n = np + hi - lo + 1;
 }
 
 // The scheduler (one warp): walks the CTA's part of the line and hands its units to the other
@@ -1422,12 +1380,14 @@ static int launch_codes(const CUtensorMap& tq, const CUtensorMap& tk, const CUte
 template <typename T>
 static int launch_chunk(const CUtensorMap& tq_n, const CUtensorMap& tq_w, const CUtensorMap& tk,
                         const CUtensorMap& tv, const ChunkParams* narrow, const ChunkParams* wide,
-                        int64_t codes, cudaStream_t st) {
+                        const CodePages& pages, int code_rows, int64_t codes, cudaStream_t st) {
   int r = FI_OK;
-  if (codes == FI_DTYPE_I8) {
-    r = launch_codes<T, CodeI8>(tq_w, tk, tv, *wide, st);
-  } else if (codes == FI_DTYPE_E4M3) {
-    r = launch_codes<T, CodeE4M3>(tq_w, tk, tv, *wide, st);
+  if (codes == FI_DTYPE_I8 || codes == FI_DTYPE_E4M3) {
+    const int64_t dtype = std::is_same_v<T, __half> ? FI_DTYPE_F16 : FI_DTYPE_BF16;
+    if (narrow) r = launch_narrow_codes(*narrow, pages, dtype, codes, code_rows, st);
+    if (r == FI_OK && wide)
+      r = codes == FI_DTYPE_I8 ? launch_codes<T, CodeI8>(tq_w, tk, tv, *wide, st)
+                               : launch_codes<T, CodeE4M3>(tq_w, tk, tv, *wide, st);
   } else {
     if (narrow) r = launch_form<T, true>(tq_n, tk, tv, *narrow, st);
     if (r == FI_OK && wide) r = launch_form<T, false>(tq_w, tk, tv, *wide, st);
@@ -1460,14 +1420,12 @@ static size_t ck_workspace(ChunkParams* p, uint8_t* ws, int rows_cap) {
 static bool ck_all_narrow(int64_t total, int64_t group) { return total * group <= kCkNarrow; }
 
 // Workspace of a call: a part for each kernel that it may launch.
-static size_t ck_workspace_size(int64_t total_tokens, int64_t num_q_heads, int64_t num_kv_heads,
-                                bool codes) {
+static size_t ck_workspace_size(int64_t total_tokens, int64_t num_q_heads, int64_t num_kv_heads) {
   if (total_tokens <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads ||
       num_q_heads % num_kv_heads != 0 || num_q_heads / num_kv_heads > 64 ||
       total_tokens > (1 << 28))
     return 0;
   const size_t narrow = ck_workspace(nullptr, nullptr, kCkNarrow);
-  if (codes) return ck_workspace(nullptr, nullptr, 2 * kChunkTile);
   if (ck_all_narrow(total_tokens, num_q_heads / num_kv_heads)) return narrow;
   return narrow + ck_workspace(nullptr, nullptr, 2 * kChunkTile);
 }
@@ -1515,7 +1473,10 @@ static int paged_chunk(const char* what, const void* q, const void* k_cache, con
   // when it has nothing to do. One sequence with more is the wide kernel's. Other batches may hold
   // both.
   const bool codes = extra.cache_dtype != dtype;
-  const int64_t per_unit = !codes && p.b.group <= kCkNarrow ? kCkNarrow / p.b.group : 0;
+  // Over codes a narrow unit has 16 rows where that is enough for the average sequence, else 32.
+  const int64_t per16 = codes && p.b.group <= 16 ? 16 / p.b.group : 0;
+  const bool few = per16 > 0 && total_tokens <= batch * per16;
+  const int64_t per_unit = few ? per16 : p.b.group <= kCkNarrow ? kCkNarrow / p.b.group : 0;
   const bool use_narrow = per_unit > 0 && (batch > 1 || total_tokens <= per_unit);
   const bool use_wide =
       per_unit == 0 || total_tokens > batch * per_unit || total_tokens - batch >= kCkManyNew;
@@ -1532,7 +1493,7 @@ static int paged_chunk(const char* what, const void* q, const void* k_cache, con
                 "%s o: needs a 16-byte aligned base, unit innermost stride and other "
                 "strides multiple of 8",
                 what);
-  const size_t need = ck_workspace_size(total_tokens, num_q_heads, num_kv_heads, codes);
+  const size_t need = ck_workspace_size(total_tokens, num_q_heads, num_kv_heads);
   if (!workspace || workspace_bytes < need)
     return fail(FI_ERR_WORKSPACE, "%s: workspace of %zu bytes, needs %zu", what,
                 workspace ? workspace_bytes : (size_t)0, need);
@@ -1543,11 +1504,26 @@ static int paged_chunk(const char* what, const void* q, const void* k_cache, con
   ChunkParams n = p;  // the narrow kernel's
   n.b.tile_tokens = per_unit > 0 ? (int)per_unit : 1;
   CUtensorMap tq_n = {}, tq_w = {}, tk, tv;
-  if (use_narrow && (r = chunk_q_map(&tq_n, type, q, n.b, q_strides, what)) != FI_OK)
+  if (use_narrow && !codes && (r = chunk_q_map(&tq_n, type, q, n.b, q_strides, what)) != FI_OK)
     return r;
   if (use_wide && (r = chunk_q_map(&tq_w, type, q, p.b, q_strides, what)) != FI_OK)
     return r;
+  CodePages pages = {};
   if (codes) {
+    pages.q = q;
+    pages.pool[0] = static_cast<const uint8_t*>(k_cache);
+    pages.pool[1] = static_cast<const uint8_t*>(v_cache);
+    for (int i = 0; i < 2; ++i) pages.qs[i] = q_strides[i];
+    for (int i = 0; i < 3; ++i) {
+      pages.st[0][i] = kc_strides[i];
+      pages.st[1][i] = vc_strides[i];
+    }
+    if (q_strides[2] != 1 || !aligned16(q) || !stride_ok(total_tokens, q_strides[0]) ||
+        !stride_ok(num_q_heads, q_strides[1]))
+      return fail(FI_ERR_ALIGNMENT,
+                  "%s q: needs a 16-byte aligned base, unit innermost stride and other strides "
+                  "multiple of 8",
+                  what);
     if ((r = chunk_code_map(&tk, k_cache, p.b, kc_strides, what)) != FI_OK) return r;
     if ((r = chunk_code_map(&tv, v_cache, p.b, vc_strides, what)) != FI_OK) return r;
     for (int kv = 0; kv < 2; ++kv) {
@@ -1572,7 +1548,7 @@ static int paged_chunk(const char* what, const void* q, const void* k_cache, con
     n = p;
     n.b = nb;
   }
-  if (!codes) ws += ck_workspace(&n, ws, kCkNarrow);
+  ws += ck_workspace(&n, ws, kCkNarrow);
   if (use_wide) ck_workspace(&p, ws, 2 * kChunkTile);
   n.unit_tokens = (int)per_unit;
   n.split_rows = use_wide ? kCkNarrow : 0x7fffffff;
@@ -1583,15 +1559,17 @@ static int paged_chunk(const char* what, const void* q, const void* k_cache, con
   const ChunkParams* np = use_narrow ? &n : nullptr;
   const ChunkParams* wp = use_wide ? &p : nullptr;
   return dtype == FI_DTYPE_F16
-             ? launch_chunk<__half>(tq_n, tq_w, tk, tv, np, wp, extra.cache_dtype, st)
-             : launch_chunk<__nv_bfloat16>(tq_n, tq_w, tk, tv, np, wp, extra.cache_dtype, st);
+             ? launch_chunk<__half>(tq_n, tq_w, tk, tv, np, wp, pages, few ? 16 : 32,
+                                    extra.cache_dtype, st)
+             : launch_chunk<__nv_bfloat16>(tq_n, tq_w, tk, tv, np, wp, pages, few ? 16 : 32,
+                                           extra.cache_dtype, st);
 }
 
 }  // namespace fi
 
 extern "C" size_t fi_paged_chunk_workspace_size(int64_t total_tokens, int64_t num_q_heads,
                                                 int64_t num_kv_heads) {
-  return fi::ck_workspace_size(total_tokens, num_q_heads, num_kv_heads, false);
+  return fi::ck_workspace_size(total_tokens, num_q_heads, num_kv_heads);
 }
 
 extern "C" int fi_paged_chunk(const void* q, const void* k_cache, const void* v_cache, void* o,
@@ -1616,9 +1594,8 @@ extern "C" int fi_paged_chunk(const void* q, const void* k_cache, const void* v_
 }
 
 extern "C" size_t fi_paged_tree_workspace_size(int64_t total_tokens, int64_t num_q_heads,
-                                               int64_t num_kv_heads, int64_t cache_dtype) {
-  return fi::ck_workspace_size(total_tokens, num_q_heads, num_kv_heads,
-                               cache_dtype == FI_DTYPE_I8 || cache_dtype == FI_DTYPE_E4M3);
+                                               int64_t num_kv_heads) {
+  return fi::ck_workspace_size(total_tokens, num_q_heads, num_kv_heads);
 }
 
 extern "C" int fi_paged_tree(const void* q, const void* k_cache, const void* v_cache,

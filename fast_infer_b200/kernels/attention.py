@@ -472,17 +472,13 @@ def paged_chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
 
 
 @functools.lru_cache(maxsize=4096)
-def _tree_workspace(device_index: int, total: int, num_q_heads: int, num_kv_heads: int,
-                    cache: int) -> int:
-    return int(_lib.load().fi_paged_tree_workspace_size(total, num_q_heads, num_kv_heads, cache))
+def _tree_workspace(device_index: int, total: int, num_q_heads: int, num_kv_heads: int) -> int:
+    return int(_lib.load().fi_paged_tree_workspace_size(total, num_q_heads, num_kv_heads))
 
 
-def paged_tree_workspace_bytes(total_tokens: int, num_q_heads: int, num_kv_heads: int,
-                               cache_dtype: torch.dtype = torch.float16) -> int:
-    """Workspace bytes ``paged_tree_attention`` needs for these sizes and pages of ``cache_dtype``
-    (current device)."""
-    return int(_lib.load().fi_paged_tree_workspace_size(total_tokens, num_q_heads, num_kv_heads,
-                                                        POOL_DTYPES[cache_dtype]))
+def paged_tree_workspace_bytes(total_tokens: int, num_q_heads: int, num_kv_heads: int) -> int:
+    """Workspace bytes ``paged_tree_attention`` needs for these sizes (current device)."""
+    return int(_lib.load().fi_paged_tree_workspace_size(total_tokens, num_q_heads, num_kv_heads))
 
 
 def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -548,8 +544,7 @@ def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         with with_device(device):
             if workspace is None:
                 workspace = torch.empty(
-                    _tree_workspace(device.index, total, num_q_heads, num_kv_heads,
-                                    POOL_DTYPES[k_cache.dtype]),
+                    _tree_workspace(device.index, total, num_q_heads, num_kv_heads),
                     dtype=torch.uint8, device=device)
             elif workspace.device != device or not workspace.is_contiguous():
                 raise ValueError("workspace must be contiguous on q's device")

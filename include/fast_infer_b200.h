@@ -237,7 +237,7 @@ int fi_paged_chunk(const void* q, const void* k_cache, const void* v_cache, void
  * All else, limits and workspace too (fi_paged_tree_workspace_size), as in fi_paged_chunk.
  */
 size_t fi_paged_tree_workspace_size(int64_t total_tokens, int64_t num_q_heads,
-                                    int64_t num_kv_heads, int64_t cache_dtype);
+                                    int64_t num_kv_heads);
 int fi_paged_tree(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
                   const float* v_scale, void* o, float* lse, const int32_t* block_table,
                   const int32_t* cu_seqlens, const int32_t* context_lens, const int32_t* tree_mask,

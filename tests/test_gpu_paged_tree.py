@@ -265,7 +265,7 @@ def test_strides_out_workspace_and_other_stream(cuda_device, device_checks, kind
         scales["v_scale"].copy_(st["vs"])
     out = torch.full((total, 9, 128), 7.0, dtype=torch.float16, device=dev)[:, 1:7]
     from fast_infer_b200.kernels.attention import paged_tree_workspace_bytes
-    ws = torch.empty(paged_tree_workspace_bytes(total, 6, 2, st["k"].dtype), dtype=torch.uint8, device=dev)
+    ws = torch.empty(paged_tree_workspace_bytes(total, 6, 2), dtype=torch.uint8, device=dev)
     stream = torch.cuda.Stream(dev)
     stream.wait_stream(torch.cuda.current_stream(dev))
     with torch.cuda.stream(stream):
@@ -321,7 +321,7 @@ def test_workspace_is_as_large_as_what_is_written(cuda_device, device_checks, ki
     """The bytes behind the workspace that the sizes ask for stay as they were."""
     from fast_infer_b200.kernels.attention import paged_tree_workspace_bytes
     st = make(cuda_device, seqs, 6, 2, torch.float16, kind, seed=7, spread=3)
-    need = paged_tree_workspace_bytes(st["q"].shape[0], 6, 2, st["k"].dtype)
+    need = paged_tree_workspace_bytes(st["q"].shape[0], 6, 2)
     ws = torch.full((need + (64 << 20),), 171, dtype=torch.uint8, device=cuda_device)
     check(st, kind, torch.float16, workspace=ws[:need])
     assert (ws[need:] == 171).all()
