@@ -1473,10 +1473,12 @@ static int paged_chunk(const char* what, const void* q, const void* k_cache, con
   // when it has nothing to do. One sequence with more is the wide kernel's. Other batches may hold
   // both.
   const bool codes = extra.cache_dtype != dtype;
-  // Over codes a narrow unit has 16 rows where that is enough for the average sequence, else 32.
-  const int64_t per16 = codes && p.b.group <= 16 ? 16 / p.b.group : 0;
-  const bool few = per16 > 0 && total_tokens <= batch * per16;
-  const int64_t per_unit = few ? per16 : p.b.group <= kCkNarrow ? kCkNarrow / p.b.group : 0;
+  // Over codes a narrow unit has 8 or 16 rows where that is enough for the average sequence, else 32.
+  int unit_rows = kCkNarrow;
+  if (codes)
+    for (int rows = 16; rows >= 8; rows /= 2)
+      if (total_tokens <= batch * (rows / p.b.group)) unit_rows = rows;
+  const int64_t per_unit = unit_rows / p.b.group;
   const bool use_narrow = per_unit > 0 && (batch > 1 || total_tokens <= per_unit);
   const bool use_wide =
       per_unit == 0 || total_tokens > batch * per_unit || total_tokens - batch >= kCkManyNew;
@@ -1559,9 +1561,9 @@ static int paged_chunk(const char* what, const void* q, const void* k_cache, con
   const ChunkParams* np = use_narrow ? &n : nullptr;
   const ChunkParams* wp = use_wide ? &p : nullptr;
   return dtype == FI_DTYPE_F16
-             ? launch_chunk<__half>(tq_n, tq_w, tk, tv, np, wp, pages, few ? 16 : 32,
+             ? launch_chunk<__half>(tq_n, tq_w, tk, tv, np, wp, pages, unit_rows,
                                     extra.cache_dtype, st)
-             : launch_chunk<__nv_bfloat16>(tq_n, tq_w, tk, tv, np, wp, pages, few ? 16 : 32,
+             : launch_chunk<__nv_bfloat16>(tq_n, tq_w, tk, tv, np, wp, pages, unit_rows,
                                            extra.cache_dtype, st);
 }
 

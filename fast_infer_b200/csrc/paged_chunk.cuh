@@ -56,7 +56,7 @@ struct CodePages {
   int64_t qs[2];
   int64_t st[2][3];        // page, slot, head
 };
-// Rows of a unit there: 16 or 32 (one or two tiles of the product).
+// Rows of a unit there: 8, 16 or 32 (columns of the products).
 int launch_narrow_codes(const ChunkParams& p, const CodePages& pages, int64_t dtype,
                         int64_t cache_dtype, int rows, cudaStream_t st);
 

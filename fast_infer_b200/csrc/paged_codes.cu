@@ -8,10 +8,11 @@
 //   does, would move 96 KB there each way; so here the codes go from shared memory to registers as they are
 //   and become fragments of m16n8k16 products (fp16, which holds every code of either type exactly): 16 bytes
 //   of a key, and of a value row, are a lane's own, for dims and keys may be permuted alike on both sides of
-//   a product. Rows of a unit are the product's 16 (or twice 16) rows.
-// * A warp is on its own: it takes 16 of each tile's 128 keys, has a ring of stages filled by cp.async three
-//   tiles ahead (across units too), and a running softmax of its own. The 8 warps meet once a unit. Work is cut
-//   into equal parts of one line as in paged_chunk.cu, and units that several CTAs hold are joined likewise.
+//   a product. Both products are transposed (S^T = K Q^T, O^T = V^T P^T), so that keys and dims fill the 16
+//   rows of a product and the unit's rows its 8 columns: 1, 2 or 4 such groups of rows.
+// * A warp is on its own: it takes 16 of a tile's 128 keys, has a ring of stages filled by cp.async ahead of
+//   it (across units too), and a running softmax of its own. The warps meet once a unit. Work is cut into equal
+//   parts of one line as in paged_chunk.cu, and units that several CTAs hold are joined likewise.
 // * Scales stay out of the products: ks multiplies scores in fp32. vs_j cannot multiply codes (fp16) nor
 //   P alone (vs may be 1e-6 or 1e30), so P' = p vs 2^(m - m') carries it, with m' a running maximum
 //   of s + log2(vs): P' is at most 2^8, and the greatest of a row's is at least one at some key. A sum
@@ -27,25 +28,31 @@
 
 namespace fi {
 
-constexpr int kPcWarps = 8;
-constexpr int kPcThreads = kPcWarps * 32;
-constexpr int kPcKeys = kChunkTile / kPcWarps;  // keys of a tile that a warp takes
-constexpr int kPcStages = 4;
+constexpr int kPcKeys = 16;                     // keys of a tile that a warp takes: 8 warps have one
 constexpr int kPcPad = 3;                       // steps that a unit's start and end are worth on the line
 constexpr int kPcStageBytes = 2 * kPcKeys * 128 + 2 * kPcKeys * 4;
 constexpr float kPcTop = 256.f;                 // p and P' up to which maxima stay as they are
+static_assert(kPcStageBytes % 16 == 0, "16-byte copies");
 
+// With 8 rows a warp has the registers for 16 of them an SM, whose halves take alternate tiles.
+template <int kNT>
+struct PcShape {
+  static constexpr int kWarps = kNT == 1 ? 16 : 8;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kStages = kNT == 1 ? 2 : 4;
+};
+
+template <int kNT>
 struct PcShared {
-  float part[kPcWarps][16][128];  // O of the warps, 16 rows at a time
-  uint8_t ring[kPcWarps][kPcStages][kPcStageBytes];
-  float m[kPcWarps][kCkNarrow], mv[kPcWarps][kCkNarrow], l[kPcWarps][kCkNarrow];
-  float inv[kCkNarrow];
-  uint32_t warp_sums[kPcWarps];
+  static constexpr int kWarps = PcShape<kNT>::kWarps;
+  float part[8][8][128];  // O of 8 warps, 8 rows at a time
+  alignas(16) uint8_t ring[kWarps][PcShape<kNT>::kStages][kPcStageBytes];
+  float m[kWarps][8 * kNT], mv[kWarps][8 * kNT], l[kWarps][8 * kNT];
+  float inv[8 * kNT];
+  uint32_t warp_sums[kWarps];
   uint32_t unit_off[kCkMaxBatch + 1];
   uint32_t work[kCkMaxUnits + 1];
 };
-static_assert(sizeof(PcShared) + 16 <= 227 * 1024, "shared memory");
-static_assert(kPcStageBytes % 16 == 0, "16-byte copies");
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0)
@@ -79,23 +86,24 @@ __device__ __forceinline__ int pc_tile(const PcCursor& c, int j) {
 
 // Fills in the cursor's unit, whose steps from `at` on are this CTA's; skips units of which it has no key
 // tile. `w`: place of the unit's step `at` on the line.
-__device__ __forceinline__ void pc_enter(const ChunkParams& p, const PcShared* s, uint32_t units,
+__device__ __forceinline__ void pc_enter(const ChunkParams& p, const uint32_t* unit_off,
+                                         const uint32_t* work, uint32_t units,
                                          int64_t total, int active, int64_t end, int64_t& w, int at,
                                          PcCursor& c) {
   while (true) {
     c.valid = w < end;
     if (!c.valid) return;
-    if (c.e < (int)s->unit_off[c.b] || c.e >= (int)s->unit_off[c.b + 1]) {
+    if (c.e < (int)unit_off[c.b] || c.e >= (int)unit_off[c.b + 1]) {
       if (c.e == 0) c.b = -1;
-      do ++c.b; while ((int)s->unit_off[c.b + 1] <= c.e);
+      do ++c.b; while ((int)unit_off[c.b + 1] <= c.e);
     }
     c.q = chunk_seq(p.b, c.b);
-    const int len = (int)(s->work[c.e + 1] - s->work[c.e]);
+    const int len = (int)(work[c.e + 1] - work[c.e]);
     const int stop = len - at <= end - w ? len : at + (int)(end - w);
     c.last_cta = stop == len ? (int)blockIdx.x : (int)(((w - at + len) * active - 1) / total);
     const int64_t next = w + stop - at;
     if (stop > kPcPad) {
-      c.t0 = (c.e - (int)s->unit_off[c.b]) * p.unit_tokens;
+      c.t0 = (c.e - (int)unit_off[c.b]) * p.unit_tokens;
       int tiles;
       ck_tiles(p.b, c.q, c.t0, min(c.t0 + p.unit_tokens, c.q.n), c.np, c.lo, tiles);
       c.n = len - kPcPad;
@@ -109,10 +117,11 @@ __device__ __forceinline__ void pc_enter(const ChunkParams& p, const PcShared* s
     if (++c.e == (int)units) c.e = 0, ++c.hk;
   }
 }
-__device__ __forceinline__ void pc_next(const ChunkParams& p, const PcShared* s, uint32_t units,
+__device__ __forceinline__ void pc_next(const ChunkParams& p, const uint32_t* unit_off,
+                                         const uint32_t* work, uint32_t units,
                                         int64_t total, int active, int64_t end, int64_t& w, PcCursor& c) {
   if (++c.e == (int)units) c.e = 0, ++c.hk;
-  pc_enter(p, s, units, total, active, end, w, 0, c);
+  pc_enter(p, unit_off, work, units, total, active, end, w, 0, c);
 }
 
 template <typename T>
@@ -126,13 +135,17 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
   return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
 
-template <typename T, typename Code, bool kCap, int kMT>
-__global__ void __launch_bounds__(kPcThreads, 1)
+template <typename T, typename Code, bool kCap, int kNT>
+__global__ void __launch_bounds__(PcShape<kNT>::kThreads, 1)
     paged_codes_kernel(const ChunkParams p, const CodePages pages) {
+  constexpr int kWarps = PcShape<kNT>::kWarps, kThreads = PcShape<kNT>::kThreads;
+  constexpr int kStages = PcShape<kNT>::kStages, kTiles = kWarps / 8;
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  PcShared* s = reinterpret_cast<PcShared*>(smem_raw);
+  PcShared<kNT>* s = reinterpret_cast<PcShared<kNT>*>(smem_raw);
+  const uint32_t *unit_off = s->unit_off, *work = s->work;
   const ChunkBatch& pb = p.b;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int slice = warp & 7, half = warp >> 3;  // keys of a tile; which tiles
   const int cta = blockIdx.x;
 
   // the line of work: units of each sequence, then key tiles of each unit, both as sums
@@ -140,7 +153,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   grid_dep_launch();
   if (tid == 0) s->unit_off[0] = s->work[0] = 0;
 #pragma unroll 1
-  for (int b = tid; b < pb.batch; b += kPcThreads) {
+  for (int b = tid; b < pb.batch; b += kThreads) {
     const ChunkSeq q = chunk_seq(pb, b);
     if (q.bad && cta == 0) set_error(p.err, FI_DEVERR_CONTEXT_LEN);
     s->unit_off[b + 1] = q.n * pb.group <= p.split_rows
@@ -150,13 +163,13 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   __syncthreads();
   block_scan(s->unit_off, pb.batch, s->warp_sums);
   // cu that is not ascending could name more units than the host counted: those are dropped
-  const uint32_t units = min(s->unit_off[pb.batch], (uint32_t)kCkMaxUnits);
-  if (units != s->unit_off[pb.batch] && tid == 0) set_error(p.err, FI_DEVERR_CONTEXT_LEN);
+  const uint32_t units = min(unit_off[pb.batch], (uint32_t)kCkMaxUnits);
+  if (units != unit_off[pb.batch] && tid == 0) set_error(p.err, FI_DEVERR_CONTEXT_LEN);
 #pragma unroll 1
-  for (int e = tid; e < (int)units; e += kPcThreads) {
-    const int b = last_le(s->unit_off, pb.batch, (uint32_t)e);
+  for (int e = tid; e < (int)units; e += kThreads) {
+    const int b = last_le(unit_off, pb.batch, (uint32_t)e);
     const ChunkSeq q = chunk_seq(pb, b);
-    const int t0 = (e - (int)s->unit_off[b]) * p.unit_tokens;
+    const int t0 = (e - (int)unit_off[b]) * p.unit_tokens;
     int np, lo, n;
     ck_tiles(pb, q, t0, min(t0 + p.unit_tokens, q.n), np, lo, n);
     s->work[e + 1] = (uint32_t)(n + kPcPad);
@@ -164,7 +177,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   __syncthreads();
   block_scan(s->work, (int)units, s->warp_sums);
 
-  const uint32_t per_head = s->work[units];
+  const uint32_t per_head = work[units];
   const int64_t total = (int64_t)per_head * pb.hk;
   const int active = (int)(total < (int64_t)gridDim.x ? total : gridDim.x);
   const int64_t begin = cta < active ? total * cta / active : 0;
@@ -174,25 +187,32 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   if (begin < end) {
     c.hk = (int)(begin / per_head);
     const uint32_t r = (uint32_t)(begin - (int64_t)c.hk * per_head);
-    c.e = last_le(s->work, (int)units, r);
-    c.b = last_le(s->unit_off, pb.batch, (uint32_t)c.e);
-    pc_enter(p, s, units, total, active, end, w_use, (int)(r - s->work[c.e]), c);
+    c.e = last_le(work, (int)units, r);
+    c.b = last_le(unit_off, pb.batch, (uint32_t)c.e);
+    pc_enter(p, unit_off, work, units, total, active, end, w_use, (int)(r - work[c.e]), c);
     w_load = w_use;
   }
   PcCursor ld = c;  // where the loads are
-  int ld_j = ld.j0;
+  int ld_j = ld.j0 + half;
+  auto next_tile = [&]() {  // units of one tile have none for the second half
+    while (ld.valid && ld_j >= ld.j1) {
+      pc_next(p, unit_off, work, units, total, active, end, w_load, ld);
+      ld_j = ld.j0 + half;
+    }
+  };
+  next_tile();
   // the page of the next load, looked up one step ahead
   auto look_up = [&]() {
-    return ld.valid ? chunk_page(pb, ld.b, ld.q.keys, pc_tile(ld, ld_j), warp >> 2) : 0;
+    return ld.valid ? chunk_page(pb, ld.b, ld.q.keys, pc_tile(ld, ld_j), slice >> 2) : 0;
   };
   int ld_page = look_up();
   const uint32_t ring = smem_u32(&s->ring[warp][0][0]);
+  uint32_t held_bits = 0;  // of the stages: whether their page exists
   // 16 keys of K, V and their scales: a lane copies 16 bytes of rows lane / 8 + 4 i. Pieces of 16 bytes are
   // placed so that the reads below meet no bank twice (K by the row's low bit, V by its low three).
-  uint32_t held_bits = 0;  // of the stages: whether their page exists
   auto load = [&](int stage) {
     if (ld.valid) {
-      const int tile = pc_tile(ld, ld_j), key0 = tile * kChunkTile + warp * kPcKeys;
+      const int tile = pc_tile(ld, ld_j), key0 = tile * kChunkTile + slice * kPcKeys;
       const bool held = ld_page != pb.num_blocks;
       if (!held && key0 < ld.q.keys && lane == 0) set_error(p.err, FI_DEVERR_BAD_BLOCK);
       const int slot0 = key0 & (kChunkPage - 1), row0 = lane >> 3, piece = lane & 7;
@@ -215,162 +235,152 @@ __global__ void __launch_bounds__(kPcThreads, 1)
       cp_async4(dst + 2 * kPcKeys * 128 + lane * 4,
                 p.scale[kv] + page * p.ss[kv][0] + ld.hk * p.ss[kv][1] + (slot0 + row) * p.ss[kv][2],
                 held && key0 + row < ld.q.keys);
-      if (++ld_j == ld.j1) {
-        pc_next(p, s, units, total, active, end, w_load, ld);
-        ld_j = ld.j0;
-      }
+      ld_j += kTiles;
+      next_tile();
       ld_page = look_up();
     }
     cp_async_commit();
   };
 #pragma unroll 1
-  for (int i = 0; i < kPcStages - 1; ++i) load(i);
+  for (int i = 0; i < kStages - 1; ++i) load(i);
 
   CkJoin join = {};
-  int step = 0;
+  int stage = 0;
 #pragma unroll 1
-  for (; c.valid; pc_next(p, s, units, total, active, end, w_use, c)) {
+  for (; c.valid; pc_next(p, unit_off, work, units, total, active, end, w_use, c)) {
     const int tokens = min(c.q.n - c.t0, p.unit_tokens), rows = tokens * pb.group;
     const int token0 = c.q.start + c.t0;
-    // Q as fragments: the four dims of step i are those of word i of a lane's 32 codes of a key
-    uint32_t qa[kMT][8][4];
-    float rs[kMT][2];  // what a row's products are multiplied with
-    int tok[kMT][2];   // its token of the unit
+    // Q as fragments: the four dims of step i are those of word i of a lane's 32 codes of a key; this lane's
+    // row of group n is 8 n + g
+    uint32_t qb[kNT][8][2];
+    float rs[kNT][2];  // what the products of rows 8 n + 2 t (+ 1) are multiplied with
 #pragma unroll
-    for (int m = 0; m < kMT; ++m)
+    for (int n = 0; n < kNT; ++n) {
+      const int row = n * 8 + g;
+      const bool live = row < rows;
+      const int64_t token = token0 + (live ? row / pb.group : 0);
+      const int head = c.hk * pb.group + (live ? row % pb.group : 0);
+      const T* src = static_cast<const T*>(pages.q) + token * pages.qs[0] + head * pages.qs[1] + t * 16;
+      uint4 raw[4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = m * 16 + h * 8 + g;
-        const bool live = row < rows;
-        tok[m][h] = live ? row / pb.group : 0;
-        const int head = c.hk * pb.group + (live ? row % pb.group : 0);
-        const T* src = static_cast<const T*>(pages.q) + (int64_t)(token0 + tok[m][h]) * pages.qs[0] +
-                       head * pages.qs[1] + t * 16;
-        uint4 raw[4];
+      for (int i = 0; i < 4; ++i)
+        raw[i] = live ? *reinterpret_cast<const uint4*>(src + (i >> 1) * 64 + (i & 1) * 8)
+                      : make_uint4(0, 0, 0, 0);
+      float unit = 1.f;
+      if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          raw[i] = live ? *reinterpret_cast<const uint4*>(src + (i >> 1) * 64 + (i & 1) * 8)
-                        : make_uint4(0, 0, 0, 0);
-        float unit = 1.f;
-        if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-          float top = 0.f;
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 f = unpack2<T>(x[j]);
-              top = fmax3f(top, fabsf(f.x), fabsf(f.y));
-            }
-          }
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          // 2^e of the greatest, e in [-125, 125]: its inverse is normal too
-          const int e = min(max((int)(__float_as_uint(top) >> 23), 2), 252);
-          unit = __uint_as_float((uint32_t)e << 23);
-          const float to = __uint_as_float((uint32_t)(254 - e) << 23);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t* x = reinterpret_cast<uint32_t*>(&raw[i]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 f = unpack2<T>(x[j]);
-              x[j] = pack_half2(f.x * to, f.y * to);
-            }
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack2<T>(x[j]);
+            top = fmax3f(top, fabsf(f.x), fabsf(f.y));
           }
         }
-        rs[m][h] = unit * (kCap ? p.f.cap_in : p.f.scale_log2);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^e of the greatest, e in [-125, 125]: its inverse is normal too
+        const int e = min(max((int)(__float_as_uint(top) >> 23), 2), 252);
+        unit = __uint_as_float((uint32_t)e << 23);
+        const float to = __uint_as_float((uint32_t)(254 - e) << 23);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {  // word i: 4 dims, 8 bytes of `raw`
-          const uint4& r = raw[i >> 1];
-          qa[m][i][h] = i & 1 ? r.z : r.x;
-          qa[m][i][2 + h] = i & 1 ? r.w : r.y;
+        for (int i = 0; i < 4; ++i) {
+          uint32_t* x = reinterpret_cast<uint32_t*>(&raw[i]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack2<T>(x[j]);
+            x[j] = pack_half2(f.x * to, f.y * to);
+          }
         }
       }
-    float o[kMT][16][4], l[kMT][2], mx[kMT][2], mv[kMT][2], neg[kMT][2], fv[kMT][2];
+      unit *= kCap ? p.f.cap_in : p.f.scale_log2;
 #pragma unroll
-    for (int m = 0; m < kMT; ++m) {
+      for (int h = 0; h < 2; ++h) rs[n][h] = __shfl_sync(0xffffffffu, unit, (2 * t + h) * 4);
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
+      for (int i = 0; i < 8; ++i) {  // word i: 4 dims, 8 bytes of `raw`
+        const uint4& r = raw[i >> 1];
+        qb[n][i][0] = i & 1 ? r.z : r.x;
+        qb[n][i][1] = i & 1 ? r.w : r.y;
+      }
+    }
+    float o[kNT][8][4], l[kNT][2], mx[kNT][2], mv[kNT][2], neg[kNT][2], fv[kNT][2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[m][i][e] = 0.f;
+    for (int n = 0; n < kNT; ++n) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         // no score yet: any finite one gives 2^FLT_MAX, past every bound, and so does any weight of V
-        l[m][h] = 0.f;
-        mx[m][h] = mv[m][h] = -INFINITY;
-        neg[m][h] = fv[m][h] = FLT_MAX;
+        l[n][h] = 0.f;
+        mx[n][h] = mv[n][h] = -INFINITY;
+        neg[n][h] = fv[n][h] = FLT_MAX;
       }
     }
     const int past = c.q.pos0;  // the sequence's first new slot
 #pragma unroll 1
-    for (int j = c.j0; j < c.j1; ++j, ++step) {
-      cp_async_wait<kPcStages - 2>();
+    for (int j = c.j0 + half; j < c.j1; j += kTiles) {
+      cp_async_wait<kStages - 2>();
       __syncwarp();  // all lanes' copies are there, and all have left the stage that is filled next
-      const bool page_ok = (held_bits >> (step % kPcStages)) & 1u;
-      load((step + kPcStages - 1) % kPcStages);
-      const uint8_t* st = s->ring[warp][step % kPcStages];
-      const int tile = pc_tile(c, j), key0 = tile * kChunkTile + warp * kPcKeys;
-      // ------------------------------------------------------------ scores
-      float sc[kMT][2][4];
+      const bool page_ok = (held_bits >> stage) & 1u;
+      const uint8_t* st = s->ring[warp][stage];
+      load(stage == 0 ? kStages - 1 : stage - 1);
+      stage = stage == kStages - 1 ? 0 : stage + 1;
+      const int tile = pc_tile(c, j), key0 = tile * kChunkTile + slice * kPcKeys;
+      // ------------------------------------------------ scores of keys g, g + 8 and rows 2 t, 2 t + 1
+      float sc[kNT][4];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const uint8_t* krow = st + (n * 8 + g) * 128;
-        const uint4 lo = *reinterpret_cast<const uint4*>(krow + ((t ^ ((g & 1) << 2)) << 4));
-        const uint4 hi = *reinterpret_cast<const uint4*>(krow + (((t + 4) ^ ((g & 1) << 2)) << 4));
-        const uint32_t kw[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      for (int n = 0; n < kNT; ++n)
 #pragma unroll
-        for (int m = 0; m < kMT; ++m)
+        for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[m][n][e] = 0.f;
+      for (int hf = 0; hf < 2; ++hf) {
+        const int at = ((t + 4 * hf) ^ ((g & 1) << 2)) << 4;
+        const uint4 ka = *reinterpret_cast<const uint4*>(st + g * 128 + at);
+        const uint4 kb = *reinterpret_cast<const uint4*>(st + (g + 8) * 128 + at);
+        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint32_t b0, b1;
-          Code::decode4(kw[i], b0, b1);
+        for (int i = 0; i < 4; ++i) {
+          uint32_t a0, a1, a2, a3;
+          Code::decode4(wa[i], a0, a2);
+          Code::decode4(wb[i], a1, a3);
 #pragma unroll
-          for (int m = 0; m < kMT; ++m)
-            mma_16816(sc[m][n], qa[m][i][0], qa[m][i][1], qa[m][i][2], qa[m][i][3], b0, b1);
+          for (int n = 0; n < kNT; ++n)
+            mma_16816(sc[n], a0, a1, a2, a3, qb[n][hf * 4 + i][0], qb[n][hf * 4 + i][1]);
         }
       }
       const float* scales = reinterpret_cast<const float*>(st + 2 * kPcKeys * 128);
-      float2 vs[2];
+      const float ks[2] = {scales[g], scales[g + 8]};
+      const float vs[2] = {scales[kPcKeys + g], scales[kPcKeys + g + 8]};
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const float2 ks = *reinterpret_cast<const float2*>(scales + n * 8 + 2 * t);
-        vs[n] = *reinterpret_cast<const float2*>(scales + kPcKeys + n * 8 + 2 * t);
+      for (int n = 0; n < kNT; ++n)
 #pragma unroll
-        for (int m = 0; m < kMT; ++m)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[m][n][e] *= (e & 1 ? ks.y : ks.x) * rs[m][e >> 1];
-      }
+        for (int e = 0; e < 4; ++e) sc[n][e] *= ks[e >> 1] * rs[n][e & 1];
       if constexpr (kCap) {
         float big = 0.f;
 #pragma unroll
-        for (int m = 0; m < kMT; ++m)
+        for (int n = 0; n < kNT; ++n)
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(sc[m][n][e]));
+          for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(sc[n][e]));
         const bool small = __all_sync(0xffffffffu, big <= 1.f);
 #pragma unroll
-        for (int m = 0; m < kMT; ++m)
+        for (int n = 0; n < kNT; ++n)
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x = sc[m][n][e];
-              sc[m][n][e] =
-                  p.f.cap_log2 * (small || fabsf(x) <= 1.f ? tanh_poly(x) : tanh_any(x));
-            }
+          for (int e = 0; e < 4; ++e) {
+            const float x = sc[n][e];
+            sc[n][e] = p.f.cap_log2 * (small || fabsf(x) <= 1.f ? tanh_poly(x) : tanh_any(x));
+          }
       }
       // hidden keys: new tokens' (by position, or the tree's bits), those a window leaves behind, those past
       // the context or without a page (whose copies are zeros)
       if (!page_ok || key0 + kPcKeys > min(past, c.q.keys) || pb.window) {
 #pragma unroll
-        for (int m = 0; m < kMT; ++m)
+        for (int n = 0; n < kNT; ++n)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int token = token0 + tok[m][h];
+            const int row = min(n * 8 + 2 * t + h, rows - 1), tok = row / pb.group, token = token0 + tok;
             uint32_t see = page_ok ? low_bits(c.q.keys - key0, 0) : 0u;
             if (pb.tree) {
               uint32_t before = low_bits(past - key0, 0), inner = 0;
@@ -380,112 +390,111 @@ __global__ void __launch_bounds__(kPcThreads, 1)
               if (key0 < past) inner &= ~low_bits(past - key0, 0);
               see &= before | inner;
             } else {
-              const int pos = past + c.t0 + tok[m][h];
+              const int pos = past + c.t0 + tok;
               see &= low_bits(pos + 1 - key0, 0);
               if (pb.window) see &= ~low_bits(pos - pb.window + 1 - key0, 0);
             }
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                if (!((see >> (n * 8 + 2 * t + e)) & 1u)) sc[m][n][h * 2 + e] = -INFINITY;
+            if (!((see >> g) & 1u)) sc[n][h] = -INFINITY;
+            if (!((see >> (g + 8)) & 1u)) sc[n][2 + h] = -INFINITY;
           }
       }
       // -------------------------------------------------- weights; maxima move where one passes 2^8
-      uint32_t pa[kMT][4];
-      float ps[kMT][2];
+      uint32_t pb0[kNT], pb1[kNT];
+      float ps[kNT][2];
 #pragma unroll 1
       for (bool moved = false;; moved = true) {
         float top = 0.f;
 #pragma unroll
-        for (int m = 0; m < kMT; ++m) {
-          ps[m][0] = ps[m][1] = 0.f;
+        for (int n = 0; n < kNT; ++n) {
+          float w[4], v[4];
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float p0 = fast_exp2(sc[m][n][2 * h] + neg[m][h]);
-              const float p1 = fast_exp2(sc[m][n][2 * h + 1] + neg[m][h]);
-              const float v0 = p0 * vs[n].x * fv[m][h], v1 = p1 * vs[n].y * fv[m][h];
-              top = fmax3f(fmax3f(top, p0, p1), v0, v1);
-              ps[m][h] += p0 + p1;
-              pa[m][n * 2 + h] = pack_half2(v0, v1);
-            }
+          for (int e = 0; e < 4; ++e) {
+            w[e] = fast_exp2(sc[n][e] + neg[n][e & 1]);
+            v[e] = w[e] * vs[e >> 1] * fv[n][e & 1];
+          }
+          top = fmax3f(fmax3f(top, w[0], w[1]), w[2], w[3]);
+          top = fmax3f(fmax3f(top, v[0], v[1]), v[2], v[3]);
+          ps[n][0] = w[0] + w[2];
+          ps[n][1] = w[1] + w[3];
+          pb0[n] = pack_half2(v[0], v[1]);
+          pb1[n] = pack_half2(v[2], v[3]);
         }
         if (moved || __all_sync(0xffffffffu, top <= kPcTop)) break;
+        const float lv[2] = {__log2f(vs[0]), __log2f(vs[1])};
 #pragma unroll
-        for (int m = 0; m < kMT; ++m)
+        for (int n = 0; n < kNT; ++n)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float a = fmaxf(fmaxf(sc[m][0][2 * h], sc[m][0][2 * h + 1]),
-                            fmaxf(sc[m][1][2 * h], sc[m][1][2 * h + 1]));
-            float b = fmaxf(fmaxf(sc[m][0][2 * h] + __log2f(vs[0].x), sc[m][0][2 * h + 1] + __log2f(vs[0].y)),
-                            fmaxf(sc[m][1][2 * h] + __log2f(vs[1].x), sc[m][1][2 * h + 1] + __log2f(vs[1].y)));
+            float a = fmaxf(sc[n][h], sc[n][2 + h]);
+            float b = fmaxf(sc[n][h] + lv[0], sc[n][2 + h] + lv[1]);
 #pragma unroll
-            for (int off = 1; off < 4; off <<= 1) {
+            for (int off = 4; off < 32; off <<= 1) {
               a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, off));
               b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, off));
             }
-            a = fmaxf(a, mx[m][h]);
-            b = fmaxf(b, mv[m][h]);
-            const float fl = mx[m][h] == -INFINITY ? 0.f : fast_exp2(mx[m][h] - a);
-            const float fo = mv[m][h] == -INFINITY ? 0.f : fast_exp2(mv[m][h] - b);
-            mx[m][h] = a;
-            mv[m][h] = b;
-            neg[m][h] = a == -INFINITY ? FLT_MAX : -a;
-            fv[m][h] = b == -INFINITY ? FLT_MAX : fast_exp2(a - b);
-            l[m][h] *= fl;
+            a = fmaxf(a, mx[n][h]);
+            b = fmaxf(b, mv[n][h]);
+            const float fl = mx[n][h] == -INFINITY ? 0.f : fast_exp2(mx[n][h] - a);
+            const float fo = mv[n][h] == -INFINITY ? 0.f : fast_exp2(mv[n][h] - b);
+            mx[n][h] = a;
+            mv[n][h] = b;
+            neg[n][h] = a == -INFINITY ? FLT_MAX : -a;
+            fv[n][h] = b == -INFINITY ? FLT_MAX : fast_exp2(a - b);
+            l[n][h] *= fl;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              o[m][i][2 * h] *= fo;
-              o[m][i][2 * h + 1] *= fo;
+            for (int i = 0; i < 8; ++i) {
+              o[n][i][h] *= fo;
+              o[n][i][2 + h] *= fo;
             }
           }
       }
 #pragma unroll
-      for (int m = 0; m < kMT; ++m) {
-        l[m][0] += ps[m][0];
-        l[m][1] += ps[m][1];
+      for (int n = 0; n < kNT; ++n) {
+        l[n][0] += ps[n][0];
+        l[n][1] += ps[n][1];
+        pb0[n] = movmatrix_t(pb0[n]);  // rows by keys, as the second product takes P
+        pb1[n] = movmatrix_t(pb1[n]);
       }
-      // ------------------------------------------------------------ P' V
+      // ------------------------------------------------------------ V^T P': dims 16 g + 2 i (+ 1) of step i
       const uint8_t* vrow = st + kPcKeys * 128;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {  // (two of the four words of each row's 16 codes at a time)
+      for (int hf = 0; hf < 2; ++hf) {  // (two of the four words of each row's 16 codes at a time)
         uint2 v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int row = 2 * t + (i & 1) + (i >> 1) * 8;
-          v[i] = *reinterpret_cast<const uint2*>(vrow + row * 128 + ((g ^ (row & 7)) << 4) + half * 8);
+          v[i] = *reinterpret_cast<const uint2*>(vrow + row * 128 + ((g ^ (row & 7)) << 4) + hf * 8);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint32_t a = i ? v[0].y : v[0].x, b = i ? v[1].y : v[1].x;
           const uint32_t x = i ? v[2].y : v[2].x, y = i ? v[3].y : v[3].x;
-          uint32_t b0[4], b1[4];  // of dims 0 .. 3 of this word
-          Code::decode4(__byte_perm(a, b, 0x5140), b0[0], b0[1]);
-          Code::decode4(__byte_perm(a, b, 0x7362), b0[2], b0[3]);
-          Code::decode4(__byte_perm(x, y, 0x5140), b1[0], b1[1]);
-          Code::decode4(__byte_perm(x, y, 0x7362), b1[2], b1[3]);
+          uint32_t lo[4], hi[4];  // pairs of keys 2 t, 2 t + 1 and 2 t + 8, 2 t + 9 for the word's 4 dims
+          Code::decode4(__byte_perm(a, b, 0x5140), lo[0], lo[1]);
+          Code::decode4(__byte_perm(a, b, 0x7362), lo[2], lo[3]);
+          Code::decode4(__byte_perm(x, y, 0x5140), hi[0], hi[1]);
+          Code::decode4(__byte_perm(x, y, 0x7362), hi[2], hi[3]);
 #pragma unroll
-          for (int d = 0; d < 4; ++d)
+          for (int d = 0; d < 2; ++d)
 #pragma unroll
-            for (int m = 0; m < kMT; ++m)
-              mma_16816(o[m][half * 8 + i * 4 + d], pa[m][0], pa[m][1], pa[m][2], pa[m][3], b0[d], b1[d]);
+            for (int n = 0; n < kNT; ++n)
+              mma_16816(o[n][hf * 4 + i * 2 + d], lo[2 * d], lo[2 * d + 1], hi[2 * d], hi[2 * d + 1],
+                        pb0[n], pb1[n]);
         }
       }
     }
     // ---------------------------------------------------------------- the warps meet
 #pragma unroll
-    for (int m = 0; m < kMT; ++m)
+    for (int n = 0; n < kNT; ++n)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        l[m][h] += __shfl_xor_sync(0xffffffffu, l[m][h], 1);
-        l[m][h] += __shfl_xor_sync(0xffffffffu, l[m][h], 2);
-        const int row = m * 16 + h * 8 + g;
-        if (t == 0) {
-          s->m[warp][row] = mx[m][h];
-          s->mv[warp][row] = mv[m][h];
-          s->l[warp][row] = l[m][h];
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], off);
+        if (g == 0) {
+          const int row = n * 8 + 2 * t + h;
+          s->m[warp][row] = mx[n][h];
+          s->mv[warp][row] = mv[n][h];
+          s->l[warp][row] = l[n][h];
         }
       }
     __syncthreads();
@@ -494,13 +503,13 @@ __global__ void __launch_bounds__(kPcThreads, 1)
     if (tid < rows) {  // a thread per row: its sum, and what O is multiplied with
       float a = -INFINITY, b = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kPcWarps; ++w) {
+      for (int w = 0; w < kWarps; ++w) {
         a = fmaxf(a, s->m[w][tid]);
         b = fmaxf(b, s->mv[w][tid]);
       }
       float sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < kPcWarps; ++w) {
+      for (int w = 0; w < kWarps; ++w) {
         const float lw = s->l[w][tid], mw = s->m[w][tid];
         sum += mw == -INFINITY ? lw : lw * exp2f(mw - a);  // (lw is 0 there, or NaN)
       }
@@ -515,54 +524,64 @@ __global__ void __launch_bounds__(kPcThreads, 1)
       }
     }
 #pragma unroll
-    for (int m = 0; m < kMT; ++m) {
-      if (m * 16 >= rows) break;
+    for (int n = 0; n < kNT; ++n) {
+      if (n * 8 >= rows) break;
+      float f[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int row = h * 8 + g;
         float b = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kPcWarps; ++w) b = fmaxf(b, s->mv[w][m * 16 + row]);
-        const float f = mv[m][h] == -INFINITY ? 0.f : fast_exp2(mv[m][h] - b);
-        // a lane has dims [32 t, 32 t + 32) of its rows, written in an order that spreads the banks
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int q4 = i ^ (lane & 7);
-          float4 x;
-          float* xf = reinterpret_cast<float*>(&x);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            // (a select over the registers: q4 is the lane's own)
-            float pick = 0.f;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const float v = o[m][(k & 3) * 4 + e][2 * h + (k >> 2)];
-              pick = q4 == k ? v : pick;
-            }
-            xf[e] = pick * f;
-          }
-          *reinterpret_cast<float4*>(&s->part[warp][row][32 * t + q4 * 4]) = x;
-        }
+        for (int w = 0; w < kWarps; ++w) b = fmaxf(b, s->mv[w][n * 8 + 2 * t + h]);
+        f[h] = mv[n][h] == -INFINITY ? 0.f : fast_exp2(mv[n][h] - b);
       }
-      __syncthreads();
+      // a lane has dims [16 g, 16 g + 16) of rows 2 t and 2 t + 1, 4 at a time in an order that spreads the
+      // banks; of 16 warps the second 8 go first, and the others add theirs
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int at = tid + i * kPcThreads, row = at >> 5, col = (at & 31) * 4, r = m * 16 + row;
+      for (int turn = 0; turn < kTiles; ++turn) {
+        if (half == kTiles - 1 - turn) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int q4 = i ^ t;
+              float x[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                x[e] = 0.f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)  // (a select over the registers: q4 is the lane's own)
+                  x[e] = q4 == k ? o[n][2 * k + (e >> 1)][2 * (e & 1) + h] * f[h] : x[e];
+              }
+              float4* to = reinterpret_cast<float4*>(&s->part[slice][2 * t + h][16 * g + q4 * 4]);
+              if (turn > 0) {
+                const float4 was = *to;
+                x[0] += was.x;
+                x[1] += was.y;
+                x[2] += was.z;
+                x[3] += was.w;
+              }
+              *to = make_float4(x[0], x[1], x[2], x[3]);
+            }
+        }
+        __syncthreads();
+      }
+      if (tid < 256) {
+        const int row = tid >> 5, col = (tid & 31) * 4, r = n * 8 + row;
         if (r < rows) {
           float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int w = 0; w < kPcWarps; ++w) {
+          for (int w = 0; w < 8; ++w) {
             const float4 x = *reinterpret_cast<const float4*>(&s->part[w][row][col]);
             sum.x += x.x;
             sum.y += x.y;
             sum.z += x.z;
             sum.w += x.w;
           }
-          const float f = s->inv[r];
-          sum.x *= f;
-          sum.y *= f;
-          sum.z *= f;
-          sum.w *= f;
+          const float f1 = s->inv[r];
+          sum.x *= f1;
+          sum.y *= f1;
+          sum.z *= f1;
+          sum.w *= f1;
           if (whole) {
             const int64_t token = token0 + r / pb.group;
             const int head = c.hk * pb.group + r % pb.group;
@@ -589,26 +608,31 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   cp_async_wait<0>();
 }
 
-template <typename T, typename Code, bool kCap, int kMT>
+template <typename T, typename Code, bool kCap, int kNT>
 static int launch_one(const ChunkParams& p, const CodePages& pages, cudaStream_t st) {
-  constexpr auto kernel = paged_codes_kernel<T, Code, kCap, kMT>;
+  constexpr auto kernel = paged_codes_kernel<T, Code, kCap, kNT>;
+  static_assert(sizeof(PcShared<kNT>) <= 227 * 1024, "shared memory");
   static DeviceOnce once;
   cudaError_t e = once.run([] {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)sizeof(PcShared));
+                                (int)sizeof(PcShared<kNT>));
   });
   if (e != cudaSuccess) return cuda_fail(e, "fi_paged_tree: kernel set-up");
-  e = launch_pdl(kernel, dim3((unsigned)sm_count()), dim3(kPcThreads), sizeof(PcShared), st, p, pages);
+  e = launch_pdl(kernel, dim3((unsigned)sm_count()), dim3(PcShape<kNT>::kThreads),
+                 sizeof(PcShared<kNT>), st, p, pages);
   return e == cudaSuccess ? FI_OK : cuda_fail(e, "fi_paged_tree: launch");
 }
 
+template <typename T, typename Code, bool kCap>
+static int launch_rows(const ChunkParams& p, const CodePages& pages, int rows, cudaStream_t st) {
+  return rows <= 8    ? launch_one<T, Code, kCap, 1>(p, pages, st)
+         : rows <= 16 ? launch_one<T, Code, kCap, 2>(p, pages, st)
+                      : launch_one<T, Code, kCap, 4>(p, pages, st);
+}
 template <typename T, typename Code>
 static int launch_form(const ChunkParams& p, const CodePages& pages, int rows, cudaStream_t st) {
-  if (p.f.cap_log2 > 0.f)
-    return rows > 16 ? launch_one<T, Code, true, 2>(p, pages, st)
-                     : launch_one<T, Code, true, 1>(p, pages, st);
-  return rows > 16 ? launch_one<T, Code, false, 2>(p, pages, st)
-                   : launch_one<T, Code, false, 1>(p, pages, st);
+  return p.f.cap_log2 > 0.f ? launch_rows<T, Code, true>(p, pages, rows, st)
+                            : launch_rows<T, Code, false>(p, pages, rows, st);
 }
 
 int launch_narrow_codes(const ChunkParams& p, const CodePages& pages, int64_t dtype,
