@@ -55,6 +55,7 @@ struct CodePages {
   const uint8_t* pool[2];  // k, v
   int64_t qs[2];
   int64_t st[2][3];        // page, slot, head
+  int stages, max_units;   // (set at the launch)
 };
 // Rows of a unit there: 8, 16 or 32 (columns of the products).
 int launch_narrow_codes(const ChunkParams& p, const CodePages& pages, int64_t dtype,

@@ -39,19 +39,18 @@ template <int kNT>
 struct PcShape {
   static constexpr int kWarps = kNT == 1 ? 16 : 8;
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kStages = kNT == 1 ? 2 : 4;
 };
+constexpr int kPcMaxStages = 5;
+constexpr int kPcMaxShared = 227 * 1024;
 
+// Then the ring, [warp][stage], and the line: unit_off [batch + 1], work [units + 1].
 template <int kNT>
 struct PcShared {
   static constexpr int kWarps = PcShape<kNT>::kWarps;
-  float part[8][8][128];  // O of 8 warps, 8 rows at a time
-  alignas(16) uint8_t ring[kWarps][PcShape<kNT>::kStages][kPcStageBytes];
+  float part[4][8][128];  // O of 4 warps, 8 rows at a time
   float m[kWarps][8 * kNT], mv[kWarps][8 * kNT], l[kWarps][8 * kNT];
   float inv[8 * kNT];
   uint32_t warp_sums[kWarps];
-  uint32_t unit_off[kCkMaxBatch + 1];
-  uint32_t work[kCkMaxUnits + 1];
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
@@ -74,15 +73,11 @@ struct PcCursor {
   int e, hk, b;      // unit, KV head, sequence
   int t0;            // first token of the unit in its sequence
   ChunkSeq q;
-  int np, lo, n;     // its key tiles (see ck_tiles)
+  int lo, n;         // its key tiles: n from lo on
   int j0, j1;        // those of this CTA
   int last_cta;
   bool valid;
 };
-
-__device__ __forceinline__ int pc_tile(const PcCursor& c, int j) {
-  return j < c.np ? j : c.lo + (j - c.np);
-}
 
 // Fills in the cursor's unit, whose steps from `at` on are this CTA's; skips units of which it has no key
 // tile. `w`: place of the unit's step `at` on the line.
@@ -104,8 +99,8 @@ __device__ __forceinline__ void pc_enter(const ChunkParams& p, const uint32_t* u
     const int64_t next = w + stop - at;
     if (stop > kPcPad) {
       c.t0 = (c.e - (int)unit_off[c.b]) * p.unit_tokens;
-      int tiles;
-      ck_tiles(p.b, c.q, c.t0, min(c.t0 + p.unit_tokens, c.q.n), c.np, c.lo, tiles);
+      int tiles, np;  // (np is 0: there is no prefix)
+      ck_tiles(p.b, c.q, c.t0, min(c.t0 + p.unit_tokens, c.q.n), np, c.lo, tiles);
       c.n = len - kPcPad;
       c.j0 = max(at - kPcPad, 0);
       c.j1 = stop - kPcPad;
@@ -139,10 +134,13 @@ template <typename T, typename Code, bool kCap, int kNT>
 __global__ void __launch_bounds__(PcShape<kNT>::kThreads, 1)
     paged_codes_kernel(const ChunkParams p, const CodePages pages) {
   constexpr int kWarps = PcShape<kNT>::kWarps, kThreads = PcShape<kNT>::kThreads;
-  constexpr int kStages = PcShape<kNT>::kStages, kTiles = kWarps / 8;
+  constexpr int kTiles = kWarps / 8;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   PcShared<kNT>* s = reinterpret_cast<PcShared<kNT>*>(smem_raw);
-  const uint32_t *unit_off = s->unit_off, *work = s->work;
+  const int stages = pages.stages;
+  uint8_t* rings = smem_raw + sizeof(PcShared<kNT>);
+  uint32_t* unit_off = reinterpret_cast<uint32_t*>(rings + kWarps * stages * kPcStageBytes);
+  uint32_t* work = unit_off + p.b.batch + 1;
   const ChunkBatch& pb = p.b;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int slice = warp & 7, half = warp >> 3;  // keys of a tile; which tiles
@@ -151,19 +149,19 @@ __global__ void __launch_bounds__(PcShape<kNT>::kThreads, 1)
   // the line of work: units of each sequence, then key tiles of each unit, both as sums
   grid_dep_wait();
   grid_dep_launch();
-  if (tid == 0) s->unit_off[0] = s->work[0] = 0;
+  if (tid == 0) unit_off[0] = work[0] = 0;
 #pragma unroll 1
   for (int b = tid; b < pb.batch; b += kThreads) {
     const ChunkSeq q = chunk_seq(pb, b);
     if (q.bad && cta == 0) set_error(p.err, FI_DEVERR_CONTEXT_LEN);
-    s->unit_off[b + 1] = q.n * pb.group <= p.split_rows
+    unit_off[b + 1] = q.n * pb.group <= p.split_rows
                              ? (uint32_t)((q.n + p.unit_tokens - 1) / p.unit_tokens)
                              : 0u;
   }
   __syncthreads();
-  block_scan(s->unit_off, pb.batch, s->warp_sums);
+  block_scan(unit_off, pb.batch, s->warp_sums);
   // cu that is not ascending could name more units than the host counted: those are dropped
-  const uint32_t units = min(unit_off[pb.batch], (uint32_t)kCkMaxUnits);
+  const uint32_t units = min(unit_off[pb.batch], (uint32_t)pages.max_units);
   if (units != unit_off[pb.batch] && tid == 0) set_error(p.err, FI_DEVERR_CONTEXT_LEN);
 #pragma unroll 1
   for (int e = tid; e < (int)units; e += kThreads) {
@@ -172,10 +170,10 @@ __global__ void __launch_bounds__(PcShape<kNT>::kThreads, 1)
     const int t0 = (e - (int)unit_off[b]) * p.unit_tokens;
     int np, lo, n;
     ck_tiles(pb, q, t0, min(t0 + p.unit_tokens, q.n), np, lo, n);
-    s->work[e + 1] = (uint32_t)(n + kPcPad);
+    work[e + 1] = (uint32_t)(n + kPcPad);
   }
   __syncthreads();
-  block_scan(s->work, (int)units, s->warp_sums);
+  block_scan(work, (int)units, s->warp_sums);
 
   const uint32_t per_head = work[units];
   const int64_t total = (int64_t)per_head * pb.hk;
@@ -192,57 +190,89 @@ __global__ void __launch_bounds__(PcShape<kNT>::kThreads, 1)
     pc_enter(p, unit_off, work, units, total, active, end, w_use, (int)(r - work[c.e]), c);
     w_load = w_use;
   }
-  PcCursor ld = c;  // where the loads are
-  int ld_j = ld.j0 + half;
-  auto next_tile = [&]() {  // units of one tile have none for the second half
-    while (ld.valid && ld_j >= ld.j1) {
-      pc_next(p, unit_off, work, units, total, active, end, w_load, ld);
-      ld_j = ld.j0 + half;
-    }
-  };
-  next_tile();
-  // the page of the next load, looked up one step ahead
+  // Where the loads are: the warp's 16 keys of one tile, K, V and their scales, a lane copying 16 bytes of
+  // rows lane / 8 + 4 i. Pieces of 16 bytes are placed so that the reads below meet no bank twice (K by the
+  // row's low bit, V by its low three). What a unit fixes is kept as addresses: the copies are a fifth of
+  // the instructions as it is.
+  PcCursor ld = c;
+  const int row0 = lane >> 3, piece = lane & 7;
+  const uint8_t *src_k, *src_v;  // of this lane in page 0
+  const float* src_s;
+  const int32_t* src_page;  // the next tile's block-table entry
+  int ld_key, ld_left;      // its first key, tiles left in the unit
+  int ld_page;              // its page, looked up one step ahead (and not looked at before)
+  const int slot0 = (slice & 3) * kPcKeys;
+  const int64_t page_step = (int64_t)2 * kTiles * pb.bts[1];
   auto look_up = [&]() {
-    return ld.valid ? chunk_page(pb, ld.b, ld.q.keys, pc_tile(ld, ld_j), slice >> 2) : 0;
+    ld_page = ld.valid && ld_key - slot0 < ld.q.keys ? *src_page : -1;
   };
-  int ld_page = look_up();
-  const uint32_t ring = smem_u32(&s->ring[warp][0][0]);
+  auto begin_unit = [&]() {  // units of one tile have none for the second half
+    while (ld.valid && (ld_left = (ld.j1 - ld.j0 - half + kTiles - 1) / kTiles) <= 0)
+      pc_next(p, unit_off, work, units, total, active, end, w_load, ld);
+    if (ld.valid) {
+      const int tile = ld.lo + ld.j0 + half;
+      ld_key = tile * kChunkTile + slice * kPcKeys;
+      src_k = pages.pool[0] + (slot0 + row0) * pages.st[0][1] + ld.hk * pages.st[0][2] + piece * 16;
+      src_v = pages.pool[1] + (slot0 + row0) * pages.st[1][1] + ld.hk * pages.st[1][2] + piece * 16;
+      const int kv = lane >> 4;
+      src_s = p.scale[kv] + ld.hk * p.ss[kv][1] + (slot0 + (lane & 15)) * p.ss[kv][2];
+      src_page = pb.bt + ld.b * pb.bts[0] + (int64_t)(tile * 2 + (slice >> 2)) * pb.bts[1];
+    }
+    look_up();
+  };
+  begin_unit();
+  const uint8_t* my_ring = rings + warp * stages * kPcStageBytes;
+  const uint32_t ring = smem_u32(my_ring);
+  const uint32_t dst_k = ring + row0 * 128 + ((piece ^ ((row0 & 1) << 2)) << 4);
+  const uint32_t dst_v = ring + kPcKeys * 128 + row0 * 128;
+  const uint32_t even_v = (uint32_t)(piece ^ row0) << 4, odd_v = (uint32_t)(piece ^ (row0 + 4)) << 4;
+  const uint32_t dst_s = ring + 2 * kPcKeys * 128 + lane * 4;
+  const int64_t step_k = 4 * pages.st[0][1], step_v = 4 * pages.st[1][1];
   uint32_t held_bits = 0;  // of the stages: whether their page exists
-  // 16 keys of K, V and their scales: a lane copies 16 bytes of rows lane / 8 + 4 i. Pieces of 16 bytes are
-  // placed so that the reads below meet no bank twice (K by the row's low bit, V by its low three).
   auto load = [&](int stage) {
     if (ld.valid) {
-      const int tile = pc_tile(ld, ld_j), key0 = tile * kChunkTile + slice * kPcKeys;
-      const bool held = ld_page != pb.num_blocks;
-      if (!held && key0 < ld.q.keys && lane == 0) set_error(p.err, FI_DEVERR_BAD_BLOCK);
-      const int slot0 = key0 & (kChunkPage - 1), row0 = lane >> 3, piece = lane & 7;
-      const uint32_t dst = ring + stage * kPcStageBytes;
-      const int64_t page = held ? ld_page : 0;
+      const uint32_t at = stage * kPcStageBytes;
+      const bool held = (uint32_t)ld_page < (uint32_t)pb.num_blocks;
       held_bits = (held_bits & ~(1u << stage)) | ((uint32_t)held << stage);
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const uint8_t* src = pages.pool[kv] + page * pages.st[kv][0] +
-                             (slot0 + row0) * pages.st[kv][1] + ld.hk * pages.st[kv][2] + piece * 16;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = row0 + 4 * i;
-          const int to = piece ^ (kv ? row & 7 : (row & 1) << 2);
-          cp_async16(dst + kv * kPcKeys * 128 + row * 128 + to * 16, src + 4 * i * pages.st[kv][1],
-                     held && key0 + row < ld.q.keys);
-        }
+      const uint8_t *k = src_k, *v = src_v;
+      const float* sc = src_s;
+      if (held) {
+        k += ld_page * pages.st[0][0];
+        v += ld_page * pages.st[1][0];
+        sc += ld_page * p.ss[lane >> 4][0];
       }
-      const int kv = lane >> 4, row = lane & 15;
-      cp_async4(dst + 2 * kPcKeys * 128 + lane * 4,
-                p.scale[kv] + page * p.ss[kv][0] + ld.hk * p.ss[kv][1] + (slot0 + row) * p.ss[kv][2],
-                held && key0 + row < ld.q.keys);
-      ld_j += kTiles;
-      next_tile();
-      ld_page = look_up();
+      if (held && ld_key + kPcKeys <= ld.q.keys) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i, k += step_k) cp_async16(dst_k + at + i * 512, k, true);
+#pragma unroll
+        for (int i = 0; i < 4; ++i, v += step_v)
+          cp_async16(dst_v + at + i * 512 + (i & 1 ? odd_v : even_v), v, true);
+        cp_async4(dst_s + at, sc, true);
+      } else {  // zeros past the context and where there is no page
+        const int n = held ? ld.q.keys - ld_key : 0;
+        if (!held && ld_key < ld.q.keys && lane == 0) set_error(p.err, FI_DEVERR_BAD_BLOCK);
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i, k += step_k, v += step_v) {
+          const bool in = row0 + 4 * i < n;
+          cp_async16(dst_k + at + i * 512, in ? k : pages.pool[0], in);
+          cp_async16(dst_v + at + i * 512 + (i & 1 ? odd_v : even_v), in ? v : pages.pool[1], in);
+        }
+        const bool in = (lane & 15) < n;
+        cp_async4(dst_s + at, in ? sc : p.scale[0], in);
+      }
+      ld_key += kTiles * kChunkTile;
+      src_page += page_step;
+      if (--ld_left > 0) {
+        look_up();
+      } else {
+        pc_next(p, unit_off, work, units, total, active, end, w_load, ld);
+        begin_unit();
+      }
     }
     cp_async_commit();
   };
 #pragma unroll 1
-  for (int i = 0; i < kStages - 1; ++i) load(i);
+  for (int i = 0; i < stages - 1; ++i) load(i);
 
   CkJoin join = {};
   int stage = 0;
@@ -320,15 +350,19 @@ __global__ void __launch_bounds__(PcShape<kNT>::kThreads, 1)
       }
     }
     const int past = c.q.pos0;  // the sequence's first new slot
+    int key0 = (c.lo + c.j0 + half) * kChunkTile + slice * kPcKeys;
+    const int plain = pb.window ? 0 : min(past, c.q.keys);  // keys before it are seen by every row
 #pragma unroll 1
-    for (int j = c.j0 + half; j < c.j1; j += kTiles) {
-      cp_async_wait<kStages - 2>();
+    for (int j = c.j0 + half; j < c.j1; j += kTiles, key0 += kTiles * kChunkTile) {
+      if (stages == 2) cp_async_wait<0>();
+      else if (stages == 3) cp_async_wait<1>();
+      else if (stages == 4) cp_async_wait<2>();
+      else cp_async_wait<kPcMaxStages - 2>();
       __syncwarp();  // all lanes' copies are there, and all have left the stage that is filled next
       const bool page_ok = (held_bits >> stage) & 1u;
-      const uint8_t* st = s->ring[warp][stage];
-      load(stage == 0 ? kStages - 1 : stage - 1);
-      stage = stage == kStages - 1 ? 0 : stage + 1;
-      const int tile = pc_tile(c, j), key0 = tile * kChunkTile + slice * kPcKeys;
+      const uint8_t* st = my_ring + stage * kPcStageBytes;
+      load(stage == 0 ? stages - 1 : stage - 1);
+      stage = stage == stages - 1 ? 0 : stage + 1;
       // ------------------------------------------------ scores of keys g, g + 8 and rows 2 t, 2 t + 1
       float sc[kNT][4];
 #pragma unroll
@@ -375,7 +409,7 @@ __global__ void __launch_bounds__(PcShape<kNT>::kThreads, 1)
       }
       // hidden keys: new tokens' (by position, or the tree's bits), those a window leaves behind, those past
       // the context or without a page (whose copies are zeros)
-      if (!page_ok || key0 + kPcKeys > min(past, c.q.keys) || pb.window) {
+      if (!page_ok || key0 + kPcKeys > plain) {
 #pragma unroll
         for (int n = 0; n < kNT; ++n)
 #pragma unroll
@@ -535,10 +569,10 @@ __global__ void __launch_bounds__(PcShape<kNT>::kThreads, 1)
         f[h] = mv[n][h] == -INFINITY ? 0.f : fast_exp2(mv[n][h] - b);
       }
       // a lane has dims [16 g, 16 g + 16) of rows 2 t and 2 t + 1, 4 at a time in an order that spreads the
-      // banks; of 16 warps the second 8 go first, and the others add theirs
-#pragma unroll
-      for (int turn = 0; turn < kTiles; ++turn) {
-        if (half == kTiles - 1 - turn) {
+      // banks; the last 4 warps go first, and the others add theirs
+#pragma unroll 1
+      for (int turn = 0; turn < kWarps / 4; ++turn) {
+        if (warp >> 2 == kWarps / 4 - 1 - turn) {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -552,7 +586,7 @@ __global__ void __launch_bounds__(PcShape<kNT>::kThreads, 1)
                 for (int k = 0; k < 4; ++k)  // (a select over the registers: q4 is the lane's own)
                   x[e] = q4 == k ? o[n][2 * k + (e >> 1)][2 * (e & 1) + h] * f[h] : x[e];
               }
-              float4* to = reinterpret_cast<float4*>(&s->part[slice][2 * t + h][16 * g + q4 * 4]);
+              float4* to = reinterpret_cast<float4*>(&s->part[warp & 3][2 * t + h][16 * g + q4 * 4]);
               if (turn > 0) {
                 const float4 was = *to;
                 x[0] += was.x;
@@ -570,7 +604,7 @@ __global__ void __launch_bounds__(PcShape<kNT>::kThreads, 1)
         if (r < rows) {
           float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int w = 0; w < 8; ++w) {
+          for (int w = 0; w < 4; ++w) {
             const float4 x = *reinterpret_cast<const float4*>(&s->part[w][row][col]);
             sum.x += x.x;
             sum.y += x.y;
@@ -609,17 +643,26 @@ __global__ void __launch_bounds__(PcShape<kNT>::kThreads, 1)
 }
 
 template <typename T, typename Code, bool kCap, int kNT>
-static int launch_one(const ChunkParams& p, const CodePages& pages, cudaStream_t st) {
+static int launch_one(const ChunkParams& p, CodePages pages, cudaStream_t st) {
   constexpr auto kernel = paged_codes_kernel<T, Code, kCap, kNT>;
-  static_assert(sizeof(PcShared<kNT>) <= 227 * 1024, "shared memory");
   static DeviceOnce once;
   cudaError_t e = once.run([] {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)sizeof(PcShared<kNT>));
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPcMaxShared);
   });
   if (e != cudaSuccess) return cuda_fail(e, "fi_paged_tree: kernel set-up");
+  // as many stages as fit beside the line, which is as long as the batch can make it
+  const int64_t units = (int64_t)p.b.total / p.unit_tokens + p.b.batch;
+  pages.max_units = units < kCkMaxUnits ? (int)units : kCkMaxUnits;
+  const size_t fixed = sizeof(PcShared<kNT>) + (size_t)(p.b.batch + 1 + pages.max_units + 1) * 4;
+  const size_t stage = (size_t)PcShape<kNT>::kWarps * kPcStageBytes;
+  pages.stages = kPcMaxStages;
+  while (pages.stages > 2 && fixed + pages.stages * stage > kPcMaxShared) --pages.stages;
+  static_assert(sizeof(PcShared<kNT>) + (kCkMaxBatch + kCkMaxUnits + 2) * 4 +
+                        2 * PcShape<kNT>::kWarps * kPcStageBytes <=
+                    kPcMaxShared,
+                "shared memory");
   e = launch_pdl(kernel, dim3((unsigned)sm_count()), dim3(PcShape<kNT>::kThreads),
-                 sizeof(PcShared<kNT>), st, p, pages);
+                 fixed + pages.stages * stage, st, p, pages);
   return e == cudaSuccess ? FI_OK : cuda_fail(e, "fi_paged_tree: launch");
 }
 
