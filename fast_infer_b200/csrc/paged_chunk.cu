@@ -50,7 +50,6 @@ constexpr int kCkRegsSoftmax = 184;  // 2 x 128 x 184 + 128 x 136 = 384 x 168
 constexpr int kCkRegsOther = 136;
 constexpr int kCkThreadsCodes = 512;  // with 8-bit codes: four more warps that turn codes into tiles
 constexpr int kCkRegsOtherCodes = 72;  // 2 x 128 x 184 + 2 x 128 x 72 = 512 x 128
-constexpr int kCkConvertBar = 14;
 // Scales of a key tile are read after its product is done, that is after its stage may be filled again: the
 // place of tile j is written for tile j + 4 once S of tile j + 2 is complete, which waits for P of tile j + 1.
 constexpr int kCkScaleSlots = 4;
@@ -88,6 +87,7 @@ struct CkBarriers {
   uint64_t unit_full[kCkSlots], unit_empty[kCkSlots];
   uint64_t kc_full[kCkStages], vc_full[kCkStages];  // codes have arrived
   alignas(16) float k_scale[kCkScaleSlots][kChunkTile];
+  alignas(16) float v_scale[kCkScaleSlots][kChunkTile];
   uint64_t merge;  // both softmax warpgroups, in a transposed unit
   uint32_t tmem_base;
   // transposed units, per warpgroup: rows' max, partial maxima / sums, scale, slope, token
@@ -314,8 +314,9 @@ __device__ __forceinline__ void score_form8(const uint32_t* raw, float* s, const
 // operands: half a step (2^-12 .. 2^-11, bf16 2^-9 .. 2^-8) of each p, which adds to the output's own
 // rounding: 3.0e-4 in place of 2.1e-4 (root mean square, relative; bf16 2.3e-3 and 1.7e-3). P as the
 // sum of two such values would take the product twice.
-template <typename T>
-__device__ __forceinline__ float ck_exp(uint32_t* sr, float sl2, float mref) {
+// With `v_scale`, P takes the scales of V's rows (and the sum does not).
+template <typename T, bool kScaled>
+__device__ __forceinline__ float ck_exp(uint32_t* sr, float sl2, float mref, const float* v_scale) {
   const uint64_t sc2 = f32x2(sl2, sl2), nm2 = f32x2(-mref, -mref);
   uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
@@ -332,6 +333,11 @@ __device__ __forceinline__ float ck_exp(uint32_t* sr, float sl2, float mref) {
       p1 = fast_exp2(x1);
     }
     sum2[(c >> 1) & 3] = add_f32x2(sum2[(c >> 1) & 3], f32x2(p0, p1));
+    if constexpr (kScaled) {
+      const float2 f = *reinterpret_cast<const float2*>(v_scale + c);
+      p0 *= f.x;
+      p1 *= f.y;
+    }
     sr[c >> 1] = Half16<T>::pack(p0, p1);
   }
   float lo, hi;
@@ -650,17 +656,23 @@ __device__ __forceinline__ void spread16(const uint4& raw, float scale, uint32_t
   }
 }
 
+// Where V's scale is applied: to P in fp32, before it is rounded, where T has fp32's range (bf16); else (fp16) to V's
+// codes, rounded once to T: half a step of 2^-12 to 2^-11 more.
+template <typename T>
+constexpr bool kCkScaleP = std::is_same_v<T, __nv_bfloat16>;
+
 // Four warps between TMA and the tensor core: the codes of a tile (128 keys x 128 bytes) lie in the first
-// half of its 16-bit place; all of them are read into registers, and then written as the swizzled tile of
-// two 64-value columns. K keeps its codes, which are exact, and its scales go to the softmax warps: scores
-// are scaled in fp32, as lse is an output. V is scaled here and rounded to T, half a step (fp16 2^-12 to
-// 2^-11) beside the one of P. Rows of keys past the context, or without a page, are zero.
+// half of its 16-bit place, a row where its first 64 values will be, so that the 8 lanes of a row read it and
+// then write over it. K keeps its codes, which are exact in T, and scores are scaled in fp32 by the softmax
+// warps, as lse is an output. A lane looks up the scales of one row of its warp, a tile ahead. Rows of keys
+// past the context are zero, like those without a page.
 template <typename T, typename Code>
 __device__ __forceinline__ void code_tiles(const ChunkParams& p, CkBarriers* bars, uint8_t* sK,
                                            uint8_t* sV) {
   const ChunkBatch& pb = p.b;
-  const int tid = threadIdx.x & 127, lane = tid & 31;
-  const int piece = tid & 7, row0 = tid >> 3;  // rows row0, row0 + 16, ...
+  const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
+  const int piece = lane & 7, sub = lane >> 3;           // this lane's 16 codes of rows 4 warp + sub + 16 i
+  const int mine = 4 * warp + (lane & 3) + 16 * (lane >> 2);  // the row whose scales it looks up
   // two 16-byte chunks of a row's column, in an order that keeps the 8 lanes of a row off each
   // other's banks (the two columns' chunks share them)
   const int column = piece >> 2, chunk = (piece & 3) * 2;
@@ -673,53 +685,56 @@ __device__ __forceinline__ void code_tiles(const ChunkParams& p, CkBarriers* bar
   for (const CkUnit* up; (up = ck_next<true>(bars, next_unit, p.err)) != nullptr;
        ck_done<true>(bars, next_unit)) {
     const CkUnit& u = *up;
+    auto page_of = [&](int j) { return chunk_page(pb, u.b, u.keys, ck_tile(u, j), mine >> 6); };
+    auto scale_of = [&](int kv, int page, int j) {
+      return page != pb.num_blocks && ck_tile(u, j) * kChunkTile + mine < u.keys
+                 ? p.scale[kv][page * p.ss[kv][0] + u.hk * p.ss[kv][1] +
+                               (mine & (kChunkPage - 1)) * p.ss[kv][2]]
+                 : 0.f;
+    };
+    int page = page_of(u.j0);
+    float k_next = scale_of(0, page, u.j0), v_next = scale_of(1, page, u.j0);
 #pragma unroll 1
     for (int j = u.j0; j < u.j1; ++j, ++g) {
-      const int s = g % kCkStages, tile = ck_tile(u, j);
+      const int s = g % kCkStages;
       const uint32_t par = (g / kCkStages) & 1;
-      int page[2];
-      for (int i = 0; i < 2; ++i) page[i] = chunk_page(pb, u.b, u.keys, tile, i);
+      const int live = u.keys - ck_tile(u, j) * kChunkTile;  // rows of keys in the context
+      const float k_scale = k_next, v_scale = v_next;
+      if (j + 1 < u.j1) page = page_of(j + 1);
+      bars->k_scale[g % kCkScaleSlots][mine] = k_scale;
+      if (kCkScaleP<T>) bars->v_scale[g % kCkScaleSlots][mine] = v_scale;
 #pragma unroll 1
       for (int kv = 0; kv < 2; ++kv) {
-        float scale[8];
-        bool held[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = row0 + 16 * i, pg = page[i >> 2];
-          held[i] = pg != pb.num_blocks && tile * kChunkTile + r < u.keys;
-          scale[i] = held[i] ? p.scale[kv][pg * p.ss[kv][0] + u.hk * p.ss[kv][1] +
-                                           (r & (kChunkPage - 1)) * p.ss[kv][2]]
-                             : 0.f;
-        }
-        uint8_t* dst = (kv ? sV : sK) + s * kChunkTileBytes;
+        uint8_t* row = (kv ? sV : sK) + s * kChunkTileBytes + (4 * warp + sub) * 128;
         wait(kv ? &bars->vc_full[s] : &bars->kc_full[s], par);
-        uint4 raw[8];
-#pragma unroll
+#pragma unroll 2
         for (int i = 0; i < 8; ++i) {
-          raw[i] = *reinterpret_cast<const uint4*>(dst + (row0 + 16 * i) * 128 + piece * 16);
-          if (!held[i]) raw[i] = make_uint4(0, 0, 0, 0);
-        }
-        __syncwarp();
-        named_bar_sync(kCkConvertBar, 128);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = row0 + 16 * i;
+          const int r = 4 * warp + sub + 16 * i;
+          uint8_t* at = row + i * 16 * 128;
+          uint4 raw = *reinterpret_cast<const uint4*>(at + piece * 16);
+          if (r >= live) raw = make_uint4(0, 0, 0, 0);
           uint32_t v[8];
-          if (kv) spread16<T, Code, true>(raw[i], scale[i], v);
-          else spread16<T, Code, false>(raw[i], 1.f, v);
-          uint8_t* col = dst + column * kChunkHalf + r * 128;
+          if (!kCkScaleP<T> && kv)
+            spread16<T, Code, true>(raw, __shfl_sync(0xffffffffu, v_scale, i * 4 + sub), v);
+          else
+            spread16<T, Code, false>(raw, 1.f, v);
+          __syncwarp();
+          at += column * kChunkHalf;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int which = h ^ column;
             const uint4 w = which ? make_uint4(v[4], v[5], v[6], v[7])
                                   : make_uint4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<uint4*>(col + (((chunk + which) ^ (r & 7)) << 4)) = w;
+            *reinterpret_cast<uint4*>(at + (((chunk + which) ^ (r & 7)) << 4)) = w;
           }
-          if (kv == 0 && piece == 0) bars->k_scale[g % kCkScaleSlots][r] = scale[i];
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(kv ? &bars->v_full[s] : &bars->k_full[s]);
+        if (kv == 0 && j + 1 < u.j1) {
+          k_next = scale_of(0, page, j + 1);
+          v_next = scale_of(1, page, j + 1);
+        }
       }
     }
   }
@@ -1181,7 +1196,8 @@ __global__ void __launch_bounds__(kCkThreadsOf<Code>, 1)
               l *= alpha;
             }
           }
-          l += ck_exp<T>(sr, sl2, m == -INFINITY ? 0.f : m);
+          l += ck_exp<T, kCode && kCkScaleP<T>>(sr, sl2, m == -INFINITY ? 0.f : m,
+                                                bars->v_scale[g % kCkScaleSlots]);
           tmem_st32(tS + 0, sr);
           tmem_st32(tS + 32, sr + 32);
           if (rescale) {
