@@ -48,8 +48,6 @@ namespace fi {
 constexpr int kCkThreads = 384;
 constexpr int kCkRegsSoftmax = 184;  // 2 x 128 x 184 + 128 x 136 = 384 x 168
 constexpr int kCkRegsOther = 136;
-constexpr int kCkThreadsCodes = 512;  // with 8-bit codes: four more warps that turn codes into tiles
-constexpr int kCkRegsOtherCodes = 72;  // 2 x 128 x 184 + 2 x 128 x 72 = 512 x 128
 // Scales of a key tile are read after its product is done, that is after its stage may be filled again: the
 // place of tile j is written for tile j + 4 once S of tile j + 2 is complete, which waits for P of tile j + 1.
 constexpr int kCkScaleSlots = 4;
@@ -97,7 +95,7 @@ struct CkBarriers {
   int64_t n_off[kCkNarrow];  // where a row's output goes
   CkUnit units[kCkSlots];
   uint8_t row_token[kChunkTile], row_head[kChunkTile];  // of a tile's rows
-  uint32_t warp_sums[kCkThreadsCodes / 32];
+  uint32_t warp_sums[kCkThreads / 32];
   uint32_t unit_off[kCkMaxBatch + 1];  // first unit of each sequence
   uint32_t work[kCkMaxUnits + 1];      // steps before each unit
 };
@@ -116,32 +114,52 @@ __device__ __forceinline__ int ck_tile(const CkUnit& u, int j) {
 // roles through a ring in shared memory. Its lanes look the units' pages over, so that no one
 // else has to unless an entry is invalid. On the line a unit is `pad` steps longer than its key
 // tiles, which stand for what it costs to begin and end one; its step j is at pad + j.
-__device__ __forceinline__ void ck_schedule(const ChunkBatch& p, int unit_tokens, int pad,
-                                            CkBarriers* s, uint32_t units, CkJoin* join_out,
-                                            int* err) {
-  const int G = gridDim.x, cta = blockIdx.x, lane = threadIdx.x & 31;
-  const uint32_t per_head = s->work[units];
-  const int64_t total = (int64_t)per_head * p.hk;
-  const int active = (int)(total < G ? total : G);  // CTAs with work
-  int64_t w = cta < active ? total * cta / active : 0;
-  const int64_t end = cta < active ? total * (cta + 1) / active : 0;
-  int hk = 0, e = 0, b = 0, at = 0;  // `at`: where in the unit this CTA begins
-  if (w < end) {
-    hk = (int)(w / per_head);
-    const uint32_t r = (uint32_t)(w - (int64_t)hk * per_head);
-    e = last_le(s->work, (int)units, r);
-    b = last_le(s->unit_off, p.batch, (uint32_t)e);
-    at = (int)(r - s->work[e]);
+struct CkScheduler {
+  const ChunkBatch& p;
+  CkBarriers* s;
+  CkJoin* join_out;
+  int* err;
+  int64_t total, w, end;
+  uint32_t units;
+  int unit_tokens, pad, active;
+  int hk, e, b, at;  // `at`: where in the unit this CTA begins
+  int i;             // units handed out
+  bool open;         // some may be left
+  ChunkSeq q;
+  CkJoin join;
+
+  __device__ __forceinline__ CkScheduler(const ChunkBatch& p, int unit_tokens, int pad,
+                                         CkBarriers* s, uint32_t units, CkJoin* join_out, int* err)
+      : p(p), s(s), join_out(join_out), err(err), units(units), unit_tokens(unit_tokens), pad(pad) {
+    const int G = gridDim.x, cta = blockIdx.x;
+    const uint32_t per_head = s->work[units];
+    total = (int64_t)per_head * p.hk;
+    active = (int)(total < G ? total : G);  // CTAs with work
+    w = cta < active ? total * cta / active : 0;
+    end = cta < active ? total * (cta + 1) / active : 0;
+    hk = e = b = at = 0;
+    if (w < end) {
+      hk = (int)(w / per_head);
+      const uint32_t r = (uint32_t)(w - (int64_t)hk * per_head);
+      e = last_le(s->work, (int)units, r);
+      b = last_le(s->unit_off, p.batch, (uint32_t)e);
+      at = (int)(r - s->work[e]);
+    }
+    q = chunk_seq(p, b);
+    join = {};
+    i = 0;
+    open = true;
   }
-  ChunkSeq q = chunk_seq(p, b);
-  const int tt = p.tile_tokens;
-  CkJoin join = {};
-#pragma unroll 1
-  for (int i = 0;; ++i) {
-    const int slot = i % kCkSlots;
+
+  // The next unit into the ring, an invalid one after the last.
+  __device__ __forceinline__ void next() {
+    const int cta = blockIdx.x, lane = threadIdx.x & 31, tt = p.tile_tokens, slot = i % kCkSlots;
     if (i >= kCkSlots &&
-        !__all_sync(0xffffffffu, mbar_wait(&s->unit_empty[slot], ((i / kCkSlots) - 1) & 1, err)))
-      break;
+        !__all_sync(0xffffffffu, mbar_wait(&s->unit_empty[slot], ((i / kCkSlots) - 1) & 1, err))) {
+      open = false;
+      return;
+    }
+    ++i;
     CkUnit u;
     const int len = w < end ? (int)(s->work[e + 1] - s->work[e]) : 0;
     const int stop = len - at <= end - w ? len : at + (int)(end - w);
@@ -195,10 +213,12 @@ __device__ __forceinline__ void ck_schedule(const ChunkBatch& p, int unit_tokens
       join.rows[0] = u.rows[0];
       join.rows[1] = u.rows[1];
     }
-    if (!u.valid) break;
+    open = u.valid;
   }
-  if (lane == 0) *join_out = join;
-}
+  __device__ __forceinline__ void finish() {
+    if ((threadIdx.x & 31) == 0) *join_out = join;
+  }
+};
 
 // The next unit of the ring, null when none is left; it stays in shared memory, read there by
 // whole warps (or one thread, kWarp = false), until ck_done gives the slot back.
@@ -661,18 +681,20 @@ __device__ __forceinline__ void spread16(const uint4& raw, float scale, uint32_t
 template <typename T>
 constexpr bool kCkScaleP = std::is_same_v<T, __nv_bfloat16>;
 
-// Four warps between TMA and the tensor core: the codes of a tile (128 keys x 128 bytes) lie in the first
-// half of its 16-bit place, a row where its first 64 values will be, so that the 8 lanes of a row read it and
-// then write over it. K keeps its codes, which are exact in T, and scores are scaled in fp32 by the softmax
-// warps, as lse is an output. A lane looks up the scales of one row of its warp, a tile ahead. Rows of keys
-// past the context are zero, like those without a page.
+// Two warps between TMA and the tensor core (the scheduler's, which hands out units on the side, and the one
+// that 16-bit pages leave idle: more warps would take registers from the softmax): the codes of a tile (128
+// keys x 128 bytes) lie in the first half of its 16-bit place, a row where its first 64 values will be, so that
+// the 8 lanes of a row read it and then write over it. K keeps its codes, which are exact in T, and scores
+// are scaled in fp32 by the softmax warps, as lse is an output. A lane looks up the scales of two rows of its
+// warp, a tile ahead. Rows of keys past the context are zero, like those without a page.
 template <typename T, typename Code>
 __device__ __forceinline__ void code_tiles(const ChunkParams& p, CkBarriers* bars, uint8_t* sK,
-                                           uint8_t* sV) {
+                                           uint8_t* sV, int warp, CkScheduler* sched) {
   const ChunkBatch& pb = p.b;
-  const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
-  const int piece = lane & 7, sub = lane >> 3;           // this lane's 16 codes of rows 4 warp + sub + 16 i
-  const int mine = 4 * warp + (lane & 3) + 16 * (lane >> 2);  // the row whose scales it looks up
+  const int lane = threadIdx.x & 31;
+  const int piece = lane & 7, sub = lane >> 3;  // this lane's 16 codes of rows 4 warp + sub + 8 i
+  // the rows whose scales it looks up: 4 warp + (lane & 3) + 8 i for i = lane / 4 and lane / 4 + 8
+  const int mine = 4 * warp + (lane & 3) + 8 * (lane >> 2);
   // two 16-byte chunks of a row's column, in an order that keeps the 8 lanes of a row off each
   // other's banks (the two columns' chunks share them)
   const int column = piece >> 2, chunk = (piece & 3) * 2;
@@ -681,71 +703,91 @@ __device__ __forceinline__ void code_tiles(const ChunkParams& p, CkBarriers* bar
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.err));
   };
+  if (sched) {
+    sched->next();
+    if (sched->open) sched->next();
+  }
 #pragma unroll 1
-  for (const CkUnit* up; (up = ck_next<true>(bars, next_unit, p.err)) != nullptr;
-       ck_done<true>(bars, next_unit)) {
+  for (const CkUnit* up; (up = ck_next<true>(bars, next_unit, p.err)) != nullptr;) {
     const CkUnit& u = *up;
-    auto page_of = [&](int j) { return chunk_page(pb, u.b, u.keys, ck_tile(u, j), mine >> 6); };
-    auto scale_of = [&](int kv, int page, int j) {
-      return page != pb.num_blocks && ck_tile(u, j) * kChunkTile + mine < u.keys
-                 ? p.scale[kv][page * p.ss[kv][0] + u.hk * p.ss[kv][1] +
-                               (mine & (kChunkPage - 1)) * p.ss[kv][2]]
-                 : 0.f;
+    float next[2][2];  // k and v of the next tile's rows `mine` and `mine` + 64
+    auto look_up = [&](const int* page, int j) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bool held = page[h] != pb.num_blocks &&
+                          ck_tile(u, j) * kChunkTile + mine + 64 * h < u.keys;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv)
+          next[kv][h] = held ? p.scale[kv][page[h] * p.ss[kv][0] + u.hk * p.ss[kv][1] +
+                                           (mine & (kChunkPage - 1)) * p.ss[kv][2]]
+                             : 0.f;
+      }
     };
-    int page = page_of(u.j0);
-    float k_next = scale_of(0, page, u.j0), v_next = scale_of(1, page, u.j0);
+    int page[2];
+    for (int h = 0; h < 2; ++h) page[h] = chunk_page(pb, u.b, u.keys, ck_tile(u, u.j0), h);
+    look_up(page, u.j0);
 #pragma unroll 1
     for (int j = u.j0; j < u.j1; ++j, ++g) {
       const int s = g % kCkStages;
       const uint32_t par = (g / kCkStages) & 1;
       const int live = u.keys - ck_tile(u, j) * kChunkTile;  // rows of keys in the context
-      const float k_scale = k_next, v_scale = v_next;
-      if (j + 1 < u.j1) page = page_of(j + 1);
-      bars->k_scale[g % kCkScaleSlots][mine] = k_scale;
-      if (kCkScaleP<T>) bars->v_scale[g % kCkScaleSlots][mine] = v_scale;
+      const float v_scale[2] = {next[1][0], next[1][1]};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        bars->k_scale[g % kCkScaleSlots][mine + 64 * h] = next[0][h];
+        if (kCkScaleP<T>) bars->v_scale[g % kCkScaleSlots][mine + 64 * h] = next[1][h];
+      }
+      if (j + 1 < u.j1)
+        for (int h = 0; h < 2; ++h) page[h] = chunk_page(pb, u.b, u.keys, ck_tile(u, j + 1), h);
 #pragma unroll 1
       for (int kv = 0; kv < 2; ++kv) {
         uint8_t* row = (kv ? sV : sK) + s * kChunkTileBytes + (4 * warp + sub) * 128;
         wait(kv ? &bars->vc_full[s] : &bars->kc_full[s], par);
-#pragma unroll 2
-        for (int i = 0; i < 8; ++i) {
-          const int r = 4 * warp + sub + 16 * i;
-          uint8_t* at = row + i * 16 * 128;
-          uint4 raw = *reinterpret_cast<const uint4*>(at + piece * 16);
-          if (r >= live) raw = make_uint4(0, 0, 0, 0);
-          uint32_t v[8];
-          if (!kCkScaleP<T> && kv)
-            spread16<T, Code, true>(raw, __shfl_sync(0xffffffffu, v_scale, i * 4 + sub), v);
-          else
-            spread16<T, Code, false>(raw, 1.f, v);
-          __syncwarp();
-          at += column * kChunkHalf;
+#pragma unroll 1
+        for (int i0 = 0; i0 < 16; i0 += 4) {  // four rows' reads before their writes
+          uint4 raw[4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int which = h ^ column;
-            const uint4 w = which ? make_uint4(v[4], v[5], v[6], v[7])
-                                  : make_uint4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<uint4*>(at + (((chunk + which) ^ (r & 7)) << 4)) = w;
+          for (int i = 0; i < 4; ++i) {
+            raw[i] = *reinterpret_cast<const uint4*>(row + (i0 + i) * 8 * 128 + piece * 16);
+            if (4 * warp + sub + 8 * (i0 + i) >= live) raw[i] = make_uint4(0, 0, 0, 0);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 4 * warp + sub + 8 * (i0 + i);
+            uint32_t v[8];
+            if (!kCkScaleP<T> && kv)
+              spread16<T, Code, true>(raw[i],
+                                      __shfl_sync(0xffffffffu, i0 < 8 ? v_scale[0] : v_scale[1],
+                                                  ((i0 + i) & 7) * 4 + sub),
+                                      v);
+            else
+              spread16<T, Code, false>(raw[i], 1.f, v);
+            uint8_t* at = row + (i0 + i) * 8 * 128 + column * kChunkHalf;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int which = h ^ column;
+              const uint4 w = which ? make_uint4(v[4], v[5], v[6], v[7])
+                                    : make_uint4(v[0], v[1], v[2], v[3]);
+              *reinterpret_cast<uint4*>(at + (((chunk + which) ^ (r & 7)) << 4)) = w;
+            }
           }
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(kv ? &bars->v_full[s] : &bars->k_full[s]);
-        if (kv == 0 && j + 1 < u.j1) {
-          k_next = scale_of(0, page, j + 1);
-          v_next = scale_of(1, page, j + 1);
-        }
+        if (kv == 0 && j + 1 < u.j1) look_up(page, j + 1);
       }
     }
+    ck_done<true>(bars, next_unit);
+    if (sched && sched->open) sched->next();  // (two ahead: the units before it are still at work)
   }
+  if (sched) sched->finish();
 }
-
-template <typename Code>
-constexpr int kCkThreadsOf = std::is_void_v<Code> ? kCkThreads : kCkThreadsCodes;
 
 // Code: the type of 8-bit pages (void: 16-bit pages of type T).
 template <typename T, bool kCap, bool kAlibi, bool kNarrow, bool kTree, typename Code>
-__global__ void __launch_bounds__(kCkThreadsOf<Code>, 1)
+__global__ void __launch_bounds__(kCkThreads, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q,
                        const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const ChunkParams p) {
@@ -757,7 +799,6 @@ __global__ void __launch_bounds__(kCkThreadsOf<Code>, 1)
   CkBarriers* bars = reinterpret_cast<CkBarriers*>(sV + kCkStages * kChunkTileBytes);
 
   constexpr bool kCode = !std::is_void_v<Code>;
-  constexpr int kThreads = kCkThreadsOf<Code>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = blockIdx.x;
 
@@ -775,9 +816,9 @@ __global__ void __launch_bounds__(kCkThreadsOf<Code>, 1)
       mbar_init(&bars->o_empty[t], 4);
     }
     for (int s = 0; s < kCkStages; ++s) {
-      mbar_init(&bars->k_full[s], kCode ? 4 : 1);
+      mbar_init(&bars->k_full[s], kCode ? 2 : 1);
       mbar_init(&bars->k_empty[s], 1);
-      mbar_init(&bars->v_full[s], kCode ? 4 : 1);
+      mbar_init(&bars->v_full[s], kCode ? 2 : 1);
       mbar_init(&bars->v_empty[s], 1);
       mbar_init(&bars->kc_full[s], 1);
       mbar_init(&bars->vc_full[s], 1);
@@ -786,7 +827,7 @@ __global__ void __launch_bounds__(kCkThreadsOf<Code>, 1)
     mbar_init(&bars->merge, 8);
     for (int s = 0; s < kCkSlots; ++s) {
       mbar_init(&bars->unit_full[s], 1);
-      mbar_init(&bars->unit_empty[s], kCode ? 14 : 10);  // TMA, UMMA, the 8 softmax (and 4 code) warps
+      mbar_init(&bars->unit_empty[s], kCode ? 12 : 10);  // TMA, UMMA, the 8 softmax (and 2 code) warps
     }
     fence_barrier_init();
   }
@@ -803,7 +844,7 @@ __global__ void __launch_bounds__(kCkThreadsOf<Code>, 1)
   constexpr int kPad = kNarrow ? kCkPadNarrow : kCkPadWide;
   bool single = true;  // at most one unit in each of this thread's sequences
 #pragma unroll 1
-  for (int b = threadIdx.x; b < pb.batch; b += kThreads) {
+  for (int b = threadIdx.x; b < pb.batch; b += kCkThreads) {
     const ChunkSeq q = chunk_seq(pb, b);
     if (q.bad && cta == 0) set_error(p.err, FI_DEVERR_CONTEXT_LEN);
     const bool here = (q.n * pb.group <= p.split_rows) == kNarrow;
@@ -819,7 +860,7 @@ __global__ void __launch_bounds__(kCkThreadsOf<Code>, 1)
   uint32_t units;
   if (__syncthreads_and(single)) {  // unit b is sequence b
     units = (uint32_t)pb.batch;
-    for (int b = threadIdx.x; b < pb.batch; b += kThreads) bars->unit_off[b + 1] = b + 1;
+    for (int b = threadIdx.x; b < pb.batch; b += kCkThreads) bars->unit_off[b + 1] = b + 1;
   } else {
     block_scan(bars->unit_off, pb.batch, bars->warp_sums);
     // cu that is not ascending could name more units than the host counted: those are dropped
@@ -827,7 +868,7 @@ __global__ void __launch_bounds__(kCkThreadsOf<Code>, 1)
     if (units != bars->unit_off[pb.batch] && threadIdx.x == 0)
       set_error(p.err, FI_DEVERR_CONTEXT_LEN);
 #pragma unroll 1
-    for (int e = threadIdx.x; e < (int)units; e += kThreads) {
+    for (int e = threadIdx.x; e < (int)units; e += kCkThreads) {
       const int b = last_le(bars->unit_off, pb.batch, (uint32_t)e);
       const ChunkSeq q = chunk_seq(pb, b);
       const int t0 = (e - (int)bars->unit_off[b]) * p.unit_tokens;
@@ -844,8 +885,7 @@ __global__ void __launch_bounds__(kCkThreadsOf<Code>, 1)
   const uint32_t tmem = bars->tmem_base;
 
   if (warp >= 8) {
-    if constexpr (kCode) setmaxnreg_dec<kCkRegsOtherCodes>();
-    else if constexpr (!kNarrow) setmaxnreg_dec<kCkRegsOther>();
+    if constexpr (!kNarrow) setmaxnreg_dec<kCkRegsOther>();
     if (warp == 8 && lane == 0) {
       // ---------------------------------------------------------- TMA producer
       prefetch_tmap(&tm_q);
@@ -920,7 +960,15 @@ __global__ void __launch_bounds__(kCkThreadsOf<Code>, 1)
         }
       }
     } else if (warp == 10) {
-      ck_schedule(pb, p.unit_tokens, kPad, bars, units, p.join + cta, p.err);
+      CkScheduler sched(pb, p.unit_tokens, kPad, bars, units, p.join + cta, p.err);
+      if constexpr (kCode) {
+        code_tiles<T, Code>(p, bars, sK, sV, 0, &sched);
+      } else {
+        while (sched.open) sched.next();
+        sched.finish();
+      }
+    } else if (kCode && warp == 11) {
+      if constexpr (kCode) code_tiles<T, Code>(p, bars, sK, sV, 1, nullptr);
     } else if (warp == 9 && lane == 0) {
       // ---------------------------------------------------------- UMMA issuer
       constexpr uint32_t idesc_qk = umma_idesc<T>(128, 128, 0, 0);
@@ -1057,11 +1105,8 @@ __global__ void __launch_bounds__(kCkThreadsOf<Code>, 1)
       umma_commit(&bars->mma_done);
       mbar_wait(&bars->mma_done, 0, p.err);
     }
-    if constexpr (kCode) {
-      if (warp >= 12) code_tiles<T, Code>(p, bars, sK, sV);
-    }
     __syncwarp();
-    named_bar_arrive(kCkTeardownBar, kThreads);
+    named_bar_arrive(kCkTeardownBar, kCkThreads);
     return;
   }
 
@@ -1279,7 +1324,7 @@ __global__ void __launch_bounds__(kCkThreadsOf<Code>, 1)
   if (p.late_wait && threadIdx.x == 0) grid_dep_wait();
   __syncwarp();
   tc_fence_before();
-  named_bar_sync(kCkTeardownBar, kThreads);
+  named_bar_sync(kCkTeardownBar, kCkThreads);
   if (warp == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -1356,15 +1401,12 @@ static int launch_main(const CUtensorMap& tq, const CUtensorMap& tk, const CUten
     cudaFuncAttributes a;
     const cudaError_t e = cudaFuncGetAttributes(&a, kernel);
     if (e != cudaSuccess) return e;
-    constexpr bool kCode = !std::is_void_v<Code>;
-    const int split = 2 * 128 * kCkRegsSoftmax +
-                      (kCode ? 2 * 128 * kCkRegsOtherCodes : 128 * kCkRegsOther);
-    if ((kCode || !kNarrow) && a.numRegs * kCkThreadsOf<Code> < split)
+    if (!kNarrow && a.numRegs * kCkThreads < 2 * 128 * kCkRegsSoftmax + 128 * kCkRegsOther)
       return cudaErrorInvalidConfiguration;
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCkSmemBytes);
   });
   if (e != cudaSuccess) return cuda_fail(e, "fi_paged_chunk: kernel set-up");
-  e = launch_pdl(kernel, dim3((unsigned)sm_count()), dim3(kCkThreadsOf<Code>), kCkSmemBytes, st, tq,
+  e = launch_pdl(kernel, dim3((unsigned)sm_count()), dim3(kCkThreads), kCkSmemBytes, st, tq,
                  tk, tv, p);
   return e == cudaSuccess ? FI_OK : cuda_fail(e, "fi_paged_chunk: launch");
 }
