@@ -104,7 +104,7 @@ int chunk_code_map(CUtensorMap* m, const void* codes, const ChunkBatch& p, const
   if (p.num_blocks == 1) sb[2] = (uint64_t)kChunkTile;
   const uint32_t box[4] = {(uint32_t)kChunkTile, 1, (uint32_t)kChunkPage, 1};
   return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, codes, dims, sb, box,
-                      CU_TENSOR_MAP_SWIZZLE_NONE, what);
+                      CU_TENSOR_MAP_SWIZZLE_128B, what);
 }
 
 }  // namespace fi

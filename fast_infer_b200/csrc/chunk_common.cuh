@@ -263,7 +263,7 @@ int chunk_q_map(CUtensorMap* m, CUtensorMapDataType type, const void* q, const C
 // of the 64 slots of a page.
 int chunk_kv_map(CUtensorMap* m, CUtensorMapDataType type, const void* kv, const ChunkBatch& p,
                  const int64_t* st, const char* what);
-// The same over a pool of 8-bit codes: a box is the 128 codes of the 64 slots of a page, unswizzled.
+// The same over a pool of 8-bit codes: a box is the 128 codes of the 64 slots of a page.
 int chunk_code_map(CUtensorMap* m, const void* codes, const ChunkBatch& p, const int64_t* st,
                    const char* what);
 

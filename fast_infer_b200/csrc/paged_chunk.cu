@@ -335,30 +335,35 @@ __device__ __forceinline__ void score_form8(const uint32_t* raw, float* s, const
 // rounding: 3.0e-4 in place of 2.1e-4 (root mean square, relative; bf16 2.3e-3 and 1.7e-3). P as the
 // sum of two such values would take the product twice.
 // With `v_scale`, P takes the scales of V's rows (and the sum does not).
-template <typename T, bool kScaled>
+template <typename T, bool kCode, bool kScaled>
 __device__ __forceinline__ float ck_exp(uint32_t* sr, float sl2, float mref, const float* v_scale) {
   const uint64_t sc2 = f32x2(sl2, sl2), nm2 = f32x2(-mref, -mref);
   uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
+  // (over codes the special function units wait for the issue slots as it is)
+  constexpr int kEmu = kCode ? 0 : kCkEmuPairs;
 #pragma unroll
-  for (int c = 0; c < kChunkTile; c += 2) {
-    const uint64_t xp =
-        fma_f32x2(f32x2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), sc2, nm2);
-    float p0, p1;
-    if (((c >> 1) & 7) < kCkEmuPairs) {
-      f32x2_split(exp2_poly5_x2(xp), p0, p1);
-    } else {
-      float x0, x1;
-      f32x2_split(xp, x0, x1);
-      p0 = fast_exp2(x0);
-      p1 = fast_exp2(x1);
+  for (int c = 0; c < kChunkTile; c += 4) {
+    ulonglong2 f = make_ulonglong2(0, 0);
+    if constexpr (kScaled) f = *reinterpret_cast<const ulonglong2*>(v_scale + c);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int d = c + 2 * i;
+      const uint64_t xp =
+          fma_f32x2(f32x2(__uint_as_float(sr[d]), __uint_as_float(sr[d + 1])), sc2, nm2);
+      float p0, p1;
+      if (((d >> 1) & 7) < kEmu) {
+        f32x2_split(exp2_poly5_x2(xp), p0, p1);
+      } else {
+        float x0, x1;
+        f32x2_split(xp, x0, x1);
+        p0 = fast_exp2(x0);
+        p1 = fast_exp2(x1);
+      }
+      uint64_t pp = f32x2(p0, p1);
+      sum2[(d >> 1) & 3] = add_f32x2(sum2[(d >> 1) & 3], pp);
+      if constexpr (kScaled) f32x2_split(mul_f32x2(pp, i ? f.y : f.x), p0, p1);
+      sr[d >> 1] = Half16<T>::pack(p0, p1);
     }
-    sum2[(c >> 1) & 3] = add_f32x2(sum2[(c >> 1) & 3], f32x2(p0, p1));
-    if constexpr (kScaled) {
-      const float2 f = *reinterpret_cast<const float2*>(v_scale + c);
-      p0 *= f.x;
-      p1 *= f.y;
-    }
-    sr[c >> 1] = Half16<T>::pack(p0, p1);
   }
   float lo, hi;
   f32x2_split(add_f32x2(add_f32x2(sum2[0], sum2[1]), add_f32x2(sum2[2], sum2[3])), lo, hi);
@@ -647,11 +652,16 @@ template <int N>
 __device__ __forceinline__ void scale_columns(uint32_t* sr, const float* scale) {
 #pragma unroll
   for (int c = 0; c < N; c += 4) {
-    const float4 f = *reinterpret_cast<const float4*>(scale + c);
-    sr[c] = __float_as_uint(__uint_as_float(sr[c]) * f.x);
-    sr[c + 1] = __float_as_uint(__uint_as_float(sr[c + 1]) * f.y);
-    sr[c + 2] = __float_as_uint(__uint_as_float(sr[c + 2]) * f.z);
-    sr[c + 3] = __float_as_uint(__uint_as_float(sr[c + 3]) * f.w);
+    const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(scale + c);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float a, b;
+      f32x2_split(mul_f32x2(f32x2(__uint_as_float(sr[c + 2 * i]), __uint_as_float(sr[c + 2 * i + 1])),
+                            i ? f.y : f.x),
+                  a, b);
+      sr[c + 2 * i] = __float_as_uint(a);
+      sr[c + 2 * i + 1] = __float_as_uint(b);
+    }
   }
 }
 
@@ -662,6 +672,10 @@ __device__ __forceinline__ void spread16(const uint4& raw, float scale, uint32_t
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint32_t h[2];
+    if constexpr (!kScaled && std::is_same_v<T, __nv_bfloat16> && std::is_same_v<Code, CodeI8>) {
+      CodeI8::decode4_bf16(r[i], out[2 * i], out[2 * i + 1]);
+      continue;
+    }
     Code::decode4(r[i], h[0], h[1]);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -681,23 +695,22 @@ __device__ __forceinline__ void spread16(const uint4& raw, float scale, uint32_t
 template <typename T>
 constexpr bool kCkScaleP = std::is_same_v<T, __nv_bfloat16>;
 
-// Two warps between TMA and the tensor core (the scheduler's, which hands out units on the side, and the one
-// that 16-bit pages leave idle: more warps would take registers from the softmax): the codes of a tile (128
-// keys x 128 bytes) lie in the first half of its 16-bit place, a row where its first 64 values will be, so that
-// the 8 lanes of a row read it and then write over it. K keeps its codes, which are exact in T, and scores
-// are scaled in fp32 by the softmax warps, as lse is an output. A lane looks up the scales of two rows of its
-// warp, a tile ahead. Rows of keys past the context are zero, like those without a page.
-template <typename T, typename Code>
-__device__ __forceinline__ void code_tiles(const ChunkParams& p, CkBarriers* bars, uint8_t* sK,
-                                           uint8_t* sV, int warp, CkScheduler* sched) {
+// Two warps between TMA and the tensor core, one for K (warp 11, which 16-bit pages leave idle) and one for
+// V (the scheduler's, which hands out units on the side): K of a tile must not wait for V of the one before.
+// The codes of a tile (128 keys x 128 bytes, 128-byte swizzle) lie in the first half of its 16-bit place, a row
+// where its first 64 values will be, so that the 8 lanes of a row read it and then write over it. Lanes are given
+// rows r and r ^ 5 such that neither the reads nor the writes of 8 lanes meet a bank twice.
+// K keeps its codes, which are exact in T, and scores are scaled in fp32 by the softmax warps, as lse is an
+// output. A lane looks up the scales of four rows, a tile ahead. Rows of keys past the context are zero, like those
+// without a page.
+template <typename T, typename Code, bool kV>
+__device__ __forceinline__ void code_tiles(const ChunkParams& p, CkBarriers* bars, uint8_t* tiles,
+                                           CkScheduler* sched) {
+  constexpr bool kScaled = kV && !kCkScaleP<T>;  // the codes are scaled here
   const ChunkBatch& pb = p.b;
   const int lane = threadIdx.x & 31;
-  const int piece = lane & 7, sub = lane >> 3;  // this lane's 16 codes of rows 4 warp + sub + 8 i
-  // the rows whose scales it looks up: 4 warp + (lane & 3) + 8 i for i = lane / 4 and lane / 4 + 8
-  const int mine = 4 * warp + (lane & 3) + 8 * (lane >> 2);
-  // two 16-byte chunks of a row's column, in an order that keeps the 8 lanes of a row off each
-  // other's banks (the two columns' chunks share them)
-  const int column = piece >> 2, chunk = (piece & 3) * 2;
+  const int q = lane & 3, flip = (lane >> 2) & 1 ? 5 : 0, column = (lane >> 3) & 1, pair = lane >> 4;
+  const int piece = column * 4 + q;
   int g = 0, next_unit = 0;
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -710,17 +723,17 @@ __device__ __forceinline__ void code_tiles(const ChunkParams& p, CkBarriers* bar
 #pragma unroll 1
   for (const CkUnit* up; (up = ck_next<true>(bars, next_unit, p.err)) != nullptr;) {
     const CkUnit& u = *up;
-    float next[2][2];  // k and v of the next tile's rows `mine` and `mine` + 64
+    float k_next[4], v_next[4];  // of the next tile's rows lane, lane + 32, ...
     auto look_up = [&](const int* page, int j) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const bool held = page[h] != pb.num_blocks &&
-                          ck_tile(u, j) * kChunkTile + mine + 64 * h < u.keys;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv)
-          next[kv][h] = held ? p.scale[kv][page[h] * p.ss[kv][0] + u.hk * p.ss[kv][1] +
-                                           (mine & (kChunkPage - 1)) * p.ss[kv][2]]
-                             : 0.f;
+      for (int h = 0; h < 4; ++h) {
+        const int row = lane + 32 * h, pg = page[h >> 1];
+        const bool held = pg != pb.num_blocks && ck_tile(u, j) * kChunkTile + row < u.keys;
+        const int64_t slot = row & (kChunkPage - 1);
+        k_next[h] = v_next[h] = 0.f;
+        if (held && !kV) k_next[h] = p.scale[0][pg * p.ss[0][0] + u.hk * p.ss[0][1] + slot * p.ss[0][2]];
+        if (held && kV != kCkScaleP<T>)
+          v_next[h] = p.scale[1][pg * p.ss[1][0] + u.hk * p.ss[1][1] + slot * p.ss[1][2]];
       }
     };
     int page[2];
@@ -729,55 +742,48 @@ __device__ __forceinline__ void code_tiles(const ChunkParams& p, CkBarriers* bar
 #pragma unroll 1
     for (int j = u.j0; j < u.j1; ++j, ++g) {
       const int s = g % kCkStages;
-      const uint32_t par = (g / kCkStages) & 1;
       const int live = u.keys - ck_tile(u, j) * kChunkTile;  // rows of keys in the context
-      const float v_scale[2] = {next[1][0], next[1][1]};
+      float v_scale[4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        bars->k_scale[g % kCkScaleSlots][mine + 64 * h] = next[0][h];
-        if (kCkScaleP<T>) bars->v_scale[g % kCkScaleSlots][mine + 64 * h] = next[1][h];
+      for (int h = 0; h < 4; ++h) {
+        v_scale[h] = v_next[h];
+        if (!kV) {
+          bars->k_scale[g % kCkScaleSlots][lane + 32 * h] = k_next[h];
+          if (kCkScaleP<T>) bars->v_scale[g % kCkScaleSlots][lane + 32 * h] = v_next[h];
+        }
       }
       if (j + 1 < u.j1)
         for (int h = 0; h < 2; ++h) page[h] = chunk_page(pb, u.b, u.keys, ck_tile(u, j + 1), h);
+      uint8_t* tile = tiles + s * kChunkTileBytes;
+      wait(kV ? &bars->vc_full[s] : &bars->kc_full[s], (g / kCkStages) & 1);
 #pragma unroll 1
-      for (int kv = 0; kv < 2; ++kv) {
-        uint8_t* row = (kv ? sV : sK) + s * kChunkTileBytes + (4 * warp + sub) * 128;
-        wait(kv ? &bars->vc_full[s] : &bars->kc_full[s], par);
-#pragma unroll 1
-        for (int i0 = 0; i0 < 16; i0 += 4) {  // four rows' reads before their writes
-          uint4 raw[4];
+      for (int i0 = 0; i0 < 32; i0 += 4) {  // 16 rows' reads before their writes
+        uint4 raw[4];
+        int row[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            raw[i] = *reinterpret_cast<const uint4*>(row + (i0 + i) * 8 * 128 + piece * 16);
-            if (4 * warp + sub + 8 * (i0 + i) >= live) raw[i] = make_uint4(0, 0, 0, 0);
-          }
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = 4 * warp + sub + 8 * (i0 + i);
-            uint32_t v[8];
-            if (!kCkScaleP<T> && kv)
-              spread16<T, Code, true>(raw[i],
-                                      __shfl_sync(0xffffffffu, i0 < 8 ? v_scale[0] : v_scale[1],
-                                                  ((i0 + i) & 7) * 4 + sub),
-                                      v);
-            else
-              spread16<T, Code, false>(raw[i], 1.f, v);
-            uint8_t* at = row + (i0 + i) * 8 * 128 + column * kChunkHalf;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int which = h ^ column;
-              const uint4 w = which ? make_uint4(v[4], v[5], v[6], v[7])
-                                    : make_uint4(v[0], v[1], v[2], v[3]);
-              *reinterpret_cast<uint4*>(at + (((chunk + which) ^ (r & 7)) << 4)) = w;
-            }
-          }
+        for (int i = 0; i < 4; ++i) {
+          row[i] = 4 * i0 + 8 * (i >> 1) + (((i & 1) * 2 + pair) ^ flip);
+          raw[i] = *reinterpret_cast<const uint4*>(tile + row[i] * 128 + ((piece ^ (row[i] & 7)) << 4));
+          if (row[i] >= live) raw[i] = make_uint4(0, 0, 0, 0);
         }
-        fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(kv ? &bars->v_full[s] : &bars->k_full[s]);
-        if (kv == 0 && j + 1 < u.j1) look_up(page, j + 1);
+        const float scale4 = i0 < 8 ? v_scale[0] : i0 < 16 ? v_scale[1] : i0 < 24 ? v_scale[2] : v_scale[3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t v[8];
+          spread16<T, Code, kScaled>(
+              raw[i], kScaled ? __shfl_sync(0xffffffffu, scale4, row[i] & 31) : 1.f, v);
+          uint8_t* to = tile + column * kChunkHalf + row[i] * 128;
+          *reinterpret_cast<uint4*>(to + (((2 * q) ^ (row[i] & 7)) << 4)) =
+              make_uint4(v[0], v[1], v[2], v[3]);
+          *reinterpret_cast<uint4*>(to + (((2 * q + 1) ^ (row[i] & 7)) << 4)) =
+              make_uint4(v[4], v[5], v[6], v[7]);
+        }
       }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(kV ? &bars->v_full[s] : &bars->k_full[s]);
+      if (j + 1 < u.j1) look_up(page, j + 1);
     }
     ck_done<true>(bars, next_unit);
     if (sched && sched->open) sched->next();  // (two ahead: the units before it are still at work)
@@ -816,9 +822,9 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       mbar_init(&bars->o_empty[t], 4);
     }
     for (int s = 0; s < kCkStages; ++s) {
-      mbar_init(&bars->k_full[s], kCode ? 2 : 1);
+      mbar_init(&bars->k_full[s], 1);
       mbar_init(&bars->k_empty[s], 1);
-      mbar_init(&bars->v_full[s], kCode ? 2 : 1);
+      mbar_init(&bars->v_full[s], 1);
       mbar_init(&bars->v_empty[s], 1);
       mbar_init(&bars->kc_full[s], 1);
       mbar_init(&bars->vc_full[s], 1);
@@ -962,13 +968,13 @@ __global__ void __launch_bounds__(kCkThreads, 1)
     } else if (warp == 10) {
       CkScheduler sched(pb, p.unit_tokens, kPad, bars, units, p.join + cta, p.err);
       if constexpr (kCode) {
-        code_tiles<T, Code>(p, bars, sK, sV, 0, &sched);
+        code_tiles<T, Code, true>(p, bars, sV, &sched);
       } else {
         while (sched.open) sched.next();
         sched.finish();
       }
     } else if (kCode && warp == 11) {
-      if constexpr (kCode) code_tiles<T, Code>(p, bars, sK, sV, 1, nullptr);
+      if constexpr (kCode) code_tiles<T, Code, false>(p, bars, sK, nullptr);
     } else if (warp == 9 && lane == 0) {
       // ---------------------------------------------------------- UMMA issuer
       constexpr uint32_t idesc_qk = umma_idesc<T>(128, 128, 0, 0);
@@ -1241,7 +1247,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
               l *= alpha;
             }
           }
-          l += ck_exp<T, kCode && kCkScaleP<T>>(sr, sl2, m == -INFINITY ? 0.f : m,
+          l += ck_exp<T, kCode, kCode && kCkScaleP<T>>(sr, sl2, m == -INFINITY ? 0.f : m,
                                                 bars->v_scale[g % kCkScaleSlots]);
           tmem_st32(tS + 0, sr);
           tmem_st32(tS + 32, sr + 32);

@@ -37,6 +37,20 @@ struct CodeI8 {
     lo = half2_of<0x4140>(b);
     hi = half2_of<0x4342>(b);
   }
+  // The same as bf16: 0x43uu is 128 + uu for uu < 128, and 256 for uu = 128, so a code is the difference of its low
+  // seven bits' number and its sign bit's.
+  __device__ static __forceinline__ void decode4_bf16(uint32_t v, uint32_t& lo, uint32_t& hi) {
+    uint32_t x[2];
+    asm("prmt.b32 %0, %1, 0x43434343, 0x4140;" : "=r"(x[0]) : "r"(v));
+    asm("prmt.b32 %0, %1, 0x43434343, 0x4342;" : "=r"(x[1]) : "r"(v));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t a = x[i] & 0xff7fff7fu, b = x[i] & 0xff80ff80u;
+      const __nv_bfloat162 d =
+          __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+      (i ? hi : lo) = *reinterpret_cast<const uint32_t*>(&d);
+    }
+  }
 };
 
 struct CodeE4M3 {
