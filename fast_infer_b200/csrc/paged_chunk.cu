@@ -695,101 +695,98 @@ __device__ __forceinline__ void spread16(const uint4& raw, float scale, uint32_t
 template <typename T>
 constexpr bool kCkScaleP = std::is_same_v<T, __nv_bfloat16>;
 
-// Two warps between TMA and the tensor core, one for K (warp 11, which 16-bit pages leave idle) and one for
-// V (the scheduler's, which hands out units on the side): K of a tile must not wait for V of the one before.
-// The codes of a tile (128 keys x 128 bytes, 128-byte swizzle) lie in the first half of its 16-bit place, a row
-// where its first 64 values will be, so that the 8 lanes of a row read it and then write over it. Lanes are given
-// rows r and r ^ 5 such that neither the reads nor the writes of 8 lanes meet a bank twice.
-// K keeps its codes, which are exact in T, and scores are scaled in fp32 by the softmax warps, as lse is an
-// output. A lane looks up the scales of four rows, a tile ahead. Rows of keys past the context are zero, like those
-// without a page.
-template <typename T, typename Code, bool kV>
-__device__ __forceinline__ void code_tiles(const ChunkParams& p, CkBarriers* bars, uint8_t* tiles,
-                                           CkScheduler* sched) {
-  constexpr bool kScaled = kV && !kCkScaleP<T>;  // the codes are scaled here
-  const ChunkBatch& pb = p.b;
+// Between TMA and the tensor core: a warpgroup spreads the codes of a tile (128 keys x 128 bytes, 128-byte swizzle),
+// which lie in the first half of the tile's 16-bit place, a row where its first 64 values will be, so that the 8
+// lanes of a row read it and then write over it. Lanes are given rows r and r ^ 5 such that neither the reads
+// nor the writes of 8 lanes meet a bank twice. `scale` is that of row 32 * quarter + lane, for kScaled.
+template <typename T, typename Code, bool kScaled>
+__device__ __forceinline__ void spread_tile(uint8_t* tile, int live, int quarter, float scale) {
   const int lane = threadIdx.x & 31;
   const int q = lane & 3, flip = (lane >> 2) & 1 ? 5 : 0, column = (lane >> 3) & 1, pair = lane >> 4;
   const int piece = column * 4 + q;
-  int g = 0, next_unit = 0;
-  bool ok = true;
-  auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.err));
-  };
-  if (sched) {
-    sched->next();
-    if (sched->open) sched->next();
-  }
 #pragma unroll 1
-  for (const CkUnit* up; (up = ck_next<true>(bars, next_unit, p.err)) != nullptr;) {
-    const CkUnit& u = *up;
-    float k_next[4], v_next[4];  // of the next tile's rows lane, lane + 32, ...
-    auto look_up = [&](const int* page, int j) {
+  for (int i0 = 0; i0 < 8; i0 += 4) {  // 16 rows' reads before their writes
+    uint4 raw[4];
+    int row[4];
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const int row = lane + 32 * h, pg = page[h >> 1];
-        const bool held = pg != pb.num_blocks && ck_tile(u, j) * kChunkTile + row < u.keys;
-        const int64_t slot = row & (kChunkPage - 1);
-        k_next[h] = v_next[h] = 0.f;
-        if (held && !kV) k_next[h] = p.scale[0][pg * p.ss[0][0] + u.hk * p.ss[0][1] + slot * p.ss[0][2]];
-        if (held && kV != kCkScaleP<T>)
-          v_next[h] = p.scale[1][pg * p.ss[1][0] + u.hk * p.ss[1][1] + slot * p.ss[1][2]];
-      }
-    };
-    int page[2];
-    for (int h = 0; h < 2; ++h) page[h] = chunk_page(pb, u.b, u.keys, ck_tile(u, u.j0), h);
-    look_up(page, u.j0);
-#pragma unroll 1
-    for (int j = u.j0; j < u.j1; ++j, ++g) {
-      const int s = g % kCkStages;
-      const int live = u.keys - ck_tile(u, j) * kChunkTile;  // rows of keys in the context
-      float v_scale[4];
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        v_scale[h] = v_next[h];
-        if (!kV) {
-          bars->k_scale[g % kCkScaleSlots][lane + 32 * h] = k_next[h];
-          if (kCkScaleP<T>) bars->v_scale[g % kCkScaleSlots][lane + 32 * h] = v_next[h];
-        }
-      }
-      if (j + 1 < u.j1)
-        for (int h = 0; h < 2; ++h) page[h] = chunk_page(pb, u.b, u.keys, ck_tile(u, j + 1), h);
-      uint8_t* tile = tiles + s * kChunkTileBytes;
-      wait(kV ? &bars->vc_full[s] : &bars->kc_full[s], (g / kCkStages) & 1);
-#pragma unroll 1
-      for (int i0 = 0; i0 < 32; i0 += 4) {  // 16 rows' reads before their writes
-        uint4 raw[4];
-        int row[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          row[i] = 4 * i0 + 8 * (i >> 1) + (((i & 1) * 2 + pair) ^ flip);
-          raw[i] = *reinterpret_cast<const uint4*>(tile + row[i] * 128 + ((piece ^ (row[i] & 7)) << 4));
-          if (row[i] >= live) raw[i] = make_uint4(0, 0, 0, 0);
-        }
-        __syncwarp();
-        const float scale4 = i0 < 8 ? v_scale[0] : i0 < 16 ? v_scale[1] : i0 < 24 ? v_scale[2] : v_scale[3];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t v[8];
-          spread16<T, Code, kScaled>(
-              raw[i], kScaled ? __shfl_sync(0xffffffffu, scale4, row[i] & 31) : 1.f, v);
-          uint8_t* to = tile + column * kChunkHalf + row[i] * 128;
-          *reinterpret_cast<uint4*>(to + (((2 * q) ^ (row[i] & 7)) << 4)) =
-              make_uint4(v[0], v[1], v[2], v[3]);
-          *reinterpret_cast<uint4*>(to + (((2 * q + 1) ^ (row[i] & 7)) << 4)) =
-              make_uint4(v[4], v[5], v[6], v[7]);
-        }
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(kV ? &bars->v_full[s] : &bars->k_full[s]);
-      if (j + 1 < u.j1) look_up(page, j + 1);
+    for (int i = 0; i < 4; ++i) {
+      row[i] = 32 * quarter + 4 * i0 + 8 * (i >> 1) + (((i & 1) * 2 + pair) ^ flip);
+      raw[i] = *reinterpret_cast<const uint4*>(tile + row[i] * 128 + ((piece ^ (row[i] & 7)) << 4));
+      if (row[i] >= live) raw[i] = make_uint4(0, 0, 0, 0);
     }
-    ck_done<true>(bars, next_unit);
-    if (sched && sched->open) sched->next();  // (two ahead: the units before it are still at work)
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t v[8];
+      spread16<T, Code, kScaled>(raw[i],
+                                 kScaled ? __shfl_sync(0xffffffffu, scale, row[i] & 31) : 1.f, v);
+      uint8_t* to = tile + column * kChunkHalf + row[i] * 128;
+      *reinterpret_cast<uint4*>(to + (((2 * q) ^ (row[i] & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<uint4*>(to + (((2 * q + 1) ^ (row[i] & 7)) << 4)) =
+          make_uint4(v[4], v[5], v[6], v[7]);
+    }
   }
-  if (sched) sched->finish();
+  fence_proxy_async_smem();
+  __syncwarp();
 }
+
+// The softmax warpgroups spread codes where they would wait: after the weights of tile j, the first one K of
+// tile j + 2 (its stage is free since S of tile j), the second one V of tile j + 1, and both the first tiles of
+// the next unit before a unit's end. (Warps of their own for it: four cost the softmax its registers,
+// two were slower than the tensor core, 408 us for 8 trees over 20 to 32 k keys.)
+// K keeps its codes, which are exact in T, and scores are scaled in fp32, as lse is an output. A thread looks up
+// the scales of one row. Rows of keys past the context are zero, like those without a page.
+template <typename T, typename Code>
+struct CodeSpreader {
+  const ChunkParams& p;
+  CkBarriers* bars;
+  uint8_t* tiles;  // K's or V's
+  int t, quarter, row;
+  int g;           // tiles spread so far
+  float k, v;      // scales of `row` of the next one
+
+  __device__ __forceinline__ CodeSpreader(const ChunkParams& p, CkBarriers* bars, uint8_t* sK,
+                                          uint8_t* sV, int t, int quarter)
+      : p(p), bars(bars), tiles(t ? sV : sK), t(t), quarter(quarter),
+        row(quarter * 32 + (threadIdx.x & 31)), g(0), k(0.f), v(0.f) {}
+
+  __device__ __forceinline__ int page(const CkUnit& u, int j) const {
+    return chunk_page(p.b, u.b, u.keys, ck_tile(u, j), row >> 6);
+  }
+  __device__ __forceinline__ void look_up(const CkUnit& u, int j, int page) {
+    const bool held = page != p.b.num_blocks && ck_tile(u, j) * kChunkTile + row < u.keys;
+    const int64_t slot = row & (kChunkPage - 1);
+    k = v = 0.f;
+    if (held && t == 0) k = p.scale[0][page * p.ss[0][0] + u.hk * p.ss[0][1] + slot * p.ss[0][2]];
+    if (held && (t == 0) == kCkScaleP<T>)
+      v = p.scale[1][page * p.ss[1][0] + u.hk * p.ss[1][1] + slot * p.ss[1][2]];
+  }
+  // Tile j of the unit, whose scales have been looked up.
+  template <typename Wait>
+  __device__ __forceinline__ void spread(const CkUnit& u, int j, Wait&& wait) {
+    const int s = g % kCkStages;
+    if (t == 0) {
+      bars->k_scale[g % kCkScaleSlots][row] = k;
+      if (kCkScaleP<T>) bars->v_scale[g % kCkScaleSlots][row] = v;
+    }
+    wait(t ? &bars->vc_full[s] : &bars->kc_full[s], (g / kCkStages) & 1);
+    const int live = u.keys - ck_tile(u, j) * kChunkTile;
+    if (kCkScaleP<T> || t == 0)
+      spread_tile<T, Code, false>(tiles + s * kChunkTileBytes, live, quarter, 1.f);
+    else
+      spread_tile<T, Code, true>(tiles + s * kChunkTileBytes, live, quarter, v);
+    if ((threadIdx.x & 31) == 0) mbar_arrive(t ? &bars->v_full[s] : &bars->k_full[s]);
+    ++g;
+  }
+  // The tiles that a unit begins with.
+  template <typename Wait>
+  __device__ __forceinline__ void begin(const CkUnit& u, Wait&& wait) {
+    for (int j = u.j0; j < min(u.j0 + 2 - t, u.j1); ++j) {
+      look_up(u, j, page(u, j));
+      spread(u, j, wait);
+    }
+  }
+};
 
 // Code: the type of 8-bit pages (void: 16-bit pages of type T).
 template <typename T, bool kCap, bool kAlibi, bool kNarrow, bool kTree, typename Code>
@@ -822,9 +819,9 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       mbar_init(&bars->o_empty[t], 4);
     }
     for (int s = 0; s < kCkStages; ++s) {
-      mbar_init(&bars->k_full[s], 1);
+      mbar_init(&bars->k_full[s], kCode ? 4 : 1);
       mbar_init(&bars->k_empty[s], 1);
-      mbar_init(&bars->v_full[s], 1);
+      mbar_init(&bars->v_full[s], kCode ? 4 : 1);
       mbar_init(&bars->v_empty[s], 1);
       mbar_init(&bars->kc_full[s], 1);
       mbar_init(&bars->vc_full[s], 1);
@@ -833,7 +830,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
     mbar_init(&bars->merge, 8);
     for (int s = 0; s < kCkSlots; ++s) {
       mbar_init(&bars->unit_full[s], 1);
-      mbar_init(&bars->unit_empty[s], kCode ? 12 : 10);  // TMA, UMMA, the 8 softmax (and 2 code) warps
+      mbar_init(&bars->unit_empty[s], 10);  // TMA, UMMA, the 8 softmax warps
     }
     fence_barrier_init();
   }
@@ -967,14 +964,8 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       }
     } else if (warp == 10) {
       CkScheduler sched(pb, p.unit_tokens, kPad, bars, units, p.join + cta, p.err);
-      if constexpr (kCode) {
-        code_tiles<T, Code, true>(p, bars, sV, &sched);
-      } else {
-        while (sched.open) sched.next();
-        sched.finish();
-      }
-    } else if (kCode && warp == 11) {
-      if constexpr (kCode) code_tiles<T, Code, false>(p, bars, sK, nullptr);
+      while (sched.open) sched.next();
+      sched.finish();
     } else if (warp == 9 && lane == 0) {
       // ---------------------------------------------------------- UMMA issuer
       constexpr uint32_t idesc_qk = umma_idesc<T>(128, 128, 0, 0);
@@ -1135,6 +1126,13 @@ __global__ void __launch_bounds__(kCkThreads, 1)
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.err));
     };
+    using Spreader =
+        std::conditional_t<kCode, CodeSpreader<T, std::conditional_t<kCode, Code, CodeI8>>, int>;
+    [[maybe_unused]] auto spreader = [&] {
+      if constexpr (kCode) return Spreader(p, bars, sK, sV, t, quarter);
+      else return 0;
+    }();
+    [[maybe_unused]] bool begun = false;  // the next unit's first tiles are spread
     int next_unit = 0;
 #pragma unroll 1
     for (const CkUnit* up; (up = ck_next<true>(bars, next_unit, p.err)) != nullptr;
@@ -1142,12 +1140,25 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       const CkUnit& u = *up;
       const int rows = t ? u.rows[1] : u.rows[0];
       const bool begins = u.j0 == 0, ends = u.j1 == u.n;
+      if constexpr (kCode) {
+        if (!begun) spreader.begin(u, wait);
+      }
       if constexpr (kNarrow) {
         narrow_unit<T, kCap, kAlibi, kTree>(p, bars, u, sQ + kChunkTileBytes, sV, tmem, t, quarter, lane, sc,
                                      g, uc, merges, cta, ok);
       } else {
       if (rows == 0) {
         g += u.j1 - u.j0;
+        if constexpr (kCode) {  // (the second warpgroup) V is spread all the same
+#pragma unroll 1
+          for (int j = u.j0 + 1; j < u.j1; ++j) {
+            spreader.look_up(u, j, spreader.page(u, j));
+            spreader.spread(u, j, wait);
+          }
+          const CkUnit* un = ck_next<true>(bars, next_unit + 1, p.err);
+          begun = un != nullptr;
+          if (begun) spreader.begin(*un, wait);
+        }
         continue;
       }
       const bool live = row < rows;             // this row is stored
@@ -1164,7 +1175,13 @@ __global__ void __launch_bounds__(kCkThreads, 1)
         // (keys past the context are masked by their number)
         const bool page0 = u.pages_ok || chunk_page(pb, u.b, u.keys, tile, 0) != pb.num_blocks;
         const bool page1 = u.pages_ok || chunk_page(pb, u.b, u.keys, tile, 1) != pb.num_blocks;
+        [[maybe_unused]] const int ahead = j + 2 - t;  // the tile that is spread after this one's weights
+        [[maybe_unused]] int ahead_page = pb.num_blocks;
+        if constexpr (kCode)
+          if (ahead < u.j1) ahead_page = spreader.page(u, ahead);
         wait(&bars->s_full[t], sc & 1);
+        if constexpr (kCode)
+          if (ahead < u.j1) spreader.look_up(u, ahead, ahead_page);
         if (!kCode && t == 0 && k0 + kChunkTile > u.keys) {
           wait(&bars->v_full[g % kCkStages], (g / kCkStages) & 1);
           zero_v_rows(sV + (g % kCkStages) * kChunkTileBytes, max(u.keys - k0, 0), threadIdx.x);
@@ -1269,6 +1286,13 @@ __global__ void __launch_bounds__(kCkThreads, 1)
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->p_full[t]);
+        if constexpr (kCode)
+          if (ahead < u.j1) spreader.spread(u, ahead, wait);
+      }
+      if constexpr (kCode) {
+        const CkUnit* un = ck_next<true>(bars, next_unit + 1, p.err);
+        begun = un != nullptr;
+        if (begun) spreader.begin(*un, wait);
       }
       // ----------------------------------------------------------- epilogue
       wait(&bars->o_full[t], uc & 1);
