@@ -125,12 +125,15 @@ struct CkScheduler {
   int hk, e, b, at;  // `at`: where in the unit this CTA begins
   int i;             // units handed out
   bool open;         // some may be left
+  bool even;         // tokens for two tiles are split evenly over them, not the first one filled
   ChunkSeq q;
   CkJoin join;
 
   __device__ __forceinline__ CkScheduler(const ChunkBatch& p, int unit_tokens, int pad,
-                                         CkBarriers* s, uint32_t units, CkJoin* join_out, int* err)
-      : p(p), s(s), join_out(join_out), err(err), units(units), unit_tokens(unit_tokens), pad(pad) {
+                                         CkBarriers* s, uint32_t units, CkJoin* join_out, int* err,
+                                         bool even)
+      : p(p), s(s), join_out(join_out), err(err), units(units), unit_tokens(unit_tokens), pad(pad),
+        even(even) {
     const int G = gridDim.x, cta = blockIdx.x;
     const uint32_t per_head = s->work[units];
     total = (int64_t)per_head * p.hk;
@@ -153,7 +156,7 @@ struct CkScheduler {
 
   // The next unit into the ring, an invalid one after the last.
   __device__ __forceinline__ void next() {
-    const int cta = blockIdx.x, lane = threadIdx.x & 31, tt = p.tile_tokens, slot = i % kCkSlots;
+    const int cta = blockIdx.x, lane = threadIdx.x & 31, slot = i % kCkSlots;
     if (i >= kCkSlots &&
         !__all_sync(0xffffffffu, mbar_wait(&s->unit_empty[slot], ((i / kCkSlots) - 1) & 1, err))) {
       open = false;
@@ -176,6 +179,9 @@ struct CkScheduler {
       u.pos = q.pos0 + t0;
       u.keys = q.keys;
       u.prefix = p.tree ? q.pos0 : q.prefix;
+      // (where two tiles are needed: 8 trees of 50 to 85 tokens over 20 to 32 k, 366 us, split evenly 349;
+      // with rows for one tile only, a second one would be work for nothing: 99 us, and 109)
+      const int tt = even && t1 - t0 > p.tile_tokens ? (t1 - t0 + 1) / 2 : p.tile_tokens;
       u.rows[0] = min(t1 - t0, tt) * p.group;
       u.rows[1] = max(t1 - t0 - tt, 0) * p.group;
       u.j0 = max(at - pad, 0);
@@ -908,7 +914,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
             if (!ok || u.rows[t] == 0) continue;
             if (qc[t] > 0) ok = mbar_wait(&bars->q_empty[t], (qc[t] - 1) & 1, p.err);
             if (!ok) continue;
-            const int token = u.token + t * pb.tile_tokens;
+            const int token = u.token + t * (kTree ? u.rows[0] / pb.group : pb.tile_tokens);
             uint8_t* dst = sQ + t * kChunkTileBytes;
             mbar_arrive_expect_tx(&bars->q_full[t], q_bytes);
             tma_load_4d(dst, &tm_q, &bars->q_full[t], 0, 0, u.hk, token);
@@ -963,7 +969,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
         }
       }
     } else if (warp == 10) {
-      CkScheduler sched(pb, p.unit_tokens, kPad, bars, units, p.join + cta, p.err);
+      CkScheduler sched(pb, p.unit_tokens, kPad, bars, units, p.join + cta, p.err, kTree && !kNarrow);
       while (sched.open) sched.next();
       sched.finish();
     } else if (warp == 9 && lane == 0) {
@@ -1164,7 +1170,9 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       const bool live = row < rows;             // this row is stored
       const bool warp_live = quarter * 32 < rows;
       const int tok = bars->row_token[row], head = u.hk * pb.group + bars->row_head[row];
-      const int pos = u.pos + t * pb.tile_tokens + tok;
+      // the tile's first token of the unit
+      const int tile0 = t * (kTree ? u.rows[0] / pb.group : pb.tile_tokens);
+      const int pos = u.pos + tile0 + tok;
       float slope2 = 0.f;
       if (kAlibi && live) slope2 = p.f.slopes[head] * kLog2e;
       float m = -INFINITY, l = 0.f;
@@ -1198,7 +1206,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
             c_hi = min(c_tree, u.keys - k0);
             c_pre = 0;
             if (pb.window && live)
-              c_lo = u.prefix + pb.depths[u.token + t * pb.tile_tokens + tok] - pb.window + 1 - k0;
+              c_lo = u.prefix + pb.depths[u.token + tile0 + tok] - pb.window + 1 - k0;
           }
           const bool all = !live || ((c_hi >= kChunkTile && c_lo <= 0) || c_pre >= kChunkTile);
           const bool mask = !__all_sync(0xffffffffu, all && page0 && page1);
@@ -1216,7 +1224,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
                 uint32_t vis = (low_bits(c_hi - cc, 0) & ~low_bits(c_lo - cc, 0)) |
                                low_bits(c_pre - cc, 0);
                 if (kTree && pb.tree && live && cc + 32 > c_tree)
-                  vis |= tree_bits(pb, u.token + t * pb.tile_tokens + tok, cc - c_tree) &
+                  vis |= tree_bits(pb, u.token + tile0 + tok, cc - c_tree) &
                          low_bits(u.keys - k0 - cc, 0);
                 if (!(cc < 64 ? page0 : page1)) vis = 0;
 #pragma unroll
@@ -1300,7 +1308,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       const bool none = m == -INFINITY;
       const float inv = none ? 0.f : 1.f / l;
       const float lse2 = none ? -INFINITY : m + log2f(l);
-      const int64_t out_row = u.token + t * pb.tile_tokens + tok;
+      const int64_t out_row = u.token + tile0 + tok;
       const int64_t part = (int64_t)(cta * 2 + (begins ? 1 : 0)) * p.rows_cap + t * 128 + row;
       T* orow = static_cast<T*>(p.o) + out_row * p.os[0] + head * p.os[1];
       float* prow = p.ws_o + (part & ~31) * 128 + (part & 31) * 4;
@@ -1410,7 +1418,7 @@ __global__ void __launch_bounds__(256, 5) chunk_combine_kernel(const ChunkParams
   }
   const bool none = sum == 0.f;
   const float inv = none ? 0.f : 1.f / sum;
-  const int64_t token = jn.token + t * p.b.tile_tokens + row / p.b.group;
+  const int64_t token = jn.token + (t ? jn.rows[0] / p.b.group : 0) + row / p.b.group;
   const int head = jn.hk * p.b.group + row % p.b.group;
   uint4 pk;
   pk.x = Half16<T>::pack(acc[0] * inv, acc[1] * inv);

@@ -214,6 +214,9 @@ struct SaPart {  // what a CTA tells the others about its slice
   int lump_count;
   uint64_t mass, lump_mass;
 };
+constexpr int kSaList = 1024;  // candidates that one CTA finishes on its own
+constexpr int kSaListK = 512;  // top_k up to which a list is tried
+
 struct SaShared {
   double tab[32];
   uint64_t step_mass[kSaWarps * kSaSteps];
@@ -224,7 +227,7 @@ struct SaShared {
   // the bin that a search chose
   uint64_t above, held;
   int64_t tie_base[2];
-  int tie_end;
+  int tie_end, list_n;
   uint32_t edge[2];
   int bin;
   uint32_t min_key;
@@ -239,7 +242,8 @@ constexpr bool kSaTable = kSaValueBins<T> > 0 && kSaValueBins<T> * 8 <= 32768;
 template <typename T>
 constexpr int kSaHistBytes = kSaTable<T>                ? kSaValueBins<T> * 8
                              : kSaValueBins<T> > 0 ? kSaValueBins<T> * 4
-                                                   : 2 * kSaBins * 12;
+                                                   : 2 * kSaBins * 12 + kSaList * 8;
+static_assert(kSaList * 12 <= 2 * kSaBins * 12, "a list's weights and order take the histograms' place");
 
 // Sums over the block's threads before this one, and of all, of N 64-bit values. `warp_sums`: N x kSaWarps.
 template <int N>
@@ -279,6 +283,112 @@ __device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
   return v;
+}
+
+// Sampling from a list of candidates, by one CTA: list[i] = key << 32 | ~index, all of the row's first k among them
+// (and whatever ties with the last or lies beside it). Ranks are counted, n^2 / threads comparisons: of the list as it is
+// for top-k and top-p, then of the indexes of what stays for the running sum.
+__device__ __forceinline__ void sample_list(SaShared* s, const uint64_t* list, uint64_t* weights, int* order,
+                                            int n, const Row& row, int64_t k, float top_p,
+                                            uint32_t min_key, float u, int32_t* out) {
+  constexpr int kEach = kSaList / kSaThreads;
+  const int tid = threadIdx.x;
+  int rank[kEach];
+  uint64_t mine[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = tid + e * kSaThreads;
+    rank[e] = 0;
+    mine[e] = i < n ? list[i] : 0;
+  }
+#pragma unroll 4
+  for (int j = 0; j < n; ++j) {
+    const uint64_t other = list[j];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) rank[e] += other > mine[e];
+  }
+  // the first k, in order
+  const int m = (int)min((int64_t)n, k);
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = tid + e * kSaThreads;
+    if (i < n && rank[e] < m) {
+      const float x = of_key((uint32_t)(mine[e] >> 32));
+      weights[rank[e]] = x >= row.floor_x ? weight(row, s->tab, x) : 0;
+    }
+  }
+  __syncthreads();
+  uint64_t w[kEach], sum = 0, before, all;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = tid * kEach + e;
+    w[e] = i < m ? weights[i] : 0;
+    sum += w[e];
+  }
+  block_exclusive<1>(&sum, s->scan, &before, &all);
+  // how many of them top-p keeps: those before which the mass is below its share
+  const double share = top_p < 1.f ? fmax((double)top_p * (double)all, 1.0) : INFINITY;
+  int stay = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    stay += tid * kEach + e < m && (double)before < share;
+    before += w[e];
+  }
+  if (tid == 0) s->bin = 0;
+  __syncthreads();
+  stay = __reduce_add_sync(0xffffffffu, stay);
+  if ((tid & 31) == 0 && stay) atomicAdd(&s->bin, stay);
+  __syncthreads();
+  stay = s->bin;
+  __syncthreads();
+  // the kept ones by index
+  bool in[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = tid + e * kSaThreads;
+    in[e] = i < n && rank[e] < stay && (uint32_t)(mine[e] >> 32) >= min_key;
+    if (i < n) order[i] = in[e] ? (int)~(uint32_t)mine[e] : INT_MAX;
+    rank[e] = 0;
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int j = 0; j < n; ++j) {
+    const int other = order[j];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) rank[e] += other < (int)~(uint32_t)mine[e];
+  }
+  for (int i = tid; i < kSaList; i += kSaThreads) weights[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    if (!in[e]) continue;
+    const float x = of_key((uint32_t)(mine[e] >> 32));
+    weights[rank[e]] = x >= row.floor_x ? weight(row, s->tab, x) : 0;
+  }
+  __syncthreads();
+  sum = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    w[e] = weights[tid * kEach + e];
+    sum += w[e];
+  }
+  block_exclusive<1>(&sum, s->scan, &before, &all);
+  const double target = (double)u * (double)all;
+  const bool none = !((double)all > target);
+  if (tid == 0) s->bin = -1;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    if (w[e] > 0 && (none ? before + w[e] == all
+                          : (double)(before + w[e]) > target &&
+                                (before == 0 || !((double)before > target))))
+      s->bin = tid * kEach + e;
+    before += w[e];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kEach; ++e)
+    if (in[e] && rank[e] == s->bin) *out = (int32_t)~(uint32_t)mine[e];
 }
 
 // A cut: tokens whose key is above `key` stay, and of those that have it the first `ties` by index.
@@ -437,6 +547,59 @@ __device__ __forceinline__ Cut tighter(const Cut& a, const Cut& b) {
   return a.ties < b.ties ? a : b;
 }
 
+// Lists the row's first `want` tokens, and those beside the last of them, in the first CTA's `list`: all that lie in the bins of
+// M - x (of a search's first level) up to the one where the count reaches `want`. Their number; -1 where the list
+// is too short for them.
+template <typename T>
+__device__ __forceinline__ int candidates(cg::cluster_group& cluster, SaShared* s,
+                                          uint32_t (*hists)[kSaBins][3], uint64_t* list, const T* x,
+                                          int steps, int chunk_base, int base, const Row& row,
+                                          uint32_t lo_key, int64_t want, int& level) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int ctas = (int)cluster.num_blocks();
+  const float range = row.top - of_key(lo_key);
+  const float scale = range > 0.f && range < FLT_MAX ? (float)(kSaBins - 1) / range : 0.f;
+  uint32_t(*hist)[3] = hists[level & 1];
+  const float least = of_key(lo_key);
+#pragma unroll 1
+  for (int st = 0; st < steps; ++st) {
+    float v[8];
+    load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (v[i] >= least) atomicAdd(&hist[linear_bin(row.top, scale, v[i])][0], 1u);
+  }
+  if (tid == 0) s->bin = -1;
+  cluster.sync();
+  ++level;
+  uint64_t mine = 0, before, all;
+  for (int r = 0; r < ctas; ++r) mine += *cluster.map_shared_rank(&hist[tid][0], r);
+  block_exclusive<1>(&mine, s->scan, &before, &all);
+  if (before < (uint64_t)want && before + mine >= (uint64_t)want) {
+    s->bin = tid;
+    s->held = before + mine;
+  }
+  __syncthreads();
+  const int bin = s->bin;
+  const int n = bin < 0 || s->held > kSaList ? -1 : (int)s->held;
+  if (n >= 0) {
+    uint64_t* to = cluster.map_shared_rank(list, 0);
+    int* count = cluster.map_shared_rank(&s->list_n, 0);
+#pragma unroll 1
+    for (int st = 0; st < steps; ++st) {
+      const int at = chunk_base + st * kSaStep + lane * 8;
+      float v[8];
+      load8<T>(x + at, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (v[i] >= least && linear_bin(row.top, scale, v[i]) <= bin)
+          to[atomicAdd(count, 1)] = (uint64_t)key_of(v[i]) << 32 | (uint32_t)~(base + at + i);
+    }
+  }
+  cluster.sync();
+  return n;
+}
+
 // The first value at which the running count passes `want` - 1, or the running mass reaches `target`: a thread has
 // kEach bins, whose count and mass are `sums`, with `before` before them. Its warp then takes a lane per bin. False: it lies in the lump (or nowhere).
 struct ValueCut {
@@ -517,6 +680,7 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
   const int steps = a.chunk / kSaStep, chunk_base = warp * a.chunk;
   for (int i = tid; i < kSaHistBytes<T> / 4; i += kSaThreads) counts[i] = 0;
   if (tid < 32) s->tab[tid] = exp2(tid / 32.0);
+  if (tid == 0) s->list_n = 0;
   grid_dep_wait();
   grid_dep_launch();
   // The slice into shared memory: 16 bytes at a time from the first aligned token on (rows of an odd
@@ -846,6 +1010,21 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
   if (!counted) {
     int level = 0;
     uint64_t drop = 0;
+    if constexpr (sizeof(T) == 4) {
+      // few tokens stay: one CTA takes them (128256 fp32, top-k of 50, top-p and min-p: 36 us, 19 so)
+      if (k > 0 && k <= kSaListK && k <= with) {
+        uint64_t* list = reinterpret_cast<uint64_t*>(&hists[2][0][0]);
+        const int n = candidates<T>(cluster, s, hists, list, x, steps, chunk_base, base, row, key_of(low), k,
+                                    level);
+        if (n >= 0) {
+          if (rank == 0)
+            sample_list(s, list, reinterpret_cast<uint64_t*>(counts),
+                        reinterpret_cast<int*>(counts) + 2 * kSaList, n, row, k, top_p, cut.key, u,
+                        a.out + row_id);
+          return;
+        }
+      }
+    }
     if (k > 0 && k < a.vocab) {
       // as many threads as `with` have a logit of at least `low`
       const float from = k <= with ? low : least;
