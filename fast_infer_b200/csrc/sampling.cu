@@ -232,11 +232,17 @@ struct SaShared {
   int bin;
   uint32_t min_key;
   uint64_t lump_mass[kSaWarps];
+  uint64_t block_mass[128], block_own[128];  // of a block of value bins: of all CTAs, of this one
+  uint32_t block_count[128];
+  uint64_t extra;
 };
 // Histograms: two of generic bins by turns, or one of 16-bit values. Where their weights fit in twice the bytes (bf16)
 // they take the same place afterwards.
 template <typename T>
 constexpr int kSaValueBins = 2 * Bits16<T>::kRegion;
+constexpr int kSaBlock = 128;  // bins that a warp looks at together, four a lane
+template <typename T>
+constexpr int kSaBlocks = kSaValueBins<T> / kSaBlock;
 template <typename T>
 constexpr bool kSaTable = kSaValueBins<T> > 0 && kSaValueBins<T> * 8 <= 32768;
 template <typename T>
@@ -600,8 +606,42 @@ __device__ __forceinline__ int candidates(cg::cluster_group& cluster, SaShared* 
   return n;
 }
 
-// The first value at which the running count passes `want` - 1, or the running mass reaches `target`: a thread has
-// kEach bins, whose count and mass are `sums`, with `before` before them. Its warp then takes a lane per bin. False: it lies in the lump (or nowhere).
+// Four value bins a lane of block `block`: counts of all CTAs and of this one, keys (0: none) and weights.
+template <typename T>
+struct BinQuad {
+  uint32_t n[4], own[4], key[4];
+  uint64_t w[4];
+  __device__ __forceinline__ BinQuad(cg::cluster_group& cluster, const uint32_t* counts, const Row& row,
+                                     const double* tab, const Values& v, int block) {
+    const int bin = block * kSaBlock + (threadIdx.x & 31) * 4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) n[j] = 0;
+    for (int r = 0; r < (int)cluster.num_blocks(); ++r) {
+      const uint4 h = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(counts, r) + bin);
+      n[0] += h.x;
+      n[1] += h.y;
+      n[2] += h.z;
+      n[3] += h.w;
+    }
+    const uint4 mine = *reinterpret_cast<const uint4*>(counts + bin);
+    own[0] = mine.x;
+    own[1] = mine.y;
+    own[2] = mine.z;
+    own[3] = mine.w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      key[j] = bin_key<T>(v, bin + j);
+      w[j] = 0;
+      if (n[j] > 0) {
+        const float x = Bits16<T>::value(key[j]);
+        if (x >= row.floor_x) w[j] = weight(row, tab, x);
+      }
+    }
+  }
+};
+
+// The first value at which the running count reaches `want`, or the running mass `target`; thread i has the sums of block
+// i of the bins, with `before` before them. False: it lies in the lump (or nowhere).
 struct ValueCut {
   uint32_t key16;
   uint32_t group;       // tokens that have the value
@@ -612,7 +652,6 @@ __device__ __forceinline__ bool value_cross(cg::cluster_group& cluster, SaShared
                                             const uint32_t* counts, const Row& row, const Values& v,
                                             const uint64_t* sums, const uint64_t* before,
                                             uint64_t want, double target, ValueCut& cut) {
-  constexpr int kEach = kSaValueBins<T> / kSaThreads;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool here = kMass ? (double)before[1] < target && (double)(before[1] + sums[1]) >= target
                           : before[0] < want && before[0] + sums[0] >= want;
@@ -627,33 +666,30 @@ __device__ __forceinline__ bool value_cross(cg::cluster_group& cluster, SaShared
   __syncthreads();
   const int owner = s->bin;
   if (owner < 0) return false;
-  if (warp == owner >> 5) {
-    const int bin = owner * kEach + lane;
-    uint32_t n = 0;
-    uint64_t w = 0;
-    const uint32_t key = lane < kEach ? bin_key<T>(v, bin) : 0;
-    if (key != 0) {
-      for (int r = 0; r < (int)cluster.num_blocks(); ++r)
-        n += cluster.map_shared_rank(counts, r)[bin];
-      const float value = Bits16<T>::value(key);
-      if (n > 0 && value >= row.floor_x) w = weight(row, s->tab, value);
-    }
-    uint64_t c = n, m = n * w;
+  if (warp == 0) {
+    const BinQuad<T> q(cluster, counts, row, s->tab, v, owner);
+    uint64_t c = 0, m = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c += q.n[j], m += q.n[j] * q.w[j];
+    uint64_t ci = c, mi = m;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const uint64_t oc = __shfl_up_sync(0xffffffffu, c, off), om = __shfl_up_sync(0xffffffffu, m, off);
-      if (lane >= off) c += oc, m += om;
+      const uint64_t oc = __shfl_up_sync(0xffffffffu, ci, off), om = __shfl_up_sync(0xffffffffu, mi, off);
+      if (lane >= off) ci += oc, mi += om;
     }
-    c += s->held;
-    m += s->above;
-    const uint32_t past = __ballot_sync(
-        0xffffffffu, n > 0 && (kMass ? (double)m >= target : c >= want));
+    uint64_t rc = s->held + ci - c, rm = s->above + mi - m;
     __syncwarp();
-    if (past && lane == __ffs((int)past) - 1) {
-      s->edge[0] = key;
-      s->edge[1] = n;
-      s->held = c - n;
-      s->above = m - n * w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint64_t nc = rc + q.n[j], nm = rm + q.n[j] * q.w[j];
+      if (q.n[j] > 0 && (kMass ? (double)rm < target && (double)nm >= target : rc < want && nc >= want)) {
+        s->edge[0] = q.key[j];
+        s->edge[1] = q.n[j];
+        s->held = rc;
+        s->above = rm;
+      }
+      rc = nc;
+      rm = nm;
     }
   }
   __syncthreads();
@@ -858,7 +894,8 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
   bool counted = false;                   // whether the values' counts tell these
   [[maybe_unused]] Values bins = {};
   if constexpr (sizeof(T) == 2) {
-    constexpr int kEach = kSaValueBins<T> / kSaThreads;
+    constexpr int kBlocks = kSaBlocks<T>, kEach = kBlocks / kSaWarps;
+    static_assert(kBlocks <= 128 && kBlocks % kSaWarps == 0, "a thread per block of bins");
     bins = value_bins<T>(row);
     int lump_n = 0;
     uint64_t lump_m = 0;
@@ -911,33 +948,29 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
       lump_count += cluster.map_shared_rank(&s->part, r)->lump_count;
       lump_mass += cluster.map_shared_rank(&s->part, r)->lump_mass;
     }
-    // the sums of this thread's bins, of all CTAs and of this one
-    uint64_t sums[2] = {0, 0}, before[2], all[2], own_mass = 0;
+    // the sums of every block of bins, of all CTAs and of this one
 #pragma unroll 1
-    for (int i = 0; i < kEach; i += 4) {
-      const int bin = tid * kEach + i;
-      uint32_t n[4] = {0, 0, 0, 0};
-      for (int r = 0; r < ctas; ++r) {
-        const uint4 h = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(counts, r) + bin);
-        n[0] += h.x;
-        n[1] += h.y;
-        n[2] += h.z;
-        n[3] += h.w;
-      }
-      const uint4 mine = *reinterpret_cast<const uint4*>(counts + bin);
-      const uint32_t mine4[4] = {mine.x, mine.y, mine.z, mine.w};
+    for (int i = 0; i < kEach; ++i) {
+      const int block = warp * kEach + i;
+      const BinQuad<T> q(cluster, counts, row, s->tab, bins, block);
+      uint32_t n = 0;
+      uint64_t m = 0, o = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (n[j] == 0) continue;
-        const float v = Bits16<T>::value(bin_key<T>(bins, bin + j));
-        const uint64_t w = v >= row.floor_x ? weight(row, s->tab, v) : 0;
-        sums[0] += n[j];
-        sums[1] += n[j] * w;
-        own_mass += mine4[j] * w;
+      for (int j = 0; j < 4; ++j) n += q.n[j], m += q.n[j] * q.w[j], o += q.own[j] * q.w[j];
+      n = __reduce_add_sync(0xffffffffu, n);
+      m = warp_sum(m);
+      o = warp_sum(o);
+      if (lane == 0) {
+        s->block_count[block] = n;
+        s->block_mass[block] = m;
+        s->block_own[block] = o;
       }
     }
+    __syncthreads();
+    uint64_t sums[2] = {0, 0}, before[2], all[2];
+    if (tid < kBlocks) sums[0] = s->block_count[tid], sums[1] = s->block_mass[tid];
     block_exclusive<2>(sums, s->scan, before, all);
-    if (tid >= kSaThreads / 2) before[0] += lump_count, before[1] += lump_mass;
+    if (tid >= kBlocks / 2) before[0] += lump_count, before[1] += lump_mass;
     all[0] += lump_count;
     all[1] += lump_mass;
     counted = true;
@@ -968,32 +1001,48 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
       const bool lump_in = lump_count > 0 && c.key <= key_of(Bits16<T>::value(lump_lo));
       if (lump_count > 0 && !lump_in && c.key <= key_of(Bits16<T>::value(lump_hi))) counted = false;
       if (counted) {
-        // this CTA's kept mass: bins above the cut, and its share of the ties
+        // this CTA's kept mass: blocks above the cut, and of the one that holds it the bins above and a share of
+        // the ties
         uint64_t m = 0;
-        const uint32_t last = bin_key<T>(bins, tid * kEach + kEach - 1);
-        if (last != 0 && key_of(Bits16<T>::value(last)) > c.key) {
-          m = own_mass;
-        } else if (sums[0] > 0) {
-#pragma unroll 1
-          for (int i = 0; i < kEach; ++i) {
-            const int bin = tid * kEach + i;
-            const uint32_t key16 = bin_key<T>(bins, bin);
-            const float v = Bits16<T>::value(key16);
-            if (key16 == 0 || key_of(v) < c.key) break;
-            int64_t n = counts[bin];
-            if (key_of(v) == c.key && !c.all_ties) {
+        if (tid == 0) {
+          s->bin = -1;
+          s->extra = 0;
+        }
+        __syncthreads();
+        if (tid < kBlocks) {
+          const uint32_t R = Bits16<T>::kRegion, first = tid * kSaBlock;
+          const uint32_t n = first < R ? bins.n1 : bins.n2, at = first < R ? first : first - R;
+          if (at < n) {
+            const uint32_t last = first + min((uint32_t)kSaBlock, n - at) - 1;
+            if (key_of(Bits16<T>::value(bin_key<T>(bins, last))) > c.key) m = s->block_own[tid];
+            else if (key_of(Bits16<T>::value(bin_key<T>(bins, first))) >= c.key) s->bin = tid;
+          }
+        }
+        __syncthreads();
+        if (warp == 0 && s->bin >= 0) {
+          const BinQuad<T> q(cluster, counts, row, s->tab, bins, s->bin);
+          uint64_t o = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t key = q.key[j] ? key_of(Bits16<T>::value(q.key[j])) : 0;
+            int64_t n = q.key[j] && key >= c.key ? q.own[j] : 0;
+            if (key == c.key && q.key[j] && !c.all_ties) {
+              const int bin = s->bin * kSaBlock + lane * 4 + j;
               int64_t ahead = 0;
               for (int r = 0; r < rank; ++r) ahead += cluster.map_shared_rank(counts, r)[bin];
               s->tie_base[0] = ahead;
               s->tie_base[1] = n;
               n = max((int64_t)0, min(n, c.ties - ahead));
             }
-            if (n > 0 && v >= row.floor_x) m += n * weight(row, s->tab, v);
+            o += n * q.w[j];
           }
+          o = warp_sum(o);
+          if (lane == 0) s->extra = o;
         }
         if (tid == 0 && lump_in) m += s->part.lump_mass;
         uint64_t unused;
         block_exclusive<1>(&m, s->scan, &unused, &own);
+        own += s->extra;
         if (!c.all_ties) {
           ties_before = s->tie_base[0];
           own_ties = s->tie_base[1];
