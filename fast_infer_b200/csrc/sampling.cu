@@ -232,7 +232,8 @@ struct SaShared {
   int bin;
   uint32_t min_key;
   uint64_t lump_mass[kSaWarps];
-  uint64_t block_mass[128], block_own[128];  // of a block of value bins: of all CTAs, of this one
+  // of this CTA's share of the blocks of value bins: of all CTAs' tokens, and of each one's
+  uint64_t block_mass[128], block_own[128];
   uint32_t block_count[128];
   uint64_t extra;
 };
@@ -894,8 +895,8 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
   bool counted = false;                   // whether the values' counts tell these
   [[maybe_unused]] Values bins = {};
   if constexpr (sizeof(T) == 2) {
-    constexpr int kBlocks = kSaBlocks<T>, kEach = kBlocks / kSaWarps;
-    static_assert(kBlocks <= 128 && kBlocks % kSaWarps == 0, "a thread per block of bins");
+    constexpr int kBlocks = kSaBlocks<T>;
+    static_assert(kBlocks <= 128 && kBlocks % kSaMaxCluster == 0, "a thread per block of bins");
     bins = value_bins<T>(row);
     int lump_n = 0;
     uint64_t lump_m = 0;
@@ -948,27 +949,37 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
       lump_count += cluster.map_shared_rank(&s->part, r)->lump_count;
       lump_mass += cluster.map_shared_rank(&s->part, r)->lump_mass;
     }
-    // the sums of every block of bins, of all CTAs and of this one
+    // the sums of every block of bins, of all CTAs' tokens and of each one's: a share of the blocks each
+    const int share = kBlocks / ctas;
 #pragma unroll 1
-    for (int i = 0; i < kEach; ++i) {
-      const int block = warp * kEach + i;
+    for (int i = warp; i < share; i += kSaWarps) {
+      const int block = rank * share + i;
       const BinQuad<T> q(cluster, counts, row, s->tab, bins, block);
       uint32_t n = 0;
-      uint64_t m = 0, o = 0;
+      uint64_t m = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) n += q.n[j], m += q.n[j] * q.w[j], o += q.own[j] * q.w[j];
+      for (int j = 0; j < 4; ++j) n += q.n[j], m += q.n[j] * q.w[j];
       n = __reduce_add_sync(0xffffffffu, n);
       m = warp_sum(m);
-      o = warp_sum(o);
       if (lane == 0) {
-        s->block_count[block] = n;
-        s->block_mass[block] = m;
-        s->block_own[block] = o;
+        s->block_count[i] = n;
+        s->block_mass[i] = m;
+      }
+      for (int r = 0; r < ctas; ++r) {
+        const uint4 h = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(counts, r) +
+                                                        block * kSaBlock + lane * 4);
+        const uint64_t o = warp_sum(h.x * q.w[0] + h.y * q.w[1] + h.z * q.w[2] + h.w * q.w[3]);
+        if (lane == 0) s->block_own[r * share + i] = o;
       }
     }
-    __syncthreads();
-    uint64_t sums[2] = {0, 0}, before[2], all[2];
-    if (tid < kBlocks) sums[0] = s->block_count[tid], sums[1] = s->block_mass[tid];
+    cluster.sync();
+    uint64_t sums[2] = {0, 0}, before[2], all[2], own_block = 0;
+    if (tid < kBlocks) {
+      const SaShared* at = cluster.map_shared_rank(s, tid / share);
+      sums[0] = at->block_count[tid % share];
+      sums[1] = at->block_mass[tid % share];
+      own_block = at->block_own[rank * share + tid % share];
+    }
     block_exclusive<2>(sums, s->scan, before, all);
     if (tid >= kBlocks / 2) before[0] += lump_count, before[1] += lump_mass;
     all[0] += lump_count;
@@ -1014,7 +1025,7 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
           const uint32_t n = first < R ? bins.n1 : bins.n2, at = first < R ? first : first - R;
           if (at < n) {
             const uint32_t last = first + min((uint32_t)kSaBlock, n - at) - 1;
-            if (key_of(Bits16<T>::value(bin_key<T>(bins, last))) > c.key) m = s->block_own[tid];
+            if (key_of(Bits16<T>::value(bin_key<T>(bins, last))) > c.key) m = own_block;
             else if (key_of(Bits16<T>::value(bin_key<T>(bins, first))) >= c.key) s->bin = tid;
           }
         }
