@@ -784,13 +784,19 @@ struct CodeSpreader {
     if ((threadIdx.x & 31) == 0) mbar_arrive(t ? &bars->v_full[s] : &bars->k_full[s]);
     ++g;
   }
-  // The tiles that a unit begins with.
+  // Tiles [from, to) of the unit.
   template <typename Wait>
-  __device__ __forceinline__ void begin(const CkUnit& u, Wait&& wait) {
-    for (int j = u.j0; j < min(u.j0 + 2 - t, u.j1); ++j) {
+  __device__ __forceinline__ void run(const CkUnit& u, int from, int to, Wait&& wait) {
+#pragma unroll 1
+    for (int j = from; j < min(to, u.j1); ++j) {
       look_up(u, j, page(u, j));
       spread(u, j, wait);
     }
+  }
+  // The tiles that a unit begins with (see `twin` for those of one row tile).
+  template <typename Wait>
+  __device__ __forceinline__ void begin(const CkUnit& u, Wait&& wait) {
+    run(u, u.j0, u.j0 + (t && u.rows[1] > 0 ? 1 : 2), wait);
   }
 };
 
@@ -982,8 +988,8 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       int sc[2] = {0, 0};  // S tiles issued per tile
       int g = 0;
       bool ok = true;
-      auto issue_s = [&](int t, int kstage) {
-        const uint64_t da = umma_desc_sw128(q_addr + t * kChunkTileBytes, 16, 1024);
+      auto issue_s = [&](int t, int kstage, int qtile) {
+        const uint64_t da = umma_desc_sw128(q_addr + qtile * kChunkTileBytes, 16, 1024);
         const uint64_t db = umma_desc_sw128(k_addr + kstage * kChunkTileBytes, 16, 1024);
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {
@@ -1057,6 +1063,42 @@ __global__ void __launch_bounds__(kCkThreads, 1)
           ++qc[0];
           ++oc[0];
           if (n > 1) ++oc[1];
+        } else if (kTree && u.rows[1] == 0) {
+          // rows for one tile: both warpgroups have it, and alternate key tiles (tile j is that of j & 1)
+          ok = mbar_wait(&bars->q_full[0], qc[0] & 1, p.err);
+          const int sc0 = sc[0], sc1 = sc[1];
+          auto step_s = [&](int j) {
+            const int st = (g + j) % kCkStages, t = j & 1;
+            if (!(ok = mbar_wait(&bars->k_full[st], ((g + j) / kCkStages) & 1, p.err))) return;
+            tc_fence_after();
+            issue_s(t, st, 0);
+            umma_commit(&bars->k_empty[st]);
+            if (j == n - 1) umma_commit(&bars->q_empty[0]);
+          };
+#pragma unroll 1
+          for (int j = -2; ok && j < n; ++j) {
+            if (j < 0) {
+              if (j + 2 < n) step_s(j + 2);
+              continue;
+            }
+            const int st = (g + j) % kCkStages, t = j & 1;
+            ok = mbar_wait(&bars->v_full[st], ((g + j) / kCkStages) & 1, p.err) &&
+                 mbar_wait(&bars->p_full[t], ((t ? sc1 : sc0) + (j >> 1)) & 1, p.err);
+            const int uses = t ? oc[1] : oc[0];
+            if (ok && j < 2 && uses > 0) ok = mbar_wait(&bars->o_empty[t], (uses - 1) & 1, p.err);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(t, st, j < 2);
+            umma_commit(&bars->v_empty[st]);
+            if (j + 2 >= n) umma_commit(&bars->o_full[t]);
+            else step_s(j + 2);  // its scores overwrite those that P was made of
+          }
+          g += n;
+          sc[0] += (n + 1) >> 1;
+          sc[1] += n >> 1;
+          ++qc[0];
+          ++oc[0];
+          if (n > 1) ++oc[1];
         } else {
         ok = mbar_wait(&bars->k_full[g % kCkStages], (g / kCkStages) & 1, p.err);
 #pragma unroll
@@ -1065,7 +1107,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
           ok = mbar_wait(&bars->q_full[t], qc[t] & 1, p.err);
           if (!ok) continue;
           tc_fence_after();
-          issue_s(t, g % kCkStages);
+          issue_s(t, g % kCkStages, t);
           ++sc[t];
           if (n == 1) umma_commit(&bars->q_empty[t]);
         }
@@ -1092,7 +1134,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
             if (!has_next) {
               umma_commit(&bars->o_full[t]);
             } else {
-              issue_s(t, (g + 1) % kCkStages);
+              issue_s(t, (g + 1) % kCkStages, t);
               ++sc[t];
               if (j + 2 == n) umma_commit(&bars->q_empty[t]);
             }
@@ -1144,7 +1186,11 @@ __global__ void __launch_bounds__(kCkThreads, 1)
     for (const CkUnit* up; (up = ck_next<true>(bars, next_unit, p.err)) != nullptr;
          ck_done<true>(bars, next_unit)) {
       const CkUnit& u = *up;
-      const int rows = t ? u.rows[1] : u.rows[0];
+      // Rows for one tile only: the warpgroups take them both, and alternate key tiles, as two running
+      // softmaxes that the first one merges at the end (16 trees of 9 to 33 tokens over 500 to 4000, scores
+      // capped: 84 us, with the second one idle 99).
+      const bool twin = kTree && !kNarrow && u.rows[1] == 0;
+      const int rows = t && !twin ? u.rows[1] : u.rows[0];
       const bool begins = u.j0 == 0, ends = u.j1 == u.n;
       if constexpr (kCode) {
         if (!begun) spreader.begin(u, wait);
@@ -1155,29 +1201,21 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       } else {
       if (rows == 0) {
         g += u.j1 - u.j0;
-        if constexpr (kCode) {  // (the second warpgroup) V is spread all the same
-#pragma unroll 1
-          for (int j = u.j0 + 1; j < u.j1; ++j) {
-            spreader.look_up(u, j, spreader.page(u, j));
-            spreader.spread(u, j, wait);
-          }
-          const CkUnit* un = ck_next<true>(bars, next_unit + 1, p.err);
-          begun = un != nullptr;
-          if (begun) spreader.begin(*un, wait);
-        }
         continue;
       }
       const bool live = row < rows;             // this row is stored
       const bool warp_live = quarter * 32 < rows;
       const int tok = bars->row_token[row], head = u.hk * pb.group + bars->row_head[row];
       // the tile's first token of the unit
-      const int tile0 = t * (kTree ? u.rows[0] / pb.group : pb.tile_tokens);
+      const int tile0 = twin ? 0 : t * (kTree ? u.rows[0] / pb.group : pb.tile_tokens);
+      const int first = twin ? u.j0 + t : u.j0, g0 = g - u.j0;
       const int pos = u.pos + tile0 + tok;
       float slope2 = 0.f;
       if (kAlibi && live) slope2 = p.f.slopes[head] * kLog2e;
       float m = -INFINITY, l = 0.f;
 #pragma unroll 1
-      for (int j = u.j0; j < u.j1; ++j, ++sc, ++g) {
+      for (int j = first; j < u.j1; j += twin ? 2 : 1, ++sc) {
+        g = g0 + j;
         const int tile = ck_tile(u, j);
         const int k0 = tile * kChunkTile;
         // (keys past the context are masked by their number)
@@ -1190,9 +1228,9 @@ __global__ void __launch_bounds__(kCkThreads, 1)
         wait(&bars->s_full[t], sc & 1);
         if constexpr (kCode)
           if (ahead < u.j1) spreader.look_up(u, ahead, ahead_page);
-        if (!kCode && t == 0 && k0 + kChunkTile > u.keys) {
+        if (!kCode && (twin || t == 0) && k0 + kChunkTile > u.keys) {
           wait(&bars->v_full[g % kCkStages], (g / kCkStages) & 1);
-          zero_v_rows(sV + (g % kCkStages) * kChunkTileBytes, max(u.keys - k0, 0), threadIdx.x);
+          zero_v_rows(sV + (g % kCkStages) * kChunkTileBytes, max(u.keys - k0, 0), threadIdx.x & 127);
           fence_proxy_async_smem();
         }
         if (warp_live) {
@@ -1261,7 +1299,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
           const float m_new = fmax_nan(m, mx * sl2);
           bool rescale = false;
           float alpha = 1.f;
-          if (j == u.j0) {
+          if (j == first) {
             m = m_new;
           } else {
             const bool need = !(m_new <= m + kCkRescale) && m == m;  // (once to NaN; it stays)
@@ -1294,34 +1332,75 @@ __global__ void __launch_bounds__(kCkThreads, 1)
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->p_full[t]);
-        if constexpr (kCode)
+        if constexpr (kCode) {
           if (ahead < u.j1) spreader.spread(u, ahead, wait);
+          if (twin) spreader.run(u, ahead + 1, ahead + 2, wait);
+        }
       }
+      g = g0 + u.j1;
       if constexpr (kCode) {
         const CkUnit* un = ck_next<true>(bars, next_unit + 1, p.err);
         begun = un != nullptr;
         if (begun) spreader.begin(*un, wait);
       }
       // ----------------------------------------------------------- epilogue
-      wait(&bars->o_full[t], uc & 1);
+      const bool mine = first < u.j1;
+      if (mine) wait(&bars->o_full[t], uc & 1);
       tc_fence_after();
-      const bool none = m == -INFINITY;
-      const float inv = none ? 0.f : 1.f / l;
-      const float lse2 = none ? -INFINITY : m + log2f(l);
+      bool none = m == -INFINITY;
+      float inv = none ? 0.f : 1.f / l, inv1 = 0.f;
+      float lse2 = none ? -INFINITY : m + log2f(l);
+      const bool two = twin && u.j1 - u.j0 > 1;  // the second warpgroup has a sum as well
+      auto meet = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->merge);
+        wait(&bars->merge, merges++ & 1);
+      };
+      if (two) {
+        if (t == 1) {
+          bars->n_red[0][quarter][lane] = m;
+          bars->n_red[1][quarter][lane] = l;
+        }
+        tc_fence_before();
+        meet();
+        tc_fence_after();
+        if (t == 0) {
+          const float m1 = bars->n_red[0][quarter][lane], l1 = bars->n_red[1][quarter][lane];
+          const float mx = fmax_nan(m, m1);
+          const float w0 = m == -INFINITY ? 0.f : exp2f(m - mx);
+          const float w1 = m1 == -INFINITY ? 0.f : exp2f(m1 - mx);
+          const float sum = w0 * l + w1 * l1;
+          none = mx == -INFINITY;
+          inv = none ? 0.f : w0 / sum;
+          inv1 = none ? 0.f : w1 / sum;
+          lse2 = none ? -INFINITY : mx + log2f(sum);
+        }
+      }
       const int64_t out_row = u.token + tile0 + tok;
-      const int64_t part = (int64_t)(cta * 2 + (begins ? 1 : 0)) * p.rows_cap + t * 128 + row;
+      const int64_t part = (int64_t)(cta * 2 + (begins ? 1 : 0)) * p.rows_cap + (twin ? 0 : t * 128) + row;
       T* orow = static_cast<T*>(p.o) + out_row * p.os[0] + head * p.os[1];
       float* prow = p.ws_o + (part & ~31) * 128 + (part & 31) * 4;
-      if (warp_live) {
+      if (warp_live && !(twin && t == 1)) {
 #pragma unroll 1
         for (int cc = 0; cc < 128; cc += 32) {
           uint32_t ov[32];
           tmem_ld32(tO + cc, ov);
           tmem_wait_ld();
           reg_fence<32>(ov);
+          // (a factor of 0 is nothing seen: the accumulator does not count)
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            ov[e] = none ? 0u : __float_as_uint(__uint_as_float(ov[e]) * inv);
+            ov[e] = none || (kTree && inv == 0.f) ? 0u : __float_as_uint(__uint_as_float(ov[e]) * inv);
+          if (two) {
+            uint32_t o1[32];
+            tmem_ld32(tO + 128 + cc, o1);
+            tmem_wait_ld();
+            reg_fence<32>(o1);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (inv1 != 0.f)
+                ov[e] = __float_as_uint(fmaf(__uint_as_float(o1[e]), inv1, __uint_as_float(ov[e])));
+          }
           if (live && begins && ends) {
 #pragma unroll
             for (int e = 0; e < 32; e += 16) {
@@ -1352,9 +1431,12 @@ __global__ void __launch_bounds__(kCkThreads, 1)
         }
       }
       tc_fence_before();
+      if (two) meet();  // (the first has read the second's sums and O)
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->o_empty[t]);
-      ++uc;
+      if (mine) {
+        if (lane == 0) mbar_arrive(&bars->o_empty[t]);
+        ++uc;
+      }
       }
     }
   }
@@ -1597,33 +1679,39 @@ static int paged_chunk(const char* what, const void* q, const void* k_cache, con
                 workspace ? workspace_bytes : (size_t)0, need);
   if (!aligned16(workspace))
     return fail(FI_ERR_ALIGNMENT, "%s: workspace not 16-byte aligned", what);
-  const CUtensorMapDataType type = dtype == FI_DTYPE_F16 ? Half16<__half>::kTmap
-                                                         : Half16<__nv_bfloat16>::kTmap;
-  ChunkParams n = p;  // the narrow kernel's
-  n.b.tile_tokens = per_unit > 0 ? (int)per_unit : 1;
-  CUtensorMap tq_n = {}, tq_w = {}, tk, tv;
-  if (use_narrow && !codes && (r = chunk_q_map(&tq_n, type, q, n.b, q_strides, what)) != FI_OK)
-    return r;
-  if (use_wide && (r = chunk_q_map(&tq_w, type, q, p.b, q_strides, what)) != FI_OK)
-    return r;
   CodePages pages = {};
   if (codes) {
     pages.q = q;
     pages.pool[0] = static_cast<const uint8_t*>(k_cache);
     pages.pool[1] = static_cast<const uint8_t*>(v_cache);
     for (int i = 0; i < 2; ++i) pages.qs[i] = q_strides[i];
+    const int64_t sizes[3] = {num_blocks, block_size, num_kv_heads};
+    bool ok = q_strides[2] == 1 && aligned16(q) && stride_ok(total_tokens, q_strides[0]) &&
+              stride_ok(num_q_heads, q_strides[1]) && aligned16(k_cache) && aligned16(v_cache) &&
+              kc_strides[3] == 1 && vc_strides[3] == 1;
     for (int i = 0; i < 3; ++i) {
       pages.st[0][i] = kc_strides[i];
       pages.st[1][i] = vc_strides[i];
+      ok = ok && (sizes[i] == 1 || (kc_strides[i] % 16 == 0 && vc_strides[i] % 16 == 0));
     }
-    if (q_strides[2] != 1 || !aligned16(q) || !stride_ok(total_tokens, q_strides[0]) ||
-        !stride_ok(num_q_heads, q_strides[1]))
+    if (!ok)
       return fail(FI_ERR_ALIGNMENT,
-                  "%s q: needs a 16-byte aligned base, unit innermost stride and other strides "
-                  "multiple of 8",
+                  "%s: q and pages of codes need 16-byte aligned bases, unit innermost strides and other "
+                  "strides that are multiples of 16 bytes",
                   what);
-    if ((r = chunk_code_map(&tk, k_cache, p.b, kc_strides, what)) != FI_OK) return r;
-    if ((r = chunk_code_map(&tv, v_cache, p.b, vc_strides, what)) != FI_OK) return r;
+  }
+  const CUtensorMapDataType type = dtype == FI_DTYPE_F16 ? Half16<__half>::kTmap
+                                                         : Half16<__nv_bfloat16>::kTmap;
+  ChunkParams n = p;  // the narrow kernel's
+  n.b.tile_tokens = per_unit > 0 ? (int)per_unit : 1;
+  CUtensorMap tq_n = {}, tq_w = {}, tk = {}, tv = {};
+  if (use_narrow && !codes && (r = chunk_q_map(&tq_n, type, q, n.b, q_strides, what)) != FI_OK)
+    return r;
+  if (use_wide && (r = chunk_q_map(&tq_w, type, q, p.b, q_strides, what)) != FI_OK)
+    return r;
+  if (codes) {
+    if (use_wide && (r = chunk_code_map(&tk, k_cache, p.b, kc_strides, what)) != FI_OK) return r;
+    if (use_wide && (r = chunk_code_map(&tv, v_cache, p.b, vc_strides, what)) != FI_OK) return r;
     for (int kv = 0; kv < 2; ++kv) {
       p.scale[kv] = extra.scale[kv];
       for (int i = 0; i < 3; ++i) p.ss[kv][i] = extra.ss[kv][i];
