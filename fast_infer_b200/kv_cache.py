@@ -224,19 +224,23 @@ class KVCache:
         move to consecutive slots in all layers (``kernels.drafting.keep_accepted``), ``seq_lens``
         shrinks to them, and pages past it go back to the free list. cu_seqlens, context_lens: as
         ``extend`` returned them; path, counts: from ``kernels.drafting.accept_drafts``. Returns the
-        counts on the host (the call waits for them)."""
+        counts on the host (the call waits for them, so it is not captured into a graph). Raises
+        before it changes anything if lengths or counts are not those of the last ``extend``."""
         from fast_infer_b200.kernels.drafting import keep_accepted
-        self.sync_block_table()
         B = context_lens.numel()
         if B > self._bt.shape[0]:
             raise ValueError("batch larger than the block table")
-        keep_accepted(self.k, self.v, self.block_table, self.block_size, cu_seqlens, context_lens,
-                      path, counts, k_scale=self.k_scale, v_scale=self.v_scale)
+        if cu_seqlens.numel() != B + 1 or counts.numel() != B:
+            raise ValueError("cu_seqlens must be [batch + 1], context_lens and counts [batch]")
         host = torch.cat([cu_seqlens.to(torch.int32), context_lens.to(torch.int32),
                           counts.to(torch.int32)]).cpu().numpy().astype(np.int64)
         new, ctx, kept = np.diff(host[:B + 1]), host[B + 1:2 * B + 1], host[2 * B + 1:]
-        if (ctx != self.seq_lens[:B]).any() or (kept < 0).any() or (kept > new).any():
+        if (host[0] != 0 or host[B] > path.numel() or (ctx != self.seq_lens[:B]).any()
+                or (kept < 0).any() or (kept > new).any() or (new > ctx).any()):
             raise ValueError("accept needs the lengths of the last extend and counts of its tokens")
+        self.sync_block_table()
+        keep_accepted(self.k, self.v, self.block_table, self.block_size, cu_seqlens, context_lens,
+                      path, counts, k_scale=self.k_scale, v_scale=self.v_scale)
         self.seq_lens[:B] = ctx - new + kept
         for b in range(B):
             self._free_past(b)

@@ -100,3 +100,58 @@ def test_loop(cuda_device, device_checks, pool):
                                      int(lengths.sum()), dtype=dtype))
         for a, b in zip(seen[:len(seen) // 2], seen[len(seen) // 2:]):
             assert torch.equal(a, b)
+
+
+def test_accept_changes_nothing_when_it_refuses(cuda_device):
+    dev = cuda_device
+    cache = KVCache(1, HK, 128, 256, 64, dev, num_blocks=8)
+    cache.k.copy_(torch.randn(cache.k.shape, device=dev))
+    cache.v.copy_(torch.randn(cache.v.shape, device=dev))
+    cache.extend([30, 60])
+    cu, ctx = cache.extend([5, 9])
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    path = ints(0, 2, 4, -1, -1, 0, 3, 8, -1, -1, -1, -1, -1, -1)
+    counts = ints(3, 3)
+    was = cache.k.clone(), cache.v.clone(), cache.seq_lens.copy(), list(cache.free_blocks)
+    for bad in ((cu, ctx, path, ints(6, 3)), (cu, ctx, path, ints(3, -1)), (cu, ctx - 1, path, counts), (cu + 1, ctx, path, counts),
+                (cu, ctx, path[:10], counts), (cu, ctx, path, ints(3)), (cu[:2], ctx, path, counts)):
+        with pytest.raises(ValueError):
+            cache.accept(*bad)
+        assert torch.equal(cache.k, was[0]) and torch.equal(cache.v, was[1])
+        assert (cache.seq_lens == was[2]).all() and cache.free_blocks == was[3]
+    assert cache.accept(cu, ctx, path, counts).tolist() == [3, 3] and cache.seq_lens.tolist() == [33, 63]
+    assert len(cache.free_blocks) == len(was[3]) + 1
+    with pytest.raises(ValueError):  # the same step twice
+        cache.accept(cu, ctx, path, counts)
+
+
+@pytest.mark.parametrize("pool", [torch.int8, torch.float8_e4m3fn])
+def test_operators_of_16_bit_pages_refuse_codes(cuda_device, pool):
+    """What does not take scales takes no codes."""
+    from fast_infer_b200.kernels.attention import attention_mass, paged_attention, paged_chunk_attention
+    from fast_infer_b200.kv_cache import rope_and_store, store_kv_decode, store_kv_prefill
+    dev = cuda_device
+    cache = KVCache(1, HK, 128, 256, 64, dev, num_blocks=8, dtype=pool)
+    cu, ctx = cache.extend([5])
+    q = torch.randn(5, HQ, 128, device=dev).half()
+    lse = torch.zeros(5, HQ, device=dev)
+    rows = torch.randn(1, 5, HK, 128, device=dev).half()
+    tables = torch.ones(256, 128, device=dev)
+    args = (cache.k[0], cache.v[0], cache.block_table, 64)
+    with pytest.raises((TypeError, ValueError)):
+        paged_chunk_attention(q, *args, cu, ctx)
+    with pytest.raises((TypeError, ValueError)):
+        paged_tree_attention(q, *args, cu, ctx)
+    with pytest.raises((TypeError, ValueError)):
+        paged_attention(q[:1], *args, 5)
+    with pytest.raises((TypeError, ValueError)):
+        attention_mass(q, cache.k[0], cache.block_table, 64, cu, ctx, lse)
+    with pytest.raises((TypeError, ValueError)):
+        cache.evict(torch.zeros(1, 1, HK, 256, device=dev), 2)
+    with pytest.raises((TypeError, ValueError)):
+        store_kv_prefill(cache, 0, rows, rows)
+    with pytest.raises((TypeError, ValueError)):
+        store_kv_decode(cache, 0, rows[:, 0], rows[:, 0], 6)
+    with pytest.raises((TypeError, ValueError)):
+        rope_and_store(cache, 0, torch.randn(1, 1, (HQ + 2 * HK) * 128, device=dev).half(), HQ, tables, tables, 0)
+    assert (cache.k.view(torch.int8) == 0).all() and (cache.v.view(torch.int8) == 0).all()

@@ -325,3 +325,40 @@ def test_workspace_is_as_large_as_what_is_written(cuda_device, device_checks, ki
     ws = torch.full((need + (64 << 20),), 171, dtype=torch.uint8, device=cuda_device)
     check(st, kind, torch.float16, workspace=ws[:need])
     assert (ws[need:] == 171).all()
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("seqs", [[(1, 300), (8, 200)], [(60, 500)], [(130, 700)]])
+def test_every_code(cuda_device, device_checks, seqs, dtype, kind):
+    """All bytes that are numbers, -128 of int8 among them, with scales that make scores of a few units."""
+    st = make(cuda_device, seqs, 6, 2, dtype, kind, seed=12, spread=4)
+    g = torch.Generator(device=cuda_device).manual_seed(5)
+    for x in "kv":
+        code = torch.randint(-128, 128, st[x].shape, generator=g, device=cuda_device, dtype=torch.int8)
+        if kind == "e4m3":
+            code = torch.where((code & 0x7f) == 0x7f, 0, code)
+        st[x].view(torch.int8).copy_(code)
+        st[x + "s"].clamp_(max=2.0 / CODES[kind][1])
+    check(st, kind, dtype)
+
+
+def test_two_streams_at_once(cuda_device):
+    """Calls on two streams, each with its own workspace, give what they give alone."""
+    dev = cuda_device
+    cases = [make(dev, [(60, 6000), (1, 3000)], 6, 2, torch.float16, k, seed=s, spread=4) for k, s in (("int8", 1), ("16bit", 2))]
+
+    def call(st):
+        return paged_tree_attention(st["q"], st["k"], st["v"], st["table"], 64, st["cu"], st["ctx"], tree_mask=st["mask"],
+                                    k_scale=st["ks"], v_scale=st["vs"])
+    want = [call(st) for st in cases]
+    streams = [torch.cuda.Stream(dev) for _ in cases]
+    torch.cuda.synchronize(dev)
+    got = [[], []]
+    for _ in range(20):
+        for st, stream, out in zip(cases, streams, got):
+            with torch.cuda.stream(stream):
+                out.append(call(st))
+    torch.cuda.synchronize(dev)
+    for w, out in zip(want, got):
+        assert all(torch.equal(w, o) for o in out)
