@@ -607,6 +607,24 @@ __device__ __forceinline__ int candidates(cg::cluster_group& cluster, SaShared* 
   return n;
 }
 
+// The counts of four bins in every CTA, four reads of distributed shared memory in flight.
+template <typename F>
+__device__ __forceinline__ void each_rank(cg::cluster_group& cluster, const uint32_t* counts, int bin,
+                                          F&& take) {
+  const int ctas = (int)cluster.num_blocks();
+#pragma unroll 1
+  for (int r0 = 0; r0 < ctas; r0 += 4) {
+    uint4 h[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (r0 + j < ctas)
+        h[j] = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(counts, r0 + j) + bin);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (r0 + j < ctas) take(r0 + j, h[j]);
+  }
+}
+
 // Four value bins a lane of block `block`: counts of all CTAs and of this one, keys (0: none) and weights.
 template <typename T>
 struct BinQuad {
@@ -617,13 +635,12 @@ struct BinQuad {
     const int bin = block * kSaBlock + (threadIdx.x & 31) * 4;
 #pragma unroll
     for (int j = 0; j < 4; ++j) n[j] = 0;
-    for (int r = 0; r < (int)cluster.num_blocks(); ++r) {
-      const uint4 h = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(counts, r) + bin);
+    each_rank(cluster, counts, bin, [&](int, const uint4& h) {
       n[0] += h.x;
       n[1] += h.y;
       n[2] += h.z;
       n[3] += h.w;
-    }
+    });
     const uint4 mine = *reinterpret_cast<const uint4*>(counts + bin);
     own[0] = mine.x;
     own[1] = mine.y;
@@ -898,6 +915,7 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
     constexpr int kBlocks = kSaBlocks<T>;
     static_assert(kBlocks <= 128 && kBlocks % kSaMaxCluster == 0, "a thread per block of bins");
     bins = value_bins<T>(row);
+    const uint32_t span = bins.top - bins.lowest;
     int lump_n = 0;
     uint64_t lump_m = 0;
 #pragma unroll 1
@@ -912,7 +930,7 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
         const uint32_t d = i & 1 ? below >> 16 : below & 0xffff;
         const int bin = value_bin<T>(bins, d);
         if (bin >= 0) atomicAdd(&counts[bin], 1u);
-        else lumps |= 1u << i;
+        else if (d <= span) lumps |= 1u << i;
       }
       if (lumps) {
 #pragma unroll 1
@@ -921,11 +939,9 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
           const uint32_t word = i < 4 ? (i < 2 ? raw.x : raw.y) : (i < 6 ? raw.z : raw.w);
           const uint32_t below = bins.top * 0x10001u - keys16(word);
           const uint32_t d = i & 1 ? below >> 16 : below & 0xffff;
-          if (d <= bins.top - bins.lowest) {
-            const float v = Bits16<T>::value(bins.top - d);
-            ++lump_n;
-            if (v >= row.floor_x) lump_m += weight(row, s->tab, v);
-          }
+          const float v = Bits16<T>::value(bins.top - d);
+          ++lump_n;
+          if (v >= row.floor_x) lump_m += weight(row, s->tab, v);
         }
       }
     }
@@ -954,22 +970,25 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
 #pragma unroll 1
     for (int i = warp; i < share; i += kSaWarps) {
       const int block = rank * share + i;
-      const BinQuad<T> q(cluster, counts, row, s->tab, bins, block);
+      uint64_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t key = bin_key<T>(bins, block * kSaBlock + lane * 4 + j);
+        const float v = Bits16<T>::value(key);
+        w[j] = key && v >= row.floor_x ? weight(row, s->tab, v) : 0;
+      }
       uint32_t n = 0;
       uint64_t m = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) n += q.n[j], m += q.n[j] * q.w[j];
+      each_rank(cluster, counts, block * kSaBlock + lane * 4, [&](int r, const uint4& h) {
+        const uint64_t o = warp_sum(h.x * w[0] + h.y * w[1] + h.z * w[2] + h.w * w[3]);
+        n += h.x + h.y + h.z + h.w;
+        m += o;
+        if (lane == 0) s->block_own[r * share + i] = o;
+      });
       n = __reduce_add_sync(0xffffffffu, n);
-      m = warp_sum(m);
       if (lane == 0) {
         s->block_count[i] = n;
         s->block_mass[i] = m;
-      }
-      for (int r = 0; r < ctas; ++r) {
-        const uint4 h = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(counts, r) +
-                                                        block * kSaBlock + lane * 4);
-        const uint64_t o = warp_sum(h.x * q.w[0] + h.y * q.w[1] + h.z * q.w[2] + h.w * q.w[3]);
-        if (lane == 0) s->block_own[r * share + i] = o;
       }
     }
     cluster.sync();
@@ -1177,21 +1196,7 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
     for (int i = 0; i < 8; ++i) {
       const uint32_t key = key_of(v[i]);
       const bool in = v[i] >= row.floor_x && (key > cut.key || (key == cut.key && at + i < tie_end));
-      w[i] = 0;
-      if (in) {
-        bool looked_up = false;
-        if constexpr (kSaTable<T>) {
-          if (counted) {
-            const uint32_t raw = reinterpret_cast<const uint16_t*>(x)[at + i];
-            const int bin = value_bin<T>(bins, bins.top - (keys16(raw) & 0xffff));
-            if (bin >= 0) {
-              w[i] = reinterpret_cast<const uint64_t*>(counts)[bin];
-              looked_up = true;
-            }
-          }
-        }
-        if (!looked_up) w[i] = weight(row, s->tab, v[i]);
-      }
+      w[i] = in ? weight(row, s->tab, v[i]) : 0;
       sum += w[i];
     }
     return sum;
@@ -1225,7 +1230,7 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
     if (m > 0) last = r;
     mass += m;
   }
-  cluster.sync();  // (all have read; from here on each CTA is on its own)
+  cluster.barrier_arrive();  // (this CTA has read; from here on it is on its own)
   // the first CTA, cell and token whose running sum passes the target; the last kept one where none
   // does (u = 1, NaN)
   const double target = (double)u * (double)mass;
@@ -1233,41 +1238,100 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
   auto passes = [&](uint64_t sum_before, uint64_t part) {
     return (double)(sum_before + part) > target && (sum_before == 0 || !((double)sum_before > target));
   };
-  if (own == 0 || !(none ? rank == last : passes(ahead, own))) return;
+  if (own == 0 || !(none ? rank == last : passes(ahead, own))) {
+    cluster.barrier_wait();
+    return;
+  }
+  int found = -1;         // the cell
+  uint64_t above = 0;     // kept mass before it
+  uint64_t w[8], sum;     // of this lane's tokens in it
   if (counted) {
     if (!cut.all_ties) {
       const int64_t keep = cut.ties - ties_before;
       if (keep < own_ties) tie_end = keep > 0 ? find_tie_end(keep, tie_counts()) : 0;
-      if (tid == 0) s->bin = -1;
     }
-    if constexpr (kSaTable<T>) {  // the values' weights, over their counts
+    [[maybe_unused]] uint32_t tie_d = 0xffffffffu;  // of the cut, where only some of its tokens stay
+    if constexpr (kSaTable<T>) {  // the values' kept weights, over their counts
+      if (tie_end != INT_MAX)
+        tie_d = bins.top - (keys16(Bits16<T>::bits_below(of_key(cut.key))) & 0xffff);
       __syncthreads();
       for (int bin = tid; bin < kSaValueBins<T>; bin += kSaThreads) {
         const uint32_t key16 = bin_key<T>(bins, bin);
         const float v = Bits16<T>::value(key16);
-        if (key16 != 0 && v >= row.floor_x && key_of(v) >= cut.key)
-          reinterpret_cast<uint64_t*>(counts)[bin] = weight(row, s->tab, v);
+        reinterpret_cast<uint64_t*>(counts)[bin] =
+            key16 != 0 && v >= row.floor_x && key_of(v) >= cut.key ? weight(row, s->tab, v) : 0;
       }
       __syncthreads();
     }
-    add_cells();
+    auto kept_by_value = [&](int at, uint64_t* w) {
+      if constexpr (!kSaTable<T>) {
+        return kept(at, w);
+      } else {
+        const uint64_t* table = reinterpret_cast<const uint64_t*>(counts);
+        const uint4 raw = *reinterpret_cast<const uint4*>(x + at);
+        const uint32_t pair[4] = {raw.x, raw.y, raw.z, raw.w};
+        bool lumps = false;
+        uint64_t sum = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t below = bins.top * 0x10001u - keys16(pair[i >> 1]);
+          const uint32_t d = i & 1 ? below >> 16 : below & 0xffff;
+          const int bin = value_bin<T>(bins, d);
+          w[i] = bin >= 0 ? table[bin] : 0;
+          lumps |= bin < 0 && d <= bins.top - bins.lowest;
+          if (d == tie_d && at + i >= tie_end) w[i] = 0;
+          sum += w[i];
+        }
+        return lumps ? kept(at, w) : sum;
+      }
+    };
+    // 256 tokens a warp in index order, as far as the target
+    uint64_t run = ahead;
+#pragma unroll 1
+    for (int cell0 = 0; found < 0 && cell0 < cells; cell0 += kSaWarps) {
+      sum = kept_by_value((cell0 + warp) * kSaStep + lane * 8, w);
+      const uint64_t mass_here = warp_sum(sum);
+      if (lane == 0) s->step_mass[cell0 + warp] = mass_here;
+      __syncthreads();
+      const uint64_t cell = lane < kSaWarps ? s->step_mass[cell0 + lane] : 0;
+      uint64_t to = cell;
+#pragma unroll
+      for (int off = 1; off < kSaWarps; off <<= 1) {
+        const uint64_t o = __shfl_up_sync(0xffffffffu, to, off);
+        if (lane >= off) to += o;
+      }
+      const bool here = cell > 0 && (none ? run + to == ahead + own : passes(run + to - cell, cell));
+      const uint32_t hit = __ballot_sync(0xffffffffu, here);
+      if (hit) {
+        const int which = __ffs((int)hit) - 1;
+        found = cell0 + which;
+        above = __shfl_sync(0xffffffffu, run + to - cell, which);
+      }
+      run += __shfl_sync(0xffffffffu, to, kSaWarps - 1);
+    }
+    if (warp != found % kSaWarps) found = -1;
+  } else {
+    if (cell > 0 && (none ? before + cell == all : passes(ahead + before, cell))) {
+      s->bin = tid;
+      s->above = ahead + before;
+    }
+    __syncthreads();
+    above = s->above;
+    if (s->bin >= 0 && warp == s->bin / steps) {
+      found = s->bin;
+      sum = kept(found * kSaStep + lane * 8, w);
+    }
   }
-  if (cell > 0 && (none ? before + cell == all : passes(ahead + before, cell))) {
-    s->bin = tid;
-    s->above = ahead + before;
-  }
-  __syncthreads();
-  if (s->bin < 0 || warp != s->bin / steps) return;
-  const int at0 = s->bin * kSaStep + lane * 8;
-  uint64_t w[8];
-  const uint64_t sum = kept(at0, w);
+  cluster.barrier_wait();
+  if (found < 0) return;
+  const int at0 = found * kSaStep + lane * 8;
   uint64_t inc = sum;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
     const uint64_t o = __shfl_up_sync(0xffffffffu, inc, off);
     if (lane >= off) inc += o;
   }
-  uint64_t run = s->above + inc - sum;
+  uint64_t run = above + inc - sum;
   int at = none ? -1 : INT_MAX;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
