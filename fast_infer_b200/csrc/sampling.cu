@@ -23,6 +23,9 @@
 #include <cuda_fp16.h>
 #include <float.h>
 
+#include <algorithm>
+#include <type_traits>
+
 #include "common.cuh"
 #include "host_common.h"
 
@@ -33,10 +36,15 @@ namespace fi {
 constexpr int kSaThreads = 512;
 constexpr int kSaWarps = kSaThreads / 32;
 constexpr int kSaBins = kSaThreads;     // a bin per thread where bins are joined
-constexpr int kSaStep = 256;            // tokens of a warp's step
-constexpr int kSaSteps = 8;             // steps of a warp at most: 32768 tokens a CTA, as the limbs allow
+constexpr int kSaStep = 256;            // tokens of a cell: of a warp's step
+constexpr int kSaRound = kSaWarps * kSaStep;
+constexpr int kSaMaxCells = kSaThreads;  // of a CTA: a thread each
 constexpr int kSaMaxCluster = 8;
-constexpr int64_t kSaMaxVocab = (int64_t)kSaMaxCluster * kSaWarps * kSaSteps * kSaStep;
+constexpr int kSaRows32 = 8 * kSaRound;  // 32-bit logits that a CTA holds in shared memory at most
+constexpr int64_t kSaMaxVocab = (int64_t)kSaMaxCluster * kSaRows32;
+constexpr int kSaMaxTokens = (1 << 17) - 8;  // of a CTA, as limbs and cells allow
+constexpr int64_t kSaPart = 4 * kSaRound;  // tokens from which on a slice is counted in parts
+constexpr int kSaMaxParts = 4, kSaMaxBlocks = 128, kSaMaxOwn = 384;
 
 struct SampleArgs {
   const void* x;
@@ -49,7 +57,7 @@ struct SampleArgs {
   float temperature1, top_p1, min_p1;
   int top_k1;
   int32_t* out;
-  int vocab, chunk;  // chunk: tokens of a warp
+  int vocab, parts, part;  // parts of a CTA's slice, positions of a part
 };
 
 template <typename T>
@@ -69,21 +77,49 @@ struct KeyGrain<__half> { static constexpr int kBits = 13; };
 template <>
 struct KeyGrain<__nv_bfloat16> { static constexpr int kBits = 16; };
 
-// Eight consecutive logits from shared memory, -0 as 0.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* x) {
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p);
-    *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(p + 4);
-  } else {
-    const uint4 raw = *reinterpret_cast<const uint4*>(p);
-    const T* t = reinterpret_cast<const T*>(&raw);
+struct Bits16;
+
+// A CTA's slice of the row by position, -inf where a position holds no token. 32-bit logits lie in shared memory;
+// 16-bit ones, of which most passes need no more than their counts, are read again from L2: positions begin at the
+// 16-byte boundary below the row (rows of an odd vocabulary begin anywhere).
+template <typename T>
+struct Slice {
+  const T* p;
+  int lo, hi;  // positions with tokens
+  int cells;   // cells with tokens
+  __device__ __noinline__ static uint4 edge(const T* p, int lo, int hi, int at) {
+    uint32_t w[4] = {};
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t none = Bits16<T>::bits_below(-INFINITY);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = logit(t[i]);
+      for (int i = 0; i < 8; ++i) {
+        const bool in = at + i >= lo && at + i < hi;
+        w[i >> 1] |= (in ? (uint32_t) reinterpret_cast<const uint16_t*>(p)[at + i] : none) << (i & 1) * 16;
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
+  // eight 16-bit values
+  __device__ __forceinline__ uint4 raw8(int at) const {
+    if (at >= lo && at + 8 <= hi) return __ldg(reinterpret_cast<const uint4*>(p + at));
+    return edge(p, lo, hi, at);
+  }
+  // eight values, -0 as 0
+  __device__ __forceinline__ void load8(int at, float* x) const {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p + at);
+      *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(p + at + 4);
+    } else {
+      const uint4 raw = raw8(at);
+      const T* t = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] += 0.f;
-}
+      for (int i = 0; i < 8; ++i) x[i] = logit(t[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] += 0.f;
+  }
+};
 
 // Unsigned keys in the order of the floats.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -127,11 +163,12 @@ __device__ __forceinline__ uint64_t weight(const Row& row, const double* tab, fl
 // 16-bit logits: keys of the raw bits, in the order of the values, both zeros alike.
 template <typename T>
 struct Bits16 {
-  static constexpr int kRegion = 0;
+  static constexpr int kRegion = 0, kMaxParts = 1;
 };
 template <>
 struct Bits16<__nv_bfloat16> {
   static constexpr int kRegion = 2048;  // 16 octaves
+  static constexpr int kMaxParts = 4;
   static constexpr uint32_t kLowest = 0x8000 - 0x7f7f;
   __device__ static __forceinline__ float value(uint32_t k) {
     return __uint_as_float((k >= 0x8000 ? k - 0x8000 : (0x8000 - k) | 0x8000) << 16);
@@ -148,6 +185,7 @@ struct Bits16<__nv_bfloat16> {
 template <>
 struct Bits16<__half> {
   static constexpr int kRegion = 8192;  // 8 octaves
+  static constexpr int kMaxParts = 3;
   static constexpr uint32_t kLowest = 0x8000 - 0x7bff;
   __device__ static __forceinline__ float value(uint32_t k) {
     return __half2float(
@@ -167,8 +205,9 @@ __device__ __forceinline__ uint32_t keys16(uint32_t pair) {
   return (pair ^ (neg | 0x80008000u)) + (neg & 0x00010001u);
 }
 
-// Bins of one 16-bit value each, descending: `n1` from the row's greatest down, `n2` further ones of negative values,
-// whose first lies `off2` below the greatest. What lies between the two (values near 0, of many octaves) is one lump.
+// Bins of one 16-bit value each, descending: n1 from the row's greatest down, a bin for all that lies between (the lump:
+// values near 0, of many octaves), n2 further ones of negative values, whose first lies `off2` below the greatest, and
+// a bin for what has no weight.
 struct Values {
   uint32_t top, lowest;  // keys: M, and of the least value with a weight
   uint32_t n1, off2, n2;
@@ -182,26 +221,40 @@ __device__ __forceinline__ Values value_bins(const Row& row) {
   const bool positive = v.top >= 0x8000;
   const uint32_t limit = positive ? max(0x8000u, v.lowest) : v.lowest;
   v.n1 = min(v.top - limit + 1, R);
-  v.n2 = v.off2 = 0;
+  v.n2 = 0;
+  v.off2 = v.top - v.lowest + 1;
   if (positive && v.lowest < 0x8000) {
-    const uint32_t top2 = min(v.lowest + R - 1, 0x7fffu);
+    const uint32_t top2 = min(v.lowest + R - 3, 0x7fffu);
     v.n2 = top2 - v.lowest + 1;
     v.off2 = v.top - top2;
   }
   return v;
 }
-// Bin of the value d keys below the greatest; -1: none.
-template <typename T>
-__device__ __forceinline__ int value_bin(const Values& v, uint32_t d) {
-  constexpr int R = Bits16<T>::kRegion;
-  return d < v.n1 ? (int)d : d - v.off2 < v.n2 ? (int)(d - v.off2) + R : -1;
+// Bins of two values at once, d keys below the greatest: min(d, n1) + max(d, off2 - 1) - (off2 - 1), with d no more than one
+// past the last that has a weight. 16-bit halves; none borrows or carries.
+__device__ __forceinline__ uint32_t value_bins2(const Values& v, uint32_t pair) {
+  const uint32_t edge = (v.off2 - 1) * 0x10001u;
+  const uint32_t below = v.top * 0x10001u - keys16(pair);
+  const uint32_t d = __vminu2(below, (v.top - v.lowest + 1) * 0x10001u);
+  return __vminu2(d, v.n1 * 0x10001u) + (__vmaxu2(d, edge) - edge);
 }
-// Key of a bin; 0 past its region's end.
-template <typename T>
+// Whether one of eight values (their bins) lies in the lump.
+__device__ __forceinline__ bool any_lump(const Values& v, const uint32_t* bins) {
+  const uint32_t lump = v.n1 * 0x10001u;
+  const uint32_t least = __vminu2(__vminu2(bins[0] ^ lump, bins[1] ^ lump),
+                                  __vminu2(bins[2] ^ lump, bins[3] ^ lump));
+  return (least & 0xffff) == 0 || least >> 16 == 0;
+}
+// Greatest and least key of a bin up to the last with a weight.
+__device__ __forceinline__ uint32_t bin_high(const Values& v, uint32_t bin) {
+  return bin <= v.n1 ? v.top - bin : v.top - v.off2 - (bin - v.n1 - 1);
+}
+__device__ __forceinline__ uint32_t bin_low(const Values& v, uint32_t bin) {
+  return bin == v.n1 ? v.top - v.off2 + 1 : bin_high(v, bin);
+}
+// Key of a bin of one value; 0 for others.
 __device__ __forceinline__ uint32_t bin_key(const Values& v, uint32_t bin) {
-  constexpr uint32_t R = Bits16<T>::kRegion;
-  if (bin < R) return bin < v.n1 ? v.top - bin : 0;
-  return bin - R < v.n2 ? v.top - v.off2 - (bin - R) : 0;
+  return bin == v.n1 || bin > v.n1 + v.n2 ? 0 : bin_high(v, bin);
 }
 
 struct SaPart {  // what a CTA tells the others about its slice
@@ -211,34 +264,34 @@ struct SaPart {  // what a CTA tells the others about its slice
   int bad;         // NaN or +inf
   int index;       // greedy: first index of the greatest
   int ties;
-  int lump_count;
-  uint64_t mass, lump_mass;
+  int lump_count[kSaMaxParts];                // per part of the slice
+  unsigned long long lump_mass[kSaMaxParts];
+  uint64_t mass[kSaMaxParts];                 // kept
 };
 constexpr int kSaList = 1024;  // candidates that one CTA finishes on its own
+constexpr int kSaLumps = 4 * kSaMaxCells;  // values of the lump that a part lists
 constexpr int kSaListK = 512;  // top_k up to which a list is tried
 
 struct SaShared {
   double tab[32];
-  uint64_t step_mass[kSaWarps * kSaSteps];
+  uint64_t step_mass[kSaMaxCells];
   uint64_t scan[2 * kSaWarps];
   SaPart part;
   float w_top[kSaWarps], w_low[kSaWarps], w_least[kSaWarps];
   int w_ties[kSaWarps];
   // the bin that a search chose
   uint64_t above, held;
-  int64_t tie_base[2];
-  int tie_end, list_n;
+  int64_t tie_base[kSaMaxParts][2];
+  int tie_end, list_n, lump_n[kSaMaxParts];
   uint32_t edge[2];
   int bin;
   uint32_t min_key;
-  uint64_t lump_mass[kSaWarps];
-  // of this CTA's share of the blocks of value bins: of all CTAs' tokens, and of each one's
-  uint64_t block_mass[128], block_own[128];
-  uint32_t block_count[128];
-  uint64_t extra;
+  // of this CTA's share of the blocks of value bins: of all CTAs' tokens, and of each part's
+  uint64_t block_mass[kSaMaxBlocks], block_own[kSaMaxOwn];
+  uint32_t block_count[kSaMaxBlocks];
 };
-// Histograms: two of generic bins by turns, or one of 16-bit values. Where their weights fit in twice the bytes (bf16)
-// they take the same place afterwards.
+// Histograms: two of generic bins by turns, or of 16-bit values, one for each part of the slice. Where weights of all
+// values fit (bf16) they take the same place afterwards; where not, counts are held two to a word.
 template <typename T>
 constexpr int kSaValueBins = 2 * Bits16<T>::kRegion;
 constexpr int kSaBlock = 128;  // bins that a warp looks at together, four a lane
@@ -247,9 +300,14 @@ constexpr int kSaBlocks = kSaValueBins<T> / kSaBlock;
 template <typename T>
 constexpr bool kSaTable = kSaValueBins<T> > 0 && kSaValueBins<T> * 8 <= 32768;
 template <typename T>
-constexpr int kSaHistBytes = kSaTable<T>                ? kSaValueBins<T> * 8
-                             : kSaValueBins<T> > 0 ? kSaValueBins<T> * 4
-                                                   : 2 * kSaBins * 12 + kSaList * 8;
+constexpr int kSaValueWords = kSaTable<T> ? kSaValueBins<T> : kSaValueBins<T> / 2;  // of a part's histogram
+template <typename T>
+__host__ __device__ constexpr int sa_hist_bytes(int parts) {
+  return kSaValueBins<T> == 0           ? 2 * kSaBins * 12 + kSaList * 8
+         : kSaTable<T> && parts < 2 ? kSaValueBins<T> * 8
+                                        : parts * kSaValueWords<T> * 4;
+}
+static_assert(sa_hist_bytes<__half>(1) >= 2 * kSaBins * 12, "a search's histograms take the values' place");
 static_assert(kSaList * 12 <= 2 * kSaBins * 12, "a list's weights and order take the histograms' place");
 
 // Sums over the block's threads before this one, and of all, of N 64-bit values. `warp_sums`: N x kSaWarps.
@@ -424,9 +482,9 @@ __device__ __forceinline__ int linear_bin(float top, float scale, float x) {
 // lo_key on, less `drop`, asks for. `above` of the result's group: what lies before it.
 template <typename T, bool kMass>
 __device__ __noinline__ Cut search(cg::cluster_group& cluster, SaShared* s,
-                                   uint32_t (*hists)[kSaBins][3], const T* x, int steps,
-                                      int chunk_base, const Row& row, uint32_t lo_key, int64_t want,
-                                      double share, uint64_t drop, int& level) {
+                                   uint32_t (*hists)[kSaBins][3], const Slice<T>& x, const Row& row,
+                                   uint32_t lo_key, int64_t want, double share, uint64_t drop,
+                                   int& level) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int ctas = (int)cluster.num_blocks();
   uint32_t hi_key = key_of(row.top);
@@ -440,9 +498,9 @@ __device__ __noinline__ Cut search(cg::cluster_group& cluster, SaShared* s,
   while (true) {
     uint32_t(*hist)[3] = hists[level & 1];
 #pragma unroll 1
-    for (int st = 0; st < steps; ++st) {
+    for (int c = warp; c < x.cells; c += kSaWarps) {
       float v[8];
-      load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
+      x.load8(c * kSaStep + lane * 8, v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t k = key_of(v[i]);
@@ -559,19 +617,19 @@ __device__ __forceinline__ Cut tighter(const Cut& a, const Cut& b) {
 // is too short for them.
 template <typename T>
 __device__ __forceinline__ int candidates(cg::cluster_group& cluster, SaShared* s,
-                                          uint32_t (*hists)[kSaBins][3], uint64_t* list, const T* x,
-                                          int steps, int chunk_base, int base, const Row& row,
-                                          uint32_t lo_key, int64_t want, int& level) {
-  const int tid = threadIdx.x, lane = tid & 31;
+                                          uint32_t (*hists)[kSaBins][3], uint64_t* list,
+                                          const Slice<T>& x, int base, const Row& row, uint32_t lo_key,
+                                          int64_t want, int& level) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int ctas = (int)cluster.num_blocks();
   const float range = row.top - of_key(lo_key);
   const float scale = range > 0.f && range < FLT_MAX ? (float)(kSaBins - 1) / range : 0.f;
   uint32_t(*hist)[3] = hists[level & 1];
   const float least = of_key(lo_key);
 #pragma unroll 1
-  for (int st = 0; st < steps; ++st) {
+  for (int c = warp; c < x.cells; c += kSaWarps) {
     float v[8];
-    load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
+    x.load8(c * kSaStep + lane * 8, v);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (v[i] >= least) atomicAdd(&hist[linear_bin(row.top, scale, v[i])][0], 1u);
@@ -593,10 +651,10 @@ __device__ __forceinline__ int candidates(cg::cluster_group& cluster, SaShared* 
     uint64_t* to = cluster.map_shared_rank(list, 0);
     int* count = cluster.map_shared_rank(&s->list_n, 0);
 #pragma unroll 1
-    for (int st = 0; st < steps; ++st) {
-      const int at = chunk_base + st * kSaStep + lane * 8;
+    for (int c = warp; c < x.cells; c += kSaWarps) {
+      const int at = c * kSaStep + lane * 8;
       float v[8];
-      load8<T>(x + at, v);
+      x.load8(at, v);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (v[i] >= least && linear_bin(row.top, scale, v[i]) <= bin)
@@ -607,54 +665,62 @@ __device__ __forceinline__ int candidates(cg::cluster_group& cluster, SaShared* 
   return n;
 }
 
-// The counts of four bins in every CTA, four reads of distributed shared memory in flight.
-template <typename F>
-__device__ __forceinline__ void each_rank(cg::cluster_group& cluster, const uint32_t* counts, int bin,
-                                          F&& take) {
-  const int ctas = (int)cluster.num_blocks();
+// The counts of four bins of block `block` a lane, in every part of the row in order; four reads of distributed shared memory in
+// flight.
+template <typename T, typename F>
+__device__ __forceinline__ void each_part(cg::cluster_group& cluster, const uint32_t* counts, int parts,
+                                          int block, F&& take) {
+  const int all = (int)cluster.num_blocks() * parts;
+  using Load = std::conditional_t<kSaTable<T>, uint4, uint2>;
+  const int at = block * (kSaBlock * kSaValueWords<T> / kSaValueBins<T>) +
+                 (threadIdx.x & 31) * (int)(sizeof(Load) / 4);
+  int cta = 0, part = 0;
 #pragma unroll 1
-  for (int r0 = 0; r0 < ctas; r0 += 4) {
-    uint4 h[4];
+  for (int r0 = 0; r0 < all; r0 += 4) {
+    Load h[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (r0 + j < ctas)
-        h[j] = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(counts, r0 + j) + bin);
+    for (int j = 0; j < 4; ++j) {
+      if (r0 + j >= all) break;
+      h[j] = *reinterpret_cast<const Load*>(cluster.map_shared_rank(counts, cta) +
+                                            part * kSaValueWords<T> + at);
+      if (++part == parts) ++cta, part = 0;
+    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (r0 + j < ctas) take(r0 + j, h[j]);
+    for (int j = 0; j < 4; ++j) {
+      if (r0 + j >= all) break;
+      if constexpr (kSaTable<T>) {
+        const uint32_t n[4] = {h[j].x, h[j].y, h[j].z, h[j].w};
+        take(r0 + j, n);
+      } else {
+        const uint32_t n[4] = {h[j].x & 0xffff, h[j].x >> 16, h[j].y & 0xffff, h[j].y >> 16};
+        take(r0 + j, n);
+      }
+    }
   }
 }
 
-// Four value bins a lane of block `block`: counts of all CTAs and of this one, keys (0: none) and weights.
+// Four value bins a lane of block `block`: keys (0: of no single value) and weights.
 template <typename T>
 struct BinQuad {
-  uint32_t n[4], own[4], key[4];
+  uint32_t key[4];
   uint64_t w[4];
-  __device__ __forceinline__ BinQuad(cg::cluster_group& cluster, const uint32_t* counts, const Row& row,
-                                     const double* tab, const Values& v, int block) {
-    const int bin = block * kSaBlock + (threadIdx.x & 31) * 4;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) n[j] = 0;
-    each_rank(cluster, counts, bin, [&](int, const uint4& h) {
-      n[0] += h.x;
-      n[1] += h.y;
-      n[2] += h.z;
-      n[3] += h.w;
-    });
-    const uint4 mine = *reinterpret_cast<const uint4*>(counts + bin);
-    own[0] = mine.x;
-    own[1] = mine.y;
-    own[2] = mine.z;
-    own[3] = mine.w;
+  int lump;  // which of them is the lump; -1: none
+  __device__ __forceinline__ BinQuad(const Row& row, const double* tab, const Values& v, int block) {
+    const uint32_t bin = block * kSaBlock + (threadIdx.x & 31) * 4;
+    lump = bin <= v.n1 && v.n1 < bin + 4 ? (int)(v.n1 - bin) : -1;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      key[j] = bin_key<T>(v, bin + j);
-      w[j] = 0;
-      if (n[j] > 0) {
-        const float x = Bits16<T>::value(key[j]);
-        if (x >= row.floor_x) w[j] = weight(row, tab, x);
-      }
+      key[j] = bin_key(v, bin + j);
+      const float x = Bits16<T>::value(key[j]);
+      w[j] = key[j] && x >= row.floor_x ? weight(row, tab, x) : 0;
     }
+  }
+  // tokens that count, of n in each bin, and their mass, `lump_mass` that of those in the lump
+  __device__ __forceinline__ uint32_t tokens(const uint32_t* n, int j) const {
+    return key[j] || j == lump ? n[j] : 0;
+  }
+  __device__ __forceinline__ uint64_t mass(const uint32_t* n, int j, uint64_t lump_mass) const {
+    return j == lump ? lump_mass : n[j] * w[j];
   }
 };
 
@@ -667,8 +733,8 @@ struct ValueCut {
 };
 template <typename T, bool kMass>
 __device__ __forceinline__ bool value_cross(cg::cluster_group& cluster, SaShared* s,
-                                            const uint32_t* counts, const Row& row, const Values& v,
-                                            const uint64_t* sums, const uint64_t* before,
+                                            const uint32_t* counts, int parts, const Row& row,
+                                            const Values& v, uint64_t lump_mass, const uint64_t* sums, const uint64_t* before,
                                             uint64_t want, double target, ValueCut& cut) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool here = kMass ? (double)before[1] < target && (double)(before[1] + sums[1]) >= target
@@ -685,10 +751,19 @@ __device__ __forceinline__ bool value_cross(cg::cluster_group& cluster, SaShared
   const int owner = s->bin;
   if (owner < 0) return false;
   if (warp == 0) {
-    const BinQuad<T> q(cluster, counts, row, s->tab, v, owner);
+    const BinQuad<T> q(row, s->tab, v, owner);
+    uint32_t n[4] = {};
+    each_part<T>(cluster, counts, parts, owner, [&](int, const uint32_t* h) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) n[j] += h[j];
+    });
     uint64_t c = 0, m = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c += q.n[j], m += q.n[j] * q.w[j];
+    for (int j = 0; j < 4; ++j) {
+      n[j] = q.tokens(n, j);
+      c += n[j];
+      m += q.mass(n, j, lump_mass);
+    }
     uint64_t ci = c, mi = m;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -699,10 +774,10 @@ __device__ __forceinline__ bool value_cross(cg::cluster_group& cluster, SaShared
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint64_t nc = rc + q.n[j], nm = rm + q.n[j] * q.w[j];
-      if (q.n[j] > 0 && (kMass ? (double)rm < target && (double)nm >= target : rc < want && nc >= want)) {
+      const uint64_t nc = rc + n[j], nm = rm + q.mass(n, j, lump_mass);
+      if (n[j] > 0 && (kMass ? (double)rm < target && (double)nm >= target : rc < want && nc >= want)) {
         s->edge[0] = q.key[j];
-        s->edge[1] = q.n[j];
+        s->edge[1] = n[j];
         s->held = rc;
         s->above = rm;
       }
@@ -715,7 +790,7 @@ __device__ __forceinline__ bool value_cross(cg::cluster_group& cluster, SaShared
   cut.group = s->edge[1];
   cut.count = s->held;
   cut.mass = s->above;
-  return true;
+  return cut.key16 != 0;
 }
 
 template <typename T>
@@ -724,32 +799,34 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
   SaShared* s = reinterpret_cast<SaShared*>(smem);
   uint32_t* counts = reinterpret_cast<uint32_t*>(smem + (sizeof(SaShared) + 15) / 16 * 16);
   auto hists = reinterpret_cast<uint32_t(*)[kSaBins][3]>(counts);
-  T* x = reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(counts) + kSaHistBytes<T>);
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int row_id = blockIdx.x / ctas;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int slice = a.chunk * kSaWarps, base = rank * slice;
-  const int here = max(0, min(slice, a.vocab - base));  // tokens of this CTA
-  const int steps = a.chunk / kSaStep, chunk_base = warp * a.chunk;
-  for (int i = tid; i < kSaHistBytes<T> / 4; i += kSaThreads) counts[i] = 0;
+  const int hist_bytes = sa_hist_bytes<T>(a.parts);
+  for (int i = tid; i < hist_bytes / 16; i += kSaThreads)
+    reinterpret_cast<uint4*>(counts)[i] = make_uint4(0, 0, 0, 0);
   if (tid < 32) s->tab[tid] = exp2(tid / 32.0);
   if (tid == 0) s->list_n = 0;
+  if (tid < kSaMaxParts) s->lump_n[tid] = s->part.lump_mass[tid] = s->part.mass[tid] = 0;
   grid_dep_wait();
   grid_dep_launch();
-  // The slice into shared memory: 16 bytes at a time from the first aligned token on (rows of an odd
-  // vocabulary begin anywhere), -inf past its end. 16-bit values show their greatest on the way.
   float top = -INFINITY, least = INFINITY;
   bool bad = false;
-  {
-    const T* g = static_cast<const T*>(a.x) + row_id * a.stride + base;
+  const int slice = a.parts * a.part;
+  const T* g = static_cast<const T*>(a.x) + row_id * a.stride;
+  Slice<T> x;
+  int base = rank * slice;  // token at position 0
+  if constexpr (sizeof(T) == 4) {
+    // into shared memory, 16 bytes at a time from the first aligned token on
+    T* to = reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(counts) + hist_bytes);
+    g += base;
+    const int here = max(0, min(slice, a.vocab - base));
     constexpr int kVec = 16 / (int)sizeof(T);
     const int off = (int)((reinterpret_cast<uintptr_t>(g) & 15) / sizeof(T));
     const int head = min(here, off == 0 ? 0 : kVec - off), vecs = (here - head) / kVec;
     const uint4* gv = reinterpret_cast<const uint4*>(g + head);
     constexpr int kBatch = 8;
-    uint4 m = make_uint4(0, 0, 0, 0);
-    if constexpr (sizeof(T) == 2) m.x = m.y = m.z = m.w = Bits16<T>::bits_below(-INFINITY) * 0x10001u;
     for (int i0 = tid; i0 < vecs; i0 += kSaThreads * kBatch) {
       uint4 v[kBatch];
 #pragma unroll
@@ -760,45 +837,24 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
         const int i = i0 + j * kSaThreads;
         if (i >= vecs) break;
         if (head == 0) {
-          *reinterpret_cast<uint4*>(x + i * kVec) = v[j];
+          *reinterpret_cast<uint4*>(to + i * kVec) = v[j];
         } else {
           const T* t = reinterpret_cast<const T*>(&v[j]);
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) x[head + i * kVec + e] = t[e];
-        }
-        if constexpr (sizeof(T) == 2) {
-          m.x = Bits16<T>::max2(m.x, v[j].x);
-          m.y = Bits16<T>::max2(m.y, v[j].y);
-          m.z = Bits16<T>::max2(m.z, v[j].z);
-          m.w = Bits16<T>::max2(m.w, v[j].w);
+          for (int e = 0; e < kVec; ++e) to[head + i * kVec + e] = t[e];
         }
       }
     }
-    if constexpr (sizeof(T) == 2) {
-      const uint32_t both = Bits16<T>::max2(Bits16<T>::max2(m.x, m.y), Bits16<T>::max2(m.z, m.w));
-      const T* t = reinterpret_cast<const T*>(&both);
-      top = fmax_nan(logit(t[0]), logit(t[1]));
-    }
-    auto single = [&](int i) {
-      x[i] = g[i];
-      if constexpr (sizeof(T) == 2) top = fmax_nan(top, logit(g[i]));
-    };
-    for (int i = tid; i < head; i += kSaThreads) single(i);
-    for (int i = head + vecs * kVec + tid; i < here; i += kSaThreads) single(i);
-    for (int i = here + tid; i < slice; i += kSaThreads) x[i] = (T)(-INFINITY);
-  }
-  __syncthreads();
-
-  // the row's greatest and least logits, and whether one is NaN or +inf
-  if constexpr (sizeof(T) == 2) {
-    top += 0.f;
-    bad = !(top < INFINITY);
-    least = -FLT_MAX;  // (a bound is all that the search asks for)
-  } else {
+    for (int i = tid; i < head; i += kSaThreads) to[i] = g[i];
+    for (int i = head + vecs * kVec + tid; i < here; i += kSaThreads) to[i] = g[i];
+    for (int i = here + tid; i < slice; i += kSaThreads) to[i] = (T)(-INFINITY);
+    __syncthreads();
+    x = {to, 0, here, (here + kSaStep - 1) / kSaStep};
+    // the row's greatest and least logits, and whether one is NaN or +inf
 #pragma unroll 1
-    for (int st = 0; st < steps; ++st) {
+    for (int c = warp; c < x.cells; c += kSaWarps) {
       float v[8];
-      load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
+      x.load8(c * kSaStep + lane * 8, v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         bad |= !(v[i] < INFINITY);
@@ -806,6 +862,36 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
         least = fminf(least, v[i] == -INFINITY ? INFINITY : v[i]);
       }
     }
+  } else {
+    // the greatest, NaN if any is
+    const int lead = (int)((reinterpret_cast<uintptr_t>(g) & 15) / sizeof(T));
+    x = {g - lead + base, base == 0 ? lead : 0, max(0, min(slice, a.vocab + lead - base)), 0};
+    x.cells = (x.hi + kSaStep - 1) / kSaStep;
+    base -= lead;
+    constexpr int kBatch = 8;
+    uint4 m;
+    m.x = m.y = m.z = m.w = Bits16<T>::bits_below(-INFINITY) * 0x10001u;
+#pragma unroll 1
+    for (int c0 = warp; c0 < x.cells; c0 += kSaWarps * kBatch) {
+      uint4 v[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        v[j] = m;
+        if (c0 + j * kSaWarps < x.cells) v[j] = x.raw8((c0 + j * kSaWarps) * kSaStep + lane * 8);
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        m.x = Bits16<T>::max2(m.x, v[j].x);
+        m.y = Bits16<T>::max2(m.y, v[j].y);
+        m.z = Bits16<T>::max2(m.z, v[j].z);
+        m.w = Bits16<T>::max2(m.w, v[j].w);
+      }
+    }
+    const uint32_t both = Bits16<T>::max2(Bits16<T>::max2(m.x, m.y), Bits16<T>::max2(m.z, m.w));
+    const T* t = reinterpret_cast<const T*>(&both);
+    top = fmax_nan(logit(t[0]), logit(t[1])) + 0.f;
+    bad = !(top < INFINITY);
+    least = -FLT_MAX;  // (a bound is all that the search asks for)
   }
   float low = top > -INFINITY ? top : INFINITY;  // least of the threads' greatest
   const int threads = __syncthreads_count(top > -INFINITY);
@@ -861,12 +947,12 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
     // the first of the greatest
     int at = INT_MAX;
 #pragma unroll 1
-    for (int st = 0; st < steps && at == INT_MAX; ++st) {
+    for (int c = warp; c < x.cells && at == INT_MAX; c += kSaWarps) {
       float v[8];
-      load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
+      x.load8(c * kSaStep + lane * 8, v);
 #pragma unroll
       for (int i = 7; i >= 0; --i)
-        if (v[i] == top) at = base + chunk_base + st * kSaStep + lane * 8 + i;
+        if (v[i] == top) at = base + c * kSaStep + lane * 8 + i;
       at = __reduce_min_sync(0xffffffffu, at);
     }
     if (lane == 0) s->w_ties[warp] = at;
@@ -907,81 +993,94 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
     cut.key = s->min_key;
   }
 
-  int64_t ties_before = 0, own_ties = 0;  // tokens that equal the cut: before this CTA, and in it
-  uint64_t own = 0;                       // kept mass of this CTA's tokens
-  bool counted = false;                   // whether the values' counts tell these
+  bool counted = false;  // whether the values' counts tell the cut and the parts' kept masses
   [[maybe_unused]] Values bins = {};
   if constexpr (sizeof(T) == 2) {
     constexpr int kBlocks = kSaBlocks<T>;
-    static_assert(kBlocks <= 128 && kBlocks % kSaMaxCluster == 0, "a thread per block of bins");
+    static_assert(kBlocks % kSaMaxCluster == 0 && kBlocks <= kSaMaxBlocks &&
+                  Bits16<T>::kMaxParts * kBlocks <= kSaMaxOwn);
     bins = value_bins<T>(row);
-    const uint32_t span = bins.top - bins.lowest;
-    int lump_n = 0;
-    uint64_t lump_m = 0;
+    const uint32_t end_bin = bins.n1 + 1 + bins.n2;  // (an add to one word by all lanes costs 32 of them)
+    // values in the lump are listed, and weighed when the part is done
+    uint16_t* lump_list = reinterpret_cast<uint16_t*>(s->step_mass);
+    auto lump_weight = [&](uint32_t k) {
+      const float v = Bits16<T>::value(k);
+      return v >= row.floor_x ? weight(row, s->tab, v) : 0;
+    };
 #pragma unroll 1
-    for (int st = 0; st < steps; ++st) {
-      const uint4 raw = *reinterpret_cast<const uint4*>(x + chunk_base + st * kSaStep + lane * 8);
-      const uint32_t pair[4] = {raw.x, raw.y, raw.z, raw.w};
-      uint32_t lumps = 0;
+    for (int part = 0; part < a.parts; ++part) {
+      uint32_t* to = counts + part * kSaValueWords<T>;
+      const int end = min((part + 1) * (a.part / kSaStep), x.cells);
+      int c = part * (a.part / kSaStep) + warp;
+      uint64_t lump_m = 0;
+      uint4 next = make_uint4(0, 0, 0, 0);
+      if (c < end) next = x.raw8(c * kSaStep + lane * 8);
+#pragma unroll 1
+      for (; c < end; c += kSaWarps) {
+        const uint4 raw = next;
+        if (c + kSaWarps < end) next = x.raw8((c + kSaWarps) * kSaStep + lane * 8);
+        const uint32_t of[4] = {value_bins2(bins, raw.x), value_bins2(bins, raw.y),
+                                value_bins2(bins, raw.z), value_bins2(bins, raw.w)};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        // (no key is above the greatest: the halves do not borrow)
-        const uint32_t below = bins.top * 0x10001u - keys16(pair[i >> 1]);
-        const uint32_t d = i & 1 ? below >> 16 : below & 0xffff;
-        const int bin = value_bin<T>(bins, d);
-        if (bin >= 0) atomicAdd(&counts[bin], 1u);
-        else if (d <= span) lumps |= 1u << i;
-      }
-      if (lumps) {
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t bin = i & 1 ? of[i >> 1] >> 16 : of[i >> 1] & 0xffff;
+          if constexpr (kSaTable<T>) atomicAdd(&to[bin], 1u);
+          else if (bin < end_bin) atomicAdd(&to[bin >> 1], 1u << (bin & 1) * 16);
+        }
+        if (any_lump(bins, of)) {
+          uint32_t lumps = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if ((i & 1 ? of[i >> 1] >> 16 : of[i >> 1] & 0xffff) == bins.n1) lumps |= 1u << i;
 #pragma unroll 1
-        for (; lumps; lumps &= lumps - 1) {
-          const int i = __ffs((int)lumps) - 1;
-          const uint32_t word = i < 4 ? (i < 2 ? raw.x : raw.y) : (i < 6 ? raw.z : raw.w);
-          const uint32_t below = bins.top * 0x10001u - keys16(word);
-          const uint32_t d = i & 1 ? below >> 16 : below & 0xffff;
-          const float v = Bits16<T>::value(bins.top - d);
-          ++lump_n;
-          if (v >= row.floor_x) lump_m += weight(row, s->tab, v);
+          for (; lumps; lumps &= lumps - 1) {
+            const int i = __ffs((int)lumps) - 1;
+            const uint32_t key = keys16(i < 4 ? (i < 2 ? raw.x : raw.y) : (i < 6 ? raw.z : raw.w));
+            const uint32_t k = i & 1 ? key >> 16 : key & 0xffff;
+            const int at = atomicAdd(&s->lump_n[part], 1);
+            if (at < kSaLumps) lump_list[at] = (uint16_t)k;
+            else lump_m += lump_weight(k);
+          }
         }
       }
+      // the lump's weights, a thread each
+      __syncthreads();
+      const int lump_n = s->lump_n[part];
+      if (lump_n > 0) {
+        for (int i = tid; i < min(lump_n, kSaLumps); i += kSaThreads) lump_m += lump_weight(lump_list[i]);
+        lump_m = warp_sum(lump_m);
+        if (lane == 0) atomicAdd(&s->part.lump_mass[part], (unsigned long long)lump_m);
+        __syncthreads();
+      }
     }
-    const uint64_t warp_lump_m = warp_sum(lump_m);
-    lump_n = __reduce_add_sync(0xffffffffu, lump_n);
-    if (lane == 0) {
-      s->w_ties[warp] = lump_n;
-      s->lump_mass[warp] = warp_lump_m;
-    }
-    __syncthreads();
-    if (tid == 0) {
-      int n = 0;
-      uint64_t m = 0;
-      for (int w = 0; w < kSaWarps; ++w) n += s->w_ties[w], m += s->lump_mass[w];
-      s->part.lump_count = n;
-      s->part.lump_mass = m;
-    }
+    if (tid < kSaMaxParts) s->part.lump_count[tid] = s->lump_n[tid];
     cluster.sync();
     uint64_t lump_count = 0, lump_mass = 0;
     for (int r = 0; r < ctas; ++r) {
-      lump_count += cluster.map_shared_rank(&s->part, r)->lump_count;
-      lump_mass += cluster.map_shared_rank(&s->part, r)->lump_mass;
+      const SaPart* p = cluster.map_shared_rank(&s->part, r);
+      for (int part = 0; part < a.parts; ++part) {
+        lump_count += p->lump_count[part];
+        lump_mass += p->lump_mass[part];
+      }
     }
-    // the sums of every block of bins, of all CTAs' tokens and of each one's: a share of the blocks each
+    // the sums of every block of bins, of all tokens and of each part's: a share of the blocks each
     const int share = kBlocks / ctas;
 #pragma unroll 1
     for (int i = warp; i < share; i += kSaWarps) {
       const int block = rank * share + i;
-      uint64_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t key = bin_key<T>(bins, block * kSaBlock + lane * 4 + j);
-        const float v = Bits16<T>::value(key);
-        w[j] = key && v >= row.floor_x ? weight(row, s->tab, v) : 0;
-      }
+      const BinQuad<T> q(row, s->tab, bins, block);
       uint32_t n = 0;
       uint64_t m = 0;
-      each_rank(cluster, counts, block * kSaBlock + lane * 4, [&](int r, const uint4& h) {
-        const uint64_t o = warp_sum(h.x * w[0] + h.y * w[1] + h.z * w[2] + h.w * w[3]);
-        n += h.x + h.y + h.z + h.w;
+      each_part<T>(cluster, counts, a.parts, block, [&](int r, const uint32_t* h) {
+        uint64_t lump = 0, o = 0;
+        if (q.lump >= 0)
+          lump = cluster.map_shared_rank(&s->part, r / a.parts)->lump_mass[r % a.parts];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          n += q.tokens(h, j);
+          o += q.mass(h, j, lump);
+        }
+        o = warp_sum(o);
         m += o;
         if (lane == 0) s->block_own[r * share + i] = o;
       });
@@ -992,22 +1091,19 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
       }
     }
     cluster.sync();
-    uint64_t sums[2] = {0, 0}, before[2], all[2], own_block = 0;
+    uint64_t sums[2] = {0, 0}, before[2], all[2];
     if (tid < kBlocks) {
       const SaShared* at = cluster.map_shared_rank(s, tid / share);
       sums[0] = at->block_count[tid % share];
       sums[1] = at->block_mass[tid % share];
-      own_block = at->block_own[rank * share + tid % share];
     }
     block_exclusive<2>(sums, s->scan, before, all);
-    if (tid >= kBlocks / 2) before[0] += lump_count, before[1] += lump_mass;
-    all[0] += lump_count;
-    all[1] += lump_mass;
     counted = true;
     Cut c = {0u, 0, true};
     ValueCut vc;
     if (k > 0 && (uint64_t)k < all[0]) {
-      counted = value_cross<T, false>(cluster, s, counts, row, bins, sums, before, (uint64_t)k, 0.0, vc);
+      counted = value_cross<T, false>(cluster, s, counts, a.parts, row, bins, lump_mass, sums, before,
+                                        (uint64_t)k, 0.0, vc);
       if (counted) {
         const float v = Bits16<T>::value(vc.key16);
         c = {key_of(v), k - (int64_t)vc.count, k - (int64_t)vc.count >= (int64_t)vc.group};
@@ -1016,7 +1112,8 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
     }
     if (counted && top_p < 1.f) {
       const double target = fmax((double)top_p * (double)all[1], 1.0);
-      counted = value_cross<T, true>(cluster, s, counts, row, bins, sums, before, 0, target, vc);
+      counted = value_cross<T, true>(cluster, s, counts, a.parts, row, bins, lump_mass, sums, before, 0,
+                                       target, vc);
       if (counted) {
         const float v = Bits16<T>::value(vc.key16);
         const int64_t r = kept_ties(target, vc.mass, weight(row, s->tab, v), vc.group);
@@ -1026,63 +1123,61 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
     if (counted) {
       c = tighter(cut, c);
       // a cut (of min-p) within the lump is left to the search
-      const uint32_t lump_hi = bins.top - bins.n1;  // its greatest key
-      const uint32_t lump_lo = bins.n2 ? bins.top - bins.off2 + 1 : bins.lowest;
-      const bool lump_in = lump_count > 0 && c.key <= key_of(Bits16<T>::value(lump_lo));
-      if (lump_count > 0 && !lump_in && c.key <= key_of(Bits16<T>::value(lump_hi))) counted = false;
+      if (lump_count > 0 && c.key > key_of(Bits16<T>::value(bin_low(bins, bins.n1))) &&
+          c.key <= key_of(Bits16<T>::value(bin_high(bins, bins.n1))))
+        counted = false;
       if (counted) {
-        // this CTA's kept mass: blocks above the cut, and of the one that holds it the bins above and a share of
-        // the ties
-        uint64_t m = 0;
-        if (tid == 0) {
-          s->bin = -1;
-          s->extra = 0;
-        }
-        __syncthreads();
-        if (tid < kBlocks) {
-          const uint32_t R = Bits16<T>::kRegion, first = tid * kSaBlock;
-          const uint32_t n = first < R ? bins.n1 : bins.n2, at = first < R ? first : first - R;
-          if (at < n) {
-            const uint32_t last = first + min((uint32_t)kSaBlock, n - at) - 1;
-            if (key_of(Bits16<T>::value(bin_key<T>(bins, last))) > c.key) m = own_block;
-            else if (key_of(Bits16<T>::value(bin_key<T>(bins, first))) >= c.key) s->bin = tid;
+        // kept masses of this CTA's parts, a warp each: blocks above the cut, and of the one that holds it the bins
+        // above and a share of the ties
+        if (warp < a.parts) {
+          const int mine = rank * a.parts + warp;
+          uint64_t m = 0;
+          int cut_block = -1;
+          for (int block = lane; block < kBlocks; block += 32) {
+            const uint32_t first = block * kSaBlock, end = bins.n1 + 1 + bins.n2;
+            if (first >= end) continue;
+            const uint32_t last = min(first + (uint32_t)kSaBlock, end) - 1;
+            if (key_of(Bits16<T>::value(bin_low(bins, last))) > c.key)
+              m += cluster.map_shared_rank(s, block / share)->block_own[mine * share + block % share];
+            else if (key_of(Bits16<T>::value(bin_high(bins, first))) >= c.key)
+              cut_block = block;
           }
-        }
-        __syncthreads();
-        if (warp == 0 && s->bin >= 0) {
-          const BinQuad<T> q(cluster, counts, row, s->tab, bins, s->bin);
-          uint64_t o = 0;
+          cut_block = __reduce_max_sync(0xffffffffu, cut_block);
+          if (cut_block >= 0) {
+            uint32_t ahead[4] = {}, own[4] = {};
+            each_part<T>(cluster, counts, a.parts, cut_block, [&](int r, const uint32_t* h) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t key = q.key[j] ? key_of(Bits16<T>::value(q.key[j])) : 0;
-            int64_t n = q.key[j] && key >= c.key ? q.own[j] : 0;
-            if (key == c.key && q.key[j] && !c.all_ties) {
-              const int bin = s->bin * kSaBlock + lane * 4 + j;
-              int64_t ahead = 0;
-              for (int r = 0; r < rank; ++r) ahead += cluster.map_shared_rank(counts, r)[bin];
-              s->tie_base[0] = ahead;
-              s->tie_base[1] = n;
-              n = max((int64_t)0, min(n, c.ties - ahead));
+              for (int j = 0; j < 4; ++j) {
+                if (r < mine) ahead[j] += h[j];
+                if (r == mine) own[j] = h[j];
+              }
+            });
+            const BinQuad<T> q(row, s->tab, bins, cut_block);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (j == q.lump && lump_count > 0 &&
+                  c.key <= key_of(Bits16<T>::value(bin_low(bins, bins.n1))))
+                m += s->part.lump_mass[warp];
+              const uint32_t key = q.key[j] ? key_of(Bits16<T>::value(q.key[j])) : 0;
+              if (q.key[j] == 0 || key < c.key) continue;
+              int64_t n = own[j];
+              if (key == c.key && !c.all_ties) {
+                s->tie_base[warp][0] = ahead[j];
+                s->tie_base[warp][1] = n;
+                n = max((int64_t)0, min(n, c.ties - (int64_t)ahead[j]));
+              }
+              m += n * q.w[j];
             }
-            o += n * q.w[j];
           }
-          o = warp_sum(o);
-          if (lane == 0) s->extra = o;
-        }
-        if (tid == 0 && lump_in) m += s->part.lump_mass;
-        uint64_t unused;
-        block_exclusive<1>(&m, s->scan, &unused, &own);
-        own += s->extra;
-        if (!c.all_ties) {
-          ties_before = s->tie_base[0];
-          own_ties = s->tie_base[1];
+          m = warp_sum(m);
+          if (lane == 0) s->part.mass[warp] = m;
         }
         cut = c;
       }
     }
     if (!counted) {  // the histograms' place is taken by the search's
       cluster.sync();
-      for (int i = tid; i < kSaHistBytes<T> / 4; i += kSaThreads) counts[i] = 0;
+      for (int i = tid; i < 2 * kSaBins * 3; i += kSaThreads) counts[i] = 0;
       __syncthreads();
     }
   }
@@ -1093,8 +1188,7 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
       // few tokens stay: one CTA takes them (128256 fp32, top-k of 50, top-p and min-p: 36 us, 19 so)
       if (k > 0 && k <= kSaListK && k <= with) {
         uint64_t* list = reinterpret_cast<uint64_t*>(&hists[2][0][0]);
-        const int n = candidates<T>(cluster, s, hists, list, x, steps, chunk_base, base, row, key_of(low), k,
-                                    level);
+        const int n = candidates<T>(cluster, s, hists, list, x, base, row, key_of(low), k, level);
         if (n >= 0) {
           if (rank == 0)
             sample_list(s, list, reinterpret_cast<uint64_t*>(counts),
@@ -1107,8 +1201,7 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
     if (k > 0 && k < a.vocab) {
       // as many threads as `with` have a logit of at least `low`
       const float from = k <= with ? low : least;
-      const Cut c = search<T, false>(cluster, s, hists, x, steps, chunk_base, row, key_of(from), k, 0.0,
-                                     0, level);
+      const Cut c = search<T, false>(cluster, s, hists, x, row, key_of(from), k, 0.0, 0, level);
       if (c.key != 0 && !c.all_ties) {
         const float value = of_key(c.key);
         if (value >= row.floor_x) drop = (s->held - (uint64_t)c.ties) * weight(row, s->tab, value);
@@ -1117,47 +1210,45 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
       const Cut before = cut;
       cut = c;
       if (top_p < 1.f) {
-        const Cut p = search<T, true>(cluster, s, hists, x, steps, chunk_base, row,
-                                      max(c.key, key_of(row.floor_x)), 0, (double)top_p, drop, level);
+        const Cut p = search<T, true>(cluster, s, hists, x, row, max(c.key, key_of(row.floor_x)), 0, (double)top_p, drop, level);
         cut = tighter(cut, p);
       }
       cut = tighter(before, cut);
     } else if (top_p < 1.f) {
-      const Cut p = search<T, true>(cluster, s, hists, x, steps, chunk_base, row,
-                                    max(key_of(least), key_of(row.floor_x)), 0, (double)top_p, 0, level);
+      const Cut p = search<T, true>(cluster, s, hists, x, row, max(key_of(least), key_of(row.floor_x)), 0, (double)top_p, 0, level);
       cut = tighter(cut, p);
     }
   }
 
-  // Which ties stay: those whose index in this CTA is below tie_end. Where that lies within the CTA, its
-  // 256-token steps' ties are counted first.
-  const int cells = kSaWarps * steps;
+  // Which ties stay: those at positions below tie_end. Where that lies within the cells from `first` to `end`, their
+  // ties are counted cell by cell.
+  int first = 0, end = x.cells;
   auto tie_counts = [&]() {  // of this thread's cell
 #pragma unroll 1
-    for (int st = 0; st < steps; ++st) {
+    for (int c = first + warp; c < end; c += kSaWarps) {
       float v[8];
-      load8<T>(x + chunk_base + st * kSaStep + lane * 8, v);
+      x.load8(c * kSaStep + lane * 8, v);
       int n = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) n += key_of(v[i]) == cut.key;
       n = __reduce_add_sync(0xffffffffu, n);
-      if (lane == 0) s->step_mass[warp * steps + st] = (uint64_t)n;
+      if (lane == 0) s->step_mass[c] = (uint64_t)n;
     }
     __syncthreads();
-    return tid < cells ? s->step_mass[tid] : 0;
+    return first + tid < end ? s->step_mass[first + tid] : 0;
   };
-  auto find_tie_end = [&](int64_t keep, uint64_t in_cell) {  // place of tie number `keep`, 0 <= keep < own_ties
+  auto find_tie_end = [&](int64_t keep, uint64_t in_cell) {  // place of tie number `keep` of them
     uint64_t before, all;
     block_exclusive<1>(&in_cell, s->scan, &before, &all);
     if (in_cell > 0 && (int64_t)before <= keep && keep < (int64_t)(before + in_cell)) {
-      s->bin = tid;
+      s->bin = first + tid;
       s->above = before;
     }
     __syncthreads();
     const int cell = s->bin;
-    if (warp == cell / steps) {
+    if (warp == 0) {
       float v[8];
-      load8<T>(x + cell * kSaStep + lane * 8, v);
+      x.load8(cell * kSaStep + lane * 8, v);
       int n = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) n += key_of(v[i]) == cut.key;
@@ -1180,18 +1271,18 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
     const uint64_t in_cell = tie_counts();
     uint64_t before, all;
     block_exclusive<1>(&in_cell, s->scan, &before, &all);
-    own_ties = (int64_t)all;
     if (tid == 0) s->part.ties = (int)all;
     cluster.sync();
+    int64_t ties_before = 0;
     for (int r = 0; r < rank; ++r) ties_before += cluster.map_shared_rank(&s->part, r)->ties;
     const int64_t keep = cut.ties - ties_before;
-    if (keep < own_ties) tie_end = keep > 0 ? find_tie_end(keep, in_cell) : 0;
+    if (keep < (int64_t)all) tie_end = keep > 0 ? find_tie_end(keep, in_cell) : 0;
   }
   // kept weights of the 8 tokens at `at`
   auto kept = [&](int at, uint64_t* w) {
     uint64_t sum = 0;
     float v[8];
-    load8<T>(x + at, v);
+    x.load8(at, v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t key = key_of(v[i]);
@@ -1201,62 +1292,64 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
     }
     return sum;
   };
-  uint64_t cell = 0, before = 0, all = 0;  // a thread's cell: 256 tokens of the CTA
-  auto add_cells = [&]() {
+  uint64_t cell = 0, before = 0, all = 0;  // a thread's cell
+  if (!counted) {
 #pragma unroll 1
-    for (int st = 0; st < steps; ++st) {
+    for (int c = warp; c < end; c += kSaWarps) {
       uint64_t w[8];
-      const uint64_t sum = warp_sum(kept(chunk_base + st * kSaStep + lane * 8, w));
-      if (lane == 0) s->step_mass[warp * steps + st] = sum;
+      const uint64_t sum = warp_sum(kept(c * kSaStep + lane * 8, w));
+      if (lane == 0) s->step_mass[c] = sum;
     }
     __syncthreads();
-    cell = tid < cells ? s->step_mass[tid] : 0;
+    cell = tid < end ? s->step_mass[tid] : 0;
     block_exclusive<1>(&cell, s->scan, &before, &all);
-  };
-  if (!counted) {
-    add_cells();
-    own = all;
+    if (tid == 0) s->part.mass[0] = all;
   }
-  if (tid == 0) {
-    s->part.mass = own;
-    s->bin = -1;
-  }
+  if (tid == 0) s->bin = -1;
   cluster.sync();
-  uint64_t mass = 0, ahead = 0;
-  int last = 0;  // the last CTA with a kept token
-  for (int r = 0; r < ctas; ++r) {
-    const uint64_t m = cluster.map_shared_rank(&s->part, r)->mass;
-    if (r < rank) ahead += m;
-    if (m > 0) last = r;
-    mass += m;
-  }
+  // the first part, cell and token whose running sum passes the target; the last kept one where none
+  // does (u = 1, NaN). A lane per part.
+  uint64_t own = 0;
+  if (lane < ctas * a.parts) own = cluster.map_shared_rank(&s->part, lane / a.parts)->mass[lane % a.parts];
   cluster.barrier_arrive();  // (this CTA has read; from here on it is on its own)
-  // the first CTA, cell and token whose running sum passes the target; the last kept one where none
-  // does (u = 1, NaN)
+  uint64_t ahead = own;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const uint64_t o = __shfl_up_sync(0xffffffffu, ahead, off);
+    if (lane >= off) ahead += o;
+  }
+  const uint64_t mass = __shfl_sync(0xffffffffu, ahead, 31);
   const double target = (double)u * (double)mass;
   const bool none = !((double)mass > target);
   auto passes = [&](uint64_t sum_before, uint64_t part) {
     return (double)(sum_before + part) > target && (sum_before == 0 || !((double)sum_before > target));
   };
-  if (own == 0 || !(none ? rank == last : passes(ahead, own))) {
+  const uint32_t in_part =
+      __ballot_sync(0xffffffffu, own > 0 && (none ? ahead == mass : passes(ahead - own, own)));
+  const int part = __ffs((int)in_part) - 1;
+  if (part < 0 || part / a.parts != rank) {
     cluster.barrier_wait();
     return;
   }
+  ahead = __shfl_sync(0xffffffffu, ahead - own, part);
+  own = __shfl_sync(0xffffffffu, own, part);
   int found = -1;         // the cell
   uint64_t above = 0;     // kept mass before it
   uint64_t w[8], sum;     // of this lane's tokens in it
   if (counted) {
+    first = part % a.parts * (a.part / kSaStep);
+    end = min(first + a.part / kSaStep, x.cells);
     if (!cut.all_ties) {
-      const int64_t keep = cut.ties - ties_before;
-      if (keep < own_ties) tie_end = keep > 0 ? find_tie_end(keep, tie_counts()) : 0;
+      const int64_t keep = cut.ties - s->tie_base[part % a.parts][0];
+      if (keep < s->tie_base[part % a.parts][1]) tie_end = keep > 0 ? find_tie_end(keep, tie_counts()) : 0;
     }
-    [[maybe_unused]] uint32_t tie_d = 0xffffffffu;  // of the cut, where only some of its tokens stay
+    [[maybe_unused]] uint32_t tie_bin = 0xffffffffu;  // of the cut, where only some of its tokens stay
     if constexpr (kSaTable<T>) {  // the values' kept weights, over their counts
       if (tie_end != INT_MAX)
-        tie_d = bins.top - (keys16(Bits16<T>::bits_below(of_key(cut.key))) & 0xffff);
+        tie_bin = value_bins2(bins, Bits16<T>::bits_below(of_key(cut.key)) * 0x10001u) & 0xffff;
       __syncthreads();
       for (int bin = tid; bin < kSaValueBins<T>; bin += kSaThreads) {
-        const uint32_t key16 = bin_key<T>(bins, bin);
+        const uint32_t key16 = bin_key(bins, bin);
         const float v = Bits16<T>::value(key16);
         reinterpret_cast<uint64_t*>(counts)[bin] =
             key16 != 0 && v >= row.floor_x && key_of(v) >= cut.key ? weight(row, s->tab, v) : 0;
@@ -1268,28 +1361,27 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
         return kept(at, w);
       } else {
         const uint64_t* table = reinterpret_cast<const uint64_t*>(counts);
-        const uint4 raw = *reinterpret_cast<const uint4*>(x + at);
-        const uint32_t pair[4] = {raw.x, raw.y, raw.z, raw.w};
-        bool lumps = false;
+        const uint4 raw = x.raw8(at);
+        const uint32_t of[4] = {value_bins2(bins, raw.x), value_bins2(bins, raw.y),
+                                value_bins2(bins, raw.z), value_bins2(bins, raw.w)};
+        if (any_lump(bins, of)) return kept(at, w);
         uint64_t sum = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const uint32_t below = bins.top * 0x10001u - keys16(pair[i >> 1]);
-          const uint32_t d = i & 1 ? below >> 16 : below & 0xffff;
-          const int bin = value_bin<T>(bins, d);
-          w[i] = bin >= 0 ? table[bin] : 0;
-          lumps |= bin < 0 && d <= bins.top - bins.lowest;
-          if (d == tie_d && at + i >= tie_end) w[i] = 0;
+          const uint32_t bin = i & 1 ? of[i >> 1] >> 16 : of[i >> 1] & 0xffff;
+          w[i] = table[bin];
+          if (bin == tie_bin && at + i >= tie_end) w[i] = 0;
           sum += w[i];
         }
-        return lumps ? kept(at, w) : sum;
+        return sum;
       }
     };
     // 256 tokens a warp in index order, as far as the target
     uint64_t run = ahead;
 #pragma unroll 1
-    for (int cell0 = 0; found < 0 && cell0 < cells; cell0 += kSaWarps) {
-      sum = kept_by_value((cell0 + warp) * kSaStep + lane * 8, w);
+    for (int cell0 = first; found < 0 && cell0 < end; cell0 += kSaWarps) {
+      sum = 0;
+      if (cell0 + warp < end) sum = kept_by_value((cell0 + warp) * kSaStep + lane * 8, w);
       const uint64_t mass_here = warp_sum(sum);
       if (lane == 0) s->step_mass[cell0 + warp] = mass_here;
       __syncthreads();
@@ -1309,7 +1401,7 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
       }
       run += __shfl_sync(0xffffffffu, to, kSaWarps - 1);
     }
-    if (warp != found % kSaWarps) found = -1;
+    if (warp != (found - first) % kSaWarps) found = -1;
   } else {
     if (cell > 0 && (none ? before + cell == all : passes(ahead + before, cell))) {
       s->bin = tid;
@@ -1317,7 +1409,7 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
     }
     __syncthreads();
     above = s->above;
-    if (s->bin >= 0 && warp == s->bin / steps) {
+    if (s->bin >= 0 && warp == s->bin % kSaWarps) {
       found = s->bin;
       sum = kept(found * kSaStep + lane * 8, w);
     }
@@ -1347,13 +1439,14 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
 
 template <typename T>
 static int launch_sample(const SampleArgs& a, int64_t rows, int ctas, cudaStream_t st) {
-  const size_t smem =
-      (sizeof(SaShared) + 15) / 16 * 16 + kSaHistBytes<T> + (size_t)a.chunk * kSaWarps * sizeof(T);
+  const size_t shared = (sizeof(SaShared) + 15) / 16 * 16;
+  constexpr int kHeld = sizeof(T) == 4 ? 4 : 0;  // bytes of a token in shared memory
+  const size_t smem = shared + sa_hist_bytes<T>(a.parts) + (size_t)a.part * kHeld;
   static DeviceOnce once;
-  cudaError_t e = once.run([] {
-    return cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)((sizeof(SaShared) + 15) / 16 * 16) + kSaHistBytes<T> +
-                                    kSaWarps * kSaSteps * kSaStep * (int)sizeof(T));
+  cudaError_t e = once.run([&] {
+    return cudaFuncSetAttribute(
+        sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        (int)shared + sa_hist_bytes<T>(Bits16<T>::kMaxParts) + kSaRows32 * kHeld);
   });
   if (e != cudaSuccess) return cuda_fail(e, "fi_sample_tokens: kernel set-up");
   e = launch_pdl_cluster(sample_kernel<T>, dim3((unsigned)(rows * ctas)), dim3(kSaThreads), smem, st,
@@ -1382,15 +1475,30 @@ extern "C" int fi_sample_tokens(const void* logits, const float* u, const float*
   const int size = dtype == FI_DTYPE_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(logits) % size != 0)
     return fail(FI_ERR_ALIGNMENT, "fi_sample_tokens: logits not aligned to their type");
-  // as few CTAs a row as its tokens allow (bf16: 32768 each, else 16384: two CTAs an SM), more where there are too
-  // few rows for two CTAs an SM
-  int ctas = 1;
-  const int64_t most = (int64_t)kSaWarps * kSaSteps * kSaStep / (dtype == FI_DTYPE_BF16 ? 1 : 2);
-  while (ctas < kSaMaxCluster && (ctas * most < vocab ||
-                                  (rows * ctas < 2 * sm_count() &&
-                                   (int64_t)ctas * kSaWarps * kSaStep < vocab)))
+  // 32-bit logits: as few CTAs a row as hold it at 16384 tokens each (two CTAs an SM), more where there are too few rows for
+  // two CTAs an SM. 16-bit ones: as many as find room at the same time, two an SM; the slice in parts.
+  int ctas = 1, parts = 1;
+  int64_t part = 0;
+  const int64_t room = 2 * sm_count();
+  auto split = [&] {
+    if (dtype != FI_DTYPE_F32) {
+      parts = (int)((vocab + ctas * kSaPart - 1) / (ctas * kSaPart));
+      parts = std::min(parts, dtype == FI_DTYPE_BF16 ? Bits16<__nv_bfloat16>::kMaxParts
+                                                     : Bits16<__half>::kMaxParts);
+    }
+    const int64_t each = (vocab + (size == 2 ? 7 : 0) + ctas * parts - 1) / (ctas * parts);
+    part = (each + kSaRound - 1) / kSaRound * kSaRound;
+  };
+  split();
+  while (ctas < kSaMaxCluster) {
+    const int64_t most = size == 4 ? kSaRows32 / 2 : kSaMaxTokens;
+    const bool needs = (parts * part < vocab ? parts * part : vocab) > most;
+    const bool wants = (int64_t)ctas * kSaRound < vocab &&
+                       (size == 4 ? rows * ctas < room : rows * ctas * 2 <= room);
+    if (!needs && !wants) break;
     ctas *= 2;
-  const int64_t per_warp = (vocab + ctas * kSaWarps - 1) / (ctas * kSaWarps);
+    split();
+  }
   SampleArgs a = {};
   a.x = logits;
   a.stride = row_stride;
@@ -1405,7 +1513,8 @@ extern "C" int fi_sample_tokens(const void* logits, const float* u, const float*
   a.min_p1 = min_p_scalar;
   a.out = out;
   a.vocab = (int)vocab;
-  a.chunk = (int)((per_warp + kSaStep - 1) / kSaStep * kSaStep);
+  a.parts = parts;
+  a.part = (int)part;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == FI_DTYPE_F32) return launch_sample<float>(a, rows, ctas, st);
   return dtype == FI_DTYPE_F16 ? launch_sample<__half>(a, rows, ctas, st)
