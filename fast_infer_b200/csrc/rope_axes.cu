@@ -68,8 +68,32 @@ __device__ __forceinline__ int axis_of(uint64_t axis_end, int f) {
 // 64 registers, so that 32 warps an SM have loads in flight: 33 us for 7742 tokens of 24 + 8 heads
 // (4.8 TB/s); 80 registers 38 us, reading further ahead in each warp instead 40 to 57 us.
 // `split` warps share a token (small batches have too few tokens to fill the GPU).
+// With codes, whose arithmetic takes the registers of loads ahead, heads come through shared memory kRaAhead ahead (each lane
+// copies what it will read): 7742 tokens of 24 + 8 heads and their way back 60 us with registers, 51 so (191 MB).
+constexpr int kRaAhead = 3;
+struct RaRing {
+  uint4 piece[kRaThreads / 32][kRaAhead][2][32];
+};
+__device__ __forceinline__ void ra_copy(uint4 (*stage)[32], int lane, const void* lo, const void* hi,
+                                        bool live) {
+  if (live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&stage[0][lane])), "l"(lo)
+                 : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&stage[1][lane])), "l"(hi)
+                 : "memory");
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void ra_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 template <typename T, typename Code>
-__global__ void __launch_bounds__(kRaThreads, std::is_void_v<Code> ? 4 : 3) rope_axes_kernel(const RopeAxesArgs a, int split) {
+__global__ void __launch_bounds__(kRaThreads, std::is_void_v<Code> ? 4 : 3)
+    rope_axes_kernel(const RopeAxesArgs a, int split) {
+  constexpr bool kCode = !std::is_void_v<Code>;
+  __shared__ std::conditional_t<kCode, RaRing, char> ring;
   grid_dep_wait();
   grid_dep_launch();
   const int lane = threadIdx.x & 31;
@@ -93,7 +117,13 @@ __global__ void __launch_bounds__(kRaThreads, std::is_void_v<Code> ? 4 : 3) rope
     const T* x = static_cast<const T*>(a.qkv) + (int64_t)t * a.xs + c * 8;
     const int h0 = part * 4 + sub, step = split * 4;
     uint4 lo_next = make_uint4(0, 0, 0, 0), hi_next = lo_next;
-    if (h0 < heads) {
+    if constexpr (kCode) {
+      ra_wait<0>();  // (a token that was left out may have left copies)
+#pragma unroll
+      for (int i = 0; i < kRaAhead; ++i)
+        ra_copy(ring.piece[threadIdx.x >> 5][i], lane, x + (h0 + i * step) * 128,
+                x + (h0 + i * step) * 128 + 64, h0 + i * step < heads);
+    } else if (h0 < heads) {
       lo_next = *reinterpret_cast<const uint4*>(x + h0 * 128);
       hi_next = *reinterpret_cast<const uint4*>(x + h0 * 128 + 64);
     }
@@ -141,14 +171,23 @@ __global__ void __launch_bounds__(kRaThreads, std::is_void_v<Code> ? 4 : 3) rope
       if (lane == 0) set_error(a.err, FI_DEVERR_CONTEXT_LEN);
       continue;
     }
+    int stage = 0;
     for (int h = h0; h < heads; h += step) {
-      const uint4 lo_raw = lo_next, hi_raw = hi_next;
-      if (h + step < heads) {
+      uint4 lo_raw = lo_next, hi_raw = hi_next;
+      if constexpr (kCode) {
+        uint4(*piece)[32] = ring.piece[threadIdx.x >> 5][stage];
+        ra_wait<kRaAhead - 1>();
+        lo_raw = piece[0][lane];
+        hi_raw = piece[1][lane];
+        const int to = h + kRaAhead * step;
+        ra_copy(piece, lane, x + to * 128, x + to * 128 + 64, to < heads);
+        stage = (stage + 1) % kRaAhead;
+      } else if (h + step < heads) {
         lo_next = *reinterpret_cast<const uint4*>(x + (h + step) * 128);
         hi_next = *reinterpret_cast<const uint4*>(x + (h + step) * 128 + 64);
       }
       uint4 lo_out = lo_raw, hi_out = hi_raw;
-      if constexpr (!std::is_void_v<Code>) {
+      if constexpr (kCode) {
         if (h >= a.nq) {
           if (!store) continue;
           const bool is_v = h >= a.nq + a.nkv;
@@ -212,6 +251,7 @@ __global__ void __launch_bounds__(kRaThreads, std::is_void_v<Code> ? 4 : 3) rope
       *reinterpret_cast<uint4*>(dst + 64 + c * 8) = hi_out;
     }
   }
+  if constexpr (kCode) ra_wait<0>();
 }
 
 // Both entry points: `cache_dtype` is that of the cache, `dtype` again where it has no scales.
