@@ -1,5 +1,5 @@
-// Attention of a chunk of new tokens over the paged KV cache (chunked prefill, verification
-// of drafted tokens, single tokens, and batches that mix them), on sm_100a tensor cores.
+// Attention of new tokens over the paged KV cache (chunked prefill, verification of drafted tokens and
+// trees of them, single tokens, and batches that mix them), on sm_100a tensor cores.
 //
 //   o_i = sum_j exp(s_ij - lse_i) v_j,  lse_i = log sum_j exp(s_ij)   (j over visible keys;
 //   the batch, visibility and score are described in chunk_common.cuh; a token that sees
@@ -34,6 +34,16 @@
 //   the 1.39 GHz that the power cap leaves. 4225 over 2000: 215 us, 992 TFLOP/s (for seconds 250, at
 //   1.69 GHz). Single tokens are bound by HBM: 64 over 4000 each, 178 us, 5.9 TB/s; one over 512 by
 //   its two launches, 12.3 us.
+// * Trees (kTree): a token sees the cached tokens before the new ones and, of the new ones, those of its bit mask; only
+//   tiles that hold new tokens read masks. New tokens of at most two row tiles are split evenly over both, and a unit
+//   with rows for one tile only is taken by both warpgroups, alternate key tiles each, merged through tensor
+//   memory at its end (16 trees of 9 to 33 tokens over 500 to 4000, scores capped: 99 us with one warpgroup idle,
+//   84 so; 8 of 50 to 85 tokens over 20000 to 32000: 366 us uneven, 349 even).
+// * Pages of 8-bit codes (Code): TMA brings a tile's codes into the half of its place that they fill, and the softmax
+//   warpgroups spread them to 16 bits in place while they would wait for the first product (in warps of their
+//   own, two or four, 408 and 426 us for the 8 trees above; 349 so, 212 with 16-bit pages). K's scales multiply scores
+//   in fp32. V's go onto P where its type has fp32's range (bf16), else onto the spread codes. Spreading and
+//   softmax, 6600 cycles a tile, bound it.
 // * Slots behind a sequence's last token may hold anything: their scores are replaced by
 //   -inf, and their V rows are zeroed in shared memory before the product (0 * NaN is NaN).
 #include <float.h>
@@ -942,7 +952,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
               set_error(p.err, FI_DEVERR_BAD_BLOCK);
           if (g >= kCkStages && !(ok = mbar_wait(&bars->k_empty[s], par, p.err))) break;
           uint8_t* dk = sK + s * kChunkTileBytes;
-          if constexpr (kCode) {  // codes into the tile's first half; the code warps spread them out
+          if constexpr (kCode) {  // codes into the tile's first half; the softmax warpgroups spread them out
             mbar_arrive_expect_tx(&bars->kc_full[s], kChunkHalf);
             for (int i = 0; i < 2; ++i)
               tma_load_4d(dk + i * kChunkHalf / 2, &tm_k, &bars->kc_full[s], 0, u.hk, 0, ph[i]);
@@ -1525,10 +1535,10 @@ static int launch_main(const CUtensorMap& tq, const CUtensorMap& tk, const CUten
       return cudaErrorInvalidConfiguration;
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCkSmemBytes);
   });
-  if (e != cudaSuccess) return cuda_fail(e, "fi_paged_chunk: kernel set-up");
+  if (e != cudaSuccess) return cuda_fail(e, "paged attention: kernel set-up");
   e = launch_pdl(kernel, dim3((unsigned)sm_count()), dim3(kCkThreads), kCkSmemBytes, st, tq,
                  tk, tv, p);
-  return e == cudaSuccess ? FI_OK : cuda_fail(e, "fi_paged_chunk: launch");
+  return e == cudaSuccess ? FI_OK : cuda_fail(e, "paged attention: launch");
 }
 
 template <typename T, bool kNarrow>
@@ -1576,7 +1586,7 @@ static int launch_chunk(const CUtensorMap& tq_n, const CUtensorMap& tq_w, const 
   const cudaError_t e =
       launch_pdl(chunk_combine_kernel<T>, dim3((unsigned)sm_count(), (unsigned)parts), dim3(256), 0,
                  st, first, narrow ? *narrow : first);
-  return e == cudaSuccess ? FI_OK : cuda_fail(e, "fi_paged_chunk: combine launch");
+  return e == cudaSuccess ? FI_OK : cuda_fail(e, "paged attention: combine launch");
 }
 
 static size_t ck_align(size_t n) { return (n + 255) / 256 * 256; }
