@@ -1667,9 +1667,14 @@ static int paged_chunk(const char* what, const void* q, const void* k_cache, con
     for (int rows = 16; rows >= 8; rows /= 2)
       if (total_tokens <= batch * (rows / p.b.group)) unit_rows = rows;
   const int64_t per_unit = unit_rows / p.b.group;
-  const bool use_narrow = per_unit > 0 && (batch > 1 || total_tokens <= per_unit);
   const bool use_wide =
       per_unit == 0 || total_tokens > batch * per_unit || total_tokens - batch >= kCkManyNew;
+  // Trees of like sizes (the mask's words bound the largest) are the wide kernel's with the few small ones among
+  // them, as a second kernel costs some 20 us however little it has to do: 16 trees of 9 to 33 tokens over 500 to 4000, one
+  // of few rows, 84 us with both kernels and 58 with one (int8 pages 138 and 115), 16 of 4 and 16 of 40 over 4000, 132
+  // and 111 (240 and 262); but 32 single tokens and 8 trees of 80 over 3000, 136 and 158 (237 and 350).
+  const bool alike = extra.tree && extra.words * 32 * batch <= 5 * total_tokens;
+  const bool use_narrow = per_unit > 0 && (batch > 1 || total_tokens <= per_unit) && !(use_wide && alike);
   const int64_t unit_tokens = use_wide ? 2 * p.b.tile_tokens : per_unit;
   if (batch > kCkMaxBatch ||
       (total_tokens + unit_tokens - 1) / unit_tokens + batch > kCkMaxUnits)
