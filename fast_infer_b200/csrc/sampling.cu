@@ -11,13 +11,22 @@
 //   (in fp64: 2^(n/32) from a table times a polynomial) and added as integers: any order gives the
 //   same sum, on every run and for every split of the row. A token is the one that 64-bit arithmetic
 //   finds, but for a boundary within 1e-11 of u.
-// * A cluster of up to 8 CTAs holds a row in shared memory, read once. The cut is found by
-//   histograms over 512 bins, first of M - x, then of the bits of x within the bin that holds it, until
-//   the bin is one value; bins add integers by shared-memory atomics (three 15- or 16-bit limbs, so
-//   that no sum of a CTA's values overflows 32 bits) and are joined through distributed
-//   shared memory.
+// * 16-bit logits are counted by value: a bin for each of the values within 16 octaves (bf16; 8 of fp16) below M, and
+//   below 0 as many above the least with a weight; what lies between, near 0, is one bin whose members are weighed one by
+//   one. Weights are then worked out once a value, and cuts found by running sums over bins. A CTA, or a cluster of up
+//   to 8, takes a row, as many as find room together; counts are held for each part of a slice, so that the part that
+//   holds the target is known from them, and only its tokens are weighed, as far as the target. The row is read twice
+//   more from L2 rather than held in shared memory, so that two CTAs find room on an SM.
+// * 32-bit logits: a cluster holds a row in shared memory, read once. The cut is found by histograms over 512 bins, first
+//   of M - x, then of the bits of x within the bin that holds it, until the bin is one value; bins add integers by
+//   shared-memory atomics (three 15-bit limbs, so that no sum of a CTA's values overflows 32 bits) and are joined
+//   through distributed shared memory. Where top_k leaves few tokens, one CTA gathers and finishes them. 16-bit rows
+//   whose cut lies in the bin near 0 come this way too.
 // * The last pass adds kept weights in index order, 256 tokens a warp at a time; the 256 that hold
 //   the target are looked at again by one warp.
+// * 253 rows of 128256: bf16 72 us (65 MB, 10 at a copy's rate), fp16 137, fp32 560. Counting bounds bf16: 13
+//   instructions and a shared-memory atomic a token, 44000 cycles of the 98000 of an SM's two rows, then the last pass and the
+//   chain of small steps. One row: fp32 with top_k 15.9 us, bf16 19.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -1476,7 +1485,8 @@ extern "C" int fi_sample_tokens(const void* logits, const float* u, const float*
   if (reinterpret_cast<uintptr_t>(logits) % size != 0)
     return fail(FI_ERR_ALIGNMENT, "fi_sample_tokens: logits not aligned to their type");
   // 32-bit logits: as few CTAs a row as hold it at 16384 tokens each (two CTAs an SM), more where there are too few rows for
-  // two CTAs an SM. 16-bit ones: as many as find room at the same time, two an SM; the slice in parts.
+  // two CTAs an SM. 16-bit ones: as many as find room at the same time, two an SM (253 rows of 128256 bf16: 72 us, with
+  // two CTAs a row 90; 64 rows: four 37, eight 61), the slice in parts (253 rows: in one part 119 us).
   int ctas = 1, parts = 1;
   int64_t part = 0;
   const int64_t room = 2 * sm_count();
