@@ -111,7 +111,7 @@ struct Slice {
   }
   // eight 16-bit values
   __device__ __forceinline__ uint4 raw8(int at) const {
-    if (at >= lo && at + 8 <= hi) return __ldg(reinterpret_cast<const uint4*>(p + at));
+    if (at >= lo && at + 8 <= hi) return *reinterpret_cast<const uint4*>(p + at);
     return edge(p, lo, hi, at);
   }
   // eight values, -0 as 0
@@ -840,7 +840,7 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_kernel(const SampleArgs 
       uint4 v[kBatch];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j)
-        if (i0 + j * kSaThreads < vecs) v[j] = __ldg(gv + i0 + j * kSaThreads);
+        if (i0 + j * kSaThreads < vecs) v[j] = gv[i0 + j * kSaThreads];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
         const int i = i0 + j * kSaThreads;

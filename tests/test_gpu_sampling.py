@@ -171,3 +171,26 @@ def test_same_token_on_every_run_stream_and_replay(cuda_device):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(got, want2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", [(155, 131064), (150, 131072), (149, 99991)])
+def test_long_slices(cuda_device, dtype, rows, vocab):
+    """As many tokens a CTA as there can be, in several parts, with and without ties across them."""
+    x, u = draw(cuda_device, rows, vocab, dtype, seed=rows)
+    x[1::3] = (x[1::3].float() * 2).round().to(dtype) / 2
+    x[2::3] = (x[2::3].float() / 4).round().to(dtype)
+    check(x, u, *(np.resize(np.array(SETTINGS), (rows, 4)).T))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [5, 150])
+def test_many_values_near_zero(cuda_device, dtype, rows):
+    """Most logits within many octaves around 0, some of them 0: where the cut lies among them and where it does not."""
+    g = torch.Generator(device=cuda_device).manual_seed(rows)
+    vocab = 60001
+    x = 1e-4 * torch.randn(rows, vocab, generator=g, device=cuda_device)
+    x[:, ::50] = 0
+    x[:, 7::2000] = 8 + torch.randn(rows, x[:, 7::2000].shape[1], generator=g, device=cuda_device)
+    x[1::2, 5::9] -= 3
+    check(x.to(dtype), torch.rand(rows, generator=g, device=cuda_device), *(np.resize(np.array(SETTINGS), (rows, 4)).T))
