@@ -45,7 +45,8 @@ static EncodeTiledFn get_encode_fn() {
 
 int encode_tiled(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t rank, const void* base,
                  const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
-                 CUtensorMapSwizzle swizzle, const char* what) {
+                 CUtensorMapSwizzle swizzle, const char* what,
+                 CUtensorMapL2promotion promotion) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) return fail(FI_ERR_CUDA, "%s: cuTensorMapEncodeTiled unavailable", what);
   if (!aligned16(base)) return fail(FI_ERR_ALIGNMENT, "%s: base pointer not 16-byte aligned", what);
@@ -64,7 +65,7 @@ int encode_tiled(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t rank, con
     }
   }
   CUresult r = fn(map, dtype, rank, const_cast<void*>(base), d, s, b, e,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(FI_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
   return FI_OK;

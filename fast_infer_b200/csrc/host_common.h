@@ -24,7 +24,8 @@ int cuda_fail(cudaError_t e, const char* what);
 // Returns FI_OK or FI_ERR_CUDA / FI_ERR_ALIGNMENT with a message.
 int encode_tiled(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t rank, const void* base,
                  const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
-                 CUtensorMapSwizzle swizzle, const char* what);
+                 CUtensorMapSwizzle swizzle, const char* what,
+                 CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 
 // Multiprocessor count of the current device (cached per device, thread-safe).
 int sm_count();
