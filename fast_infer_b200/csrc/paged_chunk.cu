@@ -38,11 +38,11 @@
 //   tiles that hold new tokens read masks. New tokens of at most two row tiles are split evenly over both, and a unit
 //   with rows for one tile only is taken by both warpgroups, alternate key tiles each, merged through tensor
 //   memory at its end (one warpgroup idle instead: 16 trees of 9 to 33 tokens over 500 to 4000, scores capped, 15 us
-//   more; uneven tiles: 8 of 50 to 85 tokens over 20000 to 32000, 17 us more). The 16 take 59 us (169 MB, 25 at a copy's
-//   rate), bound by the chain of a step and a start of 15 us; the 8 over codes take 343 us.
+//   more; uneven tiles: 8 of 50 to 85 tokens over 20000 to 32000, 17 us more). The 16 take 59 us (178 MB, 27 at a copy's
+//   rate), bound by the chain of a step and a start of 15 us; the 8 over codes take 341 us.
 // * Pages of 8-bit codes (Code): TMA brings a tile's codes into the half of its place that they fill, and the softmax
 //   warpgroups spread them to 16 bits in place while they would wait for the first product (in warps of their
-//   own, two or four, 42 and 60 us more for the 8 trees above; with 16-bit pages they take 212). K's scales multiply scores
+//   own, two or four, 40 to 60 us more for the 8 trees above; with 16-bit pages they take 212). K's scales multiply scores
 //   in fp32. V's go onto P where its type has fp32's range (bf16), else onto the spread codes. Spreading and
 //   softmax, 6600 cycles a tile, bound it.
 // * Slots behind a sequence's last token may hold anything: their scores are replaced by
