@@ -24,7 +24,7 @@
 //   whose cut lies in the bin near 0 come this way too.
 // * The last pass adds kept weights in index order, 256 tokens a warp at a time; the 256 that hold
 //   the target are looked at again by one warp.
-// * 253 rows of 128256: bf16 72 us (65 MB, 10 at a copy's rate), fp16 137, fp32 560. Counting bounds bf16: 13
+// * 253 rows of 128256: bf16 72 us (65 MB, 10 at a copy's rate), fp16 137, fp32 374. Counting bounds bf16: 13
 //   instructions and a shared-memory atomic a token, 44000 cycles of the 98000 of an SM's two rows, then the last pass and the
 //   chain of small steps. One row: fp32 with top_k 15.9 us, bf16 19.
 #include <cooperative_groups.h>
@@ -1484,9 +1484,10 @@ extern "C" int fi_sample_tokens(const void* logits, const float* u, const float*
   const int size = dtype == FI_DTYPE_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(logits) % size != 0)
     return fail(FI_ERR_ALIGNMENT, "fi_sample_tokens: logits not aligned to their type");
-  // 32-bit logits: as few CTAs a row as hold it at 16384 tokens each (two CTAs an SM), more where there are too few rows for
-  // two CTAs an SM. 16-bit ones: as many as find room at the same time, two an SM (253 rows of 128256 bf16: 72 us, with
-  // two CTAs a row 90; 64 rows: four 37, eight 61), the slice in parts (253 rows: in one part 119 us).
+  // As many CTAs a row as find room at the same time, two an SM, and as its tokens need. 32-bit logits: 16384 tokens each
+  // (two CTAs an SM), but 32768 rather than eight CTAs (253 rows of 128256: four 374 us, eight 567; 64 rows 120 and 176; of
+  // 32000, 1000 rows: two 261, one 293). 16-bit ones (253 rows of 128256 bf16: 72 us, with
+  // two CTAs a row 90; 64 rows: four 37, eight 61) count their slice in parts (253 rows: in one 119 us).
   int ctas = 1, parts = 1;
   int64_t part = 0;
   const int64_t room = 2 * sm_count();
@@ -1501,10 +1502,9 @@ extern "C" int fi_sample_tokens(const void* logits, const float* u, const float*
   };
   split();
   while (ctas < kSaMaxCluster) {
-    const int64_t most = size == 4 ? kSaRows32 / 2 : kSaMaxTokens;
+    const int64_t most = size == 4 ? kSaRows32 / (ctas < 4 ? 2 : 1) : kSaMaxTokens;
     const bool needs = (parts * part < vocab ? parts * part : vocab) > most;
-    const bool wants = (int64_t)ctas * kSaRound < vocab &&
-                       (size == 4 ? rows * ctas < room : rows * ctas * 2 <= room);
+    const bool wants = (int64_t)ctas * kSaRound < vocab && rows * ctas * 2 <= room;
     if (!needs && !wants) break;
     ctas *= 2;
     split();
