@@ -26,7 +26,7 @@
 //   the target are looked at again by one warp.
 // * 253 rows of 128256: bf16 72 us (65 MB, 10 at a copy's rate), fp16 137, fp32 374. Counting bounds bf16: 13
 //   instructions and a shared-memory atomic a token, 44000 cycles of the 98000 of an SM's two rows, then the last pass and the
-//   chain of small steps. One row: fp32 with top_k 15.9 us, bf16 19.
+//   chain of small steps. One row: fp32 with top_k 15.9 us, with top_p alone 48, bf16 19.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
