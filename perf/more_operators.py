@@ -270,7 +270,6 @@ def prepare(case, seed):
     new, ctx = _sizes(case)
     tokens = int(new.sum())
     st["cu"], st["ctx"] = _int32(np.concatenate([[0], np.cumsum(new)])), _int32(ctx)
-    st["max_new"] = int(new.max())
     if case["op"] == "tree":
         # as _parents() has them, but from the seed; a few nodes are roots as well, that is other first tokens
         node = _int32(np.concatenate([np.arange(n) for n in new]))
@@ -519,7 +518,7 @@ def _own(st, case):
                             st["ctx"], st["qkv"].shape[0], dtype=st["qkv"].dtype))
     if case["op"] == "tree":
         from fast_infer_b200.kernels.drafting import draft_tree
-        return draft_tree(st["parents"], st["cu"], st["max_new"], window=case["window"])
+        return draft_tree(st["parents"], st["cu"], int(_sizes(case)[0].max()), window=case["window"])
     if case["op"] == "attend":
         from fast_infer_b200.kernels.attention import paged_tree_attention
         return paged_tree_attention(st["q"], st["k_cache"], st["v_cache"], st["table"], PAGE, st["cu"], st["ctx"],
