@@ -64,7 +64,8 @@ __global__ void __launch_bounds__(kDrThreads)
 }
 
 // Acceptance. A warp per sequence walks from node 0: from an accepted node to its first child whose
-// token is the one sampled after the node. Children have greater numbers, so one pass over the nodes,
+// token is the one sampled after the node; a negative one is no token (a row that could not be sampled gives -1) and ends
+// the walk. Children have greater numbers, so one pass over the nodes,
 // 32 at a time in registers, finds the whole path. Bound by the launch (26 nodes 1.4 us, 48 trees of 20 to 64 nodes 2.3).
 __global__ void __launch_bounds__(kDrThreads)
     accept_kernel(const int32_t* tokens, const int32_t* sampled, const int32_t* parents,
@@ -89,7 +90,7 @@ __global__ void __launch_bounds__(kDrThreads)
       count = 1;
     }
     while (true) {
-      const uint32_t hit = __ballot_sync(0xffffffffu, live && i > cur && par == cur && tok == want);
+      const uint32_t hit = __ballot_sync(0xffffffffu, live && want >= 0 && i > cur && par == cur && tok == want);
       if (hit == 0) break;
       const int at = __ffs((int)hit) - 1;
       cur = base + at;

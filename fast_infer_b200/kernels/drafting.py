@@ -75,7 +75,9 @@ def accept_drafts(tokens: torch.Tensor, sampled: torch.Tensor, parents: torch.Te
 
     tokens, sampled, parents: int32 [total_tokens], packed by cu_seqlens: each node's token, the
     token that the model samples after it, and its parent (as in ``draft_tree``). Sampling after
-    every node and accepting by equality leaves the distribution that of sampling token by token.
+    every node and accepting by equality leaves the distribution that of sampling token by token. A
+    negative ``sampled`` (``sample_tokens`` gives -1 for a row that it cannot sample) ends the walk,
+    whatever the drafts hold.
     Returns (path, counts, next_tokens): int32 [total_tokens], entry cu_seqlens[b] + d the number of
     the d-th accepted node, ascending, -1 past the last; int32 [batch], the nodes accepted; int32
     [batch], the token sampled after the last of them (-1 for a sequence without new tokens).

@@ -439,7 +439,8 @@ int fi_draft_tree(const int32_t* parents, const int32_t* cu_seqlens, int32_t* ma
 
 /*
  * Acceptance of drafted tokens: from node 0 of each sequence (always accepted) to the first child
- * whose token is the one sampled after the node, until there is none. tokens, sampled, parents:
+ * whose token is the one sampled after the node, until there is none. A negative `sampled` (fi_sample_tokens gives
+ * -1 for a row without a token) ends the walk, whatever the drafts hold. tokens, sampled, parents:
  * int32 [total_tokens]; path: int32 [total_tokens], entry cu[b] + d the number of the d-th
  * accepted node, -1 past the last; counts, next_tokens: int32 [batch], how many nodes are accepted
  * and what was sampled after the last (0 and -1 for a sequence without new tokens).
