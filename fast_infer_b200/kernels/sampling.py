@@ -19,6 +19,8 @@ def _per_row(name: str, value, dtype: torch.dtype, rows: int, device: torch.devi
     if value.shape != (rows,) or value.device != device:
         raise ValueError(f"{name} must be a number or a [rows] tensor on the logits' device")
     if value.dtype != dtype:
+        if dtype == torch.int32:
+            value = value.to(torch.int64).clamp(0, MAX_VOCAB)  # (no wrap at 2^32; below 0 is all)
         value = value.to(dtype)
     return value.contiguous(), 0
 
@@ -77,7 +79,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, *, top
         st = _lib.load().fi_sample_tokens(
             x.data_ptr(), u.data_ptr(), *(None if r is None else r.data_ptr()
                                           for r in (t_rows, k_rows, p_rows, m_rows)),
-            float(t), int(k), float(p), float(m), out.data_ptr(), rows, vocab,
+            float(t), min(int(k), MAX_VOCAB), float(p), float(m), out.data_ptr(), rows, vocab,
             x.stride(0) if rows > 1 else vocab, _LOGITS[x.dtype], stream_of(device))
         _lib.check(st, "sample_tokens")
     return out
