@@ -43,8 +43,8 @@
 // * Pages of 8-bit codes (Code): TMA brings a tile's codes into the half of its place that they fill, and the softmax
 //   warpgroups spread them to 16 bits in place while they would wait for the first product (in warps of their
 //   own, two or four, 40 to 60 us more for the 8 trees above; with 16-bit pages they take 212). K's scales multiply scores
-//   in fp32. V's go onto P where its type has fp32's range (bf16), else onto the spread codes. Spreading and
-//   softmax, 6600 cycles a tile, bound it.
+//   in fp32, V's go onto P in fp32; for fp16, which lacks fp32's range, the softmax then runs relative to a maximum of
+//   score + log2 of V's scale (ck_reference). Spreading and softmax, 6600 cycles a tile, bound it.
 // * Slots behind a sequence's last token may hold anything: their scores are replaced by
 //   -inf, and their V rows are zeroed in shared memory before the product (0 * NaN is NaN).
 #include <float.h>
@@ -97,6 +97,7 @@ struct CkBarriers {
   uint64_t kc_full[kCkStages], vc_full[kCkStages];  // codes have arrived
   alignas(16) float k_scale[kCkScaleSlots][kChunkTile];
   alignas(16) float v_scale[kCkScaleSlots][kChunkTile];
+  alignas(16) float v_top[kCkScaleSlots][4];  // log2 of the greatest, of 32 each
   uint64_t merge;  // both softmax warpgroups, in a transposed unit
   uint32_t tmem_base;
   // transposed units, per warpgroup: rows' max, partial maxima / sums, scale, slope, token
@@ -351,8 +352,8 @@ __device__ __forceinline__ void score_form8(const uint32_t* raw, float* s, const
 // operands: half a step (2^-12 .. 2^-11, bf16 2^-9 .. 2^-8) of each p, which adds to the output's own
 // rounding: 3.0e-4 in place of 2.1e-4 (root mean square, relative; bf16 2.3e-3 and 1.7e-3). P as the
 // sum of two such values would take the product twice.
-// With `v_scale`, P takes the scales of V's rows (and the sum does not).
-template <typename T, bool kCode, bool kScaled>
+// Over codes P takes the scales of V's rows (and the sum does not).
+template <typename T, bool kCode>
 __device__ __forceinline__ float ck_exp(uint32_t* sr, float sl2, float mref, const float* v_scale) {
   const uint64_t sc2 = f32x2(sl2, sl2), nm2 = f32x2(-mref, -mref);
   uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
@@ -361,7 +362,7 @@ __device__ __forceinline__ float ck_exp(uint32_t* sr, float sl2, float mref, con
 #pragma unroll
   for (int c = 0; c < kChunkTile; c += 4) {
     ulonglong2 f = make_ulonglong2(0, 0);
-    if constexpr (kScaled) f = *reinterpret_cast<const ulonglong2*>(v_scale + c);
+    if constexpr (kCode) f = *reinterpret_cast<const ulonglong2*>(v_scale + c);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int d = c + 2 * i;
@@ -378,7 +379,7 @@ __device__ __forceinline__ float ck_exp(uint32_t* sr, float sl2, float mref, con
       }
       uint64_t pp = f32x2(p0, p1);
       sum2[(d >> 1) & 3] = add_f32x2(sum2[(d >> 1) & 3], pp);
-      if constexpr (kScaled) f32x2_split(mul_f32x2(pp, i ? f.y : f.x), p0, p1);
+      if constexpr (kCode) f32x2_split(mul_f32x2(pp, i ? f.y : f.x), p0, p1);
       sr[d >> 1] = Half16<T>::pack(p0, p1);
     }
   }
@@ -682,42 +683,72 @@ __device__ __forceinline__ void scale_columns(uint32_t* sr, const float* scale) 
   }
 }
 
-// 16 codes as 16-bit values of type T: as they are (exact), or times a scale in fp32, rounded once.
-template <typename T, typename Code, bool kScaled>
-__device__ __forceinline__ void spread16(const uint4& raw, float scale, uint32_t* out) {
+// Codes under fp16: P times V's scales does not go into 16 bits as it is (a scale may be 1e-30 or 1e30), nor do V's codes
+// times them. So weights are 2^(s - m') with m' a running maximum of s + log2(vs), less 5, in the place of the scores'
+// maximum, for O and the sum alike. It moves where a bound of s + log2(vs), the row's greatest score with the tile's greatest
+// scale, is past m' + 15: P is below 2^15, and what is 2^-19 of a row's greatest and more is rounded by half a step of its
+// own (from 2^0 on, weights of 2^-14 would lose bits: with scales far apart a good part of the keys). m' is at least the
+// scores' maximum less 80, so that weights are finite, for rows of zeros may hold all of them; what a scale of 2^-80 leaves
+// is 2^-56 of fp16's least value.
+// Here: m' for a tile of scores in tensor memory (times `k_scale`, if they are not yet), from `m` so far, in two passes over
+// it, for a unit's first tile and the few where m' may move. 8 scores at a time keep its code short: it is seldom in the
+// instruction caches (8 trees of 50 to 85 tokens over 20 to 32 k, int8 under fp16: with 32 at a time 491 us, with 8 407; with
+// 5 in place of 8 off the maximum, so that it moves less often, 361).
+template <typename T>
+constexpr bool kCkRunScale = std::is_same_v<T, __half>;
+constexpr float kCkRunTop = 15.f, kCkRunRoom = 5.f, kCkRunGap = 80.f;
+__device__ __forceinline__ float ck_reference(uint32_t tS, float sl2, const float* k_scale, const float* v_scale,
+                                              float m) {
+  float mx = -INFINITY, top = 0.f;
+#pragma unroll 1
+  for (int i = 0; i < 2 * kChunkTile; i += 8) {
+    const int cc = i % kChunkTile;
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    uint32_t sr[8];
+    tmem_ld8(tS + cc, sr);
+    tmem_wait_ld();
+    reg_fence<8>(sr);
+    if (k_scale) scale_columns<8>(sr, k_scale + cc);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const float s = __uint_as_float(sr[c]) * sl2;
+      if (i < kChunkTile) mx = fmaxf(mx, s);
+      else top = fmaxf(top, fast_exp2(s - ref) * v_scale[cc + c]);
+    }
+  }
+  return fmax3f(m, mx + (__log2f(top) - kCkRunRoom), mx - kCkRunGap);
+}
+
+// 16 codes as 16-bit values of type T (exact).
+template <typename T, typename Code>
+__device__ __forceinline__ void spread16(const uint4& raw, uint32_t* out) {
   const uint32_t r[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint32_t h[2];
-    if constexpr (!kScaled && std::is_same_v<T, __nv_bfloat16> && std::is_same_v<Code, CodeI8>) {
+    if constexpr (std::is_same_v<T, __nv_bfloat16> && std::is_same_v<Code, CodeI8>) {
       CodeI8::decode4_bf16(r[i], out[2 * i], out[2 * i + 1]);
       continue;
     }
     Code::decode4(r[i], h[0], h[1]);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      if constexpr (!kScaled && std::is_same_v<T, __half>) {
+      if constexpr (std::is_same_v<T, __half>) {
         out[2 * i + j] = h[j];
       } else {
-        float2 f = __half22float2(*reinterpret_cast<__half2*>(&h[j]));
-        if (kScaled) f.x *= scale, f.y *= scale;
+        const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h[j]));
         out[2 * i + j] = Half16<T>::pack(f.x, f.y);
       }
     }
   }
 }
 
-// Where V's scale is applied: to P in fp32, before it is rounded, where T has fp32's range (bf16); else (fp16) to V's
-// codes, rounded once to T: half a step of 2^-12 to 2^-11 more.
-template <typename T>
-constexpr bool kCkScaleP = std::is_same_v<T, __nv_bfloat16>;
-
 // Between TMA and the tensor core: a warpgroup spreads the codes of a tile (128 keys x 128 bytes, 128-byte swizzle),
 // which lie in the first half of the tile's 16-bit place, a row where its first 64 values will be, so that the 8
 // lanes of a row read it and then write over it. Lanes are given rows r and r ^ 5 such that neither the reads
-// nor the writes of 8 lanes meet a bank twice. `scale` is that of row 32 * quarter + lane, for kScaled.
-template <typename T, typename Code, bool kScaled>
-__device__ __forceinline__ void spread_tile(uint8_t* tile, int live, int quarter, float scale) {
+// nor the writes of 8 lanes meet a bank twice.
+template <typename T, typename Code>
+__device__ __forceinline__ void spread_tile(uint8_t* tile, int live, int quarter) {
   const int lane = threadIdx.x & 31;
   const int q = lane & 3, flip = (lane >> 2) & 1 ? 5 : 0, column = (lane >> 3) & 1, pair = lane >> 4;
   const int piece = column * 4 + q;
@@ -735,8 +766,7 @@ __device__ __forceinline__ void spread_tile(uint8_t* tile, int live, int quarter
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t v[8];
-      spread16<T, Code, kScaled>(raw[i],
-                                 kScaled ? __shfl_sync(0xffffffffu, scale, row[i] & 31) : 1.f, v);
+      spread16<T, Code>(raw[i], v);
       uint8_t* to = tile + column * kChunkHalf + row[i] * 128;
       *reinterpret_cast<uint4*>(to + (((2 * q) ^ (row[i] & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
       *reinterpret_cast<uint4*>(to + (((2 * q + 1) ^ (row[i] & 7)) << 4)) =
@@ -751,8 +781,7 @@ __device__ __forceinline__ void spread_tile(uint8_t* tile, int live, int quarter
 // tile j + 2 (its stage is free since S of tile j), the second one V of tile j + 1, and both the first tiles of
 // the next unit before a unit's end. (Warps of their own for it: four cost the softmax its registers,
 // two were slower than the tensor core, 408 us for 8 trees over 20 to 32 k keys.)
-// K keeps its codes, which are exact in T, and scores are scaled in fp32, as lse is an output. A thread looks up
-// the scales of one row. Rows of keys past the context are zero, like those without a page.
+// K and V keep their codes, which are exact in T. A thread of the first one looks up the scales of one row. Rows of keys past the context are zero, like those without a page.
 template <typename T, typename Code>
 struct CodeSpreader {
   const ChunkParams& p;
@@ -774,9 +803,10 @@ struct CodeSpreader {
     const bool held = page != p.b.num_blocks && ck_tile(u, j) * kChunkTile + row < u.keys;
     const int64_t slot = row & (kChunkPage - 1);
     k = v = 0.f;
-    if (held && t == 0) k = p.scale[0][page * p.ss[0][0] + u.hk * p.ss[0][1] + slot * p.ss[0][2]];
-    if (held && (t == 0) == kCkScaleP<T>)
+    if (held && t == 0) {
+      k = p.scale[0][page * p.ss[0][0] + u.hk * p.ss[0][1] + slot * p.ss[0][2]];
       v = p.scale[1][page * p.ss[1][0] + u.hk * p.ss[1][1] + slot * p.ss[1][2]];
+    }
   }
   // Tile j of the unit, whose scales have been looked up.
   template <typename Wait>
@@ -784,14 +814,15 @@ struct CodeSpreader {
     const int s = g % kCkStages;
     if (t == 0) {
       bars->k_scale[g % kCkScaleSlots][row] = k;
-      if (kCkScaleP<T>) bars->v_scale[g % kCkScaleSlots][row] = v;
+      bars->v_scale[g % kCkScaleSlots][row] = v;
+      if constexpr (kCkRunScale<T>) {  // (not negative, so in the order of their bits)
+        const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+        if ((threadIdx.x & 31) == 0) bars->v_top[g % kCkScaleSlots][quarter] = __log2f(top);
+      }
     }
     wait(t ? &bars->vc_full[s] : &bars->kc_full[s], (g / kCkStages) & 1);
     const int live = u.keys - ck_tile(u, j) * kChunkTile;
-    if (kCkScaleP<T> || t == 0)
-      spread_tile<T, Code, false>(tiles + s * kChunkTileBytes, live, quarter, 1.f);
-    else
-      spread_tile<T, Code, true>(tiles + s * kChunkTileBytes, live, quarter, v);
+    spread_tile<T, Code>(tiles + s * kChunkTileBytes, live, quarter);
     if ((threadIdx.x & 31) == 0) mbar_arrive(t ? &bars->v_full[s] : &bars->k_full[s]);
     ++g;
   }
@@ -825,6 +856,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
   CkBarriers* bars = reinterpret_cast<CkBarriers*>(sV + kCkStages * kChunkTileBytes);
 
   constexpr bool kCode = !std::is_void_v<Code>;
+  [[maybe_unused]] constexpr bool kRun = kCode && kCkRunScale<T>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = blockIdx.x;
 
@@ -1285,15 +1317,18 @@ __global__ void __launch_bounds__(kCkThreads, 1)
             tmem_wait_st();
           }
           uint32_t sr[kChunkTile];
-          tmem_ld32(tS + 0, sr + 0);
-          tmem_ld32(tS + 32, sr + 32);
-          tmem_ld32(tS + 64, sr + 64);
-          tmem_ld32(tS + 96, sr + 96);
-          tmem_wait_ld();
-          reg_fence<kChunkTile>(sr);
-          if constexpr (kCode) {
-            if (!(kCap || mask)) scale_columns<kChunkTile>(sr, bars->k_scale[g % kCkScaleSlots]);
-          }
+          auto load = [&]() {
+            tmem_ld32(tS + 0, sr + 0);
+            tmem_ld32(tS + 32, sr + 32);
+            tmem_ld32(tS + 64, sr + 64);
+            tmem_ld32(tS + 96, sr + 96);
+            tmem_wait_ld();
+            reg_fence<kChunkTile>(sr);
+            if constexpr (kCode) {
+              if (!(kCap || mask)) scale_columns<kChunkTile>(sr, bars->k_scale[g % kCkScaleSlots]);
+            }
+          };
+          load();
           float mx8[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -1307,22 +1342,35 @@ __global__ void __launch_bounds__(kCkThreads, 1)
           // NaN where any score is: the whole row is NaN then, whichever columns hold it
           const float mx = fmax_nan(fmax3_nan(mx8[0], mx8[1], mx8[2]),
                                     fmax3_nan(fmax3_nan(mx8[3], mx8[4], mx8[5]), mx8[6], mx8[7]));
-          const float m_new = fmax_nan(m, mx * sl2);
           bool rescale = false;
           float alpha = 1.f;
-          if (j == first) {
-            m = m_new;
-          } else {
-            const bool need = !(m_new <= m + kCkRescale) && m == m;  // (once to NaN; it stays)
-            rescale = __any_sync(0xffffffffu, need);
-            if (need) {
-              alpha = fast_exp2(m - m_new);
-              m = m_new;
+          if constexpr (kRun) {
+            const float4 v4 = *reinterpret_cast<const float4*>(bars->v_top[g % kCkScaleSlots]);
+            const float bound = mx * sl2 + fmaxf(fmax3f(v4.x, v4.y, v4.z) - kCkRunTop, v4.w - kCkRunTop);
+            if (__any_sync(0xffffffffu, live && (bound > m || mx * sl2 > m + kCkRunGap))) {
+              const float to = ck_reference(tS, sl2, kCap || mask ? nullptr : bars->k_scale[g % kCkScaleSlots],
+                                            bars->v_scale[g % kCkScaleSlots], m);
+              alpha = to == m ? 1.f : fast_exp2(m - to);
+              m = to;
               l *= alpha;
+              rescale = j != first;
+              load();
+            }
+          } else {
+            const float m_new = fmax_nan(m, mx * sl2);
+            if (j == first) {
+              m = m_new;
+            } else {
+              const bool need = !(m_new <= m + kCkRescale) && m == m;  // (once to NaN; it stays)
+              rescale = __any_sync(0xffffffffu, need);
+              if (need) {
+                alpha = fast_exp2(m - m_new);
+                m = m_new;
+                l *= alpha;
+              }
             }
           }
-          l += ck_exp<T, kCode, kCode && kCkScaleP<T>>(sr, sl2, m == -INFINITY ? 0.f : m,
-                                                bars->v_scale[g % kCkScaleSlots]);
+          l += ck_exp<T, kCode>(sr, sl2, m == -INFINITY ? 0.f : m, bars->v_scale[g % kCkScaleSlots]);
           tmem_st32(tS + 0, sr);
           tmem_st32(tS + 32, sr + 32);
           if (rescale) {
@@ -1358,6 +1406,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       const bool mine = first < u.j1;
       if (mine) wait(&bars->o_full[t], uc & 1);
       tc_fence_after();
+      if (kRun && l != l) m = l;  // (m' passes NaN scores over)
       bool none = m == -INFINITY;
       float inv = none ? 0.f : 1.f / l, inv1 = 0.f;
       float lse2 = none ? -INFINITY : m + log2f(l);

@@ -1,4 +1,4 @@
-"""paged_tree_attention over 8-bit codes where V's scales are far apart: rows of zeros and subnormal rows that hold most of a
+"""paged_tree_attention over 8-bit codes where scales are far apart or NaN: rows of zeros and subnormal rows that hold most of a
 softmax's weight, and rows past fp16's range. Finite caches give finite outputs, close to the definition in 64 bits,
 whatever the number of rows that share a tile."""
 
@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from fast_infer_b200.kernels.attention import paged_tree_attention
-from tests.test_gpu_paged_tree import check, make
+from tests.test_gpu_paged_tree import check, definition, make, visible
 
 pytestmark = pytest.mark.gpu
 KINDS = ["int8", "e4m3"]
@@ -66,3 +66,73 @@ def test_subnormal_rows_come_first(cuda_device, device_checks, seqs, dtype, kind
                     st["vs"][page] *= 1e-38
         o, _ = check(st, kind, dtype)
         assert torch.isfinite(o).all()
+
+
+def bound(st, dtype, softcap, window):
+    """Exact o, lse, and how far o may be off. Weights times V's scales are rounded to 16 bits relative to a running maximum
+    of theirs, so a key adds half a step of its own or 2^-25 of the greatest p max|v| of the row."""
+    exact, absv, _, lse, err = definition(st, softcap, window)
+    eps = torch.finfo(dtype).eps / 2
+    least = torch.zeros_like(lse)
+    row = 0
+    for b, ((n, c), see) in enumerate(zip(st["seqs"], visible(st, window))):
+        pages = st["table"][b, :-(-c // 64)].long()
+        for h in range(st["q"].shape[1]):
+            kh = h // (st["q"].shape[1] // st["k"].shape[2])
+            k = (st["k"][pages][:, :, kh].double() * st["ks"][pages, kh].double()[..., None]).reshape(-1, 128)[:c]
+            v = (st["v"][pages][:, :, kh].double() * st["vs"][pages, kh].double()[..., None]).reshape(-1, 128)[:c]
+            s = st["q"][row:row + n, h].double() @ k.t() / math.sqrt(128)
+            s = softcap * torch.tanh(s / softcap) if softcap else s
+            p = torch.exp(s.masked_fill(~see.to(s.device), -math.inf) - lse[row:row + n, h, None])
+            least[row:row + n, h] = c * 2.0 ** -25 * (p * v.abs().amax(-1)).amax(-1)
+        row += n
+    tol = (2 * eps * 1.01 + 2 * err[..., None]) * absv + eps * exact.abs() + least[..., None]
+    return exact, lse, tol + (2.0 ** -25 if dtype == torch.float16 else 1e-30), err
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("seqs", SHAPES)
+def test_rows_past_the_range_of_fp16(cuda_device, device_checks, seqs, dtype, kind):
+    """V rows of 1e10 at keys of little weight count for what they are; those of 1e30 at a new token do not show in rows that do
+    not see it."""
+    top = {"int8": 127.0, "e4m3": 448.0}[kind]
+    for softcap, score, size in ((0.0, -20.0, 1e10), (30.0, -27.0, 1e11), (0.0, -9.0, 1e6)):
+        st = aligned(cuda_device, seqs, dtype, kind, seed=23)
+        st["ks"] *= 0.1
+        for b, (n, c) in enumerate(seqs):
+            for slot in {c - n - 1, (c - n) // 3}:
+                page, at = peak(st, kind, b, slot, score)
+                st["vs"][page, :, at] = size / top
+            if n > 2:  # (a sibling's key: no other branch sees it)
+                page, at = place(st, b, c - n + 2)
+                st["vs"][page, :, at] = 1e30
+        exact, exact_lse, tol, err = bound(st, dtype, softcap, 0)
+        o, lse = paged_tree_attention(st["q"], st["k"], st["v"], st["table"], 64, st["cu"], st["ctx"], tree_mask=st["mask"],
+                                      k_scale=st["ks"], v_scale=st["vs"], softcap=softcap, return_lse=True)
+        assert ((lse.double() - exact_lse).abs() <= err + 2.0 ** -22 * exact_lse.abs()).all()
+        ok = exact.abs().amax(-1) < 3e4  # (rows that see the 1e30 are past fp16)
+        assert ok.any(-1).sum() >= len(seqs)
+        far = (o.double() - exact).abs()
+        assert (far <= tol)[ok].all(), (far / tol)[ok].max()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("seqs", [[(16, 640)], [(60, 800)], [(2, 300), (70, 5000)]])
+def test_nan_scores_show_in_the_rows_that_see_them(cuda_device, seqs, dtype, kind):
+    """A NaN scale of a new token's K: NaN in o and lse of the rows that see that key, finite elsewhere."""
+    st = make(cuda_device, seqs, 6, 2, dtype, kind, seed=24, spread=4)
+    row = 0
+    sees = torch.zeros(st["q"].shape[0], dtype=torch.bool)
+    for b, ((n, c), see) in enumerate(zip(seqs, visible(st, 0))):
+        page, at = place(st, b, c - n + n // 2)
+        st["ks"][page, 1, at] = math.nan
+        sees[row:row + n] = see[:, c - n + n // 2]
+        row += n
+    o, lse = paged_tree_attention(st["q"], st["k"], st["v"], st["table"], 64, st["cu"], st["ctx"], tree_mask=st["mask"],
+                                  k_scale=st["ks"], v_scale=st["vs"], return_lse=True)
+    sees = sees.to(cuda_device)
+    assert sees.any() and not sees.all()
+    assert torch.isnan(o[sees][:, 3:]).all() and torch.isnan(lse[sees][:, 3:]).all()
+    assert torch.isfinite(o[~sees]).all() and torch.isfinite(lse[~sees]).all() and torch.isfinite(o[:, :3]).all()
