@@ -59,8 +59,10 @@ namespace fi {
 constexpr int kCkThreads = 384;
 constexpr int kCkRegsSoftmax = 184;  // 2 x 128 x 184 + 128 x 136 = 384 x 168
 constexpr int kCkRegsOther = 136;
-// Scales of a key tile are read after its product is done, that is after its stage may be filled again: the
-// place of tile j is written for tile j + 4 once S of tile j + 2 is complete, which waits for P of tile j + 1.
+// Scales of a key tile are read after its product is done, that is after its stage may be filled again. The place of tile j
+// is written for tile j + 4 once K of that has arrived, so once S of tile j + 2 is complete. S of tile j + 2 is issued
+// after the product with V of tile j (where the warpgroups alternate key tiles; else of tile j + 1), which waits
+// for the weights of tile j, and S of a unit's first tiles after all products of the unit before.
 constexpr int kCkScaleSlots = 4;
 constexpr int kCkStages = 2;
 constexpr int kCkTeardownBar = 15;
@@ -812,6 +814,7 @@ struct CodeSpreader {
   template <typename Wait>
   __device__ __forceinline__ void spread(const CkUnit& u, int j, Wait&& wait) {
     const int s = g % kCkStages;
+    wait(t ? &bars->vc_full[s] : &bars->kc_full[s], (g / kCkStages) & 1);
     if (t == 0) {
       bars->k_scale[g % kCkScaleSlots][row] = k;
       bars->v_scale[g % kCkScaleSlots][row] = v;
@@ -820,7 +823,6 @@ struct CodeSpreader {
         if ((threadIdx.x & 31) == 0) bars->v_top[g % kCkScaleSlots][quarter] = __log2f(top);
       }
     }
-    wait(t ? &bars->vc_full[s] : &bars->kc_full[s], (g / kCkStages) & 1);
     const int live = u.keys - ck_tile(u, j) * kChunkTile;
     spread_tile<T, Code>(tiles + s * kChunkTileBytes, live, quarter);
     if ((threadIdx.x & 31) == 0) mbar_arrive(t ? &bars->v_full[s] : &bars->k_full[s]);
