@@ -7,10 +7,11 @@
 // cut: a value c and how many of the tokens that equal c stay (the lowest indexes). The token is the
 // first index whose running sum of kept w passes u times the whole.
 //
-// * Sums decide between neighbours whose masses lie 1e-6 apart or less, so weights are computed to 2^-45
-//   (in fp64: 2^(n/32) from a table times a polynomial) and added as integers: any order gives the
-//   same sum, on every run and for every split of the row. A token is the one that 64-bit arithmetic
-//   finds, but for a boundary within 1e-11 of u.
+// * Sums decide between neighbours whose masses lie 1e-6 apart or less, so weights are rounded to units of 2^-45
+//   (from fp64: 2^(n/32) from a table times a polynomial) and added as integers: any order gives the same sum, on every run
+//   and for every split of the row. Each is off by half a unit at most, so running sums of n tokens and their shares of the
+//   whole by n 2^-46 (the whole is 1 at least): 3.7e-9 where 262144 equal small weights all err to one side, some 1e-11 or less for
+//   logits that are spread. A token is the one of exact arithmetic but for a boundary that near to u, or to top_p.
 // * 16-bit logits are counted by value: a bin for each of the values within 16 octaves (bf16; 8 of fp16) below M, and
 //   below 0 as many above the least with a weight; what lies between, near 0, is one bin whose members are weighed one by
 //   one. Weights are then worked out once a value, and cuts found by running sums over bins. A CTA, or a cluster of up

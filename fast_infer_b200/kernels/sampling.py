@@ -35,8 +35,9 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, *, top
     logits, ties by index: top_k keeps the first ``top_k`` (0: all), top_p < 1 those of them before
     which the mass is below ``top_p`` times the mass of them all (the first always stays), min_p those
     with ``w >= min_p`` (min_p in [0, 1]). The token is the first index at which the running sum of
-    kept ``w`` is above ``u`` times their whole sum; sums are held to 2^-45. temperature 0 takes the
-    first of the greatest logits.
+    kept ``w`` is above ``u`` times their whole sum. Weights are rounded to whole units of 2^-45 (of the
+    greatest) and added exactly, so shares are off by at most vocab * 2^-46 (3.7e-9 for the largest).
+    temperature 0 takes the first of the greatest logits.
 
     A logit of -inf hides its token. A row that holds NaN or +inf, or nothing above -inf, gives -1.
     Returns int32 [rows] (``out`` if given).

@@ -478,6 +478,7 @@ int fi_keep_accepted(void* k, void* v, float* k_scale, float* v_scale,
  * min_p > 0 those with w >= min_p (in [0, 1]). out = the first index whose running sum of kept w is
  * above u times the sum of all kept w. temperature 0 (or below, or NaN): the first of the greatest
  * logits. -inf hides a token; a row with NaN or +inf, or without a logit above -inf, gives -1.
+ * Weights are rounded to units of 2^-45 and added exactly: shares are off by at most vocab * 2^-46.
  * At most 262144 tokens a row. Deterministic: the same token on every run.
  */
 int fi_sample_tokens(const void* logits, const float* u, const float* temperature,
