@@ -15,9 +15,9 @@
 //   parts of one line as in paged_chunk.cu, and units that several CTAs hold are joined likewise.
 // * Scales stay out of the products: ks multiplies scores in fp32. vs_j cannot multiply codes (fp16) nor
 //   P alone (vs may be 1e-6 or 1e30), so P' = p vs 2^(m - m') carries it, with m' a running maximum
-//   of s + log2(vs): P' is at most 2^8, and the greatest of a row's is at least one at some key. But m' is at least
-//   m - 126, as 2^(m - m') has to be finite: a row of zeros (vs = 0) that holds all the weight, or subnormal ones, leave P'
-//   below that one, and o below what 16 bits hold. A sum of p in 32 bits goes with m, the sum of P' vc with m'.
+//   of s + log2(vs), less 5: a row's greatest P' lies between 2^5 and 2^15, so that what is 2^-19 of it and more keeps all
+//   of fp16's bits. But m' is at least m - 126, as 2^(m - m') has to be finite: a row of zeros (vs = 0) that holds all the
+//   weight, or subnormal ones, leave P' below, and o below what 16 bits hold. A sum of p in 32 bits goes with m, the sum of P' vc with m'.
 // * q of bf16 is brought to fp16 by a power of two per row, exactly but for values 2^-15 and less of
 //   the row's greatest (then to 2^-25 of that). P' is rounded to fp16, half a step of 2^-12 to 2^-11.
 // * 64 single tokens over 3000 to 9000 cached ones, 24 heads over 8 of codes, 811 MB: 152 us, 5.3 TB/s where a copy
@@ -35,7 +35,8 @@ namespace fi {
 constexpr int kPcKeys = 16;                     // keys of a tile that a warp takes: 8 warps have one
 constexpr int kPcPad = 3;                       // steps that a unit's start and end are worth on the line
 constexpr int kPcStageBytes = 2 * kPcKeys * 128 + 2 * kPcKeys * 4;
-constexpr float kPcTop = 256.f;                 // p and P' up to which maxima stay as they are
+constexpr float kPcTop = 32768.f;               // p and P' up to which maxima stay as they are
+constexpr float kPcRoom = 5.f;                  // log2 of what a row's greatest P' is then
 constexpr float kPcGap = 126.f;                 // most that m' lies below m: 2^126 is finite, 2^-126 normal
 static_assert(kPcStageBytes % 16 == 0, "16-byte copies");
 
@@ -437,7 +438,7 @@ __global__ void __launch_bounds__(PcShape<kNT>::kThreads, 1)
             if (!((see >> (g + 8)) & 1u)) sc[n][2 + h] = -INFINITY;
           }
       }
-      // -------------------------------------------------- weights; maxima move where one passes 2^8
+      // ------------------------------------------------- weights; maxima move where one passes 2^15
       uint32_t pb0[kNT], pb1[kNT];
       float ps[kNT][2];
 #pragma unroll 1
@@ -472,7 +473,7 @@ __global__ void __launch_bounds__(PcShape<kNT>::kThreads, 1)
               b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, off));
             }
             a = fmaxf(a, mx[n][h]);
-            b = fmax3f(b, mv[n][h], a - kPcGap);
+            b = fmax3f(b - kPcRoom, mv[n][h], a - kPcGap);
             const float fl = mx[n][h] == -INFINITY ? 0.f : fast_exp2(mx[n][h] - a);
             const float fo = mv[n][h] == -INFINITY ? 0.f : fast_exp2(mv[n][h] - b);
             mx[n][h] = a;

@@ -70,13 +70,16 @@ def test_subnormal_rows_come_first(cuda_device, device_checks, seqs, dtype, kind
 
 def bound(st, dtype, softcap, window):
     """Exact o, lse, and how far o may be off. Weights times V's scales are rounded to 16 bits relative to a running maximum
-    of theirs, so a key adds half a step of its own or 2^-25 of the greatest p max|v| of the row."""
+    of theirs, which lies at 2^5 or above: a key adds half a step of its own or 2^-25 / 2^5 of the row's greatest p max|v|."""
     exact, absv, _, lse, err = definition(st, softcap, window)
     eps = torch.finfo(dtype).eps / 2
     least = torch.zeros_like(lse)
     row = 0
     for b, ((n, c), see) in enumerate(zip(st["seqs"], visible(st, window))):
         pages = st["table"][b, :-(-c // 64)].long()
+        if n == 0 or c == 0:
+            row += n
+            continue
         for h in range(st["q"].shape[1]):
             kh = h // (st["q"].shape[1] // st["k"].shape[2])
             k = (st["k"][pages][:, :, kh].double() * st["ks"][pages, kh].double()[..., None]).reshape(-1, 128)[:c]
@@ -84,10 +87,29 @@ def bound(st, dtype, softcap, window):
             s = st["q"][row:row + n, h].double() @ k.t() / math.sqrt(128)
             s = softcap * torch.tanh(s / softcap) if softcap else s
             p = torch.exp(s.masked_fill(~see.to(s.device), -math.inf) - lse[row:row + n, h, None])
-            least[row:row + n, h] = c * 2.0 ** -25 * (p * v.abs().amax(-1)).amax(-1)
+            least[row:row + n, h] = c * 2.0 ** -30 * (p * v.abs().amax(-1)).amax(-1)
         row += n
     tol = (2 * eps * 1.01 + 2 * err[..., None]) * absv + eps * exact.abs() + least[..., None]
     return exact, lse, tol + (2.0 ** -25 if dtype == torch.float16 else 1e-30), err
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("seqs", SHAPES + [[(1, 4)], [(5, 5)], [(2, 9000)]])
+def test_scales_six_orders_apart(cuda_device, device_checks, seqs, dtype, kind):
+    """V rows up to 10^6 apart in size: where the greatest row's values are 0, the small ones are what counts."""
+    for seed, softcap, window in ((1, 0.0, 0), (2, 30.0, 40)):
+        st = make(cuda_device, seqs, 6, 2, dtype, kind, seed=seed, spread=4, window=window)
+        g = torch.Generator(device=cuda_device).manual_seed(seed)
+        st["vs"] *= 10.0 ** (6 * torch.rand(st["vs"].shape, generator=g, device=cuda_device) - 6)
+        st["v"].view(torch.int8)[torch.rand(st["v"].shape, generator=g, device=cuda_device) < 0.2] = 0
+        exact, exact_lse, tol, err = bound(st, dtype, softcap, window)
+        o, lse = paged_tree_attention(st["q"], st["k"], st["v"], st["table"], 64, st["cu"], st["ctx"], tree_mask=st["mask"],
+                                      depths=st["depths"], k_scale=st["ks"], v_scale=st["vs"], softcap=softcap, window=window,
+                                      return_lse=True)
+        assert ((lse.double() - exact_lse).abs() <= err + 2.0 ** -22 * exact_lse.abs()).all()
+        far = (o.double() - exact).abs()
+        assert (far <= tol).all(), (far / tol).max()
 
 
 @pytest.mark.parametrize("kind", KINDS)
