@@ -39,7 +39,7 @@
 //   with rows for one tile only is taken by both warpgroups, alternate key tiles each, merged through tensor
 //   memory at its end (one warpgroup idle instead: 16 trees of 9 to 33 tokens over 500 to 4000, scores capped, 15 us
 //   more; uneven tiles: 8 of 50 to 85 tokens over 20000 to 32000, 17 us more). The 16 take 59 us (178 MB, 27 at a copy's
-//   rate), bound by the chain of a step and a start of 15 us; the 8 over codes take 341 us.
+//   rate), bound by the chain of a step and a start of 15 us; the 8 over codes take 340 us (fp16 334).
 // * Pages of 8-bit codes (Code): TMA brings a tile's codes into the half of its place that they fill, and the softmax
 //   warpgroups spread them to 16 bits in place while they would wait for the first product (in warps of their
 //   own, two or four, 40 to 60 us more for the 8 trees above; with 16-bit pages they take 212). K's scales multiply scores
@@ -107,6 +107,7 @@ struct CkBarriers {
   alignas(16) float n_neg[2][kCkNarrow];  // -max; FLT_MAX: no score yet, -inf: no such row
   float n_slope[2][kCkNarrow], n_pos[2][kCkNarrow];
   int64_t n_off[kCkNarrow];  // where a row's output goes
+  float twin_mv[4][32];      // m' of the second warpgroup's rows, where both have them
   CkUnit units[kCkSlots];
   uint8_t row_token[kChunkTile], row_head[kChunkTile];  // of a tile's rows
   uint32_t warp_sums[kCkThreads / 32];
@@ -354,9 +355,9 @@ __device__ __forceinline__ void score_form8(const uint32_t* raw, float* s, const
 // operands: half a step (2^-12 .. 2^-11, bf16 2^-9 .. 2^-8) of each p, which adds to the output's own
 // rounding: 3.0e-4 in place of 2.1e-4 (root mean square, relative; bf16 2.3e-3 and 1.7e-3). P as the
 // sum of two such values would take the product twice.
-// Over codes P takes the scales of V's rows (and the sum does not).
-template <typename T, bool kCode>
-__device__ __forceinline__ float ck_exp(uint32_t* sr, float sl2, float mref, const float* v_scale) {
+// Over codes P takes the scales of V's rows (and the sum does not), and with kRun the row's `factor` (see ck_reference).
+template <typename T, bool kCode, bool kRun>
+__device__ __forceinline__ float ck_exp(uint32_t* sr, float sl2, float mref, const float* v_scale, float factor) {
   const uint64_t sc2 = f32x2(sl2, sl2), nm2 = f32x2(-mref, -mref);
   uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
   // (over codes the special function units wait for the issue slots as it is)
@@ -381,6 +382,7 @@ __device__ __forceinline__ float ck_exp(uint32_t* sr, float sl2, float mref, con
       }
       uint64_t pp = f32x2(p0, p1);
       sum2[(d >> 1) & 3] = add_f32x2(sum2[(d >> 1) & 3], pp);
+      if constexpr (kRun) pp = mul_f32x2(pp, f32x2(factor, factor));
       if constexpr (kCode) f32x2_split(mul_f32x2(pp, i ? f.y : f.x), p0, p1);
       sr[d >> 1] = Half16<T>::pack(p0, p1);
     }
@@ -686,19 +688,19 @@ __device__ __forceinline__ void scale_columns(uint32_t* sr, const float* scale) 
 }
 
 // Codes under fp16: P times V's scales does not go into 16 bits as it is (a scale may be 1e-30 or 1e30), nor do V's codes
-// times them. So weights are 2^(s - m') with m' a running maximum of s + log2(vs), less 5, in the place of the scores'
-// maximum, for O and the sum alike. It moves where a bound of s + log2(vs), the row's greatest score with the tile's greatest
-// scale, is past m' + 15: P is below 2^15, and what is 2^-19 of a row's greatest and more is rounded by half a step of its
-// own (from 2^0 on, weights of 2^-14 would lose bits: with scales far apart a good part of the keys). m' is at least the
-// scores' maximum less 80, so that weights are finite, for rows of zeros may hold all of them; what a scale of 2^-80 leaves
-// is 2^-56 of fp16's least value.
+// times them. So P' = p vs 2^(m - m') does, with m' a running maximum of s + log2(vs), less 5; O goes with m', the sum of p
+// with m (m' for both would cost lse two bits). m' moves where a bound of s + log2(vs), the row's greatest score with the
+// tile's greatest scale, is past m' + 15: P' is below 2^15, and what is 2^-19 of a row's greatest and more is rounded by half
+// a step of its own (from 2^0 on, P' of 2^-14 would lose bits: with scales far apart a good part of the keys). m' is
+// at least m - 100, where the factor is finite, for rows of zeros may hold all the weight; what a scale of 2^-100 leaves is
+// 2^-76 of fp16's least value.
 // Here: m' for a tile of scores in tensor memory (times `k_scale`, if they are not yet), from `m` so far, in two passes over
 // it, for a unit's first tile and the few where m' may move. 8 scores at a time keep its code short: it is seldom in the
-// instruction caches (8 trees of 50 to 85 tokens over 20 to 32 k, int8 under fp16: with 32 at a time 491 us, with 8 407; with
-// 5 in place of 8 off the maximum, so that it moves less often, 361).
+// instruction caches (8 trees of 50 to 85 tokens over 20 to 32 k, int8 under fp16, in an earlier form: with 32 at a time
+// 491 us, with 8 407, and 361 where m' lies 5 rather than 8 below the maximum, so that it moves less often).
 template <typename T>
 constexpr bool kCkRunScale = std::is_same_v<T, __half>;
-constexpr float kCkRunTop = 15.f, kCkRunRoom = 5.f, kCkRunGap = 80.f;
+constexpr float kCkRunTop = 15.f, kCkRunRoom = 5.f, kCkRunGap = 100.f;
 __device__ __forceinline__ float ck_reference(uint32_t tS, float sl2, const float* k_scale, const float* v_scale,
                                               float m) {
   float mx = -INFINITY, top = 0.f;
@@ -1258,6 +1260,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       float slope2 = 0.f;
       if (kAlibi && live) slope2 = p.f.slopes[head] * kLog2e;
       float m = -INFINITY, l = 0.f;
+      [[maybe_unused]] float mv = -INFINITY;  // m' of ck_reference
 #pragma unroll 1
       for (int j = first; j < u.j1; j += twin ? 2 : 1, ++sc) {
         g = g0 + j;
@@ -1344,35 +1347,37 @@ __global__ void __launch_bounds__(kCkThreads, 1)
           // NaN where any score is: the whole row is NaN then, whichever columns hold it
           const float mx = fmax_nan(fmax3_nan(mx8[0], mx8[1], mx8[2]),
                                     fmax3_nan(fmax3_nan(mx8[3], mx8[4], mx8[5]), mx8[6], mx8[7]));
+          const float m_new = fmax_nan(m, mx * sl2);
           bool rescale = false;
           float alpha = 1.f;
+          if (j == first) {
+            m = m_new;
+          } else {
+            const bool need = !(m_new <= m + kCkRescale) && m == m;  // (once to NaN; it stays)
+            if constexpr (!kRun) rescale = __any_sync(0xffffffffu, need);
+            if (need) {
+              alpha = fast_exp2(m - m_new);
+              m = m_new;
+              l *= alpha;
+            }
+          }
+          [[maybe_unused]] float factor = 0.f;
           if constexpr (kRun) {
+            alpha = 1.f;
             const float4 v4 = *reinterpret_cast<const float4*>(bars->v_top[g % kCkScaleSlots]);
             const float bound = mx * sl2 + fmaxf(fmax3f(v4.x, v4.y, v4.z) - kCkRunTop, v4.w - kCkRunTop);
-            if (__any_sync(0xffffffffu, live && (bound > m || mx * sl2 > m + kCkRunGap))) {
+            if (__any_sync(0xffffffffu, live && (bound > mv || m > mv + kCkRunGap + kCkRescale))) {
               const float to = ck_reference(tS, sl2, kCap || mask ? nullptr : bars->k_scale[g % kCkScaleSlots],
-                                            bars->v_scale[g % kCkScaleSlots], m);
-              alpha = to == m ? 1.f : fast_exp2(m - to);
-              m = to;
-              l *= alpha;
+                                            bars->v_scale[g % kCkScaleSlots], mv);
+              alpha = to == mv ? 1.f : fast_exp2(mv - to);
+              mv = to;
               rescale = j != first;
               load();
             }
-          } else {
-            const float m_new = fmax_nan(m, mx * sl2);
-            if (j == first) {
-              m = m_new;
-            } else {
-              const bool need = !(m_new <= m + kCkRescale) && m == m;  // (once to NaN; it stays)
-              rescale = __any_sync(0xffffffffu, need);
-              if (need) {
-                alpha = fast_exp2(m - m_new);
-                m = m_new;
-                l *= alpha;
-              }
-            }
+            factor = mv == -INFINITY ? 0.f : fast_exp2(m - mv);
           }
-          l += ck_exp<T, kCode>(sr, sl2, m == -INFINITY ? 0.f : m, bars->v_scale[g % kCkScaleSlots]);
+          l += ck_exp<T, kCode, kRun>(sr, sl2, m == -INFINITY ? 0.f : m, bars->v_scale[g % kCkScaleSlots],
+                                      factor);
           tmem_st32(tS + 0, sr);
           tmem_st32(tS + 32, sr + 32);
           if (rescale) {
@@ -1408,9 +1413,8 @@ __global__ void __launch_bounds__(kCkThreads, 1)
       const bool mine = first < u.j1;
       if (mine) wait(&bars->o_full[t], uc & 1);
       tc_fence_after();
-      if (kRun && l != l) m = l;  // (m' passes NaN scores over)
       bool none = m == -INFINITY;
-      float inv = none ? 0.f : 1.f / l, inv1 = 0.f;
+      float inv = none ? 0.f : (kRun ? exp2f(mv - m) : 1.f) / l, inv1 = 0.f;
       float lse2 = none ? -INFINITY : m + log2f(l);
       const bool two = twin && u.j1 - u.j0 > 1;  // the second warpgroup has a sum as well
       auto meet = [&]() {
@@ -1422,6 +1426,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
         if (t == 1) {
           bars->n_red[0][quarter][lane] = m;
           bars->n_red[1][quarter][lane] = l;
+          if constexpr (kRun) bars->twin_mv[quarter][lane] = mv;
         }
         tc_fence_before();
         meet();
@@ -1433,8 +1438,8 @@ __global__ void __launch_bounds__(kCkThreads, 1)
           const float w1 = m1 == -INFINITY ? 0.f : exp2f(m1 - mx);
           const float sum = w0 * l + w1 * l1;
           none = mx == -INFINITY;
-          inv = none ? 0.f : w0 / sum;
-          inv1 = none ? 0.f : w1 / sum;
+          inv = none ? 0.f : (kRun ? exp2f(mv - mx) : w0) / sum;
+          inv1 = none ? 0.f : (kRun ? exp2f(bars->twin_mv[quarter][lane] - mx) : w1) / sum;
           lse2 = none ? -INFINITY : mx + log2f(sum);
         }
       }

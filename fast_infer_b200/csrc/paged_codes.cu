@@ -35,7 +35,7 @@ namespace fi {
 constexpr int kPcKeys = 16;                     // keys of a tile that a warp takes: 8 warps have one
 constexpr int kPcPad = 3;                       // steps that a unit's start and end are worth on the line
 constexpr int kPcStageBytes = 2 * kPcKeys * 128 + 2 * kPcKeys * 4;
-constexpr float kPcTop = 32768.f;               // p and P' up to which maxima stay as they are
+constexpr float kPcTopP = 256.f, kPcTop = 32768.f;  // p and P' up to which maxima stay as they are
 constexpr float kPcRoom = 5.f;                  // log2 of what a row's greatest P' is then
 constexpr float kPcGap = 126.f;                 // most that m' lies below m: 2^126 is finite, 2^-126 normal
 static_assert(kPcStageBytes % 16 == 0, "16-byte copies");
@@ -438,12 +438,12 @@ __global__ void __launch_bounds__(PcShape<kNT>::kThreads, 1)
             if (!((see >> (g + 8)) & 1u)) sc[n][2 + h] = -INFINITY;
           }
       }
-      // ------------------------------------------------- weights; maxima move where one passes 2^15
+      // ------------------------------------------------- weights; maxima move where p passes 2^8 or P' 2^15
       uint32_t pb0[kNT], pb1[kNT];
       float ps[kNT][2];
 #pragma unroll 1
       for (bool moved = false;; moved = true) {
-        float top = 0.f;
+        float top_p = 0.f, top = 0.f;
 #pragma unroll
         for (int n = 0; n < kNT; ++n) {
           float w[4], v[4];
@@ -452,14 +452,14 @@ __global__ void __launch_bounds__(PcShape<kNT>::kThreads, 1)
             w[e] = fast_exp2(sc[n][e] + neg[n][e & 1]);
             v[e] = w[e] * vs[e >> 1] * fv[n][e & 1];
           }
-          top = fmax3f(fmax3f(top, w[0], w[1]), w[2], w[3]);
+          top_p = fmax3f(fmax3f(top_p, w[0], w[1]), w[2], w[3]);
           top = fmax3f(fmax3f(top, v[0], v[1]), v[2], v[3]);
           ps[n][0] = w[0] + w[2];
           ps[n][1] = w[1] + w[3];
           pb0[n] = pack_half2(v[0], v[1]);
           pb1[n] = pack_half2(v[2], v[3]);
         }
-        if (moved || __all_sync(0xffffffffu, top <= kPcTop)) break;
+        if (moved || __all_sync(0xffffffffu, top_p <= kPcTopP && top <= kPcTop)) break;
         const float lv[2] = {__log2f(vs[0]), __log2f(vs[1])};
 #pragma unroll
         for (int n = 0; n < kNT; ++n)

@@ -158,3 +158,13 @@ def test_nan_scores_show_in_the_rows_that_see_them(cuda_device, seqs, dtype, kin
     assert sees.any() and not sees.all()
     assert torch.isnan(o[sees][:, 3:]).all() and torch.isnan(lse[sees][:, 3:]).all()
     assert torch.isfinite(o[~sees]).all() and torch.isfinite(lse[~sees]).all() and torch.isfinite(o[:, :3]).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads", [(64, 1), (33, 1), (24, 8)])
+def test_lse_of_few_small_scores(cuda_device, device_checks, heads, dtype, kind):
+    """One or two keys with scores near 0: lse is as exact as fp32 sums, whatever V's scales are."""
+    st = make(cuda_device, [(1, 1), (2, 2), (1, 2)] * 8, *heads, dtype, kind, seed=25, spread=3)
+    st["ks"] *= 1e-3
+    check(st, kind, dtype)
