@@ -353,8 +353,9 @@ __device__ __forceinline__ void score_form8(const uint32_t* raw, float* s, const
 // lse is an output, which a rougher polynomial would show in.
 // The sum takes p in 32 bits; the product with V takes it in V's type, as kind::f16 asks of both
 // operands: half a step (2^-12 .. 2^-11, bf16 2^-9 .. 2^-8) of each p, which adds to the output's own
-// rounding: 3.0e-4 in place of 2.1e-4 (root mean square, relative; bf16 2.3e-3 and 1.7e-3). P as the
-// sum of two such values would take the product twice.
+// rounding: 3.0e-4 in place of the 2.1e-4 of P in 32 bits (root mean square, relative; bf16 2.3e-3 and
+// 1.7e-3). P as the sum of two such values would take the product twice; P and V's codes in fp16 under
+// bf16, 5 to 13 % of the time over codes.
 // Over codes P takes the scales of V's rows (and the sum does not), and with kRun the row's `factor` (see ck_reference).
 template <typename T, bool kCode, bool kRun>
 __device__ __forceinline__ float ck_exp(uint32_t* sr, float sl2, float mref, const float* v_scale, float factor) {
@@ -785,7 +786,8 @@ __device__ __forceinline__ void spread_tile(uint8_t* tile, int live, int quarter
 // tile j + 2 (its stage is free since S of tile j), the second one V of tile j + 1, and both the first tiles of
 // the next unit before a unit's end. (Warps of their own for it: four cost the softmax its registers,
 // two were slower than the tensor core, 408 us for 8 trees over 20 to 32 k keys.)
-// K and V keep their codes, which are exact in T. A thread of the first one looks up the scales of one row. Rows of keys past the context are zero, like those without a page.
+// K and V keep their codes, which are exact in T. A thread of the first one looks up the scales of one row. Rows of keys past
+// the context are zero, like those without a page.
 template <typename T, typename Code>
 struct CodeSpreader {
   const ChunkParams& p;
@@ -994,12 +996,12 @@ __global__ void __launch_bounds__(kCkThreads, 1)
             for (int i = 0; i < 2; ++i)
               tma_load_4d(dk + i * kChunkHalf / 2, &tm_k, &bars->kc_full[s], 0, u.hk, 0, ph[i]);
           } else {
-          mbar_arrive_expect_tx(&bars->k_full[s], kChunkTileBytes);
-          for (int i = 0; i < 2; ++i) {
-            tma_load_4d(dk + i * kChunkHalf / 2, &tm_k, &bars->k_full[s], 0, u.hk, 0, ph[i]);
-            tma_load_4d(dk + kChunkHalf + i * kChunkHalf / 2, &tm_k, &bars->k_full[s], 64, u.hk, 0,
-                        ph[i]);
-          }
+            mbar_arrive_expect_tx(&bars->k_full[s], kChunkTileBytes);
+            for (int i = 0; i < 2; ++i) {
+              tma_load_4d(dk + i * kChunkHalf / 2, &tm_k, &bars->k_full[s], 0, u.hk, 0, ph[i]);
+              tma_load_4d(dk + kChunkHalf + i * kChunkHalf / 2, &tm_k, &bars->k_full[s], 64, u.hk, 0,
+                          ph[i]);
+            }
           }
           if (j == u.j0) load_q();
           if (!ok) break;
@@ -1010,12 +1012,12 @@ __global__ void __launch_bounds__(kCkThreads, 1)
             for (int i = 0; i < 2; ++i)
               tma_load_4d(dv + i * kChunkHalf / 2, &tm_v, &bars->vc_full[s], 0, u.hk, 0, ph[i]);
           } else {
-          mbar_arrive_expect_tx(&bars->v_full[s], kChunkTileBytes);
-          for (int i = 0; i < 2; ++i) {
-            tma_load_4d(dv + i * kChunkHalf / 2, &tm_v, &bars->v_full[s], 0, u.hk, 0, ph[i]);
-            tma_load_4d(dv + kChunkHalf + i * kChunkHalf / 2, &tm_v, &bars->v_full[s], 64, u.hk, 0,
-                        ph[i]);
-          }
+            mbar_arrive_expect_tx(&bars->v_full[s], kChunkTileBytes);
+            for (int i = 0; i < 2; ++i) {
+              tma_load_4d(dv + i * kChunkHalf / 2, &tm_v, &bars->v_full[s], 0, u.hk, 0, ph[i]);
+              tma_load_4d(dv + kChunkHalf + i * kChunkHalf / 2, &tm_v, &bars->v_full[s], 64, u.hk, 0,
+                          ph[i]);
+            }
           }
           ph[0] = next[0];
           ph[1] = next[1];
@@ -1147,51 +1149,51 @@ __global__ void __launch_bounds__(kCkThreads, 1)
           ++oc[0];
           if (n > 1) ++oc[1];
         } else {
-        ok = mbar_wait(&bars->k_full[g % kCkStages], (g / kCkStages) & 1, p.err);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (!ok || u.rows[t] == 0) continue;
-          ok = mbar_wait(&bars->q_full[t], qc[t] & 1, p.err);
-          if (!ok) continue;
-          tc_fence_after();
-          issue_s(t, g % kCkStages, t);
-          ++sc[t];
-          if (n == 1) umma_commit(&bars->q_empty[t]);
-        }
-        if (ok) umma_commit(&bars->k_empty[g % kCkStages]);
-#pragma unroll 1
-        for (int j = 0; ok && j < n; ++j, ++g) {
-          const bool has_next = j + 1 < n;
-          if (has_next) {
-            ok = mbar_wait(&bars->k_full[(g + 1) % kCkStages], ((g + 1) / kCkStages) & 1, p.err);
-            if (!ok) break;
-          }
-          ok = mbar_wait(&bars->v_full[g % kCkStages], (g / kCkStages) & 1, p.err);
-          if (!ok) break;
+          ok = mbar_wait(&bars->k_full[g % kCkStages], (g / kCkStages) & 1, p.err);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (!ok || u.rows[t] == 0) continue;
-            ok = mbar_wait(&bars->p_full[t], (sc[t] - 1) & 1, p.err);
-            // the first product of a unit overwrites O: the last unit's epilogue has read it
-            if (ok && j == 0 && oc[t] > 0)
-              ok = mbar_wait(&bars->o_empty[t], (oc[t] - 1) & 1, p.err);
+            ok = mbar_wait(&bars->q_full[t], qc[t] & 1, p.err);
             if (!ok) continue;
             tc_fence_after();
-            issue_pv(t, g % kCkStages, j == 0);
-            if (!has_next) {
-              umma_commit(&bars->o_full[t]);
-            } else {
-              issue_s(t, (g + 1) % kCkStages, t);
-              ++sc[t];
-              if (j + 2 == n) umma_commit(&bars->q_empty[t]);
-            }
+            issue_s(t, g % kCkStages, t);
+            ++sc[t];
+            if (n == 1) umma_commit(&bars->q_empty[t]);
           }
-          if (!ok) break;
-          umma_commit(&bars->v_empty[g % kCkStages]);
-          if (has_next) umma_commit(&bars->k_empty[(g + 1) % kCkStages]);
-        }
-        for (int t = 0; t < 2; ++t)
-          if (u.rows[t] > 0) ++qc[t], ++oc[t];
+          if (ok) umma_commit(&bars->k_empty[g % kCkStages]);
+#pragma unroll 1
+          for (int j = 0; ok && j < n; ++j, ++g) {
+            const bool has_next = j + 1 < n;
+            if (has_next) {
+              ok = mbar_wait(&bars->k_full[(g + 1) % kCkStages], ((g + 1) / kCkStages) & 1, p.err);
+              if (!ok) break;
+            }
+            ok = mbar_wait(&bars->v_full[g % kCkStages], (g / kCkStages) & 1, p.err);
+            if (!ok) break;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (!ok || u.rows[t] == 0) continue;
+              ok = mbar_wait(&bars->p_full[t], (sc[t] - 1) & 1, p.err);
+              // the first product of a unit overwrites O: the last unit's epilogue has read it
+              if (ok && j == 0 && oc[t] > 0)
+                ok = mbar_wait(&bars->o_empty[t], (oc[t] - 1) & 1, p.err);
+              if (!ok) continue;
+              tc_fence_after();
+              issue_pv(t, g % kCkStages, j == 0);
+              if (!has_next) {
+                umma_commit(&bars->o_full[t]);
+              } else {
+                issue_s(t, (g + 1) % kCkStages, t);
+                ++sc[t];
+                if (j + 2 == n) umma_commit(&bars->q_empty[t]);
+              }
+            }
+            if (!ok) break;
+            umma_commit(&bars->v_empty[g % kCkStages]);
+            if (has_next) umma_commit(&bars->k_empty[(g + 1) % kCkStages]);
+          }
+          for (int t = 0; t < 2; ++t)
+            if (u.rows[t] > 0) ++qc[t], ++oc[t];
         }
       }
       umma_commit(&bars->mma_done);

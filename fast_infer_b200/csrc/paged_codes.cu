@@ -20,9 +20,9 @@
 //   weight, or subnormal ones, leave P' below, and o below what 16 bits hold. A sum of p in 32 bits goes with m, the sum of P' vc with m'.
 // * q of bf16 is brought to fp16 by a power of two per row, exactly but for values 2^-15 and less of
 //   the row's greatest (then to 2^-25 of that). P' is rounded to fp16, half a step of 2^-12 to 2^-11.
-// * 64 single tokens over 3000 to 9000 cached ones, 24 heads over 8 of codes, 811 MB: 152 us, 5.3 TB/s where a copy
+// * 64 single tokens over 3000 to 9000 cached ones, 24 heads over 8 of codes, 811 MB: 154 us, 5.3 TB/s where a copy
 //   reaches 6.5. Issue slots are what is left: 81 million warp instructions, a good part of them the codes' way into
-//   fragments. One token over 517: 12.5 us, two launches and one chain of loads.
+//   fragments. One token over 517: 12.6 us, two launches and one chain of loads.
 #include <float.h>
 
 #include <type_traits>

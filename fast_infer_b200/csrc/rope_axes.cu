@@ -69,7 +69,8 @@ __device__ __forceinline__ int axis_of(uint64_t axis_end, int f) {
 // (4.8 TB/s); 80 registers 38 us, reading further ahead in each warp instead 40 to 57 us.
 // `split` warps share a token (small batches have too few tokens to fill the GPU).
 // With codes, whose arithmetic takes the registers of loads ahead, heads come through shared memory kRaAhead ahead (each lane
-// copies what it will read): 7742 tokens of 24 + 8 heads and their way back 60 us with registers, 51 so (191 MB).
+// copies what it will read): 7742 tokens of 24 + 8 heads and their way back 60 us with registers, 51 so (191 MB; the store alone
+// 37 us, 143 MB).
 constexpr int kRaAhead = 3;
 struct RaRing {
   uint4 piece[kRaThreads / 32][kRaAhead][2][32];
